@@ -34,7 +34,7 @@
 extern "C" {
 #endif
 
-#define LQ8_ABI_VERSION 3
+#define LQ8_ABI_VERSION 4
 
 typedef enum {
     LQ_OK = 0,
@@ -212,6 +212,68 @@ int lq_sample(lq_ctx* ctx, const float* logits_dev, int64_t rows, int64_t vocab,
  * implements the same function. */
 int lq_fill_bf16(lq_ctx* ctx, uint64_t seed, uint64_t tensor_id, int64_t offset, int64_t count,
                  double std_dev, uint16_t* out_dev);
+
+/* ---------------------------------------------------------------------------------------
+ * Serving a batch from a paged K/V cache (no counterpart in the reference, whose cache is one
+ * contiguous tensor per sequence, attention.rs:463-592, with text positions, rope.rs:130-303).
+ *
+ * The cache of a layer is two arrays [n_pages][n_kv_heads][page_size][head_dim] of f32 or bf16;
+ * page_stride is the distance of pages in elements (0: dense), so that the layers of a model may
+ * share an allocation. page_size is a power of two from 8 to 256. A sequence's positions lie in
+ * the pages of its row of page_table_dev [n_seqs][table_ld], in order. New rows (tokens) of all
+ * sequences follow each other: those of sequence b are rows q_start_dev[b] .. q_start_dev[b+1]-1
+ * (q_start_dev [n_seqs + 1], starting at 0 and not falling; NULL: row b is sequence b's only
+ * one), and kv_len_dev[b] is its number of own positions, those rows included, which come last.
+ * Rows past the last sequence's are padding: nothing is read or written for them. Positions
+ * outside the tables, lengths outside the page table and page ids outside the cache skip the
+ * access and are reported by lq_device_status.
+ * ------------------------------------------------------------------------------------- */
+/* Waits for the context's stream; LQ_ERR_INVALID_ARG with the first code and value that a
+ * kernel flagged since the last check (90 rotary position, 91 length, 92 page id, 93 row
+ * count). */
+int lq_device_status(lq_ctx* ctx);
+/* Rotary positions with one to four axes (e.g. time, height, width). x [rows][heads][head_dim]
+ * f32 or bf16 with the given strides (elements) to out (may be x): pair i < rot_dim/2 of a head
+ * (dims i and i + rot_dim/2, as lq_qk_norm_rope_kv) turns by cos/sin[pos[a][row]][i] with
+ * a = pair_axis_host[i] (host, rot_dim/2 entries, read during the call; NULL: axis 0);
+ * dims past rot_dim are copied. Tables [table_len][rot_dim/2] f32, of any frequencies (e.g.
+ * lq_rope_tables); pos_dev [n_axes][pos_stride] int32. inverse != 0 turns back. Computed in
+ * f32, rounded once. */
+int lq_mrope(lq_ctx* ctx, const void* x_dev, lq_dtype dtype, int64_t rows, int64_t heads, int64_t head_dim,
+             int64_t row_stride, int64_t head_stride, void* out_dev, int64_t out_row_stride,
+             int64_t out_head_stride, int64_t rot_dim, const float* cos_dev, const float* sin_dev,
+             int64_t table_len, const uint8_t* pair_axis_host, int64_t n_axes, const int32_t* pos_dev,
+             int64_t pos_stride, int inverse);
+/* Projection rows qkv [rows][(n_heads + 2 n_kv_heads) * head_dim] (f32 or bf16, row_stride
+ * elements apart, 0: dense) into the cache: per-head RMSNorm of q and k (bf16 weights [head_dim];
+ * NULL: none), the rotation of lq_mrope, q to q_out [rows][n_heads][head_dim] (cache type), k and
+ * v to the rows' slots. pos_dev NULL: position pos_base + own position, one axis. The norm is f32
+ * throughout and everything rounds once; norm_bf16 != 0 rounds its input and output to bf16 as
+ * lq_rmsnorm does, bit-identical to lq_qk_norm_rope_kv for head_dim 128. */
+int lq_paged_append(lq_ctx* ctx, const void* qkv_dev, lq_dtype qkv_dtype, int64_t row_stride, int64_t rows,
+                    int64_t n_heads, int64_t n_kv_heads, int64_t head_dim, const uint16_t* q_norm_dev,
+                    const uint16_t* k_norm_dev, float eps, int norm_bf16, int64_t rot_dim, const float* cos_dev,
+                    const float* sin_dev, int64_t table_len, const uint8_t* pair_axis_host, int64_t n_axes,
+                    const int32_t* pos_dev, int64_t pos_stride, int64_t pos_base, int64_t n_seqs,
+                    const int32_t* q_start_dev, const int32_t* kv_len_dev, const int32_t* page_table_dev,
+                    int64_t table_ld, void* k_pages_dev, void* v_pages_dev, lq_dtype kv_dtype, int64_t n_pages,
+                    int64_t page_size, int64_t page_stride, void* q_out_dev, int64_t q_out_stride);
+/* Attention of the rows q [rows][n_heads][head_dim] (cache type, q_stride elements apart) over a
+ * prefix that all sequences share (positions 0 .. prefix_len-1 in the pages of prefix_table_dev,
+ * read once for the batch; prefix_len 0: none) and over the sequence's own positions up to the
+ * row itself. head_dim 64 or 128; head h reads kv head h / (n_heads / n_kv_heads). max_q and
+ * max_kv are bounds on the rows and own positions of one sequence: they size the launch and the
+ * workspace, which the context keeps and grows outside graph capture. out [rows][n_heads *
+ * head_dim] in the cache type and/or Q8_0 rows xq [rows][n_heads * head_dim], xd (either may be
+ * NULL). A row that sees nothing gives zeros. Pointers and strides are multiples of 16 bytes.
+ * f32 caches are computed in f32; bf16 ones with bf16 products and f32 sums. */
+int lq_prefix_attention(lq_ctx* ctx, const void* q_dev, lq_dtype dtype, int64_t q_stride, int64_t rows,
+                        int64_t n_heads, int64_t n_kv_heads, int64_t head_dim, float scale,
+                        const void* k_pages_dev, const void* v_pages_dev, int64_t n_pages, int64_t page_size,
+                        int64_t page_stride, const int32_t* prefix_table_dev, int64_t prefix_len, int64_t n_seqs,
+                        const int32_t* q_start_dev, const int32_t* kv_len_dev, const int32_t* page_table_dev,
+                        int64_t table_ld, int64_t max_q, int64_t max_kv, void* out_dev, int64_t out_stride,
+                        int8_t* xq_dev, uint16_t* xd_dev);
 
 /* ---------------------------------------------------------------------------------------
  * Tensor parallelism over NCCL (one process per GPU; the reference is single-device).

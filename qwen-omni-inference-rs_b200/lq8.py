@@ -93,7 +93,7 @@ _I64 = C.c_int64
 _lib = None
 
 # name -> (restype, argtypes); the single source of the binding, checked against lq8.h
-ABI_VERSION = 3   # LQ8_ABI_VERSION of the struct layouts below
+ABI_VERSION = 4   # LQ8_ABI_VERSION of the struct layouts below
 
 SIGNATURES = {
     "lq_abi_version": (C.c_int, []),
@@ -155,6 +155,14 @@ SIGNATURES = {
                                  _P, _P, _P, _P]),
     "lq_moe_forward_ep": (C.c_int, [_P, _P, C.POINTER(Q8Tensor), C.POINTER(MoeExperts), _I64, _P, _P, _I64, _I64,
                                     C.c_int, _P, _P]),
+    "lq_device_status": (C.c_int, [_P]),
+    "lq_mrope": (C.c_int, [_P, _P, C.c_int, _I64, _I64, _I64, _I64, _I64, _P, _I64, _I64, _I64, _P, _P, _I64, _P, _I64,
+                           _P, _I64, C.c_int]),
+    "lq_paged_append": (C.c_int, [_P, _P, C.c_int, _I64, _I64, _I64, _I64, _I64, _P, _P, C.c_float, C.c_int, _I64, _P,
+                                  _P, _I64, _P, _I64, _P, _I64, _I64, _I64, _P, _P, _P, _I64, _P, _P, C.c_int, _I64,
+                                  _I64, _I64, _P, _I64]),
+    "lq_prefix_attention": (C.c_int, [_P, _P, C.c_int, _I64, _I64, _I64, _I64, _I64, C.c_float, _P, _P, _I64, _I64,
+                                      _I64, _P, _I64, _I64, _P, _P, _P, _I64, _I64, _I64, _P, _I64, _P, _P]),
 }
 
 
@@ -218,6 +226,10 @@ class Context:
 
     def synchronize(self) -> None:
         self.check(self.lib.lq_synchronize(self.h))
+
+    def device_status(self) -> None:
+        """lq_device_status: waits for the stream and raises what a kernel flagged."""
+        self.check(self.lib.lq_device_status(self.h))
 
     def close(self) -> None:
         if getattr(self, "h", None):
@@ -326,6 +338,217 @@ def matmul_q8(ctx: Context, w: QTensor, xq, xd, residual=None, out=None):
     ctx.call("lq_q8_0_matmul", C.byref(ws), xq.data_ptr(), xd.data_ptr(), m, y.data_ptr(),
              _ptr(residual), y.shape[1])
     return y
+
+
+def _paged_dtype(t, what: str) -> int:
+    import torch
+    if t.dtype == torch.float32:
+        return DTYPE_F32
+    if t.dtype == torch.bfloat16:
+        return DTYPE_BF16
+    raise ValueError(f"{what}: {t.dtype} is neither float32 nor bfloat16")
+
+
+def _need(cond: bool, msg: str) -> None:
+    if not cond:
+        raise ValueError(msg)
+
+
+def _need_i32(t, what: str, dim: int) -> None:
+    import torch
+    _need(t.dtype == torch.int32 and t.is_cuda and t.dim() == dim and (t.numel() == 0 or t.stride(-1) == 1),
+          f"{what}: int32 CUDA tensor of {dim} dimension(s), last one contiguous")
+
+
+class Rotary:
+    """Rotary angles of lq_mrope and lq_paged_append: f32 CUDA tables [positions][pairs] and, with
+    several axes, the axis of each pair (uint8 on the host, e.g. from `blocks` or `cyclic`)."""
+
+    def __init__(self, cos, sin, axis=None):
+        import torch
+        _need(cos.dtype == sin.dtype == torch.float32 and cos.dim() == 2 and cos.shape == sin.shape and
+              cos.is_cuda and sin.is_cuda and cos.is_contiguous() and sin.is_contiguous(),
+              "Rotary: cos and sin are contiguous f32 CUDA tables of one shape")
+        self.cos, self.sin = cos, sin
+        self.table_len, self.pairs = cos.shape
+        self.axis = None if axis is None else np.ascontiguousarray(axis, dtype=np.uint8)
+        _need(self.axis is None or self.axis.shape == (self.pairs,), "Rotary: one axis a pair")
+        self.n_axes = 1 if self.axis is None or not self.pairs else int(self.axis.max()) + 1
+        self._axis_ptr = None if self.axis is None else self.axis.ctypes.data
+
+    @staticmethod
+    def blocks(sections) -> np.ndarray:
+        """sections[a] pairs in a row on axis a."""
+        return np.repeat(np.arange(len(sections)), sections).astype(np.uint8)
+
+    @staticmethod
+    def cyclic(sections) -> np.ndarray:
+        """Axes in turn (0, 1, 2, 0, 1, 2, ...), axis a > 0 on the first sections[a] turns; the
+        other pairs on axis 0."""
+        n, k = int(sum(sections)), len(sections)
+        i = np.arange(n)
+        return np.where(i // k < np.asarray(sections)[i % k], i % k, 0).astype(np.uint8)
+
+    @classmethod
+    def build(cls, pairs: int, positions: int, theta: float, axis=None, per_axis: bool = False, device="cuda"):
+        """Tables with frequencies theta^(-i/pairs), angles in f64; per_axis restarts i on every
+        axis (theta^(-j/n) for the j-th of an axis' n pairs)."""
+        import torch
+        i = np.arange(pairs, dtype=np.float64)
+        if per_axis:
+            a = np.asarray(axis)
+            frac = np.empty(pairs)
+            for x in np.unique(a):
+                frac[a == x] = np.arange((a == x).sum()) / (a == x).sum()
+        else:
+            frac = i / pairs
+        ang = np.arange(positions, dtype=np.float64)[:, None] * theta ** -frac
+        put = lambda t: torch.from_numpy(t.astype(np.float32)).to(device)  # noqa: E731
+        return cls(put(np.cos(ang)), put(np.sin(ang)), axis)
+
+    def _pos(self, pos, rows: int):
+        """Checked (pointer, stride) of positions [n_axes, rows] (or [rows] for one axis)."""
+        _need_i32(pos, "pos", pos.dim())
+        if pos.dim() == 1:
+            _need(self.n_axes == 1 and pos.shape[0] == rows, f"pos: [{self.n_axes}, {rows}] expected")
+            return pos.data_ptr(), rows
+        _need(pos.dim() == 2 and pos.shape[0] >= self.n_axes and pos.shape[1] == rows,
+              f"pos: [{self.n_axes}, {rows}] expected, got {list(pos.shape)}")
+        return pos.data_ptr(), pos.stride(0) if pos.shape[0] > 1 else rows
+
+
+def mrope(ctx: Context, x, rotary: Rotary, pos, out=None, inverse: bool = False):
+    """Rotary positions with several axes: x [rows, heads, head_dim] f32 or bf16 (any row and head
+    stride, the dims contiguous), pos int32 [n_axes, rows]. out may be x. Returns out."""
+    import torch
+    dt = _paged_dtype(x, "mrope")
+    _need(x.dim() == 3 and x.is_cuda and (x.shape[2] <= 1 or x.stride(2) == 1),
+          "mrope: x is a CUDA tensor [rows, heads, head_dim] with contiguous dims")
+    if out is None:
+        out = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+    _need(out.shape == x.shape and out.dtype == x.dtype and out.is_cuda and (x.shape[2] <= 1 or out.stride(2) == 1),
+          "mrope: out has x's shape and type")
+    rows, heads, D = x.shape
+    if rows == 0:
+        return out
+    p, ps = rotary._pos(pos, rows)
+    ctx.call("lq_mrope", x.data_ptr(), dt, rows, heads, D, x.stride(0), x.stride(1), out.data_ptr(), out.stride(0),
+             out.stride(1), 2 * rotary.pairs, rotary.cos.data_ptr(), rotary.sin.data_ptr(), rotary.table_len,
+             rotary._axis_ptr, rotary.n_axes, p, ps, int(inverse))
+    return out
+
+
+class PagedBatch:
+    """The sequences of a call on a paged cache: page_table int32 [B, ld], kv_len int32 [B] (own
+    positions, the new rows included), q_start int32 [B + 1] (None: one new row a sequence),
+    bounds max_q and max_kv on one sequence's new rows and own positions (max_kv None: what the
+    page table holds), and the prefix that all share (prefix_table int32, prefix_len
+    positions)."""
+
+    def __init__(self, page_table, kv_len, q_start=None, max_q: int = 1, max_kv: int | None = None, prefix_table=None,
+                 prefix_len: int = 0):
+        _need_i32(page_table, "page_table", 2)
+        _need_i32(kv_len, "kv_len", 1)
+        self.n_seqs = kv_len.shape[0]
+        _need(page_table.shape[0] == self.n_seqs and page_table.is_contiguous(),
+              "page_table: one row a sequence, contiguous")
+        if q_start is not None:
+            _need_i32(q_start, "q_start", 1)
+            _need(q_start.shape[0] == self.n_seqs + 1, "q_start: n_seqs + 1 entries")
+        _need(prefix_len >= 0 and (prefix_len == 0 or prefix_table is not None), "a prefix needs its page table")
+        if prefix_table is not None:
+            _need_i32(prefix_table, "prefix_table", 1)
+        self.page_table, self.kv_len, self.q_start, self.prefix_table = page_table, kv_len, q_start, prefix_table
+        self.max_q, self.max_kv, self.prefix_len = max_q, max_kv, prefix_len
+        self.ld = page_table.shape[1]
+        self._seqs = (self.n_seqs, _ptr(q_start), kv_len.data_ptr(), page_table.data_ptr(), self.ld)
+
+
+class PagedKvCache:
+    """A layer's paged K/V cache: k and v [n_pages, n_kv_heads, page_size, head_dim], f32 or bf16,
+    pages dense inside and any distance apart."""
+
+    def __init__(self, ctx: Context, k, v):
+        self.dtype = _paged_dtype(k, "PagedKvCache")
+        _need(k.dim() == 4 and k.shape == v.shape and k.dtype == v.dtype and k.is_cuda and v.is_cuda,
+              "PagedKvCache: k and v are CUDA tensors [n_pages, n_kv_heads, page_size, head_dim] of one type")
+        self.n_pages, self.n_kv_heads, self.page_size, self.head_dim = k.shape
+        inner = (self.page_size * self.head_dim, self.head_dim, 1)
+        _need(k.stride()[1:] == inner and v.stride()[1:] == inner and k.stride(0) == v.stride(0) and
+              (self.n_pages <= 1 or k.stride(0) >= self.n_kv_heads * inner[0]),
+              "PagedKvCache: pages are dense inside and apart, K and V pages equally far")
+        self.ctx, self.k, self.v = ctx, k, v
+        self._pages = (k.data_ptr(), v.data_ptr())
+        self._stride = k.stride(0) if self.n_pages > 1 else self.n_kv_heads * inner[0]
+
+    @classmethod
+    def empty(cls, ctx: Context, n_pages: int, page_size: int, n_kv_heads: int, head_dim: int, dtype):
+        import torch
+        shape = (n_pages, n_kv_heads, page_size, head_dim)
+        return cls(ctx, torch.empty(shape, dtype=dtype, device="cuda"), torch.empty(shape, dtype=dtype, device="cuda"))
+
+    @staticmethod
+    def _dense_rows(t) -> bool:
+        """CUDA [rows, heads, dim] whose rows are dense inside and do not overlap."""
+        return t.is_cuda and t.stride(2) == 1 and (t.shape[1] <= 1 or t.stride(1) == t.shape[2]) and (
+            t.shape[0] <= 1 or t.stride(0) >= t.shape[1] * t.shape[2])
+
+    def append(self, qkv, n_heads: int, batch: PagedBatch, rotary: Rotary, pos=None, q_norm=None, k_norm=None,
+               eps: float = 1e-6, norm_bf16: bool = False, q_out=None):
+        """qkv [rows, (n_heads + 2 n_kv_heads) * head_dim] f32 or bf16: normalises (bf16 weights)
+        and rotates q and k, appends k and v, returns q [rows, n_heads, head_dim] in the cache's
+        type. pos None: the prefix length + the own position."""
+        import torch
+        dt = _paged_dtype(qkv, "append")
+        rows, D = qkv.shape[0], self.head_dim
+        width = (n_heads + 2 * self.n_kv_heads) * D
+        _need(qkv.dim() == 2 and qkv.is_cuda and qkv.shape[1] == width and qkv.stride(1) == 1 and
+              (rows <= 1 or qkv.stride(0) >= width), f"append: rows of {width} contiguous values expected")
+        for w in (q_norm, k_norm):
+            _need(w is None or (w.dtype in (torch.bfloat16, torch.int16) and w.shape == (D,) and w.is_cuda and
+                                w.is_contiguous()), "append: norm weights are bf16 [head_dim]")
+        if q_out is None:
+            q_out = torch.empty((rows, n_heads, D), dtype=self.k.dtype, device=qkv.device)
+        _need(q_out.shape == (rows, n_heads, D) and q_out.dtype == self.k.dtype and self._dense_rows(q_out),
+              "append: q_out [rows, n_heads, head_dim] in the cache's type, rows dense inside")
+        if rows == 0:
+            return q_out
+        _need(pos is not None or rotary.n_axes == 1, "append: several axes need positions")
+        p, ps = (None, 0) if pos is None else rotary._pos(pos, rows)
+        self.ctx.call("lq_paged_append", qkv.data_ptr(), dt, qkv.stride(0) if rows > 1 else 0, rows, n_heads,
+                      self.n_kv_heads, D, _ptr(q_norm), _ptr(k_norm), eps, int(norm_bf16), 2 * rotary.pairs,
+                      rotary.cos.data_ptr(), rotary.sin.data_ptr(), rotary.table_len, rotary._axis_ptr, rotary.n_axes,
+                      p, ps, batch.prefix_len, *batch._seqs, *self._pages, self.dtype, self.n_pages, self.page_size,
+                      self._stride, q_out.data_ptr(), q_out.stride(0) if rows > 1 else 0)
+        return q_out
+
+    def attend(self, q, batch: PagedBatch, scale: float | None = None, out=None, quantized=None):
+        """Attention of q [rows, n_heads, head_dim] over the batch's prefix and each row's own
+        positions up to itself; scale None: 1/sqrt(head_dim). Returns out (q's shape). quantized:
+        (int8 [rows, n_heads * head_dim], int16 [rows, n_heads * head_dim / 32]) also gets the
+        rows in Q8_0."""
+        import torch
+        D = self.head_dim
+        _need(q.dim() == 3 and q.dtype == self.k.dtype and q.shape[2] == D and self._dense_rows(q),
+              "attend: q [rows, n_heads, head_dim] in the cache's type, rows dense inside")
+        rows, heads = q.shape[0], q.shape[1]
+        if out is None:
+            out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+        _need(out.shape == q.shape and out.dtype == q.dtype and self._dense_rows(out),
+              "attend: out has q's shape and type, rows dense inside")
+        xq, xd = (None, None) if quantized is None else quantized
+        if xq is not None:
+            _need(xq.dtype == torch.int8 and xd.dtype == torch.int16 and xq.is_contiguous() and xd.is_contiguous() and
+                  xq.shape == (rows, heads * D) and xd.shape == (rows, heads * D // 32),
+                  "attend: quantized is (int8 [rows, heads * dim], int16 [rows, heads * dim / 32])")
+        if rows == 0:
+            return out
+        max_kv = batch.ld * self.page_size if batch.max_kv is None else batch.max_kv
+        self.ctx.call("lq_prefix_attention", q.data_ptr(), self.dtype, q.stride(0) if rows > 1 else 0, rows, heads,
+                      self.n_kv_heads, D, D ** -0.5 if scale is None else scale, *self._pages, self.n_pages,
+                      self.page_size, self._stride, _ptr(batch.prefix_table), batch.prefix_len, *batch._seqs,
+                      batch.max_q, max_kv, out.data_ptr(), out.stride(0) if rows > 1 else 0, _ptr(xq), _ptr(xd))
+        return out
 
 
 COMM_ID_BYTES = 128

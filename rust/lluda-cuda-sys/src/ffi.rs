@@ -9,7 +9,7 @@
 
 use std::os::raw::{c_char, c_int, c_void};
 
-pub const LQ8_ABI_VERSION: c_int = 3;
+pub const LQ8_ABI_VERSION: c_int = 4;
 
 pub const LQ_OK: c_int = 0;
 pub const LQ_ERR_INVALID_ARG: c_int = -1;
@@ -134,6 +134,10 @@ extern "C" {
     pub fn lq_argmax(ctx: *mut LqCtx, x_dev: *const f32, rows: i64, n: i64, out_dev: *mut i32) -> c_int;
     pub fn lq_sample(ctx: *mut LqCtx, logits_dev: *const f32, rows: i64, vocab: i64, ld: i64, generated_dev: *const i32, gen_ld: i64, n_generated: i64, cfg: *const LqSampling, out_dev: *mut i32) -> c_int;
     pub fn lq_fill_bf16(ctx: *mut LqCtx, seed: u64, tensor_id: u64, offset: i64, count: i64, std_dev: f64, out_dev: *mut u16) -> c_int;
+    pub fn lq_device_status(ctx: *mut LqCtx) -> c_int;
+    pub fn lq_mrope(ctx: *mut LqCtx, x_dev: *const c_void, dtype: c_int, rows: i64, heads: i64, head_dim: i64, row_stride: i64, head_stride: i64, out_dev: *mut c_void, out_row_stride: i64, out_head_stride: i64, rot_dim: i64, cos_dev: *const f32, sin_dev: *const f32, table_len: i64, pair_axis_host: *const u8, n_axes: i64, pos_dev: *const i32, pos_stride: i64, inverse: c_int) -> c_int;
+    pub fn lq_paged_append(ctx: *mut LqCtx, qkv_dev: *const c_void, qkv_dtype: c_int, row_stride: i64, rows: i64, n_heads: i64, n_kv_heads: i64, head_dim: i64, q_norm_dev: *const u16, k_norm_dev: *const u16, eps: f32, norm_bf16: c_int, rot_dim: i64, cos_dev: *const f32, sin_dev: *const f32, table_len: i64, pair_axis_host: *const u8, n_axes: i64, pos_dev: *const i32, pos_stride: i64, pos_base: i64, n_seqs: i64, q_start_dev: *const i32, kv_len_dev: *const i32, page_table_dev: *const i32, table_ld: i64, k_pages_dev: *mut c_void, v_pages_dev: *mut c_void, kv_dtype: c_int, n_pages: i64, page_size: i64, page_stride: i64, q_out_dev: *mut c_void, q_out_stride: i64) -> c_int;
+    pub fn lq_prefix_attention(ctx: *mut LqCtx, q_dev: *const c_void, dtype: c_int, q_stride: i64, rows: i64, n_heads: i64, n_kv_heads: i64, head_dim: i64, scale: f32, k_pages_dev: *const c_void, v_pages_dev: *const c_void, n_pages: i64, page_size: i64, page_stride: i64, prefix_table_dev: *const i32, prefix_len: i64, n_seqs: i64, q_start_dev: *const i32, kv_len_dev: *const i32, page_table_dev: *const i32, table_ld: i64, max_q: i64, max_kv: i64, out_dev: *mut c_void, out_stride: i64, xq_dev: *mut i8, xd_dev: *mut u16) -> c_int;
     pub fn lq_comm_unique_id(ctx: *mut LqCtx, id_out: *mut u8) -> c_int;
     pub fn lq_comm_init(ctx: *mut LqCtx, id: *const u8, rank: c_int, world: c_int, out: *mut *mut LqComm) -> c_int;
     pub fn lq_comm_destroy(comm: *mut LqComm) -> c_int;
