@@ -340,6 +340,20 @@ int make_tensor_map_2d(lq_ctx* ctx, CUtensorMap* map, CUtensorMapDataType dt, co
     return LQ_OK;
 }
 
+int make_tensor_map_4d(lq_ctx* ctx, CUtensorMap* map, CUtensorMapDataType dt, const void* base, const uint64_t dims[4],
+                       const uint64_t stride_bytes[3], const uint32_t box[4], CUtensorMapSwizzle swz) {
+    EncodeTiledFn fn = encode_fn(ctx);
+    if (!fn) return LQ_ERR_CUDA;
+    const cuuint64_t d[4] = {dims[0], dims[1], dims[2], dims[3]};
+    const cuuint64_t st[3] = {stride_bytes[0], stride_bytes[1], stride_bytes[2]};
+    const cuuint32_t bx[4] = {box[0], box[1], box[2], box[3]};
+    const cuuint32_t estr[4] = {1, 1, 1, 1};
+    CUresult r = fn(map, dt, 4, const_cast<void*>(base), d, st, bx, estr, CU_TENSOR_MAP_INTERLEAVE_NONE, swz,
+                    CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    if (r != CUDA_SUCCESS) return set_error(ctx, LQ_ERR_CUDA, "cuTensorMapEncodeTiled failed (%d)", (int)r);
+    return LQ_OK;
+}
+
 bool gemm_tc_supported(int64_t m, int64_t K, const void* wq, const void* xq, const void* wd, const void* xd) {
     if (m < TC_BN || K % TC_KS != 0) return false;
     // TMA: 16-byte aligned bases (row strides K and K/16 bytes are multiples of 16 here)

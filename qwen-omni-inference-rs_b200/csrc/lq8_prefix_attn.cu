@@ -3,28 +3,12 @@
 // positions and over the row's own positions up to itself.
 #include "lq8_async.cuh"
 #include "lq8_fused.cuh"
-#include "lq8_paged.cuh"
+#include "lq8_prefix_attn.cuh"
+#include "lq8_prefix_plan.cuh"
 
 #include <algorithm>
 
 namespace lq {
-
-struct PrefixAttnArgs {
-    const void* q;
-    int64_t q_stride;
-    int n_heads, n_kv;
-    float scale;
-    const void* k;
-    const void* v;
-    int64_t page_stride;
-    const int32_t* prefix_table;
-    int prefix_len, max_q, max_kv;
-    void* out;
-    int64_t out_stride;
-    int8_t* xq;
-    uint16_t* xd;
-    int* err;
-};
 
 // own positions that row r sees, in its sequence b; flags lengths the call's bounds do not hold
 __device__ __forceinline__ int visible_own(const PrefixAttnArgs& a, const PagedSeqs& s, int b, int r) {
@@ -119,6 +103,173 @@ __global__ void __launch_bounds__(128) prefix_attn_row_kernel(PrefixAttnArgs a, 
     }
 }
 
+// =========================================================================================
+// Merge: a warp per (row, head) joins the partials of the workers that had a piece of the row's
+// prefix item or own item, in the order of the line: with M the largest of their maxima,
+// o = sum 2^(m_i - M) o_i / sum 2^(m_i - M) l_i. A lane looks after one partial's m and l, then
+// the warp adds up the vectors, four dims a lane. Rows that a worker had whole are written there.
+// =========================================================================================
+template <typename T, int D>
+__global__ void __launch_bounds__(256) prefix_attn_merge_kernel(PrefixAttnArgs a, PagedSeqs s, PrefixPlan p) {
+    pdl_trigger();
+    pdl_wait();
+    const int lane = threadIdx.x & 31;
+    const int idx = blockIdx.x * (blockDim.x >> 5) + (threadIdx.x >> 5);
+    const int t = idx / a.n_heads, h = idx - t * a.n_heads;
+    if (t >= s.rows) return;
+    const int b = s.q_start ? seq_of_row(s.q_start, s.n_seqs, t, lane) : t;
+    if (b >= s.n_seqs) return;
+    const SeqInfo si = seq_info(a, s, b, false);
+    const int kh = h / a.group, gq = h - kh * a.group;
+    const OwnSteps os{a, p};
+    const Line line(p, p.cum[s.n_seqs]);
+    // this row's prefix item and own item: steps [s0, s1), first virtual worker, count, slot, row
+    int v0[2] = {0, 0}, cnt[2] = {0, 0}, s0[2], s1[2], item[2], in[2];
+    if (p.np > 0) {
+        const int r = t * a.group + gq, rb = r / p.pb;
+        item[0] = kh * p.n_rb + rb;
+        in[0] = r - rb * p.pb;
+        s0[0] = item[0] * p.np;
+        s1[0] = s0[0] + p.np;
+    } else {
+        s0[0] = s1[0] = 0;
+    }
+    s0[1] = s1[1] = 0;
+    if (t < si.q0 + si.q) {
+        const int r = (t - si.q0) * a.group + gq, rb = r / p.ob, nb = os.blocks(si);
+        int before = 0, per = 0;
+        for (int i = lane; i < nb; i += 32) {
+            const int n = os.tiles(si, i);
+            per += n;
+            if (i < rb) before += n;
+        }
+        before = __reduce_add_sync(0xffffffffu, before);
+        per = __reduce_add_sync(0xffffffffu, per);
+        item[1] = a.n_kv * os.base(si, b) + kh * nb + rb;
+        in[1] = r - rb * p.ob;
+        s0[1] = p.cum[b] + kh * per + before;
+        s1[1] = s0[1] + os.tiles(si, rb);
+    }
+#pragma unroll
+    for (int part = 0; part < 2; part++) {
+        if (s0[part] == s1[part]) continue;
+        const bool paired = part ? p.pair_o : p.pair_p;
+        int w[2];
+#pragma unroll
+        for (int e = 0; e < 2; e++) {
+            const int step = e ? s1[part] - 1 : s0[part];
+            w[e] = line.owner(step, part);
+            if (!paired) {
+                int lo, hi;
+                flow_range(line, p, w[e], 0, part, lo, hi);
+                w[e] = 2 * w[e] + (step >= hi);
+            }
+        }
+        v0[part] = w[0];
+        cnt[part] = w[1] - w[0] + 1;
+    }
+    if (p.np == 0 && cnt[1] == 1) return;  // written by its only worker
+    const int n = cnt[0] + cnt[1];
+    float m_i = -INFINITY, l_i = 0.0f;
+    int64_t at_i = -1;
+    auto look = [&](int i) {  // partial i: its slot row (-1: the worker had no step of the item), m, l
+        m_i = -INFINITY;
+        l_i = 0.0f;
+        at_i = -1;
+        if (i >= n) return;
+        const int part = i >= cnt[0], v = v0[part] + i - (part ? cnt[0] : 0);
+        const bool paired = part ? p.pair_o : p.pair_p;
+        int lo, hi;
+        flow_range(line, p, paired ? v : v >> 1, paired ? 0 : v & 1, part, lo, hi);
+        if (max(lo, s0[part]) >= min(hi, s1[part])) return;
+        at_i = (int64_t)(item[part] + v) * (part ? p.cap_o : p.cap_p) + in[part];
+        const float2 ml = (part ? p.ml_o : p.ml_p)[at_i];
+        m_i = ml.x;
+        l_i = ml.y;
+    };
+    look(lane);
+    float M = warp_max(m_i);
+    for (int i0 = 32; i0 < n; i0 += 32) {
+        look(i0 + lane);
+        M = fmaxf(M, warp_max(m_i));
+    }
+    float L = 0.0f, o[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+    const bool on = 4 * lane < D;
+    for (int i0 = 0; i0 < n; i0 += 32) {
+        if (n > 32) look(i0 + lane);
+        const float w_i = m_i == -INFINITY ? 0.0f : exp2f(m_i - M);
+        L += warp_sum(w_i * l_i);
+        const int k = min(32, n - i0);
+#pragma unroll 4
+        for (int j = 0; j < k; j++) {
+            const int64_t at = __shfl_sync(0xffffffffu, at_i, j);
+            const float w = __shfl_sync(0xffffffffu, w_i, j);
+            if (at >= 0 && on) {
+                const float4 x = *reinterpret_cast<const float4*>((i0 + j >= cnt[0] ? p.o_o : p.o_p) + at * D + 4 * lane);
+                o[0] = fmaf(w, x.x, o[0]);
+                o[1] = fmaf(w, x.y, o[1]);
+                o[2] = fmaf(w, x.z, o[2]);
+                o[3] = fmaf(w, x.w, o[3]);
+            }
+        }
+    }
+    const float inv = L > 0.0f ? 1.0f / L : L;  // a row that saw nothing: zeros; NaN stays
+#pragma unroll
+    for (int j = 0; j < 4; j++) o[j] *= inv;
+    const int64_t col = (int64_t)h * D + 4 * lane;
+    if (a.out && on) {
+        T* const y = static_cast<T*>(a.out) + (int64_t)t * a.out_stride + col;
+        if constexpr (sizeof(T) == 4) *reinterpret_cast<float4*>(y) = make_float4(o[0], o[1], o[2], o[3]);
+        else *reinterpret_cast<uint2*>(y) = make_uint2(pack_bf16x2(o[0], o[1]), pack_bf16x2(o[2], o[3]));
+    }
+    if (a.xq) {
+        const int64_t e = (int64_t)t * a.n_heads * D + col;
+        const uint32_t q = quant_group8(o, lane & 7, on ? a.xd + (e >> 5) : nullptr);
+        if (on) *reinterpret_cast<uint32_t*>(a.xq + e) = q;
+    }
+}
+
+// The plan of a call for workers of `halves` x `half` stacked rows and `tile` positions, and its
+// workspace. Sizes come from the call's bounds; what the lengths really are, the kernels read.
+static int make_plan(lq_ctx* ctx, const PrefixAttnArgs& a, const PagedSeqs& s, int half, int tile, int D, PrefixPlan* p) {
+    const int64_t R = (int64_t)s.rows * a.group, most_q = std::min<int64_t>((int64_t)a.max_q, s.rows) * a.group;
+    p->tile = tile;
+    p->pair_p = R > half;
+    p->pb = p->pair_p ? 2 * half : half;
+    p->pair_o = most_q > half;
+    p->ob = p->pair_o ? 2 * half : half;
+    p->cap_p = (int)std::min<int64_t>(p->pb, R);
+    p->cap_o = (int)std::min<int64_t>(p->ob, most_q);
+    p->n_rb = ceil_div(R, p->pb);
+    p->np = ceil_div(a.prefix_len, tile);
+    const int64_t items_p = (int64_t)a.n_kv * p->n_rb, items_o = a.n_kv * (R / p->ob + s.n_seqs + 1);
+    const int64_t steps = items_p * p->np + items_o * ceil_div(a.max_kv, tile);
+    LQ_REQUIRE(ctx, steps < (1ll << 30), "lq_prefix_attention: %lld steps, more than a launch can number", (long long)steps);
+    p->sp = (int)(items_p * p->np);
+    p->workers = (int)std::max<int64_t>(1, std::min<int64_t>(ctx->sm_count, steps));
+    p->wp = p->wo = 1;
+    const int64_t slots_p = p->np ? items_p + 2 * p->workers : 0, slots_o = items_o + 2 * p->workers;
+    auto al = [](size_t b) { return (b + 255) & ~(size_t)255; };
+    const size_t cum = al((size_t)(s.n_seqs + 1) * 4), ml_p = al((size_t)slots_p * p->cap_p * 8),
+                 ml_o = al((size_t)slots_o * p->cap_o * 8), o_p = al((size_t)slots_p * p->cap_p * D * 4),
+                 o_o = al((size_t)slots_o * p->cap_o * D * 4);
+    const int rc = ensure_paged(ctx, cum + ml_p + ml_o + o_p + o_o);
+    if (rc) return rc;
+    uint8_t* w = static_cast<uint8_t*>(ctx->paged);
+    p->cum = reinterpret_cast<int32_t*>(w);
+    p->ml_p = reinterpret_cast<float2*>(w += cum);
+    p->ml_o = reinterpret_cast<float2*>(w += ml_p);
+    p->o_p = reinterpret_cast<float*>(w += ml_o);
+    p->o_o = reinterpret_cast<float*>(w += o_p);
+    return LQ_OK;
+}
+
+template <typename T, int D>
+static int launch_merge(lq_ctx* ctx, const PrefixAttnArgs& a, const PagedSeqs& s, const PrefixPlan& p) {
+    return launch_kernel(ctx, prefix_attn_merge_kernel<T, D>, dim3((unsigned)ceil_div((int64_t)s.rows * a.n_heads, 8)),
+                         dim3(256), 0, "prefix_attn_merge", a, s, p);
+}
+
 }  // namespace lq
 
 extern "C" int lq_prefix_attention(lq_ctx* ctx, const void* q, lq_dtype dtype, int64_t q_stride, int64_t rows,
@@ -149,6 +300,7 @@ extern "C" int lq_prefix_attention(lq_ctx* ctx, const void* q, lq_dtype dtype, i
                "lq_prefix_attention: bad prefix");
     LQ_REQUIRE(ctx, max_q >= 1 && max_q < (1ll << 24) && max_kv >= 0 && max_kv < (1ll << 30),
                "lq_prefix_attention: bad bounds max_q %lld, max_kv %lld", (long long)max_q, (long long)max_kv);
+    LQ_REQUIRE(ctx, scale > 0.0f && scale < INFINITY, "lq_prefix_attention: scale must be positive and finite");
     LQ_REQUIRE(ctx, (xq == nullptr) == (xd == nullptr), "lq_prefix_attention: xq and xd go together");
     LQ_REQUIRE(ctx, rows * n_heads < (1ll << 31) / 4, "lq_prefix_attention: too many rows");
     if (rows == 0 || n_seqs == 0) return LQ_OK;
@@ -163,6 +315,7 @@ extern "C" int lq_prefix_attention(lq_ctx* ctx, const void* q, lq_dtype dtype, i
     a.q_stride = q_stride;
     a.n_heads = (int)n_heads;
     a.n_kv = (int)n_kv_heads;
+    a.group = (int)(n_heads / n_kv_heads);
     a.scale = scale;
     a.k = k_pages;
     a.v = v_pages;
@@ -176,10 +329,14 @@ extern "C" int lq_prefix_attention(lq_ctx* ctx, const void* q, lq_dtype dtype, i
     a.xq = xq;
     a.xd = xd;
     a.err = ctx->err_flag;
+    if (dtype == LQ_DTYPE_BF16) {
+        lq::PrefixPlan p;
+        if ((rc = lq::make_plan(ctx, a, s, 128, 128, (int)head_dim, &p))) return rc;
+        if ((rc = lq::launch_prefix_attn_tc(ctx, a, s, p, (int)head_dim))) return rc;
+        return head_dim == 64 ? lq::launch_merge<__nv_bfloat16, 64>(ctx, a, s, p)
+                              : lq::launch_merge<__nv_bfloat16, 128>(ctx, a, s, p);
+    }
     const dim3 grid((unsigned)rows, (unsigned)n_heads);
     auto run = [&](auto kern) { return lq::launch_kernel(ctx, kern, grid, dim3(128), 0, "prefix_attn_row", a, s); };
-    if (dtype == LQ_DTYPE_F32)
-        return head_dim == 64 ? run(lq::prefix_attn_row_kernel<float, 64>) : run(lq::prefix_attn_row_kernel<float, 128>);
-    return head_dim == 64 ? run(lq::prefix_attn_row_kernel<__nv_bfloat16, 64>)
-                          : run(lq::prefix_attn_row_kernel<__nv_bfloat16, 128>);
+    return head_dim == 64 ? run(lq::prefix_attn_row_kernel<float, 64>) : run(lq::prefix_attn_row_kernel<float, 128>);
 }

@@ -1,0 +1,133 @@
+// lq8_prefix_plan.cuh -- how the shared-prefix attention cuts its work, on the device, from the
+// lengths the call finds there.
+//
+// Query rows of one kv head are stacked: token t's heads g < G of the group are rows t G + g, so
+// that all sequences' rows form the tiles of the prefix (its K/V are read once for the batch),
+// and one sequence's rows the tiles of its own positions. An item is (kv head, row block); a step
+// is one 128-position (f32: 64) tile of an item. Steps of all items form one line, prefix items
+// first, then the sequences' own, and every worker takes an equal share of it: no split factors,
+// no empty workers, whatever the mix of lengths. An item cut between workers leaves one partial
+// (o, m, l) per worker, which the merge kernel joins in order.
+#pragma once
+
+#include "lq8_paged.cuh"
+
+namespace lq {
+
+struct PrefixAttnArgs {
+    const void* q;
+    int64_t q_stride;
+    int n_heads, n_kv, group;   // group: query heads of a kv head
+    float scale;
+    const void* k;
+    const void* v;
+    int64_t page_stride;
+    const int32_t* prefix_table;
+    int prefix_len, max_q, max_kv;
+    void* out;
+    int64_t out_stride;
+    int8_t* xq;
+    uint16_t* xd;
+    int* err;
+};
+
+struct PrefixPlan {
+    int tile;                   // positions of a step
+    int pb, ob;                 // rows of a block: prefix items, own items
+    int pair_p, pair_o;         // the two halves of a block run side by side in one worker (pb / ob = 2 halves)
+    int n_rb;                   // row blocks of the prefix, per kv head
+    int np;                     // tiles of the prefix
+    int sp;                     // steps of the prefix
+    int workers;                // CTAs that share the line
+    int wp, wo;                 // weight of a prefix step and of an own step
+    int cap_p, cap_o;           // rows a partial slot holds
+    int32_t* cum;               // [n_seqs + 1] own steps before each sequence
+    float* o_p;                 // prefix partials [slot][cap_p][D], unnormalised
+    float2* ml_p;               // [slot][cap_p]: running maximum (log2 units) and sum
+    float* o_o;                 // own partials
+    float2* ml_o;
+};
+
+// a sequence's rows and own length, with what the call's bounds do not hold taken out
+struct SeqInfo {
+    int q0, q, kv;
+};
+
+__device__ __forceinline__ SeqInfo seq_info(const PrefixAttnArgs& a, const PagedSeqs& s, int b, bool flag) {
+    int q0 = b, q1 = b + 1;
+    if (s.q_start) {
+        q0 = s.q_start[b];
+        q1 = s.q_start[b + 1];
+    }
+    SeqInfo r{q0, q1 - q0, s.kv_len[b]};
+    if (r.q < 0 || r.q > a.max_q || q0 < 0 || q1 > s.rows) {
+        // without q_start, sequences past the rows have none
+        if (flag && s.q_start) flag_error(a.err, ERR_ROW_COUNT, r.q);
+        r.q = 0;
+    }
+    const int64_t most = min((int64_t)a.max_kv, s.table_ld << s.page_shift);
+    if (r.kv < 0 || r.kv > most) {
+        if (flag) flag_error(a.err, ERR_KV_LEN, r.kv);
+        r.kv = r.kv < 0 ? 0 : (int)most;
+    }
+    return r;
+}
+
+// own positions that token j of the sequence's q sees
+__device__ __forceinline__ int own_visible(const SeqInfo& i, int j) { return max(0, i.kv - i.q + j + 1); }
+
+struct OwnSteps {
+    const PrefixAttnArgs& a;
+    const PrefixPlan& p;
+    __device__ __forceinline__ int blocks(const SeqInfo& i) const { return (i.q * a.group + p.ob - 1) / p.ob; }
+    // own positions that row block rb sees (those of its last row), and its tiles
+    __device__ __forceinline__ int visible(const SeqInfo& i, int rb) const {
+        return own_visible(i, (min(i.q * a.group, (rb + 1) * p.ob) - 1) / a.group);
+    }
+    __device__ __forceinline__ int tiles(const SeqInfo& i, int rb) const {
+        return (visible(i, rb) + p.tile - 1) / p.tile;
+    }
+    __device__ __forceinline__ int per_head(const SeqInfo& i) const {
+        int n = 0;
+        for (int rb = blocks(i) - 1; rb >= 0; rb--) n += tiles(i, rb);
+        return n;
+    }
+    // numbers a sequence's row blocks from here on; blocks(i) <= base(next) - base(i), so that no
+    // scan over the sequences is needed
+    __device__ __forceinline__ int base(const SeqInfo& i, int b) const { return i.q0 * a.group / p.ob + b; }
+};
+
+// The line of steps: prefix steps weigh wp, own steps wo; worker c takes the steps that start in
+// [W c / workers, W (c + 1) / workers).
+struct Line {
+    int64_t w, split;  // total weight; weight of the prefix part
+    int sp, so, n, wp, wo;
+    __device__ __forceinline__ Line(const PrefixPlan& p, int own_steps)
+        : sp(p.sp), so(own_steps), n(p.workers), wp(p.wp), wo(p.wo) {
+        split = (int64_t)sp * wp;
+        w = split + (int64_t)so * wo;
+    }
+    __device__ __forceinline__ int first(int c, bool own) const {
+        const int64_t x = w * c / n;
+        if (!own) return (int)min((x + wp - 1) / wp, (int64_t)sp);
+        return (int)min(max(x - split + wo - 1, (int64_t)0) / wo, (int64_t)so);
+    }
+    __device__ __forceinline__ int owner(int step, bool own) const {
+        const int64_t at = own ? split + (int64_t)step * wo : (int64_t)step * wp;
+        return (int)(((at + 1) * n - 1) / w);
+    }
+};
+
+// [lo, hi) of worker c's flow f: both halves of a paired block run the same steps, otherwise the
+// flows take one half of the steps each
+__device__ __forceinline__ void flow_range(const Line& l, const PrefixPlan& p, int c, int f, bool own, int& lo, int& hi) {
+    lo = l.first(c, own);
+    hi = l.first(c + 1, own);
+    if (!(own ? p.pair_o : p.pair_p)) {
+        const int mid = lo + (hi - lo + 1) / 2;
+        if (f == 0) hi = mid;
+        else lo = mid;
+    }
+}
+
+}  // namespace lq

@@ -100,6 +100,38 @@ int ensure_split(lq_ctx* ctx, size_t bytes) {
     return LQ_OK;
 }
 
+int ensure_paged(lq_ctx* ctx, size_t bytes) {
+    if (ctx->paged_pending) {
+        cudaStreamCaptureStatus st = cudaStreamCaptureStatusNone;
+        LQ_CUDA(ctx, cudaStreamIsCapturing(ctx->stream, &st));
+        if (st == cudaStreamCaptureStatusNone) {
+            LQ_CUDA(ctx, cudaStreamWaitEvent(ctx->stream, ctx->paged_event, 0));
+            ctx->paged_pending = false;
+        }
+    }
+    ctx->paged_used = true;
+    if (bytes <= ctx->paged_bytes) return LQ_OK;
+    if (fault_injected("ensure_paged"))
+        return set_error(ctx, LQ_ERR_INJECTED, "ensure_paged: injected fault (LQ_FAULT), %zu bytes", bytes);
+    cudaStreamCaptureStatus st = cudaStreamCaptureStatusNone;
+    LQ_CUDA(ctx, cudaStreamIsCapturing(ctx->stream, &st));
+    if (st != cudaStreamCaptureStatusNone)
+        return set_error(ctx, LQ_ERR_STATE, "paged attention workspace (%zu bytes) too small while capturing a graph", bytes);
+    LQ_CUDA(ctx, cudaStreamSynchronize(ctx->stream));
+    if (ctx->paged) LQ_CUDA(ctx, cudaFree(ctx->paged));
+    ctx->paged = nullptr;
+    ctx->paged_bytes = 0;
+    size_t sz = (bytes + 0xFFFFF) & ~(size_t)0xFFFFF;
+    cudaError_t e = cudaMalloc(&ctx->paged, sz);
+    if (e == cudaErrorMemoryAllocation) {
+        cudaGetLastError();
+        return set_error(ctx, LQ_ERR_OOM, "paged attention workspace: %zu bytes", sz);
+    }
+    LQ_CUDA(ctx, e);
+    ctx->paged_bytes = sz;
+    return LQ_OK;
+}
+
 int ensure_func_smem(lq_ctx* ctx, const void* func, size_t bytes) {
     // the attribute belongs to the function on one device; contexts on several devices (or
     // threads driving them) share this table
@@ -184,6 +216,8 @@ int lq_destroy(lq_ctx* ctx) {
     if (ctx->scratch) cudaFree(ctx->scratch);
     if (ctx->split) cudaFree(ctx->split);
     if (ctx->wide) cudaFree(ctx->wide);
+    if (ctx->paged) cudaFree(ctx->paged);
+    if (ctx->paged_event) cudaEventDestroy(ctx->paged_event);
     if (ctx->err_flag) cudaFree(ctx->err_flag);
     if (ctx->tile_cnt) cudaFree(ctx->tile_cnt);
     if (ctx->own_stream) cudaStreamDestroy(ctx->own_stream);
@@ -197,7 +231,21 @@ const char* lq_last_error(const lq_ctx* ctx) {
 
 int lq_set_stream(lq_ctx* ctx, void* stream) {
     LQ_ENTRY(ctx, "lq_set_stream");
-    ctx->stream = stream ? (cudaStream_t)stream : ctx->own_stream;
+    const cudaStream_t next = stream ? (cudaStream_t)stream : ctx->own_stream;
+    if (next != ctx->stream && ctx->paged_used) {
+        // the paged attention's workspace may still be in use on the old stream: its next user
+        // waits for this point (not while a graph is being captured: captured calls are ordered
+        // by the graph)
+        cudaStreamCaptureStatus st = cudaStreamCaptureStatusNone;
+        LQ_CUDA(ctx, cudaStreamIsCapturing(ctx->stream, &st));
+        if (st == cudaStreamCaptureStatusNone) {
+            if (!ctx->paged_event) LQ_CUDA(ctx, cudaEventCreateWithFlags(&ctx->paged_event, cudaEventDisableTiming));
+            if (ctx->paged_pending) LQ_CUDA(ctx, cudaStreamWaitEvent(ctx->stream, ctx->paged_event, 0));
+            LQ_CUDA(ctx, cudaEventRecord(ctx->paged_event, ctx->stream));
+            ctx->paged_pending = true;
+        }
+    }
+    ctx->stream = next;
     return LQ_OK;
 }
 
