@@ -244,7 +244,7 @@ static int make_plan(lq_ctx* ctx, const PrefixAttnArgs& a, const PagedSeqs& s, i
     p->np = ceil_div(a.prefix_len, tile);
     const int64_t items_p = (int64_t)a.n_kv * p->n_rb, items_o = a.n_kv * (R / p->ob + s.n_seqs + 1);
     const int64_t steps = items_p * p->np + items_o * ceil_div(a.max_kv, tile);
-    LQ_REQUIRE(ctx, steps < (1ll << 30), "lq_prefix_attention: %lld steps, more than a launch can number", (long long)steps);
+    LQ_REQUIRE(ctx, steps < (1ll << 26), "lq_prefix_attention: %lld steps, more than a launch can number", (long long)steps);
     p->sp = (int)(items_p * p->np);
     p->workers = (int)std::max<int64_t>(1, std::min<int64_t>(ctx->sm_count, steps));
     p->wp = p->wo = 1;
@@ -302,7 +302,7 @@ extern "C" int lq_prefix_attention(lq_ctx* ctx, const void* q, lq_dtype dtype, i
                "lq_prefix_attention: bad bounds max_q %lld, max_kv %lld", (long long)max_q, (long long)max_kv);
     LQ_REQUIRE(ctx, scale > 0.0f && scale < INFINITY, "lq_prefix_attention: scale must be positive and finite");
     LQ_REQUIRE(ctx, (xq == nullptr) == (xd == nullptr), "lq_prefix_attention: xq and xd go together");
-    LQ_REQUIRE(ctx, rows * n_heads < (1ll << 31) / 4, "lq_prefix_attention: too many rows");
+    LQ_REQUIRE(ctx, rows * n_heads < (1ll << 28), "lq_prefix_attention: too many rows");
     if (rows == 0 || n_seqs == 0) return LQ_OK;
     LQ_REQUIRE(ctx, q && k_pages && v_pages && (out || xq), "lq_prefix_attention: NULL pointer");
     const size_t esize = dtype == LQ_DTYPE_F32 ? 4 : 2;
@@ -316,6 +316,7 @@ extern "C" int lq_prefix_attention(lq_ctx* ctx, const void* q, lq_dtype dtype, i
     a.n_heads = (int)n_heads;
     a.n_kv = (int)n_kv_heads;
     a.group = (int)(n_heads / n_kv_heads);
+    a.group_mul = ((1ull << 36) + a.group - 1) / a.group;
     a.scale = scale;
     a.k = k_pages;
     a.v = v_pages;

@@ -15,9 +15,12 @@
 // Warps 0-3: softmax of flow 0 (TMEM lane = row = thread); warps 4-7: flow 1; warp 8: TMA
 // producer, which reads the page table and brings K and V tiles page by page into a ring of 32 KB
 // stages (128-byte swizzle; pages past the end come as zeros from an out-of-range coordinate);
-// warp 9: TMEM allocator and MMA issuer. Per round the MMA warp issues, for each flow, P V of the
-// round before and then Q K of this one: the tensor pipe works for one flow while the other is in
-// its softmax. Every wait is bounded; a timeout sets the error flag and the CTA tears down.
+// warp 9: TMEM allocator and MMA issuer; warp 10: scheduler, the only one that walks the line: it
+// hands each flow its segments (PaSeg) through a small ring, so the other roles' code stays short
+// (every role walking by itself came to 300 KB of code, and the instruction misses took ten times
+// the arithmetic). Per round the MMA warp issues, for each flow, P V of the round before and then
+// Q K of this one: the tensor pipe works for one flow while the other is in its softmax. Every
+// wait is bounded; a timeout sets the error flag and the CTA tears down.
 //
 // TMA loads here read only this GPU's memory and use no multicast.
 #include "lq8_async.cuh"
@@ -33,15 +36,35 @@ namespace lq {
 constexpr int PA_ROWS = 128;      // rows of a flow (MMA M)
 constexpr int PA_TILE = 128;      // positions of a step
 constexpr int PA_STAGES = 4;
-constexpr int PA_THREADS = 320;
+constexpr int PA_THREADS = 384;   // warps 0-7 softmax, 8 TMA, 9 MMA, 10 scheduler, 11 nothing
+constexpr int PA_SEGS = 4;        // segments handed to a flow ahead
+// registers: 384 x 168 at launch = 256 x 216 for the softmax warps + 128 x 72 for the others
+constexpr int PA_REGS = 216, PA_REGS_LOW = 72;
 constexpr int PA_SCAN = 1024;     // entries of the scan over the sequences
 constexpr int ERR_PA_WAIT = 94;   // a wait ran out
 
+enum { SEG_OWN = 1, SEG_PAIRED = 2, SEG_END = 4, SEG_WHOLE = 8 };
+// the steps [t0, t1) of one item, for one flow
+struct alignas(16) PaSeg {
+    int t0, t1;     // tiles
+    int n;          // rows of the flow (0: it sits this segment out, round by round)
+    int flags;
+    int kh, b;      // kv head; sequence (own items)
+    int kv_end;     // positions the item sees
+    int row0;       // first stacked row
+    int voff;       // own items: the stacked row of token t sees t + voff positions
+    int slot;       // first row of the flow's partial
+    int n1;         // paired: rows of the second half
+    int pad;
+};
+
 struct PaCtl {
     uint64_t full[PA_STAGES], empty[PA_STAGES];
+    uint64_t seg_full[2][PA_SEGS], seg_empty[2][PA_SEGS];
     uint64_t q_full[2], s_full[2], p_full[2], o_full[2], done;
     uint32_t tmem;
     int abort;
+    PaSeg seg[2][PA_SEGS];
     int scan[PA_SCAN + 1];
 };
 
@@ -98,20 +121,30 @@ __device__ __forceinline__ void tmem_st32(uint32_t addr, const uint32_t* r) {
         PA_I8(r, 8), PA_I8(r, 16), PA_I8(r, 24), "r"(addr)
         : "memory");
 }
+__device__ __forceinline__ void tmem_st16(uint32_t addr, const uint32_t* r) {
+    asm volatile(
+        "tcgen05.st.sync.aligned.32x32b.x16.b32 [%16], {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15};" ::PA_I8(r, 0),
+        PA_I8(r, 8), "r"(addr)
+        : "memory");
+}
 __device__ __forceinline__ void tmem_wait_ld() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
 __device__ __forceinline__ void tmem_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 
-// bounded wait: 2 s, or another warp of the CTA gave up
+// bounded wait: 2 s, or another warp of the CTA gave up. try_wait itself sleeps for a while; the
+// abort flag and the (slow, shared) global timer are looked at once in many polls.
 __device__ __forceinline__ bool pa_wait(PaCtl& c, uint64_t* bar, unsigned parity, int* err) {
-    if (mbar_try_wait(bar, parity)) return true;
-    const uint64_t t0 = global_ns();
-    for (;;) {
+    uint64_t t0 = 0;
+    for (unsigned i = 0;; i++) {
         if (mbar_try_wait(bar, parity)) return true;
-        if (*reinterpret_cast<volatile int*>(&c.abort)) return false;
-        if (global_ns() - t0 > 2000000000ull) {
-            *reinterpret_cast<volatile int*>(&c.abort) = 1;
-            flag_error(err, ERR_PA_WAIT, 0);
-            return false;
+        if ((i & 255) == 255) {
+            if (*reinterpret_cast<volatile int*>(&c.abort)) return false;
+            const uint64_t now = global_ns();
+            if (t0 == 0) t0 = now;
+            if (now - t0 > 2000000000ull) {
+                *reinterpret_cast<volatile int*>(&c.abort) = 1;
+                flag_error(err, ERR_PA_WAIT, 0);
+                return false;
+            }
         }
     }
 }
@@ -122,55 +155,35 @@ struct PaArgs {
     PrefixPlan p;
 };
 
-// A flow's place in its part of the line. Every role walks the same sequence by itself.
+// A flow's place in its part of the line (the scheduler's).
 struct PaCursor {
-    bool own;
     int step, hi;       // steps of the part: the next one, and the flow's end
     int b, kh, rb, n_rb;
     int t, nt;          // tile of the item
-    int kv_end;         // positions the item sees
-    int row0, rows;     // stacked rows of the block
     SeqInfo si;
 
-    __device__ __forceinline__ bool live() const { return step < hi; }
-
-    __device__ __forceinline__ void set_prefix(const PaArgs& g) {
-        row0 = rb * g.p.pb;
-        rows = min(g.p.pb, g.s.rows * g.a.group - row0);
-    }
-    __device__ __forceinline__ void set_own(const PaArgs& g) {
-        const OwnSteps o{g.a, g.p};
-        kv_end = o.visible(si, rb);
-        nt = (kv_end + PA_TILE - 1) / PA_TILE;
-        row0 = si.q0 * g.a.group + rb * g.p.ob;
-        rows = min(g.p.ob, si.q * g.a.group - rb * g.p.ob);
-    }
-    __device__ __forceinline__ void seek(const PaArgs& g, const int* scan, int per_entry, int n_entries, bool own_part,
-                                         int lo, int hi_) {
-        own = own_part;
-        step = lo;
-        hi = hi_;
-        if (lo >= hi_) return;
+    __device__ __forceinline__ void seek(const PaArgs& g, const int* scan, int per_entry, int n_entries, bool own) {
+        if (step >= hi) return;
         if (!own) {
-            const int item = lo / g.p.np;
-            t = lo - item * g.p.np;
+            const int item = step / g.p.np;
+            t = step - item * g.p.np;
             nt = g.p.np;
-            kv_end = g.a.prefix_len;
             n_rb = g.p.n_rb;
             kh = item / n_rb;
             rb = item - kh * n_rb;
             b = 0;
-            set_prefix(g);
             return;
         }
-        int e0 = 0, e1 = n_entries;  // the last entry with scan <= lo
+        int e0 = 0, e1 = n_entries;  // the last entry with scan <= step
+#pragma unroll 1
         while (e1 - e0 > 1) {
             const int m = (e0 + e1) >> 1;
-            if (scan[m] <= lo) e0 = m;
+            if (scan[m] <= step) e0 = m;
             else e1 = m;
         }
         const OwnSteps o{g.a, g.p};
-        int rest = lo - scan[e0], per = 0;
+        int rest = step - scan[e0], per = 0;
+#pragma unroll 1
         for (b = e0 * per_entry; b < g.s.n_seqs; b++) {
             si = seq_info(g.a, g.s, b, false);
             per = o.per_head(si);
@@ -185,43 +198,58 @@ struct PaCursor {
         rest -= kh * per;
         n_rb = o.blocks(si);
         rb = 0;
-        while (rest >= o.tiles(si, rb)) rest -= o.tiles(si, rb++);
-        set_own(g);
+#pragma unroll 1
+        while (rb + 1 < n_rb && rest >= o.tiles(si, rb)) rest -= o.tiles(si, rb++);
+        nt = o.tiles(si, rb);
         t = rest;
     }
-    __device__ __forceinline__ void next(const PaArgs& g) {
-        step++;
-        if (++t < nt || step >= hi) return;
+    // to the next item with a step, unless the flow's end is reached
+    __device__ __forceinline__ void next_item(const PaArgs& g, bool own) {
         t = 0;
-        if (!own) {
-            if (++rb == n_rb) rb = 0, kh++;
-            set_prefix(g);
-            return;
-        }
-        do {
+        while (step < hi) {
             if (++rb >= n_rb) {
                 rb = 0;
-                if (++kh == g.a.n_kv) {
+                kh++;
+                if (own && kh == g.a.n_kv) {
                     kh = 0;
-                    do {
-                        if (++b >= g.s.n_seqs) {  // lengths that changed under the kernel
-                            hi = step;
-                            return;
-                        }
-                        si = seq_info(g.a, g.s, b, false);
-                        n_rb = OwnSteps{g.a, g.p}.blocks(si);
-                    } while (n_rb == 0 || si.kv == 0);
+                    if (++b >= g.s.n_seqs) {  // lengths that changed under the kernel
+                        hi = step;
+                        return;
+                    }
+                    si = seq_info(g.a, g.s, b, false);
+                    n_rb = OwnSteps{g.a, g.p}.blocks(si);
+                    if (n_rb == 0 || si.kv == 0) {  // nothing of this sequence
+                        kh = g.a.n_kv - 1;
+                        rb = n_rb;
+                        continue;
+                    }
                 }
             }
-            set_own(g);
-        } while (nt == 0);
+            if (!own) return;
+            nt = OwnSteps{g.a, g.p}.tiles(si, rb);
+            if (nt > 0) return;
+        }
     }
-    // rows of flow f: a paired block's halves, else all of them
-    __device__ __forceinline__ int flow_rows(const PaArgs& g, int f) const {
-        return (own ? g.p.pair_o : g.p.pair_p) ? min(PA_ROWS, max(0, rows - f * PA_ROWS)) : rows;
-    }
-    __device__ __forceinline__ int flow_row0(const PaArgs& g, int f) const {
-        return (own ? g.p.pair_o : g.p.pair_p) ? row0 + f * PA_ROWS : row0;
+    __device__ __forceinline__ PaSeg segment(const PaArgs& g, bool own, bool paired, int half, int worker) const {
+        PaSeg o;
+        const int block = own ? g.p.ob : g.p.pb, cap = own ? g.p.cap_o : g.p.cap_p;
+        const int start = own ? si.q0 * g.a.group : 0, total = own ? si.q * g.a.group : g.s.rows * g.a.group;
+        const int left = total - rb * block - half * PA_ROWS;
+        const OwnSteps os{g.a, g.p};
+        o.t0 = t;
+        o.t1 = min(nt, t + hi - step);
+        o.n = max(0, min(PA_ROWS, left));
+        o.flags = (own ? SEG_OWN : 0) | (paired ? SEG_PAIRED : 0) |
+                  (g.a.prefix_len == 0 && o.t0 == 0 && o.t1 == nt ? SEG_WHOLE : 0);
+        o.kh = kh;
+        o.b = b;
+        o.kv_end = own ? os.visible(si, rb) : g.a.prefix_len;
+        o.row0 = start + rb * block + half * PA_ROWS;
+        o.voff = own ? si.kv - si.q + 1 - si.q0 : 0;
+        const int item = (own ? g.a.n_kv * os.base(si, b) : 0) + kh * n_rb + rb;
+        o.slot = (item + worker) * cap + half * PA_ROWS;
+        o.n1 = o.pad = 0;
+        return o;
     }
 };
 
@@ -246,6 +274,10 @@ prefix_attn_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_co
             mbar_init(&c.s_full[f], 1);
             mbar_init(&c.p_full[f], 4);
             mbar_init(&c.o_full[f], 1);
+            for (int i = 0; i < PA_SEGS; i++) {
+                mbar_init(&c.seg_full[f][i], 1);
+                mbar_init(&c.seg_empty[f][i], 6);  // four softmax warps, producer, MMA issuer
+            }
         }
         mbar_init(&c.done, 1);
         c.abort = 0;
@@ -265,8 +297,10 @@ prefix_attn_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_co
     const int per_entry = (g.s.n_seqs + PA_SCAN - 1) / PA_SCAN;
     const int n_entries = (g.s.n_seqs + per_entry - 1) / per_entry;
     const OwnSteps os{g.a, g.p};
+#pragma unroll 1
     for (int e = tid; e < n_entries; e += PA_THREADS) {
         int n = 0;
+#pragma unroll 1
         for (int b = e * per_entry; b < min(g.s.n_seqs, (e + 1) * per_entry); b++)
             n += os.per_head(seq_info(g.a, g.s, b, blockIdx.x == 0)) * g.a.n_kv;
         c.scan[e + 1] = n;
@@ -274,6 +308,7 @@ prefix_attn_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_co
     __syncthreads();
     if (warp == 0) {
         int run = 0;
+#pragma unroll 1
         for (int e0 = 0; e0 < n_entries; e0 += 32) {
             int v = e0 + lane < n_entries ? c.scan[e0 + lane + 1] : 0;
 #pragma unroll
@@ -292,8 +327,10 @@ prefix_attn_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_co
     const uint32_t tmem = c.tmem;
     const int so = c.scan[n_entries];
     if (blockIdx.x == 0) {  // the sequences' places in the line, for the merge
+#pragma unroll 1
         for (int e = tid; e < n_entries; e += PA_THREADS) {
             int n = c.scan[e];
+#pragma unroll 1
             for (int b = e * per_entry; b < min(g.s.n_seqs, (e + 1) * per_entry); b++) {
                 g.p.cum[b] = n;
                 if (per_entry > 1) n += os.per_head(seq_info(g.a, g.s, b, false)) * g.a.n_kv;
@@ -301,90 +338,91 @@ prefix_attn_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_co
         }
         if (tid == 0) g.p.cum[g.s.n_seqs] = so;
     }
-    const Line line(g.p, so);
     const int me = blockIdx.x;
+    // the next segment of flow f, for a reader that keeps its place (index, parity) in `at`
+    auto fetch = [&](int f, unsigned& at, PaSeg& o) {
+        const int i = at % PA_SEGS;
+        if (!pa_wait(c, &c.seg_full[f][i], (at / PA_SEGS) & 1u, err)) return false;
+        const int4* src = reinterpret_cast<const int4*>(&c.seg[f][i]);
+        const int4 x = src[0], y = src[1], z = src[2];
+        o.t0 = x.x, o.t1 = x.y, o.n = x.z, o.flags = x.w;
+        o.kh = y.x, o.b = y.y, o.kv_end = y.z, o.row0 = y.w;
+        o.voff = z.x, o.slot = z.y, o.n1 = z.z;
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&c.seg_empty[f][i]);
+        at++;
+        return true;
+    };
 
     if (warp < 8) {
         // ------------------------------ softmax ------------------------------
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(PA_REGS));
         const int f = warp >> 2, row = tid & 127, wq = warp & 3;
-        uint8_t* const sq = sm + f * Q_BYTES;
+        const uint32_t sq = smem_addr(sm + f * Q_BYTES);
         const uint32_t t_lane = (uint32_t)(wq * 32) << 16;
         const uint32_t t_s = tmem + t_lane + f * 128, t_o = tmem + t_lane + 256 + f * 128;
         const float cs = g.a.scale * 1.44269504088896340736f;  // scores in units of log2
-        unsigned s_ph = 0, o_ph = 0;
-        bool ok = true;
+        unsigned s_ph = 0, o_ph = 0, at = 0;
 
-        auto load_q = [&](const PaCursor& cu) {
-            const int n = cu.flow_rows(g, f), r0 = cu.flow_row0(g, f);
-            constexpr int CH = D / 8, PASS = PA_ROWS * CH / 128;
-            uint4 v[PASS];
-#pragma unroll
-            for (int i = 0; i < PASS; i++) {
-                const int r = (i * 128 + row) / CH, ch = (i * 128 + row) % CH;
-                v[i] = make_uint4(0, 0, 0, 0);
-                if (r < n) {
-                    const int st = r0 + r, t = st / g.a.group, h = cu.kh * g.a.group + st - t * g.a.group;
-                    v[i] = *reinterpret_cast<const uint4*>(static_cast<const __nv_bfloat16*>(g.a.q) +
-                                                           (int64_t)t * g.a.q_stride + (int64_t)h * D + ch * 8);
-                }
+        // the next segment with rows (false: none, or a wait ran out), its Q on the way
+        PaSeg nx;
+        auto begin = [&]() {
+            do {
+                if (!fetch(f, at, nx)) return false;
+                if (nx.flags & SEG_END) return false;
+            } while (nx.n == 0);
+            constexpr int CH = D / 8;
+#pragma unroll 1
+            for (int i = row; i < nx.n * CH; i += 128) {
+                const int r = i / CH, ch = i % CH, t = g.a.group_div(nx.row0 + r);
+                const int h = nx.kh * g.a.group + nx.row0 + r - t * g.a.group;
+                const uint32_t dst = sq + (ch >> 3) * HALF + r * 128 + (((ch & 7) ^ (r & 7)) << 4);
+                asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst),
+                             "l"(static_cast<const __nv_bfloat16*>(g.a.q) + (int64_t)t * g.a.q_stride + h * D + ch * 8));
             }
-#pragma unroll
-            for (int i = 0; i < PASS; i++) {
-                const int r = (i * 128 + row) / CH, ch = (i * 128 + row) % CH;
-                *reinterpret_cast<uint4*>(sq + (ch >> 3) * HALF + r * 128 + (((ch & 7) ^ (r & 7)) << 4)) = v[i];
-            }
+            asm volatile("cp.async.wait_all;" ::: "memory");
             proxy_fence();
             __syncwarp();
             if (lane == 0) mbar_arrive(&c.q_full[f]);
+            return true;
         };
 
-        PaCursor cu;
-        int part = 0;
-        // the next step of this flow that has rows; false: none left
-        auto settle = [&](bool fresh) {
-            if (!fresh) cu.next(g);
-            for (;;) {
-                while (cu.live() && cu.flow_rows(g, f) == 0) cu.next(g);
-                if (cu.live()) return true;
-                if (part == 2) return false;
-                int lo, hi;
-                flow_range(line, g.p, me, f, part == 1, lo, hi);
-                cu.seek(g, c.scan, per_entry, n_entries, part == 1, lo, hi);
-                part++;
-            }
-        };
-        cu.step = cu.hi = 0;
-        bool more = settle(true);
-        if (more) load_q(cu);
-        while (more && ok) {
-            const PaCursor it = cu;  // the segment's item and first tile
-            const int n = it.flow_rows(g, f);
-            const bool mine = row < n, busy = wq * 32 < n;
-            int vis = it.kv_end;
-            if (it.own) vis = own_visible(it.si, (it.flow_row0(g, f) + min(row, n - 1)) / g.a.group - it.si.q0);
+        bool more = begin();
+        while (more) {
+            const PaSeg sg = nx;
+            const int st = sg.row0 + min(row, sg.n - 1), tok = g.a.group_div(st);
+            const bool mine = row < sg.n, busy = wq * 32 < sg.n;
+            const int vis = sg.flags & SEG_OWN ? max(0, tok + sg.voff) : sg.kv_end;
             float m = -INFINITY, l = 0.0f;
-            bool last;
-            do {
-                ok = pa_wait(c, &c.s_full[f], s_ph, err);
-                if (!ok) break;
+            int t = sg.t0;
+#pragma unroll 1
+            for (; t < sg.t1; t++) {
+                if (!pa_wait(c, &c.s_full[f], s_ph, err)) break;
                 s_ph ^= 1;
                 tc_after();
                 if (busy) {
-                    float s[128];
+                    // two passes over S, 32 columns at a time: the maximum, then the probabilities.
+                    // Reading S twice from TMEM costs less than the registers and the straight-line
+                    // code that 128 columns at once would take.
+                    const int lim = vis - t * PA_TILE;  // columns this row sees
+                    float mt = -INFINITY;
+#pragma unroll 1
+                    for (int j = 0; j < PA_TILE; j += 32) {
+                        float s[32];
+                        tmem_ld32(reinterpret_cast<uint32_t*>(s), t_s + j);
+                        tmem_wait_ld();
+                        if (!__all_sync(0xffffffffu, lim >= j + 32)) {
 #pragma unroll
-                    for (int i = 0; i < 4; i++) tmem_ld32(reinterpret_cast<uint32_t*>(s) + 32 * i, t_s + 32 * i);
-                    tmem_wait_ld();
-                    const int lim = vis - cu.t * PA_TILE;
-                    if (!__all_sync(0xffffffffu, lim >= PA_TILE)) {
+                            for (int i = 0; i < 32; i++)
+                                if (j + i >= lim) s[i] = -INFINITY;
+                        }
+                        float mx[4] = {mt, s[0], s[1], s[2]};
 #pragma unroll
-                        for (int i = 0; i < 128; i++)
-                            if (i >= lim) s[i] = -INFINITY;
+                        for (int i = 3; i < 32; i++) mx[i & 3] = fmaxf(mx[i & 3], s[i]);
+                        mt = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3]));
                     }
-                    float mx[4] = {s[0], s[1], s[2], s[3]};
-#pragma unroll
-                    for (int i = 4; i < 128; i++) mx[i & 3] = fmaxf(mx[i & 3], s[i]);
-                    const float mt = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * cs;
-                    if (cu.t == it.t) {
+                    mt *= cs;
+                    if (t == sg.t0) {
                         m = mt;
                     } else if (__any_sync(0xffffffffu, mt > m + 8.0f)) {
                         const float mn = fmaxf(m, mt);
@@ -403,18 +441,26 @@ prefix_attn_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_co
                     }
                     const float neg = m == -INFINITY ? 0.0f : -m;
                     float sum[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll 1
+                    for (int j = 0; j < PA_TILE; j += 32) {
+                        float s[32];
+                        tmem_ld32(reinterpret_cast<uint32_t*>(s), t_s + j);
+                        tmem_wait_ld();
+                        if (!__all_sync(0xffffffffu, lim >= j + 32)) {
 #pragma unroll
-                    for (int h = 0; h < 2; h++) {
-                        uint32_t pk[32];
+                            for (int i = 0; i < 32; i++)
+                                if (j + i >= lim) s[i] = -INFINITY;
+                        }
+                        uint32_t pk[16];
 #pragma unroll
-                        for (int i = 0; i < 32; i++) {
-                            const float p0 = ex2(fmaf(s[64 * h + 2 * i], cs, neg));
-                            const float p1 = ex2(fmaf(s[64 * h + 2 * i + 1], cs, neg));
+                        for (int i = 0; i < 16; i++) {
+                            const float p0 = ex2(fmaf(s[2 * i], cs, neg)), p1 = ex2(fmaf(s[2 * i + 1], cs, neg));
                             sum[i & 1] += p0;
                             sum[2 + (i & 1)] += p1;
                             pk[i] = pack_bf16x2(p0, p1);
                         }
-                        tmem_st32(t_s + 32 * h, pk);
+                        // P of columns j.. lands on S columns j/2.., which have been read
+                        tmem_st16(t_s + j / 2, pk);
                     }
                     l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
                     tmem_wait_st();
@@ -422,29 +468,20 @@ prefix_attn_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_co
                 tc_before();
                 __syncwarp();
                 if (lane == 0) mbar_arrive(&c.p_full[f]);
-                last = cu.t + 1 == cu.nt || cu.step + 1 == cu.hi;
-                if (!last) cu.next(g);
-            } while (!last);
-            if (!ok) break;
-            const int t_last = cu.t;
-            more = settle(false);
-            if (more) load_q(cu);
-            ok = pa_wait(c, &c.o_full[f], o_ph, err);
-            if (!ok) break;
+            }
+            if (t < sg.t1) break;  // a wait ran out
+            more = begin();        // the Q of the next segment, while this one's last products run
+            if (!pa_wait(c, &c.o_full[f], o_ph, err)) break;
             o_ph ^= 1;
             tc_after();
             if (!busy) continue;
             // ---- the segment's result: the row itself, or a partial for the merge ----
-            const bool paired = it.own ? g.p.pair_o : g.p.pair_p;
-            const int worker = paired ? me : 2 * me + f;
-            const int item = it.own ? g.a.n_kv * os.base(it.si, it.b) + it.kh * it.n_rb + it.rb : it.kh * it.n_rb + it.rb;
-            const int cap = it.own ? g.p.cap_o : g.p.cap_p;
-            const int64_t at = (int64_t)(item + worker) * cap + (paired ? f * PA_ROWS : 0) + row;
-            const bool whole = g.a.prefix_len == 0 && it.t == 0 && t_last + 1 == it.nt;
-            const int st = it.flow_row0(g, f) + row, tok = st / g.a.group, head = it.kh * g.a.group + st - tok * g.a.group;
+            const bool own = sg.flags & SEG_OWN, whole = sg.flags & SEG_WHOLE;
+            const int64_t at_o = sg.slot + row;
+            const int head = sg.kh * g.a.group + st - tok * g.a.group;
             const float inv = l > 0.0f ? 1.0f / l : 0.0f;
-            if (mine && !whole) (it.own ? g.p.ml_o : g.p.ml_p)[at] = make_float2(m, l);
-            float* const po = (it.own ? g.p.o_o : g.p.o_p) + at * D;
+            if (mine && !whole) (own ? g.p.ml_o : g.p.ml_p)[at_o] = make_float2(m, l);
+            float* const po = (own ? g.p.o_o : g.p.o_p) + at_o * D;
 #pragma unroll 1
             for (int i = 0; i < D; i += 32) {
                 uint32_t r[32];
@@ -466,16 +503,15 @@ prefix_attn_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_co
         }
     } else if (warp == 8) {
         // ------------------------------ TMA producer ------------------------------
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(PA_REGS_LOW));
         const int page = 1 << g.s.page_shift, box = min(page, PA_TILE), boxes = PA_TILE / box;
-        int slot = 0, issued = 0;
-        unsigned ph = 0;
-        bool ok = true;
-        PaCursor cu[2];
-        int pg[2] = {0, 0}, krow[2] = {0, 0}, kkh[2] = {0, 0};  // this lane's page of the flow's tile, kept from K for V
-        bool live_before[2] = {false, false};
-        bool paired_before = false;
+        int issued = 0, slot = 0;
+        unsigned ph = 0, at[2] = {0, 0};
+        bool ok = true, ended[2] = {false, false}, v_due[2] = {false, false};
+        PaSeg sg[2];
+        sg[0].t0 = sg[0].t1 = sg[1].t0 = sg[1].t1 = 0;
+        int pg[2] = {0, 0}, krow[2] = {0, 0}, vkh[2] = {0, 0};  // this lane's page of the flow's tile, kept from K for V
         auto load = [&](const CUtensorMap* map, int pid, int prow, int kh) {
-            if (!ok) return;
             ok = pa_wait(c, &c.empty[slot], ph ^ 1u, err);
             if (!ok) return;
             if (lane == 0) mbar_expect_tx(&c.full[slot], KV_BYTES);
@@ -489,74 +525,69 @@ prefix_attn_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_co
             issued++;
             if (++slot == PA_STAGES) slot = 0, ph ^= 1;
         };
-        for (int part = 0; part < 2 && ok; part++) {
-            const bool paired = part ? g.p.pair_o : g.p.pair_p;
-            int lo[2], hi[2];
+        // a round brings, per flow, V of the round before and K of this one
+        while (ok && !(ended[0] && ended[1] && !v_due[0] && !v_due[1])) {
+#pragma unroll
             for (int f = 0; f < 2; f++) {
-                flow_range(line, g.p, me, f, part == 1, lo[f], hi[f]);
-                cu[f].seek(g, c.scan, per_entry, n_entries, part == 1, lo[f], hi[f]);
-            }
-            const int rounds = hi[0] - lo[0];
-            // round r brings V of the round before and K of this one; the last V of a part with
-            // the next part's first round, or at the end
-            for (int r = 0; r < rounds && ok; r++) {
-                for (int f = 0; f < 2; f++) {
-                    if (live_before[f] && (f == 0 || !paired_before)) load(&map_v, pg[f], krow[f], kkh[f]);
-                    const bool live = cu[f].live();
-                    if (live && (f == 0 || !paired)) {
-                        const int pos = cu[f].t * PA_TILE + lane * box;
-                        int id = g.s.n_pages;  // out of range: zeros
-                        if (lane < boxes && pos < cu[f].kv_end) {
-                            id = cu[f].own ? g.s.table[(int64_t)cu[f].b * g.s.table_ld + (pos >> g.s.page_shift)]
-                                           : g.a.prefix_table[pos >> g.s.page_shift];
-                            if (id < 0 || id >= g.s.n_pages) {
-                                flag_error(err, ERR_PAGE_ID, id);
-                                id = g.s.n_pages;
-                            }
-                        }
-                        pg[f] = id;
-                        krow[f] = pos & (page - 1);
-                        kkh[f] = cu[f].kh;
-                        load(&map_k, id, krow[f], kkh[f]);
-                    }
-                    live_before[f] = live;
-                    if (live) cu[f].next(g);
+                if (ok && v_due[f]) load(&map_v, pg[f], krow[f], vkh[f]);
+                v_due[f] = false;
+                if (!ok || ended[f]) continue;
+                if (sg[f].t0 == sg[f].t1) {
+                    ok = fetch(f, at[f], sg[f]);
+                    if (!ok) continue;
+                    ended[f] = sg[f].flags & SEG_END;
+                    if (ended[f]) continue;
                 }
-                paired_before = paired;
+                const int t = sg[f].t0++;
+                if (sg[f].n == 0 || (f == 1 && (sg[f].flags & SEG_PAIRED))) continue;
+                const int pos = t * PA_TILE + lane * box;
+                int id = g.s.n_pages;  // out of range: zeros
+                if (lane < boxes && pos < sg[f].kv_end) {
+                    id = sg[f].flags & SEG_OWN ? g.s.table[(int64_t)sg[f].b * g.s.table_ld + (pos >> g.s.page_shift)]
+                                               : g.a.prefix_table[pos >> g.s.page_shift];
+                    if (id < 0 || id >= g.s.n_pages) {
+                        flag_error(err, ERR_PAGE_ID, id);
+                        id = g.s.n_pages;
+                    }
+                }
+                pg[f] = id;
+                krow[f] = pos & (page - 1);
+                vkh[f] = sg[f].kh;
+                v_due[f] = true;
+                load(&map_k, id, krow[f], vkh[f]);
             }
         }
-        for (int f = 0; f < 2; f++)
-            if (live_before[f] && (f == 0 || !paired_before)) load(&map_v, pg[f], krow[f], kkh[f]);
         // no copy may still be landing when the CTA exits
         if (!ok) {
             for (int i = max(0, issued - PA_STAGES); i < issued; i++)
                 mbar_wait_ns(&c.full[i % PA_STAGES], (unsigned)(i / PA_STAGES) & 1u, 2000000000ull);
         }
-    } else {
+    } else if (warp == 9) {
         // ------------------------------ MMA issuer ------------------------------
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(PA_REGS_LOW));
         constexpr uint32_t id_qk = pa_idesc(PA_TILE, 0), id_pv = pa_idesc(D, 1);
-        int slot = 0;
-        unsigned ph = 0, q_ph[2] = {0, 0}, p_ph[2] = {0, 0};
-        bool ok = true;
-        PaCursor cu[2];
-        // what the round before left to do, per flow
-        bool pv[2] = {false, false}, pv_first[2] = {false, false}, pv_last[2] = {false, false};
+        int slot = 0, k_slot = 0, v_slot = 0;
+        unsigned ph = 0, q_ph[2] = {0, 0}, p_ph[2] = {0, 0}, at[2] = {0, 0};
+        bool ok = true, ended[2] = {false, false};
+        PaSeg sg[2];
+        sg[0].t0 = sg[0].t1 = sg[1].t0 = sg[1].t1 = 0;
+        // P V of the round before, per flow: due, shared with flow 1, first and last of a segment
+        bool pv[2] = {false, false}, pv_pair[2] = {false, false}, pv_first[2] = {false, false}, pv_last[2] = {false, false};
         int pv_valid[2] = {0, 0};
-        bool paired_before = false;
-        int v_slot = 0, k_slot = 0;
         auto take = [&](int& where) {  // the next stage of the ring
             ok = pa_wait(c, &c.full[slot], ph, err);
             where = slot;
             if (++slot == PA_STAGES) slot = 0, ph ^= 1;
         };
-        auto do_pv = [&](int f, bool other) {  // other: the second flow still reads this V
-            if (f == 0 || !paired_before) {
+        auto do_pv = [&](int f) {
+            if (f == 0 || !pv_pair[f]) {
                 take(v_slot);
                 if (!ok) return;
                 if (pv_valid[f] < PA_TILE) {
                     // positions past the end share a page with valid ones: whatever is there
                     // (NaN times a zero probability) must not reach the product
                     uint8_t* const v = ring + v_slot * KV_BYTES;
+#pragma unroll 1
                     for (int i = pv_valid[f] * 8 + lane; i < PA_TILE * 8; i += 32)
 #pragma unroll
                         for (int h = 0; h < HALVES; h++)
@@ -570,67 +601,116 @@ prefix_attn_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_co
             p_ph[f] ^= 1;
             tc_after();
             if (lane == 0) {
-                const uint32_t v = smem_addr(ring + v_slot * KV_BYTES);
+                const uint64_t v = pa_desc(smem_addr(ring + v_slot * KV_BYTES), HALF);
 #pragma unroll
                 for (int j = 0; j < PA_TILE / 16; j++)
-                    mma_ts(tmem + 256 + f * 128, tmem + f * 128 + j * 8, pa_desc(v + j * 2048, HALF), id_pv,
-                           (pv_first[f] && j == 0) ? 0u : 1u);
-                if (!other) tc_commit(&c.empty[v_slot]);
+                    mma_ts(tmem + 256 + f * 128, tmem + f * 128 + j * 8, v + j * (2048 >> 4), id_pv,
+                           j > 0 || !pv_first[f]);
+                if (!(f == 0 && pv_pair[0] && pv[1])) tc_commit(&c.empty[v_slot]);
                 if (pv_last[f]) tc_commit(&c.o_full[f]);
             }
             __syncwarp();
         };
-        for (int part = 0; part < 2 && ok; part++) {
-            const bool paired = part ? g.p.pair_o : g.p.pair_p;
-            int lo[2], hi[2];
-            bool fresh[2] = {true, true};
-            for (int f = 0; f < 2; f++) {
-                flow_range(line, g.p, me, f, part == 1, lo[f], hi[f]);
-                cu[f].seek(g, c.scan, per_entry, n_entries, part == 1, lo[f], hi[f]);
-            }
-            const int rounds = hi[0] - lo[0];
-            for (int r = 0; r < rounds && ok; r++) {
-                const bool act0 = cu[0].live(), act1 = cu[1].live() && cu[1].flow_rows(g, 1) > 0;
-                for (int f = 0; f < 2 && ok; f++) {
-                    if (pv[f]) do_pv(f, paired_before && f == 0 && pv[1]);
-                    if (!ok) break;
-                    const bool act = f ? act1 : act0;
-                    pv[f] = act;
-                    if (act) {
-                        if (f == 0 || !paired) take(k_slot);
-                        if (!ok) break;
-                        if (fresh[f] || cu[f].t == 0) {  // a new segment: its Q
-                            ok = pa_wait(c, &c.q_full[f], q_ph[f], err);
-                            if (!ok) break;
-                            q_ph[f] ^= 1;
-                        }
-                        tc_after();
-                        if (lane == 0) {
-                            const uint32_t q = smem_addr(sm + f * Q_BYTES), k = smem_addr(ring + k_slot * KV_BYTES);
+        while (ok && !(ended[0] && ended[1] && !pv[0] && !pv[1])) {
+            bool act1 = false;  // a paired round's second half has rows
 #pragma unroll
-                            for (int j = 0; j < D / 16; j++) {
-                                const uint32_t o = (j >> 2) * HALF + (j & 3) * 32;
-                                mma_ss(tmem + f * 128, pa_desc(q + o, 16), pa_desc(k + o, 16), id_qk, j > 0 ? 1u : 0u);
-                            }
-                            if (!(paired && f == 0 && act1)) tc_commit(&c.empty[k_slot]);
-                            tc_commit(&c.s_full[f]);
-                        }
-                        __syncwarp();
-                        pv_first[f] = fresh[f] || cu[f].t == 0;
-                        pv_last[f] = cu[f].t + 1 == cu[f].nt || cu[f].step + 1 == cu[f].hi;
-                        pv_valid[f] = min(PA_TILE, cu[f].kv_end - cu[f].t * PA_TILE);
-                        fresh[f] = false;
-                    }
-                    if (cu[f].live()) cu[f].next(g);
+            for (int f = 0; f < 2; f++) {
+                if (ok && pv[f]) do_pv(f);
+                pv[f] = false;
+                if (!ok || ended[f]) continue;
+                bool fresh = false;
+                if (sg[f].t0 == sg[f].t1) {
+                    ok = fetch(f, at[f], sg[f]);
+                    if (!ok) continue;
+                    ended[f] = sg[f].flags & SEG_END;
+                    if (ended[f]) continue;
+                    fresh = true;
                 }
-                paired_before = paired;
+                const int t = sg[f].t0++;
+                if (sg[f].n == 0) continue;
+                const bool paired = sg[f].flags & SEG_PAIRED;
+                if (f == 0 && paired) act1 = sg[0].n1 > 0;
+                if (f == 0 || !paired) take(k_slot);
+                if (!ok) continue;
+                if (fresh) {  // a new segment: its Q
+                    ok = pa_wait(c, &c.q_full[f], q_ph[f], err);
+                    if (!ok) continue;
+                    q_ph[f] ^= 1;
+                }
+                tc_after();
+                if (lane == 0) {
+                    const uint64_t q = pa_desc(smem_addr(sm + f * Q_BYTES), 16), k = pa_desc(smem_addr(ring + k_slot * KV_BYTES), 16);
+#pragma unroll
+                    for (int j = 0; j < D / 16; j++) {
+                        const uint32_t o = ((j >> 2) * HALF + (j & 3) * 32) >> 4;
+                        mma_ss(tmem + f * 128, q + o, k + o, id_qk, j > 0);
+                    }
+                    if (!(f == 0 && act1)) tc_commit(&c.empty[k_slot]);
+                    tc_commit(&c.s_full[f]);
+                }
+                __syncwarp();
+                pv[f] = true;
+                pv_pair[f] = paired;
+                pv_first[f] = fresh;
+                pv_last[f] = sg[f].t0 == sg[f].t1;
+                pv_valid[f] = min(PA_TILE, sg[f].kv_end - t * PA_TILE);
             }
         }
-        for (int f = 0; f < 2 && ok; f++)
-            if (pv[f]) do_pv(f, paired_before && f == 0 && pv[1]);
         if (lane == 0) tc_commit(&c.done);
         __syncwarp();
         if (!mbar_wait_ns(&c.done, 0, 2000000000ull) && lane == 0) flag_error(err, ERR_PA_WAIT, 1);
+    } else {
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(PA_REGS_LOW));
+        if (warp == 10 && lane == 0) {
+            // ------------------------------ scheduler ------------------------------
+            const Line line(g.p, so);
+            unsigned at[2] = {0, 0};
+            bool ok = true;
+            auto put = [&](int f, const PaSeg& o) {
+                const int i = at[f] % PA_SEGS;
+                ok = pa_wait(c, &c.seg_empty[f][i], ((at[f] / PA_SEGS) & 1u) ^ 1u, err);
+                if (!ok) return;
+                c.seg[f][i] = o;
+                mbar_arrive(&c.seg_full[f][i]);
+                at[f]++;
+            };
+            PaSeg stop;
+            stop.t0 = 0, stop.t1 = 1, stop.n = stop.n1 = stop.pad = 0, stop.flags = 0;
+            stop.kh = stop.b = stop.kv_end = stop.row0 = stop.voff = stop.slot = 0;
+#pragma unroll 1
+            for (int part = 0; part < 2 && ok; part++) {
+                const bool paired = part ? g.p.pair_o : g.p.pair_p;
+                PaCursor cu[2];
+                int rounds[2] = {0, 0};
+#pragma unroll 1
+                for (int f = 0; f < 2; f++) {
+                    flow_range(line, g.p, me, f, part == 1, cu[f].step, cu[f].hi);
+                    cu[f].seek(g, c.scan, per_entry, n_entries, part == 1);
+                }
+                // flows that take their steps apart: the one behind in rounds gets the next segment
+                while (ok) {
+                    const int f = paired || cu[1].step >= cu[1].hi || (cu[0].step < cu[0].hi && rounds[0] <= rounds[1]) ? 0 : 1;
+                    PaCursor& k = cu[f];
+                    if (k.step >= k.hi) break;
+                    PaSeg o = k.segment(g, part == 1, paired, 0, paired ? me : 2 * me + f);
+                    if (paired) {
+                        PaSeg o1 = k.segment(g, part == 1, true, 1, me);
+                        o.n1 = o1.n;
+                        put(0, o);
+                        if (ok) put(1, o1);
+                    } else {
+                        put(f, o);
+                    }
+                    rounds[f] += o.t1 - o.t0;
+                    k.step += o.t1 - o.t0;
+                    k.next_item(g, part == 1);
+                }
+                // both flows take the same number of rounds
+                if (!paired && rounds[1] < rounds[0] && ok) put(1, stop);
+            }
+            stop.flags = SEG_END;
+            for (int f = 0; f < 2 && ok; f++) put(f, stop);
+        }
     }
     tc_before();
     __syncthreads();

@@ -18,6 +18,7 @@ struct PrefixAttnArgs {
     const void* q;
     int64_t q_stride;
     int n_heads, n_kv, group;   // group: query heads of a kv head
+    uint64_t group_mul;         // ceil(2^36 / group)
     float scale;
     const void* k;
     const void* v;
@@ -29,6 +30,8 @@ struct PrefixAttnArgs {
     int8_t* xq;
     uint16_t* xd;
     int* err;
+    // x / group by a multiplication: exact for 0 <= x < 2^28 (group_mul * group < 2^36 + 128)
+    __host__ __device__ __forceinline__ int group_div(int x) const { return (int)(((uint64_t)x * group_mul) >> 36); }
 };
 
 struct PrefixPlan {
@@ -82,13 +85,14 @@ struct OwnSteps {
     __device__ __forceinline__ int blocks(const SeqInfo& i) const { return (i.q * a.group + p.ob - 1) / p.ob; }
     // own positions that row block rb sees (those of its last row), and its tiles
     __device__ __forceinline__ int visible(const SeqInfo& i, int rb) const {
-        return own_visible(i, (min(i.q * a.group, (rb + 1) * p.ob) - 1) / a.group);
+        return own_visible(i, a.group_div(min(i.q * a.group, (rb + 1) * p.ob) - 1));
     }
     __device__ __forceinline__ int tiles(const SeqInfo& i, int rb) const {
         return (visible(i, rb) + p.tile - 1) / p.tile;
     }
     __device__ __forceinline__ int per_head(const SeqInfo& i) const {
         int n = 0;
+#pragma unroll 1
         for (int rb = blocks(i) - 1; rb >= 0; rb--) n += tiles(i, rb);
         return n;
     }
@@ -98,23 +102,29 @@ struct OwnSteps {
 };
 
 // The line of steps: prefix steps weigh wp, own steps wo; worker c takes the steps that start in
-// [W c / workers, W (c + 1) / workers).
+// [W c / n, W (c + 1) / n), n workers, W < 2^31 as the host checks.
 struct Line {
-    int64_t w, split;  // total weight; weight of the prefix part
+    int w, split;      // total weight; weight of the prefix part
     int sp, so, n, wp, wo;
+    int quot, rem;     // W / n
     __device__ __forceinline__ Line(const PrefixPlan& p, int own_steps)
         : sp(p.sp), so(own_steps), n(p.workers), wp(p.wp), wo(p.wo) {
-        split = (int64_t)sp * wp;
-        w = split + (int64_t)so * wo;
+        split = sp * wp;
+        w = split + so * wo;
+        quot = w / n;
+        rem = w - quot * n;
     }
+    __device__ __forceinline__ int start(int c) const { return quot * c + rem * c / n; }  // floor(W c / n)
     __device__ __forceinline__ int first(int c, bool own) const {
-        const int64_t x = w * c / n;
-        if (!own) return (int)min((x + wp - 1) / wp, (int64_t)sp);
-        return (int)min(max(x - split + wo - 1, (int64_t)0) / wo, (int64_t)so);
+        const int x = start(c);
+        return own ? min((max(x - split, 0) + wo - 1) / wo, so) : min((x + wp - 1) / wp, sp);
     }
     __device__ __forceinline__ int owner(int step, bool own) const {
-        const int64_t at = own ? split + (int64_t)step * wo : (int64_t)step * wp;
-        return (int)(((at + 1) * n - 1) / w);
+        const int at = own ? split + step * wo : step * wp;
+        int c = min(n - 1, (int)(((float)at + 1.0f) * (float)n / (float)w));  // a guess, then the step's place
+        while (c > 0 && start(c) > at) c--;
+        while (c + 1 < n && start(c + 1) <= at) c++;
+        return c;
     }
 };
 
