@@ -75,6 +75,11 @@ __device__ __forceinline__ void tc_commit(uint64_t* bar) {
     asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(smem_addr(bar))
                  : "memory");
 }
+__device__ __forceinline__ bool elect_one() {
+    uint32_t p;
+    asm volatile("{\n .reg .pred p;\n elect.sync _|p, 0xffffffff;\n selp.u32 %0, 1, 0, p;\n}" : "=r"(p));
+    return p != 0;
+}
 __device__ __forceinline__ float ex2(float x) {
     float y;
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
@@ -147,6 +152,14 @@ __device__ __forceinline__ bool pa_wait(PaCtl& c, uint64_t* bar, unsigned parity
             }
         }
     }
+}
+
+// The same by a whole warp, whose control flow the vote keeps uniform: tcgen05.mma and TMA take
+// their operands from uniform registers, and moving them there lane by lane made the issue of an
+// MMA cost twice its execution.
+__device__ __forceinline__ bool pa_wait_warp(PaCtl& c, uint64_t* bar, unsigned parity, int* err) {
+    if (__all_sync(0xffffffffu, mbar_try_wait(bar, parity))) return true;
+    return __all_sync(0xffffffffu, pa_wait(c, bar, parity, err));
 }
 
 struct PaArgs {
@@ -264,7 +277,7 @@ prefix_attn_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_co
     uint8_t* const sm = smem_raw + (((raw + 1023) & ~1023u) - raw);
     uint8_t* const ring = sm + 2 * Q_BYTES;
     PaCtl& c = *reinterpret_cast<PaCtl*>(ring + PA_STAGES * KV_BYTES);
-    const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+    const int tid = threadIdx.x, warp = __shfl_sync(0xffffffffu, tid >> 5, 0), lane = tid & 31;
     int* const err = g.a.err;
 
     if (tid == 0) {
@@ -324,7 +337,7 @@ prefix_attn_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_co
     tc_before();
     __syncthreads();
     tc_after();
-    const uint32_t tmem = c.tmem;
+    const uint32_t tmem = __shfl_sync(0xffffffffu, c.tmem, 0);
     const int so = c.scan[n_entries];
     if (blockIdx.x == 0) {  // the sequences' places in the line, for the merge
 #pragma unroll 1
@@ -339,15 +352,15 @@ prefix_attn_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_co
         if (tid == 0) g.p.cum[g.s.n_seqs] = so;
     }
     const int me = blockIdx.x;
-    // the next segment of flow f, for a reader that keeps its place (index, parity) in `at`
+    // the next segment of flow f, for a warp that keeps its place in `at`
     auto fetch = [&](int f, unsigned& at, PaSeg& o) {
         const int i = at % PA_SEGS;
-        if (!pa_wait(c, &c.seg_full[f][i], (at / PA_SEGS) & 1u, err)) return false;
-        const int4* src = reinterpret_cast<const int4*>(&c.seg[f][i]);
-        const int4 x = src[0], y = src[1], z = src[2];
-        o.t0 = x.x, o.t1 = x.y, o.n = x.z, o.flags = x.w;
-        o.kh = y.x, o.b = y.y, o.kv_end = y.z, o.row0 = y.w;
-        o.voff = z.x, o.slot = z.y, o.n1 = z.z;
+        if (!pa_wait_warp(c, &c.seg_full[f][i], (at / PA_SEGS) & 1u, err)) return false;
+        const int v = reinterpret_cast<const int*>(&c.seg[f][i])[lane < 12 ? lane : 0];
+        auto field = [&](int k) { return __shfl_sync(0xffffffffu, v, k); };  // uniform in the warp
+        o.t0 = field(0), o.t1 = field(1), o.n = field(2), o.flags = field(3);
+        o.kh = field(4), o.b = field(5), o.kv_end = field(6), o.row0 = field(7);
+        o.voff = field(8), o.slot = field(9), o.n1 = field(10);
         __syncwarp();
         if (lane == 0) mbar_arrive(&c.seg_empty[f][i]);
         at++;
@@ -512,7 +525,7 @@ prefix_attn_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_co
         sg[0].t0 = sg[0].t1 = sg[1].t0 = sg[1].t1 = 0;
         int pg[2] = {0, 0}, krow[2] = {0, 0}, vkh[2] = {0, 0};  // this lane's page of the flow's tile, kept from K for V
         auto load = [&](const CUtensorMap* map, int pid, int prow, int kh) {
-            ok = pa_wait(c, &c.empty[slot], ph ^ 1u, err);
+            ok = pa_wait_warp(c, &c.empty[slot], ph ^ 1u, err);
             if (!ok) return;
             if (lane == 0) mbar_expect_tx(&c.full[slot], KV_BYTES);
             __syncwarp();
@@ -575,7 +588,7 @@ prefix_attn_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_co
         bool pv[2] = {false, false}, pv_pair[2] = {false, false}, pv_first[2] = {false, false}, pv_last[2] = {false, false};
         int pv_valid[2] = {0, 0};
         auto take = [&](int& where) {  // the next stage of the ring
-            ok = pa_wait(c, &c.full[slot], ph, err);
+            ok = pa_wait_warp(c, &c.full[slot], ph, err);
             where = slot;
             if (++slot == PA_STAGES) slot = 0, ph ^= 1;
         };
@@ -596,12 +609,12 @@ prefix_attn_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_co
                     __syncwarp();
                 }
             }
-            ok = pa_wait(c, &c.p_full[f], p_ph[f], err);
+            ok = pa_wait_warp(c, &c.p_full[f], p_ph[f], err);
             if (!ok) return;
             p_ph[f] ^= 1;
             tc_after();
-            if (lane == 0) {
-                const uint64_t v = pa_desc(smem_addr(ring + v_slot * KV_BYTES), HALF);
+            const uint64_t v = pa_desc(smem_addr(ring + v_slot * KV_BYTES), HALF);
+            if (elect_one()) {
 #pragma unroll
                 for (int j = 0; j < PA_TILE / 16; j++)
                     mma_ts(tmem + 256 + f * 128, tmem + f * 128 + j * 8, v + j * (2048 >> 4), id_pv,
@@ -633,13 +646,13 @@ prefix_attn_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_co
                 if (f == 0 || !paired) take(k_slot);
                 if (!ok) continue;
                 if (fresh) {  // a new segment: its Q
-                    ok = pa_wait(c, &c.q_full[f], q_ph[f], err);
+                    ok = pa_wait_warp(c, &c.q_full[f], q_ph[f], err);
                     if (!ok) continue;
                     q_ph[f] ^= 1;
                 }
                 tc_after();
-                if (lane == 0) {
-                    const uint64_t q = pa_desc(smem_addr(sm + f * Q_BYTES), 16), k = pa_desc(smem_addr(ring + k_slot * KV_BYTES), 16);
+                const uint64_t q = pa_desc(smem_addr(sm + f * Q_BYTES), 16), k = pa_desc(smem_addr(ring + k_slot * KV_BYTES), 16);
+                if (elect_one()) {
 #pragma unroll
                     for (int j = 0; j < D / 16; j++) {
                         const uint32_t o = ((j >> 2) * HALF + (j & 3) * 32) >> 4;
