@@ -119,12 +119,11 @@ __device__ __forceinline__ void tmem_ld32(uint32_t* r, uint32_t addr) {
         : PA_R8(r, 0), PA_R8(r, 8), PA_R8(r, 16), PA_R8(r, 24)
         : "r"(addr));
 }
-__device__ __forceinline__ void tmem_st32(uint32_t addr, const uint32_t* r) {
+__device__ __forceinline__ void tmem_ld16(uint32_t* r, uint32_t addr) {
     asm volatile(
-        "tcgen05.st.sync.aligned.32x32b.x32.b32 [%32], {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,"
-        "%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31};" ::PA_I8(r, 0),
-        PA_I8(r, 8), PA_I8(r, 16), PA_I8(r, 24), "r"(addr)
-        : "memory");
+        "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
+        : PA_R8(r, 0), PA_R8(r, 8)
+        : "r"(addr));
 }
 __device__ __forceinline__ void tmem_st16(uint32_t addr, const uint32_t* r) {
     asm volatile(
@@ -160,6 +159,12 @@ __device__ __forceinline__ bool pa_wait(PaCtl& c, uint64_t* bar, unsigned parity
 __device__ __forceinline__ bool pa_wait_warp(PaCtl& c, uint64_t* bar, unsigned parity, int* err) {
     if (__all_sync(0xffffffffu, mbar_try_wait(bar, parity))) return true;
     return __all_sync(0xffffffffu, pa_wait(c, bar, parity, err));
+}
+
+__device__ __forceinline__ float max3(float a, float b, float c) {
+    float d;
+    asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+    return d;
 }
 
 struct PaArgs {
@@ -414,68 +419,87 @@ prefix_attn_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_co
                 s_ph ^= 1;
                 tc_after();
                 if (busy) {
-                    // two passes over S, 32 columns at a time: the maximum, then the probabilities.
-                    // Reading S twice from TMEM costs less than the registers and the straight-line
-                    // code that 128 columns at once would take.
                     const int lim = vis - t * PA_TILE;  // columns this row sees
-                    float mt = -INFINITY;
+                    // a larger maximum: when a row's grew by more than 2^8, l and O follow
+                    auto raise = [&](float mt) {
+                        mt *= cs;
+                        if (t == sg.t0) {
+                            m = mt;
+                        } else if (__any_sync(0xffffffffu, mt > m + 8.0f)) {
+                            const float mn = fmaxf(m, mt);
+                            const float k = mn == -INFINITY ? 1.0f : ex2(m - mn);
+                            l *= k;
+                            m = mn;
 #pragma unroll 1
-                    for (int j = 0; j < PA_TILE; j += 32) {
-                        float s[32];
-                        tmem_ld32(reinterpret_cast<uint32_t*>(s), t_s + j);
+                            for (int i = 0; i < D; i += 16) {
+                                uint32_t r[16];
+                                tmem_ld16(r, t_o + i);
+                                tmem_wait_ld();
+#pragma unroll
+                                for (int j = 0; j < 16; j++) r[j] = __float_as_uint(__uint_as_float(r[j]) * k);
+                                tmem_st16(t_o + i, r);
+                            }
+                        }
+                        return m == -INFINITY ? 0.0f : -m;
+                    };
+                    if (__all_sync(0xffffffffu, lim >= PA_TILE)) {
+                        float s[128];
+#pragma unroll
+                        for (int j = 0; j < 4; j++) tmem_ld32(reinterpret_cast<uint32_t*>(s) + 32 * j, t_s + 32 * j);
                         tmem_wait_ld();
-                        if (!__all_sync(0xffffffffu, lim >= j + 32)) {
+                        float mx[4] = {s[0], s[1], s[2], s[3]};
 #pragma unroll
-                            for (int i = 0; i < 32; i++)
-                                if (j + i >= lim) s[i] = -INFINITY;
+                        for (int i = 4; i < 124; i += 8)
+#pragma unroll
+                            for (int j = 0; j < 4; j++) mx[j] = max3(mx[j], s[i + 2 * j], s[i + 2 * j + 1]);
+                        const float neg = raise(fmaxf(max3(mx[0], mx[1], max3(mx[2], s[124], s[125])), max3(mx[3], s[126], s[127])));
+                        const float2 cs2 = make_float2(cs, cs), neg2 = make_float2(neg, neg);
+                        float2 sum[2] = {make_float2(0.0f, 0.0f), make_float2(0.0f, 0.0f)};
+#pragma unroll
+                        for (int j = 0; j < 4; j++) {
+                            uint32_t pk[16];
+#pragma unroll
+                            for (int i = 0; i < 16; i++) {
+                                const float2 x = __ffma2_rn(make_float2(s[32 * j + 2 * i], s[32 * j + 2 * i + 1]), cs2, neg2);
+                                const float2 e = make_float2(ex2(x.x), ex2(x.y));
+                                sum[i & 1] = __fadd2_rn(sum[i & 1], e);
+                                pk[i] = pack_bf16x2(e.x, e.y);
+                            }
+                            tmem_st16(t_s + 16 * j, pk);
                         }
-                        float mx[4] = {mt, s[0], s[1], s[2]};
-#pragma unroll
-                        for (int i = 3; i < 32; i++) mx[i & 3] = fmaxf(mx[i & 3], s[i]);
-                        mt = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3]));
-                    }
-                    mt *= cs;
-                    if (t == sg.t0) {
-                        m = mt;
-                    } else if (__any_sync(0xffffffffu, mt > m + 8.0f)) {
-                        const float mn = fmaxf(m, mt);
-                        const float k = mn == -INFINITY ? 1.0f : ex2(m - mn);
-                        l *= k;
-                        m = mn;
+                        l += (sum[0].x + sum[0].y) + (sum[1].x + sum[1].y);
+                    } else {
+                        // the ends of items: two passes over S, 32 columns at a time (little code)
+                        float mt = -INFINITY, sum = 0.0f, neg = 0.0f;
 #pragma unroll 1
-                        for (int i = 0; i < D; i += 32) {
-                            uint32_t r[32];
-                            tmem_ld32(r, t_o + i);
-                            tmem_wait_ld();
-#pragma unroll
-                            for (int j = 0; j < 32; j++) r[j] = __float_as_uint(__uint_as_float(r[j]) * k);
-                            tmem_st32(t_o + i, r);
-                        }
-                    }
-                    const float neg = m == -INFINITY ? 0.0f : -m;
-                    float sum[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+                        for (int pass = 0; pass < 2; pass++) {
 #pragma unroll 1
-                    for (int j = 0; j < PA_TILE; j += 32) {
-                        float s[32];
-                        tmem_ld32(reinterpret_cast<uint32_t*>(s), t_s + j);
-                        tmem_wait_ld();
-                        if (!__all_sync(0xffffffffu, lim >= j + 32)) {
+                            for (int j = 0; j < PA_TILE; j += 32) {
+                                float s[32];
+                                tmem_ld32(reinterpret_cast<uint32_t*>(s), t_s + j);
+                                tmem_wait_ld();
 #pragma unroll
-                            for (int i = 0; i < 32; i++)
-                                if (j + i >= lim) s[i] = -INFINITY;
-                        }
-                        uint32_t pk[16];
+                                for (int i = 0; i < 32; i++)
+                                    if (j + i >= lim) s[i] = -INFINITY;
+                                if (pass == 0) {
 #pragma unroll
-                        for (int i = 0; i < 16; i++) {
-                            const float p0 = ex2(fmaf(s[2 * i], cs, neg)), p1 = ex2(fmaf(s[2 * i + 1], cs, neg));
-                            sum[i & 1] += p0;
-                            sum[2 + (i & 1)] += p1;
-                            pk[i] = pack_bf16x2(p0, p1);
+                                    for (int i = 0; i < 32; i += 2) mt = max3(mt, s[i], s[i + 1]);
+                                } else {
+                                    uint32_t pk[16];
+#pragma unroll
+                                    for (int i = 0; i < 16; i++) {
+                                        const float p0 = ex2(fmaf(s[2 * i], cs, neg)), p1 = ex2(fmaf(s[2 * i + 1], cs, neg));
+                                        sum += p0 + p1;
+                                        pk[i] = pack_bf16x2(p0, p1);
+                                    }
+                                    // P of columns j.. lands on S columns j/2.., which have been read
+                                    tmem_st16(t_s + j / 2, pk);
+                                }
+                            }
+                            if (pass == 0) neg = raise(mt);
                         }
-                        // P of columns j.. lands on S columns j/2.., which have been read
-                        tmem_st16(t_s + j / 2, pk);
+                        l += sum;
                     }
-                    l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
                     tmem_wait_st();
                 }
                 tc_before();
