@@ -247,7 +247,7 @@ static int make_plan(lq_ctx* ctx, const PrefixAttnArgs& a, const PagedSeqs& s, i
     LQ_REQUIRE(ctx, steps < (1ll << 26), "lq_prefix_attention: %lld steps, more than a launch can number", (long long)steps);
     p->sp = (int)(items_p * p->np);
     p->workers = (int)std::max<int64_t>(1, std::min<int64_t>(ctx->sm_count, steps));
-    p->wp = p->wo = 1;
+    p->workers_mul = ((1ull << 40) + p->workers - 1) / p->workers;
     const int64_t slots_p = p->np ? items_p + 2 * p->workers : 0, slots_o = items_o + 2 * p->workers;
     auto al = [](size_t b) { return (b + 255) & ~(size_t)255; };
     const size_t cum = al((size_t)(s.n_seqs + 1) * 4), ml_p = al((size_t)slots_p * p->cap_p * 8),

@@ -37,10 +37,10 @@ constexpr int PA_ROWS = 128;      // rows of a flow (MMA M)
 constexpr int PA_TILE = 128;      // positions of a step
 constexpr int PA_STAGES = 4;
 constexpr int PA_THREADS = 384;   // warps 0-7 softmax, 8 TMA, 9 MMA, 10 scheduler, 11 nothing
-constexpr int PA_SEGS = 4;        // segments handed to a flow ahead
 // registers: 384 x 168 at launch = 256 x 216 for the softmax warps + 128 x 72 for the others
 constexpr int PA_REGS = 216, PA_REGS_LOW = 72;
 constexpr int PA_SCAN = 1024;     // entries of the scan over the sequences
+constexpr int PA_BATCH = 32;      // segments the scheduler works out at a time, a lane each
 constexpr int ERR_PA_WAIT = 94;   // a wait ran out
 
 enum { SEG_OWN = 1, SEG_PAIRED = 2, SEG_END = 4, SEG_WHOLE = 8 };
@@ -60,12 +60,14 @@ struct alignas(16) PaSeg {
 
 struct PaCtl {
     uint64_t full[PA_STAGES], empty[PA_STAGES];
-    uint64_t seg_full[2][PA_SEGS], seg_empty[2][PA_SEGS];
+    uint64_t seg_full[2][2], seg_empty[2][2];  // per flow: two batches of segments
     uint64_t q_full[2], s_full[2], p_full[2], o_full[2], done;
     uint32_t tmem;
     int abort;
-    PaSeg seg[2][PA_SEGS];
-    int scan[PA_SCAN + 1];
+    int seg_n[2][2];
+    PaSeg seg[2][2][PA_BATCH];
+    int4 info[PA_SCAN];     // up to PA_SCAN sequences: q0, q, kv
+    int scan[PA_SCAN + 1];  // own steps before each entry
 };
 
 __device__ __forceinline__ void tc_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
@@ -134,31 +136,31 @@ __device__ __forceinline__ void tmem_st16(uint32_t addr, const uint32_t* r) {
 __device__ __forceinline__ void tmem_wait_ld() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
 __device__ __forceinline__ void tmem_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 
-// bounded wait: 2 s, or another warp of the CTA gave up. try_wait itself sleeps for a while; the
-// abort flag and the (slow, shared) global timer are looked at once in many polls.
-__device__ __forceinline__ bool pa_wait(PaCtl& c, uint64_t* bar, unsigned parity, int* err) {
-    uint64_t t0 = 0;
-    for (unsigned i = 0;; i++) {
+// Bounded wait: PA_POLLS polls (try_wait sleeps between them), or until another warp of the CTA
+// gave up; then the CTA tears down and reports.
+constexpr int PA_POLLS = 1 << 22;
+__device__ __forceinline__ bool pa_wait(PaCtl& c, uint64_t* bar, unsigned parity) {
+#pragma unroll 1
+    for (int i = 0; i < PA_POLLS && !*reinterpret_cast<volatile int*>(&c.abort); i++)
         if (mbar_try_wait(bar, parity)) return true;
-        if ((i & 255) == 255) {
-            if (*reinterpret_cast<volatile int*>(&c.abort)) return false;
-            const uint64_t now = global_ns();
-            if (t0 == 0) t0 = now;
-            if (now - t0 > 2000000000ull) {
-                *reinterpret_cast<volatile int*>(&c.abort) = 1;
-                flag_error(err, ERR_PA_WAIT, 0);
-                return false;
-            }
-        }
-    }
+    *reinterpret_cast<volatile int*>(&c.abort) = 1;
+    return false;
 }
-
 // The same by a whole warp, whose control flow the vote keeps uniform: tcgen05.mma and TMA take
 // their operands from uniform registers, and moving them there lane by lane made the issue of an
 // MMA cost twice its execution.
-__device__ __forceinline__ bool pa_wait_warp(PaCtl& c, uint64_t* bar, unsigned parity, int* err) {
-    if (__all_sync(0xffffffffu, mbar_try_wait(bar, parity))) return true;
-    return __all_sync(0xffffffffu, pa_wait(c, bar, parity, err));
+__device__ __forceinline__ bool pa_wait_warp(PaCtl& c, uint64_t* bar, unsigned parity) {
+#pragma unroll 1
+    for (int i = 0; i < PA_POLLS && !__any_sync(0xffffffffu, *reinterpret_cast<volatile int*>(&c.abort)); i++)
+        if (__all_sync(0xffffffffu, mbar_try_wait(bar, parity))) return true;
+    *reinterpret_cast<volatile int*>(&c.abort) = 1;
+    return false;
+}
+template <typename T>
+__device__ __forceinline__ void exchange(T& a, T& b) {
+    const T t = a;
+    a = b;
+    b = t;
 }
 
 __device__ __forceinline__ float max3(float a, float b, float c) {
@@ -173,103 +175,85 @@ struct PaArgs {
     PrefixPlan p;
 };
 
-// A flow's place in its part of the line (the scheduler's).
-struct PaCursor {
-    int step, hi;       // steps of the part: the next one, and the flow's end
-    int b, kh, rb, n_rb;
-    int t, nt;          // tile of the item
-    SeqInfo si;
+__device__ __forceinline__ int warp_scan(int v, int lane) {  // inclusive sum
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+        const int u = __shfl_up_sync(0xffffffffu, v, o);
+        if (lane >= o) v += u;
+    }
+    return v;
+}
 
-    __device__ __forceinline__ void seek(const PaArgs& g, const int* scan, int per_entry, int n_entries, bool own) {
-        if (step >= hi) return;
-        if (!own) {
-            const int item = step / g.p.np;
-            t = step - item * g.p.np;
-            nt = g.p.np;
-            n_rb = g.p.n_rb;
-            kh = item / n_rb;
-            rb = item - kh * n_rb;
-            b = 0;
-            return;
-        }
-        int e0 = 0, e1 = n_entries;  // the last entry with scan <= step
+// steps of one head of a sequence, by a warp
+__device__ __forceinline__ int per_head_warp(const OwnSteps& o, const SeqInfo& si, int lane) {
+    const int n_rb = o.blocks(si);
+    int n = 0;
 #pragma unroll 1
-        while (e1 - e0 > 1) {
-            const int m = (e0 + e1) >> 1;
-            if (scan[m] <= step) e0 = m;
-            else e1 = m;
-        }
-        const OwnSteps o{g.a, g.p};
-        int rest = step - scan[e0], per = 0;
-#pragma unroll 1
-        for (b = e0 * per_entry; b < g.s.n_seqs; b++) {
-            si = seq_info(g.a, g.s, b, false);
-            per = o.per_head(si);
-            if (rest < per * g.a.n_kv) break;
-            rest -= per * g.a.n_kv;
-        }
-        if (b >= g.s.n_seqs) {  // lengths that changed under the kernel
-            hi = step;
-            return;
-        }
-        kh = rest / per;
-        rest -= kh * per;
-        n_rb = o.blocks(si);
-        rb = 0;
-#pragma unroll 1
-        while (rb + 1 < n_rb && rest >= o.tiles(si, rb)) rest -= o.tiles(si, rb++);
-        nt = o.tiles(si, rb);
-        t = rest;
-    }
-    // to the next item with a step, unless the flow's end is reached
-    __device__ __forceinline__ void next_item(const PaArgs& g, bool own) {
-        t = 0;
-        while (step < hi) {
-            if (++rb >= n_rb) {
-                rb = 0;
-                kh++;
-                if (own && kh == g.a.n_kv) {
-                    kh = 0;
-                    if (++b >= g.s.n_seqs) {  // lengths that changed under the kernel
-                        hi = step;
-                        return;
-                    }
-                    si = seq_info(g.a, g.s, b, false);
-                    n_rb = OwnSteps{g.a, g.p}.blocks(si);
-                    if (n_rb == 0 || si.kv == 0) {  // nothing of this sequence
-                        kh = g.a.n_kv - 1;
-                        rb = n_rb;
-                        continue;
-                    }
-                }
-            }
-            if (!own) return;
-            nt = OwnSteps{g.a, g.p}.tiles(si, rb);
-            if (nt > 0) return;
-        }
-    }
-    __device__ __forceinline__ PaSeg segment(const PaArgs& g, bool own, bool paired, int half, int worker) const {
-        PaSeg o;
-        const int block = own ? g.p.ob : g.p.pb, cap = own ? g.p.cap_o : g.p.cap_p;
-        const int start = own ? si.q0 * g.a.group : 0, total = own ? si.q * g.a.group : g.s.rows * g.a.group;
-        const int left = total - rb * block - half * PA_ROWS;
-        const OwnSteps os{g.a, g.p};
-        o.t0 = t;
-        o.t1 = min(nt, t + hi - step);
-        o.n = max(0, min(PA_ROWS, left));
-        o.flags = (own ? SEG_OWN : 0) | (paired ? SEG_PAIRED : 0) |
-                  (g.a.prefix_len == 0 && o.t0 == 0 && o.t1 == nt ? SEG_WHOLE : 0);
-        o.kh = kh;
-        o.b = b;
-        o.kv_end = own ? os.visible(si, rb) : g.a.prefix_len;
-        o.row0 = start + rb * block + half * PA_ROWS;
-        o.voff = own ? si.kv - si.q + 1 - si.q0 : 0;
-        const int item = (own ? g.a.n_kv * os.base(si, b) : 0) + kh * n_rb + rb;
-        o.slot = (item + worker) * cap + half * PA_ROWS;
-        o.n1 = o.pad = 0;
-        return o;
-    }
+    for (int rb = lane; rb < n_rb; rb += 32) n += o.tiles(si, rb);
+    return __reduce_add_sync(0xffffffffu, n);
+}
+
+// A flow's place in its part of the line: the scheduler warp's, the same in every lane.
+struct PaWalk {
+    int step, hi;   // steps of the part: the next one, and the flow's end
+    int b, j;       // sequence (own part), item: kh * n_rb + rb
+    int t;          // tile of the item
 };
+
+__device__ __forceinline__ SeqInfo pa_seq(const PaArgs& g, const PaCtl& c, int b) {
+    if (g.s.n_seqs > PA_SCAN) return seq_info(g.a, g.s, b, false);
+    const int4 v = c.info[b];
+    return SeqInfo{v.x, v.y, v.z};
+}
+
+__device__ __forceinline__ void pa_seek(const PaArgs& g, const PaCtl& c, int per_entry, int n_entries, bool own, int lane,
+                                        PaWalk& w) {
+    if (w.step >= w.hi) return;
+    if (!own) {
+        w.j = w.step / g.p.np;
+        w.t = w.step - w.j * g.p.np;
+        w.b = 0;
+        return;
+    }
+    int e0 = 0, e1 = n_entries;  // the last entry with scan <= step
+#pragma unroll 1
+    while (e1 - e0 > 1) {
+        const int m = (e0 + e1) >> 1;
+        if (c.scan[m] <= w.step) e0 = m;
+        else e1 = m;
+    }
+    const OwnSteps o{g.a, g.p};
+    int rest = w.step - c.scan[e0], per = 1;
+    SeqInfo si{0, 0, 0};
+#pragma unroll 1
+    for (w.b = e0 * per_entry; w.b < g.s.n_seqs; w.b++) {
+        si = pa_seq(g, c, w.b);
+        per = per_head_warp(o, si, lane);
+        if (rest < per * g.a.n_kv) break;
+        rest -= per * g.a.n_kv;
+    }
+    if (w.b >= g.s.n_seqs) {  // lengths that changed under the kernel
+        w.hi = w.step;
+        return;
+    }
+    const int kh = rest / per, n_rb = o.blocks(si);
+    rest -= kh * per;
+    int rb = 0;
+#pragma unroll 1
+    for (; rb < n_rb; rb += 32) {
+        const int n = rb + lane < n_rb ? o.tiles(si, rb + lane) : 0;
+        const int upto = warp_scan(n, lane), all = __shfl_sync(0xffffffffu, upto, 31);
+        if (rest < all) {
+            const int l = __ffs(__ballot_sync(0xffffffffu, upto > rest)) - 1;
+            rest -= __shfl_sync(0xffffffffu, upto - n, l);
+            rb += l;
+            break;
+        }
+        rest -= all;
+    }
+    w.j = kh * n_rb + rb;
+    w.t = rest;
+}
 
 template <int D>
 __global__ void __launch_bounds__(PA_THREADS, 1)
@@ -287,12 +271,13 @@ prefix_attn_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_co
 
     if (tid == 0) {
         for (int i = 0; i < PA_STAGES; i++) mbar_init(&c.full[i], 1), mbar_init(&c.empty[i], 1);
+#pragma unroll 1
         for (int f = 0; f < 2; f++) {
             mbar_init(&c.q_full[f], 4);
             mbar_init(&c.s_full[f], 1);
             mbar_init(&c.p_full[f], 4);
             mbar_init(&c.o_full[f], 1);
-            for (int i = 0; i < PA_SEGS; i++) {
+            for (int i = 0; i < 2; i++) {
                 mbar_init(&c.seg_full[f][i], 1);
                 mbar_init(&c.seg_empty[f][i], 6);  // four softmax warps, producer, MMA issuer
             }
@@ -311,16 +296,21 @@ prefix_attn_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_co
     }
     pdl_trigger();
     pdl_wait();
-    // own steps of every entry (a run of per_entry sequences), then their running sum
+    // own steps of every entry (a run of per_entry sequences), then their running sum; a warp looks
+    // at a sequence of many row blocks, else a thread
     const int per_entry = (g.s.n_seqs + PA_SCAN - 1) / PA_SCAN;
-    const int n_entries = (g.s.n_seqs + per_entry - 1) / per_entry;
+    const int n_entries = per_entry == 1 ? g.s.n_seqs : (g.s.n_seqs + per_entry - 1) / per_entry;
     const OwnSteps os{g.a, g.p};
+    const bool by_warp = per_entry == 1 && g.p.cap_o == g.p.ob && g.a.max_q * g.a.group > 4 * g.p.ob;
 #pragma unroll 1
-    for (int e = tid; e < n_entries; e += PA_THREADS) {
+    for (int e = by_warp ? warp : tid; e < n_entries; e += by_warp ? PA_THREADS / 32 : PA_THREADS) {
         int n = 0;
 #pragma unroll 1
-        for (int b = e * per_entry; b < min(g.s.n_seqs, (e + 1) * per_entry); b++)
-            n += os.per_head(seq_info(g.a, g.s, b, blockIdx.x == 0)) * g.a.n_kv;
+        for (int b = e * per_entry; b < min(g.s.n_seqs, (e + 1) * per_entry); b++) {
+            const SeqInfo si = seq_info(g.a, g.s, b, blockIdx.x == 0);
+            n += (by_warp ? per_head_warp(os, si, lane) : os.per_head(si)) * g.a.n_kv;
+            if (per_entry == 1) c.info[b] = make_int4(si.q0, si.q, si.kv, 0);
+        }
         c.scan[e + 1] = n;
     }
     __syncthreads();
@@ -328,12 +318,7 @@ prefix_attn_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_co
         int run = 0;
 #pragma unroll 1
         for (int e0 = 0; e0 < n_entries; e0 += 32) {
-            int v = e0 + lane < n_entries ? c.scan[e0 + lane + 1] : 0;
-#pragma unroll
-            for (int o = 1; o < 32; o <<= 1) {
-                const int u = __shfl_up_sync(0xffffffffu, v, o);
-                if (lane >= o) v += u;
-            }
+            const int v = warp_scan(e0 + lane < n_entries ? c.scan[e0 + lane + 1] : 0, lane);
             if (e0 + lane < n_entries) c.scan[e0 + lane + 1] = run + v;
             run += __shfl_sync(0xffffffffu, v, 31);
         }
@@ -357,20 +342,32 @@ prefix_attn_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_co
         if (tid == 0) g.p.cum[g.s.n_seqs] = so;
     }
     const int me = blockIdx.x;
-    // the next segment of flow f, for a warp that keeps its place in `at`
-    auto fetch = [&](int f, unsigned& at, PaSeg& o) {
-        const int i = at % PA_SEGS;
-        if (!pa_wait_warp(c, &c.seg_full[f][i], (at / PA_SEGS) & 1u, err)) return false;
-        const int v = reinterpret_cast<const int*>(&c.seg[f][i])[lane < 12 ? lane : 0];
+    // a warp's place in the segments of a flow
+    struct Feed {
+        int i = 0, n = 0;   // entry of the batch, entries
+        unsigned k = 0;     // batches taken
+    };
+    auto fetch = [&](int f, Feed& d, PaSeg& o) {
+        if (d.i == d.n) {
+            if (d.k > 0) {
+                __syncwarp();
+                if (lane == 0) mbar_arrive(&c.seg_empty[f][(d.k - 1) & 1]);
+            }
+            if (!pa_wait_warp(c, &c.seg_full[f][d.k & 1], (d.k >> 1) & 1u)) return false;
+            d.n = __shfl_sync(0xffffffffu, c.seg_n[f][d.k & 1], 0);
+            d.i = 0;
+            d.k++;
+        }
+        const int v = reinterpret_cast<const int*>(&c.seg[f][(d.k - 1) & 1][d.i++])[lane < 12 ? lane : 0];
         auto field = [&](int k) { return __shfl_sync(0xffffffffu, v, k); };  // uniform in the warp
         o.t0 = field(0), o.t1 = field(1), o.n = field(2), o.flags = field(3);
         o.kh = field(4), o.b = field(5), o.kv_end = field(6), o.row0 = field(7);
         o.voff = field(8), o.slot = field(9), o.n1 = field(10);
-        __syncwarp();
-        if (lane == 0) mbar_arrive(&c.seg_empty[f][i]);
-        at++;
         return true;
     };
+    // Q of a flow: up to 64 rows take one half of the buffer and the next segment's the other
+    // (the MMA's rows past them read whatever lies there), so that they load a segment ahead
+    auto q_offset = [](const PaSeg& o, unsigned turn) { return o.n <= PA_ROWS / 2 ? (turn & 1) * (HALF / 2) : 0u; };
 
     if (warp < 8) {
         // ------------------------------ softmax ------------------------------
@@ -380,34 +377,50 @@ prefix_attn_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_co
         const uint32_t t_lane = (uint32_t)(wq * 32) << 16;
         const uint32_t t_s = tmem + t_lane + f * 128, t_o = tmem + t_lane + 256 + f * 128;
         const float cs = g.a.scale * 1.44269504088896340736f;  // scores in units of log2
-        unsigned s_ph = 0, o_ph = 0, at = 0;
+        unsigned s_ph = 0, o_ph = 0, turn = 0;
+        Feed feed;
 
-        // the next segment with rows (false: none, or a wait ran out), its Q on the way
+        // The next segment with rows: NX_NONE when there is none (or a wait ran out). Looked for
+        // ahead of time, it must not wait for the scheduler (NX_LATER), which may itself wait until
+        // the other warps are through with this segment.
+        enum { NX_NONE, NX_SEG, NX_LATER };
         PaSeg nx;
-        auto begin = [&]() {
+        auto next = [&](bool ahead) {
             do {
-                if (!fetch(f, at, nx)) return false;
-                if (nx.flags & SEG_END) return false;
+                if (ahead && feed.i == feed.n &&
+                    !__all_sync(0xffffffffu, mbar_try_wait(&c.seg_full[f][feed.k & 1], (feed.k >> 1) & 1u)))
+                    return NX_LATER;
+                if (!fetch(f, feed, nx) || (nx.flags & SEG_END)) return NX_NONE;
             } while (nx.n == 0);
+            return NX_SEG;
+        };
+        auto q_start = [&]() {  // its Q on the way to shared memory
+            const uint32_t base = sq + q_offset(nx, turn++);
             constexpr int CH = D / 8;
 #pragma unroll 1
             for (int i = row; i < nx.n * CH; i += 128) {
                 const int r = i / CH, ch = i % CH, t = g.a.group_div(nx.row0 + r);
                 const int h = nx.kh * g.a.group + nx.row0 + r - t * g.a.group;
-                const uint32_t dst = sq + (ch >> 3) * HALF + r * 128 + (((ch & 7) ^ (r & 7)) << 4);
+                const uint32_t dst = base + (ch >> 3) * HALF + r * 128 + (((ch & 7) ^ (r & 7)) << 4);
                 asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst),
                              "l"(static_cast<const __nv_bfloat16*>(g.a.q) + (int64_t)t * g.a.q_stride + h * D + ch * 8));
             }
+        };
+        auto q_finish = [&]() {
             asm volatile("cp.async.wait_all;" ::: "memory");
             proxy_fence();
             __syncwarp();
             if (lane == 0) mbar_arrive(&c.q_full[f]);
-            return true;
         };
 
-        bool more = begin();
-        while (more) {
+        int more = next(false);
+        if (more == NX_SEG) {
+            q_start();
+            q_finish();
+        }
+        while (more == NX_SEG) {
             const PaSeg sg = nx;
+            bool early = false;
             const int st = sg.row0 + min(row, sg.n - 1), tok = g.a.group_div(st);
             const bool mine = row < sg.n, busy = wq * 32 < sg.n;
             const int vis = sg.flags & SEG_OWN ? max(0, tok + sg.voff) : sg.kv_end;
@@ -415,7 +428,7 @@ prefix_attn_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_co
             int t = sg.t0;
 #pragma unroll 1
             for (; t < sg.t1; t++) {
-                if (!pa_wait(c, &c.s_full[f], s_ph, err)) break;
+                if (!pa_wait(c, &c.s_full[f], s_ph)) break;
                 s_ph ^= 1;
                 tc_after();
                 if (busy) {
@@ -442,7 +455,7 @@ prefix_attn_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_co
                         }
                         return m == -INFINITY ? 0.0f : -m;
                     };
-                    if (__all_sync(0xffffffffu, lim >= PA_TILE)) {
+                    if (sg.n > 64 && __all_sync(0xffffffffu, lim >= PA_TILE)) {
                         float s[128];
 #pragma unroll
                         for (int j = 0; j < 4; j++) tmem_ld32(reinterpret_cast<uint32_t*>(s) + 32 * j, t_s + 32 * j);
@@ -469,7 +482,9 @@ prefix_attn_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_co
                         }
                         l += (sum[0].x + sum[0].y) + (sum[1].x + sum[1].y);
                     } else {
-                        // the ends of items: two passes over S, 32 columns at a time (little code)
+                        // few rows, or the end of an item: two passes over S, 32 columns at a time, in
+                        // a tenth of the code (few rows come in many short segments, and there the
+                        // instruction fetch costs more than the arithmetic)
                         float mt = -INFINITY, sum = 0.0f, neg = 0.0f;
 #pragma unroll 1
                         for (int pass = 0; pass < 2; pass++) {
@@ -478,9 +493,11 @@ prefix_attn_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_co
                                 float s[32];
                                 tmem_ld32(reinterpret_cast<uint32_t*>(s), t_s + j);
                                 tmem_wait_ld();
+                                if (!__all_sync(0xffffffffu, lim >= j + 32)) {
 #pragma unroll
-                                for (int i = 0; i < 32; i++)
-                                    if (j + i >= lim) s[i] = -INFINITY;
+                                    for (int i = 0; i < 32; i++)
+                                        if (j + i >= lim) s[i] = -INFINITY;
+                                }
                                 if (pass == 0) {
 #pragma unroll
                                     for (int i = 0; i < 32; i += 2) mt = max3(mt, s[i], s[i + 1]);
@@ -505,10 +522,19 @@ prefix_attn_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_co
                 tc_before();
                 __syncwarp();
                 if (lane == 0) mbar_arrive(&c.p_full[f]);
+                if (t == sg.t0) {
+                    more = next(true);
+                    early = more == NX_SEG && sg.n <= PA_ROWS / 2 && nx.n <= PA_ROWS / 2;
+                    if (early) q_start();
+                }
             }
             if (t < sg.t1) break;  // a wait ran out
-            more = begin();        // the Q of the next segment, while this one's last products run
-            if (!pa_wait(c, &c.o_full[f], o_ph, err)) break;
+            if (more == NX_LATER) more = next(false);
+            if (more == NX_SEG) {
+                if (!early) q_start();  // this segment's Q has been read: its last S was complete
+                q_finish();
+            }
+            if (!pa_wait(c, &c.o_full[f], o_ph)) break;
             o_ph ^= 1;
             tc_after();
             if (!busy) continue;
@@ -543,59 +569,70 @@ prefix_attn_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_co
         asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(PA_REGS_LOW));
         const int page = 1 << g.s.page_shift, box = min(page, PA_TILE), boxes = PA_TILE / box;
         int issued = 0, slot = 0;
-        unsigned ph = 0, at[2] = {0, 0};
-        bool ok = true, ended[2] = {false, false}, v_due[2] = {false, false};
-        PaSeg sg[2];
-        sg[0].t0 = sg[0].t1 = sg[1].t0 = sg[1].t1 = 0;
-        int pg[2] = {0, 0}, krow[2] = {0, 0}, vkh[2] = {0, 0};  // this lane's page of the flow's tile, kept from K for V
-        auto load = [&](const CUtensorMap* map, int pid, int prow, int kh) {
-            ok = pa_wait_warp(c, &c.empty[slot], ph ^ 1u, err);
-            if (!ok) return;
-            if (lane == 0) mbar_expect_tx(&c.full[slot], KV_BYTES);
-            __syncwarp();
-            uint8_t* const dst = ring + slot * KV_BYTES;
-            if (lane < boxes) {
-#pragma unroll
-                for (int h = 0; h < HALVES; h++)
-                    tma_load_4d(dst + h * HALF + lane * box * 128, map, h * 64, prow, kh, pid, &c.full[slot]);
-            }
-            issued++;
-            if (++slot == PA_STAGES) slot = 0, ph ^= 1;
-        };
+        unsigned ph = 0;
+        bool ok = true;
+        struct Flow {
+            Feed feed;
+            PaSeg sg;
+            bool ended, v_due;
+            int pg, krow, kh;   // this lane's page of the tile, kept from K for V
+        } cur, oth;
+        cur.ended = oth.ended = cur.v_due = oth.v_due = false;
+        cur.sg.t0 = cur.sg.t1 = oth.sg.t0 = oth.sg.t1 = 0;
+        cur.pg = cur.krow = cur.kh = oth.pg = oth.krow = oth.kh = 0;
         // a round brings, per flow, V of the round before and K of this one
-        while (ok && !(ended[0] && ended[1] && !v_due[0] && !v_due[1])) {
+#pragma unroll 1
+        for (int f = 0; f || !(cur.ended && oth.ended && !cur.v_due && !oth.v_due); f ^= 1) {
+            bool k_due = false;
+#pragma unroll 1
+            for (int which = 0; which < 2 && ok; which++) {
+                if (which == 0 ? cur.v_due : k_due) {
+                    ok = pa_wait_warp(c, &c.empty[slot], ph ^ 1u);
+                    if (!ok) break;
+                    if (lane == 0) mbar_expect_tx(&c.full[slot], KV_BYTES);
+                    __syncwarp();
+                    uint8_t* const dst = ring + slot * KV_BYTES;
+                    const CUtensorMap* const map = which ? &map_k : &map_v;
+                    if (lane < boxes) {
 #pragma unroll
-            for (int f = 0; f < 2; f++) {
-                if (ok && v_due[f]) load(&map_v, pg[f], krow[f], vkh[f]);
-                v_due[f] = false;
-                if (!ok || ended[f]) continue;
-                if (sg[f].t0 == sg[f].t1) {
-                    ok = fetch(f, at[f], sg[f]);
-                    if (!ok) continue;
-                    ended[f] = sg[f].flags & SEG_END;
-                    if (ended[f]) continue;
+                        for (int h = 0; h < HALVES; h++)
+                            tma_load_4d(dst + h * HALF + lane * box * 128, map, h * 64, cur.krow, cur.kh, cur.pg, &c.full[slot]);
+                    }
+                    issued++;
+                    if (++slot == PA_STAGES) slot = 0, ph ^= 1;
                 }
-                const int t = sg[f].t0++;
-                if (sg[f].n == 0 || (f == 1 && (sg[f].flags & SEG_PAIRED))) continue;
+                if (which) break;
+                cur.v_due = false;
+                if (cur.ended) break;
+                if (cur.sg.t0 == cur.sg.t1) {
+                    ok = fetch(f, cur.feed, cur.sg);
+                    cur.ended = !ok || (cur.sg.flags & SEG_END);
+                    if (cur.ended) break;
+                }
+                const int t = cur.sg.t0++;
+                if (cur.sg.n == 0 || (f == 1 && (cur.sg.flags & SEG_PAIRED))) break;
                 const int pos = t * PA_TILE + lane * box;
                 int id = g.s.n_pages;  // out of range: zeros
-                if (lane < boxes && pos < sg[f].kv_end) {
-                    id = sg[f].flags & SEG_OWN ? g.s.table[(int64_t)sg[f].b * g.s.table_ld + (pos >> g.s.page_shift)]
-                                               : g.a.prefix_table[pos >> g.s.page_shift];
-                    if (id < 0 || id >= g.s.n_pages) {
+                if (lane < boxes && pos < cur.sg.kv_end) {
+                    const int32_t* const table = cur.sg.flags & SEG_OWN ? g.s.table + (int64_t)cur.sg.b * g.s.table_ld
+                                                                        : g.a.prefix_table;
+                    id = table[pos >> g.s.page_shift];
+                    if ((unsigned)id >= (unsigned)g.s.n_pages) {
                         flag_error(err, ERR_PAGE_ID, id);
                         id = g.s.n_pages;
                     }
                 }
-                pg[f] = id;
-                krow[f] = pos & (page - 1);
-                vkh[f] = sg[f].kh;
-                v_due[f] = true;
-                load(&map_k, id, krow[f], vkh[f]);
+                cur.pg = id;
+                cur.krow = pos & (page - 1);
+                cur.kh = cur.sg.kh;
+                cur.v_due = k_due = true;
             }
+            if (!ok) break;
+            exchange(cur, oth);
         }
         // no copy may still be landing when the CTA exits
         if (!ok) {
+#pragma unroll 1
             for (int i = max(0, issued - PA_STAGES); i < issued; i++)
                 mbar_wait_ns(&c.full[i % PA_STAGES], (unsigned)(i / PA_STAGES) & 1u, 2000000000ull);
         }
@@ -604,154 +641,211 @@ prefix_attn_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_co
         asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(PA_REGS_LOW));
         constexpr uint32_t id_qk = pa_idesc(PA_TILE, 0), id_pv = pa_idesc(D, 1);
         int slot = 0, k_slot = 0, v_slot = 0;
-        unsigned ph = 0, q_ph[2] = {0, 0}, p_ph[2] = {0, 0}, at[2] = {0, 0};
-        bool ok = true, ended[2] = {false, false};
-        PaSeg sg[2];
-        sg[0].t0 = sg[0].t1 = sg[1].t0 = sg[1].t1 = 0;
-        // P V of the round before, per flow: due, shared with flow 1, first and last of a segment
-        bool pv[2] = {false, false}, pv_pair[2] = {false, false}, pv_first[2] = {false, false}, pv_last[2] = {false, false};
-        int pv_valid[2] = {0, 0};
+        unsigned ph = 0;
+        bool ok = true, both = false;  // both: this round's K is for the second flow too
+        struct Flow {
+            Feed feed;
+            PaSeg sg;
+            bool ended;
+            unsigned q_ph, p_ph, turn, q_off;
+            // P V of the round before: due, V shared by the flows, first and last of a segment
+            bool pv, pv_shared, pv_first, pv_last;
+            int pv_valid;
+        } cur, oth;
+        cur.sg.t0 = cur.sg.t1 = 0;
+        cur.ended = cur.pv = cur.pv_shared = cur.pv_first = cur.pv_last = false;
+        cur.q_ph = cur.p_ph = cur.turn = cur.q_off = 0;
+        cur.pv_valid = 0;
+        oth = cur;
         auto take = [&](int& where) {  // the next stage of the ring
-            ok = pa_wait_warp(c, &c.full[slot], ph, err);
+            ok = pa_wait_warp(c, &c.full[slot], ph);
             where = slot;
             if (++slot == PA_STAGES) slot = 0, ph ^= 1;
         };
-        auto do_pv = [&](int f) {
-            if (f == 0 || !pv_pair[f]) {
-                take(v_slot);
-                if (!ok) return;
-                if (pv_valid[f] < PA_TILE) {
-                    // positions past the end share a page with valid ones: whatever is there
-                    // (NaN times a zero probability) must not reach the product
-                    uint8_t* const v = ring + v_slot * KV_BYTES;
 #pragma unroll 1
-                    for (int i = pv_valid[f] * 8 + lane; i < PA_TILE * 8; i += 32)
+        for (int f = 0; f || !(cur.ended && oth.ended && !cur.pv && !oth.pv); f ^= 1) {
+            const uint32_t t_s = tmem + f * 128, t_o = tmem + 256 + f * 128;
+            if (cur.pv) {
+                if (f == 0 || !cur.pv_shared) {
+                    take(v_slot);
+                    if (!ok) break;
+                    if (cur.pv_valid < PA_TILE) {
+                        // positions past the end share a page with valid ones: whatever is there
+                        // (NaN times a zero probability) must not reach the product
+                        uint8_t* const v = ring + v_slot * KV_BYTES;
+#pragma unroll 1
+                        for (int i = cur.pv_valid * 8 + lane; i < PA_TILE * 8; i += 32)
 #pragma unroll
-                        for (int h = 0; h < HALVES; h++)
-                            *reinterpret_cast<uint4*>(v + h * HALF + i * 16) = make_uint4(0, 0, 0, 0);
-                    proxy_fence();
-                    __syncwarp();
+                            for (int h = 0; h < HALVES; h++)
+                                *reinterpret_cast<uint4*>(v + h * HALF + i * 16) = make_uint4(0, 0, 0, 0);
+                        proxy_fence();
+                        __syncwarp();
+                    }
                 }
-            }
-            ok = pa_wait_warp(c, &c.p_full[f], p_ph[f], err);
-            if (!ok) return;
-            p_ph[f] ^= 1;
-            tc_after();
-            const uint64_t v = pa_desc(smem_addr(ring + v_slot * KV_BYTES), HALF);
-            if (elect_one()) {
-#pragma unroll
-                for (int j = 0; j < PA_TILE / 16; j++)
-                    mma_ts(tmem + 256 + f * 128, tmem + f * 128 + j * 8, v + j * (2048 >> 4), id_pv,
-                           j > 0 || !pv_first[f]);
-                if (!(f == 0 && pv_pair[0] && pv[1])) tc_commit(&c.empty[v_slot]);
-                if (pv_last[f]) tc_commit(&c.o_full[f]);
-            }
-            __syncwarp();
-        };
-        while (ok && !(ended[0] && ended[1] && !pv[0] && !pv[1])) {
-            bool act1 = false;  // a paired round's second half has rows
-#pragma unroll
-            for (int f = 0; f < 2; f++) {
-                if (ok && pv[f]) do_pv(f);
-                pv[f] = false;
-                if (!ok || ended[f]) continue;
-                bool fresh = false;
-                if (sg[f].t0 == sg[f].t1) {
-                    ok = fetch(f, at[f], sg[f]);
-                    if (!ok) continue;
-                    ended[f] = sg[f].flags & SEG_END;
-                    if (ended[f]) continue;
-                    fresh = true;
-                }
-                const int t = sg[f].t0++;
-                if (sg[f].n == 0) continue;
-                const bool paired = sg[f].flags & SEG_PAIRED;
-                if (f == 0 && paired) act1 = sg[0].n1 > 0;
-                if (f == 0 || !paired) take(k_slot);
-                if (!ok) continue;
-                if (fresh) {  // a new segment: its Q
-                    ok = pa_wait_warp(c, &c.q_full[f], q_ph[f], err);
-                    if (!ok) continue;
-                    q_ph[f] ^= 1;
-                }
+                ok = pa_wait_warp(c, &c.p_full[f], cur.p_ph);
+                if (!ok) break;
+                cur.p_ph ^= 1;
                 tc_after();
-                const uint64_t q = pa_desc(smem_addr(sm + f * Q_BYTES), 16), k = pa_desc(smem_addr(ring + k_slot * KV_BYTES), 16);
+                const uint64_t v = pa_desc(smem_addr(ring + v_slot * KV_BYTES), HALF);
                 if (elect_one()) {
 #pragma unroll
-                    for (int j = 0; j < D / 16; j++) {
-                        const uint32_t o = ((j >> 2) * HALF + (j & 3) * 32) >> 4;
-                        mma_ss(tmem + f * 128, q + o, k + o, id_qk, j > 0);
-                    }
-                    if (!(f == 0 && act1)) tc_commit(&c.empty[k_slot]);
-                    tc_commit(&c.s_full[f]);
+                    for (int j = 0; j < PA_TILE / 16; j++)
+                        mma_ts(t_o, t_s + j * 8, v + j * (2048 >> 4), id_pv, j > 0 || !cur.pv_first);
+                    if (!(f == 0 && cur.pv_shared && oth.pv)) tc_commit(&c.empty[v_slot]);
+                    if (cur.pv_last) tc_commit(&c.o_full[f]);
                 }
                 __syncwarp();
-                pv[f] = true;
-                pv_pair[f] = paired;
-                pv_first[f] = fresh;
-                pv_last[f] = sg[f].t0 == sg[f].t1;
-                pv_valid[f] = min(PA_TILE, sg[f].kv_end - t * PA_TILE);
+                cur.pv = false;
             }
+            if (!cur.ended && cur.sg.t0 == cur.sg.t1) {
+                ok = fetch(f, cur.feed, cur.sg);
+                if (!ok) break;
+                cur.ended = cur.sg.flags & SEG_END;
+                cur.pv_first = true;
+            } else {
+                cur.pv_first = false;
+            }
+            if (!cur.ended) {
+                const int t = cur.sg.t0++;
+                const bool shared = cur.sg.flags & SEG_PAIRED;
+                if (f == 0) both = shared && cur.sg.n1 > 0;
+                if (cur.sg.n > 0) {
+                    if (f == 0 || !shared) take(k_slot);
+                    if (!ok) break;
+                    if (cur.pv_first) {  // a new segment: its Q
+                        ok = pa_wait_warp(c, &c.q_full[f], cur.q_ph);
+                        if (!ok) break;
+                        cur.q_ph ^= 1;
+                        cur.q_off = q_offset(cur.sg, cur.turn++);
+                    }
+                    tc_after();
+                    const uint64_t q = pa_desc(smem_addr(sm + f * Q_BYTES) + cur.q_off, 16);
+                    const uint64_t k = pa_desc(smem_addr(ring + k_slot * KV_BYTES), 16);
+                    if (elect_one()) {
+#pragma unroll
+                        for (int j = 0; j < D / 16; j++) {
+                            const uint32_t o = ((j >> 2) * HALF + (j & 3) * 32) >> 4;
+                            mma_ss(t_s, q + o, k + o, id_qk, j > 0);
+                        }
+                        if (!(f == 0 && both)) tc_commit(&c.empty[k_slot]);
+                        tc_commit(&c.s_full[f]);
+                    }
+                    __syncwarp();
+                    cur.pv = true;
+                    cur.pv_shared = shared;
+                    cur.pv_last = cur.sg.t0 == cur.sg.t1;
+                    cur.pv_valid = min(PA_TILE, cur.sg.kv_end - t * PA_TILE);
+                }
+            }
+            exchange(cur, oth);
         }
         if (lane == 0) tc_commit(&c.done);
         __syncwarp();
-        if (!mbar_wait_ns(&c.done, 0, 2000000000ull) && lane == 0) flag_error(err, ERR_PA_WAIT, 1);
+        if (!mbar_wait_ns(&c.done, 0, 2000000000ull)) c.abort = 1;
     } else {
         asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(PA_REGS_LOW));
-        if (warp == 10 && lane == 0) {
+        if (warp == 10) {
             // ------------------------------ scheduler ------------------------------
             const Line line(g.p, so);
-            unsigned at[2] = {0, 0};
+            unsigned batch[2] = {0, 0};
             bool ok = true;
-            auto put = [&](int f, const PaSeg& o) {
-                const int i = at[f] % PA_SEGS;
-                ok = pa_wait(c, &c.seg_empty[f][i], ((at[f] / PA_SEGS) & 1u) ^ 1u, err);
+            // entries of flow f's next batch: lanes with `valid` give theirs in order
+            auto put = [&](int f, const PaSeg& o, bool valid) {
+                const unsigned k = batch[f], mask = __ballot_sync(0xffffffffu, valid);
+                ok = pa_wait_warp(c, &c.seg_empty[f][k & 1], ((k >> 1) & 1u) ^ 1u);
                 if (!ok) return;
-                c.seg[f][i] = o;
-                mbar_arrive(&c.seg_full[f][i]);
-                at[f]++;
+                if (valid) c.seg[f][k & 1][__popc(mask & ((1u << lane) - 1))] = o;
+                if (lane == 0) c.seg_n[f][k & 1] = __popc(mask);
+                __syncwarp();
+                if (lane == 0) mbar_arrive(&c.seg_full[f][k & 1]);
+                batch[f]++;
             };
-            PaSeg stop;
-            stop.t0 = 0, stop.t1 = 1, stop.n = stop.n1 = stop.pad = 0, stop.flags = 0;
-            stop.kh = stop.b = stop.kv_end = stop.row0 = stop.voff = stop.slot = 0;
+            PaSeg o{0, 1, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0};
 #pragma unroll 1
             for (int part = 0; part < 2 && ok; part++) {
-                const bool paired = part ? g.p.pair_o : g.p.pair_p;
-                PaCursor cu[2];
+                const bool own = part, paired = own ? g.p.pair_o : g.p.pair_p;
+                PaWalk walk[2];
                 int rounds[2] = {0, 0};
 #pragma unroll 1
                 for (int f = 0; f < 2; f++) {
-                    flow_range(line, g.p, me, f, part == 1, cu[f].step, cu[f].hi);
-                    cu[f].seek(g, c.scan, per_entry, n_entries, part == 1);
+                    PaWalk w;
+                    flow_range(line, g.p, me, f, own, w.step, w.hi);
+                    pa_seek(g, c, per_entry, n_entries, own, lane, w);
+                    if (f) walk[1] = w;
+                    else walk[0] = w;
                 }
-                // flows that take their steps apart: the one behind in rounds gets the next segment
+                // flows that take their steps apart: the one with fewer rounds gets the next batch
                 while (ok) {
-                    const int f = paired || cu[1].step >= cu[1].hi || (cu[0].step < cu[0].hi && rounds[0] <= rounds[1]) ? 0 : 1;
-                    PaCursor& k = cu[f];
-                    if (k.step >= k.hi) break;
-                    PaSeg o = k.segment(g, part == 1, paired, 0, paired ? me : 2 * me + f);
-                    if (paired) {
-                        PaSeg o1 = k.segment(g, part == 1, true, 1, me);
-                        o.n1 = o1.n;
-                        put(0, o);
-                        if (ok) put(1, o1);
-                    } else {
-                        put(f, o);
+                    const int f = paired || walk[1].step >= walk[1].hi ||
+                                          (walk[0].step < walk[0].hi && rounds[0] <= rounds[1]) ? 0 : 1;
+                    PaWalk w = f ? walk[1] : walk[0];
+                    if (w.step >= w.hi) break;
+                    // lane i looks at the i-th item from here on
+                    int j = w.j + lane, b = w.b, n_rb = g.p.n_rb, n = 0;
+                    SeqInfo si{0, g.s.rows, 0};
+                    if (own) {
+#pragma unroll 1
+                        for (;;) {
+                            if (b >= g.s.n_seqs) break;
+                            si = pa_seq(g, c, b);
+                            n_rb = os.blocks(si);
+                            if (j < g.a.n_kv * n_rb) break;
+                            j -= g.a.n_kv * n_rb;
+                            b++;
+                        }
                     }
-                    rounds[f] += o.t1 - o.t0;
-                    k.step += o.t1 - o.t0;
-                    k.next_item(g, part == 1);
+                    const int kh = n_rb == 1 ? j : j / max(n_rb, 1), rb = j - kh * n_rb;
+                    o.kv_end = g.a.prefix_len;
+                    int nt = g.p.np;
+                    if (own) {
+                        o.kv_end = b < g.s.n_seqs ? os.visible(si, rb) : 0;
+                        nt = (o.kv_end + PA_TILE - 1) / PA_TILE;
+                    }
+                    o.t0 = lane == 0 ? w.t : 0;
+                    const int upto = warp_scan(nt - o.t0, lane), start = w.step + upto - (nt - o.t0);
+                    n = min(nt - o.t0, w.hi - start);
+                    o.t1 = o.t0 + n;
+                    const int block = own ? g.p.ob : g.p.pb, cap = own ? g.p.cap_o : g.p.cap_p;
+                    const int rows = si.q * g.a.group - rb * block;  // of the whole block
+                    o.n = min(PA_ROWS, rows);
+                    o.n1 = paired ? max(0, min(PA_ROWS, rows - PA_ROWS)) : 0;
+                    o.flags = (own ? SEG_OWN : 0) | (paired ? SEG_PAIRED : 0) |
+                              (g.a.prefix_len == 0 && o.t0 == 0 && o.t1 == nt ? SEG_WHOLE : 0);
+                    o.kh = kh;
+                    o.b = b;
+                    o.row0 = (own ? si.q0 * g.a.group : 0) + rb * block;
+                    o.voff = own ? si.kv - si.q + 1 - si.q0 : 0;
+                    o.slot = ((own ? g.a.n_kv * os.base(si, b) : 0) + j + (paired ? me : 2 * me + f)) * cap;
+                    if (__any_sync(0xffffffffu, n > 0)) put(f, o, n > 0);
+                    if (paired && ok && __any_sync(0xffffffffu, n > 0)) {  // the other half of the block
+                        o.n = o.n1;
+                        o.row0 += PA_ROWS;
+                        o.slot += PA_ROWS;
+                        put(1, o, n > 0);
+                    }
+                    const int all = min(__shfl_sync(0xffffffffu, upto, 31), w.hi - w.step);
+                    rounds[f] += all;
+                    w.step += all;
+                    w.j = __shfl_sync(0xffffffffu, j, 31) + 1;
+                    w.b = __shfl_sync(0xffffffffu, b, 31);
+                    w.t = 0;
+                    if (own && w.b >= g.s.n_seqs) w.hi = w.step;  // (no more sequences)
+                    if (f) walk[1] = w;
+                    else walk[0] = w;
                 }
                 // both flows take the same number of rounds
-                if (!paired && rounds[1] < rounds[0] && ok) put(1, stop);
+                o = PaSeg{0, 1, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0};
+                if (!paired && rounds[1] < rounds[0] && ok) put(1, o, lane == 0);
             }
-            stop.flags = SEG_END;
-            for (int f = 0; f < 2 && ok; f++) put(f, stop);
+            o.flags = SEG_END;
+#pragma unroll 1
+            for (int f = 0; f < 2 && ok; f++) put(f, o, lane == 0);
         }
     }
     tc_before();
     __syncthreads();
     tc_after();
+    if (tid == 0 && c.abort) flag_error(err, ERR_PA_WAIT, me);
     if (warp == 9) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, 512;" ::"r"(tmem));
 }
 

@@ -42,7 +42,7 @@ struct PrefixPlan {
     int np;                     // tiles of the prefix
     int sp;                     // steps of the prefix
     int workers;                // CTAs that share the line
-    int wp, wo;                 // weight of a prefix step and of an own step
+    uint64_t workers_mul;       // ceil(2^40 / workers)
     int cap_p, cap_o;           // rows a partial slot holds
     int32_t* cum;               // [n_seqs + 1] own steps before each sequence
     float* o_p;                 // prefix partials [slot][cap_p][D], unnormalised
@@ -101,26 +101,30 @@ struct OwnSteps {
     __device__ __forceinline__ int base(const SeqInfo& i, int b) const { return i.q0 * a.group / p.ob + b; }
 };
 
-// The line of steps: prefix steps weigh wp, own steps wo; worker c takes the steps that start in
-// [W c / n, W (c + 1) / n), n workers, W < 2^31 as the host checks.
+// A step of a paired block weighs 3, one that a flow takes alone 2 (measured: a round of two
+// 128-row products takes 3300 cycles, one of two flows' separate tiles 4000). Worker c of n takes
+// the steps that start in [W c / n, W (c + 1) / n) of the whole weight W < 2^28.
 struct Line {
     int w, split;      // total weight; weight of the prefix part
-    int sp, so, n, wp, wo;
+    int sp, so, n;
+    bool pair_p, pair_o;
     int quot, rem;     // W / n
+    uint64_t mul;      // ceil(2^40 / n): x / n = x mul / 2^40, exact for x < 2^32
     __device__ __forceinline__ Line(const PrefixPlan& p, int own_steps)
-        : sp(p.sp), so(own_steps), n(p.workers), wp(p.wp), wo(p.wo) {
-        split = sp * wp;
-        w = split + so * wo;
-        quot = w / n;
+        : sp(p.sp), so(own_steps), n(p.workers), pair_p(p.pair_p), pair_o(p.pair_o), mul(p.workers_mul) {
+        split = sp * (pair_p ? 3 : 2);
+        w = split + so * (pair_o ? 3 : 2);
+        quot = (int)(((uint64_t)w * mul) >> 40);
         rem = w - quot * n;
     }
-    __device__ __forceinline__ int start(int c) const { return quot * c + rem * c / n; }  // floor(W c / n)
+    // floor(W c / n)
+    __device__ __forceinline__ int start(int c) const { return quot * c + (int)(((uint64_t)(rem * c) * mul) >> 40); }
     __device__ __forceinline__ int first(int c, bool own) const {
-        const int x = start(c);
-        return own ? min((max(x - split, 0) + wo - 1) / wo, so) : min((x + wp - 1) / wp, sp);
+        const int x = own ? max(start(c) - split, 0) : start(c);
+        return min((own ? pair_o : pair_p) ? (x + 2) / 3 : (x + 1) / 2, own ? so : sp);
     }
     __device__ __forceinline__ int owner(int step, bool own) const {
-        const int at = own ? split + step * wo : step * wp;
+        const int at = (own ? split : 0) + step * ((own ? pair_o : pair_p) ? 3 : 2);
         int c = min(n - 1, (int)(((float)at + 1.0f) * (float)n / (float)w));  // a guess, then the step's place
         while (c > 0 && start(c) > at) c--;
         while (c + 1 < n && start(c + 1) <= at) c++;
