@@ -104,128 +104,160 @@ __global__ void __launch_bounds__(128) prefix_attn_row_kernel(PrefixAttnArgs a, 
 }
 
 // =========================================================================================
-// Merge: a warp per (row, head) joins the partials of the workers that had a piece of the row's
-// prefix item or own item, in the order of the line: with M the largest of their maxima,
-// o = sum 2^(m_i - M) o_i / sum 2^(m_i - M) l_i. A lane looks after one partial's m and l, then
-// the warp adds up the vectors, four dims a lane. Rows that a worker had whole are written there.
+// Merge: joins the partials of the workers that had a piece of a row's prefix item or own item, in
+// the order of the line: with M the largest of their maxima, o = sum 2^(m_i - M) o_i /
+// sum 2^(m_i - M) l_i. With a prefix every row has at least its prefix partials: a CTA takes the
+// G stacked rows of a token and kv head. Without one only cut items are left (a whole one was
+// written by its worker): a CTA takes up to MERGE_ROWS rows of the item that a worker began. A
+// thread adds up four dims of a row; rows are next to each other in memory, so a warp reads runs
+// of 16 bytes x rows. A warp looks after the weights of a row, a lane per partial.
 // =========================================================================================
+constexpr int MERGE_ROWS = 8;
+constexpr int MERGE_MAX = 640;  // partials of a row: at most two workers a CTA in either part
+
 template <typename T, int D>
-__global__ void __launch_bounds__(256) prefix_attn_merge_kernel(PrefixAttnArgs a, PagedSeqs s, PrefixPlan p) {
-    pdl_trigger();
-    pdl_wait();
-    const int lane = threadIdx.x & 31;
-    const int idx = blockIdx.x * (blockDim.x >> 5) + (threadIdx.x >> 5);
-    const int t = idx / a.n_heads, h = idx - t * a.n_heads;
-    if (t >= s.rows) return;
-    const int b = s.q_start ? seq_of_row(s.q_start, s.n_seqs, t, lane) : t;
-    if (b >= s.n_seqs) return;
-    const SeqInfo si = seq_info(a, s, b, false);
-    const int kh = h / a.group, gq = h - kh * a.group;
+__global__ void __launch_bounds__(MERGE_ROWS * D / 4) prefix_attn_merge_kernel(PrefixAttnArgs a, PagedSeqs s, PrefixPlan p) {
+    constexpr int CH = D / 4;
+    __shared__ int slot[MERGE_MAX];
+    __shared__ float weight[MERGE_ROWS][MERGE_MAX];
+    __shared__ float inv[MERGE_ROWS];
+    __shared__ __align__(16) float stage[MERGE_ROWS][D];
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, warps = blockDim.x >> 5;
     const OwnSteps os{a, p};
-    const Line line(p, p.cum[s.n_seqs]);
-    // this row's prefix item and own item: steps [s0, s1), first virtual worker, count, slot, row
-    int v0[2] = {0, 0}, cnt[2] = {0, 0}, s0[2], s1[2], item[2], in[2];
-    if (p.np > 0) {
-        const int r = t * a.group + gq, rb = r / p.pb;
-        item[0] = kh * p.n_rb + rb;
-        in[0] = r - rb * p.pb;
-        s0[0] = item[0] * p.np;
-        s1[0] = s0[0] + p.np;
-    } else {
-        s0[0] = s1[0] = 0;
+    // the group's stacked rows st0 .. st0 + todo - 1 of kv head kh; for the two parts the item, the
+    // first row's place in it and whether it has steps
+    int st0, todo, kh, item[2] = {0, 0}, in[2] = {0, 0};
+    bool any[2] = {false, false};
+    int b = 0, t = 0;
+    SeqInfo si{0, 0, 0};
+    const bool by_row = a.prefix_len > 0;
+    if (by_row) {  // (the call's inputs: complete before the kernel that this one waits for began)
+        t = blockIdx.x / a.n_kv;
+        kh = blockIdx.x - t * a.n_kv;
+        b = s.q_start ? seq_of_row(s.q_start, s.n_seqs, t, lane) : t;
+        if (b >= s.n_seqs) return;
+        si = seq_info(a, s, b, false);
+        st0 = t * a.group;
+        todo = a.group;
     }
-    s0[1] = s1[1] = 0;
-    if (t < si.q0 + si.q) {
-        const int r = (t - si.q0) * a.group + gq, rb = r / p.ob, nb = os.blocks(si);
-        int before = 0, per = 0;
-        for (int i = lane; i < nb; i += 32) {
-            const int n = os.tiles(si, i);
-            per += n;
-            if (i < rb) before += n;
+    pdl_wait();
+    pdl_trigger();
+    if (!by_row) {
+        const SplitItem w = p.split[blockIdx.x];
+        st0 = w.row0 + blockIdx.y * MERGE_ROWS;
+        todo = min(MERGE_ROWS, w.rows - (int)blockIdx.y * MERGE_ROWS);
+        kh = w.kh;
+        item[1] = w.item;
+        in[1] = blockIdx.y * MERGE_ROWS;
+        any[1] = true;
+    }
+    const Line line(p, *p.own_steps);
+#pragma unroll 1
+    for (; todo > 0;) {
+        int run = min(todo, MERGE_ROWS);  // rows that share their items
+        if (by_row) {
+            const int rb_p = st0 / p.pb;
+            item[0] = kh * p.n_rb + rb_p;
+            in[0] = st0 - rb_p * p.pb;
+            any[0] = true;
+            run = min(run, p.pb - in[0]);
+            any[1] = false;
+            if (t < si.q0 + si.q) {
+                const int r = st0 - si.q0 * a.group, rb = r / p.ob;
+                item[1] = a.n_kv * os.base(si, b) + kh * os.blocks(si) + rb;
+                in[1] = r - rb * p.ob;
+                any[1] = os.visible(si, rb) > 0;
+                run = min(run, p.ob - in[1]);
+            }
         }
-        before = __reduce_add_sync(0xffffffffu, before);
-        per = __reduce_add_sync(0xffffffffu, per);
-        item[1] = a.n_kv * os.base(si, b) + kh * nb + rb;
-        in[1] = r - rb * p.ob;
-        s0[1] = p.cum[b] + kh * per + before;
-        s1[1] = s0[1] + os.tiles(si, rb);
-    }
+        int v0[2] = {0, 0}, cnt[2] = {0, 0};
 #pragma unroll
-    for (int part = 0; part < 2; part++) {
-        if (s0[part] == s1[part]) continue;
-        const bool paired = part ? p.pair_o : p.pair_p;
-        int w[2];
-#pragma unroll
-        for (int e = 0; e < 2; e++) {
-            const int step = e ? s1[part] - 1 : s0[part];
-            w[e] = line.owner(step, part);
-            if (!paired) {
+        for (int part = 0; part < 2; part++)
+            if (any[part]) {
+                v0[part] = p.first[part][item[part]];
+                cnt[part] = p.last[part][item[part]] - v0[part] + 1;
+            }
+        const int n = min(cnt[0] + cnt[1], MERGE_MAX);
+        __syncthreads();  // (the shared arrays are read no more)
+#pragma unroll 1
+        for (int i = tid; i < n; i += blockDim.x) {
+            const int part = i >= cnt[0], k = i - (part ? cnt[0] : 0), v = v0[part] + k;
+            const bool paired = part ? p.pair_o : p.pair_p;
+            bool has = k == 0 || k == cnt[part] - 1;
+            if (!has) {  // a worker in between may have no step at all
                 int lo, hi;
-                flow_range(line, p, w[e], 0, part, lo, hi);
-                w[e] = 2 * w[e] + (step >= hi);
+                flow_range(line, p, paired ? v : v >> 1, paired ? 0 : v & 1, part, lo, hi);
+                has = lo < hi;
             }
+            slot[i] = has ? item[part] + v : -1;
         }
-        v0[part] = w[0];
-        cnt[part] = w[1] - w[0] + 1;
-    }
-    if (p.np == 0 && cnt[1] == 1) return;  // written by its only worker
-    const int n = cnt[0] + cnt[1];
-    float m_i = -INFINITY, l_i = 0.0f;
-    int64_t at_i = -1;
-    auto look = [&](int i) {  // partial i: its slot row (-1: the worker had no step of the item), m, l
-        m_i = -INFINITY;
-        l_i = 0.0f;
-        at_i = -1;
-        if (i >= n) return;
-        const int part = i >= cnt[0], v = v0[part] + i - (part ? cnt[0] : 0);
-        const bool paired = part ? p.pair_o : p.pair_p;
-        int lo, hi;
-        flow_range(line, p, paired ? v : v >> 1, paired ? 0 : v & 1, part, lo, hi);
-        if (max(lo, s0[part]) >= min(hi, s1[part])) return;
-        at_i = (int64_t)(item[part] + v) * (part ? p.cap_o : p.cap_p) + in[part];
-        const float2 ml = (part ? p.ml_o : p.ml_p)[at_i];
-        m_i = ml.x;
-        l_i = ml.y;
-    };
-    look(lane);
-    float M = warp_max(m_i);
-    for (int i0 = 32; i0 < n; i0 += 32) {
-        look(i0 + lane);
-        M = fmaxf(M, warp_max(m_i));
-    }
-    float L = 0.0f, o[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-    const bool on = 4 * lane < D;
-    for (int i0 = 0; i0 < n; i0 += 32) {
-        if (n > 32) look(i0 + lane);
-        const float w_i = m_i == -INFINITY ? 0.0f : exp2f(m_i - M);
-        L += warp_sum(w_i * l_i);
-        const int k = min(32, n - i0);
+        __syncthreads();
+#pragma unroll 1
+        for (int r = warp; r < run; r += warps) {
+            float M = -INFINITY;
+#pragma unroll 1
+            for (int i = lane; i < n; i += 32) {
+                const int part = i >= cnt[0];
+                if (slot[i] >= 0) M = fmaxf(M, p.ml[part][(int64_t)slot[i] * p.cap[part] + in[part] + r].x);
+            }
+            M = warp_max(M);
+            float L = 0.0f;
+#pragma unroll 1
+            for (int i = lane; i < n; i += 32) {
+                const int part = i >= cnt[0];
+                float w = 0.0f;
+                if (slot[i] >= 0) {
+                    const float2 ml = p.ml[part][(int64_t)slot[i] * p.cap[part] + in[part] + r];
+                    if (ml.x != -INFINITY) w = exp2f(ml.x - M);
+                    L = fmaf(w, ml.y, L);
+                }
+                weight[r][i] = w;
+            }
+            L = warp_sum(L);
+            if (lane == 0) inv[r] = L > 0.0f ? 1.0f / L : L;  // a row that saw nothing: zeros; NaN stays
+        }
+        __syncthreads();
+        const int r = tid % MERGE_ROWS, ch = tid / MERGE_ROWS;
+        float4 o = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+        if (r < run) {
 #pragma unroll 4
-        for (int j = 0; j < k; j++) {
-            const int64_t at = __shfl_sync(0xffffffffu, at_i, j);
-            const float w = __shfl_sync(0xffffffffu, w_i, j);
-            if (at >= 0 && on) {
-                const float4 x = *reinterpret_cast<const float4*>((i0 + j >= cnt[0] ? p.o_o : p.o_p) + at * D + 4 * lane);
-                o[0] = fmaf(w, x.x, o[0]);
-                o[1] = fmaf(w, x.y, o[1]);
-                o[2] = fmaf(w, x.z, o[2]);
-                o[3] = fmaf(w, x.w, o[3]);
+            for (int i = 0; i < n; i++) {
+                const int part = i >= cnt[0];
+                const float w = weight[r][i];
+                if (slot[i] >= 0) {
+                    const float4 x = reinterpret_cast<const float4*>(p.o[part])[((int64_t)slot[i] * CH + ch) * p.cap[part] + in[part] + r];
+                    o.x = fmaf(w, x.x, o.x);
+                    o.y = fmaf(w, x.y, o.y);
+                    o.z = fmaf(w, x.z, o.z);
+                    o.w = fmaf(w, x.w, o.w);
+                }
+            }
+            const float k = inv[r];
+            *reinterpret_cast<float4*>(&stage[r][4 * ch]) = make_float4(o.x * k, o.y * k, o.z * k, o.w * k);
+        }
+        __syncthreads();
+        {  // out, a row's dims side by side
+            const int rr = tid / CH, e = tid % CH * 4, st = st0 + rr, tok = a.group_div(st);
+            const bool on = rr < run;
+            float y[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+            if (on) {
+#pragma unroll
+                for (int j = 0; j < 4; j++) y[j] = stage[rr][e + j];
+            }
+            const int64_t col = (int64_t)(kh * a.group + st - tok * a.group) * D + e;
+            if (a.out && on) {
+                T* const dst = static_cast<T*>(a.out) + (int64_t)tok * a.out_stride + col;
+                if constexpr (sizeof(T) == 4) *reinterpret_cast<float4*>(dst) = make_float4(y[0], y[1], y[2], y[3]);
+                else *reinterpret_cast<uint2*>(dst) = make_uint2(pack_bf16x2(y[0], y[1]), pack_bf16x2(y[2], y[3]));
+            }
+            if (a.xq) {
+                const int64_t at = (int64_t)tok * a.n_heads * D + col;
+                const uint32_t q = quant_group8(y, lane & 7, on ? a.xd + (at >> 5) : nullptr);
+                if (on) *reinterpret_cast<uint32_t*>(a.xq + at) = q;
             }
         }
-    }
-    const float inv = L > 0.0f ? 1.0f / L : L;  // a row that saw nothing: zeros; NaN stays
-#pragma unroll
-    for (int j = 0; j < 4; j++) o[j] *= inv;
-    const int64_t col = (int64_t)h * D + 4 * lane;
-    if (a.out && on) {
-        T* const y = static_cast<T*>(a.out) + (int64_t)t * a.out_stride + col;
-        if constexpr (sizeof(T) == 4) *reinterpret_cast<float4*>(y) = make_float4(o[0], o[1], o[2], o[3]);
-        else *reinterpret_cast<uint2*>(y) = make_uint2(pack_bf16x2(o[0], o[1]), pack_bf16x2(o[2], o[3]));
-    }
-    if (a.xq) {
-        const int64_t e = (int64_t)t * a.n_heads * D + col;
-        const uint32_t q = quant_group8(o, lane & 7, on ? a.xd + (e >> 5) : nullptr);
-        if (on) *reinterpret_cast<uint32_t*>(a.xq + e) = q;
+        st0 += run;
+        todo -= run;
     }
 }
 
@@ -238,8 +270,8 @@ static int make_plan(lq_ctx* ctx, const PrefixAttnArgs& a, const PagedSeqs& s, i
     p->pb = p->pair_p ? 2 * half : half;
     p->pair_o = most_q > half;
     p->ob = p->pair_o ? 2 * half : half;
-    p->cap_p = (int)std::min<int64_t>(p->pb, R);
-    p->cap_o = (int)std::min<int64_t>(p->ob, most_q);
+    p->cap[0] = (int)std::min<int64_t>(p->pb, R);
+    p->cap[1] = (int)std::min<int64_t>(p->ob, most_q);
     p->n_rb = ceil_div(R, p->pb);
     p->np = ceil_div(a.prefix_len, tile);
     const int64_t items_p = (int64_t)a.n_kv * p->n_rb, items_o = a.n_kv * (R / p->ob + s.n_seqs + 1);
@@ -248,26 +280,43 @@ static int make_plan(lq_ctx* ctx, const PrefixAttnArgs& a, const PagedSeqs& s, i
     p->sp = (int)(items_p * p->np);
     p->workers = (int)std::max<int64_t>(1, std::min<int64_t>(ctx->sm_count, steps));
     p->workers_mul = ((1ull << 40) + p->workers - 1) / p->workers;
-    const int64_t slots_p = p->np ? items_p + 2 * p->workers : 0, slots_o = items_o + 2 * p->workers;
-    auto al = [](size_t b) { return (b + 255) & ~(size_t)255; };
-    const size_t cum = al((size_t)(s.n_seqs + 1) * 4), ml_p = al((size_t)slots_p * p->cap_p * 8),
-                 ml_o = al((size_t)slots_o * p->cap_o * 8), o_p = al((size_t)slots_p * p->cap_p * D * 4),
-                 o_o = al((size_t)slots_o * p->cap_o * D * 4);
-    const int rc = ensure_paged(ctx, cum + ml_p + ml_o + o_p + o_o);
+    const int64_t items[2] = {p->np ? items_p : 0, items_o};
+    size_t at = 0;
+    auto place = [&at](int64_t n, size_t size) {
+        const size_t here = at;
+        at += ((size_t)n * size + 255) & ~(size_t)255;
+        return here;
+    };
+    const size_t steps_at = place(1, 4), split_at = place(2 * p->workers, sizeof(SplitItem));
+    size_t first_at[2], last_at[2], ml_at[2], o_at[2];
+    for (int k = 0; k < 2; k++) {
+        const int64_t slots = items[k] ? items[k] + 2 * p->workers : 0;
+        LQ_REQUIRE(ctx, slots < (1ll << 31), "lq_prefix_attention: too many partials");
+        first_at[k] = place(items[k], 4);
+        last_at[k] = place(items[k], 4);
+        ml_at[k] = place(slots * p->cap[k], 8);
+        o_at[k] = place(slots * p->cap[k], (size_t)D * 4);
+    }
+    const int rc = ensure_paged(ctx, at);
     if (rc) return rc;
     uint8_t* w = static_cast<uint8_t*>(ctx->paged);
-    p->cum = reinterpret_cast<int32_t*>(w);
-    p->ml_p = reinterpret_cast<float2*>(w += cum);
-    p->ml_o = reinterpret_cast<float2*>(w += ml_p);
-    p->o_p = reinterpret_cast<float*>(w += ml_o);
-    p->o_o = reinterpret_cast<float*>(w += o_p);
+    p->own_steps = reinterpret_cast<int32_t*>(w + steps_at);
+    p->split = reinterpret_cast<SplitItem*>(w + split_at);
+    for (int k = 0; k < 2; k++) {
+        p->first[k] = reinterpret_cast<int32_t*>(w + first_at[k]);
+        p->last[k] = reinterpret_cast<int32_t*>(w + last_at[k]);
+        p->ml[k] = reinterpret_cast<float2*>(w + ml_at[k]);
+        p->o[k] = reinterpret_cast<float*>(w + o_at[k]);
+    }
     return LQ_OK;
 }
 
 template <typename T, int D>
 static int launch_merge(lq_ctx* ctx, const PrefixAttnArgs& a, const PagedSeqs& s, const PrefixPlan& p) {
-    return launch_kernel(ctx, prefix_attn_merge_kernel<T, D>, dim3((unsigned)ceil_div((int64_t)s.rows * a.n_heads, 8)),
-                         dim3(256), 0, "prefix_attn_merge", a, s, p);
+    const dim3 grid = a.prefix_len > 0 ? dim3((unsigned)((int64_t)s.rows * a.n_kv))
+                                       : dim3((unsigned)(p.pair_o ? p.workers : 2 * p.workers),
+                                              (unsigned)ceil_div(p.cap[1], MERGE_ROWS));
+    return launch_kernel(ctx, prefix_attn_merge_kernel<T, D>, grid, dim3(MERGE_ROWS * D / 4), 0, "prefix_attn_merge", a, s, p);
 }
 
 }  // namespace lq

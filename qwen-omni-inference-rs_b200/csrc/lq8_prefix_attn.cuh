@@ -42,6 +42,29 @@ __device__ __forceinline__ void pa_store32(const PrefixAttnArgs& a, int tok, int
     }
 }
 
+// rows tok0 .. tok0 + n - 1, which see no position: zeros, by `threads` threads
+template <typename T, int D>
+__device__ __forceinline__ void zero_rows(const PrefixAttnArgs& a, int tok0, int n, int thread, int threads) {
+    const uint4 z = make_uint4(0, 0, 0, 0);
+    const int blocks = a.n_heads * (D / 32);  // of 32 dims
+#pragma unroll 1
+    for (int tok = tok0; tok < tok0 + n; tok++)
+#pragma unroll 1
+        for (int i = thread; i < blocks; i += threads) {
+            if (a.out) {
+                uint4* const o = reinterpret_cast<uint4*>(static_cast<T*>(a.out) + (int64_t)tok * a.out_stride + i * 32);
+#pragma unroll
+                for (int j = 0; j < (int)sizeof(T) * 2; j++) o[j] = z;
+            }
+            if (a.xq) {
+                const int64_t at = (int64_t)tok * blocks + i;
+                uint4* const q = reinterpret_cast<uint4*>(a.xq + at * 32);
+                q[0] = q[1] = z;
+                a.xd[at] = 0;
+            }
+        }
+}
+
 int launch_prefix_attn_tc(lq_ctx* ctx, const PrefixAttnArgs& a, const PagedSeqs& s, const PrefixPlan& p, int D);
 
 }  // namespace lq

@@ -15,7 +15,7 @@
 // Warps 0-3: softmax of flow 0 (TMEM lane = row = thread); warps 4-7: flow 1; warp 8: TMA
 // producer, which reads the page table and brings K and V tiles page by page into a ring of 32 KB
 // stages (128-byte swizzle; pages past the end come as zeros from an out-of-range coordinate);
-// warp 9: TMEM allocator and MMA issuer; warp 10: scheduler, the only one that walks the line: it
+// warp 9: TMEM allocator and MMA issuer; warp 11: zeros for rows that see nothing; warp 10: scheduler, the only one that walks the line: it
 // hands each flow its segments (PaSeg) through a small ring, so the other roles' code stays short
 // (every role walking by itself came to 300 KB of code, and the instruction misses took ten times
 // the arithmetic). Per round the MMA warp issues, for each flow, P V of the round before and then
@@ -36,14 +36,14 @@ namespace lq {
 constexpr int PA_ROWS = 128;      // rows of a flow (MMA M)
 constexpr int PA_TILE = 128;      // positions of a step
 constexpr int PA_STAGES = 4;
-constexpr int PA_THREADS = 384;   // warps 0-7 softmax, 8 TMA, 9 MMA, 10 scheduler, 11 nothing
+constexpr int PA_THREADS = 384;   // warps 0-7 softmax, 8 TMA, 9 MMA, 10 scheduler, 11 empty rows
 // registers: 384 x 168 at launch = 256 x 216 for the softmax warps + 128 x 72 for the others
 constexpr int PA_REGS = 216, PA_REGS_LOW = 72;
 constexpr int PA_SCAN = 1024;     // entries of the scan over the sequences
 constexpr int PA_BATCH = 32;      // segments the scheduler works out at a time, a lane each
 constexpr int ERR_PA_WAIT = 94;   // a wait ran out
 
-enum { SEG_OWN = 1, SEG_PAIRED = 2, SEG_END = 4, SEG_WHOLE = 8 };
+enum { SEG_OWN = 1, SEG_PAIRED = 2, SEG_END = 4, SEG_WHOLE = 8, SEG_HALF = 16 };  // HALF: the second of a block
 // the steps [t0, t1) of one item, for one flow
 struct alignas(16) PaSeg {
     int t0, t1;     // tiles
@@ -53,7 +53,7 @@ struct alignas(16) PaSeg {
     int kv_end;     // positions the item sees
     int row0;       // first stacked row
     int voff;       // own items: the stacked row of token t sees t + voff positions
-    int slot;       // first row of the flow's partial
+    int slot;       // slot of the partial
     int n1;         // paired: rows of the second half
     int pad;
 };
@@ -294,14 +294,14 @@ prefix_attn_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_co
         asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], 512;" ::"r"(smem_addr(&c.tmem)));
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
     }
-    pdl_trigger();
     pdl_wait();
+    pdl_trigger();  // (after the wait: the merge reads the call's lengths before its own)
     // own steps of every entry (a run of per_entry sequences), then their running sum; a warp looks
     // at a sequence of many row blocks, else a thread
     const int per_entry = (g.s.n_seqs + PA_SCAN - 1) / PA_SCAN;
     const int n_entries = per_entry == 1 ? g.s.n_seqs : (g.s.n_seqs + per_entry - 1) / per_entry;
     const OwnSteps os{g.a, g.p};
-    const bool by_warp = per_entry == 1 && g.p.cap_o == g.p.ob && g.a.max_q * g.a.group > 4 * g.p.ob;
+    const bool by_warp = per_entry == 1 && g.a.max_q * g.a.group > 4 * g.p.ob;
 #pragma unroll 1
     for (int e = by_warp ? warp : tid; e < n_entries; e += by_warp ? PA_THREADS / 32 : PA_THREADS) {
         int n = 0;
@@ -329,18 +329,7 @@ prefix_attn_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_co
     tc_after();
     const uint32_t tmem = __shfl_sync(0xffffffffu, c.tmem, 0);
     const int so = c.scan[n_entries];
-    if (blockIdx.x == 0) {  // the sequences' places in the line, for the merge
-#pragma unroll 1
-        for (int e = tid; e < n_entries; e += PA_THREADS) {
-            int n = c.scan[e];
-#pragma unroll 1
-            for (int b = e * per_entry; b < min(g.s.n_seqs, (e + 1) * per_entry); b++) {
-                g.p.cum[b] = n;
-                if (per_entry > 1) n += os.per_head(seq_info(g.a, g.s, b, false)) * g.a.n_kv;
-            }
-        }
-        if (tid == 0) g.p.cum[g.s.n_seqs] = so;
-    }
+    if (blockIdx.x == 0 && tid == 0) *g.p.own_steps = so;  // for the merge
     const int me = blockIdx.x;
     // a warp's place in the segments of a flow
     struct Feed {
@@ -455,11 +444,16 @@ prefix_attn_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_co
                         }
                         return m == -INFINITY ? 0.0f : -m;
                     };
-                    if (sg.n > 64 && __all_sync(0xffffffffu, lim >= PA_TILE)) {
+                    if (sg.n > 64) {
                         float s[128];
 #pragma unroll
                         for (int j = 0; j < 4; j++) tmem_ld32(reinterpret_cast<uint32_t*>(s) + 32 * j, t_s + 32 * j);
                         tmem_wait_ld();
+                        if (!__all_sync(0xffffffffu, lim >= PA_TILE)) {
+#pragma unroll
+                            for (int i = 0; i < 128; i++)
+                                if (i >= lim) s[i] = -INFINITY;
+                        }
                         float mx[4] = {s[0], s[1], s[2], s[3]};
 #pragma unroll
                         for (int i = 4; i < 124; i += 8)
@@ -482,9 +476,9 @@ prefix_attn_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_co
                         }
                         l += (sum[0].x + sum[0].y) + (sum[1].x + sum[1].y);
                     } else {
-                        // few rows, or the end of an item: two passes over S, 32 columns at a time, in
-                        // a tenth of the code (few rows come in many short segments, and there the
-                        // instruction fetch costs more than the arithmetic)
+                        // few rows: two passes over S, 32 columns at a time, in a tenth of the code
+                        // (they come in many short segments, where fetching the instructions costs
+                        // more than the arithmetic)
                         float mt = -INFINITY, sum = 0.0f, neg = 0.0f;
 #pragma unroll 1
                         for (int pass = 0; pass < 2; pass++) {
@@ -540,11 +534,12 @@ prefix_attn_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_co
             if (!busy) continue;
             // ---- the segment's result: the row itself, or a partial for the merge ----
             const bool own = sg.flags & SEG_OWN, whole = sg.flags & SEG_WHOLE;
-            const int64_t at_o = sg.slot + row;
             const int head = sg.kh * g.a.group + st - tok * g.a.group;
             const float inv = l > 0.0f ? 1.0f / l : 0.0f;
-            if (mine && !whole) (own ? g.p.ml_o : g.p.ml_p)[at_o] = make_float2(m, l);
-            float* const po = (own ? g.p.o_o : g.p.o_p) + at_o * D;
+            const int cap = g.p.cap[own], at_o = (sg.flags & SEG_HALF ? PA_ROWS : 0) + row;
+            if (mine && !whole) g.p.ml[own][(int64_t)sg.slot * cap + at_o] = make_float2(m, l);
+            // four dims of all rows lie together, so that a warp's stores are 512 bytes each
+            float4* po = reinterpret_cast<float4*>(g.p.o[own]) + (int64_t)sg.slot * (D / 4) * cap + at_o;
 #pragma unroll 1
             for (int i = 0; i < D; i += 32) {
                 uint32_t r[32];
@@ -552,8 +547,8 @@ prefix_attn_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_co
                 tmem_wait_ld();
                 if (mine && !whole) {
 #pragma unroll
-                    for (int j = 0; j < 32; j += 4)
-                        *reinterpret_cast<uint4*>(po + i + j) = make_uint4(r[j], r[j + 1], r[j + 2], r[j + 3]);
+                    for (int j = 0; j < 32; j += 4, po += cap)
+                        *reinterpret_cast<uint4*>(po) = make_uint4(r[j], r[j + 1], r[j + 2], r[j + 3]);
                 } else if (mine) {
                     float v[32];
 #pragma unroll
@@ -761,6 +756,8 @@ prefix_attn_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_co
                 batch[f]++;
             };
             PaSeg o{0, 1, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0};
+            if (g.a.prefix_len == 0 && lane < (g.p.pair_o ? 1 : 2)) g.p.split[g.p.pair_o ? me : 2 * me + lane].rows = 0;
+            __syncwarp();
 #pragma unroll 1
             for (int part = 0; part < 2 && ok; part++) {
                 const bool own = part, paired = own ? g.p.pair_o : g.p.pair_p;
@@ -805,7 +802,7 @@ prefix_attn_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_co
                     const int upto = warp_scan(nt - o.t0, lane), start = w.step + upto - (nt - o.t0);
                     n = min(nt - o.t0, w.hi - start);
                     o.t1 = o.t0 + n;
-                    const int block = own ? g.p.ob : g.p.pb, cap = own ? g.p.cap_o : g.p.cap_p;
+                    const int block = own ? g.p.ob : g.p.pb, worker = paired ? me : 2 * me + f;
                     const int rows = si.q * g.a.group - rb * block;  // of the whole block
                     o.n = min(PA_ROWS, rows);
                     o.n1 = paired ? max(0, min(PA_ROWS, rows - PA_ROWS)) : 0;
@@ -815,12 +812,19 @@ prefix_attn_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_co
                     o.b = b;
                     o.row0 = (own ? si.q0 * g.a.group : 0) + rb * block;
                     o.voff = own ? si.kv - si.q + 1 - si.q0 : 0;
-                    o.slot = ((own ? g.a.n_kv * os.base(si, b) : 0) + j + (paired ? me : 2 * me + f)) * cap;
+                    const int item = (own ? g.a.n_kv * os.base(si, b) : 0) + j;
+                    o.slot = item + worker;
+                    if (n > 0) {  // for the merge
+                        if (o.t0 == 0) g.p.first[own][item] = worker;
+                        if (o.t1 == nt) g.p.last[own][item] = worker;
+                        if (own && g.a.prefix_len == 0 && o.t0 == 0 && o.t1 < nt)
+                            g.p.split[worker] = SplitItem{min(rows, block), o.row0, kh, item};
+                    }
                     if (__any_sync(0xffffffffu, n > 0)) put(f, o, n > 0);
                     if (paired && ok && __any_sync(0xffffffffu, n > 0)) {  // the other half of the block
                         o.n = o.n1;
                         o.row0 += PA_ROWS;
-                        o.slot += PA_ROWS;
+                        o.flags |= SEG_HALF;
                         put(1, o, n > 0);
                     }
                     const int all = min(__shfl_sync(0xffffffffu, upto, 31), w.hi - w.step);
@@ -840,6 +844,14 @@ prefix_attn_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_co
             o.flags = SEG_END;
 #pragma unroll 1
             for (int f = 0; f < 2 && ok; f++) put(f, o, lane == 0);
+        } else if (g.a.prefix_len == 0) {
+            // warp 11: rows before their sequence's first position see nothing when there is no
+            // prefix either
+#pragma unroll 1
+            for (int b = me; b < g.s.n_seqs; b += gridDim.x) {
+                const SeqInfo si = pa_seq(g, c, b);
+                if (si.kv < si.q) zero_rows<__nv_bfloat16, D>(g.a, si.q0, si.q - si.kv, lane, 32);
+            }
         }
     }
     tc_before();

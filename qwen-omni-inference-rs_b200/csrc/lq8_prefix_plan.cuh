@@ -34,6 +34,12 @@ struct PrefixAttnArgs {
     __host__ __device__ __forceinline__ int group_div(int x) const { return (int)(((uint64_t)x * group_mul) >> 36); }
 };
 
+// an own item that is cut between workers
+struct SplitItem {
+    int rows;      // rows of its block (0: none)
+    int row0, kh, item;
+};
+
 struct PrefixPlan {
     int tile;                   // positions of a step
     int pb, ob;                 // rows of a block: prefix items, own items
@@ -43,12 +49,13 @@ struct PrefixPlan {
     int sp;                     // steps of the prefix
     int workers;                // CTAs that share the line
     uint64_t workers_mul;       // ceil(2^40 / workers)
-    int cap_p, cap_o;           // rows a partial slot holds
-    int32_t* cum;               // [n_seqs + 1] own steps before each sequence
-    float* o_p;                 // prefix partials [slot][cap_p][D], unnormalised
-    float2* ml_p;               // [slot][cap_p]: running maximum (log2 units) and sum
-    float* o_o;                 // own partials
-    float2* ml_o;
+    int cap[2];                 // rows a partial slot holds (prefix, own)
+    int32_t* own_steps;         // [1] own steps in all, written by the first CTA
+    int32_t* first[2];          // per item (prefix, own): the first worker of its steps,
+    int32_t* last[2];           // and the last
+    SplitItem* split;           // per worker, without a prefix: the cut item it begins
+    float* o[2];                // partials, unnormalised: [slot][D/4][cap] of four dims
+    float2* ml[2];              // [slot][cap]: running maximum (log2 units) and sum
 };
 
 // a sequence's rows and own length, with what the call's bounds do not hold taken out
