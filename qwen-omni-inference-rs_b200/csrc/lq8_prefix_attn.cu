@@ -106,143 +106,170 @@ __global__ void __launch_bounds__(128) prefix_attn_row_kernel(PrefixAttnArgs a, 
 // =========================================================================================
 // Merge: joins the partials of the workers that had a piece of a row's prefix item or own item, in
 // the order of the line: with M the largest of their maxima, o = sum 2^(m_i - M) o_i /
-// sum 2^(m_i - M) l_i. With a prefix every row has at least its prefix partials: a CTA takes the
-// G stacked rows of a token and kv head. Without one only cut items are left (a whole one was
-// written by its worker): a CTA takes up to MERGE_ROWS rows of the item that a worker began. A
-// thread adds up four dims of a row; rows are next to each other in memory, so a warp reads runs
-// of 16 bytes x rows. A warp looks after the weights of a row, a lane per partial.
+// sum 2^(m_i - M) l_i. A CTA takes up to MR rows of an own item (a sequence's row block and kv
+// head), which share the own item's partials and, but for a block's end, those of a prefix item.
+// Without a prefix only the items that are cut between workers are left: a worker leaves a note of
+// the one that it begins. A thread adds up CH MR / 256 vectors of four dims of one row; rows lie
+// next to each other in memory.
 // =========================================================================================
-constexpr int MERGE_ROWS = 8;
-constexpr int MERGE_MAX = 640;  // partials of a row: at most two workers a CTA in either part
+constexpr int MERGE_CHUNK = 32;   // partials looked at together
 
-template <typename T, int D>
-__global__ void __launch_bounds__(MERGE_ROWS * D / 4) prefix_attn_merge_kernel(PrefixAttnArgs a, PagedSeqs s, PrefixPlan p) {
-    constexpr int CH = D / 4;
-    __shared__ int slot[MERGE_MAX];
-    __shared__ float weight[MERGE_ROWS][MERGE_MAX];
-    __shared__ float inv[MERGE_ROWS];
-    __shared__ __align__(16) float stage[MERGE_ROWS][D];
-    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, warps = blockDim.x >> 5;
+template <typename T, int D, int MR>
+__global__ void __launch_bounds__(256) prefix_attn_merge_kernel(PrefixAttnArgs a, PagedSeqs s, PrefixPlan p) {
+    constexpr int CH = D / 4, SUBS = 256 / MR;  // vectors of a row; threads that share a row
+    constexpr int VEC = (CH + SUBS - 1) / SUBS;
+    __shared__ int slot[MERGE_CHUNK];
+    __shared__ float weight[MERGE_CHUNK][MR];
+    __shared__ float2 red[SUBS][MR];
+    __shared__ __align__(16) float stage[MR][D + 4];
+    const int tid = threadIdx.x, lane = tid & 31, r = tid % MR, sub = tid / MR;
     const OwnSteps os{a, p};
-    // the group's stacked rows st0 .. st0 + todo - 1 of kv head kh; for the two parts the item, the
-    // first row's place in it and whether it has steps
-    int st0, todo, kh, item[2] = {0, 0}, in[2] = {0, 0};
-    bool any[2] = {false, false};
-    int b = 0, t = 0;
-    SeqInfo si{0, 0, 0};
-    const bool by_row = a.prefix_len > 0;
-    if (by_row) {  // (the call's inputs: complete before the kernel that this one waits for began)
-        t = blockIdx.x / a.n_kv;
-        kh = blockIdx.x - t * a.n_kv;
-        b = s.q_start ? seq_of_row(s.q_start, s.n_seqs, t, lane) : t;
-        if (b >= s.n_seqs) return;
-        si = seq_info(a, s, b, false);
-        st0 = t * a.group;
-        todo = a.group;
+    const bool with_prefix = a.prefix_len > 0;
+    // the item, its rows st0 .. st0 + todo - 1 of this CTA, the first one's place in the item
+    int st0 = 0, todo = 0, kh = 0, own_item = 0, own_in = blockIdx.y * MR;
+    bool own = true;
+    if (with_prefix) {  // (the call's inputs: complete before the kernel that this one waits for began)
+        const int x = blockIdx.x / a.n_kv;
+        kh = blockIdx.x - x * a.n_kv;
+        // the last sequence with base(b) <= x
+        int lo = 0, n = s.n_seqs - 1;
+        while (n > 0) {
+            const int step = (n + 31) >> 5, i = lo + min(n, (lane + 1) * step);
+            const int q0 = s.q_start ? s.q_start[i] : i;
+            const int c = __popc(__ballot_sync(0xffffffffu, q0 * a.group / p.ob + i <= x));
+            if (c == 32) {
+                lo += n;
+                break;
+            }
+            const int skip = min(n, c * step);
+            n = min(step - 1, n - skip);
+            lo += skip;
+        }
+        const SeqInfo si = seq_info(a, s, lo, false);
+        const int rb = x - os.base(si, lo), nb = os.blocks(si);
+        if (rb < 0 || rb >= nb) return;
+        st0 = si.q0 * a.group + rb * p.ob + own_in;
+        todo = min(MR, min(p.ob, si.q * a.group - rb * p.ob) - own_in);
+        own_item = a.n_kv * x + kh * nb + rb - a.n_kv * rb;  // n_kv base + kh nb + rb
+        own = os.visible(si, rb) > 0;
     }
     pdl_wait();
     pdl_trigger();
-    if (!by_row) {
+    if (!with_prefix) {
         const SplitItem w = p.split[blockIdx.x];
-        st0 = w.row0 + blockIdx.y * MERGE_ROWS;
-        todo = min(MERGE_ROWS, w.rows - (int)blockIdx.y * MERGE_ROWS);
+        st0 = w.row0 + own_in;
+        todo = min(MR, w.rows - own_in);
         kh = w.kh;
-        item[1] = w.item;
-        in[1] = blockIdx.y * MERGE_ROWS;
-        any[1] = true;
+        own_item = w.item;
     }
     const Line line(p, *p.own_steps);
 #pragma unroll 1
-    for (; todo > 0;) {
-        int run = min(todo, MERGE_ROWS);  // rows that share their items
-        if (by_row) {
-            const int rb_p = st0 / p.pb;
-            item[0] = kh * p.n_rb + rb_p;
-            in[0] = st0 - rb_p * p.pb;
-            any[0] = true;
+    while (todo > 0) {
+        int run = todo, item[2] = {0, own_item}, in[2] = {0, own_in}, v0[2] = {0, 0}, cnt[2] = {0, 0};
+        if (with_prefix) {  // rows that share the prefix item
+            const int rb = st0 / p.pb;
+            item[0] = kh * p.n_rb + rb;
+            in[0] = st0 - rb * p.pb;
             run = min(run, p.pb - in[0]);
-            any[1] = false;
-            if (t < si.q0 + si.q) {
-                const int r = st0 - si.q0 * a.group, rb = r / p.ob;
-                item[1] = a.n_kv * os.base(si, b) + kh * os.blocks(si) + rb;
-                in[1] = r - rb * p.ob;
-                any[1] = os.visible(si, rb) > 0;
-                run = min(run, p.ob - in[1]);
-            }
+            v0[0] = p.first[0][item[0]];
+            cnt[0] = p.last[0][item[0]] - v0[0] + 1;
         }
-        int v0[2] = {0, 0}, cnt[2] = {0, 0};
+        if (own) {
+            v0[1] = p.first[1][item[1]];
+            cnt[1] = p.last[1][item[1]] - v0[1] + 1;
+        }
+        const int n = cnt[0] + cnt[1];
+        const bool mine = r < run;
+        // pass 0: the rows' maxima and sums; pass 1: the vectors
+        float M = -INFINITY, L = 0.0f;
+        float4 o[VEC];
 #pragma unroll
-        for (int part = 0; part < 2; part++)
-            if (any[part]) {
-                v0[part] = p.first[part][item[part]];
-                cnt[part] = p.last[part][item[part]] - v0[part] + 1;
-            }
-        const int n = min(cnt[0] + cnt[1], MERGE_MAX);
-        __syncthreads();  // (the shared arrays are read no more)
+        for (int k = 0; k < VEC; k++) o[k] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
 #pragma unroll 1
-        for (int i = tid; i < n; i += blockDim.x) {
-            const int part = i >= cnt[0], k = i - (part ? cnt[0] : 0), v = v0[part] + k;
-            const bool paired = part ? p.pair_o : p.pair_p;
-            bool has = k == 0 || k == cnt[part] - 1;
-            if (!has) {  // a worker in between may have no step at all
-                int lo, hi;
-                flow_range(line, p, paired ? v : v >> 1, paired ? 0 : v & 1, part, lo, hi);
-                has = lo < hi;
-            }
-            slot[i] = has ? item[part] + v : -1;
-        }
-        __syncthreads();
+        for (int pass = 0; pass < 2; pass++) {
 #pragma unroll 1
-        for (int r = warp; r < run; r += warps) {
-            float M = -INFINITY;
-#pragma unroll 1
-            for (int i = lane; i < n; i += 32) {
-                const int part = i >= cnt[0];
-                if (slot[i] >= 0) M = fmaxf(M, p.ml[part][(int64_t)slot[i] * p.cap[part] + in[part] + r].x);
-            }
-            M = warp_max(M);
-            float L = 0.0f;
-#pragma unroll 1
-            for (int i = lane; i < n; i += 32) {
-                const int part = i >= cnt[0];
-                float w = 0.0f;
-                if (slot[i] >= 0) {
-                    const float2 ml = p.ml[part][(int64_t)slot[i] * p.cap[part] + in[part] + r];
-                    if (ml.x != -INFINITY) w = exp2f(ml.x - M);
-                    L = fmaf(w, ml.y, L);
+            for (int c0 = 0; c0 < n; c0 += MERGE_CHUNK) {
+                const int m = min(MERGE_CHUNK, n - c0);
+                if (pass == 0 || n > MERGE_CHUNK) {
+                    __syncthreads();  // (the last chunk's slots and weights are read no more)
+                    if (tid < m) {
+                        const int i = c0 + tid, part = i >= cnt[0], k = i - (part ? cnt[0] : 0), v = v0[part] + k;
+                        bool has = k == 0 || k == cnt[part] - 1;
+                        if (!has) {  // a worker in between may have no step at all
+                            const bool paired = part ? p.pair_o : p.pair_p;
+                            int lo, hi;
+                            flow_range(line, p, paired ? v : v >> 1, paired ? 0 : v & 1, part, lo, hi);
+                            has = lo < hi;
+                        }
+                        slot[tid] = has ? item[part] + v : -1;
+                    }
+                    __syncthreads();
                 }
-                weight[r][i] = w;
-            }
-            L = warp_sum(L);
-            if (lane == 0) inv[r] = L > 0.0f ? 1.0f / L : L;  // a row that saw nothing: zeros; NaN stays
-        }
-        __syncthreads();
-        const int r = tid % MERGE_ROWS, ch = tid / MERGE_ROWS;
-        float4 o = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-        if (r < run) {
-#pragma unroll 4
-            for (int i = 0; i < n; i++) {
-                const int part = i >= cnt[0];
-                const float w = weight[r][i];
-                if (slot[i] >= 0) {
-                    const float4 x = reinterpret_cast<const float4*>(p.o[part])[((int64_t)slot[i] * CH + ch) * p.cap[part] + in[part] + r];
-                    o.x = fmaf(w, x.x, o.x);
-                    o.y = fmaf(w, x.y, o.y);
-                    o.z = fmaf(w, x.z, o.z);
-                    o.w = fmaf(w, x.w, o.w);
+#pragma unroll 1
+                for (int i = sub; i < m; i += SUBS) {
+                    const int part = c0 + i >= cnt[0];
+                    float2 ml = make_float2(-INFINITY, 0.0f);
+                    if (mine && slot[i] >= 0) ml = p.ml[part][(int64_t)slot[i] * p.cap[part] + in[part] + r];
+                    if (pass == 0) {
+                        const float up = fmaxf(M, ml.x);
+                        if (up != -INFINITY) L = L * exp2f(M - up) + ml.y * exp2f(ml.x - up);
+                        M = up;
+                    } else {
+                        weight[i][r] = ml.x == -INFINITY ? 0.0f : exp2f(ml.x - M);
+                    }
+                }
+                if (pass == 1) {
+                    __syncthreads();
+                    if (mine) {
+#pragma unroll 2
+                        for (int i = 0; i < m; i++) {
+                            const int part = c0 + i >= cnt[0];
+                            if (slot[i] < 0) continue;
+                            const float w = weight[i][r];
+                            const float4* src = reinterpret_cast<const float4*>(p.o[part]) +
+                                                ((int64_t)slot[i] * CH + sub) * p.cap[part] + in[part] + r;
+#pragma unroll
+                            for (int k = 0; k < VEC; k++) {
+                                if (CH % SUBS && sub + k * SUBS >= CH) break;
+                                const float4 x = src[(int64_t)k * SUBS * p.cap[part]];
+                                o[k].x = fmaf(w, x.x, o[k].x);
+                                o[k].y = fmaf(w, x.y, o[k].y);
+                                o[k].z = fmaf(w, x.z, o[k].z);
+                                o[k].w = fmaf(w, x.w, o[k].w);
+                            }
+                        }
+                    }
                 }
             }
-            const float k = inv[r];
-            *reinterpret_cast<float4*>(&stage[r][4 * ch]) = make_float4(o.x * k, o.y * k, o.z * k, o.w * k);
+            if (pass == 0) {  // over the threads of a row, in their order
+                red[sub][r] = make_float2(M, L);
+                __syncthreads();
+                M = -INFINITY;
+                for (int k = 0; k < min(SUBS, n); k++) M = fmaxf(M, red[k][r].x);
+                L = 0.0f;
+                for (int k = 0; k < min(SUBS, n); k++)
+                    if (red[k][r].x != -INFINITY) L += red[k][r].y * exp2f(red[k][r].x - M);
+            }
+        }
+        const float inv = L > 0.0f ? 1.0f / L : L;  // a row that saw nothing: zeros; NaN stays
+        if (mine) {
+#pragma unroll
+            for (int k = 0; k < VEC; k++) {
+                if (CH % SUBS && sub + k * SUBS >= CH) break;
+                *reinterpret_cast<float4*>(&stage[r][4 * (sub + k * SUBS)]) =
+                    make_float4(o[k].x * inv, o[k].y * inv, o[k].z * inv, o[k].w * inv);
+            }
         }
         __syncthreads();
-        {  // out, a row's dims side by side
-            const int rr = tid / CH, e = tid % CH * 4, st = st0 + rr, tok = a.group_div(st);
+        // out, a row's dims side by side
+#pragma unroll 1
+        for (int base = 0; base < run * CH; base += 256) {
+            const int rr = (base + tid) / CH, e = (base + tid) % CH * 4, st = st0 + rr, tok = a.group_div(st);
             const bool on = rr < run;
             float y[4] = {0.0f, 0.0f, 0.0f, 0.0f};
             if (on) {
-#pragma unroll
-                for (int j = 0; j < 4; j++) y[j] = stage[rr][e + j];
+                const float4 v = *reinterpret_cast<const float4*>(&stage[rr][e]);
+                y[0] = v.x, y[1] = v.y, y[2] = v.z, y[3] = v.w;
             }
             const int64_t col = (int64_t)(kh * a.group + st - tok * a.group) * D + e;
             if (a.out && on) {
@@ -256,7 +283,9 @@ __global__ void __launch_bounds__(MERGE_ROWS * D / 4) prefix_attn_merge_kernel(P
                 if (on) *reinterpret_cast<uint32_t*>(a.xq + at) = q;
             }
         }
+        __syncthreads();
         st0 += run;
+        own_in += run;
         todo -= run;
     }
 }
@@ -313,10 +342,13 @@ static int make_plan(lq_ctx* ctx, const PrefixAttnArgs& a, const PagedSeqs& s, i
 
 template <typename T, int D>
 static int launch_merge(lq_ctx* ctx, const PrefixAttnArgs& a, const PagedSeqs& s, const PrefixPlan& p) {
-    const dim3 grid = a.prefix_len > 0 ? dim3((unsigned)((int64_t)s.rows * a.n_kv))
-                                       : dim3((unsigned)(p.pair_o ? p.workers : 2 * p.workers),
-                                              (unsigned)ceil_div(p.cap[1], MERGE_ROWS));
-    return launch_kernel(ctx, prefix_attn_merge_kernel<T, D>, grid, dim3(MERGE_ROWS * D / 4), 0, "prefix_attn_merge", a, s, p);
+    // a row of few heads leaves most of a 32-row CTA idle
+    const int mr = p.cap[1] <= 8 ? 8 : 32;
+    const int64_t R = (int64_t)s.rows * a.group;
+    const dim3 grid((unsigned)(a.prefix_len > 0 ? a.n_kv * (R / p.ob + s.n_seqs) : (p.pair_o ? 1 : 2) * p.workers),
+                    (unsigned)ceil_div(p.cap[1], mr));
+    return mr == 8 ? launch_kernel(ctx, prefix_attn_merge_kernel<T, D, 8>, grid, dim3(256), 0, "prefix_attn_merge", a, s, p)
+                   : launch_kernel(ctx, prefix_attn_merge_kernel<T, D, 32>, grid, dim3(256), 0, "prefix_attn_merge", a, s, p);
 }
 
 }  // namespace lq
