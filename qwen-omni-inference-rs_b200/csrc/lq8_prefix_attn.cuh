@@ -42,6 +42,28 @@ __device__ __forceinline__ void pa_store32(const PrefixAttnArgs& a, int tok, int
     }
 }
 
+// two dims (at, at + 1) of row tok, head h, by the 16 lanes that hold the 32 dims of a block; every
+// lane of the warp calls it, those with `on` write
+template <typename T, int D>
+__device__ __forceinline__ void store2(const PrefixAttnArgs& a, int tok, int h, int at, float2 y, bool on) {
+    if (a.out && on) {
+        T* const o = static_cast<T*>(a.out) + (int64_t)tok * a.out_stride + (int64_t)h * D + at;
+        if constexpr (sizeof(T) == 4) *reinterpret_cast<float2*>(o) = y;
+        else *reinterpret_cast<uint32_t*>(o) = pack_bf16x2(y.x, y.y);
+    }
+    if (a.xq) {
+        float amax = fmaxf(fabsf(y.x), fabsf(y.y)), d, id;
+#pragma unroll
+        for (int o = 8; o > 0; o >>= 1) amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, o));
+        q8_scale(amax, d, id);
+        const int64_t i = ((int64_t)tok * a.n_heads + h) * D + at;
+        if (on) {
+            if (at % 32 == 0) a.xd[i / 32] = f2h(d);
+            *reinterpret_cast<uint16_t*>(a.xq + i) = (uint16_t)((q8_quant(y.x, id) & 0xFF) | (q8_quant(y.y, id) & 0xFF) << 8);
+        }
+    }
+}
+
 // rows tok0 .. tok0 + n - 1, which see no position: zeros, by `threads` threads
 template <typename T, int D>
 __device__ __forceinline__ void zero_rows(const PrefixAttnArgs& a, int tok0, int n, int thread, int threads) {

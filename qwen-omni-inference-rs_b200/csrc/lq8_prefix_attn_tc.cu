@@ -39,8 +39,9 @@ constexpr int PA_STAGES = 4;
 constexpr int PA_THREADS = 384;   // warps 0-7 softmax, 8 TMA, 9 MMA, 10 scheduler, 11 empty rows
 // registers: 384 x 168 at launch = 256 x 216 for the softmax warps + 128 x 72 for the others
 constexpr int PA_REGS = 216, PA_REGS_LOW = 72;
-constexpr int PA_SCAN = 1024;     // entries of the scan over the sequences
+constexpr int PA_SCAN = 512;      // entries of the scan over the sequences
 constexpr int PA_BATCH = 32;      // segments the scheduler works out at a time, a lane each
+constexpr int PA_FEW = 8;         // rows up to which the four warps of a flow share a tile's columns
 constexpr int ERR_PA_WAIT = 94;   // a wait ran out
 
 enum { SEG_OWN = 1, SEG_PAIRED = 2, SEG_END = 4, SEG_WHOLE = 8, SEG_HALF = 16 };  // HALF: the second of a block
@@ -66,6 +67,8 @@ struct PaCtl {
     int abort;
     int seg_n[2][2];
     PaSeg seg[2][2][PA_BATCH];
+    float2 few_ml[2][4][PA_FEW];
+    alignas(16) float few_o[2][4][PA_FEW][36];  // 32 dims a row, padded against bank conflicts
     int4 info[PA_SCAN];     // up to PA_SCAN sequences: q0, q, kv
     int scan[PA_SCAN + 1];  // own steps before each entry
 };
@@ -354,9 +357,15 @@ prefix_attn_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_co
         o.voff = field(8), o.slot = field(9), o.n1 = field(10);
         return true;
     };
-    // Q of a flow: up to 64 rows take one half of the buffer and the next segment's the other
-    // (the MMA's rows past them read whatever lies there), so that they load a segment ahead
-    auto q_offset = [](const PaSeg& o, unsigned turn) { return o.n <= PA_ROWS / 2 ? (turn & 1) * (HALF / 2) : 0u; };
+    // Q of a flow: up to 64 rows take one half of the buffer and the next segment's the other, up to
+    // PA_FEW rows (in every 32) 8 rows side by side, so that they load a segment ahead; the MMA's
+    // other rows read whatever lies there
+    auto q_offset = [](const PaSeg& o, unsigned turn) {
+        return o.n <= PA_FEW ? (turn & 1) * 1024u : o.n <= PA_ROWS / 2 ? (turn & 1) * (HALF / 2) : 0u;
+    };
+    auto q_ahead = [](const PaSeg& now, const PaSeg& then) {
+        return max(now.n, then.n) <= PA_FEW || (min(now.n, then.n) > PA_FEW && max(now.n, then.n) <= PA_ROWS / 2);
+    };
 
     if (warp < 8) {
         // ------------------------------ softmax ------------------------------
@@ -386,11 +395,13 @@ prefix_attn_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_co
         auto q_start = [&]() {  // its Q on the way to shared memory
             const uint32_t base = sq + q_offset(nx, turn++);
             constexpr int CH = D / 8;
+            const int copies = nx.n <= PA_FEW ? 4 : 1;  // few rows: one copy for each warp's lanes
 #pragma unroll 1
-            for (int i = row; i < nx.n * CH; i += 128) {
-                const int r = i / CH, ch = i % CH, t = g.a.group_div(nx.row0 + r);
+            for (int i = row; i < nx.n * CH * copies; i += 128) {
+                const int rr = i / CH, ch = i % CH, r = copies == 4 ? rr >> 2 : rr, t = g.a.group_div(nx.row0 + r);
                 const int h = nx.kh * g.a.group + nx.row0 + r - t * g.a.group;
-                const uint32_t dst = base + (ch >> 3) * HALF + r * 128 + (((ch & 7) ^ (r & 7)) << 4);
+                const int at = copies == 4 ? (rr & 3) * 32 + r : r;
+                const uint32_t dst = base + (ch >> 3) * HALF + at * 128 + (((ch & 7) ^ (at & 7)) << 4);
                 asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst),
                              "l"(static_cast<const __nv_bfloat16*>(g.a.q) + (int64_t)t * g.a.q_stride + h * D + ch * 8));
             }
@@ -410,8 +421,10 @@ prefix_attn_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_co
         while (more == NX_SEG) {
             const PaSeg sg = nx;
             bool early = false;
-            const int st = sg.row0 + min(row, sg.n - 1), tok = g.a.group_div(st);
-            const bool mine = row < sg.n, busy = wq * 32 < sg.n;
+            const bool few = sg.n <= PA_FEW;
+            const int my_row = few ? lane : row;
+            const int st = sg.row0 + min(my_row, sg.n - 1), tok = g.a.group_div(st);
+            const bool mine = my_row < sg.n, busy = few || wq * 32 < sg.n;
             const int vis = sg.flags & SEG_OWN ? max(0, tok + sg.voff) : sg.kv_end;
             float m = -INFINITY, l = 0.0f;
             int t = sg.t0;
@@ -444,7 +457,41 @@ prefix_attn_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_co
                         }
                         return m == -INFINITY ? 0.0f : -m;
                     };
-                    if (sg.n > 64) {
+                    if (few) {
+                        // warp w takes columns 32 w .. 32 w + 31 of its own copy of the rows, with
+                        // a maximum and a sum of its own; its P is zero elsewhere
+                        float s[32];
+                        tmem_ld32(reinterpret_cast<uint32_t*>(s), t_s + 32 * wq);
+                        tmem_wait_ld();
+                        const int upto = lim - 32 * wq;
+                        if (!__all_sync(0xffffffffu, upto >= 32)) {
+#pragma unroll
+                            for (int i = 0; i < 32; i++)
+                                if (i >= upto) s[i] = -INFINITY;
+                        }
+                        float mx[4] = {s[0], s[1], s[2], s[3]};
+#pragma unroll
+                        for (int i = 4; i < 28; i += 8)
+#pragma unroll
+                            for (int j = 0; j < 4; j++) mx[j] = max3(mx[j], s[i + 2 * j], s[i + 2 * j + 1]);
+                        const float neg = raise(fmaxf(max3(mx[0], s[28], s[29]), max3(max3(mx[1], s[30], s[31]), mx[2], mx[3])));
+                        uint32_t pk[16];
+                        float2 sum = make_float2(0.0f, 0.0f);
+#pragma unroll
+                        for (int i = 0; i < 16; i++) {
+                            const float2 x = __ffma2_rn(make_float2(s[2 * i], s[2 * i + 1]), make_float2(cs, cs), make_float2(neg, neg));
+                            const float2 e = make_float2(ex2(x.x), ex2(x.y));
+                            sum = __fadd2_rn(sum, e);
+                            pk[i] = pack_bf16x2(e.x, e.y);
+                        }
+                        l += sum.x + sum.y;
+#pragma unroll 1
+                        for (int w = 0; w < 4; w++) {
+                            tmem_st16(t_s + 16 * ((wq + w) & 3), pk);
+#pragma unroll
+                            for (int i = 0; i < 16; i++) pk[i] = 0;
+                        }
+                    } else if (sg.n > 64) {
                         float s[128];
 #pragma unroll
                         for (int j = 0; j < 4; j++) tmem_ld32(reinterpret_cast<uint32_t*>(s) + 32 * j, t_s + 32 * j);
@@ -518,7 +565,7 @@ prefix_attn_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_co
                 if (lane == 0) mbar_arrive(&c.p_full[f]);
                 if (t == sg.t0) {
                     more = next(true);
-                    early = more == NX_SEG && sg.n <= PA_ROWS / 2 && nx.n <= PA_ROWS / 2;
+                    early = more == NX_SEG && q_ahead(sg, nx);
                     if (early) q_start();
                 }
             }
@@ -535,8 +582,59 @@ prefix_attn_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_co
             // ---- the segment's result: the row itself, or a partial for the merge ----
             const bool own = sg.flags & SEG_OWN, whole = sg.flags & SEG_WHOLE;
             const int head = sg.kh * g.a.group + st - tok * g.a.group;
+            const int cap = g.p.cap[own], half = sg.flags & SEG_HALF ? PA_ROWS : 0;
+            if (few) {  // first the sum over the flow's warps
+                auto meet = [&]() { asm volatile("bar.sync %0, 128;" ::"r"(1 + f) : "memory"); };
+                if (mine) c.few_ml[f][wq][lane] = make_float2(m, l);
+                meet();
+                float M = -INFINITY, L = 0.0f;
+#pragma unroll
+                for (int w = 0; w < 4; w++) M = fmaxf(M, c.few_ml[f][w][lane & 7].x);
+#pragma unroll
+                for (int w = 0; w < 4; w++) {
+                    const float2 ml = c.few_ml[f][w][lane & 7];
+                    if (ml.x != -INFINITY) L += ml.y * ex2(ml.x - M);
+                }
+                const float k = m == -INFINITY ? 0.0f : ex2(m - M) * (whole ? (L > 0.0f ? 1.0f / L : L) : 1.0f);
+                if (mine && wq == 0 && !whole) g.p.ml[own][(int64_t)sg.slot * cap + half + lane] = make_float2(M, L);
+                const int r = row >> 4, e = (row & 15) * 2;  // two dims of a row to write
+                const int st_r = sg.row0 + min(r, sg.n - 1), tok_r = g.a.group_div(st_r);
+#pragma unroll 1
+                for (int i = 0; i < D; i += 32) {
+                    uint32_t v[32];
+                    tmem_ld32(v, t_o + i);
+                    tmem_wait_ld();
+                    if (mine) {
+#pragma unroll
+                        for (int j = 0; j < 32; j += 4)
+                            *reinterpret_cast<float4*>(&c.few_o[f][wq][lane][j]) =
+                                m == -INFINITY ? make_float4(0.0f, 0.0f, 0.0f, 0.0f)
+                                               : make_float4(__uint_as_float(v[j]) * k, __uint_as_float(v[j + 1]) * k,
+                                                             __uint_as_float(v[j + 2]) * k, __uint_as_float(v[j + 3]) * k);
+                    }
+                    meet();
+                    float2 y = make_float2(0.0f, 0.0f);
+                    if (r < sg.n) {
+#pragma unroll
+                        for (int w = 0; w < 4; w++) {
+                            const float2 x = *reinterpret_cast<const float2*>(&c.few_o[f][w][r][e]);
+                            y.x += x.x;
+                            y.y += x.y;
+                        }
+                    }
+                    if (!whole) {
+                        if (r < sg.n)
+                            *reinterpret_cast<float2*>(g.p.o[own] + (((int64_t)sg.slot * (D / 4) + (i + e) / 4) * cap + half + r) * 4 + (e & 2)) = y;
+                    } else {
+                        store2<__nv_bfloat16, D>(g.a, tok_r, sg.kh * g.a.group + st_r - tok_r * g.a.group, i + e, y, r < sg.n);
+                    }
+                    meet();
+                }
+                tc_before();
+                continue;
+            }
             const float inv = l > 0.0f ? 1.0f / l : 0.0f;
-            const int cap = g.p.cap[own], at_o = (sg.flags & SEG_HALF ? PA_ROWS : 0) + row;
+            const int at_o = half + row;
             if (mine && !whole) g.p.ml[own][(int64_t)sg.slot * cap + at_o] = make_float2(m, l);
             // four dims of all rows lie together, so that a warp's stores are 512 bytes each
             float4* po = reinterpret_cast<float4*>(g.p.o[own]) + (int64_t)sg.slot * (D / 4) * cap + at_o;
