@@ -162,7 +162,7 @@ __global__ void __launch_bounds__(256) prefix_attn_merge_kernel(PrefixAttnArgs a
         kh = w.kh;
         own_item = w.item;
     }
-    const Line line(p, *p.own_steps);
+    const Line line(p, *p.own_steps, p.pair_p, p.pair_o);
 #pragma unroll 1
     while (todo > 0) {
         int run = todo, item[2] = {0, own_item}, in[2] = {0, own_in}, v0[2] = {0, 0}, cnt[2] = {0, 0};
@@ -198,7 +198,7 @@ __global__ void __launch_bounds__(256) prefix_attn_merge_kernel(PrefixAttnArgs a
                         if (!has) {  // a worker in between may have no step at all
                             const bool paired = part ? p.pair_o : p.pair_p;
                             int lo, hi;
-                            flow_range(line, p, paired ? v : v >> 1, paired ? 0 : v & 1, part, lo, hi);
+                            flow_range(line, paired, paired ? v : v >> 1, paired ? 0 : v & 1, part, lo, hi);
                             has = lo < hi;
                         }
                         slot[tid] = has ? item[part] + v : -1;

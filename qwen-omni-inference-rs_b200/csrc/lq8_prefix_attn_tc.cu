@@ -30,6 +30,7 @@
 #include "lq8_tma.cuh"
 
 #include <algorithm>
+#include <type_traits>
 
 namespace lq {
 
@@ -40,7 +41,7 @@ constexpr int PA_THREADS = 384;   // warps 0-7 softmax, 8 TMA, 9 MMA, 10 schedul
 // registers: 384 x 168 at launch = 256 x 216 for the softmax warps + 128 x 72 for the others
 constexpr int PA_REGS = 216, PA_REGS_LOW = 72;
 constexpr int PA_SCAN = 512;      // entries of the scan over the sequences
-constexpr int PA_BATCH = 32;      // segments the scheduler works out at a time, a lane each
+constexpr int PA_BATCH = 16;      // segments a flow gets at a time, worked out by a lane each
 constexpr int PA_FEW = 8;         // rows up to which the four warps of a flow share a tile's columns
 constexpr int ERR_PA_WAIT = 94;   // a wait ran out
 
@@ -69,7 +70,7 @@ struct PaCtl {
     PaSeg seg[2][2][PA_BATCH];
     float2 few_ml[2][4][PA_FEW];
     alignas(16) float few_o[2][4][PA_FEW][36];  // 32 dims a row, padded against bank conflicts
-    int4 info[PA_SCAN];     // up to PA_SCAN sequences: q0, q, kv
+    int4 info[PA_SCAN];     // up to PA_SCAN sequences: q0, q, kv, steps of a head
     int scan[PA_SCAN + 1];  // own steps before each entry
 };
 
@@ -196,69 +197,15 @@ __device__ __forceinline__ int per_head_warp(const OwnSteps& o, const SeqInfo& s
     return __reduce_add_sync(0xffffffffu, n);
 }
 
-// A flow's place in its part of the line: the scheduler warp's, the same in every lane.
-struct PaWalk {
-    int step, hi;   // steps of the part: the next one, and the flow's end
-    int b, j;       // sequence (own part), item: kh * n_rb + rb
-    int t;          // tile of the item
-};
-
 __device__ __forceinline__ SeqInfo pa_seq(const PaArgs& g, const PaCtl& c, int b) {
     if (g.s.n_seqs > PA_SCAN) return seq_info(g.a, g.s, b, false);
     const int4 v = c.info[b];
     return SeqInfo{v.x, v.y, v.z};
 }
 
-__device__ __forceinline__ void pa_seek(const PaArgs& g, const PaCtl& c, int per_entry, int n_entries, bool own, int lane,
-                                        PaWalk& w) {
-    if (w.step >= w.hi) return;
-    if (!own) {
-        w.j = w.step / g.p.np;
-        w.t = w.step - w.j * g.p.np;
-        w.b = 0;
-        return;
-    }
-    int e0 = 0, e1 = n_entries;  // the last entry with scan <= step
-#pragma unroll 1
-    while (e1 - e0 > 1) {
-        const int m = (e0 + e1) >> 1;
-        if (c.scan[m] <= w.step) e0 = m;
-        else e1 = m;
-    }
-    const OwnSteps o{g.a, g.p};
-    int rest = w.step - c.scan[e0], per = 1;
-    SeqInfo si{0, 0, 0};
-#pragma unroll 1
-    for (w.b = e0 * per_entry; w.b < g.s.n_seqs; w.b++) {
-        si = pa_seq(g, c, w.b);
-        per = per_head_warp(o, si, lane);
-        if (rest < per * g.a.n_kv) break;
-        rest -= per * g.a.n_kv;
-    }
-    if (w.b >= g.s.n_seqs) {  // lengths that changed under the kernel
-        w.hi = w.step;
-        return;
-    }
-    const int kh = rest / per, n_rb = o.blocks(si);
-    rest -= kh * per;
-    int rb = 0;
-#pragma unroll 1
-    for (; rb < n_rb; rb += 32) {
-        const int n = rb + lane < n_rb ? o.tiles(si, rb + lane) : 0;
-        const int upto = warp_scan(n, lane), all = __shfl_sync(0xffffffffu, upto, 31);
-        if (rest < all) {
-            const int l = __ffs(__ballot_sync(0xffffffffu, upto > rest)) - 1;
-            rest -= __shfl_sync(0xffffffffu, upto - n, l);
-            rb += l;
-            break;
-        }
-        rest -= all;
-    }
-    w.j = kh * n_rb + rb;
-    w.t = rest;
-}
-
-template <int D>
+// PP, PO: blocks of the prefix / of a sequence's own rows are two halves of 128 rows that share
+// their K and V tiles
+template <int D, bool PP, bool PO>
 __global__ void __launch_bounds__(PA_THREADS, 1)
 prefix_attn_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v,
                       const __grid_constant__ PaArgs g) {
@@ -304,15 +251,16 @@ prefix_attn_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_co
     const int per_entry = (g.s.n_seqs + PA_SCAN - 1) / PA_SCAN;
     const int n_entries = per_entry == 1 ? g.s.n_seqs : (g.s.n_seqs + per_entry - 1) / per_entry;
     const OwnSteps os{g.a, g.p};
-    const bool by_warp = per_entry == 1 && g.a.max_q * g.a.group > 4 * g.p.ob;
+    const bool by_warp = PO && per_entry == 1 && g.a.max_q * g.a.group > 4 * g.p.ob;
 #pragma unroll 1
     for (int e = by_warp ? warp : tid; e < n_entries; e += by_warp ? PA_THREADS / 32 : PA_THREADS) {
         int n = 0;
 #pragma unroll 1
         for (int b = e * per_entry; b < min(g.s.n_seqs, (e + 1) * per_entry); b++) {
             const SeqInfo si = seq_info(g.a, g.s, b, blockIdx.x == 0);
-            n += (by_warp ? per_head_warp(os, si, lane) : os.per_head(si)) * g.a.n_kv;
-            if (per_entry == 1) c.info[b] = make_int4(si.q0, si.q, si.kv, 0);
+            const int per = !PO ? (si.q > 0 ? os.tiles(si, 0) : 0) : by_warp ? per_head_warp(os, si, lane) : os.per_head(si);
+            n += per * g.a.n_kv;
+            if (per_entry == 1) c.info[b] = make_int4(si.q0, si.q, si.kv, per);
         }
         c.scan[e + 1] = n;
     }
@@ -839,109 +787,161 @@ prefix_attn_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_co
         asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(PA_REGS_LOW));
         if (warp == 10) {
             // ------------------------------ scheduler ------------------------------
-            const Line line(g.p, so);
+            // Half a warp looks after a flow. In a part whose blocks are paired the two flows walk
+            // the same items, else each has its half of the CTA's steps.
+            const Line line(g.p, so, PP, PO);
+            const int f = lane >> 4, hl = lane & 15;
             unsigned batch[2] = {0, 0};
             bool ok = true;
-            // entries of flow f's next batch: lanes with `valid` give theirs in order
-            auto put = [&](int f, const PaSeg& o, bool valid) {
-                const unsigned k = batch[f], mask = __ballot_sync(0xffffffffu, valid);
-                ok = pa_wait_warp(c, &c.seg_empty[f][k & 1], ((k >> 1) & 1u) ^ 1u);
-                if (!ok) return;
-                if (valid) c.seg[f][k & 1][__popc(mask & ((1u << lane) - 1))] = o;
-                if (lane == 0) c.seg_n[f][k & 1] = __popc(mask);
-                __syncwarp();
-                if (lane == 0) mbar_arrive(&c.seg_full[f][k & 1]);
-                batch[f]++;
+            // the next batch of the flows with `valid` lanes, in the order of the lanes
+            auto put = [&](const PaSeg& o, bool valid) {
+                const unsigned all = __ballot_sync(0xffffffffu, valid);
+#pragma unroll
+                for (int q = 0; q < 2; q++) {
+                    const unsigned m = (all >> (16 * q)) & 0xffffu, k = batch[q];
+                    if (!m || !ok) continue;
+                    ok = pa_wait_warp(c, &c.seg_empty[q][k & 1], ((k >> 1) & 1u) ^ 1u);
+                    if (!ok) return;
+                    if (valid && f == q) c.seg[q][k & 1][__popc(m & ((1u << hl) - 1))] = o;
+                    if (lane == 0) c.seg_n[q][k & 1] = __popc(m);
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive(&c.seg_full[q][k & 1]);
+                    batch[q]++;
+                }
             };
             PaSeg o{0, 1, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0};
-            if (g.a.prefix_len == 0 && lane < (g.p.pair_o ? 1 : 2)) g.p.split[g.p.pair_o ? me : 2 * me + lane].rows = 0;
+            if (g.a.prefix_len == 0 && lane < (PO ? 1 : 2)) g.p.split[PO ? me : 2 * me + lane].rows = 0;
             __syncwarp();
-#pragma unroll 1
-            for (int part = 0; part < 2 && ok; part++) {
-                const bool own = part, paired = own ? g.p.pair_o : g.p.pair_p;
-                PaWalk walk[2];
-                int rounds[2] = {0, 0};
-#pragma unroll 1
-                for (int f = 0; f < 2; f++) {
-                    PaWalk w;
-                    flow_range(line, g.p, me, f, own, w.step, w.hi);
-                    pa_seek(g, c, per_entry, n_entries, own, lane, w);
-                    if (f) walk[1] = w;
-                    else walk[0] = w;
+            auto part = [&](auto own_part) {
+                constexpr bool own = decltype(own_part)::value, paired = own ? PO : PP;
+                const int block = own ? g.p.ob : g.p.pb, worker = paired ? me : 2 * me + f;
+                int step, hi, b = 0, j = 0, t = 0, rounds = 0;  // the flow's place
+                flow_range(line, paired, me, f, own, step, hi);
+                if (step < hi && !own) {
+                    j = step / g.p.np;
+                    t = step - j * g.p.np;
                 }
-                // flows that take their steps apart: the one with fewer rounds gets the next batch
-                while (ok) {
-                    const int f = paired || walk[1].step >= walk[1].hi ||
-                                          (walk[0].step < walk[0].hi && rounds[0] <= rounds[1]) ? 0 : 1;
-                    PaWalk w = f ? walk[1] : walk[0];
-                    if (w.step >= w.hi) break;
-                    // lane i looks at the i-th item from here on
-                    int j = w.j + lane, b = w.b, n_rb = g.p.n_rb, n = 0;
-                    SeqInfo si{0, g.s.rows, 0};
-                    if (own) {
+                if (own && (PO ? __any_sync(0xffffffffu, step < hi) : step < hi)) {
+                    int e0 = 0, e1 = n_entries;  // the last entry with scan <= step
 #pragma unroll 1
-                        for (;;) {
-                            if (b >= g.s.n_seqs) break;
-                            si = pa_seq(g, c, b);
-                            n_rb = os.blocks(si);
-                            if (j < g.a.n_kv * n_rb) break;
-                            j -= g.a.n_kv * n_rb;
-                            b++;
+                    while (e1 - e0 > 1) {
+                        const int m = (e0 + e1) >> 1;
+                        if (c.scan[m] <= step) e0 = m;
+                        else e1 = m;
+                    }
+                    int rest = step - c.scan[e0], per = 1;
+                    SeqInfo si{0, 0, 0};
+#pragma unroll 1
+                    for (b = e0 * per_entry; b < g.s.n_seqs; b++) {
+                        si = pa_seq(g, c, b);
+                        per = per_entry == 1 ? c.info[b].w : PO ? os.per_head(si) : si.q > 0 ? os.tiles(si, 0) : 0;
+                        if (rest < per * g.a.n_kv) break;
+                        rest -= per * g.a.n_kv;
+                    }
+                    if (b >= g.s.n_seqs) hi = step;  // lengths that changed under the kernel
+                    j = rest / max(per, 1);
+                    t = rest - j * per;
+                    if constexpr (PO) {  // (both flows are at the same place: the whole warp looks)
+                        const int n_rb = os.blocks(si);
+                        int rb = 0;
+#pragma unroll 1
+                        for (; rb < n_rb; rb += 32) {
+                            const int n = rb + lane < n_rb ? os.tiles(si, rb + lane) : 0;
+                            const int upto = warp_scan(n, lane), all = __shfl_sync(0xffffffffu, upto, 31);
+                            if (t < all) {
+                                const int l = __ffs(__ballot_sync(0xffffffffu, upto > t)) - 1;
+                                t -= __shfl_sync(0xffffffffu, upto - n, l);
+                                rb += l;
+                                break;
+                            }
+                            t -= all;
+                        }
+                        j = j * n_rb + rb;
+                    }
+                }
+                bool both = true;
+                while (ok && __any_sync(0xffffffffu, step < hi)) {
+                    // flows apart: both get a first batch, then the one with fewer rounds to go on
+                    // with (waiting for the other's could wait for this one)
+                    const int r0 = __shfl_sync(0xffffffffu, step < hi ? rounds : 0x7fffffff, 0);
+                    const int r1 = __shfl_sync(0xffffffffu, step < hi ? rounds : 0x7fffffff, 16);
+                    const bool go = step < hi && (paired || both || f == (r0 <= r1 ? 0 : 1));
+                    both = false;
+                    // a lane looks at the hl-th item from here on
+                    int jj = j + hl, bb = b, n_rb = own ? 1 : g.p.n_rb, nt = g.p.np;
+                    SeqInfo si{0, g.s.rows, 0};
+                    o.kv_end = g.a.prefix_len;
+                    if constexpr (own) {
+                        nt = o.kv_end = 0;
+#pragma unroll 1
+                        for (; bb < g.s.n_seqs; bb++) {
+                            si = pa_seq(g, c, bb);
+                            n_rb = PO ? os.blocks(si) : si.q > 0;
+                            if (jj < g.a.n_kv * n_rb) break;
+                            jj -= g.a.n_kv * n_rb;
                         }
                     }
-                    const int kh = n_rb == 1 ? j : j / max(n_rb, 1), rb = j - kh * n_rb;
-                    o.kv_end = g.a.prefix_len;
-                    int nt = g.p.np;
-                    if (own) {
-                        o.kv_end = b < g.s.n_seqs ? os.visible(si, rb) : 0;
+                    int kh = jj, rb = 0;
+                    if ((own ? PO : true) && n_rb > 1) {
+                        kh = jj / n_rb;
+                        rb = jj - kh * n_rb;
+                    }
+                    if (own && bb < g.s.n_seqs) {
+                        o.kv_end = os.visible(si, rb);
                         nt = (o.kv_end + PA_TILE - 1) / PA_TILE;
                     }
-                    o.t0 = lane == 0 ? w.t : 0;
-                    const int upto = warp_scan(nt - o.t0, lane), start = w.step + upto - (nt - o.t0);
-                    n = min(nt - o.t0, w.hi - start);
-                    o.t1 = o.t0 + n;
-                    const int block = own ? g.p.ob : g.p.pb, worker = paired ? me : 2 * me + f;
+                    o.t0 = hl == 0 ? t : 0;
+                    int upto = nt - o.t0;  // steps up to here in the batch
+#pragma unroll
+                    for (int k = 1; k < 16; k <<= 1) {
+                        const int u = __shfl_up_sync(0xffffffffu, upto, k, 16);
+                        if (hl >= k) upto += u;
+                    }
+                    const int n = min(nt - o.t0, hi - (step + upto - (nt - o.t0)));
                     const int rows = si.q * g.a.group - rb * block;  // of the whole block
-                    o.n = min(PA_ROWS, rows);
+                    const int item = (own ? g.a.n_kv * os.base(si, bb) : 0) + jj;
+                    o.t1 = o.t0 + n;
                     o.n1 = paired ? max(0, min(PA_ROWS, rows - PA_ROWS)) : 0;
-                    o.flags = (own ? SEG_OWN : 0) | (paired ? SEG_PAIRED : 0) |
-                              (g.a.prefix_len == 0 && o.t0 == 0 && o.t1 == nt ? SEG_WHOLE : 0);
+                    o.n = paired && f ? o.n1 : min(PA_ROWS, rows);
+                    o.flags = (own ? SEG_OWN : 0) | (paired ? SEG_PAIRED : 0) | (paired && f ? SEG_HALF : 0) |
+                              (own && g.a.prefix_len == 0 && o.t0 == 0 && o.t1 == nt ? SEG_WHOLE : 0);
                     o.kh = kh;
-                    o.b = b;
-                    o.row0 = (own ? si.q0 * g.a.group : 0) + rb * block;
+                    o.b = bb;
+                    const int first_row = (own ? si.q0 * g.a.group : 0) + rb * block;
+                    o.row0 = first_row + (paired && f ? PA_ROWS : 0);
                     o.voff = own ? si.kv - si.q + 1 - si.q0 : 0;
-                    const int item = (own ? g.a.n_kv * os.base(si, b) : 0) + j;
                     o.slot = item + worker;
-                    if (n > 0) {  // for the merge
+                    const bool valid = go && n > 0;
+                    if (valid && !(paired && f)) {  // for the merge
                         if (o.t0 == 0) g.p.first[own][item] = worker;
                         if (o.t1 == nt) g.p.last[own][item] = worker;
                         if (own && g.a.prefix_len == 0 && o.t0 == 0 && o.t1 < nt)
-                            g.p.split[worker] = SplitItem{min(rows, block), o.row0, kh, item};
+                            g.p.split[worker] = SplitItem{min(rows, block), first_row, kh, item};
                     }
-                    if (__any_sync(0xffffffffu, n > 0)) put(f, o, n > 0);
-                    if (paired && ok && __any_sync(0xffffffffu, n > 0)) {  // the other half of the block
-                        o.n = o.n1;
-                        o.row0 += PA_ROWS;
-                        o.flags |= SEG_HALF;
-                        put(1, o, n > 0);
+                    put(o, valid);
+                    const int all = min(__shfl_sync(0xffffffffu, upto, 15, 16), hi - step);
+                    jj = __shfl_sync(0xffffffffu, jj, 15, 16) + 1;
+                    bb = __shfl_sync(0xffffffffu, bb, 15, 16);
+                    if (go) {
+                        rounds += all;
+                        step += all;
+                        j = jj;
+                        b = bb;
+                        t = 0;
+                        if (own && b >= g.s.n_seqs) hi = step;  // (no more sequences)
                     }
-                    const int all = min(__shfl_sync(0xffffffffu, upto, 31), w.hi - w.step);
-                    rounds[f] += all;
-                    w.step += all;
-                    w.j = __shfl_sync(0xffffffffu, j, 31) + 1;
-                    w.b = __shfl_sync(0xffffffffu, b, 31);
-                    w.t = 0;
-                    if (own && w.b >= g.s.n_seqs) w.hi = w.step;  // (no more sequences)
-                    if (f) walk[1] = w;
-                    else walk[0] = w;
                 }
                 // both flows take the same number of rounds
-                o = PaSeg{0, 1, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0};
-                if (!paired && rounds[1] < rounds[0] && ok) put(1, o, lane == 0);
-            }
+                if (!paired) {
+                    const bool odd = __shfl_sync(0xffffffffu, rounds, 16) < __shfl_sync(0xffffffffu, rounds, 0);
+                    o = PaSeg{0, 1, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0};
+                    if (odd && ok) put(o, lane == 16);
+                }
+            };
+            if (line.sp > 0) part(std::false_type{});
+            if (ok) part(std::true_type{});
             o.flags = SEG_END;
-#pragma unroll 1
-            for (int f = 0; f < 2 && ok; f++) put(f, o, lane == 0);
+            if (ok) put(o, hl == 0);
         } else if (g.a.prefix_len == 0) {
             // warp 11: rows before their sequence's first position see nothing when there is no
             // prefix either
@@ -959,7 +959,7 @@ prefix_attn_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_co
     if (warp == 9) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, 512;" ::"r"(tmem));
 }
 
-template <int D>
+template <int D, bool PP, bool PO>
 static int launch_tc(lq_ctx* ctx, const PaArgs& g) {
     const int page = 1 << g.s.page_shift;
     const uint64_t dims[4] = {(uint64_t)D, (uint64_t)page, (uint64_t)g.a.n_kv, (uint64_t)g.s.n_pages};
@@ -971,15 +971,17 @@ static int launch_tc(lq_ctx* ctx, const PaArgs& g) {
     rc = make_tensor_map_4d(ctx, &mv, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, g.a.v, dims, strides, box, CU_TENSOR_MAP_SWIZZLE_128B);
     if (rc) return rc;
     const size_t smem = 1024 + 2 * PA_ROWS * D * 2 + PA_STAGES * PA_TILE * D * 2 + sizeof(PaCtl);
-    rc = ensure_func_smem(ctx, (const void*)prefix_attn_tc_kernel<D>, smem);
+    rc = ensure_func_smem(ctx, (const void*)prefix_attn_tc_kernel<D, PP, PO>, smem);
     if (rc) return rc;
-    return launch_kernel(ctx, prefix_attn_tc_kernel<D>, dim3((unsigned)g.p.workers), dim3(PA_THREADS), smem,
+    return launch_kernel(ctx, prefix_attn_tc_kernel<D, PP, PO>, dim3((unsigned)g.p.workers), dim3(PA_THREADS), smem,
                          "prefix_attn_tc", mk, mv, g);
 }
 
 int launch_prefix_attn_tc(lq_ctx* ctx, const PrefixAttnArgs& a, const PagedSeqs& s, const PrefixPlan& p, int D) {
     const PaArgs g{a, s, p};
-    return D == 64 ? launch_tc<64>(ctx, g) : launch_tc<128>(ctx, g);
+    // PO implies PP: one sequence's rows are some of all rows. Without a prefix PP says nothing.
+    if (D == 64) return p.pair_o ? launch_tc<64, true, true>(ctx, g) : p.pair_p ? launch_tc<64, true, false>(ctx, g) : launch_tc<64, false, false>(ctx, g);
+    return p.pair_o ? launch_tc<128, true, true>(ctx, g) : p.pair_p ? launch_tc<128, true, false>(ctx, g) : launch_tc<128, false, false>(ctx, g);
 }
 
 }  // namespace lq

@@ -117,8 +117,8 @@ struct Line {
     bool pair_p, pair_o;
     int quot, rem;     // W / n
     uint64_t mul;      // ceil(2^40 / n): x / n = x mul / 2^40, exact for x < 2^32
-    __device__ __forceinline__ Line(const PrefixPlan& p, int own_steps)
-        : sp(p.sp), so(own_steps), n(p.workers), pair_p(p.pair_p), pair_o(p.pair_o), mul(p.workers_mul) {
+    __device__ __forceinline__ Line(const PrefixPlan& p, int own_steps, bool pair_prefix, bool pair_own)
+        : sp(p.sp), so(own_steps), n(p.workers), pair_p(pair_prefix), pair_o(pair_own), mul(p.workers_mul) {
         split = sp * (pair_p ? 3 : 2);
         w = split + so * (pair_o ? 3 : 2);
         quot = (int)(((uint64_t)w * mul) >> 40);
@@ -130,21 +130,14 @@ struct Line {
         const int x = own ? max(start(c) - split, 0) : start(c);
         return min((own ? pair_o : pair_p) ? (x + 2) / 3 : (x + 1) / 2, own ? so : sp);
     }
-    __device__ __forceinline__ int owner(int step, bool own) const {
-        const int at = (own ? split : 0) + step * ((own ? pair_o : pair_p) ? 3 : 2);
-        int c = min(n - 1, (int)(((float)at + 1.0f) * (float)n / (float)w));  // a guess, then the step's place
-        while (c > 0 && start(c) > at) c--;
-        while (c + 1 < n && start(c + 1) <= at) c++;
-        return c;
-    }
 };
 
-// [lo, hi) of worker c's flow f: both halves of a paired block run the same steps, otherwise the
+// [lo, hi) of CTA c's flow f: both halves of a paired block run the same steps, otherwise the
 // flows take one half of the steps each
-__device__ __forceinline__ void flow_range(const Line& l, const PrefixPlan& p, int c, int f, bool own, int& lo, int& hi) {
+__device__ __forceinline__ void flow_range(const Line& l, bool paired, int c, int f, bool own, int& lo, int& hi) {
     lo = l.first(c, own);
     hi = l.first(c + 1, own);
-    if (!(own ? p.pair_o : p.pair_p)) {
+    if (!paired) {
         const int mid = lo + (hi - lo + 1) / 2;
         if (f == 0) hi = mid;
         else lo = mid;
