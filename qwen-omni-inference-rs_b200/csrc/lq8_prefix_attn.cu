@@ -10,99 +10,6 @@
 
 namespace lq {
 
-// own positions that row r sees, in its sequence b; flags lengths the call's bounds do not hold
-__device__ __forceinline__ int visible_own(const PrefixAttnArgs& a, const PagedSeqs& s, int b, int r) {
-    const int q0 = s.q_start ? s.q_start[b] : b, q1 = s.q_start ? s.q_start[b + 1] : b + 1;
-    int kv = s.kv_len[b];
-    const int64_t most = min((int64_t)a.max_kv, s.table_ld << s.page_shift);
-    if (kv < 0 || kv > most) {
-        flag_error(a.err, ERR_KV_LEN, kv);
-        kv = kv < 0 ? 0 : (int)most;
-    }
-    if (q1 - q0 > a.max_q || q1 > s.rows) flag_error(a.err, ERR_ROW_COUNT, q1 - q0);
-    return min(kv, max(0, kv - (q1 - r) + 1));
-}
-
-template <typename T>
-__device__ __forceinline__ float elem(const void* p, int64_t i);
-template <>
-__device__ __forceinline__ float elem<float>(const void* p, int64_t i) { return static_cast<const float*>(p)[i]; }
-template <>
-__device__ __forceinline__ float elem<__nv_bfloat16>(const void* p, int64_t i) {
-    return __bfloat162float(static_cast<const __nv_bfloat16*>(p)[i]);
-}
-
-// One CTA of 128 threads per (row, query head): 128 positions at a time, a thread a score, then a
-// thread a dim, with the running maximum and sum.
-template <typename T, int D>
-__global__ void __launch_bounds__(128) prefix_attn_row_kernel(PrefixAttnArgs a, PagedSeqs s) {
-    __shared__ float q[D], p[128], red[4];
-    __shared__ int64_t base[128];
-    pdl_trigger();
-    pdl_wait();
-    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-    const int row = blockIdx.x, h = blockIdx.y, kh = h / (a.n_heads / a.n_kv);
-    int b = row;
-    if (s.q_start) b = seq_of_row(s.q_start, s.n_seqs, row, lane);
-    if (b >= s.n_seqs) return;
-    const int own = visible_own(a, s, b, row), total = a.prefix_len + own;
-    if (tid < D) q[tid] = elem<T>(a.q, (int64_t)row * a.q_stride + (int64_t)h * D + tid) * a.scale;
-    float m = -INFINITY, l = 0.0f, o = 0.0f;
-    const int mask = (1 << s.page_shift) - 1;
-    for (int t0 = 0; t0 < total; t0 += 128) {
-        __syncthreads();
-        const int t = t0 + tid;
-        float sc = -INFINITY;
-        int64_t at = -1;
-        if (t < total) {
-            const int u = t < a.prefix_len ? t : t - a.prefix_len;
-            const int pg = t < a.prefix_len ? a.prefix_table[u >> s.page_shift]
-                                            : s.table[(int64_t)b * s.table_ld + (u >> s.page_shift)];
-            if (pg < 0 || pg >= s.n_pages) {
-                flag_error(a.err, ERR_PAGE_ID, pg);
-            } else {
-                at = pg * a.page_stride + (((int64_t)kh << s.page_shift) + (u & mask)) * D;
-                sc = 0.0f;
-                for (int d = 0; d < D; d++) sc = fmaf(q[d], elem<T>(a.k, at + d), sc);
-            }
-        }
-        base[tid] = at;
-        float mx = warp_max(sc);
-        if (lane == 0) red[warp] = mx;
-        __syncthreads();
-        const float m_new = fmaxf(fmaxf(fmaxf(red[0], red[1]), fmaxf(red[2], red[3])), m);
-        const float ref = m_new == -INFINITY ? 0.0f : m_new;
-        const float e = expf(sc - ref), f = expf(m - ref);
-        p[tid] = e;
-        const float sum = warp_sum(e);
-        __syncthreads();
-        if (lane == 0) red[warp] = sum;
-        __syncthreads();
-        l = l * f + (red[0] + red[1] + red[2] + red[3]);
-        m = m_new;
-        if (tid < D) {
-            o *= f;
-            for (int i = 0; i < 128; i++)
-                if (base[i] >= 0) o = fmaf(p[i], elem<T>(a.v, base[i] + tid), o);
-        }
-    }
-    const float y = l > 0.0f ? o / l : 0.0f;
-    if (tid < D && a.out) {
-        const int64_t at = (int64_t)row * a.out_stride + (int64_t)h * D + tid;
-        if constexpr (sizeof(T) == 4) static_cast<float*>(a.out)[at] = y;
-        else static_cast<__nv_bfloat16*>(a.out)[at] = __float2bfloat16_rn(y);
-    }
-    if (a.xq) {
-        float amax = warp_max(fabsf(y)), d, id;
-        q8_scale(amax, d, id);
-        const int64_t blk = ((int64_t)row * a.n_heads + h) * (D / 32) + warp;
-        if (warp < D / 32) {
-            if (lane == 0) a.xd[blk] = f2h(d);
-            a.xq[blk * 32 + lane] = (int8_t)q8_quant(y, id);
-        }
-    }
-}
-
 // =========================================================================================
 // Merge: joins the partials of the workers that had a piece of a row's prefix item or own item, in
 // the order of the line: with M the largest of their maxima, o = sum 2^(m_i - M) o_i /
@@ -290,15 +197,18 @@ __global__ void __launch_bounds__(256) prefix_attn_merge_kernel(PrefixAttnArgs a
     }
 }
 
-// The plan of a call for workers of `halves` x `half` stacked rows and `tile` positions, and its
-// workspace. Sizes come from the call's bounds; what the lengths really are, the kernels read.
-static int make_plan(lq_ctx* ctx, const PrefixAttnArgs& a, const PagedSeqs& s, int half, int tile, int D, PrefixPlan* p) {
+// The plan of a call and its workspace. Sizes come from the call's bounds; what the lengths really
+// are, the kernels read.
+static int make_plan(lq_ctx* ctx, const PrefixAttnArgs& a, const PagedSeqs& s, bool f32, int D, PrefixPlan* p) {
     const int64_t R = (int64_t)s.rows * a.group, most_q = std::min<int64_t>((int64_t)a.max_q, s.rows) * a.group;
+    // bf16: blocks of 128 rows, or two halves of 128 that share their K and V tiles; a worker is a
+    // CTA with paired halves, else one of its two flows. f32: blocks of 8 rows, a worker is a warp.
+    const int half = f32 ? 8 : 128, tile = f32 ? 32 : 128;
     p->tile = tile;
-    p->pair_p = R > half;
-    p->pb = p->pair_p ? 2 * half : half;
-    p->pair_o = most_q > half;
-    p->ob = p->pair_o ? 2 * half : half;
+    p->pair_p = f32 || R > half;
+    p->pair_o = f32 || most_q > half;
+    p->pb = f32 ? half : p->pair_p ? 2 * half : half;
+    p->ob = f32 ? half : p->pair_o ? 2 * half : half;
     p->cap[0] = (int)std::min<int64_t>(p->pb, R);
     p->cap[1] = (int)std::min<int64_t>(p->ob, most_q);
     p->n_rb = ceil_div(R, p->pb);
@@ -307,7 +217,7 @@ static int make_plan(lq_ctx* ctx, const PrefixAttnArgs& a, const PagedSeqs& s, i
     const int64_t steps = items_p * p->np + items_o * ceil_div(a.max_kv, tile);
     LQ_REQUIRE(ctx, steps < (1ll << 26), "lq_prefix_attention: %lld steps, more than a launch can number", (long long)steps);
     p->sp = (int)(items_p * p->np);
-    p->workers = (int)std::max<int64_t>(1, std::min<int64_t>(ctx->sm_count, steps));
+    p->workers = (int)std::max<int64_t>(1, std::min<int64_t>(ctx->sm_count * (f32 ? PREFIX_ATTN_F32_WARPS : 1), steps));
     p->workers_mul = ((1ull << 40) + p->workers - 1) / p->workers;
     const int64_t items[2] = {p->np ? items_p : 0, items_o};
     size_t at = 0;
@@ -411,14 +321,12 @@ extern "C" int lq_prefix_attention(lq_ctx* ctx, const void* q, lq_dtype dtype, i
     a.xq = xq;
     a.xd = xd;
     a.err = ctx->err_flag;
-    if (dtype == LQ_DTYPE_BF16) {
-        lq::PrefixPlan p;
-        if ((rc = lq::make_plan(ctx, a, s, 128, 128, (int)head_dim, &p))) return rc;
-        if ((rc = lq::launch_prefix_attn_tc(ctx, a, s, p, (int)head_dim))) return rc;
-        return head_dim == 64 ? lq::launch_merge<__nv_bfloat16, 64>(ctx, a, s, p)
-                              : lq::launch_merge<__nv_bfloat16, 128>(ctx, a, s, p);
-    }
-    const dim3 grid((unsigned)rows, (unsigned)n_heads);
-    auto run = [&](auto kern) { return lq::launch_kernel(ctx, kern, grid, dim3(128), 0, "prefix_attn_row", a, s); };
-    return head_dim == 64 ? run(lq::prefix_attn_row_kernel<float, 64>) : run(lq::prefix_attn_row_kernel<float, 128>);
+    lq::PrefixPlan p;
+    const bool f32 = dtype == LQ_DTYPE_F32;
+    const int D = (int)head_dim;
+    if ((rc = lq::make_plan(ctx, a, s, f32, D, &p))) return rc;
+    rc = f32 ? lq::launch_prefix_attn_f32(ctx, a, s, p, D) : lq::launch_prefix_attn_tc(ctx, a, s, p, D);
+    if (rc) return rc;
+    if (f32) return D == 64 ? lq::launch_merge<float, 64>(ctx, a, s, p) : lq::launch_merge<float, 128>(ctx, a, s, p);
+    return D == 64 ? lq::launch_merge<__nv_bfloat16, 64>(ctx, a, s, p) : lq::launch_merge<__nv_bfloat16, 128>(ctx, a, s, p);
 }

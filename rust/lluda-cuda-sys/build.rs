@@ -13,7 +13,7 @@ use std::process::Command;
 const SOURCES: &[&str] = &[
     "lq8_runtime.cu", "lq8_q8.cu", "lq8_gemv.cu", "lq8_gemm_tc.cu", "lq8_gemm_f16.cu", "lq8_attn_prefill.cu", "lq8_moe.cu",
     "lq8_comm.cu", "lq8_ops.cu", "lq8_attention.cu", "lq8_decode.cu", "lq8_sample.cu", "lq8_paged.cu",
-    "lq8_prefix_attn.cu", "lq8_prefix_attn_tc.cu", "lq8_qwen3.cu",
+    "lq8_prefix_attn.cu", "lq8_prefix_attn_tc.cu", "lq8_prefix_attn_f32.cu", "lq8_qwen3.cu",
 ];
 
 fn main() {
