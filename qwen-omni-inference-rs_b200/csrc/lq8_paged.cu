@@ -20,6 +20,70 @@ __device__ __forceinline__ float to_f32(__nv_bfloat16 v) { return __bfloat162flo
 __device__ __forceinline__ void from_f32(float& d, float v) { d = v; }
 __device__ __forceinline__ void from_f32(__nv_bfloat16& d, float v) { d = __float2bfloat16_rn(v); }
 
+// V consecutive values as f32, in vectors of 16 bytes (V elements aligned so)
+template <int V>
+__device__ __forceinline__ void load_v(const float* p, float v[V]) {
+#pragma unroll
+    for (int i = 0; i < V; i += 4) {
+        const float4 t = *reinterpret_cast<const float4*>(p + i);
+        v[i] = t.x, v[i + 1] = t.y, v[i + 2] = t.z, v[i + 3] = t.w;
+    }
+}
+template <int V>
+__device__ __forceinline__ void load_v(const __nv_bfloat16* p, float v[V]) {
+    const Vec<__nv_bfloat16, V> t = *reinterpret_cast<const Vec<__nv_bfloat16, V>*>(p);
+#pragma unroll
+    for (int i = 0; i < V; i++) v[i] = to_f32(t.e[i]);
+}
+template <int V>
+__device__ __forceinline__ void store_v(float* p, const float v[V]) {
+#pragma unroll
+    for (int i = 0; i < V; i += 4) *reinterpret_cast<float4*>(p + i) = make_float4(v[i], v[i + 1], v[i + 2], v[i + 3]);
+}
+template <int V>
+__device__ __forceinline__ void store_v(__nv_bfloat16* p, const float v[V]) {
+    Vec<__nv_bfloat16, V> t;
+#pragma unroll
+    for (int i = 0; i < V; i++) t.e[i] = __float2bfloat16_rn(v[i]);
+    *reinterpret_cast<Vec<__nv_bfloat16, V>*>(p) = t;
+}
+
+// cos and sin of pairs i0 .. i0 + V - 1 of a row (`at`: its position when the call gives none);
+// false, and the error flag, when a position lies outside the tables
+template <int V>
+__device__ __forceinline__ bool angles(const RopeAxes& rope, int64_t row, int64_t at, int i0, float cs[V], float sn[V], int* err) {
+    if (V >= 4 && ((V == 8 ? rope.same8 : rope.same4) >> (i0 / V) & 1)) {
+        const int64_t p = rope.pos ? (int64_t)rope.pos[(int64_t)rope.axis[i0] * rope.pos_stride + row] : at;
+        if (p < 0 || p >= rope.table_len) {
+            flag_error(err, ERR_ROPE_POS, (int)p);
+            return false;
+        }
+        if constexpr (V >= 4) {
+            load_v<V>(rope.cos + p * rope.pairs + i0, cs);
+            load_v<V>(rope.sin + p * rope.pairs + i0, sn);
+        }
+        return true;
+    }
+    bool ok = true;
+    int64_t p[V];
+#pragma unroll
+    for (int e = 0; e < V; e++) {
+        p[e] = rope.pos ? (int64_t)rope.pos[(int64_t)rope.axis[i0 + e] * rope.pos_stride + row] : at;
+        if (p[e] < 0 || p[e] >= rope.table_len) {
+            flag_error(err, ERR_ROPE_POS, (int)p[e]);
+            p[e] = 0;
+            ok = false;
+        }
+    }
+#pragma unroll
+    for (int e = 0; e < V; e++) {
+        const int64_t o = p[e] * rope.pairs + i0 + e;
+        cs[e] = rope.cos[o];
+        sn[e] = rope.sin[o];
+    }
+    return ok;
+}
+
 // =========================================================================================
 // Rotary positions with several axes: y_i = x_i cos - x_{i+n} sin, y_{i+n} = x_{i+n} cos +
 // x_i sin for the n pairs of a head, the dims past 2n copied. A thread owns V pairs (16 bytes of
@@ -42,7 +106,7 @@ struct MropeArgs {
 };
 
 template <typename T, int V>
-__global__ void __launch_bounds__(256) mrope_kernel(MropeArgs a, RopeAxes rope) {
+__global__ void __launch_bounds__(256, 3) mrope_kernel(MropeArgs a, RopeAxes rope) {
     pdl_trigger();
     pdl_wait();
     const T* x = static_cast<const T*>(a.x);
@@ -75,17 +139,9 @@ __global__ void __launch_bounds__(256) mrope_kernel(MropeArgs a, RopeAxes rope) 
                 hi[j] = *reinterpret_cast<const Vec<T, V>*>(xr + j * a.x_head + rope.pairs + i0);
             }
         float cs[V], sn[V];
-        bool ok = true;
+        const bool ok = angles<V>(rope, row, 0, i0, cs, sn, a.err);
 #pragma unroll
-        for (int e = 0; e < V; e++) {
-            const int p = rope.pos[(int64_t)rope.axis[i0 + e] * rope.pos_stride + row];
-            const bool in = p >= 0 && p < rope.table_len;
-            if (!in) flag_error(a.err, ERR_ROPE_POS, p);
-            ok &= in;
-            const int64_t o = (int64_t)(in ? p : 0) * rope.pairs + i0 + e;
-            cs[e] = rope.cos[o];
-            sn[e] = rope.sin[o] * a.sign;
-        }
+        for (int e = 0; e < V; e++) sn[e] *= a.sign;
         if (!ok) continue;
 #pragma unroll
         for (int j = 0; j < MROPE_HEADS; j++)
@@ -116,8 +172,9 @@ static int launch_mrope(lq_ctx* ctx, MropeArgs a, const RopeAxes& rope) {
 // =========================================================================================
 // Append to the paged cache: from projection rows [q heads | k heads | v heads], per-head
 // RMSNorm of q and k (when weights are given), rotation, q to q_out, k and v to their slots.
-// A warp owns HPW heads of one row; for head dimensions of 64, 128 and 256 that rotate whole
-// (E = head_dim / 64 pairs a lane) both members of a rotary pair sit in one lane.
+// A warp owns some heads of one row; for head dimensions of 64, 128 and 256 that rotate whole a lane
+// holds 8 rotary pairs of a head (both members: 16-byte vectors of either half), D / 16 lanes a
+// head, so that a warp works on 4 heads of 128 dims at a time and has IT times as many in flight.
 // =========================================================================================
 struct AppendArgs {
     const void* qkv;
@@ -170,107 +227,103 @@ __device__ __forceinline__ RowSlot find_slot(const PagedSeqs& s, int r, int lane
     return o;
 }
 
-template <typename T, int E>
-__device__ __forceinline__ void load_e(const T* p, float v[E]) {
-    const Vec<T, E> t = *reinterpret_cast<const Vec<T, E>*>(p);
-#pragma unroll
-    for (int e = 0; e < E; e++) v[e] = to_f32(t.e[e]);
-}
-template <typename T, int E>
-__device__ __forceinline__ void store_e(T* p, const float v[E]) {
-    Vec<T, E> t;
-#pragma unroll
-    for (int e = 0; e < E; e++) from_f32(t.e[e], v[e]);
-    *reinterpret_cast<Vec<T, E>*>(p) = t;
-}
-
-template <typename S, typename T, int E, int HPW>
+template <typename S, typename T, int D, int IT>
 __global__ void __launch_bounds__(256) paged_append_kernel(AppendArgs a, RopeAxes rope, PagedSeqs seqs, int groups) {
-    constexpr int D = 64 * E, N = 32 * E;
+    constexpr int LPH = D / 16, HPW = 32 / LPH, N = D / 2;  // lanes a head, heads side by side
     pdl_trigger();
     pdl_wait();
     const int lane = threadIdx.x & 31;
     const int64_t item = (int64_t)blockIdx.x * (blockDim.x >> 5) + (threadIdx.x >> 5);
     const int row = (int)(item / groups);
-    const int h0 = (int)(item - (int64_t)row * groups) * HPW;
+    const int h0 = (int)(item - (int64_t)row * groups) * (HPW * IT);  // the warp's first head
     if (row >= seqs.rows) return;
-    const int heads = a.n_heads + 2 * a.n_kv, d0 = E * lane;
-    const S* src = static_cast<const S*>(a.qkv) + (int64_t)row * a.row_stride + (int64_t)h0 * D + d0;
-    float lo[HPW][E], hi[HPW][E];
+    const int heads = a.n_heads + 2 * a.n_kv, d0 = 8 * (lane % LPH), mine = h0 + lane / LPH;
+    const S* src = static_cast<const S*>(a.qkv) + (int64_t)row * a.row_stride + (int64_t)mine * D + d0;
+    Vec<S, 16 / sizeof(S)> raw[IT][2][sizeof(S) / 2];
 #pragma unroll
-    for (int j = 0; j < HPW; j++)
-        if (h0 + j < heads) {
-            load_e<S, E>(src + j * D, lo[j]);
-            load_e<S, E>(src + j * D + N, hi[j]);
+    for (int j = 0; j < IT; j++)
+        if (mine + j * HPW < heads) {
+#pragma unroll
+            for (int k = 0; k < (int)sizeof(S) / 2; k++) {
+                raw[j][0][k] = *reinterpret_cast<const Vec<S, 16 / sizeof(S)>*>(src + j * HPW * D + k * (16 / sizeof(S)));
+                raw[j][1][k] = *reinterpret_cast<const Vec<S, 16 / sizeof(S)>*>(src + j * HPW * D + N + k * (16 / sizeof(S)));
+            }
         }
     const RowSlot slot = find_slot(seqs, row, lane, a.err);
     if (!slot.live) return;
-    float cs[E], sn[E];
+    float cs[8], sn[8];
     bool turn = true;
-    if (h0 < a.n_heads + a.n_kv) {
-#pragma unroll
-        for (int e = 0; e < E; e++) {
-            const int64_t p = rope.pos ? (int64_t)rope.pos[(int64_t)rope.axis[d0 + e] * rope.pos_stride + row]
-                                       : rope.pos_base + slot.own;
-            const bool in = p >= 0 && p < rope.table_len;
-            if (!in) flag_error(a.err, ERR_ROPE_POS, (int)p);
-            turn &= in;
-            const int64_t o = (in ? p : 0) * rope.pairs + d0 + e;
-            cs[e] = rope.cos[o];
-            sn[e] = rope.sin[o];
-        }
-        turn = __all_sync(0xffffffffu, turn);
-    }
+    if (h0 < a.n_heads + a.n_kv)
+        turn = __all_sync(0xffffffffu, angles<8>(rope, row, rope.pos_base + slot.own, d0, cs, sn, a.err));
     T* const page_k = static_cast<T*>(a.k) + slot.page * a.page_stride;
     T* const page_v = static_cast<T*>(a.v) + slot.page * a.page_stride;
 #pragma unroll
-    for (int j = 0; j < HPW; j++) {
-        const int h = h0 + j;
-        if (h >= heads) break;
-        T* dst;
-        if (h < a.n_heads) {
-            dst = static_cast<T*>(a.q_out) + (int64_t)row * a.q_stride + (int64_t)h * D;
+    for (int j = 0; j < IT; j++) {
+        if (h0 + j * HPW >= heads) break;
+        const int h = mine + j * HPW;
+        const bool is_q = h < a.n_heads, is_v = h >= a.n_heads + a.n_kv, on = h < heads && (is_q || slot.ok) && (is_v || turn);
+        float lo[8], hi[8];
+        if (h < heads) {
+#pragma unroll
+            for (int e = 0; e < 8; e++) {
+                lo[e] = to_f32(raw[j][0][e / (16 / sizeof(S))].e[e % (16 / sizeof(S))]);
+                hi[e] = to_f32(raw[j][1][e / (16 / sizeof(S))].e[e % (16 / sizeof(S))]);
+            }
         } else {
-            if (!slot.ok) continue;
-            const int kh = h < a.n_heads + a.n_kv ? h - a.n_heads : h - a.n_heads - a.n_kv;
-            dst = (h < a.n_heads + a.n_kv ? page_k : page_v) + (((int64_t)kh << seqs.page_shift) + slot.off) * D;
+#pragma unroll
+            for (int e = 0; e < 8; e++) lo[e] = hi[e] = 0.0f;
         }
-        if (h < a.n_heads + a.n_kv) {
-            if (!turn) continue;
-            const uint16_t* nw = h < a.n_heads ? a.q_norm : a.k_norm;
+        const uint16_t* const nw = is_q ? a.q_norm : is_v ? nullptr : a.k_norm;
+        if (a.q_norm || a.k_norm) {  // (the shuffles by every lane, weights or none)
+            if (nw && a.norm_bf16) {
+#pragma unroll
+                for (int e = 0; e < 8; e++) lo[e] = round_bf16(lo[e]), hi[e] = round_bf16(hi[e]);
+            }
+            // the sum of squares in the order of lq_qk_norm_rope_kv, where a lane has dims 2 v,
+            // 2 v + 1 and theirs of the upper half and a butterfly joins the lanes from bit 4 down:
+            // here v = 4 (lane % LPH) + k, so bits 4 to 2 are lanes and bits 1 and 0 are k
+            float t[4];
+#pragma unroll
+            for (int k = 0; k < 4; k++)
+                t[k] = __fadd_rn(__fadd_rn(__fmul_rn(lo[2 * k], lo[2 * k]), __fmul_rn(lo[2 * k + 1], lo[2 * k + 1])),
+                                 __fadd_rn(__fmul_rn(hi[2 * k], hi[2 * k]), __fmul_rn(hi[2 * k + 1], hi[2 * k + 1])));
+#pragma unroll
+            for (int d = LPH / 2; d > 0; d >>= 1)
+#pragma unroll
+                for (int k = 0; k < 4; k++) t[k] = __fadd_rn(t[k], __shfl_xor_sync(0xffffffffu, t[k], d));
+            const float ss = __fadd_rn(__fadd_rn(t[0], t[2]), __fadd_rn(t[1], t[3]));
             if (nw) {
-                if (a.norm_bf16) {
+                const float inv = __frcp_rn(__fsqrt_rn(__fadd_rn(__fmul_rn(ss, 1.0f / D), a.eps)));  // (1 / D is exact)
+                float w0[8], w1[8];
+                load_v<8>(reinterpret_cast<const __nv_bfloat16*>(nw) + d0, w0);
+                load_v<8>(reinterpret_cast<const __nv_bfloat16*>(nw) + N + d0, w1);
 #pragma unroll
-                    for (int e = 0; e < E; e++) lo[j][e] = round_bf16(lo[j][e]), hi[j][e] = round_bf16(hi[j][e]);
+                for (int e = 0; e < 8; e++) {
+                    lo[e] = __fmul_rn(__fmul_rn(lo[e], inv), w0[e]);
+                    hi[e] = __fmul_rn(__fmul_rn(hi[e], inv), w1[e]);
+                    if (a.norm_bf16) lo[e] = round_bf16(lo[e]), hi[e] = round_bf16(hi[e]);
                 }
-                // the sum of squares in lq_qk_norm_rope_kv's order: a lane's dims, then a butterfly
-                float ss = 0.0f, sh = 0.0f;
-#pragma unroll
-                for (int e = 0; e < E; e++) {
-                    ss = __fadd_rn(ss, __fmul_rn(lo[j][e], lo[j][e]));
-                    sh = __fadd_rn(sh, __fmul_rn(hi[j][e], hi[j][e]));
-                }
-                ss = warp_sum(__fadd_rn(ss, sh));
-                const float inv = __fdiv_rn(1.0f, __fsqrt_rn(__fadd_rn(__fdiv_rn(ss, (float)D), a.eps)));
-                float w0[E], w1[E];
-                load_e<__nv_bfloat16, E>(reinterpret_cast<const __nv_bfloat16*>(nw) + d0, w0);
-                load_e<__nv_bfloat16, E>(reinterpret_cast<const __nv_bfloat16*>(nw) + N + d0, w1);
-#pragma unroll
-                for (int e = 0; e < E; e++) {
-                    lo[j][e] = __fmul_rn(__fmul_rn(lo[j][e], inv), w0[e]);
-                    hi[j][e] = __fmul_rn(__fmul_rn(hi[j][e], inv), w1[e]);
-                    if (a.norm_bf16) lo[j][e] = round_bf16(lo[j][e]), hi[j][e] = round_bf16(hi[j][e]);
-                }
-            }
-#pragma unroll
-            for (int e = 0; e < E; e++) {
-                const float p = lo[j][e], q = hi[j][e];
-                lo[j][e] = __fsub_rn(__fmul_rn(p, cs[e]), __fmul_rn(q, sn[e]));
-                hi[j][e] = __fadd_rn(__fmul_rn(q, cs[e]), __fmul_rn(p, sn[e]));
             }
         }
-        store_e<T, E>(dst + d0, lo[j]);
-        store_e<T, E>(dst + d0 + N, hi[j]);
+        if (!is_v && turn) {
+#pragma unroll
+            for (int e = 0; e < 8; e++) {
+                const float p = lo[e], q = hi[e];
+                lo[e] = __fsub_rn(__fmul_rn(p, cs[e]), __fmul_rn(q, sn[e]));
+                hi[e] = __fadd_rn(__fmul_rn(q, cs[e]), __fmul_rn(p, sn[e]));
+            }
+        }
+        if (on) {
+            T* dst;
+            if (is_q) {
+                dst = static_cast<T*>(a.q_out) + (int64_t)row * a.q_stride + (int64_t)h * D;
+            } else {
+                const int kh = h - a.n_heads - (is_v ? a.n_kv : 0);
+                dst = (is_v ? page_v : page_k) + (((int64_t)kh << seqs.page_shift) + slot.off) * D;
+            }
+            store_v<8>(dst + d0, lo);
+            store_v<8>(dst + d0 + N, hi);
+        }
     }
 }
 
@@ -342,31 +395,30 @@ __global__ void __launch_bounds__(256) paged_append_any_kernel(AppendArgs a, Rop
     for (int e = 2 * rope.pairs + lane; e < D; e += 32) from_f32(dst[e], value(e));
 }
 
-template <typename S, typename T, int E>
-static int launch_append_e(lq_ctx* ctx, const AppendArgs& a, const RopeAxes& rope, const PagedSeqs& s) {
-    const int heads = a.n_heads + 2 * a.n_kv;
-    // few (row, head) items: a warp each, so that a decode step's handful of rows spreads over
-    // the SMs; many: four heads a warp, whose loads are in flight together and share the row's
-    // angles and slot
-    const bool few = (int64_t)s.rows * heads < 64ll * ctx->sm_count;
-    const int groups = few ? heads : ceil_div(heads, 4);
+template <typename S, typename T, int D>
+static int launch_append_d(lq_ctx* ctx, const AppendArgs& a, const RopeAxes& rope, const PagedSeqs& s) {
+    const int heads = a.n_heads + 2 * a.n_kv, side = 512 / D;  // heads side by side in a warp
+    // many rows: four heads a lane in flight (two of f32), which share the row's slot and angles;
+    // a decode step's few rows: one, so that they spread over the SMs
+    constexpr int IT = sizeof(S) == 2 ? 4 : 2;
+    const bool few = (int64_t)s.rows * ceil_div(heads, side) < 16ll * ctx->sm_count;
+    const int groups = ceil_div(heads, few ? side : side * IT);
     const dim3 grid((unsigned)ceil_div((int64_t)s.rows * groups, 8));
-    if (few) return launch_kernel(ctx, paged_append_kernel<S, T, E, 1>, grid, dim3(256), 0, "paged_append", a, rope, s, groups);
-    return launch_kernel(ctx, paged_append_kernel<S, T, E, 4>, grid, dim3(256), 0, "paged_append", a, rope, s, groups);
+    if (few) return launch_kernel(ctx, paged_append_kernel<S, T, D, 1>, grid, dim3(256), 0, "paged_append", a, rope, s, groups);
+    return launch_kernel(ctx, paged_append_kernel<S, T, D, IT>, grid, dim3(256), 0, "paged_append", a, rope, s, groups);
 }
 
 template <typename S, typename T>
 static int launch_append(lq_ctx* ctx, const AppendArgs& a, const RopeAxes& rope, const PagedSeqs& s) {
-    // the lane-local layout needs whole rotation and vector-aligned rows, weights and pages
-    const int D = a.head_dim, E = D / 64;
-    auto al = [](const void* p, size_t bytes) { return (uintptr_t)p % bytes == 0; };
-    const bool whole = rope.pairs * 2 == D && (D == 64 || D == 128 || D == 256) &&
-                       a.row_stride % E == 0 && a.q_stride % E == 0 && a.page_stride % E == 0 &&
-                       al(a.qkv, E * sizeof(S)) && al(a.q_out, E * sizeof(T)) && al(a.k, E * sizeof(T)) &&
-                       al(a.v, E * sizeof(T)) && al(a.q_norm, E * 2) && al(a.k_norm, E * 2);
-    if (whole && E == 1) return launch_append_e<S, T, 1>(ctx, a, rope, s);
-    if (whole && E == 2) return launch_append_e<S, T, 2>(ctx, a, rope, s);
-    if (whole && E == 4) return launch_append_e<S, T, 4>(ctx, a, rope, s);
+    // the lane-local layout needs whole rotation and 16-byte aligned rows, weights and pages
+    const int D = a.head_dim;
+    auto al = [](const void* p) { return (uintptr_t)p % 16 == 0; };
+    const bool whole = rope.pairs * 2 == D && a.row_stride * sizeof(S) % 16 == 0 && a.q_stride * sizeof(T) % 16 == 0 &&
+                       a.page_stride * sizeof(T) % 16 == 0 && al(a.qkv) && al(a.q_out) && al(a.k) && al(a.v) &&
+                       al(a.q_norm) && al(a.k_norm);
+    if (whole && D == 64) return launch_append_d<S, T, 64>(ctx, a, rope, s);
+    if (whole && D == 128) return launch_append_d<S, T, 128>(ctx, a, rope, s);
+    if (whole && D == 256) return launch_append_d<S, T, 256>(ctx, a, rope, s);
     const int64_t items = (int64_t)s.rows * (a.n_heads + 2 * a.n_kv);
     return launch_kernel(ctx, paged_append_any_kernel<S, T>, dim3((unsigned)ceil_div(items, 8)), dim3(256), 0,
                          "paged_append_any", a, rope, s);
@@ -397,6 +449,15 @@ int make_rope_axes(lq_ctx* ctx, const char* who, RopeAxes* r, int64_t rot_dim, i
                        (long long)n_axes);
             r->axis[i] = axis_host[i];
         }
+    // runs of pairs on one axis whose table entries are 16-byte aligned vectors
+    r->same4 = r->same8 = 0;
+    if (r->pairs % 4 == 0 && (uintptr_t)cos_dev % 16 == 0 && (uintptr_t)sin_dev % 16 == 0)
+        for (int w = 4; w <= 8; w *= 2)
+            for (int c = 0; (c + 1) * w <= r->pairs; c++) {
+                bool same = true;
+                for (int i = 1; i < w; i++) same = same && r->axis[c * w + i] == r->axis[c * w];
+                if (same) (w == 4 ? r->same4 : r->same8) |= 1u << c;
+            }
     return LQ_OK;
 }
 

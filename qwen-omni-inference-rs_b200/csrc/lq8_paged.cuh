@@ -30,6 +30,7 @@ struct RopeAxes {
     int64_t pos_stride;
     int64_t pos_base;
     int table_len, pairs;
+    uint32_t same4, same8;  // bit c: pairs 4 c .. 4 c + 3 (8 c .. 8 c + 7) share an axis and load as vectors
     uint8_t axis[ROPE_MAX_PAIRS];
 };
 
