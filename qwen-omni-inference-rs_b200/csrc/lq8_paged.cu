@@ -65,19 +65,13 @@ __device__ __forceinline__ bool angles(const RopeAxes& rope, int64_t row, int64_
         return true;
     }
     bool ok = true;
-    int64_t p[V];
 #pragma unroll
     for (int e = 0; e < V; e++) {
-        p[e] = rope.pos ? (int64_t)rope.pos[(int64_t)rope.axis[i0 + e] * rope.pos_stride + row] : at;
-        if (p[e] < 0 || p[e] >= rope.table_len) {
-            flag_error(err, ERR_ROPE_POS, (int)p[e]);
-            p[e] = 0;
-            ok = false;
-        }
-    }
-#pragma unroll
-    for (int e = 0; e < V; e++) {
-        const int64_t o = p[e] * rope.pairs + i0 + e;
+        const int64_t p = rope.pos ? (int64_t)rope.pos[(int64_t)rope.axis[i0 + e] * rope.pos_stride + row] : at;
+        const bool in = p >= 0 && p < rope.table_len;
+        if (!in) flag_error(err, ERR_ROPE_POS, (int)p);
+        ok &= in;
+        const int64_t o = (in ? p : 0) * rope.pairs + i0 + e;
         cs[e] = rope.cos[o];
         sn[e] = rope.sin[o];
     }
@@ -87,11 +81,11 @@ __device__ __forceinline__ bool angles(const RopeAxes& rope, int64_t row, int64_
 // =========================================================================================
 // Rotary positions with several axes: y_i = x_i cos - x_{i+n} sin, y_{i+n} = x_{i+n} cos +
 // x_i sin for the n pairs of a head, the dims past 2n copied. A thread owns V pairs (16 bytes of
-// x_i and of x_{i+n}) of MROPE_HEADS heads of one row: the angles are gathered once for the
-// heads, and eight 16-byte loads are in flight before the first use.
+// x_i and of x_{i+n}) of H heads of one row: the angles are gathered once for the heads, and 2 H
+// 16-byte loads are in flight before the first use. A CTA takes whole rows, so that DRAM sees runs
+// of all their heads (a thread that walks over all heads of a row instead, with the CTA spread over
+// 32 rows: 180 against 123 us for 32768 rows of 40 heads).
 // =========================================================================================
-constexpr int MROPE_HEADS = 4;
-
 struct MropeArgs {
     const void* x;
     void* y;
@@ -99,14 +93,14 @@ struct MropeArgs {
     int64_t rows;
     int heads, head_dim;
     int chunks;      // V-wide chunks of a head: pairs / V rotated ones, then the copied dims
-    int units;       // chunks * ceil(heads / MROPE_HEADS)
+    int units;       // chunks * ceil(heads / H)
     int rows_per_cta;
     float sign;      // -1: the inverse rotation
     int* err;
 };
 
-template <typename T, int V>
-__global__ void __launch_bounds__(256, 3) mrope_kernel(MropeArgs a, RopeAxes rope) {
+template <typename T, int V, int H>
+__global__ void __launch_bounds__(256, 2) mrope_kernel(MropeArgs a, RopeAxes rope) {
     pdl_trigger();
     pdl_wait();
     const T* x = static_cast<const T*>(a.x);
@@ -117,23 +111,23 @@ __global__ void __launch_bounds__(256, 3) mrope_kernel(MropeArgs a, RopeAxes rop
         const int64_t row = (int64_t)blockIdx.x * a.rows_per_cta + sub;
         if (row >= a.rows) break;
         const int hg = w / a.chunks, c = w - hg * a.chunks;
-        const int h0 = hg * MROPE_HEADS;
+        const int h0 = hg * H;
         const T* xr = x + row * a.x_row + (int64_t)h0 * a.x_head;
         T* yr = y + row * a.y_row + (int64_t)h0 * a.y_head;
         if (c >= turned) {  // dims past the rotated ones
             if (x == y) continue;
             const int e = 2 * rope.pairs + (c - turned) * V;
 #pragma unroll
-            for (int j = 0; j < MROPE_HEADS; j++)
+            for (int j = 0; j < H; j++)
                 if (h0 + j < a.heads)
                     *reinterpret_cast<Vec<T, V>*>(yr + j * a.y_head + e) =
                         *reinterpret_cast<const Vec<T, V>*>(xr + j * a.x_head + e);
             continue;
         }
         const int i0 = c * V;
-        Vec<T, V> lo[MROPE_HEADS], hi[MROPE_HEADS];
+        Vec<T, V> lo[H], hi[H];
 #pragma unroll
-        for (int j = 0; j < MROPE_HEADS; j++)
+        for (int j = 0; j < H; j++)
             if (h0 + j < a.heads) {
                 lo[j] = *reinterpret_cast<const Vec<T, V>*>(xr + j * a.x_head + i0);
                 hi[j] = *reinterpret_cast<const Vec<T, V>*>(xr + j * a.x_head + rope.pairs + i0);
@@ -144,7 +138,7 @@ __global__ void __launch_bounds__(256, 3) mrope_kernel(MropeArgs a, RopeAxes rop
         for (int e = 0; e < V; e++) sn[e] *= a.sign;
         if (!ok) continue;
 #pragma unroll
-        for (int j = 0; j < MROPE_HEADS; j++)
+        for (int j = 0; j < H; j++)
             if (h0 + j < a.heads) {
                 Vec<T, V> o0, o1;
 #pragma unroll
@@ -159,14 +153,24 @@ __global__ void __launch_bounds__(256, 3) mrope_kernel(MropeArgs a, RopeAxes rop
     }
 }
 
-template <typename T, int V>
-static int launch_mrope(lq_ctx* ctx, MropeArgs a, const RopeAxes& rope) {
+template <typename T, int V, int H>
+static int launch_mrope_h(lq_ctx* ctx, MropeArgs a, const RopeAxes& rope) {
     a.chunks = rope.pairs / V + (a.head_dim - 2 * rope.pairs) / V;
-    a.units = a.chunks * ceil_div(a.heads, MROPE_HEADS);
+    a.units = a.chunks * ceil_div(a.heads, H);
     a.rows_per_cta = std::max(1, 256 / a.units);
     const int threads = std::min(256, (a.units * a.rows_per_cta + 31) / 32 * 32);
-    return launch_kernel(ctx, mrope_kernel<T, V>, dim3((unsigned)ceil_div(a.rows, a.rows_per_cta)), dim3(threads), 0,
+    return launch_kernel(ctx, mrope_kernel<T, V, H>, dim3((unsigned)ceil_div(a.rows, a.rows_per_cta)), dim3(threads), 0,
                          "mrope", a, rope);
+}
+
+template <typename T, int V>
+static int launch_mrope(lq_ctx* ctx, const MropeArgs& a, const RopeAxes& rope) {
+    // five heads a thread when that leaves no more threads without one than four do (32768 rows of
+    // 40 heads, bf16: 123 us with five, 135 with four; six and eight spill, 180 and 218)
+    [[maybe_unused]] const bool five = ceil_div(a.heads, 5) * 5 <= ceil_div(a.heads, 4) * 4;
+    if constexpr (V > 1)
+        if (five) return launch_mrope_h<T, V, 5>(ctx, a, rope);
+    return launch_mrope_h<T, V, 4>(ctx, a, rope);
 }
 
 // =========================================================================================

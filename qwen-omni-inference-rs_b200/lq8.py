@@ -340,13 +340,19 @@ def matmul_q8(ctx: Context, w: QTensor, xq, xd, residual=None, out=None):
     return y
 
 
+# Checks below run on every decode step, next to kernels of a few microseconds: they are plain
+# comparisons, and messages are put together only when one fails.
+_PAGED_DTYPES: dict = {}
+
+
 def _paged_dtype(t, what: str) -> int:
-    import torch
-    if t.dtype == torch.float32:
-        return DTYPE_F32
-    if t.dtype == torch.bfloat16:
-        return DTYPE_BF16
-    raise ValueError(f"{what}: {t.dtype} is neither float32 nor bfloat16")
+    if not _PAGED_DTYPES:
+        import torch
+        _PAGED_DTYPES.update({torch.float32: DTYPE_F32, torch.bfloat16: DTYPE_BF16})
+    dt = _PAGED_DTYPES.get(t.dtype)
+    if dt is None:
+        raise ValueError(f"{what}: {t.dtype} is neither float32 nor bfloat16")
+    return dt
 
 
 def _need(cond: bool, msg: str) -> None:
@@ -374,7 +380,9 @@ class Rotary:
         self.axis = None if axis is None else np.ascontiguousarray(axis, dtype=np.uint8)
         _need(self.axis is None or self.axis.shape == (self.pairs,), "Rotary: one axis a pair")
         self.n_axes = 1 if self.axis is None or not self.pairs else int(self.axis.max()) + 1
-        self._axis_ptr = None if self.axis is None else self.axis.ctypes.data
+        self._args = (2 * self.pairs, cos.data_ptr(), sin.data_ptr(), self.table_len,
+                      None if self.axis is None else self.axis.ctypes.data, self.n_axes)
+        self._int32 = torch.int32
 
     @staticmethod
     def blocks(sections) -> np.ndarray:
@@ -408,33 +416,32 @@ class Rotary:
 
     def _pos(self, pos, rows: int):
         """Checked (pointer, stride) of positions [n_axes, rows] (or [rows] for one axis)."""
-        _need_i32(pos, "pos", pos.dim())
-        if pos.dim() == 1:
-            _need(self.n_axes == 1 and pos.shape[0] == rows, f"pos: [{self.n_axes}, {rows}] expected")
-            return pos.data_ptr(), rows
-        _need(pos.dim() == 2 and pos.shape[0] >= self.n_axes and pos.shape[1] == rows,
-              f"pos: [{self.n_axes}, {rows}] expected, got {list(pos.shape)}")
-        return pos.data_ptr(), pos.stride(0) if pos.shape[0] > 1 else rows
+        shape, stride = pos.shape, pos.stride()
+        if (pos.dtype != self._int32 or not pos.is_cuda or len(shape) not in (1, 2) or shape[-1] != rows or
+                (rows > 1 and stride[-1] != 1) or (shape[0] if len(shape) == 2 else 1) < self.n_axes):
+            raise ValueError(f"pos: int32 CUDA tensor [{self.n_axes}, {rows}] expected, got {pos.dtype} {list(shape)}")
+        return pos.data_ptr(), stride[0] if len(shape) == 2 and shape[0] > 1 else rows
 
 
 def mrope(ctx: Context, x, rotary: Rotary, pos, out=None, inverse: bool = False):
     """Rotary positions with several axes: x [rows, heads, head_dim] f32 or bf16 (any row and head
     stride, the dims contiguous), pos int32 [n_axes, rows]. out may be x. Returns out."""
-    import torch
     dt = _paged_dtype(x, "mrope")
-    _need(x.dim() == 3 and x.is_cuda and (x.shape[2] <= 1 or x.stride(2) == 1),
-          "mrope: x is a CUDA tensor [rows, heads, head_dim] with contiguous dims")
     if out is None:
+        import torch
         out = torch.empty(x.shape, dtype=x.dtype, device=x.device)
-    _need(out.shape == x.shape and out.dtype == x.dtype and out.is_cuda and (x.shape[2] <= 1 or out.stride(2) == 1),
-          "mrope: out has x's shape and type")
-    rows, heads, D = x.shape
+    shape, xs, ys = x.shape, x.stride(), out.stride()
+    if len(shape) != 3 or not x.is_cuda or (shape[2] > 1 and xs[2] != 1):
+        raise ValueError("mrope: x is a CUDA tensor [rows, heads, head_dim] with contiguous dims")
+    if out.shape != shape or out.dtype != x.dtype or not out.is_cuda or (shape[2] > 1 and ys[2] != 1):
+        raise ValueError("mrope: out has x's shape and type")
+    rows, heads, D = shape
     if rows == 0:
         return out
-    p, ps = rotary._pos(pos, rows)
-    ctx.call("lq_mrope", x.data_ptr(), dt, rows, heads, D, x.stride(0), x.stride(1), out.data_ptr(), out.stride(0),
-             out.stride(1), 2 * rotary.pairs, rotary.cos.data_ptr(), rotary.sin.data_ptr(), rotary.table_len,
-             rotary._axis_ptr, rotary.n_axes, p, ps, int(inverse))
+    rc = ctx.lib.lq_mrope(ctx.h, x.data_ptr(), dt, rows, heads, D, xs[0], xs[1], out.data_ptr(), ys[0], ys[1],
+                          *rotary._args, *rotary._pos(pos, rows), 1 if inverse else 0)
+    if rc:
+        ctx.check(rc)
     return out
 
 
@@ -462,6 +469,7 @@ class PagedBatch:
         self.max_q, self.max_kv, self.prefix_len = max_q, max_kv, prefix_len
         self.ld = page_table.shape[1]
         self._seqs = (self.n_seqs, _ptr(q_start), kv_len.data_ptr(), page_table.data_ptr(), self.ld)
+        self._prefix_ptr = _ptr(prefix_table)
 
 
 class PagedKvCache:
@@ -479,7 +487,9 @@ class PagedKvCache:
               "PagedKvCache: pages are dense inside and apart, K and V pages equally far")
         self.ctx, self.k, self.v = ctx, k, v
         self._pages = (k.data_ptr(), v.data_ptr())
-        self._stride = k.stride(0) if self.n_pages > 1 else self.n_kv_heads * inner[0]
+        self._layout = (self.n_pages, self.page_size, k.stride(0) if self.n_pages > 1 else self.n_kv_heads * inner[0])
+        import torch
+        self._norm_types = (torch.bfloat16, torch.int16)
 
     @classmethod
     def empty(cls, ctx: Context, n_pages: int, page_size: int, n_kv_heads: int, head_dim: int, dtype):
@@ -488,38 +498,46 @@ class PagedKvCache:
         return cls(ctx, torch.empty(shape, dtype=dtype, device="cuda"), torch.empty(shape, dtype=dtype, device="cuda"))
 
     @staticmethod
-    def _dense_rows(t) -> bool:
-        """CUDA [rows, heads, dim] whose rows are dense inside and do not overlap."""
-        return t.is_cuda and t.stride(2) == 1 and (t.shape[1] <= 1 or t.stride(1) == t.shape[2]) and (
-            t.shape[0] <= 1 or t.stride(0) >= t.shape[1] * t.shape[2])
+    def _row_stride(t, shape, dtype, what: str) -> int:
+        """Row stride of a CUDA tensor of `shape` [rows, heads, dim] whose rows are dense inside and
+        do not overlap (0: one row)."""
+        st = t.stride()
+        rows, heads, dim = shape
+        if (tuple(t.shape) != shape or t.dtype != dtype or not t.is_cuda or st[2] != 1 or (heads > 1 and st[1] != dim) or
+                (rows > 1 and st[0] < heads * dim)):
+            raise ValueError(f"{what}: CUDA tensor {list(shape)} in the cache's type, rows dense inside, expected; "
+                             f"got {t.dtype} {list(t.shape)} with strides {list(st)}")
+        return st[0] if rows > 1 else 0
 
     def append(self, qkv, n_heads: int, batch: PagedBatch, rotary: Rotary, pos=None, q_norm=None, k_norm=None,
                eps: float = 1e-6, norm_bf16: bool = False, q_out=None):
         """qkv [rows, (n_heads + 2 n_kv_heads) * head_dim] f32 or bf16: normalises (bf16 weights)
         and rotates q and k, appends k and v, returns q [rows, n_heads, head_dim] in the cache's
         type. pos None: the prefix length + the own position."""
-        import torch
         dt = _paged_dtype(qkv, "append")
-        rows, D = qkv.shape[0], self.head_dim
-        width = (n_heads + 2 * self.n_kv_heads) * D
-        _need(qkv.dim() == 2 and qkv.is_cuda and qkv.shape[1] == width and qkv.stride(1) == 1 and
-              (rows <= 1 or qkv.stride(0) >= width), f"append: rows of {width} contiguous values expected")
+        D, st = self.head_dim, qkv.stride()
+        rows, width = qkv.shape[0], (n_heads + 2 * self.n_kv_heads) * D
+        if len(st) != 2 or qkv.shape[1] != width or not qkv.is_cuda or st[1] != 1 or (rows > 1 and st[0] < width):
+            raise ValueError(f"append: rows of {width} contiguous values expected")
         for w in (q_norm, k_norm):
-            _need(w is None or (w.dtype in (torch.bfloat16, torch.int16) and w.shape == (D,) and w.is_cuda and
-                                w.is_contiguous()), "append: norm weights are bf16 [head_dim]")
+            if w is not None and (w.dtype not in self._norm_types or w.shape != (D,) or not w.is_cuda or w.stride(0) != 1):
+                raise ValueError("append: norm weights are bf16 [head_dim]")
         if q_out is None:
-            q_out = torch.empty((rows, n_heads, D), dtype=self.k.dtype, device=qkv.device)
-        _need(q_out.shape == (rows, n_heads, D) and q_out.dtype == self.k.dtype and self._dense_rows(q_out),
-              "append: q_out [rows, n_heads, head_dim] in the cache's type, rows dense inside")
+            q_out = qkv.new_empty((rows, n_heads, D), dtype=self.k.dtype)
+        q_stride = self._row_stride(q_out, (rows, n_heads, D), self.k.dtype, "append: q_out")
         if rows == 0:
             return q_out
-        _need(pos is not None or rotary.n_axes == 1, "append: several axes need positions")
+        if pos is None and rotary.n_axes != 1:
+            raise ValueError("append: several axes need positions")
         p, ps = (None, 0) if pos is None else rotary._pos(pos, rows)
-        self.ctx.call("lq_paged_append", qkv.data_ptr(), dt, qkv.stride(0) if rows > 1 else 0, rows, n_heads,
-                      self.n_kv_heads, D, _ptr(q_norm), _ptr(k_norm), eps, int(norm_bf16), 2 * rotary.pairs,
-                      rotary.cos.data_ptr(), rotary.sin.data_ptr(), rotary.table_len, rotary._axis_ptr, rotary.n_axes,
-                      p, ps, batch.prefix_len, *batch._seqs, *self._pages, self.dtype, self.n_pages, self.page_size,
-                      self._stride, q_out.data_ptr(), q_out.stride(0) if rows > 1 else 0)
+        ctx = self.ctx
+        rc = ctx.lib.lq_paged_append(
+            ctx.h, qkv.data_ptr(), dt, st[0] if rows > 1 else 0, rows, n_heads, self.n_kv_heads, D,
+            None if q_norm is None else q_norm.data_ptr(), None if k_norm is None else k_norm.data_ptr(), eps,
+            1 if norm_bf16 else 0, *rotary._args, p, ps, batch.prefix_len, *batch._seqs, *self._pages, self.dtype,
+            *self._layout, q_out.data_ptr(), q_stride)
+        if rc:
+            ctx.check(rc)
         return q_out
 
     def attend(self, q, batch: PagedBatch, scale: float | None = None, out=None, quantized=None):
@@ -527,27 +545,32 @@ class PagedKvCache:
         positions up to itself; scale None: 1/sqrt(head_dim). Returns out (q's shape). quantized:
         (int8 [rows, n_heads * head_dim], int16 [rows, n_heads * head_dim / 32]) also gets the
         rows in Q8_0."""
-        import torch
-        D = self.head_dim
-        _need(q.dim() == 3 and q.dtype == self.k.dtype and q.shape[2] == D and self._dense_rows(q),
-              "attend: q [rows, n_heads, head_dim] in the cache's type, rows dense inside")
-        rows, heads = q.shape[0], q.shape[1]
+        D, shape = self.head_dim, tuple(q.shape)
+        if len(shape) != 3 or shape[2] != D:
+            raise ValueError(f"attend: q [rows, n_heads, {D}] in the cache's type expected")
+        q_stride = self._row_stride(q, shape, self.k.dtype, "attend: q")
         if out is None:
-            out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
-        _need(out.shape == q.shape and out.dtype == q.dtype and self._dense_rows(out),
-              "attend: out has q's shape and type, rows dense inside")
-        xq, xd = (None, None) if quantized is None else quantized
-        if xq is not None:
+            out = q.new_empty(shape)
+        out_stride = self._row_stride(out, shape, self.k.dtype, "attend: out")
+        rows, heads = shape[0], shape[1]
+        xq = xd = None
+        if quantized is not None:
+            import torch
+            xq, xd = quantized
             _need(xq.dtype == torch.int8 and xd.dtype == torch.int16 and xq.is_contiguous() and xd.is_contiguous() and
                   xq.shape == (rows, heads * D) and xd.shape == (rows, heads * D // 32),
                   "attend: quantized is (int8 [rows, heads * dim], int16 [rows, heads * dim / 32])")
+            xq, xd = xq.data_ptr(), xd.data_ptr()
         if rows == 0:
             return out
-        max_kv = batch.ld * self.page_size if batch.max_kv is None else batch.max_kv
-        self.ctx.call("lq_prefix_attention", q.data_ptr(), self.dtype, q.stride(0) if rows > 1 else 0, rows, heads,
-                      self.n_kv_heads, D, D ** -0.5 if scale is None else scale, *self._pages, self.n_pages,
-                      self.page_size, self._stride, _ptr(batch.prefix_table), batch.prefix_len, *batch._seqs,
-                      batch.max_q, max_kv, out.data_ptr(), out.stride(0) if rows > 1 else 0, _ptr(xq), _ptr(xd))
+        ctx = self.ctx
+        rc = ctx.lib.lq_prefix_attention(
+            ctx.h, q.data_ptr(), self.dtype, q_stride, rows, heads, self.n_kv_heads, D,
+            D ** -0.5 if scale is None else scale, *self._pages, *self._layout, batch._prefix_ptr, batch.prefix_len,
+            *batch._seqs, batch.max_q, batch.ld * self.page_size if batch.max_kv is None else batch.max_kv,
+            out.data_ptr(), out_stride, xq, xd)
+        if rc:
+            ctx.check(rc)
         return out
 
 
