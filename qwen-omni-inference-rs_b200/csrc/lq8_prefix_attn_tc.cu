@@ -193,7 +193,7 @@ __device__ __forceinline__ int per_head_warp(const OwnSteps& o, const SeqInfo& s
     const int n_rb = o.blocks(si);
     int n = 0;
 #pragma unroll 1
-    for (int rb = lane; rb < n_rb; rb += 32) n += o.tiles(si, rb);
+    for (int rb = lane; rb < n_rb; rb += 32) n += o.steps(si, rb);
     return __reduce_add_sync(0xffffffffu, n);
 }
 
@@ -846,7 +846,7 @@ prefix_attn_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_co
                         int rb = 0;
 #pragma unroll 1
                         for (; rb < n_rb; rb += 32) {
-                            const int n = rb + lane < n_rb ? os.tiles(si, rb + lane) : 0;
+                            const int n = rb + lane < n_rb ? os.steps(si, rb + lane) : 0;
                             const int upto = warp_scan(n, lane), all = __shfl_sync(0xffffffffu, upto, 31);
                             if (t < all) {
                                 const int l = __ffs(__ballot_sync(0xffffffffu, upto > t)) - 1;
@@ -890,17 +890,19 @@ prefix_attn_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_co
                         o.kv_end = os.visible(si, rb);
                         nt = (o.kv_end + PA_TILE - 1) / PA_TILE;
                     }
-                    o.t0 = hl == 0 ? t : 0;
-                    int upto = nt - o.t0;  // steps up to here in the batch
+                    const int ns = nt + (own && PO && nt > 0 ? g.p.extra : 0);  // steps of the item
+                    const int from = hl == 0 ? t : 0;
+                    int upto = ns - from;  // steps up to here in the batch
 #pragma unroll
                     for (int k = 1; k < 16; k <<= 1) {
                         const int u = __shfl_up_sync(0xffffffffu, upto, k, 16);
                         if (hl >= k) upto += u;
                     }
-                    const int n = min(nt - o.t0, hi - (step + upto - (nt - o.t0)));
+                    o.t0 = min(from, nt);
+                    o.t1 = min(nt, from + min(ns - from, hi - (step + upto - (ns - from))));
+                    const int n = o.t1 - o.t0;
                     const int rows = si.q * g.a.group - rb * block;  // of the whole block
                     const int item = (own ? g.a.n_kv * os.base(si, bb) : 0) + jj;
-                    o.t1 = o.t0 + n;
                     o.n1 = paired ? max(0, min(PA_ROWS, rows - PA_ROWS)) : 0;
                     o.n = paired && f ? o.n1 : min(PA_ROWS, rows);
                     o.flags = (own ? SEG_OWN : 0) | (paired ? SEG_PAIRED : 0) | (paired && f ? SEG_HALF : 0) |

@@ -47,6 +47,7 @@ struct PrefixPlan {
     int n_rb;                   // row blocks of the prefix, per kv head
     int np;                     // tiles of the prefix
     int sp;                     // steps of the prefix
+    int extra;                  // steps that an own item counts for beside its tiles
     int workers;                // CTAs that share the line
     uint64_t workers_mul;       // ceil(2^40 / workers)
     int cap[2];                 // rows a partial slot holds (prefix, own)
@@ -97,10 +98,16 @@ struct OwnSteps {
     __device__ __forceinline__ int tiles(const SeqInfo& i, int rb) const {
         return (visible(i, rb) + p.tile - 1) / p.tile;
     }
+    // what the block counts for on the line: its tiles, and p.extra for the segment's beginning and
+    // end (after the tiles; a worker whose share has nothing else of the block leaves it alone)
+    __device__ __forceinline__ int steps(const SeqInfo& i, int rb) const {
+        const int n = tiles(i, rb);
+        return n > 0 ? n + p.extra : 0;
+    }
     __device__ __forceinline__ int per_head(const SeqInfo& i) const {
         int n = 0;
 #pragma unroll 1
-        for (int rb = blocks(i) - 1; rb >= 0; rb--) n += tiles(i, rb);
+        for (int rb = blocks(i) - 1; rb >= 0; rb--) n += steps(i, rb);
         return n;
     }
     // numbers a sequence's row blocks from here on; blocks(i) <= base(next) - base(i), so that no
