@@ -217,9 +217,10 @@ static int make_plan(lq_ctx* ctx, const PrefixAttnArgs& a, const PagedSeqs& s, b
     const int64_t steps = items_p * p->np + items_o * (ceil_div(a.max_kv, tile) + 1);
     LQ_REQUIRE(ctx, steps < (1ll << 26), "lq_prefix_attention: %lld steps, more than a launch can number", (long long)steps);
     p->sp = (int)(items_p * p->np);
-    // a segment of paired blocks costs about one more step (Q, the masked tiles, the store): short
-    // causal items next to a long prefix took the last CTAs of a 10-prompt batch from 105 to 152 us
-    p->extra = !f32 && p->pair_o ? 1 : 0;
+    // a segment costs about one more step than its tiles (Q, the masked tile, the store): counted
+    // so, short causal items next to a long prefix no longer hold up the last CTAs (a batch of 10
+    // prompt chunks: 152 -> 114 us)
+    p->extra = f32 ? 0 : 1;
     p->workers = (int)std::max<int64_t>(1, std::min<int64_t>(ctx->sm_count * (f32 ? PREFIX_ATTN_F32_WARPS : 1), steps));
     p->workers_mul = ((1ull << 40) + p->workers - 1) / p->workers;
     const int64_t items[2] = {p->np ? items_p : 0, items_o};

@@ -258,7 +258,7 @@ prefix_attn_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_co
 #pragma unroll 1
         for (int b = e * per_entry; b < min(g.s.n_seqs, (e + 1) * per_entry); b++) {
             const SeqInfo si = seq_info(g.a, g.s, b, blockIdx.x == 0);
-            const int per = !PO ? (si.q > 0 ? os.tiles(si, 0) : 0) : by_warp ? per_head_warp(os, si, lane) : os.per_head(si);
+            const int per = !PO ? (si.q > 0 ? os.steps(si, 0) : 0) : by_warp ? per_head_warp(os, si, lane) : os.per_head(si);
             n += per * g.a.n_kv;
             if (per_entry == 1) c.info[b] = make_int4(si.q0, si.q, si.kv, per);
         }
@@ -388,7 +388,7 @@ prefix_attn_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_co
                         mt *= cs;
                         if (t == sg.t0) {
                             m = mt;
-                        } else if (__any_sync(0xffffffffu, mt > m + 8.0f)) {
+                        } else if (__any_sync(0xffffffffu, mine && mt > m + 8.0f)) {  // (others hold anything)
                             const float mn = fmaxf(m, mt);
                             const float k = mn == -INFINITY ? 1.0f : ex2(m - mn);
                             l *= k;
@@ -834,7 +834,7 @@ prefix_attn_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_co
 #pragma unroll 1
                     for (b = e0 * per_entry; b < g.s.n_seqs; b++) {
                         si = pa_seq(g, c, b);
-                        per = per_entry == 1 ? c.info[b].w : PO ? os.per_head(si) : si.q > 0 ? os.tiles(si, 0) : 0;
+                        per = per_entry == 1 ? c.info[b].w : PO ? os.per_head(si) : si.q > 0 ? os.steps(si, 0) : 0;
                         if (rest < per * g.a.n_kv) break;
                         rest -= per * g.a.n_kv;
                     }
@@ -890,7 +890,7 @@ prefix_attn_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_co
                         o.kv_end = os.visible(si, rb);
                         nt = (o.kv_end + PA_TILE - 1) / PA_TILE;
                     }
-                    const int ns = nt + (own && PO && nt > 0 ? g.p.extra : 0);  // steps of the item
+                    const int ns = nt + (own && nt > 0 ? g.p.extra : 0);  // steps of the item
                     const int from = hl == 0 ? t : 0;
                     int upto = ns - from;  // steps up to here in the batch
 #pragma unroll
@@ -921,11 +921,14 @@ prefix_attn_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_co
                             g.p.split[worker] = SplitItem{min(rows, block), first_row, kh, item};
                     }
                     put(o, valid);
+                    int tiles = valid ? n : 0;  // rounds the batch takes
+#pragma unroll
+                    for (int k = 8; k > 0; k >>= 1) tiles += __shfl_xor_sync(0xffffffffu, tiles, k);
+                    rounds += tiles;
                     const int all = min(__shfl_sync(0xffffffffu, upto, 15, 16), hi - step);
                     jj = __shfl_sync(0xffffffffu, jj, 15, 16) + 1;
                     bb = __shfl_sync(0xffffffffu, bb, 15, 16);
                     if (go) {
-                        rounds += all;
                         step += all;
                         j = jj;
                         b = bb;
@@ -934,10 +937,10 @@ prefix_attn_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_co
                     }
                 }
                 // both flows take the same number of rounds
-                if (!paired) {
-                    const bool odd = __shfl_sync(0xffffffffu, rounds, 16) < __shfl_sync(0xffffffffu, rounds, 0);
-                    o = PaSeg{0, 1, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0};
-                    if (odd && ok) put(o, lane == 16);
+                if (!paired && ok) {
+                    const int more = __shfl_xor_sync(0xffffffffu, rounds, 16) - rounds;
+                    o = PaSeg{0, more, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0};
+                    put(o, hl == 0 && more > 0);
                 }
             };
             if (line.sp > 0) part(std::false_type{});
