@@ -144,9 +144,10 @@ __device__ __forceinline__ void tmem_wait_st() { asm volatile("tcgen05.wait::st.
 // gave up; then the CTA tears down and reports.
 constexpr int PA_POLLS = 1 << 22;
 __device__ __forceinline__ bool pa_wait(PaCtl& c, uint64_t* bar, unsigned parity) {
-#pragma unroll 1
-    for (int i = 0; i < PA_POLLS && !*reinterpret_cast<volatile int*>(&c.abort); i++)
+    int i = 0;
+    do {
         if (mbar_try_wait(bar, parity)) return true;
+    } while (++i < PA_POLLS && !*reinterpret_cast<volatile int*>(&c.abort));
     *reinterpret_cast<volatile int*>(&c.abort) = 1;
     return false;
 }
@@ -154,9 +155,10 @@ __device__ __forceinline__ bool pa_wait(PaCtl& c, uint64_t* bar, unsigned parity
 // their operands from uniform registers, and moving them there lane by lane made the issue of an
 // MMA cost twice its execution.
 __device__ __forceinline__ bool pa_wait_warp(PaCtl& c, uint64_t* bar, unsigned parity) {
-#pragma unroll 1
-    for (int i = 0; i < PA_POLLS && !__any_sync(0xffffffffu, *reinterpret_cast<volatile int*>(&c.abort)); i++)
+    int i = 0;
+    do {
         if (__all_sync(0xffffffffu, mbar_try_wait(bar, parity))) return true;
+    } while (++i < PA_POLLS && !__any_sync(0xffffffffu, *reinterpret_cast<volatile int*>(&c.abort)));
     *reinterpret_cast<volatile int*>(&c.abort) = 1;
     return false;
 }
@@ -167,9 +169,14 @@ __device__ __forceinline__ void exchange(T& a, T& b) {
     b = t;
 }
 
-__device__ __forceinline__ float max3(float a, float b, float c) {
+__device__ __forceinline__ float max3(float a, float b, float c) {  // NaN when one of them is
     float d;
-    asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+    asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+    return d;
+}
+__device__ __forceinline__ float max_nan(float a, float b) {
+    float d;
+    asm("max.NaN.f32 %0, %1, %2;" : "=f"(d) : "f"(a), "f"(b));
     return d;
 }
 
@@ -388,8 +395,8 @@ prefix_attn_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_co
                         mt *= cs;
                         if (t == sg.t0) {
                             m = mt;
-                        } else if (__any_sync(0xffffffffu, mine && mt > m + 8.0f)) {  // (others hold anything)
-                            const float mn = fmaxf(m, mt);
+                        } else if (__any_sync(0xffffffffu, mine && !(mt <= m + 8.0f))) {  // (others hold anything)
+                            const float mn = max_nan(m, mt);
                             const float k = mn == -INFINITY ? 1.0f : ex2(m - mn);
                             l *= k;
                             m = mn;
@@ -422,7 +429,7 @@ prefix_attn_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_co
                         for (int i = 4; i < 28; i += 8)
 #pragma unroll
                             for (int j = 0; j < 4; j++) mx[j] = max3(mx[j], s[i + 2 * j], s[i + 2 * j + 1]);
-                        const float neg = raise(fmaxf(max3(mx[0], s[28], s[29]), max3(max3(mx[1], s[30], s[31]), mx[2], mx[3])));
+                        const float neg = raise(max_nan(max3(mx[0], s[28], s[29]), max3(max3(mx[1], s[30], s[31]), mx[2], mx[3])));
                         uint32_t pk[16];
                         float2 sum = make_float2(0.0f, 0.0f);
 #pragma unroll
@@ -454,7 +461,7 @@ prefix_attn_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_co
                         for (int i = 4; i < 124; i += 8)
 #pragma unroll
                             for (int j = 0; j < 4; j++) mx[j] = max3(mx[j], s[i + 2 * j], s[i + 2 * j + 1]);
-                        const float neg = raise(fmaxf(max3(mx[0], mx[1], max3(mx[2], s[124], s[125])), max3(mx[3], s[126], s[127])));
+                        const float neg = raise(max_nan(max3(mx[0], mx[1], max3(mx[2], s[124], s[125])), max3(mx[3], s[126], s[127])));
                         const float2 cs2 = make_float2(cs, cs), neg2 = make_float2(neg, neg);
                         float2 sum[2] = {make_float2(0.0f, 0.0f), make_float2(0.0f, 0.0f)};
 #pragma unroll
