@@ -37,7 +37,9 @@ __device__ __forceinline__ void mma_tf32(float c[4], const uint32_t a[4], uint32
         : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
         : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
-// c += a b as 3xTF32: the small cross terms into x, big.big into c
+// c += a b as 3xTF32: the small cross terms into x, big.big into c. The tensor cores cut a sum off
+// where an f32 addition rounds it, so c takes few of them in a row: two at a time, then f32 sums
+// (chains of eight had the results 1.6 times as far off as plain f32).
 __device__ __forceinline__ void mma_3tf32(float c[4], float x[4], float a0, float a1, float a2, float a3, float b0, float b1) {
     const uint32_t ab[4] = {tf_big(a0), tf_big(a1), tf_big(a2), tf_big(a3)};
     const uint32_t as[4] = {tf_small(a0, ab[0]), tf_small(a1, ab[1]), tf_small(a2, ab[2]), tf_small(a3, ab[3])};
@@ -217,53 +219,65 @@ prefix_attn_f32_kernel(const __grid_constant__ PrefixAttnArgs a, const __grid_co
 #pragma unroll
             for (int i = 0; i < 2 * VB; i++) o[i][0] = o[i][1] = o[i][2] = o[i][3] = 0.0f;
 
-            const int pos1 = min(end * p.tile, kv_end);
+            const int pos0 = tile * p.tile, pos1 = min(end * p.tile, kv_end);
             float4 kr[2][KB], vr[4][VB];
-            // element offset of position x of this kv head (-1: none, or no such page)
-            auto offset = [&](int x) -> int64_t {
-                if (x >= pos1) return -1;
-                const int pg = table[x >> s.page_shift];
+            // 8 positions lie in one page: where the 8 from x on begin, for this kv head, and how
+            // many of them count; past the end the last 8 again, their rows from the last one on
+            // (finite where a visible row is, and masked)
+            struct Eight {
+                int64_t at;
+                int most;
+            };
+            const int last8 = (pos1 - 1) & ~7;
+            auto eight = [&](int x) {
+                x = min(x, last8);
+                int pg = table[x >> s.page_shift];
                 if ((unsigned)pg >= (unsigned)s.n_pages) {
                     flag_error(a.err, ERR_PAGE_ID, pg);
-                    return -1;
+                    pg = 0;
                 }
-                return pg * a.page_stride + (((int64_t)kh << s.page_shift) + (x & mask)) * D;
+                return Eight{pg * a.page_stride + (((int64_t)kh << s.page_shift) + (x & mask)) * D, pos1 - 1 - x};
             };
-            auto load_k = [&](int x) {
+            Eight now[2], then[2];
+            auto load_k = [&](const Eight e[2]) {
 #pragma unroll
                 for (int r = 0; r < 2; r++) {
-                    const int64_t at = offset(x + 8 * r + g);
-                    const float4* src = reinterpret_cast<const float4*>(static_cast<const float*>(a.k) + at + 4 * t4);
+                    const float4* src = reinterpret_cast<const float4*>(static_cast<const float*>(a.k) + e[r].at) +
+                                        min(g, e[r].most) * (D / 4) + t4;
 #pragma unroll
-                    for (int i = 0; i < KB; i++) kr[r][i] = at >= 0 ? src[4 * i] : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+                    for (int i = 0; i < KB; i++) kr[r][i] = src[4 * i];
                 }
             };
-            auto load_v = [&](int x) {
+            auto load_v = [&](const Eight e[2]) {
 #pragma unroll
                 for (int r = 0; r < 4; r++) {
-                    const int64_t at = offset(x + 4 * r + t4);
-                    const float4* src = reinterpret_cast<const float4*>(static_cast<const float*>(a.v) + at + 4 * g);
+                    const float4* src = reinterpret_cast<const float4*>(static_cast<const float*>(a.v) + e[r >> 1].at) +
+                                        min(4 * (r & 1) + t4, e[r >> 1].most) * (D / 4) + g;
 #pragma unroll
-                    for (int i = 0; i < VB; i++) vr[r][i] = at >= 0 ? src[8 * i] : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+                    for (int i = 0; i < VB; i++) vr[r][i] = src[8 * i];
                 }
             };
-            load_k(tile * p.tile);
-            load_v(tile * p.tile);
+            now[0] = eight(pos0), now[1] = eight(pos0 + 8);
+            load_k(now);
+            load_v(now);
 #pragma unroll 1
-            for (int x = tile * p.tile; x < pos1; x += 16) {
-                float c[2][4], y[2][4];
+            for (int x = pos0; x < pos1; x += 16) {
+                then[0] = eight(x + 16), then[1] = eight(x + 24);
+                float sc[4] = {0.0f, 0.0f, 0.0f, 0.0f}, y[2][4];
 #pragma unroll
-                for (int i = 0; i < 4; i++) c[0][i] = c[1][i] = y[0][i] = y[1][i] = 0.0f;
+                for (int i = 0; i < 4; i++) y[0][i] = y[1][i] = 0.0f;
 #pragma unroll
                 for (int i = 0; i < KB; i++) {
-                    mma_3tf32(c[0], y[0], kr[0][i].x, kr[1][i].x, kr[0][i].y, kr[1][i].y, q[i].x, q[i].y);
-                    mma_3tf32(c[1], y[1], kr[0][i].z, kr[1][i].z, kr[0][i].w, kr[1][i].w, q[i].z, q[i].w);
+                    float c[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+                    mma_3tf32(c, y[0], kr[0][i].x, kr[1][i].x, kr[0][i].y, kr[1][i].y, q[i].x, q[i].y);
+                    mma_3tf32(c, y[1], kr[0][i].z, kr[1][i].z, kr[0][i].w, kr[1][i].w, q[i].z, q[i].w);
+#pragma unroll
+                    for (int j = 0; j < 4; j++) sc[j] += c[j];
                 }
-                load_k(x + 16);
-                float sc[4];
+                load_k(then);
 #pragma unroll
                 for (int i = 0; i < 4; i++) {  // position x + g + 8 (i / 2), row 2 t4 + i % 2
-                    sc[i] = (c[0][i] + c[1][i]) + (y[0][i] + y[1][i]);
+                    sc[i] += y[0][i] + y[1][i];
                     if (x + g + 8 * (i >> 1) >= vis[i & 1]) sc[i] = -INFINITY;
                 }
                 float up[2];
@@ -274,7 +288,7 @@ prefix_attn_f32_kernel(const __grid_constant__ PrefixAttnArgs a, const __grid_co
                     for (int d = 4; d < 32; d <<= 1) up[k] = fmaxf(up[k], __shfl_xor_sync(0xffffffffu, up[k], d));
                 }
                 // a maximum that grew by less than 2^8 stays: p <= 256 costs an f32 sum nothing
-                if (__any_sync(0xffffffffu, up[0] > m[0] + 8.0f || up[1] > m[1] + 8.0f || x == tile * p.tile)) {
+                if (__any_sync(0xffffffffu, up[0] > m[0] + 8.0f || up[1] > m[1] + 8.0f || x == pos0)) {
 #pragma unroll
                     for (int k = 0; k < 2; k++) {
                         const float mn = fmaxf(m[k], up[k]);
@@ -298,25 +312,25 @@ prefix_attn_f32_kernel(const __grid_constant__ PrefixAttnArgs a, const __grid_co
 #pragma unroll
                 for (int i = 0; i < 4; i++) pb[i] = pr[t4 + 4 * i][g];
                 __syncwarp();
-                // the tensor cores' sums are cut off, not rounded: over thousands of positions that
-                // would add up, so 16 positions at a time go into the f32 sums
+                // (16 positions at a time go into the f32 sums)
 #pragma unroll
                 for (int i = 0; i < VB; i++) {
-                    float w[2][4];
+                    float w[2][4], u[2][4];
 #pragma unroll
-                    for (int j = 0; j < 4; j++) w[0][j] = w[1][j] = 0.0f;
+                    for (int j = 0; j < 4; j++) w[0][j] = w[1][j] = u[0][j] = u[1][j] = 0.0f;
 #pragma unroll
                     for (int h = 0; h < 2; h++) {
-                        mma_3tf32(w[0], w[0], vr[2 * h][i].x, vr[2 * h][i].y, vr[2 * h + 1][i].x, vr[2 * h + 1][i].y, pb[2 * h], pb[2 * h + 1]);
-                        mma_3tf32(w[1], w[1], vr[2 * h][i].z, vr[2 * h][i].w, vr[2 * h + 1][i].z, vr[2 * h + 1][i].w, pb[2 * h], pb[2 * h + 1]);
+                        mma_3tf32(w[0], u[0], vr[2 * h][i].x, vr[2 * h][i].y, vr[2 * h + 1][i].x, vr[2 * h + 1][i].y, pb[2 * h], pb[2 * h + 1]);
+                        mma_3tf32(w[1], u[1], vr[2 * h][i].z, vr[2 * h][i].w, vr[2 * h + 1][i].z, vr[2 * h + 1][i].w, pb[2 * h], pb[2 * h + 1]);
                     }
 #pragma unroll
                     for (int j = 0; j < 4; j++) {
-                        o[2 * i][j] += w[0][j];
-                        o[2 * i + 1][j] += w[1][j];
+                        o[2 * i][j] += w[0][j] + u[0][j];
+                        o[2 * i + 1][j] += w[1][j] + u[1][j];
                     }
                 }
-                load_v(x + 16);
+                load_v(then);
+                now[0] = then[0], now[1] = then[1];
             }
             // ---- its result: rows 2 t4, 2 t4 + 1, dims 32 i + 4 g .. + 3 ----
 #pragma unroll
