@@ -6,10 +6,11 @@
 // takes 8 stacked query rows through its steps of 32 positions, 16 at a time,
 //   S^T = K Q^T     mma.sync m16n8k8: 16 positions x 8 rows
 //   O^T += V^T P^T  16 dims x 8 rows, 8 positions deep
-// with K and V straight from global memory into the operand registers: the order of the dims in
-// the products is free, so that a lane's elements of K (4 dims of 2 positions) and of V (4 dims of
-// 4 positions) are 16-byte vectors and every fetched sector is used whole. No warp waits for
-// another; the running maximum and sum of a row lie in the lanes that hold its scores.
+// K and V rows come by bulk copies into a ring of three slots of the warp's own (K, V, K, V, ..., 16
+// rows each): one is worked on while two are in flight, 128 KB an SM. The order of the dims in the
+// products is free, so a lane's elements of K (4 dims of 2 positions) and of V (4 dims of 4
+// positions) are 16-byte vectors; the rows are padded so that a warp's reads meet no bank twice. No
+// warp waits for another; the running maximum and sum of a row lie in the lanes that hold its scores.
 // Bound: HBM where few rows share a position (8 rows: 96 MMAs and about 500 other instructions per
 // 16 KB), the MMA and split instructions where many do.
 #include "lq8_async.cuh"
@@ -22,7 +23,9 @@
 namespace lq {
 
 constexpr int PF_WARPS = PREFIX_ATTN_F32_WARPS;
-constexpr int PF_SCAN = 1024;
+constexpr int PF_SCAN = 256;
+constexpr int PF_SLOTS = 3;
+constexpr int ERR_PF_WAIT = 95;  // a copy did not land
 
 __device__ __forceinline__ float pf_ex2(float x) {
     float y;
@@ -40,13 +43,13 @@ __device__ __forceinline__ void mma_tf32(float c[4], const uint32_t a[4], uint32
 // c += a b as 3xTF32: the small cross terms into x, big.big into c. The tensor cores cut a sum off
 // where an f32 addition rounds it, so c takes few of them in a row: two at a time, then f32 sums
 // (chains of eight had the results 1.6 times as far off as plain f32).
-__device__ __forceinline__ void mma_3tf32(float c[4], float x[4], float a0, float a1, float a2, float a3, float b0, float b1) {
+__device__ __forceinline__ void mma_3tf32(float c[4], float x[4], float a0, float a1, float a2, float a3, uint32_t b0,
+                                          uint32_t b1, uint32_t b0_small, uint32_t b1_small) {
     const uint32_t ab[4] = {tf_big(a0), tf_big(a1), tf_big(a2), tf_big(a3)};
     const uint32_t as[4] = {tf_small(a0, ab[0]), tf_small(a1, ab[1]), tf_small(a2, ab[2]), tf_small(a3, ab[3])};
-    const uint32_t bb0 = tf_big(b0), bb1 = tf_big(b1);
-    mma_tf32(x, as, bb0, bb1);
-    mma_tf32(x, ab, tf_small(b0, bb0), tf_small(b1, bb1));
-    mma_tf32(c, ab, bb0, bb1);
+    mma_tf32(x, as, b0, b1);
+    mma_tf32(x, ab, b0_small, b1_small);
+    mma_tf32(c, ab, b0, b1);
 }
 
 template <int D>
@@ -54,10 +57,21 @@ __global__ void __launch_bounds__(PF_WARPS * 32, 1)
 prefix_attn_f32_kernel(const __grid_constant__ PrefixAttnArgs a, const __grid_constant__ PagedSeqs s,
                        const __grid_constant__ PrefixPlan p) {
     constexpr int KB = D / 16, VB = D / 32;  // 16-byte vectors of a K row, of a V row, per lane
+    constexpr int KS = D * 4 + 64, VS = D * 4 + 32, SLOT = 16 * KS;  // bytes from row to row, of a slot
+    extern __shared__ __align__(128) uint8_t slots[];
+    __shared__ uint64_t full[PF_WARPS][PF_SLOTS];
     __shared__ int scan[PF_SCAN + 1];
     __shared__ int4 info[PF_SCAN];  // up to PF_SCAN sequences: q0, q, kv, steps of a head
     __shared__ __align__(16) float prob[PF_WARPS][16][8];
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t4 = lane & 3;
+    uint8_t* const mine = slots + warp * PF_SLOTS * SLOT;
+    if (lane == 0)
+        for (int i = 0; i < PF_SLOTS; i++) mbar_init(&full[warp][i], 1);
+    mbar_fence_init();
+    __syncwarp();
+    int slot = 0;       // of the next K or V to be worked on
+    unsigned ph = 0;    // and its parity
+    bool ok = true;
     pdl_wait();
     pdl_trigger();  // (after the wait: the merge reads the call's lengths before its own)
     const int per_entry = (s.n_seqs + PF_SCAN - 1) / PF_SCAN;
@@ -173,7 +187,7 @@ prefix_attn_f32_kernel(const __grid_constant__ PrefixAttnArgs a, const __grid_co
             tile = rest;
         }
 #pragma unroll 1
-        while (step < hi) {
+        while (step < hi && ok) {
             // ---- a segment: tiles [tile, end) of one item ----
             int kv_end = a.prefix_len;
             if (own) {
@@ -195,7 +209,7 @@ prefix_attn_f32_kernel(const __grid_constant__ PrefixAttnArgs a, const __grid_co
                 tok = a.group_div(row0 + r);
                 head = kh * a.group + row0 + r - tok * a.group;
             };
-            float4 q[KB];
+            uint32_t qb[KB][4], qm[KB][4];  // big and small parts
             {
                 int tok, head;
                 row_of(min(g, n - 1), tok, head);
@@ -204,7 +218,12 @@ prefix_attn_f32_kernel(const __grid_constant__ PrefixAttnArgs a, const __grid_co
 #pragma unroll
                 for (int i = 0; i < KB; i++) {
                     const float4 x = g < n ? src[4 * i] : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-                    q[i] = make_float4(x.x * qs, x.y * qs, x.z * qs, x.w * qs);
+                    const float v[4] = {x.x * qs, x.y * qs, x.z * qs, x.w * qs};
+#pragma unroll
+                    for (int j = 0; j < 4; j++) {
+                        qb[i][j] = tf_big(v[j]);
+                        qm[i][j] = tf_small(v[j], qb[i][j]);
+                    }
                 }
             }
             // positions that rows 2 t4 and 2 t4 + 1 see
@@ -220,61 +239,66 @@ prefix_attn_f32_kernel(const __grid_constant__ PrefixAttnArgs a, const __grid_co
             for (int i = 0; i < 2 * VB; i++) o[i][0] = o[i][1] = o[i][2] = o[i][3] = 0.0f;
 
             const int pos0 = tile * p.tile, pos1 = min(end * p.tile, kv_end);
-            float4 kr[2][KB], vr[4][VB];
-            // 8 positions lie in one page: where the 8 from x on begin, for this kv head, and how
-            // many of them count; past the end the last 8 again, their rows from the last one on
-            // (finite where a visible row is, and masked)
-            struct Eight {
-                int64_t at;
-                int most;
-            };
-            const int last8 = (pos1 - 1) & ~7;
-            auto eight = [&](int x) {
-                x = min(x, last8);
-                int pg = table[x >> s.page_shift];
+            // where position min(x + lane, the last one) lies for this kv head, lanes 0 to 15: rows
+            // past the end repeat the last one (finite where that is, and masked)
+            auto page_of = [&](int x) { return table[min(x + (lane & 15), pos1 - 1) >> s.page_shift]; };
+            auto place = [&](int x, int pg) -> int64_t {
                 if ((unsigned)pg >= (unsigned)s.n_pages) {
                     flag_error(a.err, ERR_PAGE_ID, pg);
                     pg = 0;
                 }
-                return Eight{pg * a.page_stride + (((int64_t)kh << s.page_shift) + (x & mask)) * D, pos1 - 1 - x};
+                return pg * a.page_stride + (((int64_t)kh << s.page_shift) + (min(x + (lane & 15), pos1 - 1) & mask)) * D;
             };
-            Eight now[2], then[2];
-            auto load_k = [&](const Eight e[2]) {
-#pragma unroll
-                for (int r = 0; r < 2; r++) {
-                    const float4* src = reinterpret_cast<const float4*>(static_cast<const float*>(a.k) + e[r].at) +
-                                        min(g, e[r].most) * (D / 4) + t4;
-#pragma unroll
-                    for (int i = 0; i < KB; i++) kr[r][i] = src[4 * i];
-                }
+            auto fetch = [&](int to, const void* base, int64_t at, int stride) {
+                if (lane == 0) mbar_expect_tx(&full[warp][to], 16 * D * 4);
+                __syncwarp();
+                if (lane < 16) bulk_g2s(mine + to * SLOT + lane * stride, static_cast<const float*>(base) + at, D * 4, &full[warp][to]);
             };
-            auto load_v = [&](const Eight e[2]) {
-#pragma unroll
-                for (int r = 0; r < 4; r++) {
-                    const float4* src = reinterpret_cast<const float4*>(static_cast<const float*>(a.v) + e[r >> 1].at) +
-                                        min(4 * (r & 1) + t4, e[r >> 1].most) * (D / 4) + g;
-#pragma unroll
-                    for (int i = 0; i < VB; i++) vr[r][i] = src[8 * i];
-                }
+            auto after = [](int i, int by) { return (i + by) % PF_SLOTS; };
+            auto landed = [&]() {
+                ok = mbar_wait(&full[warp][slot], ph, 1ll << 22);
+                ok = __all_sync(0xffffffffu, ok);
+                return ok;
             };
-            now[0] = eight(pos0), now[1] = eight(pos0 + 8);
-            load_k(now);
-            load_v(now);
+            auto done = [&]() {
+                __syncwarp();  // (read by every lane)
+                if (++slot == PF_SLOTS) slot = 0, ph ^= 1;
+            };
+            // in flight: K and V of the first 16 positions, K of the next
+            int64_t at_v = place(pos0, page_of(pos0)), at_k = 0;
+            int pg = page_of(pos0 + 16);
+            fetch(slot, a.k, at_v, KS);
+            fetch(after(slot, 1), a.v, at_v, VS);
+            if (pos0 + 16 < pos1) {
+                at_k = place(pos0 + 16, pg);
+                fetch(after(slot, 2), a.k, at_k, KS);
+            }
 #pragma unroll 1
             for (int x = pos0; x < pos1; x += 16) {
-                then[0] = eight(x + 16), then[1] = eight(x + 24);
+                if (x + 32 < pos1) pg = page_of(x + 32);
                 float sc[4] = {0.0f, 0.0f, 0.0f, 0.0f}, y[2][4];
 #pragma unroll
                 for (int i = 0; i < 4; i++) y[0][i] = y[1][i] = 0.0f;
+                if (!landed()) break;
+                {
+                    const uint8_t* const k0 = mine + slot * SLOT + g * KS + t4 * 16;
 #pragma unroll
-                for (int i = 0; i < KB; i++) {
-                    float c[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-                    mma_3tf32(c, y[0], kr[0][i].x, kr[1][i].x, kr[0][i].y, kr[1][i].y, q[i].x, q[i].y);
-                    mma_3tf32(c, y[1], kr[0][i].z, kr[1][i].z, kr[0][i].w, kr[1][i].w, q[i].z, q[i].w);
+                    for (int i = 0; i < KB; i++) {
+                        const float4 lo = *reinterpret_cast<const float4*>(k0 + 64 * i);
+                        const float4 hi8 = *reinterpret_cast<const float4*>(k0 + 8 * KS + 64 * i);
+                        float c[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+                        mma_3tf32(c, y[0], lo.x, hi8.x, lo.y, hi8.y, qb[i][0], qb[i][1], qm[i][0], qm[i][1]);
+                        mma_3tf32(c, y[1], lo.z, hi8.z, lo.w, hi8.w, qb[i][2], qb[i][3], qm[i][2], qm[i][3]);
 #pragma unroll
-                    for (int j = 0; j < 4; j++) sc[j] += c[j];
+                        for (int j = 0; j < 4; j++) sc[j] += c[j];
+                    }
                 }
-                load_k(then);
+                done();
+                // the slot's next: V of the 16 positions after these
+                if (x + 16 < pos1) {
+                    fetch(after(slot, 2), a.v, at_k, VS);
+                    at_v = at_k;
+                }
 #pragma unroll
                 for (int i = 0; i < 4; i++) {  // position x + g + 8 (i / 2), row 2 t4 + i % 2
                     sc[i] += y[0][i] + y[1][i];
@@ -308,29 +332,45 @@ prefix_attn_f32_kernel(const __grid_constant__ PrefixAttnArgs a, const __grid_co
                 *reinterpret_cast<float2*>(&pr[g][2 * t4]) = make_float2(e[0], e[1]);
                 *reinterpret_cast<float2*>(&pr[g + 8][2 * t4]) = make_float2(e[2], e[3]);
                 __syncwarp();
-                float pb[4];  // positions x + t4 + 4 i, row g
+                uint32_t pb[4], pm[4];  // positions x + t4 + 4 i, row g: big and small parts
 #pragma unroll
-                for (int i = 0; i < 4; i++) pb[i] = pr[t4 + 4 * i][g];
-                __syncwarp();
-                // (16 positions at a time go into the f32 sums)
+                for (int i = 0; i < 4; i++) {
+                    const float v = pr[t4 + 4 * i][g];
+                    pb[i] = tf_big(v);
+                    pm[i] = tf_small(v, pb[i]);
+                }
+                if (!landed()) break;
+                {
+                    const uint8_t* const v0 = mine + slot * SLOT + t4 * VS + g * 16;
 #pragma unroll
-                for (int i = 0; i < VB; i++) {
-                    float w[2][4], u[2][4];
+                    for (int i = 0; i < VB; i++) {  // (16 positions at a time go into the f32 sums)
+                        float w[2][4], u[2][4];
 #pragma unroll
-                    for (int j = 0; j < 4; j++) w[0][j] = w[1][j] = u[0][j] = u[1][j] = 0.0f;
+                        for (int j = 0; j < 4; j++) w[0][j] = w[1][j] = u[0][j] = u[1][j] = 0.0f;
 #pragma unroll
-                    for (int h = 0; h < 2; h++) {
-                        mma_3tf32(w[0], u[0], vr[2 * h][i].x, vr[2 * h][i].y, vr[2 * h + 1][i].x, vr[2 * h + 1][i].y, pb[2 * h], pb[2 * h + 1]);
-                        mma_3tf32(w[1], u[1], vr[2 * h][i].z, vr[2 * h][i].w, vr[2 * h + 1][i].z, vr[2 * h + 1][i].w, pb[2 * h], pb[2 * h + 1]);
-                    }
+                        for (int h = 0; h < 2; h++) {
+                            const float4 r0 = *reinterpret_cast<const float4*>(v0 + (8 * h) * VS + 128 * i);
+                            const float4 r1 = *reinterpret_cast<const float4*>(v0 + (8 * h + 4) * VS + 128 * i);
+                            mma_3tf32(w[0], u[0], r0.x, r0.y, r1.x, r1.y, pb[2 * h], pb[2 * h + 1], pm[2 * h], pm[2 * h + 1]);
+                            mma_3tf32(w[1], u[1], r0.z, r0.w, r1.z, r1.w, pb[2 * h], pb[2 * h + 1], pm[2 * h], pm[2 * h + 1]);
+                        }
 #pragma unroll
-                    for (int j = 0; j < 4; j++) {
-                        o[2 * i][j] += w[0][j] + u[0][j];
-                        o[2 * i + 1][j] += w[1][j] + u[1][j];
+                        for (int j = 0; j < 4; j++) {
+                            o[2 * i][j] += w[0][j] + u[0][j];
+                            o[2 * i + 1][j] += w[1][j] + u[1][j];
+                        }
                     }
                 }
-                load_v(then);
-                now[0] = then[0], now[1] = then[1];
+                done();
+                // the slot's next: K of the 16 positions after those
+                if (x + 32 < pos1) {
+                    at_k = place(x + 32, pg);
+                    fetch(after(slot, 2), a.k, at_k, KS);
+                }
+            }
+            if (!ok) {
+                flag_error(a.err, ERR_PF_WAIT, worker);
+                break;
             }
             // ---- its result: rows 2 t4, 2 t4 + 1, dims 32 i + 4 g .. + 3 ----
 #pragma unroll
@@ -338,25 +378,25 @@ prefix_attn_f32_kernel(const __grid_constant__ PrefixAttnArgs a, const __grid_co
 #pragma unroll
                 for (int d = 4; d < 32; d <<= 1) l[k] += __shfl_xor_sync(0xffffffffu, l[k], d);
                 const int r = 2 * t4 + k;
-                const bool mine = r < n;
+                const bool real = r < n;
                 int tok, head;
                 row_of(min(r, n - 1), tok, head);
                 const int64_t slot = item + worker;
                 const int cap = p.cap[part];
-                if (mine && !whole && g == 0) p.ml[part][slot * cap + r] = make_float2(m[k], l[k]);
+                if (real && !whole && g == 0) p.ml[part][slot * cap + r] = make_float2(m[k], l[k]);
                 const float inv = l[k] > 0.0f ? 1.0f / l[k] : l[k];
 #pragma unroll
                 for (int i = 0; i < VB; i++) {
                     float v[4] = {o[2 * i][k], o[2 * i][2 + k], o[2 * i + 1][k], o[2 * i + 1][2 + k]};
                     if (!whole) {
-                        if (mine)
+                        if (real)
                             reinterpret_cast<float4*>(p.o[part])[(slot * (D / 4) + 8 * i + g) * cap + r] =
                                 make_float4(v[0], v[1], v[2], v[3]);
                         continue;
                     }
 #pragma unroll
                     for (int j = 0; j < 4; j++) v[j] = l[k] == 0.0f ? 0.0f : v[j] * inv;
-                    if (mine && a.out)
+                    if (real && a.out)
                         *reinterpret_cast<float4*>(static_cast<float*>(a.out) + (int64_t)tok * a.out_stride + (int64_t)head * D +
                                                    32 * i + 4 * g) = make_float4(v[0], v[1], v[2], v[3]);
                     if (a.xq) {  // the 8 lanes of a row hold a block of 32 dims
@@ -368,7 +408,7 @@ prefix_attn_f32_kernel(const __grid_constant__ PrefixAttnArgs a, const __grid_co
                         uint32_t w = 0;
 #pragma unroll
                         for (int j = 0; j < 4; j++) w |= (uint32_t)(q8_quant(v[j], id) & 0xFF) << (8 * j);
-                        if (mine) {
+                        if (real) {
                             if (g == 0) a.xd[at / 32] = f2h(d);
                             *reinterpret_cast<uint32_t*>(a.xq + at + 4 * g) = w;
                         }
@@ -403,10 +443,17 @@ prefix_attn_f32_kernel(const __grid_constant__ PrefixAttnArgs a, const __grid_co
     }
 }
 
+template <int D>
+static int launch_f32(lq_ctx* ctx, const PrefixAttnArgs& a, const PagedSeqs& s, const PrefixPlan& p) {
+    const size_t smem = (size_t)PF_WARPS * PF_SLOTS * 16 * (D * 4 + 64);
+    const int rc = ensure_func_smem(ctx, (const void*)prefix_attn_f32_kernel<D>, smem);
+    if (rc) return rc;
+    return launch_kernel(ctx, prefix_attn_f32_kernel<D>, dim3((unsigned)std::min(ctx->sm_count, p.workers)),
+                         dim3(PF_WARPS * 32), smem, "prefix_attn_f32", a, s, p);
+}
+
 int launch_prefix_attn_f32(lq_ctx* ctx, const PrefixAttnArgs& a, const PagedSeqs& s, const PrefixPlan& p, int D) {
-    const dim3 grid((unsigned)std::min(ctx->sm_count, p.workers));
-    return D == 64 ? launch_kernel(ctx, prefix_attn_f32_kernel<64>, grid, dim3(PF_WARPS * 32), 0, "prefix_attn_f32", a, s, p)
-                   : launch_kernel(ctx, prefix_attn_f32_kernel<128>, grid, dim3(PF_WARPS * 32), 0, "prefix_attn_f32", a, s, p);
+    return D == 64 ? launch_f32<64>(ctx, a, s, p) : launch_f32<128>(ctx, a, s, p);
 }
 
 }  // namespace lq
