@@ -27,7 +27,7 @@ __global__ void __launch_bounds__(256) prefix_attn_merge_kernel(PrefixAttnArgs a
     constexpr int VEC = (CH + SUBS - 1) / SUBS;
     __shared__ int slot[MERGE_CHUNK];
     __shared__ float weight[MERGE_CHUNK][MR];
-    __shared__ float2 red[SUBS][MR];
+    __shared__ float2 red[8][MR];
     __shared__ __align__(16) float stage[MR][D + 4];
     const int tid = threadIdx.x, lane = tid & 31, r = tid % MR, sub = tid / MR;
     const OwnSteps os{a, p};
@@ -109,10 +109,12 @@ __global__ void __launch_bounds__(256) prefix_attn_merge_kernel(PrefixAttnArgs a
                             has = lo < hi;
                         }
                         slot[tid] = has ? item[part] + v : -1;
+                    } else if (tid < MERGE_CHUNK) {
+                        slot[tid] = -1;
                     }
                     __syncthreads();
                 }
-#pragma unroll 1
+                // a thread's share of the row's partials: (m, l) in pass 0, weights in pass 1
                 for (int i = sub; i < m; i += SUBS) {
                     const int part = c0 + i >= cnt[0];
                     float2 ml = make_float2(-INFINITY, 0.0f);
@@ -128,34 +130,54 @@ __global__ void __launch_bounds__(256) prefix_attn_merge_kernel(PrefixAttnArgs a
                 if (pass == 1) {
                     __syncthreads();
                     if (mine) {
-#pragma unroll 2
-                        for (int i = 0; i < m; i++) {
-                            const int part = c0 + i >= cnt[0];
-                            if (slot[i] < 0) continue;
-                            const float w = weight[i][r];
-                            const float4* src = reinterpret_cast<const float4*>(p.o[part]) +
-                                                ((int64_t)slot[i] * CH + sub) * p.cap[part] + in[part] + r;
+#pragma unroll 1
+                        for (int i0 = 0; i0 < m; i0 += 8 / VEC) {
+                            float4 x[8 / VEC][VEC];
+                            float w[8 / VEC];
 #pragma unroll
-                            for (int k = 0; k < VEC; k++) {
-                                if (CH % SUBS && sub + k * SUBS >= CH) break;
-                                const float4 x = src[(int64_t)k * SUBS * p.cap[part]];
-                                o[k].x = fmaf(w, x.x, o[k].x);
-                                o[k].y = fmaf(w, x.y, o[k].y);
-                                o[k].z = fmaf(w, x.z, o[k].z);
-                                o[k].w = fmaf(w, x.w, o[k].w);
+                            for (int j = 0; j < 8 / VEC; j++) {
+                                const int part = c0 + i0 + j >= cnt[0], at = slot[i0 + j];
+                                w[j] = at >= 0 ? weight[i0 + j][r] : 0.0f;
+#pragma unroll
+                                for (int k = 0; k < VEC; k++) {
+                                    x[j][k] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+                                    if (at >= 0 && !(CH % SUBS && sub + k * SUBS >= CH))
+                                        x[j][k] = reinterpret_cast<const float4*>(p.o[part])[((int64_t)at * CH + sub + k * SUBS) * p.cap[part] + in[part] + r];
+                                }
                             }
+#pragma unroll
+                            for (int j = 0; j < 8 / VEC; j++)
+#pragma unroll
+                                for (int k = 0; k < VEC; k++) {
+                                    o[k].x = fmaf(w[j], x[j][k].x, o[k].x);
+                                    o[k].y = fmaf(w[j], x[j][k].y, o[k].y);
+                                    o[k].z = fmaf(w[j], x[j][k].z, o[k].z);
+                                    o[k].w = fmaf(w[j], x[j][k].w, o[k].w);
+                                }
                         }
                     }
                 }
             }
-            if (pass == 0) {  // over the threads of a row, in their order
-                red[sub][r] = make_float2(M, L);
+            if (pass == 0) {  // over the threads of a row: of a warp, then the warps in order
+                auto join = [&](float m2, float l2) {
+                    const float up = fmaxf(M, m2);
+                    if (up != -INFINITY) L = L * exp2f(M - up) + l2 * exp2f(m2 - up);
+                    M = up;
+                };
+#pragma unroll
+                for (int d = MR; d < 32; d <<= 1) {
+                    const float m2 = __shfl_xor_sync(0xffffffffu, M, d), l2 = __shfl_xor_sync(0xffffffffu, L, d);
+                    // (both sides form the same sum: the lower lane's part first)
+                    const float up = fmaxf(M, m2), a0 = M == -INFINITY ? 0.0f : L * exp2f(M - up), a1 = m2 == -INFINITY ? 0.0f : l2 * exp2f(m2 - up);
+                    L = lane & d ? a1 + a0 : a0 + a1;
+                    M = up;
+                }
+                if (lane < MR) red[tid >> 5][r] = make_float2(M, L);
                 __syncthreads();
                 M = -INFINITY;
-                for (int k = 0; k < min(SUBS, n); k++) M = fmaxf(M, red[k][r].x);
                 L = 0.0f;
-                for (int k = 0; k < min(SUBS, n); k++)
-                    if (red[k][r].x != -INFINITY) L += red[k][r].y * exp2f(red[k][r].x - M);
+#pragma unroll
+                for (int k = 0; k < 8; k++) join(red[k][r].x, red[k][r].y);
             }
         }
         const float inv = L > 0.0f ? 1.0f / L : L;  // a row that saw nothing: zeros; NaN stays

@@ -36,7 +36,8 @@ namespace lq {
 
 constexpr int PA_ROWS = 128;      // rows of a flow (MMA M)
 constexpr int PA_TILE = 128;      // positions of a step
-constexpr int PA_STAGES = 4;
+// stages of the ring: 128 KB for either head dimension's tiles of 32 and 16 KB, or what is left
+constexpr int pa_stages(int D) { return D == 64 ? 10 : 4; }
 constexpr int PA_THREADS = 384;   // warps 0-7 softmax, 8 TMA, 9 MMA, 10 scheduler, 11 empty rows
 // registers: 384 x 168 at launch = 256 x 216 for the softmax warps + 128 x 72 for the others
 constexpr int PA_REGS = 216, PA_REGS_LOW = 72;
@@ -61,7 +62,7 @@ struct alignas(16) PaSeg {
 };
 
 struct PaCtl {
-    uint64_t full[PA_STAGES], empty[PA_STAGES];
+    uint64_t full[pa_stages(64)], empty[pa_stages(64)];
     uint64_t seg_full[2][2], seg_empty[2][2];  // per flow: two batches of segments
     uint64_t q_full[2], s_full[2], p_full[2], o_full[2], done;
     uint32_t tmem;
@@ -216,18 +217,18 @@ template <int D, bool PP, bool PO>
 __global__ void __launch_bounds__(PA_THREADS, 1)
 prefix_attn_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v,
                       const __grid_constant__ PaArgs g) {
-    constexpr int HALVES = D / 64;
+    constexpr int HALVES = D / 64, STAGES = pa_stages(D);
     constexpr int Q_BYTES = PA_ROWS * D * 2, KV_BYTES = PA_TILE * D * 2, HALF = 128 * 128;
     extern __shared__ uint8_t smem_raw[];
     const uint32_t raw = smem_addr(smem_raw);
     uint8_t* const sm = smem_raw + (((raw + 1023) & ~1023u) - raw);
     uint8_t* const ring = sm + 2 * Q_BYTES;
-    PaCtl& c = *reinterpret_cast<PaCtl*>(ring + PA_STAGES * KV_BYTES);
+    PaCtl& c = *reinterpret_cast<PaCtl*>(ring + STAGES * KV_BYTES);
     const int tid = threadIdx.x, warp = __shfl_sync(0xffffffffu, tid >> 5, 0), lane = tid & 31;
     int* const err = g.a.err;
 
     if (tid == 0) {
-        for (int i = 0; i < PA_STAGES; i++) mbar_init(&c.full[i], 1), mbar_init(&c.empty[i], 1);
+        for (int i = 0; i < STAGES; i++) mbar_init(&c.full[i], 1), mbar_init(&c.empty[i], 1);
 #pragma unroll 1
         for (int f = 0; f < 2; f++) {
             mbar_init(&c.q_full[f], 4);
@@ -647,7 +648,7 @@ prefix_attn_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_co
                             tma_load_4d(dst + h * HALF + lane * box * 128, map, h * 64, cur.krow, cur.kh, cur.pg, &c.full[slot]);
                     }
                     issued++;
-                    if (++slot == PA_STAGES) slot = 0, ph ^= 1;
+                    if (++slot == STAGES) slot = 0, ph ^= 1;
                 }
                 if (which) break;
                 cur.v_due = false;
@@ -681,8 +682,8 @@ prefix_attn_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_co
         // no copy may still be landing when the CTA exits
         if (!ok) {
 #pragma unroll 1
-            for (int i = max(0, issued - PA_STAGES); i < issued; i++)
-                mbar_wait_ns(&c.full[i % PA_STAGES], (unsigned)(i / PA_STAGES) & 1u, 2000000000ull);
+            for (int i = max(0, issued - STAGES); i < issued; i++)
+                mbar_wait_ns(&c.full[i % STAGES], (unsigned)(i / STAGES) & 1u, 2000000000ull);
         }
     } else if (warp == 9) {
         // ------------------------------ MMA issuer ------------------------------
@@ -708,7 +709,7 @@ prefix_attn_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_co
         auto take = [&](int& where) {  // the next stage of the ring
             ok = pa_wait_warp(c, &c.full[slot], ph);
             where = slot;
-            if (++slot == PA_STAGES) slot = 0, ph ^= 1;
+            if (++slot == STAGES) slot = 0, ph ^= 1;
         };
 #pragma unroll 1
         for (int f = 0; f || !(cur.ended && oth.ended && !cur.pv && !oth.pv); f ^= 1) {
@@ -982,7 +983,7 @@ static int launch_tc(lq_ctx* ctx, const PaArgs& g) {
     if (rc) return rc;
     rc = make_tensor_map_4d(ctx, &mv, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, g.a.v, dims, strides, box, CU_TENSOR_MAP_SWIZZLE_128B);
     if (rc) return rc;
-    const size_t smem = 1024 + 2 * PA_ROWS * D * 2 + PA_STAGES * PA_TILE * D * 2 + sizeof(PaCtl);
+    const size_t smem = 1024 + 2 * PA_ROWS * D * 2 + pa_stages(D) * PA_TILE * D * 2 + sizeof(PaCtl);
     rc = ensure_func_smem(ctx, (const void*)prefix_attn_tc_kernel<D, PP, PO>, smem);
     if (rc) return rc;
     return launch_kernel(ctx, prefix_attn_tc_kernel<D, PP, PO>, dim3((unsigned)g.p.workers), dim3(PA_THREADS), smem,
