@@ -232,7 +232,7 @@ __device__ __forceinline__ RowSlot find_slot(const PagedSeqs& s, int r, int lane
 }
 
 template <typename S, typename T, int D, int IT>
-__global__ void __launch_bounds__(256) paged_append_kernel(AppendArgs a, RopeAxes rope, PagedSeqs seqs, int groups) {
+__global__ void __launch_bounds__(256, 3) paged_append_kernel(AppendArgs a, RopeAxes rope, PagedSeqs seqs, int groups) {
     constexpr int LPH = D / 16, HPW = 32 / LPH, N = D / 2;  // lanes a head, heads side by side
     pdl_trigger();
     pdl_wait();
@@ -253,12 +253,15 @@ __global__ void __launch_bounds__(256) paged_append_kernel(AppendArgs a, RopeAxe
                 raw[j][1][k] = *reinterpret_cast<const Vec<S, 16 / sizeof(S)>*>(src + j * HPW * D + N + k * (16 / sizeof(S)));
             }
         }
-    const RowSlot slot = find_slot(seqs, row, lane, a.err);
-    if (!slot.live) return;
+    // (given positions do not wait for the row's place, whose loads depend on one another)
     float cs[8], sn[8];
     bool turn = true;
-    if (h0 < a.n_heads + a.n_kv)
-        turn = __all_sync(0xffffffffu, angles<8>(rope, row, rope.pos_base + slot.own, d0, cs, sn, a.err));
+    const bool turned = h0 < a.n_heads + a.n_kv;
+    if (turned && rope.pos) turn = angles<8>(rope, row, 0, d0, cs, sn, a.err);
+    const RowSlot slot = find_slot(seqs, row, lane, a.err);
+    if (!slot.live) return;
+    if (turned && !rope.pos) turn = angles<8>(rope, row, rope.pos_base + slot.own, d0, cs, sn, a.err);
+    turn = __all_sync(0xffffffffu, turn);
     T* const page_k = static_cast<T*>(a.k) + slot.page * a.page_stride;
     T* const page_v = static_cast<T*>(a.v) + slot.page * a.page_stride;
 #pragma unroll
@@ -404,7 +407,7 @@ static int launch_append_d(lq_ctx* ctx, const AppendArgs& a, const RopeAxes& rop
     const int heads = a.n_heads + 2 * a.n_kv, side = 512 / D;  // heads side by side in a warp
     // many rows: four heads a lane in flight (two of f32), which share the row's slot and angles;
     // a decode step's few rows: one, so that they spread over the SMs
-    constexpr int IT = sizeof(S) == 2 ? 4 : 2;
+    constexpr int IT = sizeof(S) == 2 ? 2 : 2;
     const bool few = (int64_t)s.rows * ceil_div(heads, side) < 16ll * ctx->sm_count;
     const int groups = ceil_div(heads, few ? side : side * IT);
     const dim3 grid((unsigned)ceil_div((int64_t)s.rows * groups, 8));

@@ -22,9 +22,9 @@ namespace lq {
 constexpr int MERGE_CHUNK = 32;   // partials looked at together
 
 template <typename T, int D, int MR>
-__global__ void __launch_bounds__(256) prefix_attn_merge_kernel(PrefixAttnArgs a, PagedSeqs s, PrefixPlan p) {
+__global__ void __launch_bounds__(256, MR == 32 ? 5 : 4) prefix_attn_merge_kernel(PrefixAttnArgs a, PagedSeqs s, PrefixPlan p) {
     constexpr int CH = D / 4, SUBS = 256 / MR;  // vectors of a row; threads that share a row
-    constexpr int VEC = (CH + SUBS - 1) / SUBS;
+    constexpr int VEC = (CH + SUBS - 1) / SUBS, BATCH = VEC == 1 ? 8 : 1;  // partials whose loads go out together
     __shared__ int slot[MERGE_CHUNK];
     __shared__ float weight[MERGE_CHUNK][MR];
     __shared__ float2 red[8][MR];
@@ -131,11 +131,11 @@ __global__ void __launch_bounds__(256) prefix_attn_merge_kernel(PrefixAttnArgs a
                     __syncthreads();
                     if (mine) {
 #pragma unroll 1
-                        for (int i0 = 0; i0 < m; i0 += 8 / VEC) {
-                            float4 x[8 / VEC][VEC];
-                            float w[8 / VEC];
+                        for (int i0 = 0; i0 < m; i0 += BATCH) {
+                            float4 x[BATCH][VEC];
+                            float w[BATCH];
 #pragma unroll
-                            for (int j = 0; j < 8 / VEC; j++) {
+                            for (int j = 0; j < BATCH; j++) {
                                 const int part = c0 + i0 + j >= cnt[0], at = slot[i0 + j];
                                 w[j] = at >= 0 ? weight[i0 + j][r] : 0.0f;
 #pragma unroll
@@ -146,7 +146,7 @@ __global__ void __launch_bounds__(256) prefix_attn_merge_kernel(PrefixAttnArgs a
                                 }
                             }
 #pragma unroll
-                            for (int j = 0; j < 8 / VEC; j++)
+                            for (int j = 0; j < BATCH; j++)
 #pragma unroll
                                 for (int k = 0; k < VEC; k++) {
                                     o[k].x = fmaf(w[j], x[j][k].x, o[k].x);
