@@ -142,13 +142,13 @@ __device__ __forceinline__ void tmem_wait_ld() { asm volatile("tcgen05.wait::ld.
 __device__ __forceinline__ void tmem_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 
 // Bounded wait: PA_POLLS polls (try_wait sleeps between them), or until another warp of the CTA
-// gave up; then the CTA tears down and reports.
+// gave up; then the CTA tears down and reports. The flag is looked at first: with the poll first,
+// 128 sequences behind 32768 positions took 212 us instead of 202.
 constexpr int PA_POLLS = 1 << 22;
 __device__ __forceinline__ bool pa_wait(PaCtl& c, uint64_t* bar, unsigned parity) {
-    int i = 0;
-    do {
+#pragma unroll 1
+    for (int i = 0; i < PA_POLLS && !*reinterpret_cast<volatile int*>(&c.abort); i++)
         if (mbar_try_wait(bar, parity)) return true;
-    } while (++i < PA_POLLS && !*reinterpret_cast<volatile int*>(&c.abort));
     *reinterpret_cast<volatile int*>(&c.abort) = 1;
     return false;
 }
@@ -156,10 +156,9 @@ __device__ __forceinline__ bool pa_wait(PaCtl& c, uint64_t* bar, unsigned parity
 // their operands from uniform registers, and moving them there lane by lane made the issue of an
 // MMA cost twice its execution.
 __device__ __forceinline__ bool pa_wait_warp(PaCtl& c, uint64_t* bar, unsigned parity) {
-    int i = 0;
-    do {
+#pragma unroll 1
+    for (int i = 0; i < PA_POLLS && !__any_sync(0xffffffffu, *reinterpret_cast<volatile int*>(&c.abort)); i++)
         if (__all_sync(0xffffffffu, mbar_try_wait(bar, parity))) return true;
-    } while (++i < PA_POLLS && !__any_sync(0xffffffffu, *reinterpret_cast<volatile int*>(&c.abort)));
     *reinterpret_cast<volatile int*>(&c.abort) = 1;
     return false;
 }
