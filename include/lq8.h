@@ -230,7 +230,7 @@ int lq_fill_bf16(lq_ctx* ctx, uint64_t seed, uint64_t tensor_id, int64_t offset,
  * ------------------------------------------------------------------------------------- */
 /* Waits for the context's stream; LQ_ERR_INVALID_ARG with the first code and value that a
  * kernel flagged since the last check (90 rotary position, 91 length, 92 page id, 93 row
- * count). */
+ * count, 94 and 95 a wait inside the attention that ran out: its output is not valid). */
 int lq_device_status(lq_ctx* ctx);
 /* Rotary positions with one to four axes (e.g. time, height, width). x [rows][heads][head_dim]
  * f32 or bf16 with the given strides (elements) to out (may be x): pair i < rot_dim/2 of a head
@@ -266,7 +266,9 @@ int lq_paged_append(lq_ctx* ctx, const void* qkv_dev, lq_dtype qkv_dtype, int64_
  * workspace, which the context keeps and grows outside graph capture. out [rows][n_heads *
  * head_dim] in the cache type and/or Q8_0 rows xq [rows][n_heads * head_dim], xd (either may be
  * NULL). A row that sees nothing gives zeros. Pointers and strides are multiples of 16 bytes.
- * f32 caches are computed in f32; bf16 ones with bf16 products and f32 sums. */
+ * f32 caches are computed in f32; bf16 ones with bf16 products and f32 sums. What a page holds past
+ * a sequence's end is never used; a NaN or infinity in V of a row of this call may reach earlier
+ * rows of its sequence. */
 int lq_prefix_attention(lq_ctx* ctx, const void* q_dev, lq_dtype dtype, int64_t q_stride, int64_t rows,
                         int64_t n_heads, int64_t n_kv_heads, int64_t head_dim, float scale,
                         const void* k_pages_dev, const void* v_pages_dev, int64_t n_pages, int64_t page_size,
