@@ -15,7 +15,7 @@ namespace lq {
 // the order of the line: with M the largest of their maxima, o = sum 2^(m_i - M) o_i /
 // sum 2^(m_i - M) l_i. A CTA takes up to MR rows of an own item (a sequence's row block and kv
 // head), which share the own item's partials and, but for a block's end, those of a prefix item.
-// Without a prefix only the items that are cut between workers are left: a worker leaves a note of
+// Without prefix items only the items that are cut between workers are left: a worker leaves a note of
 // the one that it begins. A thread adds up CH MR / 256 vectors of four dims of one row; rows lie
 // next to each other in memory.
 // =========================================================================================
@@ -31,7 +31,7 @@ __global__ void __launch_bounds__(256, MR == 32 ? 5 : 4) prefix_attn_merge_kerne
     __shared__ __align__(16) float stage[MR][D + 4];
     const int tid = threadIdx.x, lane = tid & 31, r = tid % MR, sub = tid / MR;
     const OwnSteps os{a, p};
-    const bool with_prefix = a.prefix_len > 0;
+    const bool with_prefix = p.np > 0;
     // the item, its rows st0 .. st0 + todo - 1 of this CTA, the first one's place in the item
     int st0 = 0, todo = 0, kh = 0, own_item = 0, own_in = blockIdx.y * MR;
     bool own = true;
@@ -235,8 +235,17 @@ static int make_plan(lq_ctx* ctx, const PrefixAttnArgs& a, const PagedSeqs& s, b
     p->cap[1] = (int)std::min<int64_t>(p->ob, most_q);
     p->n_rb = ceil_div(R, p->pb);
     p->np = ceil_div(a.prefix_len, tile);
+    // The prefix's tiles at the front of the own items: that costs at most n_seqs - 1 blocks more of
+    // np steps each, and saves a block's two partials and their merge, about as long as 9 steps
+    // (CHAINFIG).
+    p->chain = 0;
+    if (!f32 && p->pair_o && (s.n_seqs - 1) * (int64_t)p->np <= 9 * (R / p->pb) &&
+        (int64_t)a.prefix_len + a.max_kv < (1 << 30)) {
+        p->chain = p->np;
+        p->np = 0;
+    }
     const int64_t items_p = (int64_t)a.n_kv * p->n_rb, items_o = a.n_kv * (R / p->ob + s.n_seqs + 1);
-    const int64_t steps = items_p * p->np + items_o * (ceil_div(a.max_kv, tile) + 1);
+    const int64_t steps = items_p * p->np + items_o * (p->chain + ceil_div(a.max_kv, tile) + 1);
     LQ_REQUIRE(ctx, steps < (1ll << 26), "lq_prefix_attention: %lld steps, more than a launch can number", (long long)steps);
     p->sp = (int)(items_p * p->np);
     // a segment costs about one more step than its tiles (Q, the masked tile, the store): counted
@@ -281,7 +290,7 @@ static int launch_merge(lq_ctx* ctx, const PrefixAttnArgs& a, const PagedSeqs& s
     // a row of few heads leaves most of a 32-row CTA idle
     const int mr = p.cap[1] <= 8 ? 8 : 32;
     const int64_t R = (int64_t)s.rows * a.group;
-    const dim3 grid((unsigned)(a.prefix_len > 0 ? a.n_kv * (R / p.ob + s.n_seqs) : (p.pair_o ? 1 : 2) * p.workers),
+    const dim3 grid((unsigned)(p.np > 0 ? a.n_kv * (R / p.ob + s.n_seqs) : (p.pair_o ? 1 : 2) * p.workers),
                     (unsigned)ceil_div(p.cap[1], mr));
     return mr == 8 ? launch_kernel(ctx, prefix_attn_merge_kernel<T, D, 8>, grid, dim3(256), 0, "prefix_attn_merge", a, s, p)
                    : launch_kernel(ctx, prefix_attn_merge_kernel<T, D, 32>, grid, dim3(256), 0, "prefix_attn_merge", a, s, p);

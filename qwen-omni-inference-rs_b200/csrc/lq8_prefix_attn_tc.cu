@@ -53,7 +53,7 @@ struct alignas(16) PaSeg {
     int n;          // rows of the flow (0: it sits this segment out, round by round)
     int flags;
     int kh, b;      // kv head; sequence (own items)
-    int kv_end;     // positions the item sees
+    int kv_end;     // positions the item sees (own items: from the chain's first tile on)
     int row0;       // first stacked row
     int voff;       // own items: the stacked row of token t sees t + voff positions
     int slot;       // slot of the partial
@@ -289,6 +289,9 @@ prefix_attn_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_co
     const int so = c.scan[n_entries];
     if (blockIdx.x == 0 && tid == 0) *g.p.own_steps = so;  // for the merge
     const int me = blockIdx.x;
+    // own items count positions from the first tile of the prefix they begin with, whose last tile
+    // may be partly empty
+    const int chain = PO ? g.p.chain : 0;
     // a warp's place in the segments of a flow
     struct Feed {
         int i = 0, n = 0;   // entry of the batch, entries
@@ -380,7 +383,7 @@ prefix_attn_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_co
             const int my_row = few ? lane : row;
             const int st = sg.row0 + min(my_row, sg.n - 1), tok = g.a.group_div(st);
             const bool mine = my_row < sg.n, busy = few || wq * 32 < sg.n;
-            const int vis = sg.flags & SEG_OWN ? max(0, tok + sg.voff) : sg.kv_end;
+            const int vis = sg.flags & SEG_OWN ? chain * PA_TILE + max(0, tok + sg.voff) : sg.kv_end;
             float m = -INFINITY, l = 0.0f;
             int t = sg.t0;
 #pragma unroll 1
@@ -389,7 +392,7 @@ prefix_attn_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_co
                 s_ph ^= 1;
                 tc_after();
                 if (busy) {
-                    const int lim = vis - t * PA_TILE;  // columns this row sees
+                    const int lim = (t < chain ? g.a.prefix_len : vis) - t * PA_TILE;  // columns this row sees
                     // a larger maximum: when a row's grew by more than 2^8, l and O follow
                     auto raise = [&](float mt) {
                         mt *= cs;
@@ -659,11 +662,11 @@ prefix_attn_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_co
                 }
                 const int t = cur.sg.t0++;
                 if (cur.sg.n == 0 || (f == 1 && (cur.sg.flags & SEG_PAIRED))) break;
-                const int pos = t * PA_TILE + lane * box;
+                const bool own = (cur.sg.flags & SEG_OWN) && t >= chain;
+                const int pos = (own ? t - chain : t) * PA_TILE + lane * box;
                 int id = g.s.n_pages;  // out of range: zeros
-                if (lane < boxes && pos < cur.sg.kv_end) {
-                    const int32_t* const table = cur.sg.flags & SEG_OWN ? g.s.table + (int64_t)cur.sg.b * g.s.table_ld
-                                                                        : g.a.prefix_table;
+                if (lane < boxes && pos < (own ? cur.sg.kv_end - chain * PA_TILE : g.a.prefix_len)) {
+                    const int32_t* const table = own ? g.s.table + (int64_t)cur.sg.b * g.s.table_ld : g.a.prefix_table;
                     id = table[pos >> g.s.page_shift];
                     if ((unsigned)id >= (unsigned)g.s.n_pages) {
                         flag_error(err, ERR_PAGE_ID, id);
@@ -782,7 +785,7 @@ prefix_attn_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_co
                     cur.pv = true;
                     cur.pv_shared = shared;
                     cur.pv_last = cur.sg.t0 == cur.sg.t1;
-                    cur.pv_valid = min(PA_TILE, cur.sg.kv_end - t * PA_TILE);
+                    cur.pv_valid = min(PA_TILE, (t < chain ? g.a.prefix_len : cur.sg.kv_end) - t * PA_TILE);
                 }
             }
             exchange(cur, oth);
@@ -817,7 +820,7 @@ prefix_attn_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_co
                 }
             };
             PaSeg o{0, 1, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0};
-            if (g.a.prefix_len == 0 && lane < (PO ? 1 : 2)) g.p.split[PO ? me : 2 * me + lane].rows = 0;
+            if (g.p.np == 0 && lane < (PO ? 1 : 2)) g.p.split[PO ? me : 2 * me + lane].rows = 0;
             __syncwarp();
             auto part = [&](auto own_part) {
                 constexpr bool own = decltype(own_part)::value, paired = own ? PO : PP;
@@ -894,7 +897,7 @@ prefix_attn_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_co
                         rb = jj - kh * n_rb;
                     }
                     if (own && bb < g.s.n_seqs) {
-                        o.kv_end = os.visible(si, rb);
+                        o.kv_end = chain * PA_TILE + os.visible(si, rb);
                         nt = (o.kv_end + PA_TILE - 1) / PA_TILE;
                     }
                     const int ns = nt + (own && nt > 0 ? g.p.extra : 0);  // steps of the item
@@ -913,7 +916,7 @@ prefix_attn_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_co
                     o.n1 = paired ? max(0, min(PA_ROWS, rows - PA_ROWS)) : 0;
                     o.n = paired && f ? o.n1 : min(PA_ROWS, rows);
                     o.flags = (own ? SEG_OWN : 0) | (paired ? SEG_PAIRED : 0) | (paired && f ? SEG_HALF : 0) |
-                              (own && g.a.prefix_len == 0 && o.t0 == 0 && o.t1 == nt ? SEG_WHOLE : 0);
+                              (own && g.p.np == 0 && o.t0 == 0 && o.t1 == nt ? SEG_WHOLE : 0);
                     o.kh = kh;
                     o.b = bb;
                     const int first_row = (own ? si.q0 * g.a.group : 0) + rb * block;
@@ -924,7 +927,7 @@ prefix_attn_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_co
                     if (valid && !(paired && f)) {  // for the merge
                         if (o.t0 == 0) g.p.first[own][item] = worker;
                         if (o.t1 == nt) g.p.last[own][item] = worker;
-                        if (own && g.a.prefix_len == 0 && o.t0 == 0 && o.t1 < nt)
+                        if (own && g.p.np == 0 && o.t0 == 0 && o.t1 < nt)
                             g.p.split[worker] = SplitItem{min(rows, block), first_row, kh, item};
                     }
                     put(o, valid);

@@ -8,6 +8,10 @@
 // first, then the sequences' own, and every worker takes an equal share of it: no split factors,
 // no empty workers, whatever the mix of lengths. An item cut between workers leaves one partial
 // (o, m, l) per worker, which the merge kernel joins in order.
+//
+// Where the sequences bring many rows each (prompt chunks), stacking over sequences saves few
+// tiles, while two partials of every row would go through memory. There the prefix has no items of
+// its own: its tiles come first in each own item (chain of them).
 #pragma once
 
 #include "lq8_paged.cuh"
@@ -45,7 +49,8 @@ struct PrefixPlan {
     int pb, ob;                 // rows of a block: prefix items, own items
     int pair_p, pair_o;         // the two halves of a block run side by side in one worker (pb / ob = 2 halves)
     int n_rb;                   // row blocks of the prefix, per kv head
-    int np;                     // tiles of the prefix
+    int np;                     // tiles of a prefix item (0: there are none)
+    int chain;                  // tiles of the prefix at the front of every own item
     int sp;                     // steps of the prefix
     int extra;                  // steps that an own item counts for beside its tiles
     int workers;                // CTAs that share the line
@@ -91,12 +96,12 @@ struct OwnSteps {
     const PrefixAttnArgs& a;
     const PrefixPlan& p;
     __device__ __forceinline__ int blocks(const SeqInfo& i) const { return (i.q * a.group + p.ob - 1) / p.ob; }
-    // own positions that row block rb sees (those of its last row), and its tiles
+    // own positions that row block rb sees (those of its last row), and its tiles (the chain's too)
     __device__ __forceinline__ int visible(const SeqInfo& i, int rb) const {
         return own_visible(i, a.group_div(min(i.q * a.group, (rb + 1) * p.ob) - 1));
     }
     __device__ __forceinline__ int tiles(const SeqInfo& i, int rb) const {
-        return (visible(i, rb) + p.tile - 1) / p.tile;
+        return p.chain + (visible(i, rb) + p.tile - 1) / p.tile;
     }
     // what the block counts for on the line: its tiles, and p.extra for the segment's beginning and
     // end (after the tiles; a worker whose share has nothing else of the block leaves it alone)
