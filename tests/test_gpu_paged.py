@@ -388,6 +388,22 @@ def test_attention_long(ctx, lq8_lib, dtype, kv, q, Hq, Hkv, D, page, prefix):
 
 
 @pytest.mark.parametrize("dtype", ["bf16", "f32"])
+@pytest.mark.parametrize("kv,q,Hq,Hkv,D,page,prefix", [
+    # a chunk next to many decode rows: the prefix keeps blocks over all sequences
+    ([200] + [3] * 39, [200] + [1] * 39, 32, 8, 128, 16, 2000),
+    ([70, 1, 300, 0, 50] * 6, [70, 1, 40, 2, 1] * 6, 28, 4, 64, 32, 1500),
+    # chunks of whole blocks: each takes the prefix and its own positions in one go
+    ([600, 300], [600, 300], 16, 2, 128, 256, 129),
+    ([700, 64, 900], [513, 64, 200], 32, 4, 64, 256, 640),
+    ([0, 513, 40], [300, 513, 100], 8, 1, 128, 8, 255),      # rows before their first own position
+    ([2000], [256], 64, 8, 128, 64, 4097),
+    ([33], [33], 96, 1, 128, 128, 1),
+])
+def test_attention_chunks_behind_a_prefix(ctx, lq8_lib, dtype, kv, q, Hq, Hkv, D, page, prefix):
+    attention_case(ctx, lq8_lib, dtype, kv, q, Hq, Hkv, D, page, prefix)
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "f32"])
 @pytest.mark.parametrize("qscale", [0.0, 40.0])
 def test_attention_flat_and_sharp(ctx, lq8_lib, dtype, qscale):
     """Equal probabilities, and scores in the hundreds whose maximum moves from tile to tile
