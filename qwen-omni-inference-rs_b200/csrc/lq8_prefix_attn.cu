@@ -17,7 +17,8 @@ namespace lq {
 // head), which share the own item's partials and, but for a block's end, those of a prefix item.
 // Without prefix items only the items that are cut between workers are left: a worker leaves a note of
 // the one that it begins. A thread adds up CH MR / 256 vectors of four dims of one row; rows lie
-// next to each other in memory.
+// next to each other in memory. Bound: latency (launch, lengths, maxima, vectors): 10 us for 64
+// sequences, 16 us for 128 behind 32768 positions (9 MB of partials).
 // =========================================================================================
 constexpr int MERGE_CHUNK = 32;   // partials looked at together
 

@@ -15,12 +15,20 @@
 // Warps 0-3: softmax of flow 0 (TMEM lane = row = thread); warps 4-7: flow 1; warp 8: TMA
 // producer, which reads the page table and brings K and V tiles page by page into a ring of 32 KB
 // stages (128-byte swizzle; pages past the end come as zeros from an out-of-range coordinate);
-// warp 9: TMEM allocator and MMA issuer; warp 11: zeros for rows that see nothing; warp 10: scheduler, the only one that walks the line: it
-// hands each flow its segments (PaSeg) through a small ring, so the other roles' code stays short
-// (every role walking by itself came to 300 KB of code, and the instruction misses took ten times
-// the arithmetic). Per round the MMA warp issues, for each flow, P V of the round before and then
+// warp 9: TMEM allocator and MMA issuer; warp 11: zeros for rows that see nothing; warp 10:
+// scheduler, the only one that walks the line: it hands each flow its segments (PaSeg) through a
+// small ring, so the other roles' code stays short (every role walking by itself came to 300 KB of
+// code, and the instruction misses took ten times the arithmetic). Per round the MMA warp issues,
+// for each flow, P V of the round before and then
 // Q K of this one: the tensor pipe works for one flow while the other is in its softmax. Every
 // wait is bounded; a timeout sets the error flag and the CTA tears down.
+//
+// Bound: a round of two 128-row halves at D = 128 needs 2048 cycles of the tensor pipe and as many
+// of the exponentials'; it takes 3550, of which the MMA warp issues for 2880 (QK reads both operands
+// from shared memory at its full rate: 86 cycles an MMA instead of 64) and waits 670 for copies and
+// P. 128 sequences of 64 heads behind 32768 positions: 170 us for the prefix (804 TFLOP/s), 200 us
+// with 1000 own positions; 64 sequences of 32 heads behind 8191: 51 us (3.3 TB/s); 4 chunks of 1000
+// tokens behind 8192: 480 us (1030 TFLOP/s), all from cold L2, the merge in the first and last.
 //
 // TMA loads here read only this GPU's memory and use no multicast.
 #include "lq8_async.cuh"
