@@ -150,8 +150,8 @@ __device__ __forceinline__ void tmem_wait_ld() { asm volatile("tcgen05.wait::ld.
 __device__ __forceinline__ void tmem_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 
 // Bounded wait: PA_POLLS polls (try_wait sleeps between them), or until another warp of the CTA
-// gave up; then the CTA tears down and reports. The flag is looked at first: with the poll first,
-// 128 sequences behind 32768 positions took 212 us instead of 202.
+// gave up; then the CTA tears down and reports. A softmax thread looks at the flag first: with the
+// poll first, 128 sequences behind 32768 positions took 212 us instead of 202.
 constexpr int PA_POLLS = 1 << 22;
 __device__ __forceinline__ bool pa_wait(PaCtl& c, uint64_t* bar, unsigned parity) {
 #pragma unroll 1
@@ -162,11 +162,13 @@ __device__ __forceinline__ bool pa_wait(PaCtl& c, uint64_t* bar, unsigned parity
 }
 // The same by a whole warp, whose control flow the vote keeps uniform: tcgen05.mma and TMA take
 // their operands from uniform registers, and moving them there lane by lane made the issue of an
-// MMA cost twice its execution.
+// MMA cost twice its execution. These poll first (202 -> 200 us, a chunk of 2048 tokens 222 -> 218).
 __device__ __forceinline__ bool pa_wait_warp(PaCtl& c, uint64_t* bar, unsigned parity) {
 #pragma unroll 1
-    for (int i = 0; i < PA_POLLS && !__any_sync(0xffffffffu, *reinterpret_cast<volatile int*>(&c.abort)); i++)
+    for (int i = 0; i < PA_POLLS; i++) {
         if (__all_sync(0xffffffffu, mbar_try_wait(bar, parity))) return true;
+        if (__any_sync(0xffffffffu, *reinterpret_cast<volatile int*>(&c.abort))) break;
+    }
     *reinterpret_cast<volatile int*>(&c.abort) = 1;
     return false;
 }
