@@ -109,7 +109,7 @@ __global__ void __launch_bounds__(256, MR == 32 ? 5 : 4) prefix_attn_merge_kerne
                             flow_range(line, paired, paired ? v : v >> 1, paired ? 0 : v & 1, part, lo, hi);
                             has = lo < hi;
                         }
-                        slot[tid] = has ? item[part] + v : -1;
+                        slot[tid] = !has ? -1 : part ? p.own_slot(item[1], v, k == 0) : item[0] + v;
                     } else if (tid < MERGE_CHUNK) {
                         slot[tid] = -1;
                     }
@@ -266,7 +266,7 @@ static int make_plan(lq_ctx* ctx, const PrefixAttnArgs& a, const PagedSeqs& s, b
     const size_t steps_at = place(1, 4), split_at = place(2 * p->workers, sizeof(SplitItem));
     size_t first_at[2], last_at[2], ml_at[2], o_at[2];
     for (int k = 0; k < 2; k++) {
-        const int64_t slots = items[k] ? items[k] + 2 * p->workers : 0;
+        const int64_t slots = k == 1 && p->np == 0 ? 4 * p->workers : items[k] ? items[k] + 2 * p->workers : 0;
         LQ_REQUIRE(ctx, slots < (1ll << 31), "lq_prefix_attention: too many partials");
         first_at[k] = place(items[k], 4);
         last_at[k] = place(items[k], 4);

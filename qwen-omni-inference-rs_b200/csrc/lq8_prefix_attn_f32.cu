@@ -200,7 +200,7 @@ prefix_attn_f32_kernel(const __grid_constant__ PrefixAttnArgs a, const __grid_co
             const int row0 = (own ? si.q0 * a.group : 0) + rb * p.pb;
             const int n = min(p.pb, (own ? si.q : s.rows) * a.group - rb * p.pb);
             const int item = (own ? a.n_kv * os.base(si, b) : 0) + kh * n_rb + rb;
-            const bool whole = a.prefix_len == 0 && tile == 0 && end == nt;
+            const bool begins = tile == 0, whole = a.prefix_len == 0 && begins && end == nt;
             if (lane == 0) {
                 if (tile == 0) p.first[part][item] = worker;
                 if (end == nt) p.last[part][item] = worker;
@@ -383,7 +383,7 @@ prefix_attn_f32_kernel(const __grid_constant__ PrefixAttnArgs a, const __grid_co
                 const bool real = r < n;
                 int tok, head;
                 row_of(min(r, n - 1), tok, head);
-                const int64_t slot = item + worker;
+                const int64_t slot = own ? p.own_slot(item, worker, begins) : item + worker;
                 const int cap = p.cap[part];
                 if (real && !whole && g == 0) p.ml[part][slot * cap + r] = make_float2(m[k], l[k]);
                 const float inv = l[k] > 0.0f ? 1.0f / l[k] : l[k];

@@ -932,7 +932,7 @@ prefix_attn_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_co
                     const int first_row = (own ? si.q0 * g.a.group : 0) + rb * block;
                     o.row0 = first_row + (paired && f ? PA_ROWS : 0);
                     o.voff = own ? si.kv - si.q + 1 - si.q0 : 0;
-                    o.slot = item + worker;
+                    o.slot = own ? g.p.own_slot(item, worker, o.t0 == 0) : item + worker;
                     const bool valid = go && n > 0;
                     if (valid && !(paired && f)) {  // for the merge
                         if (o.t0 == 0) g.p.first[own][item] = worker;

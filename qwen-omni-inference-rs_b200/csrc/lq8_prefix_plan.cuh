@@ -62,6 +62,11 @@ struct PrefixPlan {
     SplitItem* split;           // per worker, without a prefix: the cut item it begins
     float* o[2];                // partials, unnormalised: [slot][D/4][cap] of four dims
     float2* ml[2];              // [slot][cap]: running maximum (log2 units) and sum
+    // Where a worker's piece of an own item goes. Without prefix items only cut items leave partials:
+    // a worker has one piece at most of an item that it begins and one of an item begun before it.
+    __device__ __forceinline__ int own_slot(int item, int worker, bool begins) const {
+        return np > 0 ? item + worker : 2 * worker + (begins ? 1 : 0);
+    }
 };
 
 // a sequence's rows and own length, with what the call's bounds do not hold taken out
