@@ -220,42 +220,12 @@ __global__ void __launch_bounds__(256, MR == 32 ? 5 : 4) prefix_attn_merge_kerne
     }
 }
 
-// The plan of a call and its workspace. Sizes come from the call's bounds; what the lengths really
-// are, the kernels read.
+// the plan of a call and its workspace
 static int make_plan(lq_ctx* ctx, const PrefixAttnArgs& a, const PagedSeqs& s, bool f32, int D, PrefixPlan* p) {
-    const int64_t R = (int64_t)s.rows * a.group, most_q = std::min<int64_t>((int64_t)a.max_q, s.rows) * a.group;
-    // bf16: blocks of 128 rows, or two halves of 128 that share their K and V tiles; a worker is a
-    // CTA with paired halves, else one of its two flows. f32: blocks of 8 rows, a worker is a warp.
-    const int half = f32 ? 8 : 128, tile = f32 ? 32 : 128;
-    p->tile = tile;
-    p->pair_p = f32 || R > half;
-    p->pair_o = f32 || most_q > half;
-    p->pb = f32 ? half : p->pair_p ? 2 * half : half;
-    p->ob = f32 ? half : p->pair_o ? 2 * half : half;
-    p->cap[0] = (int)std::min<int64_t>(p->pb, R);
-    p->cap[1] = (int)std::min<int64_t>(p->ob, most_q);
-    p->n_rb = ceil_div(R, p->pb);
-    p->np = ceil_div(a.prefix_len, tile);
-    // The prefix's tiles at the front of the own items: that costs at most n_seqs - 1 blocks more of
-    // np steps each, and saves a block's two partials and their merge, about as long as 9 steps
-    // (a chunk of 2048 tokens behind 2048 positions: 273 us apart, 222 in one line; ten ragged ones behind
-    // 2049: 146 and 136).
-    p->chain = 0;
-    if (!f32 && p->pair_o && (s.n_seqs - 1) * (int64_t)p->np <= 9 * (R / p->pb) &&
-        (int64_t)a.prefix_len + a.max_kv < (1 << 30)) {
-        p->chain = p->np;
-        p->np = 0;
-    }
-    const int64_t items_p = (int64_t)a.n_kv * p->n_rb, items_o = a.n_kv * (R / p->ob + s.n_seqs + 1);
-    const int64_t steps = items_p * p->np + items_o * (p->chain + ceil_div(a.max_kv, tile) + 1);
-    LQ_REQUIRE(ctx, steps < (1ll << 26), "lq_prefix_attention: %lld steps, more than a launch can number", (long long)steps);
-    p->sp = (int)(items_p * p->np);
-    // a segment costs about one more step than its tiles (Q, the masked tile, the store): counted
-    // so, short causal items next to a long prefix no longer hold up the last CTAs (a batch of 10
-    // prompt chunks: 152 -> 114 us)
-    p->extra = f32 ? 0 : 1;
-    p->workers = (int)std::max<int64_t>(1, std::min<int64_t>(ctx->sm_count * (f32 ? PREFIX_ATTN_F32_WARPS : 1), steps));
-    p->workers_mul = ((1ull << 40) + p->workers - 1) / p->workers;
+    const int64_t steps = plan_cut(a, s, f32, ctx->sm_count, p);
+    LQ_REQUIRE(ctx, steps < PREFIX_MAX_STEPS, "lq_prefix_attention: %lld steps, more than a launch can number", (long long)steps);
+    const int64_t items_p = (int64_t)a.n_kv * p->n_rb;
+    const int64_t items_o = a.n_kv * ((int64_t)s.rows * a.group / p->ob + s.n_seqs + 1);
     const int64_t items[2] = {p->np ? items_p : 0, items_o};
     size_t at = 0;
     auto place = [&at](int64_t n, size_t size) {

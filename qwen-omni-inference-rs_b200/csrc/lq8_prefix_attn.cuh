@@ -87,7 +87,6 @@ __device__ __forceinline__ void zero_rows(const PrefixAttnArgs& a, int tok0, int
         }
 }
 
-constexpr int PREFIX_ATTN_F32_WARPS = 8;  // workers of a CTA of the f32 kernel
 int launch_prefix_attn_f32(lq_ctx* ctx, const PrefixAttnArgs& a, const PagedSeqs& s, const PrefixPlan& p, int D);
 int launch_prefix_attn_tc(lq_ctx* ctx, const PrefixAttnArgs& a, const PagedSeqs& s, const PrefixPlan& p, int D);
 

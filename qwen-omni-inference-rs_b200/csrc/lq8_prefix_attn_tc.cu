@@ -879,14 +879,21 @@ prefix_attn_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_co
                         j = j * n_rb + rb;
                     }
                 }
-                bool both = true;
+                bool first = true;
                 while (ok && __any_sync(0xffffffffu, step < hi)) {
-                    // flows apart: both get a first batch, then the one with fewer rounds to go on
-                    // with (waiting for the other's could wait for this one)
-                    const int r0 = __shfl_sync(0xffffffffu, step < hi ? rounds : 0x7fffffff, 0);
-                    const int r1 = __shfl_sync(0xffffffffu, step < hi ? rounds : 0x7fffffff, 16);
-                    const bool go = step < hi && (paired || both || f == (r0 <= r1 ? 0 : 1));
-                    both = false;
+                    bool go = step < hi;
+                    if constexpr (!paired) {
+                        const int others = __shfl_xor_sync(0xffffffffu, rounds, 16);
+                        const bool other_live = __shfl_xor_sync(0xffffffffu, (int)go, 16);
+                        const HandOut turn = hand_out(f, first, go, other_live, rounds, others);
+                        go = turn.go;
+                        if (__any_sync(0xffffffffu, turn.idle > 0)) {
+                            o = PaSeg{0, turn.idle, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0};
+                            put(o, hl == 0 && turn.idle > 0);
+                            rounds += turn.idle;
+                        }
+                    }
+                    first = false;
                     // a lane looks at the hl-th item from here on
                     int jj = j + hl, bb = b, n_rb = own ? 1 : g.p.n_rb, nt = g.p.np;
                     SeqInfo si{0, g.s.rows, 0};

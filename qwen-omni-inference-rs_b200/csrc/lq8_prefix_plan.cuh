@@ -14,6 +14,8 @@
 // its own: its tiles come first in each own item (chain of them).
 #pragma once
 
+#include <algorithm>
+
 #include "lq8_paged.cuh"
 
 namespace lq {
@@ -95,26 +97,26 @@ __device__ __forceinline__ SeqInfo seq_info(const PrefixAttnArgs& a, const Paged
 }
 
 // own positions that token j of the sequence's q sees
-__device__ __forceinline__ int own_visible(const SeqInfo& i, int j) { return max(0, i.kv - i.q + j + 1); }
+__host__ __device__ __forceinline__ int own_visible(const SeqInfo& i, int j) { return max(0, i.kv - i.q + j + 1); }
 
 struct OwnSteps {
     const PrefixAttnArgs& a;
     const PrefixPlan& p;
-    __device__ __forceinline__ int blocks(const SeqInfo& i) const { return (i.q * a.group + p.ob - 1) / p.ob; }
+    __host__ __device__ __forceinline__ int blocks(const SeqInfo& i) const { return (i.q * a.group + p.ob - 1) / p.ob; }
     // own positions that row block rb sees (those of its last row), and its tiles (the chain's too)
-    __device__ __forceinline__ int visible(const SeqInfo& i, int rb) const {
+    __host__ __device__ __forceinline__ int visible(const SeqInfo& i, int rb) const {
         return own_visible(i, a.group_div(min(i.q * a.group, (rb + 1) * p.ob) - 1));
     }
-    __device__ __forceinline__ int tiles(const SeqInfo& i, int rb) const {
+    __host__ __device__ __forceinline__ int tiles(const SeqInfo& i, int rb) const {
         return p.chain + (visible(i, rb) + p.tile - 1) / p.tile;
     }
     // what the block counts for on the line: its tiles, and p.extra for the segment's beginning and
     // end (after the tiles; a worker whose share has nothing else of the block leaves it alone)
-    __device__ __forceinline__ int steps(const SeqInfo& i, int rb) const {
+    __host__ __device__ __forceinline__ int steps(const SeqInfo& i, int rb) const {
         const int n = tiles(i, rb);
         return n > 0 ? n + p.extra : 0;
     }
-    __device__ __forceinline__ int per_head(const SeqInfo& i) const {
+    __host__ __device__ __forceinline__ int per_head(const SeqInfo& i) const {
         int n = 0;
 #pragma unroll 1
         for (int rb = blocks(i) - 1; rb >= 0; rb--) n += steps(i, rb);
@@ -122,7 +124,7 @@ struct OwnSteps {
     }
     // numbers a sequence's row blocks from here on; blocks(i) <= base(next) - base(i), so that no
     // scan over the sequences is needed
-    __device__ __forceinline__ int base(const SeqInfo& i, int b) const { return i.q0 * a.group / p.ob + b; }
+    __host__ __device__ __forceinline__ int base(const SeqInfo& i, int b) const { return i.q0 * a.group / p.ob + b; }
 };
 
 // A step of a paired block weighs 3, one that a flow takes alone 2 (measured: a round of two
@@ -134,7 +136,7 @@ struct Line {
     bool pair_p, pair_o;
     int quot, rem;     // W / n
     uint64_t mul;      // ceil(2^40 / n): x / n = x mul / 2^40, exact for x < 2^32
-    __device__ __forceinline__ Line(const PrefixPlan& p, int own_steps, bool pair_prefix, bool pair_own)
+    __host__ __device__ __forceinline__ Line(const PrefixPlan& p, int own_steps, bool pair_prefix, bool pair_own)
         : sp(p.sp), so(own_steps), n(p.workers), pair_p(pair_prefix), pair_o(pair_own), mul(p.workers_mul) {
         split = sp * (pair_p ? 3 : 2);
         w = split + so * (pair_o ? 3 : 2);
@@ -142,8 +144,8 @@ struct Line {
         rem = w - quot * n;
     }
     // floor(W c / n)
-    __device__ __forceinline__ int start(int c) const { return quot * c + (int)(((uint64_t)(rem * c) * mul) >> 40); }
-    __device__ __forceinline__ int first(int c, bool own) const {
+    __host__ __device__ __forceinline__ int start(int c) const { return quot * c + (int)(((uint64_t)(rem * c) * mul) >> 40); }
+    __host__ __device__ __forceinline__ int first(int c, bool own) const {
         const int x = own ? max(start(c) - split, 0) : start(c);
         return min((own ? pair_o : pair_p) ? (x + 2) / 3 : (x + 1) / 2, own ? so : sp);
     }
@@ -151,7 +153,7 @@ struct Line {
 
 // [lo, hi) of CTA c's flow f: both halves of a paired block run the same steps, otherwise the
 // flows take one half of the steps each
-__device__ __forceinline__ void flow_range(const Line& l, bool paired, int c, int f, bool own, int& lo, int& hi) {
+__host__ __device__ __forceinline__ void flow_range(const Line& l, bool paired, int c, int f, bool own, int& lo, int& hi) {
     lo = l.first(c, own);
     hi = l.first(c + 1, own);
     if (!paired) {
@@ -159,6 +161,62 @@ __device__ __forceinline__ void flow_range(const Line& l, bool paired, int c, in
         if (f == 0) hi = mid;
         else lo = mid;
     }
+}
+
+// What a flow of a CTA gets next in a part whose flows are apart: a batch of its items (go), or
+// `idle` rounds without work. The warps that serve the flows take a round of each in turn, and a
+// flow's batch is only taken back when they have begun its next one. So a batch goes to the flow
+// with fewer rounds, and a flow that ran out of steps is given the rounds that it lacks before the
+// other one gets more: else those warps would wait for it, and the scheduler for them. `mine` and
+// `other`: rounds that the flows were given; live: steps left.
+struct HandOut {
+    bool go;
+    int idle;
+};
+__host__ __device__ __forceinline__ HandOut hand_out(int f, bool first, bool live, bool other_live, int mine, int other) {
+    return HandOut{live && (first || !other_live || mine < other || (mine == other && f == 0)),
+                   !live && other_live && mine < other ? other - mine : 0};
+}
+
+// host: cuts a call's work for sm_count SMs, from the bounds that the call gives (what the lengths
+// really are, the kernels read); the most steps that there can be, to be checked against
+// PREFIX_MAX_STEPS before the plan is used
+constexpr int64_t PREFIX_MAX_STEPS = 1ll << 26;
+constexpr int PREFIX_ATTN_F32_WARPS = 8;  // workers of a CTA of the f32 kernel
+inline int64_t plan_cut(const PrefixAttnArgs& a, const PagedSeqs& s, bool f32, int sm_count, PrefixPlan* p) {
+    const int64_t R = (int64_t)s.rows * a.group, most_q = std::min<int64_t>((int64_t)a.max_q, s.rows) * a.group;
+    // bf16: blocks of 128 rows, or two halves of 128 that share their K and V tiles; a worker is a
+    // CTA with paired halves, else one of its two flows. f32: blocks of 8 rows, a worker is a warp.
+    const int half = f32 ? 8 : 128, tile = f32 ? 32 : 128;
+    p->tile = tile;
+    p->pair_p = f32 || R > half;
+    p->pair_o = f32 || most_q > half;
+    p->pb = f32 ? half : p->pair_p ? 2 * half : half;
+    p->ob = f32 ? half : p->pair_o ? 2 * half : half;
+    p->cap[0] = (int)std::min<int64_t>(p->pb, R);
+    p->cap[1] = (int)std::min<int64_t>(p->ob, most_q);
+    p->n_rb = ceil_div(R, p->pb);
+    p->np = ceil_div(a.prefix_len, tile);
+    // The prefix's tiles at the front of the own items: that costs at most n_seqs - 1 blocks more of
+    // np steps each, and saves a block's two partials and their merge, about as long as 9 steps
+    // (a chunk of 2048 tokens behind 2048 positions: 273 us apart, 222 in one line; ten ragged ones behind
+    // 2049: 146 and 136).
+    p->chain = 0;
+    if (!f32 && p->pair_o && (s.n_seqs - 1) * (int64_t)p->np <= 9 * (R / p->pb) &&
+        (int64_t)a.prefix_len + a.max_kv < (1 << 30)) {
+        p->chain = p->np;
+        p->np = 0;
+    }
+    const int64_t items_p = (int64_t)a.n_kv * p->n_rb, items_o = a.n_kv * (R / p->ob + s.n_seqs + 1);
+    const int64_t steps = items_p * p->np + items_o * (p->chain + ceil_div(a.max_kv, tile) + 1);
+    p->sp = (int)(items_p * p->np);
+    // a segment costs about one more step than its tiles (Q, the masked tile, the store): counted
+    // so, short causal items next to a long prefix no longer hold up the last CTAs (a batch of 10
+    // prompt chunks: 152 -> 114 us)
+    p->extra = f32 ? 0 : 1;
+    p->workers = (int)std::max<int64_t>(1, std::min<int64_t>(sm_count * (f32 ? PREFIX_ATTN_F32_WARPS : 1), steps));
+    p->workers_mul = ((1ull << 40) + p->workers - 1) / p->workers;
+    return steps;
 }
 
 }  // namespace lq
