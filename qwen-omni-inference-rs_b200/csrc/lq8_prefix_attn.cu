@@ -74,18 +74,19 @@ __global__ void __launch_bounds__(256, MR == 32 ? 5 : 4) prefix_attn_merge_kerne
 #pragma unroll 1
     while (todo > 0) {
         int run = todo, item[2] = {0, own_item}, in[2] = {0, own_in}, v0[2] = {0, 0}, cnt[2] = {0, 0};
+        auto workers_of = [&](int k) {  // (within bounds, even where a kernel that gave up left them unwritten)
+            const int most = 2 * p.workers - 1;
+            v0[k] = min(max(p.first[k][item[k]], 0), most);
+            cnt[k] = min(max(p.last[k][item[k]], 0), most) - v0[k] + 1;
+        };
         if (with_prefix) {  // rows that share the prefix item
             const int rb = st0 / p.pb;
             item[0] = kh * p.n_rb + rb;
             in[0] = st0 - rb * p.pb;
             run = min(run, p.pb - in[0]);
-            v0[0] = p.first[0][item[0]];
-            cnt[0] = p.last[0][item[0]] - v0[0] + 1;
+            workers_of(0);
         }
-        if (own) {
-            v0[1] = p.first[1][item[1]];
-            cnt[1] = p.last[1][item[1]] - v0[1] + 1;
-        }
+        if (own) workers_of(1);
         const int n = cnt[0] + cnt[1];
         const bool mine = r < run;
         // pass 0: the rows' maxima and sums; pass 1: the vectors
@@ -224,6 +225,9 @@ __global__ void __launch_bounds__(256, MR == 32 ? 5 : 4) prefix_attn_merge_kerne
 static int make_plan(lq_ctx* ctx, const PrefixAttnArgs& a, const PagedSeqs& s, bool f32, int D, PrefixPlan* p) {
     const int64_t steps = plan_cut(a, s, f32, ctx->sm_count, p);
     LQ_REQUIRE(ctx, steps < PREFIX_MAX_STEPS, "lq_prefix_attention: %lld steps, more than a launch can number", (long long)steps);
+    // LQ_FAULT=prefix_attn_wait: waits inside the kernel run out (tests of what follows then)
+    p->hold = fault_injected("prefix_attn_wait");
+    p->polls = p->hold ? 1 << 12 : 1 << 22;
     const int64_t items_p = (int64_t)a.n_kv * p->n_rb;
     const int64_t items_o = a.n_kv * ((int64_t)s.rows * a.group / p->ob + s.n_seqs + 1);
     const int64_t items[2] = {p->np ? items_p : 0, items_o};

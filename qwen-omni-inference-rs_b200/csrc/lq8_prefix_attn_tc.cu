@@ -21,7 +21,9 @@
 // code, and the instruction misses took ten times the arithmetic). Per round the MMA warp issues,
 // for each flow, P V of the round before and then
 // Q K of this one: the tensor pipe works for one flow while the other is in its softmax. Every
-// wait is bounded; a timeout sets the error flag and the CTA tears down.
+// wait is bounded by a number of polls (4 us each where nothing comes, so 16 s in all; the
+// tear-down's by 2 s); when one runs out, all warps of the CTA leave, its copies and MMAs in flight
+// are waited for, and the error flag is set.
 //
 // Bound: a round of two 128-row halves at D = 128 needs 2048 cycles of the tensor pipe and as many
 // of the exponentials'; it takes 3550, of which the MMA warp issues for 2880 (QK reads both operands
@@ -75,6 +77,8 @@ struct PaCtl {
     uint64_t q_full[2], s_full[2], p_full[2], o_full[2], done;
     uint32_t tmem;
     int abort;
+    int issued;     // copies that the producer started
+    int agreed[2];  // per flow: segments of few rows that its warps went on with, or -1
     int seg_n[2][2];
     PaSeg seg[2][2][PA_BATCH];
     float2 few_ml[2][4][PA_FEW];
@@ -149,23 +153,31 @@ __device__ __forceinline__ void tmem_st16(uint32_t addr, const uint32_t* r) {
 __device__ __forceinline__ void tmem_wait_ld() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
 __device__ __forceinline__ void tmem_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 
-// Bounded wait: PA_POLLS polls (try_wait sleeps between them), or until another warp of the CTA
-// gave up; then the CTA tears down and reports. A softmax thread looks at the flag first: with the
-// poll first, 128 sequences behind 32768 positions took 212 us instead of 202.
 constexpr int PA_POLLS = 1 << 22;
+// Bounded wait by a whole warp: PA_POLLS polls (try_wait sleeps between them), or until another warp
+// of the CTA gave up; then the CTA tears down and reports. Every lane polls for itself, and the
+// vote at the end has the warp go one way: a lane that went on alone would be missing in the
+// other's collective instructions. A softmax thread looks at the flag first: with the poll first, 128
+// sequences behind 32768 positions took 212 us instead of 202.
 __device__ __forceinline__ bool pa_wait(PaCtl& c, uint64_t* bar, unsigned parity) {
+    bool there = false;
 #pragma unroll 1
     for (int i = 0; i < PA_POLLS && !*reinterpret_cast<volatile int*>(&c.abort); i++)
-        if (mbar_try_wait(bar, parity)) return true;
+        if (mbar_try_wait(bar, parity)) {
+            there = true;
+            break;
+        }
+    if (__all_sync(0xffffffffu, there)) return true;
     *reinterpret_cast<volatile int*>(&c.abort) = 1;
     return false;
 }
 // The same by a whole warp, whose control flow the vote keeps uniform: tcgen05.mma and TMA take
 // their operands from uniform registers, and moving them there lane by lane made the issue of an
 // MMA cost twice its execution. These poll first (202 -> 200 us, a chunk of 2048 tokens 222 -> 218).
-__device__ __forceinline__ bool pa_wait_warp(PaCtl& c, uint64_t* bar, unsigned parity) {
+// Waits for segments have a limit from the call (a limit from there in every wait: 1 us more).
+__device__ __forceinline__ bool pa_wait_warp(PaCtl& c, uint64_t* bar, unsigned parity, int polls = PA_POLLS) {
 #pragma unroll 1
-    for (int i = 0; i < PA_POLLS; i++) {
+    for (int i = 0; i < polls; i++) {
         if (__all_sync(0xffffffffu, mbar_try_wait(bar, parity))) return true;
         if (__any_sync(0xffffffffu, *reinterpret_cast<volatile int*>(&c.abort))) break;
     }
@@ -244,13 +256,14 @@ prefix_attn_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_co
             mbar_init(&c.s_full[f], 1);
             mbar_init(&c.p_full[f], 4);
             mbar_init(&c.o_full[f], 1);
+            c.agreed[f] = 0;
             for (int i = 0; i < 2; i++) {
                 mbar_init(&c.seg_full[f][i], 1);
                 mbar_init(&c.seg_empty[f][i], 6);  // four softmax warps, producer, MMA issuer
             }
         }
         mbar_init(&c.done, 1);
-        c.abort = 0;
+        c.abort = c.issued = 0;
         mbar_fence_init();
     }
     if (warp == 8 && lane == 0) {
@@ -298,7 +311,7 @@ prefix_attn_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_co
     const uint32_t tmem = __shfl_sync(0xffffffffu, c.tmem, 0);
     const int so = c.scan[n_entries];
     if (blockIdx.x == 0 && tid == 0) *g.p.own_steps = so;  // for the merge
-    const int me = blockIdx.x;
+    const int me = blockIdx.x, polls = g.p.polls;
     // own items count positions from the first tile of the prefix they begin with, whose last tile
     // may be partly empty
     const int chain = PO ? g.p.chain : 0;
@@ -313,7 +326,7 @@ prefix_attn_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_co
                 __syncwarp();
                 if (lane == 0) mbar_arrive(&c.seg_empty[f][(d.k - 1) & 1]);
             }
-            if (!pa_wait_warp(c, &c.seg_full[f][d.k & 1], (d.k >> 1) & 1u)) return false;
+            if (!pa_wait_warp(c, &c.seg_full[f][d.k & 1], (d.k >> 1) & 1u, polls)) return false;
             d.n = __shfl_sync(0xffffffffu, c.seg_n[f][d.k & 1], 0);
             d.i = 0;
             d.k++;
@@ -344,6 +357,7 @@ prefix_attn_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_co
         const uint32_t t_s = tmem + t_lane + f * 128, t_o = tmem + t_lane + 256 + f * 128;
         const float cs = g.a.scale * 1.44269504088896340736f;  // scores in units of log2
         unsigned s_ph = 0, o_ph = 0, turn = 0;
+        int joint = 0;  // segments of few rows
         Feed feed;
 
         // The next segment with rows: NX_NONE when there is none (or a wait ran out). Looked for
@@ -543,7 +557,18 @@ prefix_attn_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_co
                 if (!early) q_start();  // this segment's Q has been read: its last S was complete
                 q_finish();
             }
-            if (!pa_wait(c, &c.o_full[f], o_ph)) break;
+            bool there = pa_wait(c, &c.o_full[f], o_ph);
+            if (few) {
+                // The flow's warps meet below, so that all of them go on or none: the first one to
+                // know decides. One that saw O complete knows that the others come here (all have
+                // delivered their last P); one that gave up follows it.
+                int was = 0;
+                if (lane == 0) was = atomicCAS(&c.agreed[f], joint, there ? joint + 1 : -1);
+                was = __shfl_sync(0xffffffffu, was, 0);
+                if (was != joint) there = was > joint && mbar_wait(&c.o_full[f], o_ph, PA_POLLS);
+                joint++;
+            }
+            if (!there) break;
             o_ph ^= 1;
             tc_after();
             if (!busy) continue;
@@ -625,6 +650,7 @@ prefix_attn_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_co
             }
             tc_before();
         }
+        asm volatile("cp.async.wait_all;" ::: "memory");  // (after a wait that ran out: Q of the next segment)
     } else if (warp == 8) {
         // ------------------------------ TMA producer ------------------------------
         asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(PA_REGS_LOW));
@@ -691,12 +717,7 @@ prefix_attn_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_co
             if (!ok) break;
             exchange(cur, oth);
         }
-        // no copy may still be landing when the CTA exits
-        if (!ok) {
-#pragma unroll 1
-            for (int i = max(0, issued - STAGES); i < issued; i++)
-                mbar_wait_ns(&c.full[i % STAGES], (unsigned)(i / STAGES) & 1u, 2000000000ull);
-        }
+        if (lane == 0) c.issued = issued;
     } else if (warp == 9) {
         // ------------------------------ MMA issuer ------------------------------
         asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(PA_REGS_LOW));
@@ -800,7 +821,7 @@ prefix_attn_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_co
             }
             exchange(cur, oth);
         }
-        if (lane == 0) tc_commit(&c.done);
+        if (elect_one()) tc_commit(&c.done);  // (by the thread that issued the MMAs)
         __syncwarp();
         if (!mbar_wait_ns(&c.done, 0, 2000000000ull)) c.abort = 1;
     } else {
@@ -812,6 +833,7 @@ prefix_attn_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_co
             const Line line(g.p, so, PP, PO);
             const int f = lane >> 4, hl = lane & 15;
             unsigned batch[2] = {0, 0};
+            const unsigned hold = g.p.hold ? me % 8 : ~0u;  // (fault injection: batches handed out)
             bool ok = true;
             // the next batch of the flows with `valid` lanes, in the order of the lanes
             auto put = [&](const PaSeg& o, bool valid) {
@@ -820,7 +842,7 @@ prefix_attn_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_co
                 for (int q = 0; q < 2; q++) {
                     const unsigned m = (all >> (16 * q)) & 0xffffu, k = batch[q];
                     if (!m || !ok) continue;
-                    ok = pa_wait_warp(c, &c.seg_empty[q][k & 1], ((k >> 1) & 1u) ^ 1u);
+                    ok = batch[0] + batch[1] < hold && pa_wait_warp(c, &c.seg_empty[q][k & 1], ((k >> 1) & 1u) ^ 1u, polls);
                     if (!ok) return;
                     if (valid && f == q) c.seg[q][k & 1][__popc(m & ((1u << hl) - 1))] = o;
                     if (lane == 0) c.seg_n[q][k & 1] = __popc(m);
@@ -987,7 +1009,15 @@ prefix_attn_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_co
     tc_before();
     __syncthreads();
     tc_after();
-    if (tid == 0 && c.abort) flag_error(err, ERR_PA_WAIT, me);
+    if (c.abort) {
+        if (tid == 0) flag_error(err, ERR_PA_WAIT, me);
+        // no copy may still be landing when the CTA exits
+        if (warp == 8) {
+#pragma unroll 1
+            for (int i = max(0, c.issued - STAGES); i < c.issued; i++)
+                mbar_wait_ns(&c.full[i % STAGES], (unsigned)(i / STAGES) & 1u, 2000000000ull);
+        }
+    }
     if (warp == 9) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, 512;" ::"r"(tmem));
 }
 

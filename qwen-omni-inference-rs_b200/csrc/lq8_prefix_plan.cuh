@@ -57,6 +57,8 @@ struct PrefixPlan {
     int extra;                  // steps that an own item counts for beside its tiles
     int workers;                // CTAs that share the line
     uint64_t workers_mul;       // ceil(2^40 / workers)
+    int polls;                  // polls of a wait for segments before the CTA gives up
+    int hold;                   // fault injection: every CTA stops handing out segments after a few batches
     int cap[2];                 // rows a partial slot holds (prefix, own)
     int32_t* own_steps;         // [1] own steps in all, written by the first CTA
     int32_t* first[2];          // per item (prefix, own): the first worker of its steps,
