@@ -227,7 +227,7 @@ static int make_plan(lq_ctx* ctx, const PrefixAttnArgs& a, const PagedSeqs& s, b
     LQ_REQUIRE(ctx, steps < PREFIX_MAX_STEPS, "lq_prefix_attention: %lld steps, more than a launch can number", (long long)steps);
     // LQ_FAULT=prefix_attn_wait: waits inside the kernel run out (tests of what follows then)
     p->hold = fault_injected("prefix_attn_wait");
-    p->polls = p->hold ? 1 << 12 : 1 << 22;
+    p->polls = !p->hold ? 1 << 22 : f32 ? 0 : 1 << 12;
     const int64_t items_p = (int64_t)a.n_kv * p->n_rb;
     const int64_t items_o = a.n_kv * ((int64_t)s.rows * a.group / p->ob + s.n_seqs + 1);
     const int64_t items[2] = {p->np ? items_p : 0, items_o};

@@ -258,9 +258,16 @@ prefix_attn_f32_kernel(const __grid_constant__ PrefixAttnArgs a, const __grid_co
             };
             auto after = [](int i, int by) { return (i + by) % PF_SLOTS; };
             auto landed = [&]() {
-                ok = mbar_wait(&full[warp][slot], ph, 1ll << 22);
+                ok = mbar_wait(&full[warp][slot], ph, p.polls);
                 ok = __all_sync(0xffffffffu, ok);
                 return ok;
+            };
+            // after a copy that did not land: it and the later ones of `n` in flight may not land in
+            // shared memory that is no longer this kernel's
+            auto drain = [&](int n) {
+#pragma unroll 1
+                for (int i = 0; i < n; i++)
+                    mbar_wait_ns(&full[warp][after(slot, i)], slot + i < PF_SLOTS ? ph : ph ^ 1u, 2000000000ull);
             };
             auto done = [&]() {
                 __syncwarp();  // (read by every lane)
@@ -281,7 +288,10 @@ prefix_attn_f32_kernel(const __grid_constant__ PrefixAttnArgs a, const __grid_co
                 float sc[4] = {0.0f, 0.0f, 0.0f, 0.0f}, y[2][4];
 #pragma unroll
                 for (int i = 0; i < 4; i++) y[0][i] = y[1][i] = 0.0f;
-                if (!landed()) break;
+                if (!landed()) {
+                    drain(x + 16 < pos1 ? 3 : 2);  // K, V, the next K
+                    break;
+                }
                 {
                     const uint8_t* const k0 = mine + slot * SLOT + g * KS + t4 * 16;
 #pragma unroll
@@ -341,7 +351,10 @@ prefix_attn_f32_kernel(const __grid_constant__ PrefixAttnArgs a, const __grid_co
                     pb[i] = tf_big(v);
                     pm[i] = tf_small(v, pb[i]);
                 }
-                if (!landed()) break;
+                if (!landed()) {
+                    drain(x + 16 < pos1 ? 3 : 1);  // V, the next K and V
+                    break;
+                }
                 {
                     const uint8_t* const v0 = mine + slot * SLOT + t4 * VS + g * 16;
 #pragma unroll

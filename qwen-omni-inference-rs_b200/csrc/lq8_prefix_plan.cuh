@@ -57,7 +57,7 @@ struct PrefixPlan {
     int extra;                  // steps that an own item counts for beside its tiles
     int workers;                // CTAs that share the line
     uint64_t workers_mul;       // ceil(2^40 / workers)
-    int polls;                  // polls of a wait for segments before the CTA gives up
+    int polls;                  // polls of a wait (f32: for a copy; bf16: for segments) before it gives up
     int hold;                   // fault injection: every CTA stops handing out segments after a few batches
     int cap[2];                 // rows a partial slot holds (prefix, own)
     int32_t* own_steps;         // [1] own steps in all, written by the first CTA

@@ -42,3 +42,20 @@ def test_attention_whose_waits_run_out(ctx, lq8_lib, monkeypatch, kv, q, prefix,
             ctx.device_status()
         assert torch.equal(s.cache.attend(x, s.batch), want)
         ctx.device_status()
+
+
+def test_f32_attention_whose_waits_run_out(ctx, lq8_lib, monkeypatch):
+    """The same for an f32 cache: every wait for a copy gives up at once, with the copies in flight."""
+    import torch
+    s = Setup(lq8_lib, ctx, "f32", [40 + 7 * (b % 90) for b in range(300)], [1] * 300, 2, 128, 16, 500, seed=3, garbage=False).fill()
+    x = randn(3, s.rows, 8, 128)
+    want = s.cache.attend(x, s.batch)
+    ctx.device_status()
+    for _ in range(3):
+        monkeypatch.setenv("LQ_FAULT", "prefix_attn_wait")
+        s.cache.attend(x, s.batch)
+        monkeypatch.delenv("LQ_FAULT")
+        with pytest.raises(lq8_lib.LQ8Error, match="code 95"):
+            ctx.device_status()
+        assert torch.equal(s.cache.attend(x, s.batch), want)
+        ctx.device_status()
