@@ -7,6 +7,7 @@
 #include <cstdio>
 #include <cstring>
 #include <string>
+#include <vector>
 
 #include "../../include/lq8.h"
 
@@ -14,6 +15,11 @@
 // context
 // ------------------------------------------------------------------------------------------
 constexpr int kTileCounters = 1024;
+
+struct PagedBuffer {
+    void* p = nullptr;
+    size_t bytes = 0;
+};
 
 struct lq_ctx {
     int device = 0;
@@ -33,10 +39,12 @@ struct lq_ctx {
     // on demand outside graph capture
     void* wide = nullptr;
     size_t wide_bytes = 0;
-    // partial results of the paged attention; grown on demand outside graph capture. After a
-    // change of stream the next user waits for the event recorded on the old one.
-    void* paged = nullptr;
-    size_t paged_bytes = 0;
+    // partial results of the paged attention; grown on demand. After a change of stream the next
+    // user waits for the event recorded on the old one. Calls that are captured into a graph have
+    // buffers of their own, which stay until lq_destroy, outgrown ones too: graphs hold their
+    // addresses, and replays may run next to other calls.
+    PagedBuffer paged;
+    std::vector<PagedBuffer> paged_captured;
     cudaEvent_t paged_event = nullptr;
     bool paged_used = false, paged_pending = false;
     int* err_flag = nullptr;      // device int[4]: kernels report bad inputs here
@@ -60,9 +68,9 @@ int ensure_scratch(lq_ctx* ctx, size_t bytes);
 int ensure_split(lq_ctx* ctx, size_t bytes);
 // grows ctx->wide (an error while the stream is capturing a graph)
 int ensure_wide(lq_ctx* ctx, size_t bytes);
-// grows ctx->paged (an error while the stream is capturing a graph) and orders this stream after
-// the buffer's users on the stream the context had before
-int ensure_paged(lq_ctx* ctx, size_t bytes);
+// a buffer for the paged attention's partial results, ordered after its users on the stream the
+// context had before
+int ensure_paged(lq_ctx* ctx, size_t bytes, void** out);
 // partial-sum bytes the M x (N, K) Q8_0 GEMM needs when it splits K (0: no split)
 size_t gemm_split_bytes(lq_ctx* ctx, int64_t n, int64_t k, int64_t m);
 // read + clear the device error flag (synchronises the stream)

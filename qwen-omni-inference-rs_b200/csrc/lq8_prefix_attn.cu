@@ -247,9 +247,10 @@ static int make_plan(lq_ctx* ctx, const PrefixAttnArgs& a, const PagedSeqs& s, b
         ml_at[k] = place(slots * p->cap[k], 8);
         o_at[k] = place(slots * p->cap[k], (size_t)D * 4);
     }
-    const int rc = ensure_paged(ctx, at);
+    void* buffer = nullptr;
+    const int rc = ensure_paged(ctx, at, &buffer);
     if (rc) return rc;
-    uint8_t* w = static_cast<uint8_t*>(ctx->paged);
+    uint8_t* w = static_cast<uint8_t*>(buffer);
     p->own_steps = reinterpret_cast<int32_t*>(w + steps_at);
     p->split = reinterpret_cast<SplitItem*>(w + split_at);
     for (int k = 0; k < 2; k++) {

@@ -100,35 +100,53 @@ int ensure_split(lq_ctx* ctx, size_t bytes) {
     return LQ_OK;
 }
 
-int ensure_paged(lq_ctx* ctx, size_t bytes) {
-    if (ctx->paged_pending) {
-        cudaStreamCaptureStatus st = cudaStreamCaptureStatusNone;
-        LQ_CUDA(ctx, cudaStreamIsCapturing(ctx->stream, &st));
-        if (st == cudaStreamCaptureStatusNone) {
-            LQ_CUDA(ctx, cudaStreamWaitEvent(ctx->stream, ctx->paged_event, 0));
-            ctx->paged_pending = false;
-        }
-    }
-    ctx->paged_used = true;
-    if (bytes <= ctx->paged_bytes) return LQ_OK;
+static int alloc_paged(lq_ctx* ctx, size_t bytes, PagedBuffer* b) {
     if (fault_injected("ensure_paged"))
         return set_error(ctx, LQ_ERR_INJECTED, "ensure_paged: injected fault (LQ_FAULT), %zu bytes", bytes);
-    cudaStreamCaptureStatus st = cudaStreamCaptureStatusNone;
-    LQ_CUDA(ctx, cudaStreamIsCapturing(ctx->stream, &st));
-    if (st != cudaStreamCaptureStatusNone)
-        return set_error(ctx, LQ_ERR_STATE, "paged attention workspace (%zu bytes) too small while capturing a graph", bytes);
-    LQ_CUDA(ctx, cudaStreamSynchronize(ctx->stream));
-    if (ctx->paged) LQ_CUDA(ctx, cudaFree(ctx->paged));
-    ctx->paged = nullptr;
-    ctx->paged_bytes = 0;
-    size_t sz = (bytes + 0xFFFFF) & ~(size_t)0xFFFFF;
-    cudaError_t e = cudaMalloc(&ctx->paged, sz);
+    const size_t sz = (bytes + 0xFFFFF) & ~(size_t)0xFFFFF;
+    // (an allocation is no stream work: it may be made while a graph is being captured)
+    cudaStreamCaptureMode mode = cudaStreamCaptureModeRelaxed;
+    LQ_CUDA(ctx, cudaThreadExchangeStreamCaptureMode(&mode));
+    void* p = nullptr;
+    const cudaError_t e = cudaMalloc(&p, sz);
+    LQ_CUDA(ctx, cudaThreadExchangeStreamCaptureMode(&mode));
     if (e == cudaErrorMemoryAllocation) {
         cudaGetLastError();
         return set_error(ctx, LQ_ERR_OOM, "paged attention workspace: %zu bytes", sz);
     }
     LQ_CUDA(ctx, e);
-    ctx->paged_bytes = sz;
+    b->p = p;
+    b->bytes = sz;
+    return LQ_OK;
+}
+
+int ensure_paged(lq_ctx* ctx, size_t bytes, void** out) {
+    cudaStreamCaptureStatus st = cudaStreamCaptureStatusNone;
+    LQ_CUDA(ctx, cudaStreamIsCapturing(ctx->stream, &st));
+    if (st != cudaStreamCaptureStatusNone) {
+        std::vector<PagedBuffer>& have = ctx->paged_captured;
+        if (have.empty() || have.back().bytes < bytes) {
+            PagedBuffer b;
+            const int rc = alloc_paged(ctx, bytes, &b);
+            if (rc) return rc;
+            have.push_back(b);
+        }
+        *out = have.back().p;
+        return LQ_OK;
+    }
+    if (ctx->paged_pending) {
+        LQ_CUDA(ctx, cudaStreamWaitEvent(ctx->stream, ctx->paged_event, 0));
+        ctx->paged_pending = false;
+    }
+    ctx->paged_used = true;
+    if (bytes > ctx->paged.bytes) {
+        LQ_CUDA(ctx, cudaStreamSynchronize(ctx->stream));
+        if (ctx->paged.p) LQ_CUDA(ctx, cudaFree(ctx->paged.p));
+        ctx->paged = PagedBuffer{};
+        const int rc = alloc_paged(ctx, bytes, &ctx->paged);
+        if (rc) return rc;
+    }
+    *out = ctx->paged.p;
     return LQ_OK;
 }
 
@@ -216,7 +234,8 @@ int lq_destroy(lq_ctx* ctx) {
     if (ctx->scratch) cudaFree(ctx->scratch);
     if (ctx->split) cudaFree(ctx->split);
     if (ctx->wide) cudaFree(ctx->wide);
-    if (ctx->paged) cudaFree(ctx->paged);
+    if (ctx->paged.p) cudaFree(ctx->paged.p);
+    for (const PagedBuffer& b : ctx->paged_captured) cudaFree(b.p);
     if (ctx->paged_event) cudaEventDestroy(ctx->paged_event);
     if (ctx->err_flag) cudaFree(ctx->err_flag);
     if (ctx->tile_cnt) cudaFree(ctx->tile_cnt);

@@ -59,3 +59,80 @@ def test_f32_attention_whose_waits_run_out(ctx, lq8_lib, monkeypatch):
             ctx.device_status()
         assert torch.equal(s.cache.attend(x, s.batch), want)
         ctx.device_status()
+
+
+# ------------------------------------------------------------------------------------------
+# graphs and streams
+# ------------------------------------------------------------------------------------------
+
+def decode(ctx, lq8_lib, seqs, prefix, seed):
+    """A decode batch: setup, q and the result of a plain call."""
+    s = Setup(lq8_lib, ctx, "bf16", [40 + 13 * b for b in range(seqs)], [1] * seqs, 2, 128, 16, prefix, seed=seed, garbage=False).fill()
+    x = randn(seed, seqs, 8, 128, dtype="bf16")
+    return s, x, s.cache.attend(x, s.batch).clone()
+
+
+def capture(ctx, s, x):
+    import torch
+    out = torch.zeros_like(x)
+    torch.cuda.synchronize()
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g, stream=ctx._torch_stream):
+        s.cache.attend(x, s.batch, out=out)
+    return g, out
+
+
+def test_a_graph_outlives_a_larger_call(ctx, lq8_lib):
+    """A captured decode step, then eager calls and captures that need more workspace and memory
+    that takes what was freed; the replays give the same bits and write nothing else."""
+    import torch
+    c = lq8_lib.Context(0)
+    s, x, want = decode(c, lq8_lib, 5, 300, 1)
+    g, out = capture(c, s, x)
+    big, y, _ = decode(c, lq8_lib, 200, 3000, 2)
+    taken = [torch.full((1 << 20,), 7, dtype=torch.uint8, device="cuda") for _ in range(64)]
+    g2, out2 = capture(c, big, y)
+    for _ in range(3):
+        out.zero_(), out2.zero_()
+        g.replay()
+        g2.replay()
+        assert torch.equal(out, want) and torch.equal(out2, big.cache.attend(y, big.batch))
+    assert all(bool((t == 7).all()) for t in taken)
+    c.device_status()
+    del g, g2
+    c.close()
+
+
+def test_a_capture_may_be_the_first_call(ctx, lq8_lib):
+    """No warm-up: the workspace is made while the graph is captured."""
+    import torch
+    s, x, want = decode(ctx, lq8_lib, 70, 900, 3)
+    c = lq8_lib.Context(0)
+    cache = lq8_lib.PagedKvCache(c, s.k, s.v)
+    out = torch.zeros_like(x)
+    torch.cuda.synchronize()
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g, stream=c._torch_stream):
+        cache.attend(x, s.batch, out=out)
+    g.replay()
+    torch.cuda.synchronize()
+    assert torch.equal(out, want)
+    del g
+    c.close()
+
+
+def test_replays_next_to_eager_calls_on_another_stream(ctx, lq8_lib):
+    import torch
+    s, x, want = decode(ctx, lq8_lib, 60, 4000, 4)
+    t, y, want2 = decode(ctx, lq8_lib, 90, 3000, 5)
+    g, out = capture(ctx, s, x)
+    other = torch.cuda.Stream()
+    got, got2 = [torch.empty_like(out) for _ in range(20)], [torch.empty_like(y) for _ in range(20)]
+    torch.cuda.synchronize()
+    for i in range(20):
+        with torch.cuda.stream(other):
+            g.replay()
+            got[i].copy_(out)
+        t.cache.attend(y, t.batch, out=got2[i])
+    torch.cuda.synchronize()
+    assert all(torch.equal(o, want) for o in got) and all(torch.equal(o, want2) for o in got2)
