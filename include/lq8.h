@@ -263,9 +263,9 @@ int lq_paged_append(lq_ctx* ctx, const void* qkv_dev, lq_dtype qkv_dtype, int64_
  * read once for the batch; prefix_len 0: none) and over the sequence's own positions up to the
  * row itself. head_dim 64 or 128; head h reads kv head h / (n_heads / n_kv_heads). max_q and
  * max_kv are bounds on the rows and own positions of one sequence: they size the launch and the
- * workspace, which the context keeps and grows. Calls captured into a graph have a workspace of
- * their own, kept until lq_destroy: graphs stay valid whatever is called later and may be replayed
- * next to other calls, but not at the same time as each other. out [rows][n_heads *
+ * workspace, which the context keeps, one a stream, and grows. Calls captured into a graph have
+ * another, kept until lq_destroy: graphs stay valid whatever is called later and may be replayed
+ * next to other calls, but those captured on one stream not at the same time as each other. out [rows][n_heads *
  * head_dim] in the cache type and/or Q8_0 rows xq [rows][n_heads * head_dim], xd (either may be
  * NULL). A row that sees nothing gives zeros. Pointers and strides are multiples of 16 bytes.
  * f32 caches are computed in f32; bf16 ones with bf16 products and f32 sums. What a page holds past

@@ -19,7 +19,9 @@ constexpr int kTileCounters = 1024;
 struct PagedBuffer {
     void* p = nullptr;
     size_t bytes = 0;
+    unsigned long long stream = 0;  // id of its user, unlike a handle never used again
 };
+constexpr size_t kPagedStreams = 4;  // streams that keep a buffer at a time
 
 struct lq_ctx {
     int device = 0;
@@ -39,14 +41,14 @@ struct lq_ctx {
     // on demand outside graph capture
     void* wide = nullptr;
     size_t wide_bytes = 0;
-    // partial results of the paged attention; grown on demand. After a change of stream the next
-    // user waits for the event recorded on the old one. Calls that are captured into a graph have
-    // buffers of their own, which stay until lq_destroy, outgrown ones too: graphs hold their
-    // addresses, and replays may run next to other calls.
-    PagedBuffer paged;
+    // partial results of the paged attention; grown on demand. Every stream that the context works
+    // on has its own, so that nothing is left to order when the context moves to another one (the
+    // old stream may be gone by then). Calls that are captured into a graph have others, which
+    // stay until lq_destroy, outgrown ones too: graphs hold their addresses, and replays may run
+    // next to other calls.
+    std::vector<PagedBuffer> paged;           // the one used last at the end
     std::vector<PagedBuffer> paged_captured;
-    cudaEvent_t paged_event = nullptr;
-    bool paged_used = false, paged_pending = false;
+    unsigned long long paged_stream = 0;      // id of the context's stream
     int* err_flag = nullptr;      // device int[4]: kernels report bad inputs here
     // device unsigned[kTileCounters], zero between launches: arrivals of the CTAs that share a
     // GEMM tile (the skinny GEMM's stream-K combine; the last CTA resets its counter)
@@ -68,8 +70,9 @@ int ensure_scratch(lq_ctx* ctx, size_t bytes);
 int ensure_split(lq_ctx* ctx, size_t bytes);
 // grows ctx->wide (an error while the stream is capturing a graph)
 int ensure_wide(lq_ctx* ctx, size_t bytes);
-// a buffer for the paged attention's partial results, ordered after its users on the stream the
-// context had before
+// takes down the id of the context's stream
+void note_stream(lq_ctx* ctx);
+// a buffer for the paged attention's partial results on the context's stream
 int ensure_paged(lq_ctx* ctx, size_t bytes, void** out);
 // partial-sum bytes the M x (N, K) Q8_0 GEMM needs when it splits K (0: no split)
 size_t gemm_split_bytes(lq_ctx* ctx, int64_t n, int64_t k, int64_t m);

@@ -1,11 +1,13 @@
 // lq8_runtime.cu -- context, errors, fault injection and device memory of liblq8.
 #include "lq8_internal.cuh"
 
+#include <algorithm>
 #include <cstdarg>
 #include <cstdlib>
 #include <cstring>
 #include <map>
 #include <mutex>
+#include <new>
 #include <utility>
 
 namespace {
@@ -120,33 +122,58 @@ static int alloc_paged(lq_ctx* ctx, size_t bytes, PagedBuffer* b) {
     return LQ_OK;
 }
 
+void note_stream(lq_ctx* ctx) {
+    cudaStreamCaptureStatus st = cudaStreamCaptureStatusNone;
+    ctx->paged_stream = 0;
+    if (cudaStreamIsCapturing(ctx->stream, &st) != cudaSuccess || st != cudaStreamCaptureStatusNone ||
+        cudaStreamGetId(ctx->stream, &ctx->paged_stream) != cudaSuccess)
+        cudaGetLastError();
+    // (the id of a stream that is capturing is not to be had; its handle, marked, stands in for it)
+    if (ctx->paged_stream == 0) ctx->paged_stream = 1ull << 63 | (unsigned long long)(uintptr_t)ctx->stream;
+}
+
 int ensure_paged(lq_ctx* ctx, size_t bytes, void** out) {
     cudaStreamCaptureStatus st = cudaStreamCaptureStatusNone;
     LQ_CUDA(ctx, cudaStreamIsCapturing(ctx->stream, &st));
-    if (st != cudaStreamCaptureStatusNone) {
-        std::vector<PagedBuffer>& have = ctx->paged_captured;
-        if (have.empty() || have.back().bytes < bytes) {
-            PagedBuffer b;
+    const bool capturing = st != cudaStreamCaptureStatusNone;
+    std::vector<PagedBuffer>& have = capturing ? ctx->paged_captured : ctx->paged;
+    size_t at = have.size();
+    while (at > 0 && have[at - 1].stream != ctx->paged_stream) at--;
+    if (at == 0 || have[at - 1].bytes < bytes) {
+        if (capturing) {
+            at = 0;  // (an outgrown one stays)
+        } else if (at > 0) {
+            LQ_CUDA(ctx, cudaStreamSynchronize(ctx->stream));
+        } else if (have.size() >= kPagedStreams) {
+            LQ_CUDA(ctx, cudaDeviceSynchronize());  // the stream used longest ago gives its buffer up
+            at = 1;
+        }
+        try {
+            have.reserve(have.size() + 1);
+        } catch (const std::bad_alloc&) {
+            return set_error(ctx, LQ_ERR_OOM, "paged attention workspace: no host memory");
+        }
+        PagedBuffer b;
+        b.stream = ctx->paged_stream;
+        if (at > 0) {
+            const PagedBuffer old = have[at - 1];
+            have.erase(have.begin() + (at - 1));
+            if (old.bytes >= bytes) {
+                b.p = old.p;
+                b.bytes = old.bytes;
+            } else {
+                LQ_CUDA(ctx, cudaFree(old.p));
+            }
+        }
+        if (!b.p) {
             const int rc = alloc_paged(ctx, bytes, &b);
             if (rc) return rc;
-            have.push_back(b);
         }
-        *out = have.back().p;
-        return LQ_OK;
+        have.push_back(b);
+        at = have.size();
     }
-    if (ctx->paged_pending) {
-        LQ_CUDA(ctx, cudaStreamWaitEvent(ctx->stream, ctx->paged_event, 0));
-        ctx->paged_pending = false;
-    }
-    ctx->paged_used = true;
-    if (bytes > ctx->paged.bytes) {
-        LQ_CUDA(ctx, cudaStreamSynchronize(ctx->stream));
-        if (ctx->paged.p) LQ_CUDA(ctx, cudaFree(ctx->paged.p));
-        ctx->paged = PagedBuffer{};
-        const int rc = alloc_paged(ctx, bytes, &ctx->paged);
-        if (rc) return rc;
-    }
-    *out = ctx->paged.p;
+    *out = have[at - 1].p;
+    if (!capturing) std::rotate(have.begin() + (at - 1), have.begin() + at, have.end());
     return LQ_OK;
 }
 
@@ -221,6 +248,7 @@ int lq_init(int device, lq_ctx** out) {
         return lq::set_error(nullptr, LQ_ERR_CUDA, "lq_init: stream/flag allocation failed");
     }
     c->stream = c->own_stream;
+    lq::note_stream(c);
     // LQ_NO_PDL=1 launches every kernel with plain stream ordering (no programmatic overlap)
     c->pdl = getenv("LQ_NO_PDL") == nullptr;
     *out = c;
@@ -234,9 +262,8 @@ int lq_destroy(lq_ctx* ctx) {
     if (ctx->scratch) cudaFree(ctx->scratch);
     if (ctx->split) cudaFree(ctx->split);
     if (ctx->wide) cudaFree(ctx->wide);
-    if (ctx->paged.p) cudaFree(ctx->paged.p);
+    for (const PagedBuffer& b : ctx->paged) cudaFree(b.p);
     for (const PagedBuffer& b : ctx->paged_captured) cudaFree(b.p);
-    if (ctx->paged_event) cudaEventDestroy(ctx->paged_event);
     if (ctx->err_flag) cudaFree(ctx->err_flag);
     if (ctx->tile_cnt) cudaFree(ctx->tile_cnt);
     if (ctx->own_stream) cudaStreamDestroy(ctx->own_stream);
@@ -250,21 +277,8 @@ const char* lq_last_error(const lq_ctx* ctx) {
 
 int lq_set_stream(lq_ctx* ctx, void* stream) {
     LQ_ENTRY(ctx, "lq_set_stream");
-    const cudaStream_t next = stream ? (cudaStream_t)stream : ctx->own_stream;
-    if (next != ctx->stream && ctx->paged_used) {
-        // the paged attention's workspace may still be in use on the old stream: its next user
-        // waits for this point (not while a graph is being captured: captured calls are ordered
-        // by the graph)
-        cudaStreamCaptureStatus st = cudaStreamCaptureStatusNone;
-        LQ_CUDA(ctx, cudaStreamIsCapturing(ctx->stream, &st));
-        if (st == cudaStreamCaptureStatusNone) {
-            if (!ctx->paged_event) LQ_CUDA(ctx, cudaEventCreateWithFlags(&ctx->paged_event, cudaEventDisableTiming));
-            if (ctx->paged_pending) LQ_CUDA(ctx, cudaStreamWaitEvent(ctx->stream, ctx->paged_event, 0));
-            LQ_CUDA(ctx, cudaEventRecord(ctx->paged_event, ctx->stream));
-            ctx->paged_pending = true;
-        }
-    }
-    ctx->stream = next;
+    ctx->stream = stream ? (cudaStream_t)stream : ctx->own_stream;
+    lq::note_stream(ctx);
     return LQ_OK;
 }
 

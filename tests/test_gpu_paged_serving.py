@@ -136,3 +136,45 @@ def test_replays_next_to_eager_calls_on_another_stream(ctx, lq8_lib):
         t.cache.attend(y, t.batch, out=got2[i])
     torch.cuda.synchronize()
     assert all(torch.equal(o, want) for o in got) and all(torch.equal(o, want2) for o in got2)
+
+
+def test_the_stream_that_the_context_leaves_may_be_gone(ctx, lq8_lib):
+    import ctypes as C
+    import torch
+    s, x, want = decode(ctx, lq8_lib, 60, 4000, 6)
+    home, rt = ctx.stream, torch.cuda.cudart()
+    got = [torch.empty_like(want) for _ in range(8)]
+    torch.cuda.synchronize()
+    try:
+        for i in range(0, 8, 2):
+            h = C.c_void_p()
+            assert int(rt.cudaStreamCreate(C.addressof(h))) == 0
+            ctx.check(ctx.lib.lq_set_stream(ctx.h, h))
+            s.cache.attend(x, s.batch, out=got[i])
+            torch.cuda.synchronize()
+            assert int(rt.cudaStreamDestroy(h.value)) == 0
+            ctx.check(ctx.lib.lq_set_stream(ctx.h, home))
+            s.cache.attend(x, s.batch, out=got[i + 1])
+    finally:
+        ctx.check(ctx.lib.lq_set_stream(ctx.h, home))
+    torch.cuda.synchronize()
+    assert all(torch.equal(g, want) for g in got)
+
+
+def test_more_streams_than_workspaces(ctx, lq8_lib):
+    """Calls of two sizes in turn on seven streams, with no wait in between."""
+    import torch
+    a, b = decode(ctx, lq8_lib, 60, 4000, 7), decode(ctx, lq8_lib, 150, 5000, 8)
+    streams, home = [torch.cuda.Stream() for _ in range(7)], ctx.stream
+    assert len({t.cuda_stream for t in streams}) == 7
+    got = [(torch.empty_like(a[2]), torch.empty_like(b[2])) for _ in range(21)]
+    torch.cuda.synchronize()
+    try:
+        for i, (ga, gb) in enumerate(got):
+            ctx.check(ctx.lib.lq_set_stream(ctx.h, streams[i * 3 % 7].cuda_stream))
+            for (s, x, _), g in ((a, ga), (b, gb)) if i % 2 else ((b, gb), (a, ga)):
+                s.cache.attend(x, s.batch, out=g)
+    finally:
+        ctx.check(ctx.lib.lq_set_stream(ctx.h, home))
+    torch.cuda.synchronize()
+    assert all(torch.equal(ga, a[2]) and torch.equal(gb, b[2]) for ga, gb in got)
