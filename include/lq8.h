@@ -267,7 +267,7 @@ int lq_paged_append(lq_ctx* ctx, const void* qkv_dev, lq_dtype qkv_dtype, int64_
  * another, kept until lq_destroy: graphs stay valid whatever is called later and may be replayed
  * next to other calls, but those captured on one stream not at the same time as each other. out [rows][n_heads *
  * head_dim] in the cache type and/or Q8_0 rows xq [rows][n_heads * head_dim], xd (either may be
- * NULL). A row that sees nothing gives zeros. Pointers and strides are multiples of 16 bytes.
+ * NULL). A row that sees nothing gives zeros. Pointers and strides are multiples of 16 bytes (xd_dev: of 2).
  * f32 caches are computed in f32; bf16 ones with bf16 products and f32 sums. What a page holds past
  * a sequence's end is never used; a NaN or infinity in V of a row of this call may reach earlier
  * rows of its sequence. */

@@ -310,9 +310,9 @@ extern "C" int lq_prefix_attention(lq_ctx* ctx, const void* q, lq_dtype dtype, i
     LQ_REQUIRE(ctx, q && k_pages && v_pages && (out || xq), "lq_prefix_attention: NULL pointer");
     const size_t esize = dtype == LQ_DTYPE_F32 ? 4 : 2;
     auto al = [](const void* p) { return (uintptr_t)p % 16 == 0; };
-    LQ_REQUIRE(ctx, al(q) && al(k_pages) && al(v_pages) && al(out) && q_stride * esize % 16 == 0 &&
+    LQ_REQUIRE(ctx, al(q) && al(k_pages) && al(v_pages) && al(out) && al(xq) && (uintptr_t)xd % 2 == 0 && q_stride * esize % 16 == 0 &&
                         out_stride * esize % 16 == 0 && page_stride * esize % 16 == 0,
-               "lq_prefix_attention: pointers and strides must be multiples of 16 bytes");
+               "lq_prefix_attention: pointers and strides must be multiples of 16 bytes (xd: of 2)");
     lq::PrefixAttnArgs a;
     a.q = q;
     a.q_stride = q_stride;

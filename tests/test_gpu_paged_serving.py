@@ -178,3 +178,21 @@ def test_more_streams_than_workspaces(ctx, lq8_lib):
         ctx.check(ctx.lib.lq_set_stream(ctx.h, home))
     torch.cuda.synchronize()
     assert all(torch.equal(ga, a[2]) and torch.equal(gb, b[2]) for ga, gb in got)
+
+
+# ------------------------------------------------------------------------------------------
+# refusals
+# ------------------------------------------------------------------------------------------
+
+@pytest.mark.parametrize("dtype", ["bf16", "f32"])
+def test_q8_rows_that_are_not_aligned_are_refused(ctx, lq8_lib, dtype):
+    import torch
+    s = Setup(lq8_lib, ctx, dtype, [30, 2], [1, 1], 2, 64, 16, 0, garbage=False).fill()
+    x = randn(1, 2, 4, 64, dtype=dtype)
+    q, d = torch.zeros(2 * 256 + 8, dtype=torch.int8, device="cuda"), torch.zeros(2 * 8, dtype=torch.int16, device="cuda")
+    with pytest.raises(lq8_lib.LQ8Error, match="multiples of 16 bytes"):
+        s.cache.attend(x, s.batch, quantized=(q[8:].view(2, 256), d.view(2, 8)))
+    with pytest.raises(lq8_lib.LQ8Error, match="multiples of 16 bytes"):
+        ctx.call("lq_prefix_attention", x.data_ptr(), s.cache.dtype, 0, 2, 4, 2, 64, 0.125, *s.cache._pages, s.n_pages, 16, 0,
+                 None, 0, *s.batch._seqs, 1, 30, None, 0, q.data_ptr(), d.data_ptr() + 1)
+    ctx.device_status()
