@@ -558,8 +558,8 @@ class PagedKvCache:
             import torch
             xq, xd = quantized
             _need(xq.dtype == torch.int8 and xd.dtype == torch.int16 and xq.is_contiguous() and xd.is_contiguous() and
-                  xq.shape == (rows, heads * D) and xd.shape == (rows, heads * D // 32),
-                  "attend: quantized is (int8 [rows, heads * dim], int16 [rows, heads * dim / 32])")
+                  xq.is_cuda and xd.is_cuda and xq.shape == (rows, heads * D) and xd.shape == (rows, heads * D // 32),
+                  "attend: quantized is (int8 [rows, heads * dim], int16 [rows, heads * dim / 32]) on the GPU")
             xq, xd = xq.data_ptr(), xd.data_ptr()
         if rows == 0:
             return out

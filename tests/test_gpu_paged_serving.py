@@ -196,3 +196,13 @@ def test_q8_rows_that_are_not_aligned_are_refused(ctx, lq8_lib, dtype):
         ctx.call("lq_prefix_attention", x.data_ptr(), s.cache.dtype, 0, 2, 4, 2, 64, 0.125, *s.cache._pages, s.n_pages, 16, 0,
                  None, 0, *s.batch._seqs, 1, 30, None, 0, q.data_ptr(), d.data_ptr() + 1)
     ctx.device_status()
+
+
+def test_q8_rows_on_the_host_are_refused(ctx, lq8_lib):
+    import torch
+    s = Setup(lq8_lib, ctx, "bf16", [30, 2], [1, 1], 2, 64, 16, 0, garbage=False).fill()
+    x = randn(1, 2, 4, 64, dtype="bf16")
+    q, d = torch.zeros(2, 256, dtype=torch.int8), torch.zeros(2, 8, dtype=torch.int16)
+    for pair in ((q, d), (q.cuda(), d), (q, d.cuda())):
+        with pytest.raises(ValueError, match="on the GPU"):
+            s.cache.attend(x, s.batch, quantized=pair)
