@@ -259,8 +259,8 @@ int lq_paged_append(lq_ctx* ctx, const void* qkv_dev, lq_dtype qkv_dtype, int64_
                     int64_t table_ld, void* k_pages_dev, void* v_pages_dev, lq_dtype kv_dtype, int64_t n_pages,
                     int64_t page_size, int64_t page_stride, void* q_out_dev, int64_t q_out_stride);
 /* Attention of the rows q [rows][n_heads][head_dim] (cache type, q_stride elements apart) over a
- * prefix that all sequences share (positions 0 .. prefix_len-1 in the pages of prefix_table_dev,
- * read once for the batch; prefix_len 0: none) and over the sequence's own positions up to the
+ * prefix that all sequences share (positions 0 .. prefix_len-1 in the pages of prefix_table_dev
+ * [ceil(prefix_len / page_size)], read once for the batch; prefix_len 0: none) and over the sequence's own positions up to the
  * row itself. head_dim 64 or 128; head h reads kv head h / (n_heads / n_kv_heads). max_q and
  * max_kv are bounds on the rows and own positions of one sequence: they size the launch and the
  * workspace, which the context keeps, one a stream, and grows. Calls captured into a graph have

@@ -470,6 +470,7 @@ class PagedBatch:
         self.ld = page_table.shape[1]
         self._seqs = (self.n_seqs, _ptr(q_start), kv_len.data_ptr(), page_table.data_ptr(), self.ld)
         self._prefix_ptr = _ptr(prefix_table)
+        self._prefix_pages = 0 if prefix_table is None else prefix_table.shape[0]
 
 
 class PagedKvCache:
@@ -561,6 +562,9 @@ class PagedKvCache:
                   xq.is_cuda and xd.is_cuda and xq.shape == (rows, heads * D) and xd.shape == (rows, heads * D // 32),
                   "attend: quantized is (int8 [rows, heads * dim], int16 [rows, heads * dim / 32]) on the GPU")
             xq, xd = xq.data_ptr(), xd.data_ptr()
+        if batch.prefix_len > batch._prefix_pages * self.page_size:
+            raise ValueError(f"attend: {batch.prefix_len} prefix positions, prefix_table has {batch._prefix_pages} pages of "
+                             f"{self.page_size}")
         if rows == 0:
             return out
         ctx = self.ctx

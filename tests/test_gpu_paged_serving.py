@@ -206,3 +206,20 @@ def test_q8_rows_on_the_host_are_refused(ctx, lq8_lib):
     for pair in ((q, d), (q.cuda(), d), (q, d.cuda())):
         with pytest.raises(ValueError, match="on the GPU"):
             s.cache.attend(x, s.batch, quantized=pair)
+
+
+def test_a_prefix_longer_than_its_page_table_is_refused(ctx, lq8_lib):
+    import torch
+    s = Setup(lq8_lib, ctx, "bf16", [30, 2], [1, 1], 2, 64, 16, 33, garbage=False).fill()
+    x = randn(1, 2, 4, 64, dtype="bf16")
+    want = s.cache.attend(x, s.batch)
+    part = dict(prefix_table=s.batch.prefix_table[:2])
+    bad = lq8_lib.PagedBatch(s.batch.page_table, s.batch.kv_len, prefix_len=33, **part)
+    with pytest.raises(ValueError, match="33 prefix positions"):
+        s.cache.attend(x, bad)
+    good = lq8_lib.PagedBatch(s.batch.page_table, s.batch.kv_len, prefix_len=32, **part)
+    assert not torch.equal(s.cache.attend(x, good), want)
+    good.prefix_len = 48
+    with pytest.raises(ValueError, match="48 prefix positions"):
+        s.cache.attend(x, good)
+    ctx.device_status()
