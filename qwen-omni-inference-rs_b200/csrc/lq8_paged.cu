@@ -78,6 +78,15 @@ __device__ __forceinline__ bool angles(const RopeAxes& rope, int64_t row, int64_
     return ok;
 }
 
+// flags a position of pairs i0 .. i0 + n - 1 of a row that lies outside the tables
+__device__ __forceinline__ void flag_positions(const RopeAxes& rope, int64_t row, int i0, int n, int* err) {
+#pragma unroll 1
+    for (int i = i0; i < i0 + n; i++) {
+        const int p = rope.pos[(int64_t)rope.axis[i] * rope.pos_stride + row];
+        if (p < 0 || p >= rope.table_len) flag_error(err, ERR_ROPE_POS, p);
+    }
+}
+
 // =========================================================================================
 // Rotary positions with several axes: y_i = x_i cos - x_{i+n} sin, y_{i+n} = x_{i+n} cos +
 // x_i sin for the n pairs of a head, the dims past 2n copied. A thread owns V pairs (16 bytes of
@@ -260,9 +269,10 @@ __global__ void __launch_bounds__(256, 3) paged_append_kernel(AppendArgs a, Rope
     float cs[8], sn[8];
     bool turn = true;
     const bool turned = h0 < a.n_heads + a.n_kv;
-    if (turned && rope.pos) turn = angles<8>(rope, row, 0, d0, cs, sn, a.err);
+    if (turned && rope.pos) turn = angles<8>(rope, row, 0, d0, cs, sn, nullptr);
     const RowSlot slot = find_slot(seqs, row, lane, a.err);
-    if (!slot.live) return;
+    if (!slot.live) return;  // (padding, whatever its position)
+    if (!turn) flag_positions(rope, row, d0, 8, a.err);
     if (turned && !rope.pos) turn = angles<8>(rope, row, rope.pos_base + slot.own, d0, cs, sn, a.err);
     turn = __all_sync(0xffffffffu, turn);
     T* const page_k = static_cast<T*>(a.k) + slot.page * a.page_stride;

@@ -4,7 +4,7 @@ tolerances are those of test_gpu_paged.py."""
 import numpy as np
 import pytest
 
-from test_gpu_paged import Setup, attention_case, randn
+from test_gpu_paged import Setup, attention_case, i32, randn
 
 pytestmark = pytest.mark.gpu
 
@@ -178,6 +178,38 @@ def test_more_streams_than_workspaces(ctx, lq8_lib):
         ctx.check(ctx.lib.lq_set_stream(ctx.h, home))
     torch.cuda.synchronize()
     assert all(torch.equal(ga, a[2]) and torch.equal(gb, b[2]) for ga, gb in got)
+
+
+# ------------------------------------------------------------------------------------------
+# padding
+# ------------------------------------------------------------------------------------------
+
+@pytest.mark.parametrize("D,rot", [(64, 64), (128, 128), (256, 256), (128, 64), (80, 80)])
+@pytest.mark.parametrize("axes", [1, 3])
+def test_positions_of_padding_rows_are_not_looked_at(ctx, lq8_lib, D, rot, axes):
+    """A batch of fixed size: what stands in the padding's positions is no error; a live row's is."""
+    import torch
+    n = rot // 2
+    rotary = lq8_lib.Rotary.build(n, 100, 1e4, lq8_lib.Rotary.cyclic([n - 2 * (n // 4), n // 4, n // 4]) if axes == 3 else None)
+    qkv = randn(1, 9, 3 * D)
+
+    def run(pos):
+        s = Setup(lq8_lib, ctx, "f32", [3, 5], [1, 2], 1, D, 8, garbage=False)
+        out = torch.full((9, 1, D), 9.0, device="cuda")
+        s.cache.append(qkv, 1, s.batch, rotary, pos=i32(pos), q_out=out)
+        return s, out
+
+    pos = np.random.default_rng(1).integers(0, 100, (axes, 9))
+    want, out = run(pos)
+    ctx.device_status()
+    pos[:, 3:] = [100, -1, 2 ** 31 - 1, -2 ** 31, 12345, 7]
+    got, out2 = run(pos)
+    ctx.device_status()
+    assert torch.equal(out, out2) and (out2[3:] == 9.0).all() and torch.equal(want.k, got.k) and torch.equal(want.v, got.v)
+    pos[axes - 1, 1] = 100
+    run(pos)
+    with pytest.raises(lq8_lib.LQ8Error, match="code 90, value 100"):
+        ctx.device_status()
 
 
 # ------------------------------------------------------------------------------------------
