@@ -224,7 +224,8 @@ int lq_fill_bf16(lq_ctx* ctx, uint64_t seed, uint64_t tensor_id, int64_t offset,
  * sequences follow each other: those of sequence b are rows q_start_dev[b] .. q_start_dev[b+1]-1
  * (q_start_dev [n_seqs + 1], starting at 0 and not falling; NULL: row b is sequence b's only
  * one), and kv_len_dev[b] is its number of own positions, those rows included, which come last.
- * Rows past the last sequence's are padding: nothing is read or written for them. Positions
+ * Rows past the last sequence's are padding: what they hold has no effect, and nothing is written
+ * for them. Positions
  * outside the tables, lengths outside the page table and page ids outside the cache skip the
  * access and are reported by lq_device_status.
  * ------------------------------------------------------------------------------------- */

@@ -125,7 +125,7 @@ prefix_attn_f32_kernel(const __grid_constant__ PrefixAttnArgs a, const __grid_co
             if (si.kv < si.q) zero_rows<float, D>(a, si.q0, si.q - si.kv, lane, 32);
         }
     }
-    const int worker = warp * gridDim.x + blockIdx.x;
+    const int worker = warp * gridDim.x + blockIdx.x, live = live_rows(s);
     if (worker >= p.workers) return;
     const Line line(p, so, true, true);
     if (a.prefix_len == 0 && lane == 0) p.split[worker].rows = 0;
@@ -198,7 +198,8 @@ prefix_attn_f32_kernel(const __grid_constant__ PrefixAttnArgs a, const __grid_co
             }
             const int end = min(nt, tile + hi - step);
             const int row0 = (own ? si.q0 * a.group : 0) + rb * p.pb;
-            const int n = min(p.pb, (own ? si.q : s.rows) * a.group - rb * p.pb);
+            // (a block of padding: its first row, for nothing)
+            const int n = max(1, min(p.pb, (own ? si.q : live) * a.group - rb * p.pb));
             const int item = (own ? a.n_kv * os.base(si, b) : 0) + kh * n_rb + rb;
             const bool begins = tile == 0, whole = a.prefix_len == 0 && begins && end == nt;
             if (lane == 0) {

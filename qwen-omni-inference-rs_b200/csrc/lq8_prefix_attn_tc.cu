@@ -857,6 +857,7 @@ prefix_attn_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_co
             auto part = [&](auto own_part) {
                 constexpr bool own = decltype(own_part)::value, paired = own ? PO : PP;
                 const int block = own ? g.p.ob : g.p.pb, worker = paired ? me : 2 * me + f;
+                const int live = own ? 0 : live_rows(g.s);
                 int step, hi, b = 0, j = 0, t = 0, rounds = 0;  // the flow's place
                 flow_range(line, paired, me, f, own, step, hi);
                 if (step < hi && !own) {
@@ -918,7 +919,7 @@ prefix_attn_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_co
                     first = false;
                     // a lane looks at the hl-th item from here on
                     int jj = j + hl, bb = b, n_rb = own ? 1 : g.p.n_rb, nt = g.p.np;
-                    SeqInfo si{0, g.s.rows, 0};
+                    SeqInfo si{0, live, 0};
                     o.kv_end = g.a.prefix_len;
                     if constexpr (own) {
                         nt = o.kv_end = 0;
@@ -953,7 +954,7 @@ prefix_attn_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_co
                     const int rows = si.q * g.a.group - rb * block;  // of the whole block
                     const int item = (own ? g.a.n_kv * os.base(si, bb) : 0) + jj;
                     o.n1 = paired ? max(0, min(PA_ROWS, rows - PA_ROWS)) : 0;
-                    o.n = paired && f ? o.n1 : min(PA_ROWS, rows);
+                    o.n = paired && f ? o.n1 : max(0, min(PA_ROWS, rows));  // (0: a block of padding)
                     o.flags = (own ? SEG_OWN : 0) | (paired ? SEG_PAIRED : 0) | (paired && f ? SEG_HALF : 0) |
                               (own && g.p.np == 0 && o.t0 == 0 && o.t1 == nt ? SEG_WHOLE : 0);
                     o.kh = kh;

@@ -98,6 +98,11 @@ __device__ __forceinline__ SeqInfo seq_info(const PrefixAttnArgs& a, const Paged
     return r;
 }
 
+// rows before the padding: those that the prefix's blocks hold
+__device__ __forceinline__ int live_rows(const PagedSeqs& s) {
+    return s.q_start ? min(max(s.q_start[s.n_seqs], 0), s.rows) : s.rows;
+}
+
 // own positions that token j of the sequence's q sees
 __host__ __device__ __forceinline__ int own_visible(const SeqInfo& i, int j) { return max(0, i.kv - i.q + j + 1); }
 

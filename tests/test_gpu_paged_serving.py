@@ -212,6 +212,29 @@ def test_positions_of_padding_rows_are_not_looked_at(ctx, lq8_lib, D, rot, axes)
         ctx.device_status()
 
 
+@pytest.mark.parametrize("dtype", ["bf16", "f32"])
+@pytest.mark.parametrize("q,pad,prefix", [([1, 2, 1], 1, 1000), ([1] * 40, 200, 3000), ([1, 3, 0, 60], 500, 500), ([300, 200], 70, 900),
+                                          ([200] + [1] * 30, 300, 2000)])
+def test_what_padding_rows_hold_has_no_effect(ctx, lq8_lib, dtype, q, pad, prefix):
+    """Finite values, NaN or infinities in the padding: the other rows' bits are the same, and its own
+    outputs are left alone."""
+    import torch
+    s = Setup(lq8_lib, ctx, dtype, [n + 20 + 3 * (b % 50) for b, n in enumerate(q)], q, 2, 128, 16, prefix, seed=5).fill()
+    s.batch = lq8_lib.PagedBatch(s.batch.page_table, s.batch.kv_len, q_start=i32(s.start), max_q=max(q), max_kv=int(s.kv.max()),
+                                 prefix_table=s.batch.prefix_table, prefix_len=prefix)
+    x = torch.cat([randn(5, s.rows, 8, 128, dtype=dtype), randn(6, pad, 8, 128, dtype=dtype, scale=30.0)])
+    outs = []
+    for fill in (None, 0.0, float("nan"), float("inf")):
+        if fill is not None:
+            x[s.rows:] = fill
+        out = torch.full_like(x, 9.0)
+        s.cache.attend(x, s.batch, out=out)
+        ctx.device_status()
+        assert (out[s.rows:] == 9.0).all() and torch.isfinite(out).all()
+        outs.append(out)
+    assert all(torch.equal(o, outs[0]) for o in outs)
+
+
 # ------------------------------------------------------------------------------------------
 # refusals
 # ------------------------------------------------------------------------------------------
