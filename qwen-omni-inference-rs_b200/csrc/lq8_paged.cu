@@ -453,6 +453,8 @@ int make_rope_axes(lq_ctx* ctx, const char* who, RopeAxes* r, int64_t rot_dim, i
                ROPE_MAX_AXES);
     LQ_REQUIRE(ctx, rot_dim == 0 || (cos_dev && sin_dev && table_len > 0 && table_len < (1ll << 31)),
                "%s: cos/sin tables missing or empty", who);
+    LQ_REQUIRE(ctx, aligned_to(cos_dev, 4) && aligned_to(sin_dev, 4) && aligned_to(pos_dev, 4),
+               "%s: tables and positions must be aligned to their elements", who);
     LQ_REQUIRE(ctx, !pos_dev || n_axes == 1 || pos_stride >= rows, "%s: pos_stride %lld < rows %lld", who,
                (long long)pos_stride, (long long)rows);
     r->cos = cos_dev;
@@ -496,6 +498,8 @@ int make_paged_seqs(lq_ctx* ctx, const char* who, PagedSeqs* s, int64_t n_seqs, 
                (long long)table_ld);
     LQ_REQUIRE(ctx, n_seqs == 0 || rows == 0 || (kv_len_dev && (page_table_dev || table_ld == 0)),
                "%s: NULL sequence lengths or page table", who);
+    LQ_REQUIRE(ctx, aligned_to(q_start_dev, 4) && aligned_to(kv_len_dev, 4) && aligned_to(page_table_dev, 4),
+               "%s: lengths and page tables must be aligned to their elements", who);
     s->q_start = q_start_dev;
     s->kv_len = kv_len_dev;
     s->table = page_table_dev;
@@ -539,6 +543,8 @@ int lq_mrope(lq_ctx* ctx, const void* x, lq_dtype dtype, int64_t rows, int64_t h
     if (rc) return rc;
     if (rows == 0) return LQ_OK;
     LQ_REQUIRE(ctx, x && out && (pos_dev || rot_dim == 0), "lq_mrope: NULL pointer");
+    const size_t size = dtype == LQ_DTYPE_F32 ? 4 : 2;
+    LQ_REQUIRE(ctx, lq::aligned_to(x, size) && lq::aligned_to(out, size), "lq_mrope: x and out must be aligned to their elements");
     lq::MropeArgs a;
     a.x = x;
     a.y = out;
@@ -594,6 +600,10 @@ int lq_paged_append(lq_ctx* ctx, const void* qkv, lq_dtype qkv_dtype, int64_t ro
     LQ_REQUIRE(ctx, rows * (n_heads + 2 * n_kv_heads) < (1ll << 33), "lq_paged_append: too many rows");
     if (rows == 0 || n_seqs == 0) return LQ_OK;
     LQ_REQUIRE(ctx, qkv && k_pages && v_pages && (q_out || n_heads == 0), "lq_paged_append: NULL pointer");
+    const size_t src_size = qkv_dtype == LQ_DTYPE_F32 ? 4 : 2, size = kv_dtype == LQ_DTYPE_F32 ? 4 : 2;
+    LQ_REQUIRE(ctx, lq::aligned_to(qkv, src_size) && lq::aligned_to(k_pages, size) && lq::aligned_to(v_pages, size) &&
+                        lq::aligned_to(q_out, size) && lq::aligned_to(q_norm, 2) && lq::aligned_to(k_norm, 2),
+               "lq_paged_append: pointers must be aligned to their elements");
     lq::AppendArgs a;
     a.qkv = qkv;
     a.row_stride = row_stride;

@@ -71,6 +71,8 @@ __device__ __forceinline__ uint32_t pack_bf16x2(float a, float b) {
     return *reinterpret_cast<const uint32_t*>(&h);
 }
 
+// host: whether a device pointer (or NULL) is aligned to elements of n bytes
+inline bool aligned_to(const void* p, size_t n) { return (uintptr_t)p % n == 0; }
 // host: the rotary tables of a call; axis_host NULL puts every pair on axis 0
 int make_rope_axes(lq_ctx* ctx, const char* who, RopeAxes* r, int64_t rot_dim, int64_t head_dim, const float* cos_dev,
                    const float* sin_dev, int64_t table_len, const uint8_t* axis_host, int64_t n_axes,

@@ -301,6 +301,7 @@ extern "C" int lq_prefix_attention(lq_ctx* ctx, const void* q, lq_dtype dtype, i
                "lq_prefix_attention: row stride too small");
     LQ_REQUIRE(ctx, prefix_len >= 0 && prefix_len < (1ll << 30) && (prefix_len == 0 || prefix_table),
                "lq_prefix_attention: bad prefix");
+    LQ_REQUIRE(ctx, lq::aligned_to(prefix_table, 4), "lq_prefix_attention: the prefix's page table must be aligned to its elements");
     LQ_REQUIRE(ctx, max_q >= 1 && max_q < (1ll << 24) && max_kv >= 0 && max_kv < (1ll << 30),
                "lq_prefix_attention: bad bounds max_q %lld, max_kv %lld", (long long)max_q, (long long)max_kv);
     LQ_REQUIRE(ctx, scale > 0.0f && scale < INFINITY, "lq_prefix_attention: scale must be positive and finite");
@@ -310,7 +311,7 @@ extern "C" int lq_prefix_attention(lq_ctx* ctx, const void* q, lq_dtype dtype, i
     LQ_REQUIRE(ctx, q && k_pages && v_pages && (out || xq), "lq_prefix_attention: NULL pointer");
     const size_t esize = dtype == LQ_DTYPE_F32 ? 4 : 2;
     auto al = [](const void* p) { return (uintptr_t)p % 16 == 0; };
-    LQ_REQUIRE(ctx, al(q) && al(k_pages) && al(v_pages) && al(out) && al(xq) && (uintptr_t)xd % 2 == 0 && q_stride * esize % 16 == 0 &&
+    LQ_REQUIRE(ctx, al(q) && al(k_pages) && al(v_pages) && al(out) && al(xq) && lq::aligned_to(xd, 2) && q_stride * esize % 16 == 0 &&
                         out_stride * esize % 16 == 0 && page_stride * esize % 16 == 0,
                "lq_prefix_attention: pointers and strides must be multiples of 16 bytes (xd: of 2)");
     lq::PrefixAttnArgs a;

@@ -278,3 +278,29 @@ def test_a_prefix_longer_than_its_page_table_is_refused(ctx, lq8_lib):
     with pytest.raises(ValueError, match="48 prefix positions"):
         s.cache.attend(x, good)
     ctx.device_status()
+
+
+def test_pointers_that_are_not_aligned_to_their_elements_are_refused(ctx, lq8_lib):
+    """Every device pointer of the three entries, one byte past where it belongs."""
+    import torch
+    z = torch.zeros(1 << 16, device="cuda")
+    p = z.data_ptr()
+
+    def refused(name, args, pointers):
+        for i in pointers:
+            bad = list(args)
+            bad[i] = p + 1
+            with pytest.raises(lq8_lib.LQ8Error, match="aligned|multiples of 16 bytes"):
+                ctx.call(name, *bad)
+
+    # x, dtype, rows, heads, dim, strides, out, strides, rot, cos, sin, len, axes of pairs, axes, pos, stride, inverse
+    refused("lq_mrope", (p, 1, 2, 2, 64, 128, 64, p, 128, 64, 64, p, p, 4, None, 1, p, 2, 0), (0, 7, 11, 12, 16))
+    # qkv, dtype, stride, rows, heads, kv heads, dim, norms, eps, bf16, rot, cos, sin, len, axes of pairs, axes, pos, stride, base,
+    # sequences, starts, lengths, pages, ld, k, v, dtype, pages, size, stride, q out, stride
+    refused("lq_paged_append", (p, 1, 0, 2, 2, 1, 64, p, p, 1e-6, 0, 64, p, p, 4, None, 1, p, 2, 0, 2, p, p, p, 1, p, p, 1, 4, 8, 0, p, 0),
+            (0, 7, 8, 12, 13, 17, 21, 22, 23, 25, 26, 31))
+    # q, dtype, stride, rows, heads, kv heads, dim, scale, k, v, pages, size, stride, prefix, length, sequences, starts, lengths,
+    # pages, ld, most rows, most positions, out, stride, xq, xd
+    refused("lq_prefix_attention", (p, 1, 0, 2, 2, 1, 64, 1.0, p, p, 4, 8, 0, p, 8, 2, p, p, p, 1, 1, 8, p, 0, p, p),
+            (0, 8, 9, 13, 16, 17, 18, 22, 24, 25))
+    ctx.device_status()
