@@ -533,7 +533,12 @@ int lq_mrope(lq_ctx* ctx, const void* x, lq_dtype dtype, int64_t rows, int64_t h
                "lq_mrope: head_dim %lld must be even and at most 256", (long long)head_dim);
     LQ_REQUIRE(ctx, row_stride >= 0 && out_row_stride >= 0 && head_stride >= 0 && out_head_stride >= 0,
                "lq_mrope: negative stride");
-    LQ_REQUIRE(ctx, (heads == 1 || out_head_stride >= head_dim) && (rows <= 1 || out_row_stride >= head_dim),
+    // the output's rows and heads: the ones that lie closer follow each other without overlap, and
+    // all of them fit between two of the others
+    const bool by_row = rows > 1 && (heads == 1 || out_row_stride < out_head_stride);
+    const int64_t near = by_row ? out_row_stride : out_head_stride, n_near = by_row ? rows : heads;
+    const int64_t apart = by_row ? out_head_stride : out_row_stride, n_apart = by_row ? heads : rows;
+    LQ_REQUIRE(ctx, (n_near <= 1 || near >= head_dim) && (n_apart <= 1 || (apart - head_dim) / std::max<int64_t>(1, near) >= n_near - 1),
                "lq_mrope: output heads overlap");
     LQ_REQUIRE(ctx, x != out || (row_stride == out_row_stride && head_stride == out_head_stride),
                "lq_mrope: in place needs equal strides");

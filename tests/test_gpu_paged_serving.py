@@ -304,3 +304,22 @@ def test_pointers_that_are_not_aligned_to_their_elements_are_refused(ctx, lq8_li
     refused("lq_prefix_attention", (p, 1, 0, 2, 2, 1, 64, 1.0, p, p, 4, 8, 0, p, 8, 2, p, p, p, 1, 1, 8, p, 0, p, p),
             (0, 8, 9, 13, 16, 17, 18, 22, 24, 25))
     ctx.device_status()
+
+
+def test_mrope_refuses_rows_and_heads_of_the_output_that_overlap(ctx, lq8_lib):
+    import torch
+    rot = lq8_lib.Rotary.build(32, 100, 1e4)
+    x, pos = randn(1, 5, 3, 64), i32(np.arange(5))
+    want = lq8_lib.mrope(ctx, x, rot, pos)
+    buf = torch.full((8192,), 9.0, device="cuda")
+    for row, head in [(64, 64), (64, 128), (128, 64), (191, 64), (64, 319), (0, 64), (64, 0), (32, 1000), (1000, 32)]:
+        with pytest.raises(lq8_lib.LQ8Error, match="overlap"):
+            lq8_lib.mrope(ctx, x, rot, pos, out=torch.as_strided(buf, (5, 3, 64), (row, head, 1)))
+    assert (buf == 9.0).all()
+    for row, head in [(192, 64), (64, 320), (200, 64), (65, 330), (256, 66), (400, 130)]:
+        assert torch.equal(lq8_lib.mrope(ctx, x, rot, pos, out=torch.as_strided(buf, (5, 3, 64), (row, head, 1))), want)
+    one = torch.as_strided(buf, (1, 3, 64), (0, 64, 1))
+    assert torch.equal(lq8_lib.mrope(ctx, x[:1], rot, pos[:1], out=one), want[:1])
+    one = torch.as_strided(buf, (5, 1, 64), (64, 0, 1))
+    assert torch.equal(lq8_lib.mrope(ctx, x[:, :1], rot, pos, out=one), want[:, :1])
+    ctx.device_status()
