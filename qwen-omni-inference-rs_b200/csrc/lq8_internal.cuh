@@ -41,6 +41,9 @@ struct lq_ctx {
     // on demand outside graph capture
     void* wide = nullptr;
     size_t wide_bytes = 0;
+    // which of the three a graph may hold (they are then kept when they are outgrown)
+    bool scratch_captured = false, split_captured = false, wide_captured = false;
+    std::vector<void*> outgrown;
     // partial results of the paged attention; grown on demand. Every stream that the context works
     // on has its own, so that nothing is left to order when the context moves to another one (the
     // old stream may be gone by then). Calls that are captured into a graph have others, which

@@ -49,16 +49,40 @@ bool fault_injected(const char* entry) {
     return false;
 }
 
+// remembers that a call captured into a graph uses a buffer
+static int note_capture(lq_ctx* ctx, bool* captured) {
+    if (*captured) return LQ_OK;
+    cudaStreamCaptureStatus st = cudaStreamCaptureStatusNone;
+    LQ_CUDA(ctx, cudaStreamIsCapturing(ctx->stream, &st));
+    *captured = st != cudaStreamCaptureStatusNone;
+    return LQ_OK;
+}
+
+// frees an outgrown buffer; one that a graph may hold stays until lq_destroy
+static int give_up(lq_ctx* ctx, void** buffer, bool* captured) {
+    if (*buffer && *captured) {
+        try {
+            ctx->outgrown.push_back(*buffer);
+        } catch (const std::bad_alloc&) {
+            return set_error(ctx, LQ_ERR_OOM, "outgrown buffer: no host memory");
+        }
+    } else if (*buffer) {
+        LQ_CUDA(ctx, cudaFree(*buffer));
+    }
+    *buffer = nullptr;
+    *captured = false;
+    return LQ_OK;
+}
+
 int ensure_scratch(lq_ctx* ctx, size_t bytes) {
-    if (bytes <= ctx->scratch_bytes) return LQ_OK;
+    if (bytes <= ctx->scratch_bytes) return note_capture(ctx, &ctx->scratch_captured);
     // LQ_FAULT=ensure_scratch turns every scratch allocation into an error (tests use it to
     // show that a path allocates nothing)
     if (fault_injected("ensure_scratch"))
         return set_error(ctx, LQ_ERR_INJECTED, "ensure_scratch: injected fault (LQ_FAULT), %zu bytes", bytes);
     // the old scratch may still be in use by queued work
     LQ_CUDA(ctx, cudaStreamSynchronize(ctx->stream));
-    if (ctx->scratch) LQ_CUDA(ctx, cudaFree(ctx->scratch));
-    ctx->scratch = nullptr;
+    if (const int rc = give_up(ctx, &ctx->scratch, &ctx->scratch_captured)) return rc;
     ctx->scratch_bytes = 0;
     size_t sz = (bytes + 0xFFFFF) & ~(size_t)0xFFFFF;  // 1 MiB granularity
     LQ_CUDA(ctx, cudaMalloc(&ctx->scratch, sz));
@@ -67,7 +91,7 @@ int ensure_scratch(lq_ctx* ctx, size_t bytes) {
 }
 
 int ensure_wide(lq_ctx* ctx, size_t bytes) {
-    if (bytes <= ctx->wide_bytes) return LQ_OK;
+    if (bytes <= ctx->wide_bytes) return note_capture(ctx, &ctx->wide_captured);
     if (fault_injected("ensure_wide"))
         return set_error(ctx, LQ_ERR_INJECTED, "ensure_wide: injected fault (LQ_FAULT), %zu bytes", bytes);
     cudaStreamCaptureStatus st = cudaStreamCaptureStatusNone;
@@ -75,8 +99,7 @@ int ensure_wide(lq_ctx* ctx, size_t bytes) {
     if (st != cudaStreamCaptureStatusNone)
         return set_error(ctx, LQ_ERR_STATE, "fp16 operand buffer (%zu bytes) too small while capturing a graph", bytes);
     LQ_CUDA(ctx, cudaStreamSynchronize(ctx->stream));
-    if (ctx->wide) LQ_CUDA(ctx, cudaFree(ctx->wide));
-    ctx->wide = nullptr;
+    if (const int rc = give_up(ctx, &ctx->wide, &ctx->wide_captured)) return rc;
     ctx->wide_bytes = 0;
     size_t sz = (bytes + 0xFFFFF) & ~(size_t)0xFFFFF;
     LQ_CUDA(ctx, cudaMalloc(&ctx->wide, sz));
@@ -85,7 +108,7 @@ int ensure_wide(lq_ctx* ctx, size_t bytes) {
 }
 
 int ensure_split(lq_ctx* ctx, size_t bytes) {
-    if (bytes <= ctx->split_bytes) return LQ_OK;
+    if (bytes <= ctx->split_bytes) return note_capture(ctx, &ctx->split_captured);
     if (fault_injected("ensure_split"))
         return set_error(ctx, LQ_ERR_INJECTED, "ensure_split: injected fault (LQ_FAULT), %zu bytes", bytes);
     cudaStreamCaptureStatus st = cudaStreamCaptureStatusNone;
@@ -93,8 +116,7 @@ int ensure_split(lq_ctx* ctx, size_t bytes) {
     if (st != cudaStreamCaptureStatusNone)
         return set_error(ctx, LQ_ERR_STATE, "split-K buffer (%zu bytes) too small while capturing a graph", bytes);
     LQ_CUDA(ctx, cudaStreamSynchronize(ctx->stream));
-    if (ctx->split) LQ_CUDA(ctx, cudaFree(ctx->split));
-    ctx->split = nullptr;
+    if (const int rc = give_up(ctx, &ctx->split, &ctx->split_captured)) return rc;
     ctx->split_bytes = 0;
     size_t sz = (bytes + 0xFFFFF) & ~(size_t)0xFFFFF;
     LQ_CUDA(ctx, cudaMalloc(&ctx->split, sz));
@@ -262,6 +284,7 @@ int lq_destroy(lq_ctx* ctx) {
     if (ctx->scratch) cudaFree(ctx->scratch);
     if (ctx->split) cudaFree(ctx->split);
     if (ctx->wide) cudaFree(ctx->wide);
+    for (void* p : ctx->outgrown) cudaFree(p);
     for (const PagedBuffer& b : ctx->paged) cudaFree(b.p);
     for (const PagedBuffer& b : ctx->paged_captured) cudaFree(b.p);
     if (ctx->err_flag) cudaFree(ctx->err_flag);

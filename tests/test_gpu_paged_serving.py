@@ -103,6 +103,42 @@ def test_a_graph_outlives_a_larger_call(ctx, lq8_lib):
     c.close()
 
 
+@pytest.mark.parametrize("name,m", [("lq_q8_0_linear", 3), ("lq_q8_0_linear", 16), ("lq_q8_0_matmul", 16), ("lq_q8_0_matmul_prefill", 128)])
+def test_a_graph_of_a_linear_outlives_a_larger_call(ctx, lq8_lib, name, m):
+    """The layers' buffers next to those of the paged attention: quantized rows, K-split partials, fp16
+    operands."""
+    import ctypes as C
+    import torch
+    c = lq8_lib.Context(0)
+
+    def call(n, k, rows, seed):
+        t = lq8_lib.QTensor.quantize(c, randn(seed, n, k, scale=0.02))
+        w = t.struct()
+        x, y = randn(seed + 1, rows, k), torch.zeros(rows, n, device="cuda")
+        rows8 = lq8_lib.QTensor.quantize(c, x)
+        if name == "lq_q8_0_linear":
+            args = (C.byref(w), x.data_ptr(), lq8_lib.DTYPE_F32, rows, y.data_ptr())
+        else:
+            args = (C.byref(w), rows8.qs.data_ptr(), rows8.d.data_ptr(), rows, y.data_ptr(), None, n)
+        return (lambda: c.call(name, *args)), y, (t, w, x, rows8)
+
+    run, y, keep = call(256, 4096, m, 1)
+    run()
+    want = y.clone()
+    torch.cuda.synchronize()
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g, stream=c._torch_stream):
+        run()
+    larger, y2, keep2 = call(1024, 16384, 4 * m, 3)
+    larger()
+    taken = [torch.full((1 << 20,), 7, dtype=torch.uint8, device="cuda") for _ in range(64)]
+    y.zero_()
+    g.replay()
+    assert torch.equal(y, want) and all(bool((t == 7).all()) for t in taken)
+    del g
+    c.close()
+
+
 def test_a_capture_may_be_the_first_call(ctx, lq8_lib):
     """No warm-up: the workspace is made while the graph is captured."""
     import torch
