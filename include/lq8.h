@@ -225,9 +225,9 @@ int lq_fill_bf16(lq_ctx* ctx, uint64_t seed, uint64_t tensor_id, int64_t offset,
  * (q_start_dev [n_seqs + 1], starting at 0 and not falling; NULL: row b is sequence b's only
  * one), and kv_len_dev[b] is its number of own positions, those rows included, which come last.
  * Rows past the last sequence's are padding: what they hold has no effect, and nothing is written
- * for them. Positions
- * outside the tables, lengths outside the page table and page ids outside the cache skip the
- * access and are reported by lq_device_status. Pointers are aligned to their elements.
+ * for them. Positions outside the tables, lengths outside the page table and page ids outside the
+ * cache skip the access and are reported by lq_device_status. Pointers are aligned to their
+ * elements.
  * ------------------------------------------------------------------------------------- */
 /* Waits for the context's stream; LQ_ERR_INVALID_ARG with the first code and value that a
  * kernel flagged since the last check (90 rotary position, 91 length, 92 page id, 93 row
@@ -248,9 +248,10 @@ int lq_mrope(lq_ctx* ctx, const void* x_dev, lq_dtype dtype, int64_t rows, int64
 /* Projection rows qkv [rows][(n_heads + 2 n_kv_heads) * head_dim] (f32 or bf16, row_stride
  * elements apart, 0: dense) into the cache: per-head RMSNorm of q and k (bf16 weights [head_dim];
  * NULL: none), the rotation of lq_mrope, q to q_out [rows][n_heads][head_dim] (cache type), k and
- * v to the rows' slots. pos_dev NULL: position pos_base + own position, one axis. The norm is f32
- * throughout and everything rounds once; norm_bf16 != 0 rounds its input and output to bf16 as
- * lq_rmsnorm does, bit-identical to lq_qk_norm_rope_kv for head_dim 128. */
+ * v to the rows' slots. head_dim: even, up to 256 (lq_prefix_attention reads 64 and 128). pos_dev
+ * NULL: position pos_base + own position, one axis. The norm is f32 throughout and everything
+ * rounds once; norm_bf16 != 0 rounds its input and output to bf16 as lq_rmsnorm does, bit-identical
+ * to lq_qk_norm_rope_kv for head_dim 128. */
 int lq_paged_append(lq_ctx* ctx, const void* qkv_dev, lq_dtype qkv_dtype, int64_t row_stride, int64_t rows,
                     int64_t n_heads, int64_t n_kv_heads, int64_t head_dim, const uint16_t* q_norm_dev,
                     const uint16_t* k_norm_dev, float eps, int norm_bf16, int64_t rot_dim, const float* cos_dev,
@@ -261,17 +262,18 @@ int lq_paged_append(lq_ctx* ctx, const void* qkv_dev, lq_dtype qkv_dtype, int64_
                     int64_t page_size, int64_t page_stride, void* q_out_dev, int64_t q_out_stride);
 /* Attention of the rows q [rows][n_heads][head_dim] (cache type, q_stride elements apart) over a
  * prefix that all sequences share (positions 0 .. prefix_len-1 in the pages of prefix_table_dev
- * [ceil(prefix_len / page_size)], read once for the batch; prefix_len 0: none) and over the sequence's own positions up to the
- * row itself. head_dim 64 or 128; head h reads kv head h / (n_heads / n_kv_heads). max_q and
- * max_kv are bounds on the rows and own positions of one sequence: they size the launch and the
- * workspace, which the context keeps, one a stream, and grows. Calls captured into a graph have
- * another, kept until lq_destroy: graphs stay valid whatever is called later and may be replayed
- * next to other calls, but those captured on one stream not at the same time as each other. out [rows][n_heads *
- * head_dim] in the cache type and/or Q8_0 rows xq [rows][n_heads * head_dim], xd (either may be
- * NULL). A row that sees nothing gives zeros. Pointers and strides are multiples of 16 bytes (xd_dev: of 2).
- * f32 caches are computed in f32; bf16 ones with bf16 products and f32 sums. What a page holds past
- * a sequence's end is never used; a NaN or infinity in V of a row of this call may reach earlier
- * rows of its sequence. */
+ * [ceil(prefix_len / page_size)], read once for the batch; prefix_len 0: none) and over the
+ * sequence's own positions up to the row itself. head_dim 64 or 128; head h reads kv head
+ * h / (n_heads / n_kv_heads). max_q and max_kv are bounds on the rows and own positions of one
+ * sequence: they size the launch and the workspace, which the context keeps, one a stream, and
+ * grows. Calls captured into a graph have another, kept until lq_destroy: graphs stay valid whatever
+ * is called later and may be replayed next to other calls, but those captured on one stream not at
+ * the same time as each other. out [rows][n_heads * head_dim] in the cache type and/or Q8_0 rows
+ * xq [rows][n_heads * head_dim], xd (either may be NULL). A row that sees nothing gives zeros.
+ * Pointers and strides are multiples of 16 bytes (xd_dev: of 2). Products of f32 caches are 3xTF32
+ * (about 22 bits; infinities give NaN), of bf16 ones bf16, P rounded to it; sums are f32. What a page
+ * holds past a sequence's end is never used; a NaN or infinity in V of a row of this call may reach
+ * earlier rows of its sequence. */
 int lq_prefix_attention(lq_ctx* ctx, const void* q_dev, lq_dtype dtype, int64_t q_stride, int64_t rows,
                         int64_t n_heads, int64_t n_kv_heads, int64_t head_dim, float scale,
                         const void* k_pages_dev, const void* v_pages_dev, int64_t n_pages, int64_t page_size,

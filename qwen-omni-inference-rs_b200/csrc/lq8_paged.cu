@@ -189,8 +189,9 @@ static int launch_mrope(lq_ctx* ctx, const MropeArgs& a, const RopeAxes& rope) {
 // A warp owns some heads of one row; for head dimensions of 64, 128 and 256 that rotate whole a lane
 // holds 8 rotary pairs of a head (both members: 16-byte vectors of either half), D / 16 lanes a
 // head, so that a warp works on 4 heads of 128 dims at a time and has IT times as many in flight.
-// Bound: HBM for large prompts (16 of up to 2000 f32 rows of 32 + 8 heads: 110 us, 6.0 TB/s), the
-// latency of loads that depend on one another for smaller ones (1860 bf16 rows: 23 us).
+// Bound: HBM for large prompts (16 of up to 2000 f32 rows of 32 + 8 heads: 109 us, 6.1 TB/s); for
+// smaller ones instructions (2.2 of 4 a cycle) as much as the latency of loads that depend on one
+// another (1860 bf16 rows: 23 us).
 // =========================================================================================
 struct AppendArgs {
     const void* qkv;
@@ -418,9 +419,9 @@ __global__ void __launch_bounds__(256) paged_append_any_kernel(AppendArgs a, Rop
 template <typename S, typename T, int D>
 static int launch_append_d(lq_ctx* ctx, const AppendArgs& a, const RopeAxes& rope, const PagedSeqs& s) {
     const int heads = a.n_heads + 2 * a.n_kv, side = 512 / D;  // heads side by side in a warp
-    // many rows: four heads a lane in flight (two of f32), which share the row's slot and angles;
-    // a decode step's few rows: one, so that they spread over the SMs
-    constexpr int IT = sizeof(S) == 2 ? 2 : 2;
+    // many rows: two heads a lane in flight, which share the row's slot and angles; a decode step's
+    // few rows: one, so that they spread over the SMs
+    constexpr int IT = 2;
     const bool few = (int64_t)s.rows * ceil_div(heads, side) < 16ll * ctx->sm_count;
     const int groups = ceil_div(heads, few ? side : side * IT);
     const dim3 grid((unsigned)ceil_div((int64_t)s.rows * groups, 8));

@@ -11,10 +11,13 @@
 // products is free, so a lane's elements of K (4 dims of 2 positions) and of V (4 dims of 4
 // positions) are 16-byte vectors; the rows are padded so that a warp's reads meet no bank twice. No
 // warp waits for another; the running maximum and sum of a row lie in the lanes that hold its scores.
-// Bound: HBM where few rows share a position (8 rows: 96 MMAs and about 500 other instructions per
-// 16 KB), the MMA and split instructions where many do. 8 sequences of 64 heads behind 1024
-// positions: 27 us (1.1 TB/s, IPC 1.5, tensor pipe 20 %), 48 with loads into registers; 64 sequences
-// of 32 heads behind 4096: 228 us (20 TFLOP/s) with the merge.
+// Bound: the latency of a step's chain (copy, split, MMA, shuffles, exponential, MMA), which two
+// warps a scheduler (255 registers a thread) do not hide: no unit is busy. A step of 16 positions
+// takes 96 MMAs and about 500 other instructions, and every block of 8 rows splits K and V for
+// itself. 8 sequences of 64 heads behind 1024 positions: 27 us (1.1 TB/s, 1.5 instructions of 4 a
+// cycle, tensor pipe 20 %), 48 with loads into registers; 64 sequences of 32 heads behind 4096: 230 us
+// (20 TFLOP/s) with the merge. An infinity has no second part (it minus itself), so that one in
+// Q, K or V gives NaN.
 #include "lq8_async.cuh"
 #include "lq8_fused.cuh"
 #include "lq8_prefix_attn.cuh"

@@ -4,7 +4,7 @@
 // Query rows of one kv head are stacked: token t's heads g < G of the group are rows t G + g, so
 // that all sequences' rows form the tiles of the prefix (its K/V are read once for the batch),
 // and one sequence's rows the tiles of its own positions. An item is (kv head, row block); a step
-// is one 128-position (f32: 64) tile of an item. Steps of all items form one line, prefix items
+// is one 128-position (f32: 32) tile of an item. Steps of all items form one line, prefix items
 // first, then the sequences' own, and every worker takes an equal share of it: no split factors,
 // no empty workers, whatever the mix of lengths. An item cut between workers leaves one partial
 // (o, m, l) per worker, which the merge kernel joins in order.
@@ -142,7 +142,7 @@ struct Line {
     int sp, so, n;
     bool pair_p, pair_o;
     int quot, rem;     // W / n
-    uint64_t mul;      // ceil(2^40 / n): x / n = x mul / 2^40, exact for x < 2^32
+    uint64_t mul;      // ceil(2^40 / n): x / n = x mul / 2^40, exact while x n < 2^40 (x < 2^28, n < 2^11)
     __host__ __device__ __forceinline__ Line(const PrefixPlan& p, int own_steps, bool pair_prefix, bool pair_own)
         : sp(p.sp), so(own_steps), n(p.workers), pair_p(pair_prefix), pair_o(pair_own), mul(p.workers_mul) {
         split = sp * (pair_p ? 3 : 2);

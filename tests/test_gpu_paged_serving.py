@@ -4,7 +4,7 @@ tolerances are those of test_gpu_paged.py."""
 import numpy as np
 import pytest
 
-from test_gpu_paged import Setup, attention_case, i32, randn
+from test_gpu_paged import U, Setup, attention64, attention_case, i32, randn, within
 
 pytestmark = pytest.mark.gpu
 
@@ -18,6 +18,26 @@ def test_attention_of_ragged_decode_batches(ctx, lq8_lib, kv, prefix):
     """Batches whose CTAs have flows of very unequal length (their schedules end by the CPU's model,
     test_prefix_schedule.py)."""
     attention_case(ctx, lq8_lib, "bf16", kv, [1] * len(kv), 8, 8, 64, 128, prefix)
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "f32"])
+def test_attention_in_another_batch_order(ctx, lq8_lib, dtype):
+    """The same sequences in another order: each result within the tolerance, whatever shares its
+    tiles (the bits may differ)."""
+    import torch
+    kv, n = [600, 90, 33, 1, 250] * 8, 40
+    s = Setup(lq8_lib, ctx, dtype, kv, [1] * n, 4, 128, 16, 2000, seed=12).fill()
+    x = randn(12, n, 16, 128, scale=1.5, dtype=dtype)
+    want, mass = attention64(s, x, 128 ** -0.5)
+    for seed in range(3):
+        order = np.random.default_rng(seed).permutation(n)
+        at = i32(order).long()
+        b = lq8_lib.PagedBatch(s.batch.page_table[at].contiguous(), s.batch.kv_len[at], max_kv=600, prefix_table=s.batch.prefix_table,
+                               prefix_len=2000)
+        out = torch.empty_like(x)
+        out[at] = s.cache.attend(x[at], b)
+        within(out, want, (U[dtype] + 2e-5) * mass + U[dtype] * want.abs())
+    ctx.device_status()
 
 
 @pytest.mark.parametrize("kv,q,prefix,page", [
