@@ -226,7 +226,8 @@ int lq_fill_bf16(lq_ctx* ctx, uint64_t seed, uint64_t tensor_id, int64_t offset,
  * one), and kv_len_dev[b] is its number of own positions, those rows included, which come last.
  * Rows past the last sequence's are padding: what they hold has no effect, and nothing is written
  * for them. Positions outside the tables, lengths outside the page table and page ids outside the
- * cache skip the access and are reported by lq_device_status. Pointers are aligned to their
+ * cache skip the access and are reported by lq_device_status; so are row starts that fall, with which
+ * the attention computes nothing. Pointers are aligned to their
  * elements.
  * ------------------------------------------------------------------------------------- */
 /* Waits for the context's stream; LQ_ERR_INVALID_ARG with the first code and value that a

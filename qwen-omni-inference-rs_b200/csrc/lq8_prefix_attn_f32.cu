@@ -90,19 +90,21 @@ prefix_attn_f32_kernel(const __grid_constant__ PrefixAttnArgs a, const __grid_co
         return __reduce_add_sync(0xffffffffu, n);
     };
     const bool by_warp = a.max_q * a.group > 8 * p.ob;
+    bool fell = false;
 #pragma unroll 1
     for (int e = by_warp ? warp : tid; e < n_entries; e += by_warp ? PF_WARPS : PF_WARPS * 32) {
         int n = 0;
 #pragma unroll 1
         for (int b = e * per_entry; b < min(s.n_seqs, (e + 1) * per_entry); b++) {
             const SeqInfo si = seq_info(a, s, b, blockIdx.x == 0);
+            fell |= falls(s, b);
             const int per = by_warp ? per_head(si) : os.per_head(si);
             n += per * a.n_kv;
             if (per_entry == 1) info[b] = make_int4(si.q0, si.q, si.kv, per);
         }
         scan[e + 1] = n;
     }
-    __syncthreads();
+    fell = __syncthreads_or(fell);
     if (warp == 0) {
         int run = 0;
 #pragma unroll 1
@@ -119,7 +121,7 @@ prefix_attn_f32_kernel(const __grid_constant__ PrefixAttnArgs a, const __grid_co
         if (lane == 0) scan[0] = 0;
     }
     __syncthreads();
-    const int so = scan[n_entries];
+    const int so = fell ? 0 : scan[n_entries];
     if (blockIdx.x == 0 && tid == 0) *p.own_steps = so;
     if (a.prefix_len == 0) {  // rows before their sequence's first position see nothing
 #pragma unroll 1

@@ -282,19 +282,21 @@ prefix_attn_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_co
     const int n_entries = per_entry == 1 ? g.s.n_seqs : (g.s.n_seqs + per_entry - 1) / per_entry;
     const OwnSteps os{g.a, g.p};
     const bool by_warp = PO && per_entry == 1 && g.a.max_q * g.a.group > 4 * g.p.ob;
+    bool fell = false;
 #pragma unroll 1
     for (int e = by_warp ? warp : tid; e < n_entries; e += by_warp ? PA_THREADS / 32 : PA_THREADS) {
         int n = 0;
 #pragma unroll 1
         for (int b = e * per_entry; b < min(g.s.n_seqs, (e + 1) * per_entry); b++) {
             const SeqInfo si = seq_info(g.a, g.s, b, blockIdx.x == 0);
+            fell |= falls(g.s, b);
             const int per = !PO ? (si.q > 0 ? os.steps(si, 0) : 0) : by_warp ? per_head_warp(os, si, lane) : os.per_head(si);
             n += per * g.a.n_kv;
             if (per_entry == 1) c.info[b] = make_int4(si.q0, si.q, si.kv, per);
         }
         c.scan[e + 1] = n;
     }
-    __syncthreads();
+    fell = __syncthreads_or(fell);
     if (warp == 0) {
         int run = 0;
 #pragma unroll 1
@@ -309,7 +311,7 @@ prefix_attn_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_co
     __syncthreads();
     tc_after();
     const uint32_t tmem = __shfl_sync(0xffffffffu, c.tmem, 0);
-    const int so = c.scan[n_entries];
+    const int so = fell ? 0 : c.scan[n_entries];
     if (blockIdx.x == 0 && tid == 0) *g.p.own_steps = so;  // for the merge
     const int me = blockIdx.x, polls = g.p.polls;
     // own items count positions from the first tile of the prefix they begin with, whose last tile

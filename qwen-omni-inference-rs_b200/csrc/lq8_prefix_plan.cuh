@@ -98,6 +98,10 @@ __device__ __forceinline__ SeqInfo seq_info(const PrefixAttnArgs& a, const Paged
     return r;
 }
 
+// Whether the next sequence's rows begin before this one's. Such a batch may name a row several times,
+// and more steps than the plan has numbers for: it gets none.
+__device__ __forceinline__ bool falls(const PagedSeqs& s, int b) { return s.q_start && s.q_start[b + 1] < s.q_start[b]; }
+
 // rows before the padding: those that the prefix's blocks hold
 __device__ __forceinline__ int live_rows(const PagedSeqs& s) {
     return s.q_start ? min(max(s.q_start[s.n_seqs], 0), s.rows) : s.rows;

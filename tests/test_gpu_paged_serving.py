@@ -379,3 +379,23 @@ def test_mrope_refuses_rows_and_heads_of_the_output_that_overlap(ctx, lq8_lib):
     one = torch.as_strided(buf, (5, 1, 64), (64, 0, 1))
     assert torch.equal(lq8_lib.mrope(ctx, x[:, :1], rot, pos, out=one), want[:, :1])
     ctx.device_status()
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "f32"])
+@pytest.mark.parametrize("prefix", [0, 300])
+@pytest.mark.parametrize("starts", [[0, 4, 2, 6], [0, 6, 0, 6], [0, 3, 6, 5]])
+def test_row_starts_that_fall_are_reported(ctx, lq8_lib, dtype, prefix, starts):
+    """Such a batch names rows several times, and with many sequences more work than a launch can
+    number: nothing of it is computed."""
+    import torch
+    s = Setup(lq8_lib, ctx, dtype, [30, 50, 70], [2, 2, 2], 2, 128, 16, prefix, seed=6, garbage=False).fill()
+    s.batch.max_q = 6  # (the bounds of a call shape its sums: the same ones throughout)
+    x = randn(1, 6, 8, 128, dtype=dtype)
+    want = s.cache.attend(x, s.batch).clone()
+    s.batch.q_start.copy_(i32(starts))
+    s.cache.attend(x, s.batch)
+    with pytest.raises(lq8_lib.LQ8Error, match="code 93"):
+        ctx.device_status()
+    s.batch.q_start.copy_(i32([0, 2, 4, 6]))
+    assert torch.equal(s.cache.attend(x, s.batch), want)
+    ctx.device_status()
