@@ -93,8 +93,8 @@ __device__ __forceinline__ void flag_positions(const RopeAxes& rope, int64_t row
 // x_i and of x_{i+n}) of H heads of one row: the angles are gathered once for the heads, and 2 H
 // 16-byte loads are in flight before the first use. A CTA takes whole rows, so that DRAM sees runs
 // of all their heads (a thread that walks over all heads of a row instead, with the CTA spread over
-// 32 rows: 180 against 123 us for 32768 rows of 40 heads). Bound: HBM; those rows in 121 to 128 us
-// (5.4 TB/s, 83 % of a plain copy), 4805 rows of 32 + 16 heads of 80 dims in f32 in 20 us.
+// 32 rows: 180 against 123 us for 32768 rows of 40 heads). Bound: HBM; those rows in 121 to 126 us
+// (5.5 TB/s, 85 % of a plain copy), 4805 rows of 32 + 16 heads of 80 dims in f32 in 20 us.
 // =========================================================================================
 struct MropeArgs {
     const void* x;
@@ -190,7 +190,7 @@ static int launch_mrope(lq_ctx* ctx, const MropeArgs& a, const RopeAxes& rope) {
 // holds 8 rotary pairs of a head (both members: 16-byte vectors of either half), D / 16 lanes a
 // head, so that a warp works on 4 heads of 128 dims at a time and has IT times as many in flight.
 // Bound: HBM for large prompts (16 of up to 2000 f32 rows of 32 + 8 heads: 109 us, 6.1 TB/s); for
-// smaller ones instructions (2.2 of 4 a cycle) as much as the latency of loads that depend on one
+// smaller ones instructions (2.1 of 4 a cycle) as much as the latency of loads that depend on one
 // another (1860 bf16 rows: 23 us).
 // =========================================================================================
 struct AppendArgs {

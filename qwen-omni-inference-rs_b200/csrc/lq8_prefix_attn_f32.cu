@@ -14,8 +14,8 @@
 // Bound: the latency of a step's chain (copy, split, MMA, shuffles, exponential, MMA), which two
 // warps a scheduler (255 registers a thread) do not hide: no unit is busy. A step of 16 positions
 // takes 96 MMAs and about 500 other instructions, and every block of 8 rows splits K and V for
-// itself. 8 sequences of 64 heads behind 1024 positions: 27 us (1.1 TB/s, 1.5 instructions of 4 a
-// cycle, tensor pipe 20 %), 48 with loads into registers; 64 sequences of 32 heads behind 4096: 230 us
+// itself. 8 sequences of 64 heads behind 1024 positions: 27 us (1.1 TB/s, 1.4 instructions of 4 a
+// cycle, tensor pipe 18 %), 48 with loads into registers; 64 sequences of 32 heads behind 4096: 230 us
 // (20 TFLOP/s) with the merge. An infinity has no second part (it minus itself), so that one in
 // Q, K or V gives NaN.
 #include "lq8_async.cuh"

@@ -28,9 +28,9 @@
 // Bound: a round of two 128-row halves at D = 128 needs 2048 cycles of the tensor pipe and as many
 // of the exponentials'; it takes 3550, of which the MMA warp issues for 2880 (QK reads both operands
 // from shared memory at its full rate: 86 cycles an MMA instead of 64) and waits 670 for copies and
-// P. 128 sequences of 64 heads behind 32768 positions: 167 us for the prefix (824 TFLOP/s), 200 us
+// P. 128 sequences of 64 heads behind 32768 positions: 164 us for the prefix (837 TFLOP/s), 200 us
 // with 1000 own positions; 64 sequences of 32 heads behind 8191: 51 us (3.3 TB/s); 4 chunks of 1000
-// tokens behind 8192: 470 us (1056 TFLOP/s), all from cold L2, the merge in the first and last.
+// tokens behind 8192: 474 us (1047 TFLOP/s), all from cold L2, the merge in the first and last.
 //
 // TMA loads here read only this GPU's memory and use no multicast.
 #include "lq8_async.cuh"
