@@ -232,7 +232,7 @@ int lq_fill_bf16(lq_ctx* ctx, uint64_t seed, uint64_t tensor_id, int64_t offset,
  * ------------------------------------------------------------------------------------- */
 /* Waits for the context's stream; LQ_ERR_INVALID_ARG with the first code and value that a
  * kernel flagged since the last check (90 rotary position, 91 length, 92 page id, 93 row
- * count, 94 and 95 a wait inside the attention that ran out: its output is not valid). */
+ * count, 94 to 96 a wait inside the attention that ran out: its output is not valid). */
 int lq_device_status(lq_ctx* ctx);
 /* Rotary positions with one to four axes (e.g. time, height, width). x [rows][heads][head_dim]
  * f32 or bf16 with the given strides (elements) to out (may be x): pair i < rot_dim/2 of a head
@@ -282,6 +282,50 @@ int lq_prefix_attention(lq_ctx* ctx, const void* q_dev, lq_dtype dtype, int64_t 
                         const int32_t* q_start_dev, const int32_t* kv_len_dev, const int32_t* page_table_dev,
                         int64_t table_ld, int64_t max_q, int64_t max_kv, void* out_dev, int64_t out_stride,
                         int8_t* xq_dev, uint16_t* xd_dev);
+
+/* ---------------------------------------------------------------------------------------
+ * The paged cache held in 8 bits: K and V are int8 codes [n_pages][n_kv_heads][page_size][head_dim]
+ * (page_stride codes from page to page, a multiple of 16; 0: dense) and f32 scales
+ * [n_pages][n_kv_heads][page_size / block] (scale_stride scales from page to page, 0: dense), one for
+ * every `block` positions of a kv head (16, 32, 64 or 128, no more than page_size). A value is
+ * code * scale. head_dim is 64 or 128, codes are aligned to 16 bytes, page_size is 16 to 256; sequences,
+ * rows and what is skipped and reported are as above. The sequences of one call append to pages of
+ * their own: a block that two of them append to holds anything afterwards.
+ * ------------------------------------------------------------------------------------- */
+/* lq_paged_append into such a cache. q to q_out as bf16. For the call's rows of one block and kv head,
+ * with a the largest |x|: the scale becomes a / 127 where they begin the block, and the larger of
+ * a / 127 and the present scale where older positions do; if it grows, the older codes become
+ * rint(code * old / new). New codes are rint(x / scale), computed in f32. An infinity or a NaN makes
+ * the scale NaN, and the block reads as NaN until its first position is appended again; a scale
+ * below 2^-126 becomes zero. */
+int lq_paged_append_q8(lq_ctx* ctx, const void* qkv_dev, lq_dtype qkv_dtype, int64_t row_stride, int64_t rows,
+                       int64_t n_heads, int64_t n_kv_heads, int64_t head_dim, const uint16_t* q_norm_dev,
+                       const uint16_t* k_norm_dev, float eps, int norm_bf16, int64_t rot_dim, const float* cos_dev,
+                       const float* sin_dev, int64_t table_len, const uint8_t* pair_axis_host, int64_t n_axes,
+                       const int32_t* pos_dev, int64_t pos_stride, int64_t pos_base, int64_t n_seqs,
+                       const int32_t* q_start_dev, const int32_t* kv_len_dev, const int32_t* page_table_dev,
+                       int64_t table_ld, int8_t* k_codes_dev, int8_t* v_codes_dev, float* k_scale_dev,
+                       float* v_scale_dev, int64_t n_pages, int64_t page_size, int64_t page_stride, int64_t block,
+                       int64_t scale_stride, uint16_t* q_out_dev, int64_t q_out_stride);
+/* Reads the rows of a batch (the last q_start[b+1] - q_start[b] of sequence b's kv_len[b] positions, as the
+ * append places them; all of them with row starts that are the sums of the lengths) as code * scale
+ * to k_out, v_out [rows][n_kv_heads][head_dim] (f32, or bf16 rounded to nearest), out_stride elements
+ * apart (0: dense); 16-byte aligned. Rows without a slot stay as they were. */
+int lq_paged_read_q8(lq_ctx* ctx, const int8_t* k_codes_dev, const int8_t* v_codes_dev, const float* k_scale_dev,
+                     const float* v_scale_dev, int64_t n_kv_heads, int64_t head_dim, int64_t n_pages,
+                     int64_t page_size, int64_t page_stride, int64_t block, int64_t scale_stride, int64_t n_seqs,
+                     const int32_t* q_start_dev, const int32_t* kv_len_dev, const int32_t* page_table_dev,
+                     int64_t table_ld, int64_t rows, void* k_out_dev, void* v_out_dev, lq_dtype out_dtype,
+                     int64_t out_stride);
+/* lq_prefix_attention over such a cache, q and out bf16. */
+int lq_prefix_attention_q8(lq_ctx* ctx, const uint16_t* q_dev, int64_t q_stride, int64_t rows, int64_t n_heads,
+                           int64_t n_kv_heads, int64_t head_dim, float scale, const int8_t* k_codes_dev,
+                           const int8_t* v_codes_dev, const float* k_scale_dev, const float* v_scale_dev,
+                           int64_t n_pages, int64_t page_size, int64_t page_stride, int64_t block,
+                           int64_t scale_stride, const int32_t* prefix_table_dev, int64_t prefix_len, int64_t n_seqs,
+                           const int32_t* q_start_dev, const int32_t* kv_len_dev, const int32_t* page_table_dev,
+                           int64_t table_ld, int64_t max_q, int64_t max_kv, uint16_t* out_dev, int64_t out_stride,
+                           int8_t* xq_dev, uint16_t* xd_dev);
 
 /* ---------------------------------------------------------------------------------------
  * Tensor parallelism over NCCL (one process per GPU; the reference is single-device).

@@ -222,9 +222,10 @@ __global__ void __launch_bounds__(256, MR == 32 ? 5 : 4) prefix_attn_merge_kerne
 }
 
 // the plan of a call and its workspace
-static int make_plan(lq_ctx* ctx, const PrefixAttnArgs& a, const PagedSeqs& s, bool f32, int D, PrefixPlan* p) {
-    const int64_t steps = plan_cut(a, s, f32, ctx->sm_count, p);
-    LQ_REQUIRE(ctx, steps < PREFIX_MAX_STEPS, "lq_prefix_attention: %lld steps, more than a launch can number", (long long)steps);
+static int make_plan(lq_ctx* ctx, const char* who, const PrefixAttnArgs& a, const PagedSeqs& s, bool f32, int D, PrefixPlan* p,
+                     int warp_rows = 8) {
+    const int64_t steps = plan_cut(a, s, f32, ctx->sm_count, p, warp_rows);
+    LQ_REQUIRE(ctx, steps < PREFIX_MAX_STEPS, "%s: %lld steps, more than a launch can number", who, (long long)steps);
     // LQ_FAULT=prefix_attn_wait: waits inside the kernel run out (tests of what follows then)
     p->hold = fault_injected("prefix_attn_wait");
     p->polls = !p->hold ? 1 << 22 : f32 ? 0 : 1 << 12;
@@ -241,7 +242,7 @@ static int make_plan(lq_ctx* ctx, const PrefixAttnArgs& a, const PagedSeqs& s, b
     size_t first_at[2], last_at[2], ml_at[2], o_at[2];
     for (int k = 0; k < 2; k++) {
         const int64_t slots = k == 1 && p->np == 0 ? 4 * p->workers : items[k] ? items[k] + 2 * p->workers : 0;
-        LQ_REQUIRE(ctx, slots < (1ll << 31), "lq_prefix_attention: too many partials");
+        LQ_REQUIRE(ctx, slots < (1ll << 31), "%s: too many partials", who);
         first_at[k] = place(items[k], 4);
         last_at[k] = place(items[k], 4);
         ml_at[k] = place(slots * p->cap[k], 8);
@@ -273,6 +274,54 @@ static int launch_merge(lq_ctx* ctx, const PrefixAttnArgs& a, const PagedSeqs& s
                    : launch_kernel(ctx, prefix_attn_merge_kernel<T, D, 32>, grid, dim3(256), 0, "prefix_attn_merge", a, s, p);
 }
 
+// checks and arguments shared by the entry points; esize: bytes of an element of q and out. page_stride:
+// in elements of the cache, which is checked by the caller
+static int make_attn_args(lq_ctx* ctx, const char* who, PrefixAttnArgs* a, PagedSeqs* s, const void* q, size_t esize, int64_t q_stride,
+                          int64_t rows, int64_t n_heads, int64_t n_kv_heads, int64_t head_dim, float scale, int64_t n_pages,
+                          int64_t page_size, const int32_t* prefix_table, int64_t prefix_len, int64_t n_seqs,
+                          const int32_t* q_start, const int32_t* kv_len, const int32_t* page_table, int64_t table_ld,
+                          int64_t max_q, int64_t max_kv, void* out, int64_t out_stride, int8_t* xq, uint16_t* xd) {
+    LQ_REQUIRE(ctx, n_heads >= 1 && n_kv_heads >= 1 && n_heads % n_kv_heads == 0 && n_heads <= 4096, "%s: bad head counts", who);
+    LQ_REQUIRE(ctx, n_heads / n_kv_heads <= 128, "%s: more than 128 query heads a kv head", who);
+    LQ_REQUIRE(ctx, head_dim == 64 || head_dim == 128, "%s: head_dim %lld must be 64 or 128", who, (long long)head_dim);
+    const int rc = make_paged_seqs(ctx, who, s, n_seqs, q_start, kv_len, page_table, table_ld, rows, n_pages, page_size);
+    if (rc) return rc;
+    if (q_stride == 0) q_stride = n_heads * head_dim;
+    if (out_stride == 0) out_stride = n_heads * head_dim;
+    LQ_REQUIRE(ctx, q_stride >= n_heads * head_dim && out_stride >= n_heads * head_dim, "%s: row stride too small", who);
+    LQ_REQUIRE(ctx, prefix_len >= 0 && prefix_len < (1ll << 30) && (prefix_len == 0 || prefix_table), "%s: bad prefix", who);
+    LQ_REQUIRE(ctx, aligned_to(prefix_table, 4), "%s: the prefix's page table must be aligned to its elements", who);
+    LQ_REQUIRE(ctx, max_q >= 1 && max_q < (1ll << 24) && max_kv >= 0 && max_kv < (1ll << 30),
+               "%s: bad bounds max_q %lld, max_kv %lld", who, (long long)max_q, (long long)max_kv);
+    LQ_REQUIRE(ctx, scale > 0.0f && scale < INFINITY, "%s: scale must be positive and finite", who);
+    LQ_REQUIRE(ctx, (xq == nullptr) == (xd == nullptr), "%s: xq and xd go together", who);
+    LQ_REQUIRE(ctx, rows * n_heads < (1ll << 28), "%s: too many rows", who);
+    if (rows == 0 || n_seqs == 0) return LQ_OK;
+    LQ_REQUIRE(ctx, q && (out || xq), "%s: NULL pointer", who);
+    LQ_REQUIRE(ctx, aligned_to(q, 16) && aligned_to(out, 16) && aligned_to(xq, 16) && aligned_to(xd, 2) &&
+                        q_stride * esize % 16 == 0 && out_stride * esize % 16 == 0,
+               "%s: pointers and strides must be multiples of 16 bytes (xd: of 2)", who);
+    a->q = q;
+    a->q_stride = q_stride;
+    a->n_heads = (int)n_heads;
+    a->n_kv = (int)n_kv_heads;
+    a->group = (int)(n_heads / n_kv_heads);
+    a->group_mul = ((1ull << 36) + a->group - 1) / a->group;
+    a->scale = scale;
+    a->k = a->v = nullptr;
+    a->page_stride = 0;
+    a->prefix_table = prefix_table;
+    a->prefix_len = (int)prefix_len;
+    a->max_q = (int)max_q;
+    a->max_kv = (int)max_kv;
+    a->out = out;
+    a->out_stride = out_stride;
+    a->xq = xq;
+    a->xd = xd;
+    a->err = ctx->err_flag;
+    return LQ_OK;
+}
+
 }  // namespace lq
 
 extern "C" int lq_prefix_attention(lq_ctx* ctx, const void* q, lq_dtype dtype, int64_t q_stride, int64_t rows,
@@ -284,62 +333,57 @@ extern "C" int lq_prefix_attention(lq_ctx* ctx, const void* q, lq_dtype dtype, i
                                    int8_t* xq, uint16_t* xd) {
     LQ_ENTRY(ctx, "lq_prefix_attention");
     LQ_REQUIRE(ctx, dtype == LQ_DTYPE_F32 || dtype == LQ_DTYPE_BF16, "lq_prefix_attention: dtype must be F32 or BF16");
-    LQ_REQUIRE(ctx, n_heads >= 1 && n_kv_heads >= 1 && n_heads % n_kv_heads == 0 && n_heads <= 4096,
-               "lq_prefix_attention: bad head counts");
-    LQ_REQUIRE(ctx, n_heads / n_kv_heads <= 128, "lq_prefix_attention: more than 128 query heads a kv head");
-    LQ_REQUIRE(ctx, head_dim == 64 || head_dim == 128, "lq_prefix_attention: head_dim %lld must be 64 or 128",
-               (long long)head_dim);
+    const bool f32 = dtype == LQ_DTYPE_F32;
+    const size_t esize = f32 ? 4 : 2;
+    lq::PrefixAttnArgs a;
     lq::PagedSeqs s;
-    int rc = lq::make_paged_seqs(ctx, "lq_prefix_attention", &s, n_seqs, q_start, kv_len, page_table, table_ld, rows,
-                                 n_pages, page_size);
+    int rc = lq::make_attn_args(ctx, "lq_prefix_attention", &a, &s, q, esize, q_stride, rows, n_heads, n_kv_heads, head_dim, scale,
+                                n_pages, page_size, prefix_table, prefix_len, n_seqs, q_start, kv_len, page_table, table_ld,
+                                max_q, max_kv, out, out_stride, xq, xd);
     if (rc) return rc;
     if (page_stride == 0) page_stride = n_kv_heads * page_size * head_dim;
-    if (q_stride == 0) q_stride = n_heads * head_dim;
-    if (out_stride == 0) out_stride = n_heads * head_dim;
     LQ_REQUIRE(ctx, page_stride >= n_kv_heads * page_size * head_dim, "lq_prefix_attention: page_stride too small");
-    LQ_REQUIRE(ctx, q_stride >= n_heads * head_dim && out_stride >= n_heads * head_dim,
-               "lq_prefix_attention: row stride too small");
-    LQ_REQUIRE(ctx, prefix_len >= 0 && prefix_len < (1ll << 30) && (prefix_len == 0 || prefix_table),
-               "lq_prefix_attention: bad prefix");
-    LQ_REQUIRE(ctx, lq::aligned_to(prefix_table, 4), "lq_prefix_attention: the prefix's page table must be aligned to its elements");
-    LQ_REQUIRE(ctx, max_q >= 1 && max_q < (1ll << 24) && max_kv >= 0 && max_kv < (1ll << 30),
-               "lq_prefix_attention: bad bounds max_q %lld, max_kv %lld", (long long)max_q, (long long)max_kv);
-    LQ_REQUIRE(ctx, scale > 0.0f && scale < INFINITY, "lq_prefix_attention: scale must be positive and finite");
-    LQ_REQUIRE(ctx, (xq == nullptr) == (xd == nullptr), "lq_prefix_attention: xq and xd go together");
-    LQ_REQUIRE(ctx, rows * n_heads < (1ll << 28), "lq_prefix_attention: too many rows");
     if (rows == 0 || n_seqs == 0) return LQ_OK;
-    LQ_REQUIRE(ctx, q && k_pages && v_pages && (out || xq), "lq_prefix_attention: NULL pointer");
-    const size_t esize = dtype == LQ_DTYPE_F32 ? 4 : 2;
-    auto al = [](const void* p) { return (uintptr_t)p % 16 == 0; };
-    LQ_REQUIRE(ctx, al(q) && al(k_pages) && al(v_pages) && al(out) && al(xq) && lq::aligned_to(xd, 2) && q_stride * esize % 16 == 0 &&
-                        out_stride * esize % 16 == 0 && page_stride * esize % 16 == 0,
+    LQ_REQUIRE(ctx, k_pages && v_pages, "lq_prefix_attention: NULL pointer");
+    LQ_REQUIRE(ctx, lq::aligned_to(k_pages, 16) && lq::aligned_to(v_pages, 16) && page_stride * esize % 16 == 0,
                "lq_prefix_attention: pointers and strides must be multiples of 16 bytes (xd: of 2)");
-    lq::PrefixAttnArgs a;
-    a.q = q;
-    a.q_stride = q_stride;
-    a.n_heads = (int)n_heads;
-    a.n_kv = (int)n_kv_heads;
-    a.group = (int)(n_heads / n_kv_heads);
-    a.group_mul = ((1ull << 36) + a.group - 1) / a.group;
-    a.scale = scale;
     a.k = k_pages;
     a.v = v_pages;
     a.page_stride = page_stride;
-    a.prefix_table = prefix_table;
-    a.prefix_len = (int)prefix_len;
-    a.max_q = (int)max_q;
-    a.max_kv = (int)max_kv;
-    a.out = out;
-    a.out_stride = out_stride;
-    a.xq = xq;
-    a.xd = xd;
-    a.err = ctx->err_flag;
     lq::PrefixPlan p;
-    const bool f32 = dtype == LQ_DTYPE_F32;
     const int D = (int)head_dim;
-    if ((rc = lq::make_plan(ctx, a, s, f32, D, &p))) return rc;
+    if ((rc = lq::make_plan(ctx, "lq_prefix_attention", a, s, f32, D, &p))) return rc;
     rc = f32 ? lq::launch_prefix_attn_f32(ctx, a, s, p, D) : lq::launch_prefix_attn_tc(ctx, a, s, p, D);
     if (rc) return rc;
     if (f32) return D == 64 ? lq::launch_merge<float, 64>(ctx, a, s, p) : lq::launch_merge<float, 128>(ctx, a, s, p);
+    return D == 64 ? lq::launch_merge<__nv_bfloat16, 64>(ctx, a, s, p) : lq::launch_merge<__nv_bfloat16, 128>(ctx, a, s, p);
+}
+
+extern "C" int lq_prefix_attention_q8(lq_ctx* ctx, const uint16_t* q, int64_t q_stride, int64_t rows, int64_t n_heads,
+                                      int64_t n_kv_heads, int64_t head_dim, float scale, const int8_t* k_codes,
+                                      const int8_t* v_codes, const float* k_scale, const float* v_scale, int64_t n_pages,
+                                      int64_t page_size, int64_t page_stride, int64_t block, int64_t scale_stride,
+                                      const int32_t* prefix_table, int64_t prefix_len, int64_t n_seqs, const int32_t* q_start,
+                                      const int32_t* kv_len, const int32_t* page_table, int64_t table_ld, int64_t max_q,
+                                      int64_t max_kv, uint16_t* out, int64_t out_stride, int8_t* xq, uint16_t* xd) {
+    LQ_ENTRY(ctx, "lq_prefix_attention_q8");
+    lq::PrefixAttnArgs a;
+    lq::PagedSeqs s;
+    lq::PagedQ8 c;
+    int rc = lq::make_attn_args(ctx, "lq_prefix_attention_q8", &a, &s, q, 2, q_stride, rows, n_heads, n_kv_heads, head_dim, scale,
+                                n_pages, page_size, prefix_table, prefix_len, n_seqs, q_start, kv_len, page_table, table_ld,
+                                max_q, max_kv, out, out_stride, xq, xd);
+    if (rc) return rc;
+    rc = lq::make_paged_q8(ctx, "lq_prefix_attention_q8", &c, const_cast<int8_t*>(k_codes), const_cast<int8_t*>(v_codes),
+                           const_cast<float*>(k_scale), const_cast<float*>(v_scale), n_kv_heads, head_dim, page_size, page_stride,
+                           block, scale_stride, rows > 0 && n_seqs > 0);
+    if (rc) return rc;
+    if (rows == 0 || n_seqs == 0) return LQ_OK;
+    const int D = (int)head_dim;
+    lq::PrefixPlan p;
+    const int64_t stacked = (prefix_len > 0 ? rows : std::min(max_q, rows)) * a.group;
+    if ((rc = lq::make_plan(ctx, "lq_prefix_attention_q8", a, s, true, D, &p, stacked > 8 ? 16 : 8))) return rc;
+    rc = lq::launch_prefix_attn_q8(ctx, a, s, c, p, D);
+    if (rc) return rc;
     return D == 64 ? lq::launch_merge<__nv_bfloat16, 64>(ctx, a, s, p) : lq::launch_merge<__nv_bfloat16, 128>(ctx, a, s, p);
 }

@@ -2,6 +2,7 @@
 #pragma once
 
 #include "lq8_fused.cuh"
+#include "lq8_paged_q8.cuh"
 #include "lq8_prefix_plan.cuh"
 
 namespace lq {
@@ -88,6 +89,7 @@ __device__ __forceinline__ void zero_rows(const PrefixAttnArgs& a, int tok0, int
 }
 
 int launch_prefix_attn_f32(lq_ctx* ctx, const PrefixAttnArgs& a, const PagedSeqs& s, const PrefixPlan& p, int D);
+int launch_prefix_attn_q8(lq_ctx* ctx, const PrefixAttnArgs& a, const PagedSeqs& s, const PagedQ8& c, const PrefixPlan& p, int D);
 int launch_prefix_attn_tc(lq_ctx* ctx, const PrefixAttnArgs& a, const PagedSeqs& s, const PrefixPlan& p, int D);
 
 }  // namespace lq

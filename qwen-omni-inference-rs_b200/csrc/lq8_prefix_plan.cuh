@@ -194,11 +194,12 @@ __host__ __device__ __forceinline__ HandOut hand_out(int f, bool first, bool liv
 // PREFIX_MAX_STEPS before the plan is used
 constexpr int64_t PREFIX_MAX_STEPS = 1ll << 26;
 constexpr int PREFIX_ATTN_F32_WARPS = 8;  // workers of a CTA of the f32 kernel
-inline int64_t plan_cut(const PrefixAttnArgs& a, const PagedSeqs& s, bool f32, int sm_count, PrefixPlan* p) {
+inline int64_t plan_cut(const PrefixAttnArgs& a, const PagedSeqs& s, bool f32, int sm_count, PrefixPlan* p, int warp_rows = 8) {
     const int64_t R = (int64_t)s.rows * a.group, most_q = std::min<int64_t>((int64_t)a.max_q, s.rows) * a.group;
     // bf16: blocks of 128 rows, or two halves of 128 that share their K and V tiles; a worker is a
-    // CTA with paired halves, else one of its two flows. f32: blocks of 8 rows, a worker is a warp.
-    const int half = f32 ? 8 : 128, tile = f32 ? 32 : 128;
+    // CTA with paired halves, else one of its two flows. f32: blocks of 8 rows (warp_rows), a worker is a
+    // warp.
+    const int half = f32 ? warp_rows : 128, tile = f32 ? 32 : 128;
     p->tile = tile;
     p->pair_p = f32 || R > half;
     p->pair_o = f32 || most_q > half;

@@ -163,6 +163,13 @@ SIGNATURES = {
                                   _I64, _I64, _P, _I64]),
     "lq_prefix_attention": (C.c_int, [_P, _P, C.c_int, _I64, _I64, _I64, _I64, _I64, C.c_float, _P, _P, _I64, _I64,
                                       _I64, _P, _I64, _I64, _P, _P, _P, _I64, _I64, _I64, _P, _I64, _P, _P]),
+    "lq_paged_append_q8": (C.c_int, [_P, _P, C.c_int, _I64, _I64, _I64, _I64, _I64, _P, _P, C.c_float, C.c_int, _I64, _P,
+                                     _P, _I64, _P, _I64, _P, _I64, _I64, _I64, _P, _P, _P, _I64, _P, _P, _P, _P, _I64,
+                                     _I64, _I64, _I64, _I64, _P, _I64]),
+    "lq_paged_read_q8": (C.c_int, [_P, _P, _P, _P, _P, _I64, _I64, _I64, _I64, _I64, _I64, _I64, _I64, _P, _P, _P, _I64,
+                                   _I64, _P, _P, C.c_int, _I64]),
+    "lq_prefix_attention_q8": (C.c_int, [_P, _P, _I64, _I64, _I64, _I64, _I64, C.c_float, _P, _P, _P, _P, _I64, _I64,
+                                         _I64, _I64, _I64, _P, _I64, _I64, _P, _P, _P, _I64, _I64, _I64, _P, _I64, _P, _P]),
 }
 
 
@@ -473,30 +480,8 @@ class PagedBatch:
         self._prefix_pages = 0 if prefix_table is None else prefix_table.shape[0]
 
 
-class PagedKvCache:
-    """A layer's paged K/V cache: k and v [n_pages, n_kv_heads, page_size, head_dim], f32 or bf16,
-    pages dense inside and any distance apart."""
-
-    def __init__(self, ctx: Context, k, v):
-        self.dtype = _paged_dtype(k, "PagedKvCache")
-        _need(k.dim() == 4 and k.shape == v.shape and k.dtype == v.dtype and k.is_cuda and v.is_cuda,
-              "PagedKvCache: k and v are CUDA tensors [n_pages, n_kv_heads, page_size, head_dim] of one type")
-        self.n_pages, self.n_kv_heads, self.page_size, self.head_dim = k.shape
-        inner = (self.page_size * self.head_dim, self.head_dim, 1)
-        _need(k.stride()[1:] == inner and v.stride()[1:] == inner and k.stride(0) == v.stride(0) and
-              (self.n_pages <= 1 or k.stride(0) >= self.n_kv_heads * inner[0]),
-              "PagedKvCache: pages are dense inside and apart, K and V pages equally far")
-        self.ctx, self.k, self.v = ctx, k, v
-        self._pages = (k.data_ptr(), v.data_ptr())
-        self._layout = (self.n_pages, self.page_size, k.stride(0) if self.n_pages > 1 else self.n_kv_heads * inner[0])
-        import torch
-        self._norm_types = (torch.bfloat16, torch.int16)
-
-    @classmethod
-    def empty(cls, ctx: Context, n_pages: int, page_size: int, n_kv_heads: int, head_dim: int, dtype):
-        import torch
-        shape = (n_pages, n_kv_heads, page_size, head_dim)
-        return cls(ctx, torch.empty(shape, dtype=dtype, device="cuda"), torch.empty(shape, dtype=dtype, device="cuda"))
+class _PagedCache:
+    """What the paged caches of all types share. `type` is that of q and of the attention's rows."""
 
     @staticmethod
     def _row_stride(t, shape, dtype, what: str) -> int:
@@ -514,7 +499,7 @@ class PagedKvCache:
                eps: float = 1e-6, norm_bf16: bool = False, q_out=None):
         """qkv [rows, (n_heads + 2 n_kv_heads) * head_dim] f32 or bf16: normalises (bf16 weights)
         and rotates q and k, appends k and v, returns q [rows, n_heads, head_dim] in the cache's
-        type. pos None: the prefix length + the own position."""
+        type (bf16 for a cache in 8 bits). pos None: the prefix length + the own position."""
         dt = _paged_dtype(qkv, "append")
         D, st = self.head_dim, qkv.stride()
         rows, width = qkv.shape[0], (n_heads + 2 * self.n_kv_heads) * D
@@ -524,21 +509,19 @@ class PagedKvCache:
             if w is not None and (w.dtype not in self._norm_types or w.shape != (D,) or not w.is_cuda or w.stride(0) != 1):
                 raise ValueError("append: norm weights are bf16 [head_dim]")
         if q_out is None:
-            q_out = qkv.new_empty((rows, n_heads, D), dtype=self.k.dtype)
-        q_stride = self._row_stride(q_out, (rows, n_heads, D), self.k.dtype, "append: q_out")
+            q_out = qkv.new_empty((rows, n_heads, D), dtype=self.type)
+        q_stride = self._row_stride(q_out, (rows, n_heads, D), self.type, "append: q_out")
         if rows == 0:
             return q_out
         if pos is None and rotary.n_axes != 1:
             raise ValueError("append: several axes need positions")
         p, ps = (None, 0) if pos is None else rotary._pos(pos, rows)
-        ctx = self.ctx
-        rc = ctx.lib.lq_paged_append(
-            ctx.h, qkv.data_ptr(), dt, st[0] if rows > 1 else 0, rows, n_heads, self.n_kv_heads, D,
-            None if q_norm is None else q_norm.data_ptr(), None if k_norm is None else k_norm.data_ptr(), eps,
-            1 if norm_bf16 else 0, *rotary._args, p, ps, batch.prefix_len, *batch._seqs, *self._pages, self.dtype,
-            *self._layout, q_out.data_ptr(), q_stride)
+        rc = self._append(qkv.data_ptr(), dt, st[0] if rows > 1 else 0, rows, n_heads, self.n_kv_heads, D,
+                          None if q_norm is None else q_norm.data_ptr(), None if k_norm is None else k_norm.data_ptr(), eps,
+                          1 if norm_bf16 else 0, *rotary._args, p, ps, batch.prefix_len, *batch._seqs, *self._pages,
+                          *self._layout, q_out.data_ptr(), q_stride)
         if rc:
-            ctx.check(rc)
+            self.ctx.check(rc)
         return q_out
 
     def attend(self, q, batch: PagedBatch, scale: float | None = None, out=None, quantized=None):
@@ -549,10 +532,10 @@ class PagedKvCache:
         D, shape = self.head_dim, tuple(q.shape)
         if len(shape) != 3 or shape[2] != D:
             raise ValueError(f"attend: q [rows, n_heads, {D}] in the cache's type expected")
-        q_stride = self._row_stride(q, shape, self.k.dtype, "attend: q")
+        q_stride = self._row_stride(q, shape, self.type, "attend: q")
         if out is None:
             out = q.new_empty(shape)
-        out_stride = self._row_stride(out, shape, self.k.dtype, "attend: out")
+        out_stride = self._row_stride(out, shape, self.type, "attend: out")
         rows, heads = shape[0], shape[1]
         xq = xd = None
         if quantized is not None:
@@ -567,15 +550,117 @@ class PagedKvCache:
                              f"{self.page_size}")
         if rows == 0:
             return out
-        ctx = self.ctx
-        rc = ctx.lib.lq_prefix_attention(
-            ctx.h, q.data_ptr(), self.dtype, q_stride, rows, heads, self.n_kv_heads, D,
-            D ** -0.5 if scale is None else scale, *self._pages, *self._layout, batch._prefix_ptr, batch.prefix_len,
-            *batch._seqs, batch.max_q, batch.ld * self.page_size if batch.max_kv is None else batch.max_kv,
-            out.data_ptr(), out_stride, xq, xd)
+        rc = self._attend(q.data_ptr(), q_stride, rows, heads, self.n_kv_heads, D, D ** -0.5 if scale is None else scale,
+                          *self._pages, *self._layout, batch._prefix_ptr, batch.prefix_len, *batch._seqs, batch.max_q,
+                          batch.ld * self.page_size if batch.max_kv is None else batch.max_kv, out.data_ptr(), out_stride, xq, xd)
         if rc:
-            ctx.check(rc)
+            self.ctx.check(rc)
         return out
+
+
+class PagedKvCache(_PagedCache):
+    """A layer's paged K/V cache: k and v [n_pages, n_kv_heads, page_size, head_dim], f32 or bf16,
+    pages dense inside and any distance apart."""
+
+    def __init__(self, ctx: Context, k, v):
+        self.dtype = _paged_dtype(k, "PagedKvCache")
+        _need(k.dim() == 4 and k.shape == v.shape and k.dtype == v.dtype and k.is_cuda and v.is_cuda,
+              "PagedKvCache: k and v are CUDA tensors [n_pages, n_kv_heads, page_size, head_dim] of one type")
+        self.n_pages, self.n_kv_heads, self.page_size, self.head_dim = k.shape
+        inner = (self.page_size * self.head_dim, self.head_dim, 1)
+        _need(k.stride()[1:] == inner and v.stride()[1:] == inner and k.stride(0) == v.stride(0) and
+              (self.n_pages <= 1 or k.stride(0) >= self.n_kv_heads * inner[0]),
+              "PagedKvCache: pages are dense inside and apart, K and V pages equally far")
+        self.ctx, self.k, self.v, self.type = ctx, k, v, k.dtype
+        self._pages = (k.data_ptr(), v.data_ptr())
+        self._layout = (self.n_pages, self.page_size, k.stride(0) if self.n_pages > 1 else self.n_kv_heads * inner[0])
+        import torch
+        self._norm_types = (torch.bfloat16, torch.int16)
+
+    @classmethod
+    def empty(cls, ctx: Context, n_pages: int, page_size: int, n_kv_heads: int, head_dim: int, dtype):
+        import torch
+        shape = (n_pages, n_kv_heads, page_size, head_dim)
+        return cls(ctx, torch.empty(shape, dtype=dtype, device="cuda"), torch.empty(shape, dtype=dtype, device="cuda"))
+
+    def _append(self, *args):
+        # the cache's type stands between its pages and their layout
+        at = len(args) - 2 - len(self._layout)
+        return self.ctx.lib.lq_paged_append(self.ctx.h, *args[:at], self.dtype, *args[at:])
+
+    def _attend(self, q, *args):
+        return self.ctx.lib.lq_prefix_attention(self.ctx.h, q, self.dtype, *args)
+
+
+class PagedKvCacheQ8(_PagedCache):
+    """A layer's paged K/V cache in 8 bits: codes k and v int8 [n_pages, n_kv_heads, page_size, head_dim]
+    (head_dim 64 or 128, pages of 16 to 256 positions) and scales k_scale and v_scale f32 [n_pages,
+    n_kv_heads, page_size / block], one for each block of 16, 32, 64 or 128 positions of a kv head; a value is
+    code * scale. Pages are dense inside and any distance apart. append rounds the rows' values to
+    their block's codes (and the block's older ones again, where its largest value grows), attend takes q
+    and gives rows in bf16, read gives rows of the cache back."""
+
+    def __init__(self, ctx: Context, k, v, k_scale, v_scale):
+        import torch
+        _need(k.dim() == 4 and k.shape == v.shape and k.dtype == v.dtype == torch.int8 and k.is_cuda and v.device == k.device,
+              "PagedKvCacheQ8: k and v are int8 CUDA tensors [n_pages, n_kv_heads, page_size, head_dim]")
+        self.n_pages, self.n_kv_heads, self.page_size, self.head_dim = k.shape
+        _need(k_scale.dim() == 3 and k_scale.shape == v_scale.shape and k_scale.dtype == v_scale.dtype == torch.float32 and
+              k_scale.device == v_scale.device == k.device and k_scale.shape[:2] == k.shape[:2] and k_scale.shape[2] > 0 and
+              self.page_size % k_scale.shape[2] == 0,
+              "PagedKvCacheQ8: k_scale and v_scale are f32 CUDA tensors [n_pages, n_kv_heads, page_size / block]")
+        self.block = self.page_size // k_scale.shape[2]
+        inner, blocks = (self.page_size * self.head_dim, self.head_dim, 1), k_scale.shape[2]
+        _need(k.stride()[1:] == inner and v.stride()[1:] == inner and k.stride(0) == v.stride(0) and
+              (self.n_pages <= 1 or k.stride(0) >= self.n_kv_heads * inner[0]) and
+              k_scale.stride()[1:] == v_scale.stride()[1:] == (blocks, 1) and k_scale.stride(0) == v_scale.stride(0) and
+              (self.n_pages <= 1 or k_scale.stride(0) >= self.n_kv_heads * blocks),
+              "PagedKvCacheQ8: pages are dense inside and apart, K and V pages equally far")
+        self.ctx, self.k, self.v, self.k_scale, self.v_scale, self.type = ctx, k, v, k_scale, v_scale, torch.bfloat16
+        self._pages = (k.data_ptr(), v.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr())
+        apart = (k.stride(0), k_scale.stride(0)) if self.n_pages > 1 else (0, 0)
+        self._layout = (self.n_pages, self.page_size, apart[0], self.block, apart[1])
+        self._norm_types = (torch.bfloat16, torch.int16)
+
+    @classmethod
+    def empty(cls, ctx: Context, n_pages: int, page_size: int, n_kv_heads: int, head_dim: int, block: int = 16):
+        import torch
+        shape, scales = (n_pages, n_kv_heads, page_size, head_dim), (n_pages, n_kv_heads, page_size // block)
+        return cls(ctx, *(torch.empty(shape, dtype=torch.int8, device="cuda") for _ in range(2)),
+                   *(torch.empty(scales, dtype=torch.float32, device="cuda") for _ in range(2)))
+
+    def _append(self, *args):
+        return self.ctx.lib.lq_paged_append_q8(self.ctx.h, *args)
+
+    def _attend(self, *args):
+        return self.ctx.lib.lq_prefix_attention_q8(self.ctx.h, *args)
+
+    def read(self, batch: PagedBatch, k_out=None, v_out=None, rows: int | None = None, dtype=None):
+        """The batch's rows as the cache holds them, code * scale: (k, v), [rows, n_kv_heads, head_dim] in f32
+        or bf16. Rows are those that an append of the batch writes; with q_start the running sums of kv_len
+        that is all a sequence has. Without k_out and v_out, rows (with q_start, its last entry) and the
+        type (None: bf16) are given instead."""
+        if k_out is None or v_out is None:
+            _need(k_out is None and v_out is None, "read: k_out and v_out go together")
+            import torch
+            if rows is None:
+                _need(batch.q_start is None, "read: the number of rows, or k_out and v_out, expected")
+                rows = batch.n_seqs
+            shape = (rows, self.n_kv_heads, self.head_dim)
+            k_out, v_out = (torch.empty(shape, dtype=dtype or torch.bfloat16, device=self.k.device) for _ in range(2))
+        else:
+            _need(rows in (None, k_out.shape[0]) and dtype in (None, k_out.dtype), "read: rows and dtype are k_out's")
+        dt = _paged_dtype(k_out, "read")
+        shape = (k_out.shape[0], self.n_kv_heads, self.head_dim)
+        stride = self._row_stride(k_out, shape, k_out.dtype, "read: k_out")
+        _need(self._row_stride(v_out, shape, k_out.dtype, "read: v_out") == stride, "read: k_out and v_out have one row stride")
+        if shape[0] == 0:
+            return k_out, v_out
+        rc = self.ctx.lib.lq_paged_read_q8(self.ctx.h, *self._pages, self.n_kv_heads, self.head_dim, *self._layout, *batch._seqs,
+                                           shape[0], k_out.data_ptr(), v_out.data_ptr(), dt, stride)
+        if rc:
+            self.ctx.check(rc)
+        return k_out, v_out
 
 
 COMM_ID_BYTES = 128

@@ -138,6 +138,9 @@ extern "C" {
     pub fn lq_mrope(ctx: *mut LqCtx, x_dev: *const c_void, dtype: c_int, rows: i64, heads: i64, head_dim: i64, row_stride: i64, head_stride: i64, out_dev: *mut c_void, out_row_stride: i64, out_head_stride: i64, rot_dim: i64, cos_dev: *const f32, sin_dev: *const f32, table_len: i64, pair_axis_host: *const u8, n_axes: i64, pos_dev: *const i32, pos_stride: i64, inverse: c_int) -> c_int;
     pub fn lq_paged_append(ctx: *mut LqCtx, qkv_dev: *const c_void, qkv_dtype: c_int, row_stride: i64, rows: i64, n_heads: i64, n_kv_heads: i64, head_dim: i64, q_norm_dev: *const u16, k_norm_dev: *const u16, eps: f32, norm_bf16: c_int, rot_dim: i64, cos_dev: *const f32, sin_dev: *const f32, table_len: i64, pair_axis_host: *const u8, n_axes: i64, pos_dev: *const i32, pos_stride: i64, pos_base: i64, n_seqs: i64, q_start_dev: *const i32, kv_len_dev: *const i32, page_table_dev: *const i32, table_ld: i64, k_pages_dev: *mut c_void, v_pages_dev: *mut c_void, kv_dtype: c_int, n_pages: i64, page_size: i64, page_stride: i64, q_out_dev: *mut c_void, q_out_stride: i64) -> c_int;
     pub fn lq_prefix_attention(ctx: *mut LqCtx, q_dev: *const c_void, dtype: c_int, q_stride: i64, rows: i64, n_heads: i64, n_kv_heads: i64, head_dim: i64, scale: f32, k_pages_dev: *const c_void, v_pages_dev: *const c_void, n_pages: i64, page_size: i64, page_stride: i64, prefix_table_dev: *const i32, prefix_len: i64, n_seqs: i64, q_start_dev: *const i32, kv_len_dev: *const i32, page_table_dev: *const i32, table_ld: i64, max_q: i64, max_kv: i64, out_dev: *mut c_void, out_stride: i64, xq_dev: *mut i8, xd_dev: *mut u16) -> c_int;
+    pub fn lq_paged_append_q8(ctx: *mut LqCtx, qkv_dev: *const c_void, qkv_dtype: c_int, row_stride: i64, rows: i64, n_heads: i64, n_kv_heads: i64, head_dim: i64, q_norm_dev: *const u16, k_norm_dev: *const u16, eps: f32, norm_bf16: c_int, rot_dim: i64, cos_dev: *const f32, sin_dev: *const f32, table_len: i64, pair_axis_host: *const u8, n_axes: i64, pos_dev: *const i32, pos_stride: i64, pos_base: i64, n_seqs: i64, q_start_dev: *const i32, kv_len_dev: *const i32, page_table_dev: *const i32, table_ld: i64, k_codes_dev: *mut i8, v_codes_dev: *mut i8, k_scale_dev: *mut f32, v_scale_dev: *mut f32, n_pages: i64, page_size: i64, page_stride: i64, block: i64, scale_stride: i64, q_out_dev: *mut u16, q_out_stride: i64) -> c_int;
+    pub fn lq_paged_read_q8(ctx: *mut LqCtx, k_codes_dev: *const i8, v_codes_dev: *const i8, k_scale_dev: *const f32, v_scale_dev: *const f32, n_kv_heads: i64, head_dim: i64, n_pages: i64, page_size: i64, page_stride: i64, block: i64, scale_stride: i64, n_seqs: i64, q_start_dev: *const i32, kv_len_dev: *const i32, page_table_dev: *const i32, table_ld: i64, rows: i64, k_out_dev: *mut c_void, v_out_dev: *mut c_void, out_dtype: c_int, out_stride: i64) -> c_int;
+    pub fn lq_prefix_attention_q8(ctx: *mut LqCtx, q_dev: *const u16, q_stride: i64, rows: i64, n_heads: i64, n_kv_heads: i64, head_dim: i64, scale: f32, k_codes_dev: *const i8, v_codes_dev: *const i8, k_scale_dev: *const f32, v_scale_dev: *const f32, n_pages: i64, page_size: i64, page_stride: i64, block: i64, scale_stride: i64, prefix_table_dev: *const i32, prefix_len: i64, n_seqs: i64, q_start_dev: *const i32, kv_len_dev: *const i32, page_table_dev: *const i32, table_ld: i64, max_q: i64, max_kv: i64, out_dev: *mut u16, out_stride: i64, xq_dev: *mut i8, xd_dev: *mut u16) -> c_int;
     pub fn lq_comm_unique_id(ctx: *mut LqCtx, id_out: *mut u8) -> c_int;
     pub fn lq_comm_init(ctx: *mut LqCtx, id: *const u8, rank: c_int, world: c_int, out: *mut *mut LqComm) -> c_int;
     pub fn lq_comm_destroy(comm: *mut LqComm) -> c_int;
