@@ -382,8 +382,9 @@ extern "C" int lq_prefix_attention_q8(lq_ctx* ctx, const uint16_t* q, int64_t q_
     const int D = (int)head_dim;
     lq::PrefixPlan p;
     const int64_t stacked = (prefix_len > 0 ? rows : std::min(max_q, rows)) * a.group;
-    if ((rc = lq::make_plan(ctx, "lq_prefix_attention_q8", a, s, true, D, &p, stacked > 8 ? 16 : 8))) return rc;
-    rc = lq::launch_prefix_attn_q8(ctx, a, s, c, p, D);
+    const bool few = stacked <= 16;
+    if ((rc = lq::make_plan(ctx, "lq_prefix_attention_q8", a, s, few, D, &p, stacked > 8 ? 16 : 8))) return rc;
+    rc = few ? lq::launch_prefix_attn_q8(ctx, a, s, c, p, D) : lq::launch_prefix_attn_tc(ctx, a, s, p, D, &c);
     if (rc) return rc;
     return D == 64 ? lq::launch_merge<__nv_bfloat16, 64>(ctx, a, s, p) : lq::launch_merge<__nv_bfloat16, 128>(ctx, a, s, p);
 }

@@ -47,10 +47,16 @@ namespace lq {
 constexpr int PA_ROWS = 128;      // rows of a flow (MMA M)
 constexpr int PA_TILE = 128;      // positions of a step
 // stages of the ring: 128 KB for either head dimension's tiles of 32 and 16 KB, or what is left
-constexpr int pa_stages(int D) { return D == 64 ? 10 : 4; }
-constexpr int PA_THREADS = 384;   // warps 0-7 softmax, 8 TMA, 9 MMA, 10 scheduler, 11 empty rows
-// registers: 384 x 168 at launch = 256 x 216 for the softmax warps + 128 x 72 for the others
-constexpr int PA_REGS = 216, PA_REGS_LOW = 72;
+constexpr int pa_stages(int D, bool q8 = false) { return q8 ? D == 64 ? 7 : 3 : D == 64 ? 10 : 4; }
+// 8-bit caches: tiles of codes (16 and 8 KB) on their way into the ring
+constexpr int pa_raw(int D) { return D == 64 ? 5 : 2; }
+constexpr int PA_SCALES = 4;      // rounds of a flow whose scales are kept
+// warps 0-7 softmax, 8 TMA, 9 MMA, 10 scheduler, 11 empty rows, 12-15 (8-bit caches) codes to bf16
+constexpr int pa_threads(bool q8) { return q8 ? 512 : 384; }
+// registers: 384 x 168 at launch = 256 x 216 for the softmax warps + 128 x 72 for the others;
+// 512 x 128 = 256 x 184 + 256 x 72
+constexpr int pa_regs(bool q8) { return q8 ? 184 : 216; }
+constexpr int PA_REGS_LOW = 72;
 constexpr int PA_SCAN = 512;      // entries of the scan over the sequences
 constexpr int PA_BATCH = 16;      // segments a flow gets at a time, worked out by a lane each
 constexpr int PA_FEW = 8;         // rows up to which the four warps of a flow share a tile's columns
@@ -75,6 +81,10 @@ struct PaCtl {
     uint64_t full[pa_stages(64)], empty[pa_stages(64)];
     uint64_t seg_full[2][2], seg_empty[2][2];  // per flow: two batches of segments
     uint64_t q_full[2], s_full[2], p_full[2], o_full[2], done;
+    // 8-bit caches: tiles of codes; scales of a flow's rounds, those of K and V of 16 positions each
+    uint64_t raw_full[pa_raw(64)], raw_empty[pa_raw(64)], sc_full[2][PA_SCALES], sc_empty[2][PA_SCALES];
+    alignas(16) float sc[2][PA_SCALES][2][8];
+    int raw_end;    // the tile after the last one
     uint32_t tmem;
     int abort;
     int issued;     // copies that the producer started
@@ -206,6 +216,7 @@ struct PaArgs {
     PrefixAttnArgs a;
     PagedSeqs s;
     PrefixPlan p;
+    PagedQ8 q8;     // 8-bit caches
 };
 
 __device__ __forceinline__ int warp_scan(int v, int lane) {  // inclusive sum
@@ -232,24 +243,39 @@ __device__ __forceinline__ SeqInfo pa_seq(const PaArgs& g, const PaCtl& c, int b
     return SeqInfo{v.x, v.y, v.z};
 }
 
+// bytes 2 j, 2 j + 1 of w (sel 0x4140, 0x4342) as a pair of bf16: 0x4300 + b has the value 128 + b for
+// b < 128; so a code is (128 + its low seven bits) - (128, or 256 where the sign is set), exactly
+__device__ __forceinline__ uint32_t codes_bf16(uint32_t w, uint32_t sel) {
+    const uint32_t x = __byte_perm(w, 0x43434343u, sel), lo = x & 0xff7fff7fu, up = x & 0xff80ff80u;
+    const __nv_bfloat162 d = __hsub2(*reinterpret_cast<const __nv_bfloat162*>(&lo), *reinterpret_cast<const __nv_bfloat162*>(&up));
+    return *reinterpret_cast<const uint32_t*>(&d);
+}
+
 // PP, PO: blocks of the prefix / of a sequence's own rows are two halves of 128 rows that share
 // their K and V tiles
-template <int D, bool PP, bool PO>
-__global__ void __launch_bounds__(PA_THREADS, 1)
+template <int D, bool PP, bool PO, bool Q8>
+__global__ void __launch_bounds__(pa_threads(Q8), 1)
 prefix_attn_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v,
                       const __grid_constant__ PaArgs g) {
-    constexpr int HALVES = D / 64, STAGES = pa_stages(D);
+    constexpr int HALVES = D / 64, STAGES = pa_stages(D, Q8), PA_THREADS = pa_threads(Q8);
+    constexpr int RAW = Q8 ? pa_raw(D) : 0, RAW_BYTES = PA_TILE * D;
     constexpr int Q_BYTES = PA_ROWS * D * 2, KV_BYTES = PA_TILE * D * 2, HALF = 128 * 128;
     extern __shared__ uint8_t smem_raw[];
     const uint32_t raw = smem_addr(smem_raw);
     uint8_t* const sm = smem_raw + (((raw + 1023) & ~1023u) - raw);
     uint8_t* const ring = sm + 2 * Q_BYTES;
-    PaCtl& c = *reinterpret_cast<PaCtl*>(ring + STAGES * KV_BYTES);
+    uint8_t* const codes = ring + STAGES * KV_BYTES;
+    PaCtl& c = *reinterpret_cast<PaCtl*>(codes + RAW * RAW_BYTES);
     const int tid = threadIdx.x, warp = __shfl_sync(0xffffffffu, tid >> 5, 0), lane = tid & 31;
     int* const err = g.a.err;
 
     if (tid == 0) {
-        for (int i = 0; i < STAGES; i++) mbar_init(&c.full[i], 1), mbar_init(&c.empty[i], 1);
+        for (int i = 0; i < STAGES; i++) mbar_init(&c.full[i], Q8 ? 4 : 1), mbar_init(&c.empty[i], 1);
+        if constexpr (Q8) {
+            for (int i = 0; i < RAW; i++) mbar_init(&c.raw_full[i], 1), mbar_init(&c.raw_empty[i], 4);
+            for (int i = 0; i < 2 * PA_SCALES; i++) mbar_init(&c.sc_full[0][i], 32), mbar_init(&c.sc_empty[0][i], 4);
+            c.raw_end = -1;
+        }
 #pragma unroll 1
         for (int f = 0; f < 2; f++) {
             mbar_init(&c.q_full[f], 4);
@@ -352,13 +378,15 @@ prefix_attn_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_co
 
     if (warp < 8) {
         // ------------------------------ softmax ------------------------------
-        asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(PA_REGS));
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(pa_regs(Q8)));
         const int f = warp >> 2, row = tid & 127, wq = warp & 3;
         const uint32_t sq = smem_addr(sm + f * Q_BYTES);
         const uint32_t t_lane = (uint32_t)(wq * 32) << 16;
         const uint32_t t_s = tmem + t_lane + f * 128, t_o = tmem + t_lane + 256 + f * 128;
         const float cs = g.a.scale * 1.44269504088896340736f;  // scores in units of log2
         unsigned s_ph = 0, o_ph = 0, turn = 0;
+        [[maybe_unused]] int sc_slot = 0;  // 8-bit caches: the round's scales
+        [[maybe_unused]] unsigned sc_ph = 0;
         int joint = 0;  // segments of few rows
         Feed feed;
 
@@ -417,11 +445,18 @@ prefix_attn_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_co
                 if (!pa_wait(c, &c.s_full[f], s_ph)) break;
                 s_ph ^= 1;
                 tc_after();
+                if constexpr (Q8) {
+                    if (!pa_wait(c, &c.sc_full[f][sc_slot], sc_ph)) break;
+                }
+                // K's scale of 16 positions, in units of log2 (never so small that a masked score loses
+                // its minus infinity), and V's
+                [[maybe_unused]] auto k_of = [&](int i) { return max_nan(c.sc[f][sc_slot][0][i] * cs, 1e-37f); };
+                [[maybe_unused]] auto v_of = [&](int i) { return c.sc[f][sc_slot][1][i]; };
                 if (busy) {
                     const int lim = (t < chain ? g.a.prefix_len : vis) - t * PA_TILE;  // columns this row sees
                     // a larger maximum: when a row's grew by more than 2^8, l and O follow
                     auto raise = [&](float mt) {
-                        mt *= cs;
+                        if constexpr (!Q8) mt *= cs;
                         if (t == sg.t0) {
                             m = mt;
                         } else if (__any_sync(0xffffffffu, mine && !(mt <= m + 8.0f))) {  // (others hold anything)
@@ -453,19 +488,34 @@ prefix_attn_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_co
                             for (int i = 0; i < 32; i++)
                                 if (i >= upto) s[i] = -INFINITY;
                         }
-                        float mx[4] = {s[0], s[1], s[2], s[3]};
+                        float mt, kc[2] = {cs, cs}, vc[2] = {1.0f, 1.0f};  // (halves of the columns: two scales)
+                        if constexpr (Q8) {
 #pragma unroll
-                        for (int i = 4; i < 28; i += 8)
+                            for (int h = 0; h < 2; h++) {
+                                kc[h] = k_of(2 * wq + h);
+                                vc[h] = v_of(2 * wq + h);
+                                float mh = max_nan(s[16 * h], s[16 * h + 1]);
 #pragma unroll
-                            for (int j = 0; j < 4; j++) mx[j] = max3(mx[j], s[i + 2 * j], s[i + 2 * j + 1]);
-                        const float neg = raise(max_nan(max3(mx[0], s[28], s[29]), max3(max3(mx[1], s[30], s[31]), mx[2], mx[3])));
+                                for (int i = 2; i < 16; i += 2) mh = max3(mh, s[16 * h + i], s[16 * h + i + 1]);
+                                mt = h ? max_nan(mt, mh * kc[1]) : mh * kc[0];
+                            }
+                        } else {
+                            float mx[4] = {s[0], s[1], s[2], s[3]};
+#pragma unroll
+                            for (int i = 4; i < 28; i += 8)
+#pragma unroll
+                                for (int j = 0; j < 4; j++) mx[j] = max3(mx[j], s[i + 2 * j], s[i + 2 * j + 1]);
+                            mt = max_nan(max3(mx[0], s[28], s[29]), max3(max3(mx[1], s[30], s[31]), mx[2], mx[3]));
+                        }
+                        const float neg = raise(mt);
                         uint32_t pk[16];
                         float2 sum = make_float2(0.0f, 0.0f);
 #pragma unroll
                         for (int i = 0; i < 16; i++) {
-                            const float2 x = __ffma2_rn(make_float2(s[2 * i], s[2 * i + 1]), make_float2(cs, cs), make_float2(neg, neg));
-                            const float2 e = make_float2(ex2(x.x), ex2(x.y));
+                            const float2 x = __ffma2_rn(make_float2(s[2 * i], s[2 * i + 1]), make_float2(kc[i / 8], kc[i / 8]), make_float2(neg, neg));
+                            float2 e = make_float2(ex2(x.x), ex2(x.y));
                             sum = __fadd2_rn(sum, e);
+                            if constexpr (Q8) e = __fmul2_rn(e, make_float2(vc[i / 8], vc[i / 8]));
                             pk[i] = pack_bf16x2(e.x, e.y);
                         }
                         l += sum.x + sum.y;
@@ -485,22 +535,42 @@ prefix_attn_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_co
                             for (int i = 0; i < 128; i++)
                                 if (i >= lim) s[i] = -INFINITY;
                         }
-                        float mx[4] = {s[0], s[1], s[2], s[3]};
+                        float mt = -INFINITY;
+                        if constexpr (Q8) {
 #pragma unroll
-                        for (int i = 4; i < 124; i += 8)
+                            for (int h = 0; h < 8; h++) {
+                                float mh = max_nan(s[16 * h], s[16 * h + 1]);
 #pragma unroll
-                            for (int j = 0; j < 4; j++) mx[j] = max3(mx[j], s[i + 2 * j], s[i + 2 * j + 1]);
-                        const float neg = raise(max_nan(max3(mx[0], mx[1], max3(mx[2], s[124], s[125])), max3(mx[3], s[126], s[127])));
-                        const float2 cs2 = make_float2(cs, cs), neg2 = make_float2(neg, neg);
+                                for (int i = 2; i < 16; i += 2) mh = max3(mh, s[16 * h + i], s[16 * h + i + 1]);
+                                mt = max_nan(mt, mh * k_of(h));
+                            }
+                        } else {
+                            float mx[4] = {s[0], s[1], s[2], s[3]};
+#pragma unroll
+                            for (int i = 4; i < 124; i += 8)
+#pragma unroll
+                                for (int j = 0; j < 4; j++) mx[j] = max3(mx[j], s[i + 2 * j], s[i + 2 * j + 1]);
+                            mt = max_nan(max3(mx[0], mx[1], max3(mx[2], s[124], s[125])), max3(mx[3], s[126], s[127]));
+                        }
+                        const float neg = raise(mt);
+                        float2 cs2 = make_float2(cs, cs), vs2 = make_float2(1.0f, 1.0f);
+                        const float2 neg2 = make_float2(neg, neg);
                         float2 sum[2] = {make_float2(0.0f, 0.0f), make_float2(0.0f, 0.0f)};
 #pragma unroll
                         for (int j = 0; j < 4; j++) {
                             uint32_t pk[16];
 #pragma unroll
                             for (int i = 0; i < 16; i++) {
+                                if constexpr (Q8)
+                                    if (i % 8 == 0) {
+                                        const float kc = k_of(2 * j + i / 8), vc = v_of(2 * j + i / 8);
+                                        cs2 = make_float2(kc, kc);
+                                        vs2 = make_float2(vc, vc);
+                                    }
                                 const float2 x = __ffma2_rn(make_float2(s[32 * j + 2 * i], s[32 * j + 2 * i + 1]), cs2, neg2);
-                                const float2 e = make_float2(ex2(x.x), ex2(x.y));
+                                float2 e = make_float2(ex2(x.x), ex2(x.y));
                                 sum[i & 1] = __fadd2_rn(sum[i & 1], e);
+                                if constexpr (Q8) e = __fmul2_rn(e, vs2);
                                 pk[i] = pack_bf16x2(e.x, e.y);
                             }
                             tmem_st16(t_s + 16 * j, pk);
@@ -523,16 +593,31 @@ prefix_attn_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_co
                                     for (int i = 0; i < 32; i++)
                                         if (j + i >= lim) s[i] = -INFINITY;
                                 }
-                                if (pass == 0) {
+                                float kc[2] = {cs, cs}, vc[2] = {1.0f, 1.0f};
+                                if constexpr (Q8) {
 #pragma unroll
-                                    for (int i = 0; i < 32; i += 2) mt = max3(mt, s[i], s[i + 1]);
+                                    for (int h = 0; h < 2; h++) kc[h] = k_of(j / 16 + h), vc[h] = v_of(j / 16 + h);
+                                }
+                                if (pass == 0) {
+                                    if constexpr (Q8) {
+#pragma unroll
+                                        for (int h = 0; h < 2; h++) {
+                                            float mh = max_nan(s[16 * h], s[16 * h + 1]);
+#pragma unroll
+                                            for (int i = 2; i < 16; i += 2) mh = max3(mh, s[16 * h + i], s[16 * h + i + 1]);
+                                            mt = max_nan(mt, mh * kc[h]);
+                                        }
+                                    } else {
+#pragma unroll
+                                        for (int i = 0; i < 32; i += 2) mt = max3(mt, s[i], s[i + 1]);
+                                    }
                                 } else {
                                     uint32_t pk[16];
 #pragma unroll
                                     for (int i = 0; i < 16; i++) {
-                                        const float p0 = ex2(fmaf(s[2 * i], cs, neg)), p1 = ex2(fmaf(s[2 * i + 1], cs, neg));
+                                        const float p0 = ex2(fmaf(s[2 * i], kc[i / 8], neg)), p1 = ex2(fmaf(s[2 * i + 1], kc[i / 8], neg));
                                         sum += p0 + p1;
-                                        pk[i] = pack_bf16x2(p0, p1);
+                                        pk[i] = Q8 ? pack_bf16x2(p0 * vc[i / 8], p1 * vc[i / 8]) : pack_bf16x2(p0, p1);
                                     }
                                     // P of columns j.. lands on S columns j/2.., which have been read
                                     tmem_st16(t_s + j / 2, pk);
@@ -547,6 +632,10 @@ prefix_attn_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_co
                 tc_before();
                 __syncwarp();
                 if (lane == 0) mbar_arrive(&c.p_full[f]);
+                if constexpr (Q8) {
+                    if (lane == 0) mbar_arrive(&c.sc_empty[f][sc_slot]);
+                    if (++sc_slot == PA_SCALES) sc_slot = 0, sc_ph ^= 1;
+                }
                 if (t == sg.t0) {
                     more = next(true);
                     early = more == NX_SEG && q_ahead(sg, nx);
@@ -665,7 +754,9 @@ prefix_attn_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_co
             PaSeg sg;
             bool ended, v_due;
             int pg, krow, kh;   // this lane's page of the tile, kept from K for V
+            unsigned rounds;    // 8-bit caches: rounds whose scales are on their way
         } cur, oth;
+        cur.rounds = oth.rounds = 0;
         cur.ended = oth.ended = cur.v_due = oth.v_due = false;
         cur.sg.t0 = cur.sg.t1 = oth.sg.t0 = oth.sg.t1 = 0;
         cur.pg = cur.krow = cur.kh = oth.pg = oth.krow = oth.kh = 0;
@@ -676,19 +767,25 @@ prefix_attn_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_co
 #pragma unroll 1
             for (int which = 0; which < 2 && ok; which++) {
                 if (which == 0 ? cur.v_due : k_due) {
-                    ok = pa_wait_warp(c, &c.empty[slot], ph ^ 1u);
+                    uint64_t* const there = Q8 ? &c.raw_full[slot] : &c.full[slot];
+                    ok = pa_wait_warp(c, Q8 ? &c.raw_empty[slot] : &c.empty[slot], ph ^ 1u);
                     if (!ok) break;
-                    if (lane == 0) mbar_expect_tx(&c.full[slot], KV_BYTES);
+                    if (lane == 0) mbar_expect_tx(there, Q8 ? RAW_BYTES : KV_BYTES);
                     __syncwarp();
-                    uint8_t* const dst = ring + slot * KV_BYTES;
                     const CUtensorMap* const map = which ? &map_k : &map_v;
-                    if (lane < boxes) {
+                    if constexpr (Q8) {
+                        if (lane < boxes)
+                            tma_load_4d(codes + slot * RAW_BYTES + lane * box * D, map, 0, cur.krow, cur.kh, cur.pg, there);
+                    } else {
+                        uint8_t* const dst = ring + slot * KV_BYTES;
+                        if (lane < boxes) {
 #pragma unroll
-                        for (int h = 0; h < HALVES; h++)
-                            tma_load_4d(dst + h * HALF + lane * box * 128, map, h * 64, cur.krow, cur.kh, cur.pg, &c.full[slot]);
+                            for (int h = 0; h < HALVES; h++)
+                                tma_load_4d(dst + h * HALF + lane * box * 128, map, h * 64, cur.krow, cur.kh, cur.pg, there);
+                        }
                     }
                     issued++;
-                    if (++slot == STAGES) slot = 0, ph ^= 1;
+                    if (++slot == (Q8 ? RAW : STAGES)) slot = 0, ph ^= 1;
                 }
                 if (which) break;
                 cur.v_due = false;
@@ -699,17 +796,38 @@ prefix_attn_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_co
                     if (cur.ended) break;
                 }
                 const int t = cur.sg.t0++;
-                if (cur.sg.n == 0 || (f == 1 && (cur.sg.flags & SEG_PAIRED))) break;
+                const bool second = f == 1 && (cur.sg.flags & SEG_PAIRED);  // its tiles come with the first flow's
+                if (cur.sg.n == 0 || (!Q8 && second)) break;
                 const bool own = (cur.sg.flags & SEG_OWN) && t >= chain;
                 const int pos = (own ? t - chain : t) * PA_TILE + lane * box;
+                const int limit = own ? cur.sg.kv_end - chain * PA_TILE : g.a.prefix_len;
                 int id = g.s.n_pages;  // out of range: zeros
-                if (lane < boxes && pos < (own ? cur.sg.kv_end - chain * PA_TILE : g.a.prefix_len)) {
+                if (lane < boxes && pos < limit) {
                     const int32_t* const table = own ? g.s.table + (int64_t)cur.sg.b * g.s.table_ld : g.a.prefix_table;
                     id = table[pos >> g.s.page_shift];
                     if ((unsigned)id >= (unsigned)g.s.n_pages) {
                         flag_error(err, ERR_PAGE_ID, id);
                         id = g.s.n_pages;
                     }
+                }
+                if constexpr (Q8) {
+                    // scales of the round: lanes 0-7 K's of 16 positions each, lanes 8-15 V's
+                    const int at = cur.rounds % PA_SCALES;
+                    ok = pa_wait_warp(c, &c.sc_empty[f][at], (cur.rounds / PA_SCALES & 1u) ^ 1u);
+                    if (!ok) break;
+                    cur.rounds++;
+                    const int i = lane & 7, x = (own ? t - chain : t) * PA_TILE + 16 * i;
+                    const int pg = __shfl_sync(0xffffffffu, id, 16 * i / box);
+                    const float* const base = lane & 8 ? g.q8.v_scale : g.q8.k_scale;
+                    const bool there = x < limit && pg < g.s.n_pages;
+                    if (lane < 16)
+                        cp_async4(&c.sc[f][at][lane >> 3][i],
+                                  there ? base + pg * g.q8.scale_stride + ((int64_t)cur.sg.kh << (g.s.page_shift - g.q8.block_shift)) +
+                                              ((x & (page - 1)) >> g.q8.block_shift)
+                                        : base,
+                                  there);
+                    asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(smem_addr(&c.sc_full[f][at])) : "memory");
+                    if (second) break;
                 }
                 cur.pg = id;
                 cur.krow = pos & (page - 1);
@@ -720,6 +838,16 @@ prefix_attn_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_co
             exchange(cur, oth);
         }
         if (lane == 0) c.issued = issued;
+        if constexpr (Q8) {
+            asm volatile("cp.async.wait_all;" ::: "memory");  // (scales, after a wait that ran out)
+            if (ok && pa_wait_warp(c, &c.raw_empty[slot], ph ^ 1u)) {  // for the converters: no more tiles
+                if (lane == 0) {
+                    *reinterpret_cast<volatile int*>(&c.raw_end) = issued;
+                    mbar_arrive(&c.raw_full[slot]);
+                }
+                __syncwarp();
+            }
+        }
     } else if (warp == 9) {
         // ------------------------------ MMA issuer ------------------------------
         asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(PA_REGS_LOW));
@@ -753,7 +881,7 @@ prefix_attn_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_co
                 if (f == 0 || !cur.pv_shared) {
                     take(v_slot);
                     if (!ok) break;
-                    if (cur.pv_valid < PA_TILE) {
+                    if (!Q8 && cur.pv_valid < PA_TILE) {  // (codes are finite)
                         // positions past the end share a page with valid ones: whatever is there
                         // (NaN times a zero probability) must not reach the product
                         uint8_t* const v = ring + v_slot * KV_BYTES;
@@ -999,6 +1127,53 @@ prefix_attn_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_co
             if (ok) part(std::true_type{});
             o.flags = SEG_END;
             if (ok) put(o, hl == 0);
+        } else if (Q8 && warp >= 12) {
+            // ------------------------------ codes to bf16 ------------------------------
+            // A quarter warp reads 16 bytes a lane of two positions of opposite parity (r and r ^ 5, with
+            // D = 64 r and r + 1) and writes their two vectors of 8 dims each: under the swizzle both
+            // touch every bank once.
+            int rs = 0, slot = 0;
+            unsigned rph = 0, ph = 0;
+            bool ok = true;
+#pragma unroll 1
+            for (int tile = 0;; tile++) {
+                ok = pa_wait_warp(c, &c.raw_full[rs], rph);
+                if (!ok || *reinterpret_cast<volatile int*>(&c.raw_end) == tile) break;
+                ok = pa_wait_warp(c, &c.empty[slot], ph ^ 1u);
+                if (!ok) break;
+                const uint8_t* const src = codes + rs * RAW_BYTES;
+                uint8_t* const dst = ring + slot * KV_BYTES;
+                const int w = warp - 12, q = lane >> 3, l = lane & 7;
+#pragma unroll
+                for (int i = 0; i < D / 16; i++) {
+                    // vector v (16 dims) of row r
+                    int r, v;
+                    if constexpr (D == 128) {
+                        const int k = 4 * i + q, pair = k & 3;   // 32 rows a warp: 8 groups of 4 positions' pairs ...
+                        r = 32 * w + 8 * (i >> 1) + (l < 4 ? pair : pair ^ 5);
+                        v = (l & 3) + 4 * (i & 1);
+                    } else {
+                        r = 32 * w + 8 * i + 2 * q + (l >> 2);
+                        v = l & 3;
+                    }
+                    const uint4 u = *reinterpret_cast<const uint4*>(src + (D == 128 ? r * 128 + ((v ^ (r & 7)) << 4) : r * 64 + v * 16));
+                    const uint32_t x[4] = {u.x, u.y, u.z, u.w};
+                    uint8_t* const to = dst + (v >> 2) * HALF + r * 128;
+#pragma unroll
+                    for (int j = 0; j < 2; j++)
+                        *reinterpret_cast<uint4*>(to + (((2 * (v & 3) + j) ^ (r & 7)) << 4)) =
+                            make_uint4(codes_bf16(x[2 * j], 0x4140), codes_bf16(x[2 * j], 0x4342),
+                                       codes_bf16(x[2 * j + 1], 0x4140), codes_bf16(x[2 * j + 1], 0x4342));
+                }
+                proxy_fence();
+                __syncwarp();
+                if (lane == 0) {
+                    mbar_arrive(&c.full[slot]);
+                    mbar_arrive(&c.raw_empty[rs]);
+                }
+                if (++rs == RAW) rs = 0, rph ^= 1;
+                if (++slot == STAGES) slot = 0, ph ^= 1;
+            }
         } else if (g.a.prefix_len == 0) {
             // warp 11: rows before their sequence's first position see nothing when there is no
             // prefix either
@@ -1017,36 +1192,45 @@ prefix_attn_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_co
         // no copy may still be landing when the CTA exits
         if (warp == 8) {
 #pragma unroll 1
-            for (int i = max(0, c.issued - STAGES); i < c.issued; i++)
-                mbar_wait_ns(&c.full[i % STAGES], (unsigned)(i / STAGES) & 1u, 2000000000ull);
+            for (int i = max(0, c.issued - (Q8 ? RAW : STAGES)); i < c.issued; i++) {
+                if constexpr (Q8) mbar_wait_ns(&c.raw_full[i % RAW], (unsigned)(i / RAW) & 1u, 2000000000ull);
+                else mbar_wait_ns(&c.full[i % STAGES], (unsigned)(i / STAGES) & 1u, 2000000000ull);
+            }
         }
     }
     if (warp == 9) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, 512;" ::"r"(tmem));
 }
 
-template <int D, bool PP, bool PO>
+template <int D, bool PP, bool PO, bool Q8>
 static int launch_tc(lq_ctx* ctx, const PaArgs& g) {
     const int page = 1 << g.s.page_shift;
+    const uint64_t size = Q8 ? 1 : 2, stride = Q8 ? g.q8.page_stride : g.a.page_stride * 2;
     const uint64_t dims[4] = {(uint64_t)D, (uint64_t)page, (uint64_t)g.a.n_kv, (uint64_t)g.s.n_pages};
-    const uint64_t strides[3] = {(uint64_t)D * 2, (uint64_t)D * 2 * page, (uint64_t)g.a.page_stride * 2};
-    const uint32_t box[4] = {64, (uint32_t)std::min(page, PA_TILE), 1, 1};
+    const uint64_t strides[3] = {D * size, D * size * page, stride};
+    const uint32_t box[4] = {Q8 ? D : 64, (uint32_t)std::min(page, PA_TILE), 1, 1};
+    const CUtensorMapDataType type = Q8 ? CU_TENSOR_MAP_DATA_TYPE_UINT8 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16;
+    const CUtensorMapSwizzle swz = Q8 && D == 64 ? CU_TENSOR_MAP_SWIZZLE_NONE : CU_TENSOR_MAP_SWIZZLE_128B;
     CUtensorMap mk, mv;
-    int rc = make_tensor_map_4d(ctx, &mk, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, g.a.k, dims, strides, box, CU_TENSOR_MAP_SWIZZLE_128B);
+    int rc = make_tensor_map_4d(ctx, &mk, type, Q8 ? (const void*)g.q8.k : g.a.k, dims, strides, box, swz);
     if (rc) return rc;
-    rc = make_tensor_map_4d(ctx, &mv, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, g.a.v, dims, strides, box, CU_TENSOR_MAP_SWIZZLE_128B);
+    rc = make_tensor_map_4d(ctx, &mv, type, Q8 ? (const void*)g.q8.v : g.a.v, dims, strides, box, swz);
     if (rc) return rc;
-    const size_t smem = 1024 + 2 * PA_ROWS * D * 2 + pa_stages(D) * PA_TILE * D * 2 + sizeof(PaCtl);
-    rc = ensure_func_smem(ctx, (const void*)prefix_attn_tc_kernel<D, PP, PO>, smem);
+    const size_t smem = 1024 + 2 * PA_ROWS * D * 2 + pa_stages(D, Q8) * PA_TILE * D * 2 + (Q8 ? pa_raw(D) * PA_TILE * D : 0) + sizeof(PaCtl);
+    rc = ensure_func_smem(ctx, (const void*)prefix_attn_tc_kernel<D, PP, PO, Q8>, smem);
     if (rc) return rc;
-    return launch_kernel(ctx, prefix_attn_tc_kernel<D, PP, PO>, dim3((unsigned)g.p.workers), dim3(PA_THREADS), smem,
+    return launch_kernel(ctx, prefix_attn_tc_kernel<D, PP, PO, Q8>, dim3((unsigned)g.p.workers), dim3(pa_threads(Q8)), smem,
                          "prefix_attn_tc", mk, mv, g);
 }
 
-int launch_prefix_attn_tc(lq_ctx* ctx, const PrefixAttnArgs& a, const PagedSeqs& s, const PrefixPlan& p, int D) {
-    const PaArgs g{a, s, p};
+template <bool Q8>
+static int launch_tc_of(lq_ctx* ctx, const PaArgs& g, int D) {
     // PO implies PP: one sequence's rows are some of all rows. Without a prefix PP says nothing.
-    if (D == 64) return p.pair_o ? launch_tc<64, true, true>(ctx, g) : p.pair_p ? launch_tc<64, true, false>(ctx, g) : launch_tc<64, false, false>(ctx, g);
-    return p.pair_o ? launch_tc<128, true, true>(ctx, g) : p.pair_p ? launch_tc<128, true, false>(ctx, g) : launch_tc<128, false, false>(ctx, g);
+    if (D == 64) return g.p.pair_o ? launch_tc<64, true, true, Q8>(ctx, g) : g.p.pair_p ? launch_tc<64, true, false, Q8>(ctx, g) : launch_tc<64, false, false, Q8>(ctx, g);
+    return g.p.pair_o ? launch_tc<128, true, true, Q8>(ctx, g) : g.p.pair_p ? launch_tc<128, true, false, Q8>(ctx, g) : launch_tc<128, false, false, Q8>(ctx, g);
+}
+
+int launch_prefix_attn_tc(lq_ctx* ctx, const PrefixAttnArgs& a, const PagedSeqs& s, const PrefixPlan& p, int D, const PagedQ8* q8) {
+    return q8 ? launch_tc_of<true>(ctx, PaArgs{a, s, p, *q8}, D) : launch_tc_of<false>(ctx, PaArgs{a, s, p, PagedQ8{}}, D);
 }
 
 }  // namespace lq
