@@ -232,7 +232,7 @@ int lq_fill_bf16(lq_ctx* ctx, uint64_t seed, uint64_t tensor_id, int64_t offset,
  * ------------------------------------------------------------------------------------- */
 /* Waits for the context's stream; LQ_ERR_INVALID_ARG with the first code and value that a
  * kernel flagged since the last check (90 rotary position, 91 length, 92 page id, 93 row
- * count, 94 to 96 a wait inside the attention that ran out: its output is not valid). */
+ * count, 94 to 97 a wait inside the attention that ran out: its output is not valid). */
 int lq_device_status(lq_ctx* ctx);
 /* Rotary positions with one to four axes (e.g. time, height, width). x [rows][heads][head_dim]
  * f32 or bf16 with the given strides (elements) to out (may be x): pair i < rot_dim/2 of a head

@@ -23,7 +23,9 @@ namespace lq {
 constexpr int MERGE_CHUNK = 32;   // partials looked at together
 
 template <typename T, int D, int MR>
-__global__ void __launch_bounds__(256, MR == 32 ? 5 : 4) prefix_attn_merge_kernel(PrefixAttnArgs a, PagedSeqs s, PrefixPlan p) {
+__global__ void __launch_bounds__(256, MR == 32 ? 5 : 4)
+prefix_attn_merge_kernel(const __grid_constant__ PrefixAttnArgs a, const __grid_constant__ PagedSeqs s,
+                         const __grid_constant__ PrefixPlan p, const __grid_constant__ PrefixPlan pp) {
     constexpr int CH = D / 4, SUBS = 256 / MR;  // vectors of a row; threads that share a row
     constexpr int VEC = (CH + SUBS - 1) / SUBS, BATCH = VEC == 1 ? 8 : 1;  // partials whose loads go out together
     __shared__ int slot[MERGE_CHUNK];
@@ -55,7 +57,13 @@ __global__ void __launch_bounds__(256, MR == 32 ? 5 : 4) prefix_attn_merge_kerne
         }
         const SeqInfo si = seq_info(a, s, lo, false);
         const int rb = x - os.base(si, lo), nb = os.blocks(si);
-        if (rb < 0 || rb >= nb) return;
+        if (rb < 0 || rb >= nb) {
+            if (p.chunks > 0 && blockIdx.x == 0 && blockIdx.y == 0) {
+                pdl_wait();
+                if (tid == 0) *p.claimed = 0;
+            }
+            return;
+        }
         st0 = si.q0 * a.group + rb * p.ob + own_in;
         todo = min(MR, min(p.ob, si.q * a.group - rb * p.ob) - own_in);
         own_item = a.n_kv * x + kh * nb + rb - a.n_kv * rb;  // n_kv base + kh nb + rb
@@ -63,27 +71,50 @@ __global__ void __launch_bounds__(256, MR == 32 ? 5 : 4) prefix_attn_merge_kerne
     }
     pdl_wait();
     pdl_trigger();
-    if (!with_prefix) {
-        const SplitItem w = p.split[blockIdx.x];
-        st0 = w.row0 + own_in;
-        todo = min(MR, w.rows - own_in);
-        kh = w.kh;
-        own_item = w.item;
-    }
-    const Line line(p, *p.own_steps, p.pair_p, p.pair_o);
+    if (p.chunks > 0 && blockIdx.x == 0 && blockIdx.y == 0 && tid == 0) *p.claimed = 0;  // for the next call
+    const int own_steps = *p.own_steps;
+    const Line line(pp, pp.streams == p.streams ? own_steps : 0, pp.pair_p, pp.pair_o);
+    const Shares shares(p, p.streams ? own_steps : 0);
+    // whether a worker between an item's first and last one has a step of it
+    auto works = [&](int part, int v) {
+        int lo, hi;
+        if (part ? p.streams & 2 : pp.streams & 1) {
+            shares.range(v, part, lo, hi);
+        } else {
+            const bool paired = part ? pp.pair_o : pp.pair_p;
+            flow_range(line, paired, paired ? v : v >> 1, paired ? 0 : v & 1, part, lo, hi);
+        }
+        return lo < hi;
+    };
+    int note = blockIdx.x;
 #pragma unroll 1
-    while (todo > 0) {
+    while (true) {
+    if (!with_prefix) {
+        if (todo <= 0) {
+            if (note >= p.notes) break;
+            const SplitItem w = p.split[note];
+            note += gridDim.x;
+            own_in = blockIdx.y * MR;
+            st0 = w.row0 + own_in;
+            todo = min(MR, w.rows - own_in);
+            kh = w.kh;
+            own_item = w.item;
+            if (todo <= 0) continue;
+        }
+    } else if (todo <= 0) {
+        break;
+    }
         int run = todo, item[2] = {0, own_item}, in[2] = {0, own_in}, v0[2] = {0, 0}, cnt[2] = {0, 0};
         auto workers_of = [&](int k) {  // (within bounds, even where a kernel that gave up left them unwritten)
-            const int most = 2 * p.workers - 1;
+            const int most = (k ? p : pp).streams ? p.workers + p.chunks - 1 : 2 * pp.workers - 1;
             v0[k] = min(max(p.first[k][item[k]], 0), most);
             cnt[k] = min(max(p.last[k][item[k]], 0), most) - v0[k] + 1;
         };
         if (with_prefix) {  // rows that share the prefix item
-            const int rb = st0 / p.pb;
-            item[0] = kh * p.n_rb + rb;
-            in[0] = st0 - rb * p.pb;
-            run = min(run, p.pb - in[0]);
+            const int rb = st0 / pp.pb;
+            item[0] = kh * pp.n_rb + rb;
+            in[0] = st0 - rb * pp.pb;
+            run = min(run, pp.pb - in[0]);
             workers_of(0);
         }
         if (own) workers_of(1);
@@ -104,12 +135,7 @@ __global__ void __launch_bounds__(256, MR == 32 ? 5 : 4) prefix_attn_merge_kerne
                     if (tid < m) {
                         const int i = c0 + tid, part = i >= cnt[0], k = i - (part ? cnt[0] : 0), v = v0[part] + k;
                         bool has = k == 0 || k == cnt[part] - 1;
-                        if (!has) {  // a worker in between may have no step at all
-                            const bool paired = part ? p.pair_o : p.pair_p;
-                            int lo, hi;
-                            flow_range(line, paired, paired ? v : v >> 1, paired ? 0 : v & 1, part, lo, hi);
-                            has = lo < hi;
-                        }
+                        if (!has) has = works(part, v);  // a worker in between may have no step at all
                         slot[tid] = !has ? -1 : part ? p.own_slot(item[1], v, k == 0) : item[0] + v;
                     } else if (tid < MERGE_CHUNK) {
                         slot[tid] = -1;
@@ -221,27 +247,32 @@ __global__ void __launch_bounds__(256, MR == 32 ? 5 : 4) prefix_attn_merge_kerne
     }
 }
 
-// the plan of a call and its workspace
-static int make_plan(lq_ctx* ctx, const char* who, const PrefixAttnArgs& a, const PagedSeqs& s, bool f32, int D, PrefixPlan* p,
-                     int warp_rows = 8) {
-    const int64_t steps = plan_cut(a, s, f32, ctx->sm_count, p, warp_rows);
-    LQ_REQUIRE(ctx, steps < PREFIX_MAX_STEPS, "%s: %lld steps, more than a launch can number", who, (long long)steps);
-    // LQ_FAULT=prefix_attn_wait: waits inside the kernel run out (tests of what follows then)
+// LQ_FAULT=prefix_attn_wait: waits inside the kernel run out (tests of what follows then)
+static void set_polls(PrefixPlan* p, bool f32) {
     p->hold = fault_injected("prefix_attn_wait");
     p->polls = !p->hold ? 1 << 22 : f32 ? 0 : 1 << 12;
-    const int64_t items_p = (int64_t)a.n_kv * p->n_rb;
+}
+
+// The workspace of a call whose prefix items are cut by pp and whose own items by p (the same plan, but
+// where two kernels share the work)
+static int make_workspace(lq_ctx* ctx, const char* who, const PrefixAttnArgs& a, const PagedSeqs& s, int D, PrefixPlan* p, PrefixPlan* pp) {
+    const int64_t items_p = (int64_t)a.n_kv * pp->n_rb;
     const int64_t items_o = a.n_kv * ((int64_t)s.rows * a.group / p->ob + s.n_seqs + 1);
-    const int64_t items[2] = {p->np ? items_p : 0, items_o};
+    const int64_t items[2] = {pp->np ? items_p : 0, items_o};
+    // workers, or flows of a CTA, that may have a piece
+    const int64_t most[2] = {pp->streams ? pp->workers + pp->chunks : 2ll * pp->workers,
+                             p->streams ? p->workers + p->chunks : 2ll * p->workers};
     size_t at = 0;
     auto place = [&at](int64_t n, size_t size) {
         const size_t here = at;
         at += ((size_t)n * size + 255) & ~(size_t)255;
         return here;
     };
-    const size_t steps_at = place(1, 4), split_at = place(2 * p->workers, sizeof(SplitItem));
+    p->notes = (int)(p->streams ? most[1] : (p->pair_o ? 1 : 2) * p->workers);
+    const size_t steps_at = place(1, 4), split_at = place(most[1], sizeof(SplitItem));
     size_t first_at[2], last_at[2], ml_at[2], o_at[2];
     for (int k = 0; k < 2; k++) {
-        const int64_t slots = k == 1 && p->np == 0 ? 4 * p->workers : items[k] ? items[k] + 2 * p->workers : 0;
+        const int64_t slots = k == 1 && p->np == 0 ? 2 * most[1] : items[k] ? items[k] + most[k] : 0;
         LQ_REQUIRE(ctx, slots < (1ll << 31), "%s: too many partials", who);
         first_at[k] = place(items[k], 4);
         last_at[k] = place(items[k], 4);
@@ -253,6 +284,7 @@ static int make_plan(lq_ctx* ctx, const char* who, const PrefixAttnArgs& a, cons
     if (rc) return rc;
     uint8_t* w = static_cast<uint8_t*>(buffer);
     p->own_steps = reinterpret_cast<int32_t*>(w + steps_at);
+    p->claimed = reinterpret_cast<unsigned*>(w + steps_at + 128);
     p->split = reinterpret_cast<SplitItem*>(w + split_at);
     for (int k = 0; k < 2; k++) {
         p->first[k] = reinterpret_cast<int32_t*>(w + first_at[k]);
@@ -260,18 +292,77 @@ static int make_plan(lq_ctx* ctx, const char* who, const PrefixAttnArgs& a, cons
         p->ml[k] = reinterpret_cast<float2*>(w + ml_at[k]);
         p->o[k] = reinterpret_cast<float*>(w + o_at[k]);
     }
+    if (pp != p) {
+        pp->own_steps = p->own_steps;
+        pp->claimed = p->claimed;
+        pp->split = p->split;
+        pp->notes = p->notes;
+        pp->cap[1] = p->cap[1];
+        for (int k = 0; k < 2; k++) pp->first[k] = p->first[k], pp->last[k] = p->last[k], pp->ml[k] = p->ml[k], pp->o[k] = p->o[k];
+    }
     return LQ_OK;
 }
 
+// the plan of a call and its workspace
+static int make_plan(lq_ctx* ctx, const PrefixAttnArgs& a, const PagedSeqs& s, bool f32, int D, PrefixPlan* p) {
+    const int64_t steps = plan_cut(a, s, f32, ctx->sm_count, p);
+    LQ_REQUIRE(ctx, steps < PREFIX_MAX_STEPS, "lq_prefix_attention: %lld steps, more than a launch can number", (long long)steps);
+    set_polls(p, f32);
+    return make_workspace(ctx, "lq_prefix_attention", a, s, D, p, p);
+}
+
 template <typename T, int D>
-static int launch_merge(lq_ctx* ctx, const PrefixAttnArgs& a, const PagedSeqs& s, const PrefixPlan& p) {
+static int launch_merge(lq_ctx* ctx, const PrefixAttnArgs& a, const PagedSeqs& s, const PrefixPlan& p, const PrefixPlan& pp) {
     // a row of few heads leaves most of a 32-row CTA idle
     const int mr = p.cap[1] <= 8 ? 8 : 32;
     const int64_t R = (int64_t)s.rows * a.group;
-    const dim3 grid((unsigned)(p.np > 0 ? a.n_kv * (R / p.ob + s.n_seqs) : (p.pair_o ? 1 : 2) * p.workers),
+    const dim3 grid((unsigned)(p.np > 0 ? a.n_kv * (R / p.ob + s.n_seqs) : p.streams ? std::min(p.notes, 8 * ctx->sm_count) : p.notes),
                     (unsigned)ceil_div(p.cap[1], mr));
-    return mr == 8 ? launch_kernel(ctx, prefix_attn_merge_kernel<T, D, 8>, grid, dim3(256), 0, "prefix_attn_merge", a, s, p)
-                   : launch_kernel(ctx, prefix_attn_merge_kernel<T, D, 32>, grid, dim3(256), 0, "prefix_attn_merge", a, s, p);
+    return mr == 8 ? launch_kernel(ctx, prefix_attn_merge_kernel<T, D, 8>, grid, dim3(256), 0, "prefix_attn_merge", a, s, p, pp)
+                   : launch_kernel(ctx, prefix_attn_merge_kernel<T, D, 32>, grid, dim3(256), 0, "prefix_attn_merge", a, s, p, pp);
+}
+
+// An 8-bit cache: which kernel takes which items.
+template <int D>
+static int attend_q8(lq_ctx* ctx, const PrefixAttnArgs& a, const PagedSeqs& s, const PagedQ8& c) {
+    const char* const who = "lq_prefix_attention_q8";
+    const int64_t own_rows = std::min<int64_t>(a.max_q, s.rows) * a.group, all_rows = (int64_t)s.rows * a.group;
+    const bool stream_own = own_rows <= PREFIX_ATTN_Q8_ROWS;
+    const bool stream_prefix = a.prefix_len == 0 ? stream_own : all_rows <= PREFIX_ATTN_Q8_ROWS;
+    PrefixPlan tc, st;
+    int64_t steps_tc = 0, steps_st = 0;
+    if (!stream_own || !stream_prefix) {
+        steps_tc = plan_cut(a, s, false, ctx->sm_count, &tc);
+        set_polls(&tc, false);
+    }
+    if (stream_own) {
+        const int rows = (stream_prefix && a.prefix_len > 0 ? all_rows : own_rows) > 8 ? 16 : 8;
+        if constexpr (D == 128) steps_st = plan_cut(a, s, true, ctx->sm_count, &st, rows, prefix_attn_q8_decode_ctas(rows), 128);
+        else steps_st = plan_cut(a, s, true, ctx->sm_count, &st, rows, PREFIX_ATTN_Q8_WARPS);
+        set_polls(&st, true);
+        st.streams = stream_prefix ? 3 : 2;
+        if (D == 128) st.chunks = 2 * st.workers;
+    }
+    LQ_REQUIRE(ctx, steps_tc < PREFIX_MAX_STEPS && steps_st < PREFIX_MAX_STEPS, "%s: %lld steps, more than a launch can number", who,
+               (long long)std::max(steps_tc, steps_st));
+    PrefixPlan* const own = stream_own ? &st : &tc;
+    PrefixPlan* const pre = stream_prefix ? &st : &tc;
+    if (own != pre) {  // the prefix for itself, and the own items for themselves
+        tc.workers = std::max(1, std::min(ctx->sm_count, tc.sp));
+        tc.workers_mul = ((1ull << 40) + tc.workers - 1) / tc.workers;
+        tc.apart = 1;
+        st.sp = 0;
+        st.cap[0] = tc.cap[0];
+    }
+    int rc = make_workspace(ctx, who, a, s, D, own, pre);
+    if (rc) return rc;
+    if (pre == &tc && (rc = launch_prefix_attn_tc(ctx, a, s, tc, D, &c))) return rc;
+    if (own == &st) {
+        if constexpr (D == 128) rc = launch_prefix_attn_q8_decode(ctx, a, s, c, st);
+        else rc = launch_prefix_attn_q8(ctx, a, s, c, st, D);
+        if (rc) return rc;
+    }
+    return launch_merge<__nv_bfloat16, D>(ctx, a, s, *own, *pre);
 }
 
 // checks and arguments shared by the entry points; esize: bytes of an element of q and out. page_stride:
@@ -352,11 +443,11 @@ extern "C" int lq_prefix_attention(lq_ctx* ctx, const void* q, lq_dtype dtype, i
     a.page_stride = page_stride;
     lq::PrefixPlan p;
     const int D = (int)head_dim;
-    if ((rc = lq::make_plan(ctx, "lq_prefix_attention", a, s, f32, D, &p))) return rc;
+    if ((rc = lq::make_plan(ctx, a, s, f32, D, &p))) return rc;
     rc = f32 ? lq::launch_prefix_attn_f32(ctx, a, s, p, D) : lq::launch_prefix_attn_tc(ctx, a, s, p, D);
     if (rc) return rc;
-    if (f32) return D == 64 ? lq::launch_merge<float, 64>(ctx, a, s, p) : lq::launch_merge<float, 128>(ctx, a, s, p);
-    return D == 64 ? lq::launch_merge<__nv_bfloat16, 64>(ctx, a, s, p) : lq::launch_merge<__nv_bfloat16, 128>(ctx, a, s, p);
+    if (f32) return D == 64 ? lq::launch_merge<float, 64>(ctx, a, s, p, p) : lq::launch_merge<float, 128>(ctx, a, s, p, p);
+    return D == 64 ? lq::launch_merge<__nv_bfloat16, 64>(ctx, a, s, p, p) : lq::launch_merge<__nv_bfloat16, 128>(ctx, a, s, p, p);
 }
 
 extern "C" int lq_prefix_attention_q8(lq_ctx* ctx, const uint16_t* q, int64_t q_stride, int64_t rows, int64_t n_heads,
@@ -379,12 +470,5 @@ extern "C" int lq_prefix_attention_q8(lq_ctx* ctx, const uint16_t* q, int64_t q_
                            block, scale_stride, rows > 0 && n_seqs > 0);
     if (rc) return rc;
     if (rows == 0 || n_seqs == 0) return LQ_OK;
-    const int D = (int)head_dim;
-    lq::PrefixPlan p;
-    const int64_t stacked = (prefix_len > 0 ? rows : std::min(max_q, rows)) * a.group;
-    const bool few = stacked <= 16;
-    if ((rc = lq::make_plan(ctx, "lq_prefix_attention_q8", a, s, few, D, &p, stacked > 8 ? 16 : 8))) return rc;
-    rc = few ? lq::launch_prefix_attn_q8(ctx, a, s, c, p, D) : lq::launch_prefix_attn_tc(ctx, a, s, p, D, &c);
-    if (rc) return rc;
-    return D == 64 ? lq::launch_merge<__nv_bfloat16, 64>(ctx, a, s, p) : lq::launch_merge<__nv_bfloat16, 128>(ctx, a, s, p);
+    return head_dim == 64 ? lq::attend_q8<64>(ctx, a, s, c) : lq::attend_q8<128>(ctx, a, s, c);
 }

@@ -7,12 +7,14 @@
 //               amax / 65024) and split into two bytes, the high ones rows 0-7 of the left operand of
 //               mma.sync m16n8k32 (s8), the low ones rows 8-15, so that K's codes are the right operand
 //               as they lie in memory; 256 hi + lo is exact in 32 bits
-//   P = exp2(S q k_scale - m), running maximum and sum in f32
-//   O += (P v_scale) V   mma.sync m16n8k16 (bf16): V's codes are exact in bf16, and P v_scale is split into
-//               two bf16 parts (16 bits together), again rows 0-7 and 8-15; the accumulators of Q K^T lie
-//               just as the left operand of this product wants them
-// The scales of 16 positions (a block's or a part of one) are one number each, so that they cost a
-// multiplication a score and none a code.
+//   P = exp2(S f - m), l = sum P, in f32, with f = q's and K's scale
+//   O += P' V   mma.sync m16n8k16 (fp16, 16 rows), with V's codes exact in fp16 and P' = exp2(S f + log2
+//               V's scale - m' + 7): m' is a running maximum of its own, so that the weights that count
+//               lie between 2^7 and 2^15 whatever the scales are, and a rounding is 2^-12 (below 2^-21 of the
+//               largest, an absolute 2^-32 of it). The accumulators of Q K^T lie just as the left
+//               operand of this product wants them.
+// The scales of 16 positions (a block's or a part of one) are one number each, so that they cost
+// nothing a code and no more than an addend a score.
 // K and V come by TMA, 32 positions a stage, into a ring of the warp's own; swizzled so that a warp's
 // 16-byte reads meet every bank once. A lane reads 16 bytes of K of one position and of V of one
 // position at a time; which dims they are is the same for all positions, and free. No warp waits
@@ -26,11 +28,13 @@
 #include "lq8_prefix_plan.cuh"
 #include "lq8_tma.cuh"
 
+#include <cuda_fp16.h>
+
 #include <algorithm>
 
 namespace lq {
 
-constexpr int PQ_WARPS = PREFIX_ATTN_F32_WARPS;
+constexpr int PQ_WARPS = PREFIX_ATTN_Q8_WARPS;
 constexpr int PQ_SCAN = 256;
 constexpr int PQ_STAGE = 32;               // positions of a stage
 constexpr int PQ_BATCH = 512;              // positions whose pages and scales lie in the lanes
@@ -42,23 +46,38 @@ __device__ __forceinline__ float pq_ex2(float x) {
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
     return y;
 }
-// c += a b: s8 with s32 sums, bf16 with f32 sums
+// a b with s32 sums (FIRST: from zero), c += a b with f32 sums
+template <bool FIRST>
 __device__ __forceinline__ void pq_mma_s8(int c[4], const uint32_t a[4], uint32_t b0, uint32_t b1) {
-    asm("mma.sync.aligned.m16n8k32.row.col.s32.s8.s8.s32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
-        : "+r"(c[0]), "+r"(c[1]), "+r"(c[2]), "+r"(c[3])
-        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+    if constexpr (FIRST)
+        asm("mma.sync.aligned.m16n8k32.row.col.s32.s8.s8.s32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%10,%10,%10};"
+            : "=r"(c[0]), "=r"(c[1]), "=r"(c[2]), "=r"(c[3])
+            : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "r"(0));
+    else
+        asm("mma.sync.aligned.m16n8k32.row.col.s32.s8.s8.s32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+            : "+r"(c[0]), "+r"(c[1]), "+r"(c[2]), "+r"(c[3])
+            : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
-__device__ __forceinline__ void pq_mma_bf16(float c[4], const uint32_t a[4], uint32_t b0, uint32_t b1) {
-    asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+__device__ __forceinline__ void pq_mma_f16(float c[4], const uint32_t a[4], uint32_t b0, uint32_t b1) {
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
         : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
         : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
-// bytes `sel` of w (two of them, as halves 0x43 b) as a pair of bf16: 0x4300 + b has the value 128 + b for
-// b < 128; so a code is (128 + its low seven bits) - (128, or 256 where the sign is set), exactly
-__device__ __forceinline__ uint32_t pq_bf16(uint32_t w, uint32_t sel) {
-    const uint32_t x = __byte_perm(w, 0x43434343u, sel), lo = x & 0xff7fff7fu, up = x & 0xff80ff80u;
-    const __nv_bfloat162 d = __hsub2(*reinterpret_cast<const __nv_bfloat162*>(&lo), *reinterpret_cast<const __nv_bfloat162*>(&up));
+// two bytes of w (sel 0x4140: the lower ones), which are codes + 128, as a pair of fp16: 0x6400 + b has the
+// value 1024 + b; less 1152 that is the code, exactly
+__device__ __forceinline__ uint32_t pq_f16(uint32_t w, uint32_t sel) {
+    const uint32_t x = __byte_perm(w, 0x64646464u, sel), bias = 0x64806480u;
+    const __half2 d = __hsub2(*reinterpret_cast<const __half2*>(&x), *reinterpret_cast<const __half2*>(&bias));
     return *reinterpret_cast<const uint32_t*>(&d);
+}
+__device__ __forceinline__ uint32_t pq_pack(float a, float b) {
+    const __half2 h = __floats2half2_rn(a, b);
+    return *reinterpret_cast<const uint32_t*>(&h);
+}
+__device__ __forceinline__ float pq_max_nan(float a, float b) {
+    float d;
+    asm("max.NaN.f32 %0, %1, %2;" : "=f"(d) : "f"(a), "f"(b));
+    return d;
 }
 
 // D / 4 dims (from dim t4 D / 4) of a row; every lane calls it, those of real rows write
@@ -127,7 +146,10 @@ prefix_attn_q8_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_co
     int slot = 0;       // of the next stage to be worked on
     unsigned ph = 0;    // and its parity
     bool ok = true;
-    pdl_wait();
+    // Behind the kernel that takes the prefix this one need not wait for it: that one began after its
+    // own wait for what came before, and let this one begin after that. It is waited for at the end.
+    const bool alone = p.streams == 3;
+    if (alone) pdl_wait();
     pdl_trigger();  // (after the wait: the merge reads the call's lengths before its own)
     const int per_entry = (s.n_seqs + PQ_SCAN - 1) / PQ_SCAN;
     const int n_entries = (s.n_seqs + per_entry - 1) / per_entry;
@@ -180,11 +202,12 @@ prefix_attn_q8_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_co
             if (si.kv < si.q) zero_rows<__nv_bfloat16, D>(a, si.q0, si.q - si.kv, lane, 32);
         }
     }
-    const int worker = warp * gridDim.x + blockIdx.x, live = live_rows(s);
-    if (worker >= p.workers) return;
-    const Line line(p, so, true, true);
-    if (a.prefix_len == 0 && lane == 0) p.split[worker].rows = 0;
-    __syncwarp();
+    int worker = warp * gridDim.x + blockIdx.x;
+    const int live = live_rows(s);
+    const Shares line(p, so);
+    if (a.prefix_len == 0)  // pieces that there are not
+        for (int i = worker + line.n + line.pieces; i < p.notes; i += PQ_WARPS * gridDim.x)
+            if (lane == 0) p.split[i].rows = 0;
     const int box = min(1 << s.page_shift, PQ_STAGE), boxes = PQ_STAGE / box, mask = (1 << s.page_shift) - 1;
     // column n of a tile of Q K^T is position perm(n) of its 8: with D = 64, where two positions share the
     // 128 bytes of all banks, in an order that keeps V's reads apart
@@ -193,11 +216,18 @@ prefix_attn_q8_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_co
     // where in a stage vector `ch` (16 bytes) of position x lies
     auto vec = [](int x, int ch) { return D == 128 ? x * 128 + ((ch ^ (x & 7)) << 4) : x * 64 + ((ch ^ ((x >> 1) & 3)) << 4); };
 
+    if (worker >= p.workers) worker = line.n + line.pieces;
+#pragma unroll 1
+    while (worker < line.n + line.pieces && ok) {
+    unsigned next = 0;  // the piece after this one
+    if (line.pieces > 0 && lane == 0) next = atomicAdd(p.claimed, 1u);
+    if (a.prefix_len == 0 && lane == 0) p.split[worker].rows = 0;
+    __syncwarp();
 #pragma unroll 1
     for (int part = 0; part < 2; part++) {
         const bool own = part;
         int step, hi;
-        flow_range(line, true, worker, 0, own, step, hi);
+        line.range(worker, own, step, hi);
         if (step >= hi) continue;
         // the item of the first step: sequence, kv head, row block, tile
         int b = 0, kh, rb, tile, n_rb = p.n_rb, nt = p.np;
@@ -281,14 +311,16 @@ prefix_attn_q8_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_co
                 }
                 return id;
             };
-            auto scales_at = [&](int x, int id, float& ks, float& vs) {
-                ks = vs = 0.0f;
+            auto scales_at = [&](int x, int id, float& ks, float& lv) {  // V's as its logarithm
+                float vs = 0.0f;
+                ks = 0.0f;
                 if (id < s.n_pages) {
                     const int64_t at = id * cc.scale_stride + ((int64_t)kh << (s.page_shift - cc.block_shift)) +
                                        (((x + 16 * lane) & mask) >> cc.block_shift);
                     ks = cc.k_scale[at];
                     vs = cc.v_scale[at];
                 }
+                lv = __log2f(vs);
             };
             int pg = page_at(pos0), pg_next = page_at(pos0 + PQ_BATCH), pg_then = 0;
             int sent = 0;                                 // stages on the way or done
@@ -312,8 +344,8 @@ prefix_attn_q8_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_co
             };
 #pragma unroll 1
             for (int i = 0; i < SLOTS && i < stages; i++) send(0);
-            float ks, vs, ks_next = 0.0f, vs_next = 0.0f;
-            scales_at(pos0, pg, ks, vs);
+            float ks, lv, ks_next = 0.0f, lv_next = 0.0f;
+            scales_at(pos0, pg, ks, lv);
             // ---- Q, in two bytes ----
             uint32_t q[NR][KS][4];
             float qf[NR];      // what a whole number of Q K^T counts for, in units of log2, without K's scale
@@ -357,14 +389,17 @@ prefix_attn_q8_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_co
                         q[r][i][2 * h + 1] = dn;
                     }
             }
-            float m[NR], l[NR], o[NR][NT][4];
+            int all_see = vis[0];  // positions that all of the warp's rows see
 #pragma unroll
-            for (int r = 0; r < NR; r++) {
-                m[r] = -INFINITY;
-                l[r] = 0.0f;
+            for (int r = 1; r < NR; r++) all_see = min(all_see, vis[r]);
+            all_see = __reduce_min_sync(0xffffffffu, all_see);
+            // running maxima of the scores (for l) and of the scores + log2 V's scale (for O, 2^7 times as
+            // large as that says), sums
+            float m[NR], mv[NR], l[NR], o[NT][4];
 #pragma unroll
-                for (int i = 0; i < NT; i++) o[r][i][0] = o[r][i][1] = o[r][i][2] = o[r][i][3] = 0.0f;
-            }
+            for (int r = 0; r < NR; r++) m[r] = mv[r] = -INFINITY, l[r] = 0.0f;
+#pragma unroll
+            for (int i = 0; i < NT; i++) o[i][0] = o[i][1] = o[i][2] = o[i][3] = 0.0f;
 #pragma unroll 1
             for (int i = 0; i < stages; i++) {
                 const int x = pos0 + i * PQ_STAGE, in = (i * PQ_STAGE) & (PQ_BATCH - 1);
@@ -373,10 +408,10 @@ prefix_attn_q8_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_co
                         pg = pg_next;
                         pg_next = pg_then;
                         ks = ks_next;
-                        vs = vs_next;
+                        lv = lv_next;
                     }
                     pg_then = page_at(x + 2 * PQ_BATCH);
-                    scales_at(x + PQ_BATCH, pg_next, ks_next, vs_next);
+                    scales_at(x + PQ_BATCH, pg_next, ks_next, lv_next);
                 }
                 ok = __all_sync(0xffffffffu, mbar_wait(&full[warp][slot], ph, p.polls));
                 if (!ok) {  // this copy and the later ones may not land in shared memory that is no longer this kernel's
@@ -387,12 +422,15 @@ prefix_attn_q8_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_co
                 }
                 const uint8_t* const kt = mine + slot * SLOT;
                 const uint8_t* const vt = kt + HALF;
-                float sc[NR][2][2][2], top[NR];  // scores: positions 16 h + 8 t + my_p[e]
-#pragma unroll
-                for (int r = 0; r < NR; r++) top[r] = -INFINITY;
+                // scores, without the factor f of the row and of 16 positions: positions 16 h + 8 t + my_p[e]
+                float sc[NR][2][2][2], f[NR][2], l1[2];
 #pragma unroll
                 for (int h = 0; h < 2; h++) {
                     const float k1 = __shfl_sync(0xffffffffu, ks, (in >> 4) + h);
+                    l1[h] = __shfl_sync(0xffffffffu, lv, (in >> 4) + h);
+                    // (never so small that a masked score loses its minus infinity)
+#pragma unroll
+                    for (int r = 0; r < NR; r++) f[r][h] = pq_max_nan(qf[r] * k1, 1e-37f);
 #pragma unroll
                     for (int t = 0; t < 2; t++) {
                         uint32_t w[KS * 2];
@@ -403,52 +441,63 @@ prefix_attn_q8_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_co
                         }
 #pragma unroll
                         for (int r = 0; r < NR; r++) {
-                            int c[4] = {0, 0, 0, 0};
+                            int c[4];
+                            pq_mma_s8<true>(c, q[r][0], w[0], w[1]);
 #pragma unroll
-                            for (int j = 0; j < KS; j++) pq_mma_s8(c, q[r][j], w[2 * j], w[2 * j + 1]);
-                            const float f = qf[r] * k1;
+                            for (int j = 1; j < KS; j++) pq_mma_s8<false>(c, q[r][j], w[2 * j], w[2 * j + 1]);
 #pragma unroll
-                            for (int e = 0; e < 2; e++) {
-                                float v = (float)(c[e] * 256 + c[2 + e]) * f;
-                                if (x + 16 * h + 8 * t + my_p[e] >= vis[r]) v = -INFINITY;
-                                sc[r][h][t][e] = v;
-                                top[r] = fmaxf(top[r], v);
-                            }
+                            for (int e = 0; e < 2; e++) sc[r][h][t][e] = (float)(c[e] * 256 + c[2 + e]);
                         }
                     }
                 }
+                if (x + PQ_STAGE > all_see) {
+#pragma unroll
+                    for (int r = 0; r < NR; r++)
+#pragma unroll
+                        for (int j = 0; j < 8; j++)
+                            if (x + 8 * (j >> 1) + my_p[j & 1] >= vis[r]) sc[r][j >> 2][(j >> 1) & 1][j & 1] = -INFINITY;
+                }
+                float top[NR], tov[NR];
+                bool grows = i == 0;
 #pragma unroll
                 for (int r = 0; r < NR; r++) {
-                    top[r] = fmaxf(top[r], __shfl_xor_sync(0xffffffffu, top[r], 1));
-                    top[r] = fmaxf(top[r], __shfl_xor_sync(0xffffffffu, top[r], 2));
-                    // a maximum that grew by less than 2^8 stays: p <= 256 costs an f32 sum nothing
-                    if (__any_sync(0xffffffffu, top[r] > m[r] + 8.0f || i == 0)) {
-                        const float mn = fmaxf(m[r], top[r]);
-                        const float f = mn == -INFINITY ? 1.0f : pq_ex2(m[r] - mn);
+                    float a0 = fmaxf(fmaxf(sc[r][0][0][0], sc[r][0][0][1]), fmaxf(sc[r][0][1][0], sc[r][0][1][1])) * f[r][0];
+                    float a1 = fmaxf(fmaxf(sc[r][1][0][0], sc[r][1][0][1]), fmaxf(sc[r][1][1][0], sc[r][1][1][1])) * f[r][1];
+                    top[r] = fmaxf(a0, a1);
+                    tov[r] = fmaxf(a0 + l1[0], a1 + l1[1]);
+                    // (each lane for itself: a row's lanes follow the one that looks up its own)
+                    grows |= top[r] > m[r] + 8.0f || tov[r] > mv[r] + 8.0f;
+                }
+                // a maximum that grew by less than 2^8 stays: p <= 2^8 costs an f32 sum nothing, and
+                // 2^15 is still an fp16
+                if (__any_sync(0xffffffffu, grows)) {
+#pragma unroll
+                    for (int r = 0; r < NR; r++) {
+#pragma unroll
+                        for (int d = 1; d < 4; d <<= 1) {
+                            top[r] = fmaxf(top[r], __shfl_xor_sync(0xffffffffu, top[r], d));
+                            tov[r] = fmaxf(tov[r], __shfl_xor_sync(0xffffffffu, tov[r], d));
+                        }
+                        const float mn = fmaxf(m[r], top[r]), vn = fmaxf(mv[r], tov[r]);
+                        l[r] *= mn == -INFINITY ? 1.0f : pq_ex2(m[r] - mn);
+                        const float fo = vn == -INFINITY ? 1.0f : pq_ex2(mv[r] - vn);
                         m[r] = mn;
-                        l[r] *= f;
+                        mv[r] = vn;
 #pragma unroll
-                        for (int j = 0; j < NT; j++)
-#pragma unroll
-                            for (int e = 0; e < 4; e++) o[r][j][e] *= f;
+                        for (int j = 0; j < NT; j++) o[j][2 * r] *= fo, o[j][2 * r + 1] *= fo;
                     }
                 }
 #pragma unroll
                 for (int h = 0; h < 2; h++) {
-                    const float v1 = __shfl_sync(0xffffffffu, vs, (in >> 4) + h);
-                    uint32_t pa[NR][4];
+                    uint32_t pa[4] = {0, 0, 0, 0};  // rows 0-7 and 8-15 of either eight positions
 #pragma unroll
                     for (int r = 0; r < NR; r++) {
                         const float neg = m[r] == -INFINITY ? 0.0f : -m[r];
+                        const float add = mv[r] == -INFINITY ? 0.0f : l1[h] - mv[r] + 7.0f;
 #pragma unroll
                         for (int t = 0; t < 2; t++) {
-                            float e0 = pq_ex2(sc[r][h][t][0] + neg), e1 = pq_ex2(sc[r][h][t][1] + neg);
-                            l[r] += e0 + e1;
-                            e0 *= v1;
-                            e1 *= v1;
-                            const uint32_t big = pack_bf16x2(e0, e1);
-                            pa[r][2 * t] = big;
-                            pa[r][2 * t + 1] = pack_bf16x2(e0 - __uint_as_float(big << 16), e1 - __uint_as_float(big & 0xffff0000u));
+                            l[r] += pq_ex2(fmaf(sc[r][h][t][0], f[r][h], neg)) + pq_ex2(fmaf(sc[r][h][t][1], f[r][h], neg));
+                            pa[2 * t + r] = pq_pack(pq_ex2(fmaf(sc[r][h][t][0], f[r][h], add)), pq_ex2(fmaf(sc[r][h][t][1], f[r][h], add)));
                         }
                     }
                     // V of the four positions that this lane's part of the right operand holds
@@ -464,6 +513,8 @@ prefix_attn_q8_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_co
                             const uint2 u = *reinterpret_cast<const uint2*>(vt + vec(at, gr >> 1) + (gr & 1) * 8);
                             w[j][0] = u.x, w[j][1] = u.y;
                         }
+#pragma unroll
+                        for (int k = 0; k < VW; k++) w[j][k] ^= 0x80808080u;
                     }
 #pragma unroll
                     for (int j = 0; j < VW; j++)
@@ -471,13 +522,8 @@ prefix_attn_q8_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_co
                         for (int e = 0; e < 2; e++) {  // dims 4 j + 2 e, 4 j + 2 e + 1
                             const uint32_t x0 = __byte_perm(w[0][j], w[1][j], e ? 0x7362 : 0x5140);
                             const uint32_t x1 = __byte_perm(w[2][j], w[3][j], e ? 0x7362 : 0x5140);
-                            const uint32_t b0 = pq_bf16(x0, 0x4140), b1 = pq_bf16(x1, 0x4140);
-                            const uint32_t b2 = pq_bf16(x0, 0x4342), b3 = pq_bf16(x1, 0x4342);
-#pragma unroll
-                            for (int r = 0; r < NR; r++) {
-                                pq_mma_bf16(o[r][4 * j + 2 * e], pa[r], b0, b1);
-                                pq_mma_bf16(o[r][4 * j + 2 * e + 1], pa[r], b2, b3);
-                            }
+                            pq_mma_f16(o[4 * j + 2 * e], pa, pq_f16(x0, 0x4140), pq_f16(x1, 0x4140));
+                            pq_mma_f16(o[4 * j + 2 * e + 1], pa, pq_f16(x0, 0x4342), pq_f16(x1, 0x4342));
                         }
                 }
                 __syncwarp();  // (read by every lane)
@@ -498,11 +544,13 @@ prefix_attn_q8_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_co
                 const int tok = a.group_div(row0 + min(row, n - 1)), head = kh * a.group + row0 + min(row, n - 1) - tok * a.group;
                 const int64_t at = own ? p.own_slot(item, worker, begins) : item + worker;
                 const int cap = p.cap[part];
+                // O in the units of m
+                const float back = m[r] == -INFINITY || mv[r] == -INFINITY ? 0.0f : pq_ex2(mv[r] - 7.0f - m[r]);
                 float v[D / 4];
 #pragma unroll
                 for (int j = 0; j < NT; j++) {
-                    v[j] = o[r][j][0] + o[r][j][2];
-                    v[NT + j] = o[r][j][1] + o[r][j][3];
+                    v[j] = o[j][2 * r] * back;
+                    v[NT + j] = o[j][2 * r + 1] * back;
                 }
                 if (!whole) {
                     if (real) {
@@ -545,6 +593,9 @@ prefix_attn_q8_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_co
             }
         }
     }
+    worker = line.pieces > 0 ? line.n + (int)min(__shfl_sync(0xffffffffu, next, 0), (unsigned)line.pieces) : line.n;
+    }
+    if (!alone) pdl_wait();
 }
 
 template <int D, int NR>

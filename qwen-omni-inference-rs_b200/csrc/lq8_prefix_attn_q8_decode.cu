@@ -1,0 +1,747 @@
+// lq8_prefix_attn_q8_decode.cu -- the shared-prefix attention for 8-bit caches with up to 16 stacked rows
+// a kv head (a decode step), head dimension 128: codes go from memory into int8 products on tcgen05
+// as they are, and no thread ever touches one.
+//
+// A CTA walks its share of the line of steps (Shares in lq8_prefix_plan.cuh), 128 positions each; three
+// CTAs fit on an SM (two with 16 rows) and hide each other's latency. With R = 8 or 16 rows:
+//   S^T = K Q^T   kind::i8, M 128 positions, N 2 R, K 128 dims: a row of Q is rounded to 16 bits of its
+//                 largest value (within amax / 65024) and split into two bytes, which are two
+//                 columns; 256 high + low is exact in 32 bits. K's tile as TMA brings it.
+//   a thread has one position of all rows: s = S q k_scale, t = s + log2 v_scale, u the tile's largest
+//   t of each row (a warp reduction, four warps by way of shared memory), e = 2^(t - u),
+//   l += e 2^(u - m) / v_scale, and e rounded to 15 bits as two bytes of P^T in shared memory
+//   O^T = V^T P^T kind::i8, M 128 dims, N 2 R, K 128 positions: V's tile as TMA brings it, the
+//                 MN-major operand
+//   a thread has one dim of all rows: o += (256 high + low) 2^(u - m)
+// m is a running maximum of u; o and l are multiplied by 2^(m_old - m_new) when it grew by more than
+// 2^8. Since a tile's weights are rounded relative to its own largest one, long tails of small
+// weights keep their 15 bits. S and O are double-buffered in TMEM: the next tile's S and the last tile's
+// O are in the tensor pipe while a tile is in its softmax.
+//
+// Warps 0-3: softmax (TMEM lane = position = dim = thread); warp 4: walks the line, reads the page table
+// and brings tiles page by page (128-byte swizzle; pages past the end come as zeros); warp 5: TMEM
+// allocator and MMA issuer. Every wait is bounded by a number of polls; when one runs out all warps of the CTA
+// leave, its copies and MMAs in flight are waited for, and the error flag is set.
+// TMA loads here read only this GPU's memory and use no multicast.
+#include "lq8_async.cuh"
+#include "lq8_fused.cuh"
+#include "lq8_paged_q8.cuh"
+#include "lq8_prefix_attn.cuh"
+#include "lq8_prefix_plan.cuh"
+#include "lq8_tcgen05.cuh"
+#include "lq8_tma.cuh"
+
+#include <algorithm>
+
+namespace lq {
+
+constexpr int PD_TILE = 128;     // positions of a step
+constexpr int PD_STAGES = 4;     // tiles of K or V (16 KB)
+constexpr int PD_BYTES = PD_TILE * 128;
+constexpr int PD_THREADS = 192;
+constexpr int PD_SCAN = 128;     // entries of the scan over the sequences
+constexpr int ERR_PD_WAIT = 97;  // a wait ran out
+constexpr int pd_ctas(int R) { return R == 8 ? 3 : 2; }
+
+enum { PD_OWN = 1, PD_END = 2, PD_WHOLE = 4 };
+// the steps [t0, t1) of one item
+struct alignas(16) PdSeg {
+    int t0, t1;     // tiles
+    int n;          // rows
+    int flags;
+    int kh, b;      // kv head; sequence (own items)
+    int kv_end;     // positions the item sees
+    int row0;       // first stacked row
+    int voff;       // own items: the stacked row of token t sees t + voff positions
+    int slot;       // slot of the partial
+    int pad[2];
+};
+
+template <int R>
+struct PdCtl {
+    uint64_t full[PD_STAGES], empty[PD_STAGES], seg_full[2], seg_empty[2];
+    uint64_t q_full, s_full[2], p_full[2], o_full[2], met[2], done;
+    uint32_t tmem;
+    int abort;
+    int issued;     // copies that the producer started
+    int pad;
+    PdSeg seg[2];
+    alignas(16) float red[2][4][R];  // a warp's maxima, and at a segment's end its sums
+    alignas(16) float qf[R];         // what a whole number of S counts for, without K's scale
+    int scan[PD_SCAN + 1];           // own steps before each entry
+};
+
+struct PdArgs {
+    PrefixAttnArgs a;
+    PagedSeqs s;
+    PrefixPlan p;
+    PagedQ8 c;
+};
+
+// D s32, A and B s8, M 128, N n; A MN-major or K-major
+__host__ __device__ constexpr uint32_t pd_idesc(int n, int a_mn) {
+    return (2u << 4) | (1u << 7) | (1u << 10) | ((uint32_t)a_mn << 15) | ((uint32_t)(n >> 3) << 17) | (8u << 24);
+}
+__device__ __forceinline__ void mma_i8(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t acc) {
+    asm volatile(
+        "{\n .reg .pred p;\n setp.ne.b32 p, %4, 0;\n"
+        " tcgen05.mma.cta_group::1.kind::i8 [%0], %1, %2, %3, {%5, %5, %5, %5}, p;\n}\n" ::"r"(d),
+        "l"(a), "l"(b), "r"(idesc), "r"(acc), "r"(0));
+}
+
+// Bounded wait by a whole warp: `polls` polls (try_wait sleeps between them), or until another warp of the CTA
+// gave up; then the CTA tears down and reports. The vote keeps the warp together.
+__device__ __forceinline__ bool pd_wait(int* abort, uint64_t* bar, unsigned parity, int polls) {
+#pragma unroll 1
+    for (int i = 0; i < polls; i++) {
+        if (__all_sync(0xffffffffu, mbar_try_wait(bar, parity))) return true;
+        if (__any_sync(0xffffffffu, *reinterpret_cast<volatile int*>(abort))) break;
+    }
+    *reinterpret_cast<volatile int*>(abort) = 1;
+    return false;
+}
+
+// 2 R columns of the warp's 32 TMEM lanes
+template <int R>
+__device__ __forceinline__ void pd_ld(uint32_t* r, uint32_t addr) {
+    if constexpr (R == 8) tmem_ld16(r, addr);
+    else tmem_ld32(r, addr);
+    tmem_wait_ld();
+}
+
+// the largest of the warp's values
+__device__ __forceinline__ float pd_warp_max(float v) {
+    float d;
+    asm volatile("redux.sync.max.f32 %0, %1, 0xffffffff;" : "=f"(d) : "f"(v));
+    return d;
+}
+
+// sums over the warp of R values a lane; lane 32 / R i has the i-th
+template <int R>
+__device__ __forceinline__ float pd_warp_sums(float* v, int lane) {
+    int half = 16;
+#pragma unroll
+    for (int n = R / 2; n >= 1; n >>= 1, half >>= 1) {
+        const bool up = lane & half;
+#pragma unroll
+        for (int i = 0; i < n; i++) {
+            const float give = up ? v[i] : v[i + n], keep = up ? v[i + n] : v[i];
+            v[i] = keep + __shfl_xor_sync(0xffffffffu, give, half);
+        }
+    }
+    float t = v[0];
+#pragma unroll
+    for (int d = 16 / R; d > 0; d >>= 1) t += __shfl_xor_sync(0xffffffffu, t, d);
+    return t;
+}
+
+template <int R>
+__global__ void __launch_bounds__(PD_THREADS, pd_ctas(R))
+prefix_attn_q8_decode_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v,
+                             const __grid_constant__ PdArgs g) {
+    constexpr int D = 128, N = 2 * R;             // columns of S^T and O^T
+    constexpr uint32_t OPERAND = N * 128;         // bytes of Q^T's or P^T's planes
+    constexpr uint32_t COLUMNS = R == 8 ? 64 : 128;
+    const PrefixAttnArgs& a = g.a;
+    const PagedSeqs& s = g.s;
+    const PrefixPlan& p = g.p;
+    extern __shared__ uint8_t smem_raw[];
+    const uint32_t raw = smem_addr(smem_raw);
+    uint8_t* const ring = smem_raw + (((raw + 1023) & ~1023u) - raw);
+    uint8_t* const q_sm = ring + PD_STAGES * PD_BYTES;
+    uint8_t* const p_sm = q_sm + OPERAND;         // two of them
+    PdCtl<R>& c = *reinterpret_cast<PdCtl<R>*>(p_sm + 2 * OPERAND);
+    const int tid = threadIdx.x, warp = __shfl_sync(0xffffffffu, tid >> 5, 0), lane = tid & 31;
+
+    if (tid == 0) {
+        for (int i = 0; i < PD_STAGES; i++) mbar_init(&c.full[i], 1), mbar_init(&c.empty[i], 1);
+        for (int i = 0; i < 2; i++) {
+            mbar_init(&c.seg_full[i], 1);
+            mbar_init(&c.seg_empty[i], 5);  // four softmax warps, MMA issuer
+            mbar_init(&c.s_full[i], 1);
+            mbar_init(&c.p_full[i], 4);
+            mbar_init(&c.o_full[i], 1);
+            mbar_init(&c.met[i], 4);
+        }
+        mbar_init(&c.q_full, 4);
+        mbar_init(&c.done, 1);
+        c.abort = c.issued = 0;
+        mbar_fence_init();
+    }
+    if (warp == 4 && lane == 0) {
+        tma_prefetch_map(&map_k);
+        tma_prefetch_map(&map_v);
+    }
+    if (warp == 5) {
+        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_addr(&c.tmem)), "n"(COLUMNS));
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
+    }
+    // Behind the kernel that takes the prefix this one need not wait for it: that one began after its
+    // own wait for what came before, and let this one begin after that. It is waited for at the end.
+    const bool alone = p.streams == 3;
+    if (alone) pdl_wait();
+    pdl_trigger();  // (after the wait: the merge reads the call's lengths before its own)
+    // own steps of every entry (a run of per_entry sequences), then their running sum
+    const int per_entry = (s.n_seqs + PD_SCAN - 1) / PD_SCAN;
+    const int n_entries = (s.n_seqs + per_entry - 1) / per_entry;
+    const OwnSteps os{a, p};
+    bool fell = false;
+#pragma unroll 1
+    for (int e = tid; e < n_entries; e += PD_THREADS) {
+        int n = 0;
+#pragma unroll 1
+        for (int b = e * per_entry; b < min(s.n_seqs, (e + 1) * per_entry); b++) {
+            const SeqInfo si = seq_info(a, s, b, blockIdx.x == 0);
+            fell |= falls(s, b);
+            n += os.per_head(si) * a.n_kv;
+        }
+        c.scan[e + 1] = n;
+    }
+    fell = __syncthreads_or(fell);
+    if (warp == 0) {
+        int run = 0;
+#pragma unroll 1
+        for (int e0 = 0; e0 < n_entries; e0 += 32) {
+            int v = e0 + lane < n_entries ? c.scan[e0 + lane + 1] : 0;
+#pragma unroll
+            for (int o = 1; o < 32; o <<= 1) {
+                const int u = __shfl_up_sync(0xffffffffu, v, o);
+                if (lane >= o) v += u;
+            }
+            if (e0 + lane < n_entries) c.scan[e0 + lane + 1] = run + v;
+            run += __shfl_sync(0xffffffffu, v, 31);
+        }
+        if (lane == 0) c.scan[0] = 0;
+    }
+    tc_before();
+    __syncthreads();
+    tc_after();
+    const uint32_t tmem = __shfl_sync(0xffffffffu, c.tmem, 0);
+    const int so = fell ? 0 : c.scan[n_entries];
+    if (blockIdx.x == 0 && tid == 0) *p.own_steps = so;
+    // a warp's next segment
+    unsigned taken = 0;
+    auto fetch = [&](PdSeg& o) {
+        if (!pd_wait(&c.abort, &c.seg_full[taken & 1], (taken >> 1) & 1u, p.polls)) return false;
+        const int v = reinterpret_cast<const int*>(&c.seg[taken & 1])[lane < 12 ? lane : 0];
+        auto field = [&](int k) { return __shfl_sync(0xffffffffu, v, k); };  // uniform in the warp
+        o.t0 = field(0), o.t1 = field(1), o.n = field(2), o.flags = field(3), o.kh = field(4), o.b = field(5);
+        o.kv_end = field(6), o.row0 = field(7), o.voff = field(8), o.slot = field(9);
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&c.seg_empty[taken & 1]);
+        taken++;
+        return !(o.flags & PD_END);
+    };
+
+    if (warp < 4) {
+        // ------------------------------ softmax ------------------------------
+        const uint32_t t_lane = tmem + ((uint32_t)(warp * 32) << 16);
+        const float cs = a.scale * 1.44269504088896340736f;  // scores in units of log2
+        const int mask = (1 << s.page_shift) - 1;
+        int n_tile = 0;          // tiles so far (buffer and parity of S, P, O)
+        unsigned meetings = 0, q_ph = 0;
+        // values of the warps: each warp's to shared memory, then all of them
+        auto meet = [&]() {
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&c.met[meetings & 1]);
+            const bool there = pd_wait(&c.abort, &c.met[meetings & 1], (meetings >> 1) & 1u, p.polls);
+            meetings++;
+            return there;
+        };
+        PdSeg sg;
+        bool ok = true;
+#pragma unroll 1
+        while (ok && fetch(sg)) {
+            // ---- this position's scales: pages two tiles ahead, scales one ----
+            const int32_t* const table = sg.flags & PD_OWN ? s.table + (int64_t)sg.b * s.table_ld : a.prefix_table;
+            auto page_at = [&](int t) {
+                const int x = t * PD_TILE + tid;
+                int id = -1;
+                if (t < sg.t1 && x < sg.kv_end) id = table[x >> s.page_shift];
+                return (unsigned)id < (unsigned)s.n_pages ? id : -1;  // (reported by the producer)
+            };
+            auto scales_at = [&](int t, int id, float& ks, float& vs) {
+                ks = 0.0f;
+                vs = 1.0f;
+                if (id >= 0) {
+                    const int64_t at = id * g.c.scale_stride + ((int64_t)sg.kh << (s.page_shift - g.c.block_shift)) +
+                                       (((t * PD_TILE + tid) & mask) >> g.c.block_shift);
+                    ks = g.c.k_scale[at];
+                    vs = g.c.v_scale[at];
+                }
+            };
+            int id_next = page_at(sg.t0), id_then = page_at(sg.t0 + 1);
+            // ---- Q in two bytes ----
+            {
+                constexpr int TPR = 128 / R, DIMS = D / TPR;  // threads of a row, dims of a thread
+                const int r = tid / TPR, part = tid % TPR, st = sg.row0 + min(r, sg.n - 1), tok = a.group_div(st);
+                const uint4* src = reinterpret_cast<const uint4*>(static_cast<const __nv_bfloat16*>(a.q) + (int64_t)tok * a.q_stride +
+                                                                  (int64_t)(sg.kh * a.group + st - tok * a.group) * D + part * DIMS);
+                uint32_t w[DIMS / 2], top = 0;
+#pragma unroll
+                for (int i = 0; i < DIMS / 8; i++) {
+                    const uint4 u = src[i];
+                    w[4 * i] = u.x, w[4 * i + 1] = u.y, w[4 * i + 2] = u.z, w[4 * i + 3] = u.w;
+                }
+#pragma unroll
+                for (int i = 0; i < DIMS / 2; i++) top = max(top, max(w[i] & 0x7fff0000u, (w[i] << 16) & 0x7fff0000u));
+#pragma unroll
+                for (int d = 1; d < TPR; d <<= 1) top = max(top, __shfl_xor_sync(0xffffffffu, top, d));
+                const float amax = __uint_as_float(top);
+                // (a row of values below 2^-100 counts as zero)
+                const bool fine = amax >= 7.8886e-31f && amax < INFINITY;
+                const float by = fine ? 32512.0f / amax : 0.0f;
+                uint32_t up[DIMS / 4], dn[DIMS / 4];
+#pragma unroll
+                for (int i = 0; i < DIMS / 4; i++) {
+                    up[i] = dn[i] = 0;
+#pragma unroll
+                    for (int e = 0; e < 4; e++) {
+                        const uint32_t u = w[2 * i + (e >> 1)];
+                        const int v = __float2int_rn(__uint_as_float(e & 1 ? u & 0xffff0000u : u << 16) * by);
+                        up[i] |= (uint32_t)(((v + 128) >> 8) & 0xff) << (8 * e);
+                        dn[i] |= (uint32_t)(v & 0xff) << (8 * e);
+                    }
+                }
+                // (rows r and R + r swizzle alike: both are r modulo 8)
+                const uint32_t at = (((part * DIMS >> 4) ^ (r & 7)) << 4) + (part * DIMS & 15);
+#pragma unroll
+                for (int i = 0; i < DIMS / 4; i += 2) {
+                    *reinterpret_cast<uint2*>(q_sm + r * 128 + at + 4 * i) = make_uint2(up[i], up[i + 1]);
+                    *reinterpret_cast<uint2*>(q_sm + (R + r) * 128 + at + 4 * i) = make_uint2(dn[i], dn[i + 1]);
+                }
+                if (part == 0) c.qf[r] = fine ? amax * (1.0f / 32512.0f) * cs : amax < INFINITY ? 0.0f : __uint_as_float(0x7fffffffu);
+                proxy_fence();
+                __syncwarp();
+                if (lane == 0) mbar_arrive(&c.q_full);
+            }
+            float ks, vs;
+            scales_at(sg.t0, id_next, ks, vs);
+            ok = pd_wait(&c.abort, &c.q_full, q_ph, p.polls);
+            if (!ok) break;
+            q_ph ^= 1;
+            auto seen_by = [&](int r) {  // positions that row r sees
+                return sg.flags & PD_OWN ? min(sg.kv_end, max(0, a.group_div(sg.row0 + min(r, sg.n - 1)) + sg.voff)) : sg.kv_end;
+            };
+            const int all_see = seen_by(0);  // (the first row's token comes first)
+            float m[R], l[R], o[R], w[R];    // w: what the last tile's O counts for
+#pragma unroll
+            for (int r = 0; r < R; r++) m[r] = -INFINITY, l[r] = o[r] = w[r] = 0.0f;
+            // O of the tile before
+            auto take_o = [&](int k) {
+                if (!pd_wait(&c.abort, &c.o_full[k & 1], (k >> 1) & 1u, p.polls)) return false;
+                tc_after();
+                uint32_t v[N];
+                pd_ld<R>(v, t_lane + 2 * N + (k & 1) * N);
+#pragma unroll
+                for (int r = 0; r < R; r++) o[r] = fmaf((float)((int)v[r] * 256 + (int)v[R + r]), w[r], o[r]);
+                tc_before();
+                return true;
+            };
+#pragma unroll 1
+            for (int t = sg.t0; t < sg.t1; t++, n_tile++) {
+                const float k1 = ks, v1 = vs > 0.0f || vs != vs ? vs : 8.6736e-19f;  // (codes of a scale of zero are zero)
+                const float lv = __log2f(v1), per = __frcp_rn(v1);
+                id_next = id_then;
+                id_then = page_at(t + 2);
+                scales_at(t + 1, id_next, ks, vs);
+                ok = pd_wait(&c.abort, &c.s_full[n_tile & 1], (n_tile >> 1) & 1u, p.polls);
+                if (!ok) break;
+                tc_after();
+                float e[R];
+                {
+                    uint32_t v[N];
+                    pd_ld<R>(v, t_lane + (n_tile & 1) * N);
+#pragma unroll
+                    for (int r = 0; r < R; r++) e[r] = fmaf((float)((int)v[r] * 256 + (int)v[R + r]), c.qf[r] * k1, lv);
+                }
+                if ((t + 1) * PD_TILE > all_see) {
+#pragma unroll
+                    for (int r = 0; r < R; r++)
+                        if (t * PD_TILE + tid >= seen_by(r)) e[r] = -INFINITY;
+                }
+                float* const mine = c.red[meetings & 1][warp];
+                {
+                    float top[R];
+#pragma unroll
+                    for (int r = 0; r < R; r++) top[r] = pd_warp_max(e[r]);
+                    if (lane == 0) {
+#pragma unroll
+                        for (int r = 0; r < R; r += 4) *reinterpret_cast<float4*>(mine + r) = make_float4(top[r], top[r + 1], top[r + 2], top[r + 3]);
+                    }
+                }
+                const float(*const all)[R] = c.red[meetings & 1];
+                ok = meet();
+                if (!ok) break;
+                float u[R];
+                bool grows = false;
+#pragma unroll
+                for (int r = 0; r < R; r++) {
+                    u[r] = fmaxf(fmaxf(all[0][r], all[1][r]), fmaxf(all[2][r], all[3][r]));
+                    grows |= u[r] > m[r] + 8.0f;
+                }
+                // ---- P^T: column r the high bytes, R + r the low ones ----
+                uint8_t* const pt = p_sm + (n_tile & 1) * OPERAND;
+#pragma unroll
+                for (int r = 0; r < R; r++) {
+                    e[r] = ex2(e[r] - (u[r] == -INFINITY ? 0.0f : u[r]));
+                    const uint32_t v = __float_as_uint(fmaf(e[r], 32512.0f, 12582912.0f));  // (whole number in the low bits)
+                    const uint32_t at = r * 128 + (((tid >> 4) ^ (r & 7)) << 4) + (tid & 15);
+                    pt[at] = (uint8_t)((v + 128) >> 8);
+                    pt[at + R * 128] = (uint8_t)v;
+                }
+                proxy_fence();
+                tc_before();
+                __syncwarp();
+                if (lane == 0) mbar_arrive(&c.p_full[n_tile & 1]);
+                // ---- O of the tile before, then the sums ----
+                if (t > sg.t0) {
+                    ok = take_o(n_tile - 1);
+                    if (!ok) break;
+                }
+                if (grows) {  // (the same in all threads: u and m are)
+#pragma unroll
+                    for (int r = 0; r < R; r++) {
+                        const float mn = fmaxf(m[r], u[r]), f = mn == -INFINITY ? 1.0f : ex2(m[r] - mn);
+                        m[r] = mn;
+                        o[r] *= f;
+                        l[r] *= f;
+                    }
+                }
+#pragma unroll
+                for (int r = 0; r < R; r++) {
+                    const float f = m[r] == -INFINITY ? 0.0f : ex2(u[r] - m[r]);
+                    l[r] = fmaf(e[r], per * f, l[r]);
+                    w[r] = f * (1.0f / 32512.0f);
+                }
+            }
+            if (!ok) break;
+            ok = take_o(n_tile - 1);
+            if (!ok) break;
+            // ---- the segment's result: one dim of each row ----
+            {
+                const float sum = pd_warp_sums<R>(l, lane);
+                if (lane % (32 / R) == 0) c.red[meetings & 1][warp][lane / (32 / R)] = sum;
+                const float(*const all)[R] = c.red[meetings & 1];
+                ok = meet();
+                if (!ok) break;
+#pragma unroll
+                for (int r = 0; r < R; r++) l[r] = (all[0][r] + all[1][r]) + (all[2][r] + all[3][r]);
+            }
+            const bool own = sg.flags & PD_OWN;
+            const int cap = p.cap[own];
+            if (!(sg.flags & PD_WHOLE)) {
+#pragma unroll
+                for (int r = 0; r < R; r++)
+                    if (r < sg.n) {
+                        if (tid == r) p.ml[own][(int64_t)sg.slot * cap + r] = make_float2(m[r], l[r]);
+                        p.o[own][(((int64_t)sg.slot * (D / 4) + (tid >> 2)) * cap + r) * 4 + (tid & 3)] = o[r];
+                    }
+            } else {
+#pragma unroll
+                for (int r = 0; r < R; r++)
+                    if (r < sg.n) {
+                        const float y = l[r] == 0.0f ? 0.0f : o[r] * (l[r] > 0.0f ? 1.0f / l[r] : l[r]);
+                        const int st = sg.row0 + r, tok = a.group_div(st);
+                        const int64_t col = (int64_t)(sg.kh * a.group + st - tok * a.group) * D + tid;
+                        if (a.out) static_cast<__nv_bfloat16*>(a.out)[(int64_t)tok * a.out_stride + col] = __float2bfloat16_rn(y);
+                        if (a.xq) {  // a warp has a block of 32 dims
+                            float d, id;
+                            q8_scale(warp_max(fabsf(y)), d, id);
+                            const int64_t at = (int64_t)tok * a.n_heads * D + col;
+                            if (lane == 0) a.xd[at / 32] = f2h(d);
+                            a.xq[at] = (int8_t)q8_quant(y, id);
+                        }
+                    }
+            }
+        }
+    } else if (warp == 4) {
+        // ------------------------------ the line, and TMA ------------------------------
+        const int page = 1 << s.page_shift, box = min(page, PD_TILE), boxes = PD_TILE / box;
+        const Shares line(p, so);
+        if (a.prefix_len == 0)  // pieces that there are not
+            for (int i = blockIdx.x + line.n + line.pieces; i < p.notes; i += gridDim.x)
+                if (lane == 0) p.split[i].rows = 0;
+        int issued = 0, slot = 0;
+        unsigned ph = 0, segs = 0;
+        bool ok = true;
+        auto put = [&](const PdSeg& o) {
+            ok = pd_wait(&c.abort, &c.seg_empty[segs & 1], ((segs >> 1) & 1u) ^ 1u, p.polls);
+            if (!ok) return;
+            if (lane == 0) {
+                c.seg[segs & 1] = o;
+                mbar_arrive(&c.seg_full[segs & 1]);
+            }
+            __syncwarp();
+            segs++;
+        };
+        auto load = [&](const CUtensorMap* map, int kh, int x, int id) {  // a tile from position x on; this lane's page
+            ok = pd_wait(&c.abort, &c.empty[slot], ph ^ 1u, p.polls);
+            if (!ok) return;
+            if (lane == 0) mbar_expect_tx(&c.full[slot], PD_BYTES);
+            __syncwarp();
+            if (lane < boxes)
+                tma_load_4d(ring + slot * PD_BYTES + lane * box * D, map, 0, (x + lane * box) & (page - 1), kh, id, &c.full[slot]);
+            issued++;
+            if (++slot == PD_STAGES) slot = 0, ph ^= 1;
+        };
+        int worker = blockIdx.x;
+#pragma unroll 1
+        while (worker < line.n + line.pieces && ok) {
+            unsigned next = 0;  // the piece after this one
+            if (line.pieces > 0 && lane == 0) next = atomicAdd(p.claimed, 1u);
+            if (a.prefix_len == 0 && lane == 0) p.split[worker].rows = 0;
+            __syncwarp();
+#pragma unroll 1
+            for (int part = 0; part < 2 && ok; part++) {
+                const bool own = part;
+                int step, hi;
+                line.range(worker, own, step, hi);
+                if (step >= hi) continue;
+                // the item of the first step: sequence, kv head, tile
+                int b = 0, kh, rb = 0, tile, n_rb = p.n_rb, nt = p.np;
+                SeqInfo si{0, s.rows, 0};
+                if (!own) {
+                    const int item = step / p.np;
+                    tile = step - item * p.np;
+                    kh = item / n_rb;
+                    rb = item - kh * n_rb;
+                } else {
+                    int e0 = 0, e1 = n_entries;  // the last entry with scan <= step
+#pragma unroll 1
+                    while (e1 - e0 > 1) {
+                        const int mid = (e0 + e1) >> 1;
+                        if (c.scan[mid] <= step) e0 = mid;
+                        else e1 = mid;
+                    }
+                    int rest = step - c.scan[e0], per = 1;
+                    // a lane looks at a sequence of the entry
+#pragma unroll 1
+                    for (b = e0 * per_entry; b < s.n_seqs; b += 32) {
+                        int n = 0;
+                        if (b + lane < s.n_seqs) {
+                            si = seq_info(a, s, b + lane, false);
+                            n = os.per_head(si);
+                        }
+                        int upto = n * a.n_kv;
+#pragma unroll
+                        for (int d = 1; d < 32; d <<= 1) {
+                            const int u = __shfl_up_sync(0xffffffffu, upto, d);
+                            if (lane >= d) upto += u;
+                        }
+                        const unsigned past = __ballot_sync(0xffffffffu, upto > rest);
+                        if (past) {
+                            const int at = __ffs(past) - 1;
+                            rest -= __shfl_sync(0xffffffffu, upto - n * a.n_kv, at);
+                            per = __shfl_sync(0xffffffffu, n, at);
+                            si.q0 = __shfl_sync(0xffffffffu, si.q0, at);
+                            si.q = __shfl_sync(0xffffffffu, si.q, at);
+                            si.kv = __shfl_sync(0xffffffffu, si.kv, at);
+                            b += at;
+                            break;
+                        }
+                        rest -= __shfl_sync(0xffffffffu, upto, 31);
+                    }
+                    if (b >= s.n_seqs) break;  // lengths that changed under the kernel
+                    kh = rest / per;
+                    rest -= kh * per;
+                    n_rb = os.blocks(si);
+#pragma unroll 1
+                    for (; rb < n_rb; rb++) {
+                        const int n = os.tiles(si, rb);
+                        if (rest < n) break;
+                        rest -= n;
+                    }
+                    tile = rest;
+                }
+#pragma unroll 1
+                while (step < hi && ok) {
+                    // ---- a segment: tiles [tile, end) of one item ----
+                    int kv_end = a.prefix_len;
+                    if (own) {
+                        kv_end = os.visible(si, rb);
+                        nt = (kv_end + PD_TILE - 1) / PD_TILE;
+                    }
+                    const int end = min(nt, tile + hi - step);
+                    if (end <= tile) break;  // lengths that changed under the kernel
+                    const int row0 = (own ? si.q0 * a.group : 0) + rb * p.pb;
+                    // (a block of padding: its first row, for nothing)
+                    const int n = max(1, min(p.pb, (own ? si.q : live_rows(s)) * a.group - rb * p.pb));
+                    const int item = (own ? a.n_kv * os.base(si, b) : 0) + kh * n_rb + rb;
+                    const bool begins = tile == 0, whole = a.prefix_len == 0 && begins && end == nt;
+                    if (lane == 0) {
+                        if (tile == 0) p.first[part][item] = worker;
+                        if (end == nt) p.last[part][item] = worker;
+                        if (a.prefix_len == 0 && tile == 0 && end < nt) p.split[worker] = SplitItem{n, row0, kh, item};
+                    }
+                    PdSeg sg;
+                    sg.t0 = tile, sg.t1 = end, sg.n = n, sg.flags = (own ? PD_OWN : 0) | (whole ? PD_WHOLE : 0);
+                    sg.kh = kh, sg.b = b, sg.kv_end = kv_end, sg.row0 = row0, sg.voff = own ? si.kv - si.q + 1 - si.q0 : 0;
+                    sg.slot = own ? p.own_slot(item, worker, begins) : item + worker;
+                    sg.pad[0] = sg.pad[1] = 0;
+                    const int32_t* const table = own ? s.table + (int64_t)b * s.table_ld : a.prefix_table;
+                    auto page_at = [&](int t) {  // this lane's page of tile t; none: zeros
+                        const int x = t * PD_TILE + lane * box;
+                        int id = s.n_pages;
+                        if (lane < boxes && t < end && x < kv_end) {
+                            id = table[x >> s.page_shift];
+                            if ((unsigned)id >= (unsigned)s.n_pages) {
+                                flag_error(a.err, ERR_PAGE_ID, id);
+                                id = s.n_pages;
+                            }
+                        }
+                        return id;
+                    };
+                    int id = page_at(tile), id_next = page_at(tile + 1);
+                    put(sg);
+                    // K of the next tile before V of this one, as the MMA warp takes them
+                    if (ok) load(&map_k, kh, tile * PD_TILE, id);
+#pragma unroll 1
+                    for (int t = tile; t < end && ok; t++) {
+                        const int id_then = page_at(t + 2);
+                        if (t + 1 < end) load(&map_k, kh, (t + 1) * PD_TILE, id_next);
+                        if (ok) load(&map_v, kh, t * PD_TILE, id);
+                        id = id_next;
+                        id_next = id_then;
+                    }
+                    // ---- the next item with a step ----
+                    step += end - tile;
+                    tile = 0;
+                    while (step < hi) {
+                        if (++rb >= n_rb) {
+                            rb = 0;
+                            kh++;
+                            if (own && kh == a.n_kv) {
+                                kh = 0;
+                                if (++b >= s.n_seqs) {  // lengths that changed under the kernel
+                                    hi = step;
+                                    break;
+                                }
+                                si = seq_info(a, s, b, false);
+                                n_rb = os.blocks(si);
+                                if (n_rb == 0 || si.kv == 0) {  // nothing of this sequence
+                                    kh = a.n_kv - 1;
+                                    rb = n_rb;
+                                    continue;
+                                }
+                            }
+                        }
+                        if (!own || os.tiles(si, rb) > 0) break;
+                    }
+                }
+            }
+            worker = line.pieces > 0 ? line.n + (int)min(__shfl_sync(0xffffffffu, next, 0), (unsigned)line.pieces) : line.n;
+        }
+        PdSeg last;
+        last.t0 = last.t1 = last.n = last.kh = last.b = last.kv_end = last.row0 = last.voff = last.slot = 0;
+        last.pad[0] = last.pad[1] = 0;
+        last.flags = PD_END;
+        if (ok) put(last);
+        if (lane == 0) c.issued = issued;
+    } else {
+        // ------------------------------ MMA issuer ------------------------------
+        constexpr uint32_t id_qk = pd_idesc(N, 0), id_pv = pd_idesc(N, 1);
+        int n_tile = 0, slot = 0;
+        unsigned ph = 0, q_ph = 0;
+        bool ok = true;
+        PdSeg sg;
+        const uint64_t q = tc_desc(smem_addr(q_sm), 16);
+        auto take = [&]() {  // the next stage of the ring
+            ok = pd_wait(&c.abort, &c.full[slot], ph, p.polls);
+            const int at = slot;
+            if (++slot == PD_STAGES) slot = 0, ph ^= 1;
+            return at;
+        };
+        auto scores = [&](int k) {  // of tile k
+            const int at = take();
+            if (!ok) return;
+            tc_after();
+            const uint64_t kt = tc_desc(smem_addr(ring + at * PD_BYTES), 16);
+            if (elect_one()) {
+#pragma unroll
+                for (int j = 0; j < 4; j++) mma_i8(tmem + (k & 1) * N, kt + 2 * j, q + 2 * j, id_qk, j > 0);
+                tc_commit(&c.empty[at]);
+                tc_commit(&c.s_full[k & 1]);
+            }
+            __syncwarp();
+        };
+#pragma unroll 1
+        while (ok && fetch(sg)) {
+            ok = pd_wait(&c.abort, &c.q_full, q_ph, p.polls);
+            if (!ok) break;
+            q_ph ^= 1;
+            scores(n_tile);
+#pragma unroll 1
+            for (int t = sg.t0; t < sg.t1 && ok; t++, n_tile++) {
+                if (t + 1 < sg.t1) scores(n_tile + 1);
+                if (!ok) break;
+                const int at = take();
+                if (!ok) break;
+                ok = pd_wait(&c.abort, &c.p_full[n_tile & 1], (n_tile >> 1) & 1u, p.polls);
+                if (!ok) break;
+                tc_after();
+                const uint64_t v = tc_desc(smem_addr(ring + at * PD_BYTES), PD_BYTES);
+                const uint64_t pt = tc_desc(smem_addr(p_sm + (n_tile & 1) * OPERAND), 16);
+                if (elect_one()) {
+#pragma unroll
+                    for (int j = 0; j < 4; j++) mma_i8(tmem + 2 * N + (n_tile & 1) * N, v + j * (4096 >> 4), pt + 2 * j, id_pv, j > 0);
+                    tc_commit(&c.empty[at]);
+                    tc_commit(&c.o_full[n_tile & 1]);
+                }
+                __syncwarp();
+            }
+        }
+        if (elect_one()) tc_commit(&c.done);  // (by the thread that issued the MMAs)
+        __syncwarp();
+        if (!mbar_wait_ns(&c.done, 0, 2000000000ull)) c.abort = 1;
+    }
+    tc_before();
+    __syncthreads();
+    tc_after();
+    if (a.prefix_len == 0) {  // rows before their sequence's first position see nothing
+#pragma unroll 1
+        for (int b = blockIdx.x * (PD_THREADS / 32) + warp; b < s.n_seqs; b += gridDim.x * (PD_THREADS / 32)) {
+            const SeqInfo si = seq_info(a, s, b, false);
+            if (si.kv < si.q) zero_rows<__nv_bfloat16, D>(a, si.q0, si.q - si.kv, lane, 32);
+        }
+    }
+    if (c.abort) {
+        if (tid == 0) flag_error(a.err, ERR_PD_WAIT, blockIdx.x);
+        // no copy may still be landing when the CTA exits
+        if (warp == 4) {
+#pragma unroll 1
+            for (int i = max(0, c.issued - PD_STAGES); i < c.issued; i++)
+                mbar_wait_ns(&c.full[i % PD_STAGES], (unsigned)(i / PD_STAGES) & 1u, 2000000000ull);
+        }
+    }
+    if (warp == 5) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "n"(COLUMNS));
+    if (!alone) pdl_wait();
+}
+
+template <int R>
+static int launch_decode(lq_ctx* ctx, const PdArgs& g) {
+    constexpr int D = 128;
+    const int page = 1 << g.s.page_shift;
+    const uint64_t dims[4] = {(uint64_t)D, (uint64_t)page, (uint64_t)g.c.n_kv, (uint64_t)g.s.n_pages};
+    const uint64_t strides[3] = {(uint64_t)D, (uint64_t)D * page, (uint64_t)g.c.page_stride};
+    const uint32_t box[4] = {D, (uint32_t)std::min(page, PD_TILE), 1, 1};
+    CUtensorMap mk, mv;
+    int rc = make_tensor_map_4d(ctx, &mk, CU_TENSOR_MAP_DATA_TYPE_UINT8, g.c.k, dims, strides, box, CU_TENSOR_MAP_SWIZZLE_128B);
+    if (rc) return rc;
+    rc = make_tensor_map_4d(ctx, &mv, CU_TENSOR_MAP_DATA_TYPE_UINT8, g.c.v, dims, strides, box, CU_TENSOR_MAP_SWIZZLE_128B);
+    if (rc) return rc;
+    const size_t smem = 1024 + PD_STAGES * PD_BYTES + 3 * 2 * R * 128 + sizeof(PdCtl<R>);
+    rc = ensure_func_smem(ctx, (const void*)prefix_attn_q8_decode_kernel<R>, smem);
+    if (rc) return rc;
+    return launch_kernel(ctx, prefix_attn_q8_decode_kernel<R>, dim3((unsigned)g.p.workers), dim3(PD_THREADS), smem,
+                         "prefix_attn_q8_decode", mk, mv, g);
+}
+
+int prefix_attn_q8_decode_ctas(int rows) { return pd_ctas(rows <= 8 ? 8 : 16); }
+
+int launch_prefix_attn_q8_decode(lq_ctx* ctx, const PrefixAttnArgs& a, const PagedSeqs& s, const PagedQ8& c, const PrefixPlan& p) {
+    const PdArgs g{a, s, p, c};
+    return p.pb == 8 ? launch_decode<8>(ctx, g) : launch_decode<16>(ctx, g);
+}
+
+}  // namespace lq

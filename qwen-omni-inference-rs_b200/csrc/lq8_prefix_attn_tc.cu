@@ -37,6 +37,7 @@
 #include "lq8_fused.cuh"
 #include "lq8_prefix_plan.cuh"
 #include "lq8_prefix_attn.cuh"
+#include "lq8_tcgen05.cuh"
 #include "lq8_tma.cuh"
 
 #include <algorithm>
@@ -97,30 +98,6 @@ struct PaCtl {
     int scan[PA_SCAN + 1];  // own steps before each entry
 };
 
-__device__ __forceinline__ void tc_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
-__device__ __forceinline__ void tc_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
-__device__ __forceinline__ void proxy_fence() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
-__device__ __forceinline__ void tc_commit(uint64_t* bar) {
-    asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(smem_addr(bar))
-                 : "memory");
-}
-__device__ __forceinline__ bool elect_one() {
-    uint32_t p;
-    asm volatile("{\n .reg .pred p;\n elect.sync _|p, 0xffffffff;\n selp.u32 %0, 1, 0, p;\n}" : "=r"(p));
-    return p != 0;
-}
-__device__ __forceinline__ float ex2(float x) {
-    float y;
-    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-    return y;
-}
-
-// 128-byte swizzled operand tiles of 128-byte rows, 8-row groups 1024 bytes apart; lead: distance
-// of the 64-element chunks of an MN-major operand
-__device__ __forceinline__ uint64_t pa_desc(uint32_t saddr, uint32_t lead) {
-    return (uint64_t)((saddr >> 4) & 0x3FFF) | (uint64_t)((lead >> 4) & 0x3FFF) << 16 | (uint64_t)(1024 >> 4) << 32 |
-           (uint64_t)1 << 46 | (uint64_t)2 << 61;
-}
 // D f32, A and B bf16, M 128, N n; B MN-major or K-major
 __host__ __device__ constexpr uint32_t pa_idesc(int n, int b_mn) {
     return (1u << 4) | (1u << 7) | (1u << 10) | ((uint32_t)b_mn << 16) | ((uint32_t)(n >> 3) << 17) | (8u << 24);
@@ -137,31 +114,6 @@ __device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint64_t b, uint3
         " tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, {%5, %5, %5, %5}, p;\n}\n" ::"r"(d),
         "r"(a), "l"(b), "r"(idesc), "r"(acc), "r"(0));
 }
-
-#define PA_R8(r, o) "=r"(r[o]), "=r"(r[o + 1]), "=r"(r[o + 2]), "=r"(r[o + 3]), "=r"(r[o + 4]), "=r"(r[o + 5]), "=r"(r[o + 6]), "=r"(r[o + 7])
-#define PA_I8(r, o) "r"(r[o]), "r"(r[o + 1]), "r"(r[o + 2]), "r"(r[o + 3]), "r"(r[o + 4]), "r"(r[o + 5]), "r"(r[o + 6]), "r"(r[o + 7])
-// 32 columns of the warp's 32 TMEM lanes, a lane per thread
-__device__ __forceinline__ void tmem_ld32(uint32_t* r, uint32_t addr) {
-    asm volatile(
-        "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,"
-        "%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];"
-        : PA_R8(r, 0), PA_R8(r, 8), PA_R8(r, 16), PA_R8(r, 24)
-        : "r"(addr));
-}
-__device__ __forceinline__ void tmem_ld16(uint32_t* r, uint32_t addr) {
-    asm volatile(
-        "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
-        : PA_R8(r, 0), PA_R8(r, 8)
-        : "r"(addr));
-}
-__device__ __forceinline__ void tmem_st16(uint32_t addr, const uint32_t* r) {
-    asm volatile(
-        "tcgen05.st.sync.aligned.32x32b.x16.b32 [%16], {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15};" ::PA_I8(r, 0),
-        PA_I8(r, 8), "r"(addr)
-        : "memory");
-}
-__device__ __forceinline__ void tmem_wait_ld() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
-__device__ __forceinline__ void tmem_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 
 constexpr int PA_POLLS = 1 << 22;
 // Bounded wait by a whole warp: PA_POLLS polls (try_wait sleeps between them), or until another warp
@@ -199,17 +151,6 @@ __device__ __forceinline__ void exchange(T& a, T& b) {
     const T t = a;
     a = b;
     b = t;
-}
-
-__device__ __forceinline__ float max3(float a, float b, float c) {  // NaN when one of them is
-    float d;
-    asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
-    return d;
-}
-__device__ __forceinline__ float max_nan(float a, float b) {
-    float d;
-    asm("max.NaN.f32 %0, %1, %2;" : "=f"(d) : "f"(a), "f"(b));
-    return d;
 }
 
 struct PaArgs {
@@ -310,7 +251,7 @@ prefix_attn_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_co
     const bool by_warp = PO && per_entry == 1 && g.a.max_q * g.a.group > 4 * g.p.ob;
     bool fell = false;
 #pragma unroll 1
-    for (int e = by_warp ? warp : tid; e < n_entries; e += by_warp ? PA_THREADS / 32 : PA_THREADS) {
+    for (int e = by_warp ? warp : tid; e < n_entries && !g.p.apart; e += by_warp ? PA_THREADS / 32 : PA_THREADS) {
         int n = 0;
 #pragma unroll 1
         for (int b = e * per_entry; b < min(g.s.n_seqs, (e + 1) * per_entry); b++) {
@@ -337,8 +278,8 @@ prefix_attn_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_co
     __syncthreads();
     tc_after();
     const uint32_t tmem = __shfl_sync(0xffffffffu, c.tmem, 0);
-    const int so = fell ? 0 : c.scan[n_entries];
-    if (blockIdx.x == 0 && tid == 0) *g.p.own_steps = so;  // for the merge
+    const int so = fell || g.p.apart ? 0 : c.scan[n_entries];
+    if (blockIdx.x == 0 && tid == 0 && !g.p.apart) *g.p.own_steps = so;  // for the merge
     const int me = blockIdx.x, polls = g.p.polls;
     // own items count positions from the first tile of the prefix they begin with, whose last tile
     // may be partly empty
@@ -898,7 +839,7 @@ prefix_attn_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_co
                 if (!ok) break;
                 cur.p_ph ^= 1;
                 tc_after();
-                const uint64_t v = pa_desc(smem_addr(ring + v_slot * KV_BYTES), HALF);
+                const uint64_t v = tc_desc(smem_addr(ring + v_slot * KV_BYTES), HALF);
                 if (elect_one()) {
 #pragma unroll
                     for (int j = 0; j < PA_TILE / 16; j++)
@@ -931,8 +872,8 @@ prefix_attn_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_co
                         cur.q_off = q_offset(cur.sg, cur.turn++);
                     }
                     tc_after();
-                    const uint64_t q = pa_desc(smem_addr(sm + f * Q_BYTES) + cur.q_off, 16);
-                    const uint64_t k = pa_desc(smem_addr(ring + k_slot * KV_BYTES), 16);
+                    const uint64_t q = tc_desc(smem_addr(sm + f * Q_BYTES) + cur.q_off, 16);
+                    const uint64_t k = tc_desc(smem_addr(ring + k_slot * KV_BYTES), 16);
                     if (elect_one()) {
 #pragma unroll
                         for (int j = 0; j < D / 16; j++) {

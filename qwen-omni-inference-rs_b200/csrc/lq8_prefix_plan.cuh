@@ -59,8 +59,13 @@ struct PrefixPlan {
     uint64_t workers_mul;       // ceil(2^40 / workers)
     int polls;                  // polls of a wait (f32: for a copy; bf16: for segments) before it gives up
     int hold;                   // fault injection: every CTA stops handing out segments after a few batches
+    int streams;                // parts whose items the streaming kernel takes (1: prefix, 2: own; 8-bit caches)
+    int chunks;                 // pieces of the line that it hands out at its end
+    int apart;                  // own items are another launch's
+    int notes;                  // entries of split
     int cap[2];                 // rows a partial slot holds (prefix, own)
     int32_t* own_steps;         // [1] own steps in all, written by the first CTA
+    unsigned* claimed;          // [1] pieces handed out (behind own_steps; zero between calls)
     int32_t* first[2];          // per item (prefix, own): the first worker of its steps,
     int32_t* last[2];           // and the last
     SplitItem* split;           // per worker, without a prefix: the cut item it begins
@@ -174,6 +179,39 @@ __host__ __device__ __forceinline__ void flow_range(const Line& l, bool paired, 
     }
 }
 
+// The line of the streaming kernel, prefix items first. Workers 0 .. n - 1, its warps, have equal
+// shares of the line up to `from`; the rest is cut into pieces, numbered n, n + 1, ..., that warps take as
+// they come through: SMs differ by a quarter in how fast memory serves them (64 sequences of up to 8000
+// positions: the slowest SM took 196,000 cycles where the mean was 157,000). Which warp takes a piece
+// changes no result. Below 16 steps a warp there is nothing to hand out.
+struct Shares {
+    int n, sp, total, from, piece, pieces, quot, rem;
+    uint64_t mul;
+    __host__ __device__ __forceinline__ Shares(const PrefixPlan& p, int own_steps)
+        : n(p.workers), sp(p.sp), total(p.sp + own_steps), from(total), piece(1), pieces(0), mul(p.workers_mul) {
+        if (p.chunks > 0 && total >= 16 * n) {
+            const int rest = total / 10 * 3;
+            from = total - rest;
+            piece = (rest + p.chunks - 1) / p.chunks;
+            pieces = (rest + piece - 1) / piece;
+        }
+        quot = (int)(((uint64_t)from * mul) >> 40);
+        rem = from - quot * n;
+    }
+    // the first step of worker or piece c <= n + pieces
+    __host__ __device__ __forceinline__ int start(int c) const {
+        if (c > n) return min(total, from + (c - n) * piece);
+        return quot * c + (int)(((uint64_t)(rem * c) * mul) >> 40);
+    }
+    // its steps of the prefix or of the own items
+    __host__ __device__ __forceinline__ void range(int c, bool own, int& lo, int& hi) const {
+        lo = start(c);
+        hi = start(c + 1);
+        if (own) lo = max(lo - sp, 0), hi = max(hi - sp, 0);
+        else lo = min(lo, sp), hi = min(hi, sp);
+    }
+};
+
 // What a flow of a CTA gets next in a part whose flows are apart: a batch of its items (go), or
 // `idle` rounds without work. The warps that serve the flows take a round of each in turn, and a
 // flow's batch is only taken back when they have begun its next one. So a batch goes to the flow
@@ -194,12 +232,16 @@ __host__ __device__ __forceinline__ HandOut hand_out(int f, bool first, bool liv
 // PREFIX_MAX_STEPS before the plan is used
 constexpr int64_t PREFIX_MAX_STEPS = 1ll << 26;
 constexpr int PREFIX_ATTN_F32_WARPS = 8;  // workers of a CTA of the f32 kernel
-inline int64_t plan_cut(const PrefixAttnArgs& a, const PagedSeqs& s, bool f32, int sm_count, PrefixPlan* p, int warp_rows = 8) {
+constexpr int PREFIX_ATTN_Q8_WARPS = 8;  // and of the streaming one for 8-bit caches
+constexpr int PREFIX_ATTN_Q8_ROWS = 16;   // stacked rows of an item that it takes
+inline int64_t plan_cut(const PrefixAttnArgs& a, const PagedSeqs& s, bool f32, int sm_count, PrefixPlan* p, int warp_rows = 8,
+                        int warps = PREFIX_ATTN_F32_WARPS, int warp_tile = 32) {
     const int64_t R = (int64_t)s.rows * a.group, most_q = std::min<int64_t>((int64_t)a.max_q, s.rows) * a.group;
     // bf16: blocks of 128 rows, or two halves of 128 that share their K and V tiles; a worker is a
     // CTA with paired halves, else one of its two flows. f32: blocks of 8 rows (warp_rows), a worker is a
     // warp.
-    const int half = f32 ? warp_rows : 128, tile = f32 ? 32 : 128;
+    const int half = f32 ? warp_rows : 128, tile = f32 ? warp_tile : 128;
+    p->streams = p->chunks = p->apart = 0;
     p->tile = tile;
     p->pair_p = f32 || R > half;
     p->pair_o = f32 || most_q > half;
@@ -226,7 +268,7 @@ inline int64_t plan_cut(const PrefixAttnArgs& a, const PagedSeqs& s, bool f32, i
     // so, short causal items next to a long prefix no longer hold up the last CTAs (a batch of 10
     // prompt chunks: 152 -> 114 us)
     p->extra = f32 ? 0 : 1;
-    p->workers = (int)std::max<int64_t>(1, std::min<int64_t>(sm_count * (f32 ? PREFIX_ATTN_F32_WARPS : 1), steps));
+    p->workers = (int)std::max<int64_t>(1, std::min<int64_t>(sm_count * (f32 ? warps : 1), steps));
     p->workers_mul = ((1ull << 40) + p->workers - 1) / p->workers;
     return steps;
 }

@@ -139,6 +139,22 @@ static int alloc_paged(lq_ctx* ctx, size_t bytes, PagedBuffer* b) {
         return set_error(ctx, LQ_ERR_OOM, "paged attention workspace: %zu bytes", sz);
     }
     LQ_CUDA(ctx, e);
+    // Its first 256 bytes begin at zero: a counter there is zero between calls. On a stream of its own, so
+    // that it belongs to no capture.
+    cudaStream_t st = nullptr;
+    mode = cudaStreamCaptureModeRelaxed;
+    cudaThreadExchangeStreamCaptureMode(&mode);
+    cudaError_t z = cudaStreamCreateWithFlags(&st, cudaStreamNonBlocking);
+    if (z == cudaSuccess) {
+        z = cudaMemsetAsync(p, 0, 256, st);
+        if (z == cudaSuccess) z = cudaStreamSynchronize(st);
+        cudaStreamDestroy(st);
+    }
+    cudaThreadExchangeStreamCaptureMode(&mode);
+    if (z != cudaSuccess) {
+        cudaFree(p);
+        return check_cuda(ctx, z, "paged attention workspace");
+    }
     b->p = p;
     b->bytes = sz;
     return LQ_OK;

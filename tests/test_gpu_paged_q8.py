@@ -8,10 +8,15 @@ Tolerances, with u = 2^-8 the unit roundoff of a bf16 output (0 for f32):
   a code is within 0.5 + 0.001 (and 2^-10 for the f32 product by the scale's reciprocal) of the exact
   quotient, the scale within 2^-17 of its own size; given the f32 values, codes and scales are exact;
 - codes rounded again, and rows read back: exact, in f32;
-- attention, streaming kernel (up to 16 stacked rows): q is rounded to amax / 65024 at most, which
-  moves a score by at most d = c amax / 65024 sum |k| and a weight by a factor within e^(+-2d); a
-  weight is two bf16 numbers, 2^-16; f32 sums and exponentials stay within 2e-5 sum p |v| (the
-  framework's tolerance for its f32 attention), the result is rounded once, u |o|;
+- attention with up to 16 stacked rows a kv head: q is rounded to amax / 65024 at most, which moves a
+  score by at most d = c amax / 65024 sum |k| and a weight by a factor within e^(+-2d); f32 sums and
+  exponentials stay within 2e-5 sum p |v| (the framework's tolerance for its f32 attention), the result
+  is rounded once, u |o|. Weights p, times V's scale s, are rounded too:
+  - head_dim 128: to whole 1 / 32512 parts of the largest p s of their 128 positions (the tiles begin at the
+    prefix's and at the own positions' first), half of that at most: codes are up to 127, so that a tile
+    gives at most 128 127 max(p s) / 65024; w is the sum of 128 127 max(p s) over the tiles;
+  - head_dim 64: to fp16, 2^-11, with the largest p s at 2^7 at least, so that half the smallest step,
+    2^-25, is 2^-32 of it: over n positions n 127 2^-32 max(p s), at most 2^-26 w for n up to 2^13;
 - attention, tensor-core kernel: q is exact, a weight is rounded to bf16 once, u sum p |v|; the rest as
   above;
 - both: a weight below 2^-126 of the largest is zero in f32 (and flushed). Over up to 2^13 positions of
@@ -378,8 +383,8 @@ def test_read_reports_rows_without_a_slot(ctx, lq8_lib):
 # ------------------------------------------------------------------------------------------
 
 def attention64(s, q, scale, dead=()):
-    """(o, sum p |v|, d) of every row in f64, d the bound on what rounding q does to a score; rows that
-    see nothing give zeros."""
+    """(o, sum p |v|, d, w) of every row in f64, d and w as in the tolerances; rows that see nothing give
+    zeros."""
     import torch
     Hkv, D = s.n_kv, s.D
     rows, Hq = q.shape[0], q.shape[1]
@@ -387,6 +392,7 @@ def attention64(s, q, scale, dead=()):
     o = torch.zeros(rows, Hq, D, dtype=torch.float64, device="cuda")
     a = torch.zeros_like(o)
     d = torch.zeros(rows, Hq, 1, dtype=torch.float64, device="cuda")
+    w1 = torch.zeros_like(d)
     pk, pv = s.read("k"), s.read("v")
     for b in range(len(s.q)):
         r0, n = int(s.start[b]), int(s.q[b])
@@ -405,13 +411,23 @@ def attention64(s, q, scale, dead=()):
         for dst, w in ((o, v), (a, v.abs())):
             dst[r0:r0 + n] = torch.einsum("hgnt,htd->hgnd", p, w).permute(2, 0, 1, 3).reshape(n, Hq, D)
         d[r0:r0 + n, :, 0] = bound.permute(2, 0, 1).reshape(n, Hq)
-    return o, a, d
+        for which, p1 in ((None, p[..., :s.prefix]), (b, p[..., s.prefix:])):
+            pg, off = (i32(u).long() for u in s.slots(which))
+            if len(pg):
+                ps = p1 * s.vs[pg, :, off // s.block].double().T[:, None, None]
+                ps = torch.nn.functional.pad(ps, (0, -ps.shape[-1] % 128)).unflatten(-1, (-1, 128)).amax(-1).sum(-1)
+                w1[r0:r0 + n, :, 0] += 128 * 127 * ps.permute(2, 0, 1).reshape(n, Hq)
+    return o, a, d, w1
 
 
 def tolerance(want, streaming=True):
     import torch
-    o, a, d = want
-    return 2.0 ** -110 + U * o.abs() + ((torch.expm1(2 * d) + 2.0 ** -16 if streaming else U) + 2e-5) * a
+    o, a, d, w = want
+    if not streaming:
+        return 2.0 ** -110 + U * o.abs() + (U + 2e-5) * a
+    if o.shape[-1] == 128:
+        return 2.0 ** -110 + w / 65024 + U * o.abs() + (torch.expm1(2 * d) + 2e-5) * a
+    return 2.0 ** -110 + 2.0 ** -26 * w + U * o.abs() + (torch.expm1(2 * d) + 2.0 ** -11 + 2e-5) * a
 
 
 def attention_case(ctx, lq8_lib, kv, q, Hq, Hkv, D, page, block, prefix, seed=11, layers=1, qscale=1.0, quantized=False):
