@@ -57,13 +57,7 @@ prefix_attn_merge_kernel(const __grid_constant__ PrefixAttnArgs a, const __grid_
         }
         const SeqInfo si = seq_info(a, s, lo, false);
         const int rb = x - os.base(si, lo), nb = os.blocks(si);
-        if (rb < 0 || rb >= nb) {
-            if (p.chunks > 0 && blockIdx.x == 0 && blockIdx.y == 0) {
-                pdl_wait();
-                if (tid == 0) *p.claimed = 0;
-            }
-            return;
-        }
+        if (rb < 0 || rb >= nb) return;
         st0 = si.q0 * a.group + rb * p.ob + own_in;
         todo = min(MR, min(p.ob, si.q * a.group - rb * p.ob) - own_in);
         own_item = a.n_kv * x + kh * nb + rb - a.n_kv * rb;  // n_kv base + kh nb + rb
@@ -71,7 +65,6 @@ prefix_attn_merge_kernel(const __grid_constant__ PrefixAttnArgs a, const __grid_
     }
     pdl_wait();
     pdl_trigger();
-    if (p.chunks > 0 && blockIdx.x == 0 && blockIdx.y == 0 && tid == 0) *p.claimed = 0;  // for the next call
     const int own_steps = *p.own_steps;
     const Line line(pp, pp.streams == p.streams ? own_steps : 0, pp.pair_p, pp.pair_o);
     const Shares shares(p, p.streams ? own_steps : 0);
@@ -106,7 +99,7 @@ prefix_attn_merge_kernel(const __grid_constant__ PrefixAttnArgs a, const __grid_
     }
         int run = todo, item[2] = {0, own_item}, in[2] = {0, own_in}, v0[2] = {0, 0}, cnt[2] = {0, 0};
         auto workers_of = [&](int k) {  // (within bounds, even where a kernel that gave up left them unwritten)
-            const int most = (k ? p : pp).streams ? p.workers + p.chunks - 1 : 2 * pp.workers - 1;
+            const int most = (k ? p : pp).ranges - 1;
             v0[k] = min(max(p.first[k][item[k]], 0), most);
             cnt[k] = min(max(p.last[k][item[k]], 0), most) - v0[k] + 1;
         };
@@ -259,16 +252,16 @@ static int make_workspace(lq_ctx* ctx, const char* who, const PrefixAttnArgs& a,
     const int64_t items_p = (int64_t)a.n_kv * pp->n_rb;
     const int64_t items_o = a.n_kv * ((int64_t)s.rows * a.group / p->ob + s.n_seqs + 1);
     const int64_t items[2] = {pp->np ? items_p : 0, items_o};
-    // workers, or flows of a CTA, that may have a piece
-    const int64_t most[2] = {pp->streams ? pp->workers + pp->chunks : 2ll * pp->workers,
-                             p->streams ? p->workers + p->chunks : 2ll * p->workers};
+    // workers, ranges, or flows of a CTA that may have a piece
+    for (PrefixPlan* x : {p, pp}) x->ranges = (x->chunks ? 5 : x->streams ? 1 : 2) * x->workers;
+    const int64_t most[2] = {pp->ranges, p->ranges};
     size_t at = 0;
     auto place = [&at](int64_t n, size_t size) {
         const size_t here = at;
         at += ((size_t)n * size + 255) & ~(size_t)255;
         return here;
     };
-    p->notes = (int)(p->streams ? most[1] : (p->pair_o ? 1 : 2) * p->workers);
+    p->notes = p->streams ? p->ranges : (p->pair_o ? 1 : 2) * p->workers;
     const size_t steps_at = place(1, 4), split_at = place(most[1], sizeof(SplitItem));
     size_t first_at[2], last_at[2], ml_at[2], o_at[2];
     for (int k = 0; k < 2; k++) {
@@ -318,6 +311,9 @@ static int launch_merge(lq_ctx* ctx, const PrefixAttnArgs& a, const PagedSeqs& s
     const int64_t R = (int64_t)s.rows * a.group;
     const dim3 grid((unsigned)(p.np > 0 ? a.n_kv * (R / p.ob + s.n_seqs) : p.streams ? std::min(p.notes, 8 * ctx->sm_count) : p.notes),
                     (unsigned)ceil_div(p.cap[1], mr));
+    const void* const func = mr == 8 ? (const void*)prefix_attn_merge_kernel<T, D, 8> : (const void*)prefix_attn_merge_kernel<T, D, 32>;
+    const int rc = ensure_func_carveout(ctx, func);
+    if (rc) return rc;
     return mr == 8 ? launch_kernel(ctx, prefix_attn_merge_kernel<T, D, 8>, grid, dim3(256), 0, "prefix_attn_merge", a, s, p, pp)
                    : launch_kernel(ctx, prefix_attn_merge_kernel<T, D, 32>, grid, dim3(256), 0, "prefix_attn_merge", a, s, p, pp);
 }
@@ -341,13 +337,16 @@ static int attend_q8(lq_ctx* ctx, const PrefixAttnArgs& a, const PagedSeqs& s, c
         else steps_st = plan_cut(a, s, true, ctx->sm_count, &st, rows, PREFIX_ATTN_Q8_WARPS);
         set_polls(&st, true);
         st.streams = stream_prefix ? 3 : 2;
-        if (D == 128) st.chunks = 2 * st.workers;
+        st.chunks = D == 128;
     }
     LQ_REQUIRE(ctx, steps_tc < PREFIX_MAX_STEPS && steps_st < PREFIX_MAX_STEPS, "%s: %lld steps, more than a launch can number", who,
                (long long)std::max(steps_tc, steps_st));
     PrefixPlan* const own = stream_own ? &st : &tc;
     PrefixPlan* const pre = stream_prefix ? &st : &tc;
     if (own != pre) {  // the prefix for itself, and the own items for themselves
+        // (All SMs for the prefix, then for the own items. With the SMs divided between them, by how long
+        // either takes, 128 sequences behind 32768 positions took 295 us instead of 216, 64 behind 8191 64
+        // instead of 60: an SM with few neighbours at work reads no faster.)
         tc.workers = std::max(1, std::min(ctx->sm_count, tc.sp));
         tc.workers_mul = ((1ull << 40) + tc.workers - 1) / tc.workers;
         tc.apart = 1;

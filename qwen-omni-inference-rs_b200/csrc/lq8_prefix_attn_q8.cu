@@ -202,11 +202,11 @@ prefix_attn_q8_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_co
             if (si.kv < si.q) zero_rows<__nv_bfloat16, D>(a, si.q0, si.q - si.kv, lane, 32);
         }
     }
-    int worker = warp * gridDim.x + blockIdx.x;
+    const int worker = warp * gridDim.x + blockIdx.x;
     const int live = live_rows(s);
     const Shares line(p, so);
-    if (a.prefix_len == 0)  // pieces that there are not
-        for (int i = worker + line.n + line.pieces; i < p.notes; i += PQ_WARPS * gridDim.x)
+    if (a.prefix_len == 0)  // ranges that there are not
+        for (int i = worker + line.ranges; i < p.notes; i += PQ_WARPS * gridDim.x)
             if (lane == 0) p.split[i].rows = 0;
     const int box = min(1 << s.page_shift, PQ_STAGE), boxes = PQ_STAGE / box, mask = (1 << s.page_shift) - 1;
     // column n of a tile of Q K^T is position perm(n) of its 8: with D = 64, where two positions share the
@@ -216,11 +216,10 @@ prefix_attn_q8_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_co
     // where in a stage vector `ch` (16 bytes) of position x lies
     auto vec = [](int x, int ch) { return D == 128 ? x * 128 + ((ch ^ (x & 7)) << 4) : x * 64 + ((ch ^ ((x >> 1) & 3)) << 4); };
 
-    if (worker >= p.workers) worker = line.n + line.pieces;
-#pragma unroll 1
-    while (worker < line.n + line.pieces && ok) {
-    unsigned next = 0;  // the piece after this one
-    if (line.pieces > 0 && lane == 0) next = atomicAdd(p.claimed, 1u);
+    if (worker >= line.ranges) {
+        if (!alone) pdl_wait();
+        return;
+    }
     if (a.prefix_len == 0 && lane == 0) p.split[worker].rows = 0;
     __syncwarp();
 #pragma unroll 1
@@ -592,8 +591,6 @@ prefix_attn_q8_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_co
                 if (!own || os.tiles(si, rb) > 0) break;
             }
         }
-    }
-    worker = line.pieces > 0 ? line.n + (int)min(__shfl_sync(0xffffffffu, next, 0), (unsigned)line.pieces) : line.n;
     }
     if (!alone) pdl_wait();
 }

@@ -181,6 +181,8 @@ prefix_attn_q8_decode_kernel(const __grid_constant__ CUtensorMap map_k, const __
     const bool alone = p.streams == 3;
     if (alone) pdl_wait();
     pdl_trigger();  // (after the wait: the merge reads the call's lengths before its own)
+    unsigned claim = 0;  // the first range
+    if (warp == 4 && lane == 0) claim = atomicAdd(p.claimed, 1u);
     // own steps of every entry (a run of per_entry sequences), then their running sum
     const int per_entry = (s.n_seqs + PD_SCAN - 1) / PD_SCAN;
     const int n_entries = (s.n_seqs + per_entry - 1) / per_entry;
@@ -250,6 +252,24 @@ prefix_attn_q8_decode_kernel(const __grid_constant__ CUtensorMap map_k, const __
         };
         PdSeg sg;
         bool ok = true;
+        float m[R], l[R], o[R];
+        auto finish = [&]() {    // rows of sg
+#pragma unroll
+            for (int r = 0; r < R; r++)
+                if (r < sg.n) {
+                    const float y = l[r] == 0.0f ? 0.0f : o[r] * (l[r] > 0.0f ? 1.0f / l[r] : l[r]);
+                    const int st = sg.row0 + r, tok = a.group_div(st);
+                    const int64_t col = (int64_t)(sg.kh * a.group + st - tok * a.group) * D + tid;
+                    if (a.out) static_cast<__nv_bfloat16*>(a.out)[(int64_t)tok * a.out_stride + col] = __float2bfloat16_rn(y);
+                    if (a.xq) {  // a warp has a block of 32 dims
+                        float d, id;
+                        q8_scale(warp_max(fabsf(y)), d, id);
+                        const int64_t at = (int64_t)tok * a.n_heads * D + col;
+                        if (lane == 0) a.xd[at / 32] = f2h(d);
+                        a.xq[at] = (int8_t)q8_quant(y, id);
+                    }
+                }
+        };
 #pragma unroll 1
         while (ok && fetch(sg)) {
             // ---- this position's scales: pages two tiles ahead, scales one ----
@@ -324,7 +344,7 @@ prefix_attn_q8_decode_kernel(const __grid_constant__ CUtensorMap map_k, const __
                 return sg.flags & PD_OWN ? min(sg.kv_end, max(0, a.group_div(sg.row0 + min(r, sg.n - 1)) + sg.voff)) : sg.kv_end;
             };
             const int all_see = seen_by(0);  // (the first row's token comes first)
-            float m[R], l[R], o[R], w[R];    // w: what the last tile's O counts for
+            float w[R];                      // what the last tile's O counts for
 #pragma unroll
             for (int r = 0; r < R; r++) m[r] = -INFINITY, l[r] = o[r] = w[r] = 0.0f;
             // O of the tile before
@@ -430,28 +450,14 @@ prefix_attn_q8_decode_kernel(const __grid_constant__ CUtensorMap map_k, const __
             }
             const bool own = sg.flags & PD_OWN;
             const int cap = p.cap[own];
-            if (!(sg.flags & PD_WHOLE)) {
+            if (sg.flags & PD_WHOLE) {
+                finish();
+            } else {
 #pragma unroll
                 for (int r = 0; r < R; r++)
                     if (r < sg.n) {
                         if (tid == r) p.ml[own][(int64_t)sg.slot * cap + r] = make_float2(m[r], l[r]);
                         p.o[own][(((int64_t)sg.slot * (D / 4) + (tid >> 2)) * cap + r) * 4 + (tid & 3)] = o[r];
-                    }
-            } else {
-#pragma unroll
-                for (int r = 0; r < R; r++)
-                    if (r < sg.n) {
-                        const float y = l[r] == 0.0f ? 0.0f : o[r] * (l[r] > 0.0f ? 1.0f / l[r] : l[r]);
-                        const int st = sg.row0 + r, tok = a.group_div(st);
-                        const int64_t col = (int64_t)(sg.kh * a.group + st - tok * a.group) * D + tid;
-                        if (a.out) static_cast<__nv_bfloat16*>(a.out)[(int64_t)tok * a.out_stride + col] = __float2bfloat16_rn(y);
-                        if (a.xq) {  // a warp has a block of 32 dims
-                            float d, id;
-                            q8_scale(warp_max(fabsf(y)), d, id);
-                            const int64_t at = (int64_t)tok * a.n_heads * D + col;
-                            if (lane == 0) a.xd[at / 32] = f2h(d);
-                            a.xq[at] = (int8_t)q8_quant(y, id);
-                        }
                     }
             }
         }
@@ -459,8 +465,8 @@ prefix_attn_q8_decode_kernel(const __grid_constant__ CUtensorMap map_k, const __
         // ------------------------------ the line, and TMA ------------------------------
         const int page = 1 << s.page_shift, box = min(page, PD_TILE), boxes = PD_TILE / box;
         const Shares line(p, so);
-        if (a.prefix_len == 0)  // pieces that there are not
-            for (int i = blockIdx.x + line.n + line.pieces; i < p.notes; i += gridDim.x)
+        if (a.prefix_len == 0)  // ranges that there are not
+            for (int i = blockIdx.x + line.ranges; i < p.notes; i += gridDim.x)
                 if (lane == 0) p.split[i].rows = 0;
         int issued = 0, slot = 0;
         unsigned ph = 0, segs = 0;
@@ -485,11 +491,9 @@ prefix_attn_q8_decode_kernel(const __grid_constant__ CUtensorMap map_k, const __
             issued++;
             if (++slot == PD_STAGES) slot = 0, ph ^= 1;
         };
-        int worker = blockIdx.x;
+        int worker = (int)min(__shfl_sync(0xffffffffu, claim, 0), (unsigned)line.ranges);
 #pragma unroll 1
-        while (worker < line.n + line.pieces && ok) {
-            unsigned next = 0;  // the piece after this one
-            if (line.pieces > 0 && lane == 0) next = atomicAdd(p.claimed, 1u);
+        while (worker < line.ranges && ok) {
             if (a.prefix_len == 0 && lane == 0) p.split[worker].rows = 0;
             __syncwarp();
 #pragma unroll 1
@@ -630,7 +634,9 @@ prefix_attn_q8_decode_kernel(const __grid_constant__ CUtensorMap map_k, const __
                     }
                 }
             }
-            worker = line.pieces > 0 ? line.n + (int)min(__shfl_sync(0xffffffffu, next, 0), (unsigned)line.pieces) : line.n;
+            // (asked for when all of this is on its way, two tiles before it is done with)
+            if (lane == 0) claim = atomicAdd(p.claimed, 1u);
+            worker = (int)min(__shfl_sync(0xffffffffu, claim, 0), (unsigned)line.ranges);
         }
         PdSeg last;
         last.t0 = last.t1 = last.n = last.kh = last.b = last.kv_end = last.row0 = last.voff = last.slot = 0;
@@ -715,6 +721,10 @@ prefix_attn_q8_decode_kernel(const __grid_constant__ CUtensorMap map_k, const __
         }
     }
     if (warp == 5) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "n"(COLUMNS));
+    if (tid == 0) {  // the last CTA leaves the counters at zero
+        __threadfence();
+        if (atomicAdd(p.claimed + 1, 1u) == gridDim.x - 1) p.claimed[0] = p.claimed[1] = 0;
+    }
     if (!alone) pdl_wait();
 }
 

@@ -60,12 +60,13 @@ struct PrefixPlan {
     int polls;                  // polls of a wait (f32: for a copy; bf16: for segments) before it gives up
     int hold;                   // fault injection: every CTA stops handing out segments after a few batches
     int streams;                // parts whose items the streaming kernel takes (1: prefix, 2: own; 8-bit caches)
-    int chunks;                 // pieces of the line that it hands out at its end
+    int chunks;                 // 1: it may hand out the line in ranges of falling size
     int apart;                  // own items are another launch's
+    int ranges;                 // workers, or ranges of the line, that may have a piece of an item
     int notes;                  // entries of split
     int cap[2];                 // rows a partial slot holds (prefix, own)
     int32_t* own_steps;         // [1] own steps in all, written by the first CTA
-    unsigned* claimed;          // [1] pieces handed out (behind own_steps; zero between calls)
+    unsigned* claimed;          // [2] ranges handed out, CTAs that are through (behind own_steps; zero between calls)
     int32_t* first[2];          // per item (prefix, own): the first worker of its steps,
     int32_t* last[2];           // and the last
     SplitItem* split;           // per worker, without a prefix: the cut item it begins
@@ -179,29 +180,36 @@ __host__ __device__ __forceinline__ void flow_range(const Line& l, bool paired, 
     }
 }
 
-// The line of the streaming kernel, prefix items first. Workers 0 .. n - 1, its warps, have equal
-// shares of the line up to `from`; the rest is cut into pieces, numbered n, n + 1, ..., that warps take as
-// they come through: SMs differ by a quarter in how fast memory serves them (64 sequences of up to 8000
-// positions: the slowest SM took 196,000 cycles where the mean was 157,000). Which warp takes a piece
-// changes no result. Below 16 steps a warp there is nothing to hand out.
+// The line of a streaming kernel, prefix items first, cut into ranges that its workers take in turn: with
+// n workers and 16 steps for each, n ranges with half of the line, n with a quarter, n with three twentieths
+// and 2 n with the rest, else n equal ones. A worker may begin late (an SM that still holds another kernel's shared
+// memory took its third CTA 80 us late, and a fixed share for each ended 25 us after all others), and
+// memory serves some SMs faster than others. Which worker takes a range changes no result.
 struct Shares {
-    int n, sp, total, from, piece, pieces, quot, rem;
-    uint64_t mul;
+    int n, sp, total, ranges;
+    int size[4];   // steps of the four parts
+    uint64_t mul;  // ceil(2^40 / n)
     __host__ __device__ __forceinline__ Shares(const PrefixPlan& p, int own_steps)
-        : n(p.workers), sp(p.sp), total(p.sp + own_steps), from(total), piece(1), pieces(0), mul(p.workers_mul) {
+        : n(p.workers), sp(p.sp), total(p.sp + own_steps), ranges(n), size{total, 0, 0, 0}, mul(p.workers_mul) {
         if (p.chunks > 0 && total >= 16 * n) {
-            const int rest = total / 10 * 3;
-            from = total - rest;
-            piece = (rest + p.chunks - 1) / p.chunks;
-            pieces = (rest + piece - 1) / piece;
+            size[3] = total / 10;
+            size[2] = total / 20 * 3;
+            size[1] = total / 4;
+            size[0] = total - size[1] - size[2] - size[3];
+            ranges = 5 * n;
         }
-        quot = (int)(((uint64_t)from * mul) >> 40);
-        rem = from - quot * n;
     }
-    // the first step of worker or piece c <= n + pieces
-    __host__ __device__ __forceinline__ int start(int c) const {
-        if (c > n) return min(total, from + (c - n) * piece);
+    // floor(w c / n), c <= 2 n
+    __host__ __device__ __forceinline__ int part(int w, int c) const {
+        const int quot = (int)(((uint64_t)w * mul) >> 40), rem = w - quot * n;
         return quot * c + (int)(((uint64_t)(rem * c) * mul) >> 40);
+    }
+    // the first step of range c <= ranges
+    __host__ __device__ __forceinline__ int start(int c) const {
+        if (c <= n) return part(size[0], c);
+        if (c <= 2 * n) return size[0] + part(size[1], c - n);
+        if (c <= 3 * n) return size[0] + size[1] + part(size[2], c - 2 * n);
+        return size[0] + size[1] + size[2] + (part(size[3], c - 3 * n) >> 1);
     }
     // its steps of the prefix or of the own items
     __host__ __device__ __forceinline__ void range(int c, bool own, int& lo, int& hi) const {

@@ -139,8 +139,8 @@ static int alloc_paged(lq_ctx* ctx, size_t bytes, PagedBuffer* b) {
         return set_error(ctx, LQ_ERR_OOM, "paged attention workspace: %zu bytes", sz);
     }
     LQ_CUDA(ctx, e);
-    // Its first 256 bytes begin at zero: a counter there is zero between calls. On a stream of its own, so
-    // that it belongs to no capture.
+    // Counters in its first 256 bytes are zero between calls. On a stream of its own, so that this belongs to no
+    // capture.
     cudaStream_t st = nullptr;
     mode = cudaStreamCaptureModeRelaxed;
     cudaThreadExchangeStreamCaptureMode(&mode);
@@ -225,6 +225,17 @@ int ensure_func_smem(lq_ctx* ctx, const void* func, size_t bytes) {
     if (have >= bytes) return LQ_OK;
     LQ_CUDA(ctx, cudaFuncSetAttribute(func, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)bytes));
     have = bytes;
+    return LQ_OK;
+}
+
+int ensure_func_carveout(lq_ctx* ctx, const void* func) {
+    static std::mutex mu;
+    static std::map<std::pair<const void*, int>, bool> done;
+    std::lock_guard<std::mutex> lock(mu);
+    bool& have = done[std::make_pair(func, ctx->device)];
+    if (have) return LQ_OK;
+    LQ_CUDA(ctx, cudaFuncSetAttribute(func, cudaFuncAttributePreferredSharedMemoryCarveout, cudaSharedmemCarveoutMaxShared));
+    have = true;
     return LQ_OK;
 }
 
