@@ -29,7 +29,6 @@ struct TeamInfo {
     int first;       // the block's first position
     int page, slot;  // its page, its place there
     int ok;
-    float scale;     // as the cache has it
 };
 
 // the last sequence whose blocks begin at or before x (by a warp; base is increasing)
@@ -46,9 +45,8 @@ __device__ __forceinline__ int seq_of_block(const PagedSeqs& s, int shift, int64
     return lo;
 }
 
-__device__ __forceinline__ TeamInfo find_block(const PagedSeqs& s, const PagedQ8& c, const float* scales, int64_t x, int kh,
-                                               int lane, int* err) {
-    TeamInfo t{0, 0, 0, 0, 0, 0, 0, 0, 0.0f};
+__device__ __forceinline__ TeamInfo find_block(const PagedSeqs& s, const PagedQ8& c, int64_t x, int lane, int* err) {
+    TeamInfo t{0, 0, 0, 0, 0, 0, 0, 0};
     const int shift = c.block_shift;
     int b = (int)x, q1 = (int)x + 1;
     int64_t j = 0;  // the block's place among those that the sequence's rows touch
@@ -87,7 +85,6 @@ __device__ __forceinline__ TeamInfo find_block(const PagedSeqs& s, const PagedQ8
         return t;
     }
     t.slot = (t.first & ((1 << s.page_shift) - 1)) >> shift;
-    t.scale = scales[t.page * c.scale_stride + ((int64_t)kh << (s.page_shift - shift)) + t.slot];
     t.ok = 1;
     return t;
 }
@@ -110,11 +107,69 @@ __device__ __forceinline__ uint32_t codes_again(uint32_t w, float by) {
     return pack_codes(u[0], u[1], u[2], u[3]);
 }
 
-// WIDE: heads that rotate whole, rows and weights aligned to 16 bytes
-template <typename S, int D, bool WIDE>
-__global__ void __launch_bounds__(256, 2) paged_append_q8_kernel(AppendArgs a, RopeAxes rope, PagedSeqs seqs, PagedQ8 c,
-                                                                 int kv_ctas, int groups) {
-    constexpr int LPH = D / 16, HPW = 32 / LPH, IT = 16 / HPW, N = D / 2;  // lanes a position, positions side by side
+// Query heads of a row: IT times 32 / (D / 16) of them a warp, as append_heads; where positions are given
+// nothing is looked up but whether the row is padding
+template <typename S, int D, int IT>
+__device__ __forceinline__ void append_query(const AppendArgs& a, const RopeAxes& rope, const PagedSeqs& seqs, int groups, int64_t item) {
+    constexpr int LPH = D / 16, HPW = 32 / LPH, N = D / 2;
+    const int lane = threadIdx.x & 31;
+    const int row = (int)(item / groups);
+    const int d0 = 8 * (lane % LPH), mine = (int)(item - (int64_t)row * groups) * (HPW * IT) + lane / LPH;
+    if (row >= seqs.rows) return;
+    const S* src = static_cast<const S*>(a.qkv) + (int64_t)row * a.row_stride + (int64_t)mine * D + d0;
+    Vec<S, 16 / sizeof(S)> raw[IT][2][sizeof(S) / 2];
+#pragma unroll
+    for (int j = 0; j < IT; j++)
+        if (mine + j * HPW < a.n_heads) {
+#pragma unroll
+            for (int k = 0; k < (int)sizeof(S) / 2; k++) {
+                raw[j][0][k] = *reinterpret_cast<const Vec<S, 16 / sizeof(S)>*>(src + j * HPW * D + k * (16 / sizeof(S)));
+                raw[j][1][k] = *reinterpret_cast<const Vec<S, 16 / sizeof(S)>*>(src + j * HPW * D + N + k * (16 / sizeof(S)));
+            }
+        }
+    float cs[8], sn[8];
+    bool turn = true;
+    if (rope.pos) {
+        turn = angles<8>(rope, row, 0, d0, cs, sn, nullptr);
+        if (row >= (seqs.q_start ? seqs.q_start[seqs.n_seqs] : seqs.n_seqs)) return;  // (padding, whatever its position)
+        if (!turn) flag_positions(rope, row, d0, 8, a.err);
+    } else {
+        int b = row, end = row + 1;
+        if (seqs.q_start) {
+            b = seq_of_row(seqs.q_start, seqs.n_seqs, row, lane);
+            if (b < seqs.n_seqs) end = seqs.q_start[b + 1];
+        }
+        if (b >= seqs.n_seqs) return;
+        const int own = seqs.kv_len[b] - (end - row);
+        if ((own < 0 || own >> seqs.page_shift >= seqs.table_ld) && lane == 0) flag_error(a.err, ERR_KV_LEN, own);
+        turn = angles<8>(rope, row, rope.pos_base + own, d0, cs, sn, a.err);
+    }
+    if (!__all_sync(0xffffffffu, turn)) return;
+#pragma unroll
+    for (int j = 0; j < IT; j++) {
+        const bool on = mine + j * HPW < a.n_heads;
+        float lo[8], hi[8];
+#pragma unroll
+        for (int e = 0; e < 8; e++) {
+            lo[e] = on ? to_f32(raw[j][0][e / (16 / sizeof(S))].e[e % (16 / sizeof(S))]) : 0.0f;
+            hi[e] = on ? to_f32(raw[j][1][e / (16 / sizeof(S))].e[e % (16 / sizeof(S))]) : 0.0f;
+        }
+        if (a.q_norm) norm_head<D>(a, a.q_norm, d0, lo, hi);
+        turn_head(cs, sn, lo, hi);
+        if (on) {
+            __nv_bfloat16* dst = static_cast<__nv_bfloat16*>(a.q_out) + (int64_t)row * a.q_stride + (int64_t)(mine + j * HPW) * D + d0;
+            store_v<8>(dst, lo);
+            store_v<8>(dst + N, hi);
+        }
+    }
+}
+
+// WIDE: heads that rotate whole, rows and weights aligned to 16 bytes. P: positions of a warp. ITQ: heads a
+// lane of the query part has in flight.
+template <typename S, int D, bool WIDE, int P, int ITQ>
+__global__ void __launch_bounds__(256, P == 8 ? 3 : 2) paged_append_q8_kernel(AppendArgs a, RopeAxes rope, PagedSeqs seqs, PagedQ8 c,
+                                                                             int kv_ctas, int groups) {
+    constexpr int LPH = D / 16, HPW = 32 / LPH, IT = P / HPW, N = D / 2;  // lanes a position, positions side by side
     __shared__ TeamInfo info[8];
     __shared__ uint32_t most[8];
     __shared__ float part[WIDE ? 1 : 8][WIDE ? 1 : HPW][WIDE ? 1 : D];
@@ -125,11 +180,11 @@ __global__ void __launch_bounds__(256, 2) paged_append_q8_kernel(AppendArgs a, R
         AppendArgs qa = a;
         qa.n_kv = 0;
         const int64_t item = (int64_t)(blockIdx.x - kv_ctas) * 8 + warp;
-        if constexpr (WIDE) append_heads<S, __nv_bfloat16, D, 1>(qa, rope, seqs, groups, item);
+        if constexpr (WIDE) append_query<S, D, ITQ>(qa, rope, seqs, groups, item);
         else append_any_head<S, __nv_bfloat16>(qa, rope, seqs, item);
         return;
     }
-    const int wshift = c.block_shift - 4;  // log2 of a team's warps
+    const int wshift = c.block_shift - (P == 8 ? 3 : 4);  // log2 of a team's warps
     const int team = warp >> wshift, sub = warp & ((1 << wshift) - 1);
     const int64_t item = ((int64_t)blockIdx.x << (3 - wshift)) + team;
     const int64_t x = item / (2 * c.n_kv);
@@ -138,14 +193,14 @@ __global__ void __launch_bounds__(256, 2) paged_append_q8_kernel(AppendArgs a, R
     const int kh = is_v ? hk - c.n_kv : hk;
     float* const scales = is_v ? c.v_scale : c.k_scale;
     if (sub == 0) {
-        const TeamInfo t = find_block(seqs, c, scales, x, kh, lane, a.err);
+        const TeamInfo t = find_block(seqs, c, x, lane, a.err);
         if (lane == 0) info[team] = t;
     }
     __syncthreads();
     const TeamInfo t = info[team];
-    const int d0 = 8 * (lane % LPH), r = lane / LPH, base = t.first + 16 * sub;
+    const int64_t scale_at = t.page * c.scale_stride + ((int64_t)kh << (seqs.page_shift - c.block_shift)) + t.slot;
+    const int d0 = 8 * (lane % LPH), r = lane / LPH, base = t.first + P * sub;
     const int head = a.n_heads + hk;
-    const uint16_t* const nw = is_v ? nullptr : a.k_norm;
     float lo[IT][8], hi[IT][8];
     unsigned bits = 0;
     uint32_t live = 0;  // iterations whose position this lane has a row for
@@ -168,21 +223,20 @@ __global__ void __launch_bounds__(256, 2) paged_append_q8_kernel(AppendArgs a, R
             for (int e = 0; e < 8; e++) lo[i][e] = hi[i][e] = 0.0f;
         }
     }
+    const float old = t.ok ? scales[scale_at] : 0.0f;  // as the cache has it
     if (!is_v) {
 #pragma unroll
         for (int i = 0; i < IT; i++) {
-            if (!__any_sync(0xffffffffu, live >> i & 1)) continue;
             const int at = base + i * HPW + r;
             const int64_t row = t.q0 + (at - t.p0);
-            if (a.k_norm) norm_head<D, WIDE>(a, nw, d0, lo[i], hi[i]);
             bool turn = true;
             if constexpr (WIDE) {
                 float cs[8], sn[8];
-                if (live >> i & 1) {
-                    turn = angles<8>(rope, row, rope.pos_base + at, d0, cs, sn, a.err);
-                    if (turn) turn_head(cs, sn, lo[i], hi[i]);
-                }
+                if (live >> i & 1) turn = angles<8>(rope, row, rope.pos_base + at, d0, cs, sn, a.err);
+                if (a.k_norm) norm_head<D>(a, a.k_norm, d0, lo[i], hi[i]);  // (by every lane)
+                if (turn && (live >> i & 1)) turn_head(cs, sn, lo[i], hi[i]);
             } else {  // any pairs (d, d + n): the other one by way of shared memory
+                if (a.k_norm) norm_head<D, false>(a, a.k_norm, d0, lo[i], hi[i]);
                 float* const buf = part[warp][r];
                 const int n = rope.pairs;
 #pragma unroll
@@ -222,7 +276,7 @@ __global__ void __launch_bounds__(256, 2) paged_append_q8_kernel(AppendArgs a, R
     bits = __reduce_max_sync(0xffffffffu, bits);
     const bool any = __any_sync(0xffffffffu, live != 0);
     if (lane == 0) most[warp] = any ? bits : ~0u;  // ~0: no row
-    __syncthreads();
+    __syncthreads();  // (and every warp of the team has read the scale)
     if (!t.ok) return;
     uint32_t top = 0;
     bool rows = false;
@@ -234,12 +288,12 @@ __global__ void __launch_bounds__(256, 2) paged_append_q8_kernel(AppendArgs a, R
     const float wants = top >= 0x7f800000u ? __uint_as_float(0x7fffffffu) : __fdiv_rn(__uint_as_float(top), 127.0f);
     const bool fresh = t.lo == t.first;
     float s = wants < 1.17549435e-38f ? 0.0f : wants;
-    if (!fresh && !(s > t.scale) && s == s) s = t.scale;
+    if (!fresh && !(s > old) && s == s) s = old;
     const float by = s > 0.0f ? __frcp_rn(s) : 0.0f;  // (zero for NaN too)
     int8_t* const page = (is_v ? c.v : c.k) + t.page * c.page_stride + ((int64_t)kh << seqs.page_shift) * D;
     const int in_page = base & ((1 << seqs.page_shift) - 1);
-    if (!fresh && s > t.scale) {  // (s not NaN, nor the old one)
-        const float ratio = __fdiv_rn(t.scale, s);
+    if (!fresh && s > old) {  // (s not NaN, nor the old one)
+        const float ratio = __fdiv_rn(old, s);
 #pragma unroll 1
         for (int i = 0; i < IT; i++) {
             if (base + i * HPW + r >= t.lo) continue;
@@ -256,19 +310,31 @@ __global__ void __launch_bounds__(256, 2) paged_append_q8_kernel(AppendArgs a, R
             *reinterpret_cast<uint2*>(at) = codes8(lo[i], by);
             *reinterpret_cast<uint2*>(at + N) = codes8(hi[i], by);
         }
-    if (sub == 0 && lane == 0)
-        scales[t.page * c.scale_stride + ((int64_t)kh << (seqs.page_shift - c.block_shift)) + t.slot] = s;
+    if (sub == 0 && lane == 0) scales[scale_at] = s;
 }
 
-template <typename S, int D, bool WIDE>
+template <typename S, int D, bool WIDE, int P, int ITQ>
 static int launch_append_q8(lq_ctx* ctx, const AppendArgs& a, const RopeAxes& rope, const PagedSeqs& s, const PagedQ8& c) {
     const int64_t blocks = s.q_start ? (int64_t)(s.rows >> c.block_shift) + 2ll * s.n_seqs : (int64_t)std::min(s.rows, s.n_seqs);
-    const int64_t kv_ctas = (blocks * 2 * c.n_kv + (8 >> (c.block_shift - 4)) - 1) / (8 >> (c.block_shift - 4));
-    const int groups = WIDE ? ceil_div(a.n_heads, 512 / D) : a.n_heads;  // warps a row
+    const int teams = 8 >> (c.block_shift - (P == 8 ? 3 : 4));
+    const int64_t kv_ctas = (blocks * 2 * c.n_kv + teams - 1) / teams;
+    const int groups = WIDE ? ceil_div(a.n_heads, 512 / D * ITQ) : a.n_heads;  // warps a row
     const int64_t q_ctas = ((int64_t)s.rows * groups + 7) / 8;
     LQ_REQUIRE(ctx, kv_ctas + q_ctas < (1ll << 31), "lq_paged_append_q8: too many rows");
-    return launch_kernel(ctx, paged_append_q8_kernel<S, D, WIDE>, dim3((unsigned)(kv_ctas + q_ctas)), dim3(256), 0,
+    return launch_kernel(ctx, paged_append_q8_kernel<S, D, WIDE, P, ITQ>, dim3((unsigned)(kv_ctas + q_ctas)), dim3(256), 0,
                          "paged_append_q8", a, rope, s, c, (int)kv_ctas, groups);
+}
+
+template <typename S, int D>
+static int append_q8_d(lq_ctx* ctx, const AppendArgs& a, const RopeAxes& rope, const PagedSeqs& s, const PagedQ8& c, bool wide) {
+    if (!wide) return launch_append_q8<S, D, false, 16, 1>(ctx, a, rope, s, c);
+    // many rows: two query heads a lane, which share the row's angles; a decode step's few: one, so that they
+    // spread over the SMs
+    const bool few = (int64_t)s.rows * ceil_div(a.n_heads, 512 / D) < 16ll * ctx->sm_count;
+    // a block of 128 positions takes all eight warps of a CTA 16 each; of 8 a warp has twice as many
+    // neighbours on its SM
+    if (c.block_shift == 7) return few ? launch_append_q8<S, D, true, 16, 1>(ctx, a, rope, s, c) : launch_append_q8<S, D, true, 16, 2>(ctx, a, rope, s, c);
+    return few ? launch_append_q8<S, D, true, 8, 1>(ctx, a, rope, s, c) : launch_append_q8<S, D, true, 8, 2>(ctx, a, rope, s, c);
 }
 
 template <typename S>
@@ -276,8 +342,7 @@ static int append_q8(lq_ctx* ctx, const AppendArgs& a, const RopeAxes& rope, con
     auto al = [](const void* p) { return (uintptr_t)p % 16 == 0; };
     const bool wide = rope.pairs * 2 == a.head_dim && a.row_stride * sizeof(S) % 16 == 0 && a.q_stride * 2 % 16 == 0 &&
                       al(a.qkv) && al(a.q_out) && al(a.q_norm) && al(a.k_norm);
-    if (a.head_dim == 64) return wide ? launch_append_q8<S, 64, true>(ctx, a, rope, s, c) : launch_append_q8<S, 64, false>(ctx, a, rope, s, c);
-    return wide ? launch_append_q8<S, 128, true>(ctx, a, rope, s, c) : launch_append_q8<S, 128, false>(ctx, a, rope, s, c);
+    return a.head_dim == 64 ? append_q8_d<S, 64>(ctx, a, rope, s, c, wide) : append_q8_d<S, 128>(ctx, a, rope, s, c, wide);
 }
 
 // =========================================================================================
