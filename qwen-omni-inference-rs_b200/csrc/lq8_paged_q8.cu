@@ -346,11 +346,16 @@ static int append_q8(lq_ctx* ctx, const AppendArgs& a, const RopeAxes& rope, con
 }
 
 // =========================================================================================
-// Reading rows back: code * scale. A CTA looks up the slots of 32 rows of the batch, then its
-// threads take 16 codes each (one vector), neighbours along a position's dims and along positions,
-// which lie next to each other in a page of a kv head.
+// Reading rows back: code * scale. The last warp of a CTA looks up where the next 32 rows of the batch lie
+// while the others read and write 32 rows: a thread takes 16 codes at a time (one vector), eight of them
+// in flight, neighbours along a position's dims and along positions, which lie next to each other in
+// a page of a kv head. Bound: HBM, which likes few streams here: 24 whole sequences of up to 9000
+// positions to bf16 take 98 us with two CTAs an SM (5.3 TB/s, 81 % of a plain copy), 107 with three, 124 with
+// four, 102 to 120 with a CTA for every 32 rows. A call that is done in one round gets three (14054 rows of 4
+// heads of 64 dims to f32: 11.7 us instead of 14.3).
 // =========================================================================================
-constexpr int READ_ROWS = 32;
+constexpr int READ_ROWS = 32, READ_THREADS = 256;
+static_assert(READ_ROWS == 32, "a warp looks them up");
 
 struct ReadArgs {
     void* k_out;
@@ -360,66 +365,119 @@ struct ReadArgs {
     int* err;
 };
 
-template <typename T, int D>
-__global__ void __launch_bounds__(256) paged_read_q8_kernel(ReadArgs a, PagedSeqs s, PagedQ8 c) {
+// where row r lies, page * page size + position there, or -1: find_slot by a thread, whose neighbours look up
+// the neighbouring rows (a warp a row, four in turn: 6 us of a CTA's life)
+__device__ __forceinline__ int slot_of_row(const PagedSeqs& s, int r, int* err) {
+    int b = r, end = r + 1;
+    if (s.q_start) {
+        int n = s.n_seqs;  // the number of ends q_start[1..B] that are <= r lies in [b, b + n]
+        b = 0;
+        while (n > 0) {
+            const int half = n >> 1;
+            if (s.q_start[b + half + 1] <= r) b += half + 1, n -= half + 1;
+            else n = half;
+        }
+        if (b >= s.n_seqs) return -1;
+        end = s.q_start[b + 1];
+    } else if (b >= s.n_seqs) {
+        return -1;
+    }
+    const int own = s.kv_len[b] - (end - r), pg = own >> s.page_shift;
+    if (own < 0 || pg >= s.table_ld) {
+        flag_error(err, ERR_KV_LEN, own);
+        return -1;
+    }
+    const int page = s.table[(int64_t)b * s.table_ld + pg];
+    if ((unsigned)page >= (unsigned)s.n_pages) {
+        flag_error(err, ERR_PAGE_ID, page);
+        return -1;
+    }
+    return (page << s.page_shift) + (own & ((1 << s.page_shift) - 1));
+}
+
+__device__ __forceinline__ void store_cs(float* p, const float* v) {
+#pragma unroll
+    for (int i = 0; i < 16; i += 4) __stcs(reinterpret_cast<float4*>(p + i), make_float4(v[i], v[i + 1], v[i + 2], v[i + 3]));
+}
+__device__ __forceinline__ void store_cs(__nv_bfloat16* p, const float* v) {
+#pragma unroll
+    for (int i = 0; i < 16; i += 8)
+        __stcs(reinterpret_cast<uint4*>(p + i), make_uint4(pack_bf16x2(v[i], v[i + 1]), pack_bf16x2(v[i + 2], v[i + 3]),
+                                                           pack_bf16x2(v[i + 4], v[i + 5]), pack_bf16x2(v[i + 6], v[i + 7])));
+}
+
+// CTAS: on an SM
+template <typename T, int D, int CTAS>
+__global__ void __launch_bounds__(READ_THREADS + 32, CTAS) paged_read_q8_kernel(ReadArgs a, PagedSeqs s, PagedQ8 c) {
     constexpr int CH = D / 16;  // vectors of a position
-    __shared__ int slot[READ_ROWS];  // page * page size + position there, or -1
+    __shared__ int slots[2][READ_ROWS];  // page * page size + position there, or -1
     pdl_trigger();
     pdl_wait();
-    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-    const int64_t row0 = (int64_t)(blockIdx.x / a.parts) * READ_ROWS;
-    const int part = blockIdx.x % a.parts, n = (int)min((int64_t)READ_ROWS, s.rows - row0);
-#pragma unroll 1
-    for (int i = warp; i < READ_ROWS; i += 8) {
-        RowSlot o{0, 0, 0, false, false};
-        if (i < n) o = find_slot(s, (int)(row0 + i), lane, part == 0 ? a.err : nullptr);
-        if (lane == 0) slot[i] = o.live && o.ok ? (o.page << s.page_shift) + o.off : -1;
-    }
-    __syncthreads();
+    const int tid = threadIdx.x, part = blockIdx.x % a.parts;
+    const int groups = (s.rows + READ_ROWS - 1) / READ_ROWS, step = gridDim.x / a.parts;
     const int heads = 2 * c.n_kv, h0 = heads * part / a.parts, h1 = heads * (part + 1) / a.parts;
     const int mask = (1 << s.page_shift) - 1, sshift = s.page_shift - c.block_shift;
-    constexpr int STEP = 256 / CH, BATCH = 4;
+    constexpr int STEP = READ_THREADS / CH, BATCH = 8;
     const int ch = tid % CH;
-    // (rows fastest, then heads)
+    auto look = [&](int g, int buf) {  // by the last warp: the slots of a group
+        const int i = tid - READ_THREADS, row = g * READ_ROWS + i;
+        if (g < groups) slots[buf][i] = row < s.rows ? slot_of_row(s, row, part == 0 ? a.err : nullptr) : -1;
+    };
+    int g = blockIdx.x / a.parts, buf = 0;
+    if (tid >= READ_THREADS) look(g, 0);
+    __syncthreads();
 #pragma unroll 1
-    for (int i0 = h0 * READ_ROWS + tid / CH; i0 < h1 * READ_ROWS; i0 += STEP * BATCH) {
-        uint4 w[BATCH];
-        float sc[BATCH];
+    for (; g < groups; g += step, buf ^= 1) {
+        if (tid >= READ_THREADS) {
+            look(g + step, buf ^ 1);
+        } else {
+            const int* const slot = slots[buf];
+            const int64_t row0 = (int64_t)g * READ_ROWS;
+            // (rows fastest, then heads)
+#pragma unroll 1
+            for (int i0 = h0 * READ_ROWS + tid / CH; i0 < h1 * READ_ROWS; i0 += STEP * BATCH) {
+                uint4 w[BATCH];
+                float sc[BATCH];
 #pragma unroll
-        for (int j = 0; j < BATCH; j++) {
-            const int i = i0 + j * STEP, hk = i / READ_ROWS;
-            const int at = i < h1 * READ_ROWS ? slot[i % READ_ROWS] : -1;
-            if (at < 0) continue;
-            const bool is_v = hk >= c.n_kv;
-            const int kh = is_v ? hk - c.n_kv : hk, page = at >> s.page_shift, off = at & mask;
-            w[j] = __ldcs(reinterpret_cast<const uint4*>((is_v ? c.v : c.k) + page * c.page_stride +
-                                                         (((int64_t)kh << s.page_shift) + off) * D + 16 * ch));
-            sc[j] = (is_v ? c.v_scale : c.k_scale)[page * c.scale_stride + ((int64_t)kh << sshift) + (off >> c.block_shift)];
+                for (int j = 0; j < BATCH; j++) {
+                    const int i = i0 + j * STEP, hk = i / READ_ROWS;
+                    const int at = i < h1 * READ_ROWS ? slot[i % READ_ROWS] : -1;
+                    if (at < 0) continue;
+                    const bool is_v = hk >= c.n_kv;
+                    const int kh = is_v ? hk - c.n_kv : hk, page = at >> s.page_shift, off = at & mask;
+                    w[j] = __ldcs(reinterpret_cast<const uint4*>((is_v ? c.v : c.k) + page * c.page_stride +
+                                                                 (((int64_t)kh << s.page_shift) + off) * D + 16 * ch));
+                    sc[j] = (is_v ? c.v_scale : c.k_scale)[page * c.scale_stride + ((int64_t)kh << sshift) + (off >> c.block_shift)];
+                }
+#pragma unroll
+                for (int j = 0; j < BATCH; j++) {
+                    const int i = i0 + j * STEP, hk = i / READ_ROWS;
+                    if (i >= h1 * READ_ROWS || slot[i % READ_ROWS] < 0) continue;
+                    const bool is_v = hk >= c.n_kv;
+                    T* const dst = static_cast<T*>(is_v ? a.v_out : a.k_out) + (row0 + i % READ_ROWS) * a.out_stride +
+                                   (int64_t)(is_v ? hk - c.n_kv : hk) * D + 16 * ch;
+                    float v[16];
+                    const uint32_t u[4] = {w[j].x, w[j].y, w[j].z, w[j].w};
+#pragma unroll
+                    for (int e = 0; e < 16; e++) v[e] = (float)(int8_t)(u[e / 4] >> (8 * (e % 4))) * sc[j];
+                    store_cs(dst, v);
+                }
+            }
         }
-#pragma unroll
-        for (int j = 0; j < BATCH; j++) {
-            const int i = i0 + j * STEP, hk = i / READ_ROWS;
-            if (i >= h1 * READ_ROWS || slot[i % READ_ROWS] < 0) continue;
-            const bool is_v = hk >= c.n_kv;
-            T* const dst = static_cast<T*>(is_v ? a.v_out : a.k_out) + (row0 + i % READ_ROWS) * a.out_stride +
-                           (int64_t)(is_v ? hk - c.n_kv : hk) * D + 16 * ch;
-            float v[16];
-            const uint32_t u[4] = {w[j].x, w[j].y, w[j].z, w[j].w};
-#pragma unroll
-            for (int e = 0; e < 16; e++) v[e] = (float)(int8_t)(u[e / 4] >> (8 * (e % 4))) * sc[j];
-            store_v<8>(dst, v);
-            store_v<8>(dst + 8, v + 8);
-        }
+        __syncthreads();
     }
 }
 
 template <typename T, int D>
 static int launch_read_q8(lq_ctx* ctx, ReadArgs a, const PagedSeqs& s, const PagedQ8& c) {
     const int64_t groups = ceil_div(s.rows, READ_ROWS);
-    // few rows: their heads over several CTAs, so that two of them fall on an SM
-    a.parts = (int)std::max<int64_t>(1, std::min<int64_t>(2 * c.n_kv, 2 * ctx->sm_count / groups));
-    LQ_REQUIRE(ctx, groups * a.parts < (1ll << 31), "lq_paged_read_q8: too many rows");
-    return launch_kernel(ctx, paged_read_q8_kernel<T, D>, dim3((unsigned)(groups * a.parts)), dim3(256), 0, "paged_read_q8", a, s, c);
+    // few rows: their heads over several CTAs
+    a.parts = (int)std::max<int64_t>(1, std::min<int64_t>(2 * c.n_kv, 3 * ctx->sm_count / groups));
+    if (groups * a.parts <= 3 * ctx->sm_count)
+        return launch_kernel(ctx, paged_read_q8_kernel<T, D, 3>, dim3((unsigned)(groups * a.parts)), dim3(READ_THREADS + 32), 0,
+                             "paged_read_q8", a, s, c);
+    const int ctas = std::max(1, 2 * ctx->sm_count / a.parts) * a.parts;
+    return launch_kernel(ctx, paged_read_q8_kernel<T, D, 2>, dim3((unsigned)ctas), dim3(READ_THREADS + 32), 0, "paged_read_q8", a, s, c);
 }
 
 int make_paged_q8(lq_ctx* ctx, const char* who, PagedQ8* c, int8_t* k, int8_t* v, float* k_scale, float* v_scale,
