@@ -383,16 +383,25 @@ prefix_attn_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_co
             int t = sg.t0;
 #pragma unroll 1
             for (; t < sg.t1; t++) {
+                // 8-bit caches, lane i: the scales of the i-th 16 positions. K's in units of log2 (never so small
+                // that a masked score loses its minus infinity); V's as what a score gets on top and what a
+                // weight then counts for in l (codes of a scale of zero are zero: any other does)
+                [[maybe_unused]] float k_mul = 0.0f, v_add = 0.0f, v_per = 0.0f;
+                if constexpr (Q8) {
+                    if (!pa_wait(c, &c.sc_full[f][sc_slot], sc_ph)) break;
+                    k_mul = max_nan(c.sc[f][sc_slot][0][lane & 7] * cs, 1e-37f);
+                    float v = c.sc[f][sc_slot][1][lane & 7];
+                    v = v > 0.0f || v != v ? v : 8.6736e-19f;
+                    v_add = __log2f(v);
+                    v_per = __frcp_rn(v);
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive(&c.sc_empty[f][sc_slot]);
+                    if (++sc_slot == PA_SCALES) sc_slot = 0, sc_ph ^= 1;
+                }
+                auto of = [](float x, int i) { return __shfl_sync(0xffffffffu, x, i); };
                 if (!pa_wait(c, &c.s_full[f], s_ph)) break;
                 s_ph ^= 1;
                 tc_after();
-                if constexpr (Q8) {
-                    if (!pa_wait(c, &c.sc_full[f][sc_slot], sc_ph)) break;
-                }
-                // K's scale of 16 positions, in units of log2 (never so small that a masked score loses
-                // its minus infinity), and V's
-                [[maybe_unused]] auto k_of = [&](int i) { return max_nan(c.sc[f][sc_slot][0][i] * cs, 1e-37f); };
-                [[maybe_unused]] auto v_of = [&](int i) { return c.sc[f][sc_slot][1][i]; };
                 if (busy) {
                     const int lim = (t < chain ? g.a.prefix_len : vis) - t * PA_TILE;  // columns this row sees
                     // a larger maximum: when a row's grew by more than 2^8, l and O follow
@@ -429,12 +438,11 @@ prefix_attn_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_co
                             for (int i = 0; i < 32; i++)
                                 if (i >= upto) s[i] = -INFINITY;
                         }
-                        float mt, kc[2] = {cs, cs}, vc[2] = {1.0f, 1.0f};  // (halves of the columns: two scales)
+                        float mt, kc[2] = {cs, cs};  // (halves of the columns: two scales)
                         if constexpr (Q8) {
 #pragma unroll
                             for (int h = 0; h < 2; h++) {
-                                kc[h] = k_of(2 * wq + h);
-                                vc[h] = v_of(2 * wq + h);
+                                kc[h] = of(k_mul, 2 * wq + h);
                                 float mh = max_nan(s[16 * h], s[16 * h + 1]);
 #pragma unroll
                                 for (int i = 2; i < 16; i += 2) mh = max3(mh, s[16 * h + i], s[16 * h + i + 1]);
@@ -453,13 +461,17 @@ prefix_attn_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_co
                         float2 sum = make_float2(0.0f, 0.0f);
 #pragma unroll
                         for (int i = 0; i < 16; i++) {
-                            const float2 x = __ffma2_rn(make_float2(s[2 * i], s[2 * i + 1]), make_float2(kc[i / 8], kc[i / 8]), make_float2(neg, neg));
-                            float2 e = make_float2(ex2(x.x), ex2(x.y));
+                            const float add = Q8 ? neg + of(v_add, 2 * wq + i / 8) : neg;
+                            const float2 x = __ffma2_rn(make_float2(s[2 * i], s[2 * i + 1]), make_float2(kc[i / 8], kc[i / 8]), make_float2(add, add));
+                            const float2 e = make_float2(ex2(x.x), ex2(x.y));
                             sum = __fadd2_rn(sum, e);
-                            if constexpr (Q8) e = __fmul2_rn(e, make_float2(vc[i / 8], vc[i / 8]));
                             pk[i] = pack_bf16x2(e.x, e.y);
+                            if (Q8 && i % 8 == 7) {
+                                l = fmaf(sum.x + sum.y, of(v_per, 2 * wq + i / 8), l);
+                                sum = make_float2(0.0f, 0.0f);
+                            }
                         }
-                        l += sum.x + sum.y;
+                        if constexpr (!Q8) l += sum.x + sum.y;
 #pragma unroll 1
                         for (int w = 0; w < 4; w++) {
                             tmem_st16(t_s + 16 * ((wq + w) & 3), pk);
@@ -483,7 +495,7 @@ prefix_attn_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_co
                                 float mh = max_nan(s[16 * h], s[16 * h + 1]);
 #pragma unroll
                                 for (int i = 2; i < 16; i += 2) mh = max3(mh, s[16 * h + i], s[16 * h + i + 1]);
-                                mt = max_nan(mt, mh * k_of(h));
+                                mt = max_nan(mt, mh * of(k_mul, h));
                             }
                         } else {
                             float mx[4] = {s[0], s[1], s[2], s[3]};
@@ -494,8 +506,7 @@ prefix_attn_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_co
                             mt = max_nan(max3(mx[0], mx[1], max3(mx[2], s[124], s[125])), max3(mx[3], s[126], s[127]));
                         }
                         const float neg = raise(mt);
-                        float2 cs2 = make_float2(cs, cs), vs2 = make_float2(1.0f, 1.0f);
-                        const float2 neg2 = make_float2(neg, neg);
+                        float2 cs2 = make_float2(cs, cs), neg2 = make_float2(neg, neg);
                         float2 sum[2] = {make_float2(0.0f, 0.0f), make_float2(0.0f, 0.0f)};
 #pragma unroll
                         for (int j = 0; j < 4; j++) {
@@ -504,19 +515,23 @@ prefix_attn_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_co
                             for (int i = 0; i < 16; i++) {
                                 if constexpr (Q8)
                                     if (i % 8 == 0) {
-                                        const float kc = k_of(2 * j + i / 8), vc = v_of(2 * j + i / 8);
+                                        const float kc = of(k_mul, 2 * j + i / 8), add = neg + of(v_add, 2 * j + i / 8);
                                         cs2 = make_float2(kc, kc);
-                                        vs2 = make_float2(vc, vc);
+                                        neg2 = make_float2(add, add);
                                     }
                                 const float2 x = __ffma2_rn(make_float2(s[32 * j + 2 * i], s[32 * j + 2 * i + 1]), cs2, neg2);
-                                float2 e = make_float2(ex2(x.x), ex2(x.y));
+                                const float2 e = make_float2(ex2(x.x), ex2(x.y));
                                 sum[i & 1] = __fadd2_rn(sum[i & 1], e);
-                                if constexpr (Q8) e = __fmul2_rn(e, vs2);
                                 pk[i] = pack_bf16x2(e.x, e.y);
+                                if constexpr (Q8)
+                                    if (i % 8 == 7) {
+                                        l = fmaf((sum[0].x + sum[0].y) + (sum[1].x + sum[1].y), of(v_per, 2 * j + i / 8), l);
+                                        sum[0] = sum[1] = make_float2(0.0f, 0.0f);
+                                    }
                             }
                             tmem_st16(t_s + 16 * j, pk);
                         }
-                        l += (sum[0].x + sum[0].y) + (sum[1].x + sum[1].y);
+                        if constexpr (!Q8) l += (sum[0].x + sum[0].y) + (sum[1].x + sum[1].y);
                     } else {
                         // few rows: two passes over S, 32 columns at a time, in a tenth of the code
                         // (they come in many short segments, where fetching the instructions costs
@@ -534,10 +549,14 @@ prefix_attn_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_co
                                     for (int i = 0; i < 32; i++)
                                         if (j + i >= lim) s[i] = -INFINITY;
                                 }
-                                float kc[2] = {cs, cs}, vc[2] = {1.0f, 1.0f};
+                                float kc[2] = {cs, cs}, add[2] = {neg, neg}, per[2] = {1.0f, 1.0f};
                                 if constexpr (Q8) {
 #pragma unroll
-                                    for (int h = 0; h < 2; h++) kc[h] = k_of(j / 16 + h), vc[h] = v_of(j / 16 + h);
+                                    for (int h = 0; h < 2; h++) {
+                                        kc[h] = of(k_mul, j / 16 + h);
+                                        add[h] = neg + of(v_add, j / 16 + h);
+                                        per[h] = of(v_per, j / 16 + h);
+                                    }
                                 }
                                 if (pass == 0) {
                                     if constexpr (Q8) {
@@ -556,9 +575,10 @@ prefix_attn_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_co
                                     uint32_t pk[16];
 #pragma unroll
                                     for (int i = 0; i < 16; i++) {
-                                        const float p0 = ex2(fmaf(s[2 * i], kc[i / 8], neg)), p1 = ex2(fmaf(s[2 * i + 1], kc[i / 8], neg));
-                                        sum += p0 + p1;
-                                        pk[i] = Q8 ? pack_bf16x2(p0 * vc[i / 8], p1 * vc[i / 8]) : pack_bf16x2(p0, p1);
+                                        const float p0 = ex2(fmaf(s[2 * i], kc[i / 8], add[i / 8])), p1 = ex2(fmaf(s[2 * i + 1], kc[i / 8], add[i / 8]));
+                                        if constexpr (Q8) sum = fmaf(p0 + p1, per[i / 8], sum);
+                                        else sum += p0 + p1;
+                                        pk[i] = pack_bf16x2(p0, p1);
                                     }
                                     // P of columns j.. lands on S columns j/2.., which have been read
                                     tmem_st16(t_s + j / 2, pk);
@@ -573,10 +593,6 @@ prefix_attn_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_co
                 tc_before();
                 __syncwarp();
                 if (lane == 0) mbar_arrive(&c.p_full[f]);
-                if constexpr (Q8) {
-                    if (lane == 0) mbar_arrive(&c.sc_empty[f][sc_slot]);
-                    if (++sc_slot == PA_SCALES) sc_slot = 0, sc_ph ^= 1;
-                }
                 if (t == sg.t0) {
                     more = next(true);
                     early = more == NX_SEG && q_ahead(sg, nx);
