@@ -78,6 +78,16 @@ __device__ __forceinline__ bool mbar_try_wait(uint64_t* bar, unsigned parity) {
         : "memory");
     return ok != 0;
 }
+// whether the phase is complete, without waiting for it
+__device__ __forceinline__ bool mbar_test_wait(uint64_t* bar, unsigned parity) {
+    uint32_t ok;
+    asm volatile(
+        "{\n .reg .pred p;\n mbarrier.test_wait.parity.shared::cta.b64 p, [%1], %2;\n selp.u32 %0, 1, 0, p;\n}"
+        : "=r"(ok)
+        : "r"(smem_addr(bar)), "r"(parity)
+        : "memory");
+    return ok != 0;
+}
 // Bounded wait: gives up after `limit` polls (each try_wait itself blocks for a while), so a
 // copy that never lands ends the kernel with an error instead of a hang.
 __device__ __forceinline__ bool mbar_wait(uint64_t* bar, unsigned parity, long long limit = (1ll << 24)) {

@@ -333,11 +333,15 @@ static int attend_q8(lq_ctx* ctx, const PrefixAttnArgs& a, const PagedSeqs& s, c
     }
     if (stream_own) {
         const int rows = (stream_prefix && a.prefix_len > 0 ? all_rows : own_rows) > 8 ? 16 : 8;
-        if constexpr (D == 128) steps_st = plan_cut(a, s, true, ctx->sm_count, &st, rows, prefix_attn_q8_decode_ctas(rows), 128);
-        else steps_st = plan_cut(a, s, true, ctx->sm_count, &st, rows, PREFIX_ATTN_Q8_WARPS);
+        steps_st = plan_cut(a, s, true, ctx->sm_count, &st, rows, PREFIX_ATTN_Q8_CTAS, 128);
         set_polls(&st, true);
         st.streams = stream_prefix ? 3 : 2;
-        st.chunks = D == 128;
+        st.chunks = 1;
+        // an item's beginning and end take as long as three of its tiles (with 0, 1, 2 and 3 of them 48
+        // sequences of up to 4000 positions, head dimension 64, took 38, 36.5, 30.5 and 29.4 us: short items
+        // in a row held up their CTA)
+        st.extra = 3;
+        steps_st += 3 * (int64_t)a.n_kv * ((int64_t)s.rows * a.group / st.ob + s.n_seqs + 1);
     }
     LQ_REQUIRE(ctx, steps_tc < PREFIX_MAX_STEPS && steps_st < PREFIX_MAX_STEPS, "%s: %lld steps, more than a launch can number", who,
                (long long)std::max(steps_tc, steps_st));
@@ -356,11 +360,7 @@ static int attend_q8(lq_ctx* ctx, const PrefixAttnArgs& a, const PagedSeqs& s, c
     int rc = make_workspace(ctx, who, a, s, D, own, pre);
     if (rc) return rc;
     if (pre == &tc && (rc = launch_prefix_attn_tc(ctx, a, s, tc, D, &c))) return rc;
-    if (own == &st) {
-        if constexpr (D == 128) rc = launch_prefix_attn_q8_decode(ctx, a, s, c, st);
-        else rc = launch_prefix_attn_q8(ctx, a, s, c, st, D);
-        if (rc) return rc;
-    }
+    if (own == &st && (rc = launch_prefix_attn_q8_decode(ctx, a, s, c, st, D))) return rc;
     return launch_merge<__nv_bfloat16, D>(ctx, a, s, *own, *pre);
 }
 

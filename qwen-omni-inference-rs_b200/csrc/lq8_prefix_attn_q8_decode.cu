@@ -1,6 +1,6 @@
 // lq8_prefix_attn_q8_decode.cu -- the shared-prefix attention for 8-bit caches with up to 16 stacked rows
-// a kv head (a decode step), head dimension 128: codes go from memory into int8 products on tcgen05
-// as they are, and no thread ever touches one.
+// a kv head (a decode step): codes go from memory into int8 products on tcgen05 as they are, and no
+// thread ever touches one.
 //
 // A CTA walks its share of the line of steps (Shares in lq8_prefix_plan.cuh), 128 positions each; three
 // CTAs fit on an SM (two with 16 rows) and hide each other's latency. With R = 8 or 16 rows:
@@ -36,12 +36,11 @@
 namespace lq {
 
 constexpr int PD_TILE = 128;     // positions of a step
-constexpr int PD_STAGES = 4;     // tiles of K or V (16 KB)
-constexpr int PD_BYTES = PD_TILE * 128;
+constexpr int pd_stages(int D) { return D == 64 ? 8 : 4; }  // tiles of K or V (64 KB)
 constexpr int PD_THREADS = 192;
 constexpr int PD_SCAN = 128;     // entries of the scan over the sequences
 constexpr int ERR_PD_WAIT = 97;  // a wait ran out
-constexpr int pd_ctas(int R) { return R == 8 ? 3 : 2; }
+constexpr int PD_CTAS = PREFIX_ATTN_Q8_CTAS;
 
 enum { PD_OWN = 1, PD_END = 2, PD_WHOLE = 4 };
 // the steps [t0, t1) of one item
@@ -59,7 +58,7 @@ struct alignas(16) PdSeg {
 
 template <int R>
 struct PdCtl {
-    uint64_t full[PD_STAGES], empty[PD_STAGES], seg_full[2], seg_empty[2];
+    uint64_t full[pd_stages(64)], empty[pd_stages(64)], seg_full[2], seg_empty[2];
     uint64_t q_full, s_full[2], p_full[2], o_full[2], met[2], done;
     uint32_t tmem;
     int abort;
@@ -78,9 +77,20 @@ struct PdArgs {
     PagedQ8 c;
 };
 
-// D s32, A and B s8, M 128, N n; A MN-major or K-major
-__host__ __device__ constexpr uint32_t pd_idesc(int n, int a_mn) {
-    return (2u << 4) | (1u << 7) | (1u << 10) | ((uint32_t)a_mn << 15) | ((uint32_t)(n >> 3) << 17) | (8u << 24);
+// D s32, A and B s8, M m, N n; A MN-major or K-major
+__host__ __device__ constexpr uint32_t pd_idesc(int m, int n, int a_mn) {
+    return (2u << 4) | (1u << 7) | (1u << 10) | ((uint32_t)a_mn << 15) | ((uint32_t)(n >> 3) << 17) | ((uint32_t)(m >> 4) << 24);
+}
+// operands of rows of `row` bytes (128 or 64), swizzled over as many, 8-row groups next to each other
+template <int row>
+__device__ __forceinline__ uint64_t pd_desc(uint32_t saddr) {
+    return (uint64_t)((saddr >> 4) & 0x3FFF) | (uint64_t)1 << 16 | (uint64_t)(8 * row >> 4) << 32 | (uint64_t)1 << 46 |
+           (uint64_t)(row == 128 ? 2 : 4) << 61;
+}
+// where in such an operand byte x of row r lies
+template <int row>
+__device__ __forceinline__ uint32_t pd_at(int r, int x) {
+    return r * row + (((x >> 4) ^ (row == 128 ? r & 7 : (r >> 1) & 3)) << 4) + (x & 15);
 }
 __device__ __forceinline__ void mma_i8(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t acc) {
     asm volatile(
@@ -135,12 +145,13 @@ __device__ __forceinline__ float pd_warp_sums(float* v, int lane) {
     return t;
 }
 
-template <int R>
-__global__ void __launch_bounds__(PD_THREADS, pd_ctas(R))
+template <int D, int R>
+__global__ void __launch_bounds__(PD_THREADS, PD_CTAS)
 prefix_attn_q8_decode_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v,
                              const __grid_constant__ PdArgs g) {
-    constexpr int D = 128, N = 2 * R;             // columns of S^T and O^T
-    constexpr uint32_t OPERAND = N * 128;         // bytes of Q^T's or P^T's planes
+    constexpr int N = 2 * R;                      // columns of S^T and O^T
+    constexpr int PD_STAGES = pd_stages(D), PD_BYTES = PD_TILE * D;
+    constexpr uint32_t OPERAND = N * 128;         // bytes of P^T's planes (and of Q^T's at most)
     constexpr uint32_t COLUMNS = R == 8 ? 64 : 128;
     const PrefixAttnArgs& a = g.a;
     const PagedSeqs& s = g.s;
@@ -253,56 +264,86 @@ prefix_attn_q8_decode_kernel(const __grid_constant__ CUtensorMap map_k, const __
         PdSeg sg;
         bool ok = true;
         float m[R], l[R], o[R];
+        // this thread's dim of O: TMEM lanes are dims, or, with 64 of them, lanes 0-15 of each warp are
+        const int dim = D == 128 ? tid : 16 * warp + lane;
+        const bool has = D == 128 || lane < 16;
         auto finish = [&]() {    // rows of sg
 #pragma unroll
             for (int r = 0; r < R; r++)
                 if (r < sg.n) {
                     const float y = l[r] == 0.0f ? 0.0f : o[r] * (l[r] > 0.0f ? 1.0f / l[r] : l[r]);
                     const int st = sg.row0 + r, tok = a.group_div(st);
-                    const int64_t col = (int64_t)(sg.kh * a.group + st - tok * a.group) * D + tid;
-                    if (a.out) static_cast<__nv_bfloat16*>(a.out)[(int64_t)tok * a.out_stride + col] = __float2bfloat16_rn(y);
-                    if (a.xq) {  // a warp has a block of 32 dims
-                        float d, id;
-                        q8_scale(warp_max(fabsf(y)), d, id);
+                    const int64_t col = (int64_t)(sg.kh * a.group + st - tok * a.group) * D + dim;
+                    if (a.out && has) static_cast<__nv_bfloat16*>(a.out)[(int64_t)tok * a.out_stride + col] = __float2bfloat16_rn(y);
+                    if (a.xq) {  // a warp has a block of 32 dims, or two warps do
+                        float amax = warp_max(has ? fabsf(y) : 0.0f), d, id;
+                        if constexpr (D == 64) {
+                            const float(*const all)[R] = c.red[meetings & 1];
+                            if (lane == 0) c.red[meetings & 1][warp][0] = amax;
+                            ok = meet();
+                            if (!ok) return;
+                            amax = fmaxf(all[warp & 2][0], all[warp | 1][0]);
+                        }
+                        q8_scale(amax, d, id);
                         const int64_t at = (int64_t)tok * a.n_heads * D + col;
-                        if (lane == 0) a.xd[at / 32] = f2h(d);
-                        a.xq[at] = (int8_t)q8_quant(y, id);
+                        if (lane == 0 && dim % 32 == 0) a.xd[at / 32] = f2h(d);
+                        if (has) a.xq[at] = (int8_t)q8_quant(y, id);
                     }
                 }
         };
+        // The next segment is begun while the last tile of one is worked on, if the producer has got
+        // there: its pages and Q are on their way, then its scales (without that its start took 1.7 us, 3
+        // while memory is busy).
+        constexpr int TPR = 128 / R, DIMS = D / TPR;  // threads of a row of Q, dims of a thread
+        const int q_row = tid / TPR, q_part = tid % TPR;
+        PdSeg nx;
+        bool have = false, ended = false;
+        int nx_id[2] = {-1, -1};
+        uint2 nx_q[DIMS / 4];
+        float ks = 0.0f, vs = 1.0f;
+        // pages two tiles ahead, scales one
+        auto page_at = [&](const PdSeg& o, int t) {
+            const int32_t* const table = o.flags & PD_OWN ? s.table + (int64_t)o.b * s.table_ld : a.prefix_table;
+            const int x = t * PD_TILE + tid;
+            int id = -1;
+            if (t < o.t1 && x < o.kv_end) id = table[x >> s.page_shift];
+            return (unsigned)id < (unsigned)s.n_pages ? id : -1;  // (reported by the producer)
+        };
+        auto scales_at = [&](const PdSeg& o, int t, int id) {  // of this position
+            ks = 0.0f;
+            vs = 1.0f;
+            if (id >= 0) {
+                const int64_t at = id * g.c.scale_stride + ((int64_t)o.kh << (s.page_shift - g.c.block_shift)) +
+                                   (((t * PD_TILE + tid) & mask) >> g.c.block_shift);
+                ks = g.c.k_scale[at];
+                vs = g.c.v_scale[at];
+            }
+        };
+        auto begin = [&]() {
+            nx_id[0] = page_at(nx, nx.t0);
+            nx_id[1] = page_at(nx, nx.t0 + 1);
+            const int st = nx.row0 + min(q_row, nx.n - 1), tok = a.group_div(st);
+            const uint2* src = reinterpret_cast<const uint2*>(static_cast<const __nv_bfloat16*>(a.q) + (int64_t)tok * a.q_stride +
+                                                              (int64_t)(nx.kh * a.group + st - tok * a.group) * D + q_part * DIMS);
+#pragma unroll
+            for (int i = 0; i < DIMS / 4; i++) nx_q[i] = src[i];
+        };
 #pragma unroll 1
-        while (ok && fetch(sg)) {
-            // ---- this position's scales: pages two tiles ahead, scales one ----
-            const int32_t* const table = sg.flags & PD_OWN ? s.table + (int64_t)sg.b * s.table_ld : a.prefix_table;
-            auto page_at = [&](int t) {
-                const int x = t * PD_TILE + tid;
-                int id = -1;
-                if (t < sg.t1 && x < sg.kv_end) id = table[x >> s.page_shift];
-                return (unsigned)id < (unsigned)s.n_pages ? id : -1;  // (reported by the producer)
-            };
-            auto scales_at = [&](int t, int id, float& ks, float& vs) {
-                ks = 0.0f;
-                vs = 1.0f;
-                if (id >= 0) {
-                    const int64_t at = id * g.c.scale_stride + ((int64_t)sg.kh << (s.page_shift - g.c.block_shift)) +
-                                       (((t * PD_TILE + tid) & mask) >> g.c.block_shift);
-                    ks = g.c.k_scale[at];
-                    vs = g.c.v_scale[at];
-                }
-            };
-            int id_next = page_at(sg.t0), id_then = page_at(sg.t0 + 1);
+        while (ok && !ended) {
+            if (!have) {
+                if (!fetch(nx)) break;
+                begin();
+                scales_at(nx, nx.t0, nx_id[0]);
+            }
+            have = false;
+            sg = nx;
+            int id_next = nx_id[0], id_then = nx_id[1];
             // ---- Q in two bytes ----
             {
-                constexpr int TPR = 128 / R, DIMS = D / TPR;  // threads of a row, dims of a thread
-                const int r = tid / TPR, part = tid % TPR, st = sg.row0 + min(r, sg.n - 1), tok = a.group_div(st);
-                const uint4* src = reinterpret_cast<const uint4*>(static_cast<const __nv_bfloat16*>(a.q) + (int64_t)tok * a.q_stride +
-                                                                  (int64_t)(sg.kh * a.group + st - tok * a.group) * D + part * DIMS);
+                const int r = q_row, part = q_part;
                 uint32_t w[DIMS / 2], top = 0;
 #pragma unroll
-                for (int i = 0; i < DIMS / 8; i++) {
-                    const uint4 u = src[i];
-                    w[4 * i] = u.x, w[4 * i + 1] = u.y, w[4 * i + 2] = u.z, w[4 * i + 3] = u.w;
-                }
+                for (int i = 0; i < DIMS / 4; i++) w[2 * i] = nx_q[i].x, w[2 * i + 1] = nx_q[i].y;
 #pragma unroll
                 for (int i = 0; i < DIMS / 2; i++) top = max(top, max(w[i] & 0x7fff0000u, (w[i] << 16) & 0x7fff0000u));
 #pragma unroll
@@ -323,20 +364,16 @@ prefix_attn_q8_decode_kernel(const __grid_constant__ CUtensorMap map_k, const __
                         dn[i] |= (uint32_t)(v & 0xff) << (8 * e);
                     }
                 }
-                // (rows r and R + r swizzle alike: both are r modulo 8)
-                const uint32_t at = (((part * DIMS >> 4) ^ (r & 7)) << 4) + (part * DIMS & 15);
 #pragma unroll
-                for (int i = 0; i < DIMS / 4; i += 2) {
-                    *reinterpret_cast<uint2*>(q_sm + r * 128 + at + 4 * i) = make_uint2(up[i], up[i + 1]);
-                    *reinterpret_cast<uint2*>(q_sm + (R + r) * 128 + at + 4 * i) = make_uint2(dn[i], dn[i + 1]);
+                for (int i = 0; i < DIMS / 4; i++) {
+                    *reinterpret_cast<uint32_t*>(q_sm + pd_at<D>(r, part * DIMS + 4 * i)) = up[i];
+                    *reinterpret_cast<uint32_t*>(q_sm + pd_at<D>(R + r, part * DIMS + 4 * i)) = dn[i];
                 }
                 if (part == 0) c.qf[r] = fine ? amax * (1.0f / 32512.0f) * cs : amax < INFINITY ? 0.0f : __uint_as_float(0x7fffffffu);
                 proxy_fence();
                 __syncwarp();
                 if (lane == 0) mbar_arrive(&c.q_full);
             }
-            float ks, vs;
-            scales_at(sg.t0, id_next, ks, vs);
             ok = pd_wait(&c.abort, &c.q_full, q_ph, p.polls);
             if (!ok) break;
             q_ph ^= 1;
@@ -363,8 +400,14 @@ prefix_attn_q8_decode_kernel(const __grid_constant__ CUtensorMap map_k, const __
                 const float k1 = ks, v1 = vs > 0.0f || vs != vs ? vs : 8.6736e-19f;  // (codes of a scale of zero are zero)
                 const float lv = __log2f(v1), per = __frcp_rn(v1);
                 id_next = id_then;
-                id_then = page_at(t + 2);
-                scales_at(t + 1, id_next, ks, vs);
+                id_then = page_at(sg, t + 2);
+                if (t + 1 < sg.t1) {
+                    scales_at(sg, t + 1, id_next);
+                } else if (__all_sync(0xffffffffu, mbar_test_wait(&c.seg_full[taken & 1], (taken >> 1) & 1u))) {
+                    have = fetch(nx);
+                    ended = !have;
+                    if (have) begin();
+                }
                 ok = pd_wait(&c.abort, &c.s_full[n_tile & 1], (n_tile >> 1) & 1u, p.polls);
                 if (!ok) break;
                 tc_after();
@@ -406,7 +449,7 @@ prefix_attn_q8_decode_kernel(const __grid_constant__ CUtensorMap map_k, const __
                 for (int r = 0; r < R; r++) {
                     e[r] = ex2(e[r] - (u[r] == -INFINITY ? 0.0f : u[r]));
                     const uint32_t v = __float_as_uint(fmaf(e[r], 32512.0f, 12582912.0f));  // (whole number in the low bits)
-                    const uint32_t at = r * 128 + (((tid >> 4) ^ (r & 7)) << 4) + (tid & 15);
+                    const uint32_t at = pd_at<128>(r, tid);  // (rows r and R + r swizzle alike)
                     pt[at] = (uint8_t)((v + 128) >> 8);
                     pt[at + R * 128] = (uint8_t)v;
                 }
@@ -436,6 +479,7 @@ prefix_attn_q8_decode_kernel(const __grid_constant__ CUtensorMap map_k, const __
                 }
             }
             if (!ok) break;
+            if (have) scales_at(nx, nx.t0, nx_id[0]);
             ok = take_o(n_tile - 1);
             if (!ok) break;
             // ---- the segment's result: one dim of each row ----
@@ -457,7 +501,7 @@ prefix_attn_q8_decode_kernel(const __grid_constant__ CUtensorMap map_k, const __
                 for (int r = 0; r < R; r++)
                     if (r < sg.n) {
                         if (tid == r) p.ml[own][(int64_t)sg.slot * cap + r] = make_float2(m[r], l[r]);
-                        p.o[own][(((int64_t)sg.slot * (D / 4) + (tid >> 2)) * cap + r) * 4 + (tid & 3)] = o[r];
+                        if (has) p.o[own][(((int64_t)sg.slot * (D / 4) + (dim >> 2)) * cap + r) * 4 + (dim & 3)] = o[r];
                     }
             }
         }
@@ -552,7 +596,7 @@ prefix_attn_q8_decode_kernel(const __grid_constant__ CUtensorMap map_k, const __
                     n_rb = os.blocks(si);
 #pragma unroll 1
                     for (; rb < n_rb; rb++) {
-                        const int n = os.tiles(si, rb);
+                        const int n = os.steps(si, rb);
                         if (rest < n) break;
                         rest -= n;
                     }
@@ -566,50 +610,53 @@ prefix_attn_q8_decode_kernel(const __grid_constant__ CUtensorMap map_k, const __
                         kv_end = os.visible(si, rb);
                         nt = (kv_end + PD_TILE - 1) / PD_TILE;
                     }
-                    const int end = min(nt, tile + hi - step);
-                    if (end <= tile) break;  // lengths that changed under the kernel
-                    const int row0 = (own ? si.q0 * a.group : 0) + rb * p.pb;
-                    // (a block of padding: its first row, for nothing)
-                    const int n = max(1, min(p.pb, (own ? si.q : live_rows(s)) * a.group - rb * p.pb));
-                    const int item = (own ? a.n_kv * os.base(si, b) : 0) + kh * n_rb + rb;
-                    const bool begins = tile == 0, whole = a.prefix_len == 0 && begins && end == nt;
-                    if (lane == 0) {
-                        if (tile == 0) p.first[part][item] = worker;
-                        if (end == nt) p.last[part][item] = worker;
-                        if (a.prefix_len == 0 && tile == 0 && end < nt) p.split[worker] = SplitItem{n, row0, kh, item};
-                    }
-                    PdSeg sg;
-                    sg.t0 = tile, sg.t1 = end, sg.n = n, sg.flags = (own ? PD_OWN : 0) | (whole ? PD_WHOLE : 0);
-                    sg.kh = kh, sg.b = b, sg.kv_end = kv_end, sg.row0 = row0, sg.voff = own ? si.kv - si.q + 1 - si.q0 : 0;
-                    sg.slot = own ? p.own_slot(item, worker, begins) : item + worker;
-                    sg.pad[0] = sg.pad[1] = 0;
-                    const int32_t* const table = own ? s.table + (int64_t)b * s.table_ld : a.prefix_table;
-                    auto page_at = [&](int t) {  // this lane's page of tile t; none: zeros
-                        const int x = t * PD_TILE + lane * box;
-                        int id = s.n_pages;
-                        if (lane < boxes && t < end && x < kv_end) {
-                            id = table[x >> s.page_shift];
-                            if ((unsigned)id >= (unsigned)s.n_pages) {
-                                flag_error(a.err, ERR_PAGE_ID, id);
-                                id = s.n_pages;
-                            }
+                    // (an own item counts for a step more than its tiles: a segment's beginning and end)
+                    const int ns = nt + (own && nt > 0 ? p.extra : 0), upto = min(ns, tile + hi - step), end = min(nt, upto);
+                    if (upto <= tile) break;  // lengths that changed under the kernel
+                    if (end > tile) {
+                        const int row0 = (own ? si.q0 * a.group : 0) + rb * p.pb;
+                        // (a block of padding: its first row, for nothing)
+                        const int n = max(1, min(p.pb, (own ? si.q : live_rows(s)) * a.group - rb * p.pb));
+                        const int item = (own ? a.n_kv * os.base(si, b) : 0) + kh * n_rb + rb;
+                        const bool begins = tile == 0, whole = a.prefix_len == 0 && begins && end == nt;
+                        if (lane == 0) {
+                            if (tile == 0) p.first[part][item] = worker;
+                            if (end == nt) p.last[part][item] = worker;
+                            if (a.prefix_len == 0 && tile == 0 && end < nt) p.split[worker] = SplitItem{n, row0, kh, item};
                         }
-                        return id;
-                    };
-                    int id = page_at(tile), id_next = page_at(tile + 1);
-                    put(sg);
-                    // K of the next tile before V of this one, as the MMA warp takes them
-                    if (ok) load(&map_k, kh, tile * PD_TILE, id);
-#pragma unroll 1
-                    for (int t = tile; t < end && ok; t++) {
-                        const int id_then = page_at(t + 2);
-                        if (t + 1 < end) load(&map_k, kh, (t + 1) * PD_TILE, id_next);
-                        if (ok) load(&map_v, kh, t * PD_TILE, id);
-                        id = id_next;
-                        id_next = id_then;
+                        PdSeg sg;
+                        sg.t0 = tile, sg.t1 = end, sg.n = n, sg.flags = (own ? PD_OWN : 0) | (whole ? PD_WHOLE : 0);
+                        sg.kh = kh, sg.b = b, sg.kv_end = kv_end, sg.row0 = row0, sg.voff = own ? si.kv - si.q + 1 - si.q0 : 0;
+                        sg.slot = own ? p.own_slot(item, worker, begins) : item + worker;
+                        sg.pad[0] = sg.pad[1] = 0;
+                        const int32_t* const table = own ? s.table + (int64_t)b * s.table_ld : a.prefix_table;
+                        auto page_at = [&](int t) {  // this lane's page of tile t; none: zeros
+                            const int x = t * PD_TILE + lane * box;
+                            int id = s.n_pages;
+                            if (lane < boxes && t < end && x < kv_end) {
+                                id = table[x >> s.page_shift];
+                                if ((unsigned)id >= (unsigned)s.n_pages) {
+                                    flag_error(a.err, ERR_PAGE_ID, id);
+                                    id = s.n_pages;
+                                }
+                            }
+                            return id;
+                        };
+                        int id = page_at(tile), id_next = page_at(tile + 1);
+                        put(sg);
+                        // K of the next tile before V of this one, as the MMA warp takes them
+                        if (ok) load(&map_k, kh, tile * PD_TILE, id);
+    #pragma unroll 1
+                        for (int t = tile; t < end && ok; t++) {
+                            const int id_then = page_at(t + 2);
+                            if (t + 1 < end) load(&map_k, kh, (t + 1) * PD_TILE, id_next);
+                            if (ok) load(&map_v, kh, t * PD_TILE, id);
+                            id = id_next;
+                            id_next = id_then;
+                        }
                     }
                     // ---- the next item with a step ----
-                    step += end - tile;
+                    step += upto - tile;
                     tile = 0;
                     while (step < hi) {
                         if (++rb >= n_rb) {
@@ -646,12 +693,12 @@ prefix_attn_q8_decode_kernel(const __grid_constant__ CUtensorMap map_k, const __
         if (lane == 0) c.issued = issued;
     } else {
         // ------------------------------ MMA issuer ------------------------------
-        constexpr uint32_t id_qk = pd_idesc(N, 0), id_pv = pd_idesc(N, 1);
+        constexpr uint32_t id_qk = pd_idesc(128, N, 0), id_pv = pd_idesc(D, N, 1);
         int n_tile = 0, slot = 0;
         unsigned ph = 0, q_ph = 0;
         bool ok = true;
         PdSeg sg;
-        const uint64_t q = tc_desc(smem_addr(q_sm), 16);
+        const uint64_t q = pd_desc<D>(smem_addr(q_sm));
         auto take = [&]() {  // the next stage of the ring
             ok = pd_wait(&c.abort, &c.full[slot], ph, p.polls);
             const int at = slot;
@@ -662,10 +709,10 @@ prefix_attn_q8_decode_kernel(const __grid_constant__ CUtensorMap map_k, const __
             const int at = take();
             if (!ok) return;
             tc_after();
-            const uint64_t kt = tc_desc(smem_addr(ring + at * PD_BYTES), 16);
+            const uint64_t kt = pd_desc<D>(smem_addr(ring + at * PD_BYTES));
             if (elect_one()) {
 #pragma unroll
-                for (int j = 0; j < 4; j++) mma_i8(tmem + (k & 1) * N, kt + 2 * j, q + 2 * j, id_qk, j > 0);
+                for (int j = 0; j < D / 32; j++) mma_i8(tmem + (k & 1) * N, kt + 2 * j, q + 2 * j, id_qk, j > 0);
                 tc_commit(&c.empty[at]);
                 tc_commit(&c.s_full[k & 1]);
             }
@@ -686,11 +733,11 @@ prefix_attn_q8_decode_kernel(const __grid_constant__ CUtensorMap map_k, const __
                 ok = pd_wait(&c.abort, &c.p_full[n_tile & 1], (n_tile >> 1) & 1u, p.polls);
                 if (!ok) break;
                 tc_after();
-                const uint64_t v = tc_desc(smem_addr(ring + at * PD_BYTES), PD_BYTES);
-                const uint64_t pt = tc_desc(smem_addr(p_sm + (n_tile & 1) * OPERAND), 16);
+                const uint64_t v = pd_desc<D>(smem_addr(ring + at * PD_BYTES));
+                const uint64_t pt = pd_desc<128>(smem_addr(p_sm + (n_tile & 1) * OPERAND));
                 if (elect_one()) {
 #pragma unroll
-                    for (int j = 0; j < 4; j++) mma_i8(tmem + 2 * N + (n_tile & 1) * N, v + j * (4096 >> 4), pt + 2 * j, id_pv, j > 0);
+                    for (int j = 0; j < 4; j++) mma_i8(tmem + 2 * N + (n_tile & 1) * N, v + j * (32 * D >> 4), pt + 2 * j, id_pv, j > 0);
                     tc_commit(&c.empty[at]);
                     tc_commit(&c.o_full[n_tile & 1]);
                 }
@@ -728,30 +775,29 @@ prefix_attn_q8_decode_kernel(const __grid_constant__ CUtensorMap map_k, const __
     if (!alone) pdl_wait();
 }
 
-template <int R>
+template <int D, int R>
 static int launch_decode(lq_ctx* ctx, const PdArgs& g) {
-    constexpr int D = 128;
     const int page = 1 << g.s.page_shift;
     const uint64_t dims[4] = {(uint64_t)D, (uint64_t)page, (uint64_t)g.c.n_kv, (uint64_t)g.s.n_pages};
     const uint64_t strides[3] = {(uint64_t)D, (uint64_t)D * page, (uint64_t)g.c.page_stride};
     const uint32_t box[4] = {D, (uint32_t)std::min(page, PD_TILE), 1, 1};
+    const CUtensorMapSwizzle swz = D == 128 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_64B;
     CUtensorMap mk, mv;
-    int rc = make_tensor_map_4d(ctx, &mk, CU_TENSOR_MAP_DATA_TYPE_UINT8, g.c.k, dims, strides, box, CU_TENSOR_MAP_SWIZZLE_128B);
+    int rc = make_tensor_map_4d(ctx, &mk, CU_TENSOR_MAP_DATA_TYPE_UINT8, g.c.k, dims, strides, box, swz);
     if (rc) return rc;
-    rc = make_tensor_map_4d(ctx, &mv, CU_TENSOR_MAP_DATA_TYPE_UINT8, g.c.v, dims, strides, box, CU_TENSOR_MAP_SWIZZLE_128B);
+    rc = make_tensor_map_4d(ctx, &mv, CU_TENSOR_MAP_DATA_TYPE_UINT8, g.c.v, dims, strides, box, swz);
     if (rc) return rc;
-    const size_t smem = 1024 + PD_STAGES * PD_BYTES + 3 * 2 * R * 128 + sizeof(PdCtl<R>);
-    rc = ensure_func_smem(ctx, (const void*)prefix_attn_q8_decode_kernel<R>, smem);
+    const size_t smem = 1024 + pd_stages(D) * PD_TILE * D + 3 * 2 * R * 128 + sizeof(PdCtl<R>);
+    rc = ensure_func_smem(ctx, (const void*)prefix_attn_q8_decode_kernel<D, R>, smem);
     if (rc) return rc;
-    return launch_kernel(ctx, prefix_attn_q8_decode_kernel<R>, dim3((unsigned)g.p.workers), dim3(PD_THREADS), smem,
+    return launch_kernel(ctx, prefix_attn_q8_decode_kernel<D, R>, dim3((unsigned)g.p.workers), dim3(PD_THREADS), smem,
                          "prefix_attn_q8_decode", mk, mv, g);
 }
 
-int prefix_attn_q8_decode_ctas(int rows) { return pd_ctas(rows <= 8 ? 8 : 16); }
-
-int launch_prefix_attn_q8_decode(lq_ctx* ctx, const PrefixAttnArgs& a, const PagedSeqs& s, const PagedQ8& c, const PrefixPlan& p) {
+int launch_prefix_attn_q8_decode(lq_ctx* ctx, const PrefixAttnArgs& a, const PagedSeqs& s, const PagedQ8& c, const PrefixPlan& p, int D) {
     const PdArgs g{a, s, p, c};
-    return p.pb == 8 ? launch_decode<8>(ctx, g) : launch_decode<16>(ctx, g);
+    if (D == 64) return p.pb == 8 ? launch_decode<64, 8>(ctx, g) : launch_decode<64, 16>(ctx, g);
+    return p.pb == 8 ? launch_decode<128, 8>(ctx, g) : launch_decode<128, 16>(ctx, g);
 }
 
 }  // namespace lq

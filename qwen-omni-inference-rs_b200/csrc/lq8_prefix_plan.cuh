@@ -240,7 +240,7 @@ __host__ __device__ __forceinline__ HandOut hand_out(int f, bool first, bool liv
 // PREFIX_MAX_STEPS before the plan is used
 constexpr int64_t PREFIX_MAX_STEPS = 1ll << 26;
 constexpr int PREFIX_ATTN_F32_WARPS = 8;  // workers of a CTA of the f32 kernel
-constexpr int PREFIX_ATTN_Q8_WARPS = 8;  // and of the streaming one for 8-bit caches
+constexpr int PREFIX_ATTN_Q8_CTAS = 2;    // CTAs of the streaming kernel for 8-bit caches on an SM
 constexpr int PREFIX_ATTN_Q8_ROWS = 16;   // stacked rows of an item that it takes
 inline int64_t plan_cut(const PrefixAttnArgs& a, const PagedSeqs& s, bool f32, int sm_count, PrefixPlan* p, int warp_rows = 8,
                         int warps = PREFIX_ATTN_F32_WARPS, int warp_tile = 32) {

@@ -11,13 +11,11 @@ Tolerances, with u = 2^-8 the unit roundoff of a bf16 output (0 for f32):
 - attention with up to 16 stacked rows a kv head: q is rounded to amax / 65024 at most, which moves a
   score by at most d = c amax / 65024 sum |k| and a weight by a factor within e^(+-2d); f32 sums and
   exponentials stay within 2e-5 sum p |v| (the framework's tolerance for its f32 attention), the result
-  is rounded once, u |o|. Weights p, times V's scale s, are rounded too:
-  - head_dim 128: to whole 1 / 32512 parts of the largest p s of their 128 positions (the tiles begin at the
-    prefix's and at the own positions' first), half of that at most: codes are up to 127, so that a tile
-    gives at most 128 127 max(p s) / 65024; w is the sum of 128 127 max(p s) over the tiles;
-  - head_dim 64: to fp16, 2^-11, with the largest p s at 2^7 at least, so that half the smallest step,
-    2^-25, is 2^-32 of it: over n positions n 127 2^-32 max(p s), at most 2^-26 w for n up to 2^13;
-- attention, tensor-core kernel: q is exact, a weight is rounded to bf16 once, u sum p |v|; the rest as
+  is rounded once, u |o|. Weights p, times V's scale s, are rounded
+  to whole 1 / 32512 parts of the largest p s of their 128 positions (the tiles begin at the prefix's and
+  at the own positions' first), half of that at most: codes are up to 127, so that a tile gives at most
+  128 127 max(p s) / 65024; w is the sum of 128 127 max(p s) over the tiles;
+- attention with more: q is exact, a weight is rounded to bf16 once, u sum p |v|; the rest as
   above;
 - both: a weight below 2^-126 of the largest is zero in f32 (and flushed). Over up to 2^13 positions of
   |v| < 2^3 that is up to 2^-110, where the 64-bit result may be the like of 1e-116."""
@@ -425,9 +423,7 @@ def tolerance(want, streaming=True):
     o, a, d, w = want
     if not streaming:
         return 2.0 ** -110 + U * o.abs() + (U + 2e-5) * a
-    if o.shape[-1] == 128:
-        return 2.0 ** -110 + w / 65024 + U * o.abs() + (torch.expm1(2 * d) + 2e-5) * a
-    return 2.0 ** -110 + 2.0 ** -26 * w + U * o.abs() + (torch.expm1(2 * d) + 2.0 ** -11 + 2e-5) * a
+    return 2.0 ** -110 + w / 65024 + U * o.abs() + (torch.expm1(2 * d) + 2e-5) * a
 
 
 def attention_case(ctx, lq8_lib, kv, q, Hq, Hkv, D, page, block, prefix, seed=11, layers=1, qscale=1.0, quantized=False):
