@@ -79,24 +79,15 @@ prefix_attn_merge_kernel(const __grid_constant__ PrefixAttnArgs a, const __grid_
         }
         return lo < hi;
     };
-    int note = blockIdx.x;
-#pragma unroll 1
-    while (true) {
     if (!with_prefix) {
-        if (todo <= 0) {
-            if (note >= p.notes) break;
-            const SplitItem w = p.split[note];
-            note += gridDim.x;
-            own_in = blockIdx.y * MR;
-            st0 = w.row0 + own_in;
-            todo = min(MR, w.rows - own_in);
-            kh = w.kh;
-            own_item = w.item;
-            if (todo <= 0) continue;
-        }
-    } else if (todo <= 0) {
-        break;
+        const SplitItem w = p.split[blockIdx.x];
+        st0 = w.row0 + own_in;
+        todo = min(MR, w.rows - own_in);
+        kh = w.kh;
+        own_item = w.item;
     }
+#pragma unroll 1
+    while (todo > 0) {
         int run = todo, item[2] = {0, own_item}, in[2] = {0, own_in}, v0[2] = {0, 0}, cnt[2] = {0, 0};
         auto workers_of = [&](int k) {  // (within bounds, even where a kernel that gave up left them unwritten)
             const int most = (k ? p : pp).ranges - 1;
@@ -309,7 +300,7 @@ static int launch_merge(lq_ctx* ctx, const PrefixAttnArgs& a, const PagedSeqs& s
     // a row of few heads leaves most of a 32-row CTA idle
     const int mr = p.cap[1] <= 8 ? 8 : 32;
     const int64_t R = (int64_t)s.rows * a.group;
-    const dim3 grid((unsigned)(p.np > 0 ? a.n_kv * (R / p.ob + s.n_seqs) : p.streams ? std::min(p.notes, 8 * ctx->sm_count) : p.notes),
+    const dim3 grid((unsigned)(p.np > 0 ? a.n_kv * (R / p.ob + s.n_seqs) : p.notes),
                     (unsigned)ceil_div(p.cap[1], mr));
     const void* const func = mr == 8 ? (const void*)prefix_attn_merge_kernel<T, D, 8> : (const void*)prefix_attn_merge_kernel<T, D, 32>;
     const int rc = ensure_func_carveout(ctx, func);
@@ -361,7 +352,8 @@ static int attend_q8(lq_ctx* ctx, const PrefixAttnArgs& a, const PagedSeqs& s, c
     if (rc) return rc;
     if (pre == &tc && (rc = launch_prefix_attn_tc(ctx, a, s, tc, D, &c))) return rc;
     if (own == &st && (rc = launch_prefix_attn_q8_decode(ctx, a, s, c, st, D))) return rc;
-    return launch_merge<__nv_bfloat16, D>(ctx, a, s, *own, *pre);
+    return own->streams == 3 && own->np == 0 ? launch_prefix_attn_q8_join(ctx, a, *own, D)
+                                             : launch_merge<__nv_bfloat16, D>(ctx, a, s, *own, *pre);
 }
 
 // checks and arguments shared by the entry points; esize: bytes of an element of q and out. page_stride:

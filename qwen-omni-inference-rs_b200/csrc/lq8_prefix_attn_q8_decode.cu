@@ -622,7 +622,8 @@ prefix_attn_q8_decode_kernel(const __grid_constant__ CUtensorMap map_k, const __
                         if (lane == 0) {
                             if (tile == 0) p.first[part][item] = worker;
                             if (end == nt) p.last[part][item] = worker;
-                            if (a.prefix_len == 0 && tile == 0 && end < nt) p.split[worker] = SplitItem{n, row0, kh, item};
+                            if (a.prefix_len == 0 && tile == 0 && end < nt)
+                                p.split[worker] = SplitItem{n, row0, kh, line.owner(line.sp + step + nt - 1)};
                         }
                         PdSeg sg;
                         sg.t0 = tile, sg.t1 = end, sg.n = n, sg.flags = (own ? PD_OWN : 0) | (whole ? PD_WHOLE : 0);
@@ -773,6 +774,111 @@ prefix_attn_q8_decode_kernel(const __grid_constant__ CUtensorMap map_k, const __
         if (atomicAdd(p.claimed + 1, 1u) == gridDim.x - 1) p.claimed[0] = p.claimed[1] = 0;
     }
     if (!alone) pdl_wait();
+}
+
+// =========================================================================================
+// Joins the pieces of the own items that are cut, without a prefix: o = sum 2^(m_i - M) o_i /
+// sum 2^(m_i - M) l_i in the order of the line, M the largest m_i. The range that begins a cut item leaves a
+// note of it; a CTA takes some notes, the next one on its way meanwhile. A thread has four dims of a row
+// and asks for the first eight pieces' vectors together with their maxima and sums.
+// =========================================================================================
+constexpr int PD_PIECES = 64;  // pieces looked at together
+
+template <int D, int R>
+__global__ void __launch_bounds__(D / 4 * R, 1024 / (D / 4 * R)) prefix_attn_q8_join_kernel(const __grid_constant__ PrefixAttnArgs a, const __grid_constant__ PrefixPlan p) {
+    constexpr int CH = D / 4, THREADS = CH * R, AHEAD = 8;
+    __shared__ float2 ml[PD_PIECES][R];
+    __shared__ __align__(16) float stage[R][D + 4];
+    const int tid = threadIdx.x, r = tid % R, ch = tid / R, cap = p.cap[1];
+    pdl_wait();
+    pdl_trigger();
+    const int ranges = Shares(p, *p.own_steps).ranges;
+    SplitItem next{0, 0, 0, 0};
+    if (blockIdx.x < p.notes) next = p.split[blockIdx.x];
+#pragma unroll 1
+    for (int note = blockIdx.x; note < p.notes; note += gridDim.x) {
+        const SplitItem w = next;
+        if (note + gridDim.x < p.notes) next = p.split[note + gridDim.x];
+        if (w.rows <= 0) continue;
+        const int v1 = min(max(w.item, note), ranges - 1), n = v1 - note + 1;
+        auto slot = [&](int i) { return (int64_t)p.own_slot(0, note + i, i == 0); };
+        const float4* const po = reinterpret_cast<const float4*>(p.o[1]) + (int64_t)ch * cap + r;
+        const bool mine = r < w.rows;
+        float M = -INFINITY, L = 0.0f;
+        float4 o = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+#pragma unroll 1
+        for (int c0 = 0; c0 < n; c0 += PD_PIECES) {
+            const int m = min(PD_PIECES, n - c0);
+            float4 x[AHEAD];
+            auto ask = [&](int i0) {
+#pragma unroll
+                for (int j = 0; j < AHEAD; j++) {
+                    x[j] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+                    if (i0 + j < m && mine) x[j] = po[slot(c0 + i0 + j) * CH * cap];
+                }
+            };
+            ask(0);
+            __syncthreads();  // (the maxima and sums before these are read no more)
+            for (int i = tid; i < m * R; i += THREADS)
+                ml[i / R][i % R] = i % R < w.rows ? p.ml[1][slot(c0 + i / R) * cap + i % R] : make_float2(-INFINITY, 0.0f);
+            __syncthreads();
+            float up = M;
+            for (int i = 0; i < m; i++) up = fmaxf(up, ml[i][r].x);
+            if (up != -INFINITY) {
+                const float k = M == -INFINITY ? 0.0f : exp2f(M - up);
+                L *= k;
+                o.x *= k, o.y *= k, o.z *= k, o.w *= k;
+            }
+            M = up;
+#pragma unroll 1
+            for (int i0 = 0; i0 < m; i0 += AHEAD) {
+                if (i0 > 0) ask(i0);
+#pragma unroll
+                for (int j = 0; j < AHEAD; j++) {
+                    if (i0 + j >= m) break;
+                    const float2 y = ml[i0 + j][r];
+                    const float k = y.x == -INFINITY ? 0.0f : exp2f(y.x - M);
+                    L = fmaf(k, y.y, L);
+                    o.x = fmaf(k, x[j].x, o.x);
+                    o.y = fmaf(k, x[j].y, o.y);
+                    o.z = fmaf(k, x[j].z, o.z);
+                    o.w = fmaf(k, x[j].w, o.w);
+                }
+            }
+        }
+        const float inv = L > 0.0f ? 1.0f / L : L;  // a row that saw nothing: zeros; NaN stays
+        *reinterpret_cast<float4*>(&stage[r][4 * ch]) = make_float4(o.x * inv, o.y * inv, o.z * inv, o.w * inv);
+        __syncthreads();
+        // out, a row's dims side by side
+        {
+            const int rr = tid / CH, e = tid % CH * 4, st = w.row0 + min(rr, w.rows - 1), tok = a.group_div(st);
+            const bool on = rr < w.rows;
+            const float4 v = *reinterpret_cast<const float4*>(&stage[rr][e]);
+            const float y[4] = {v.x, v.y, v.z, v.w};
+            const int64_t col = (int64_t)(w.kh * a.group + st - tok * a.group) * D + e;
+            if (a.out && on)
+                *reinterpret_cast<uint2*>(static_cast<__nv_bfloat16*>(a.out) + (int64_t)tok * a.out_stride + col) =
+                    make_uint2(pack_bf16x2(y[0], y[1]), pack_bf16x2(y[2], y[3]));
+            if (a.xq) {
+                const int64_t at = (int64_t)tok * a.n_heads * D + col;
+                const uint32_t q = quant_group8(y, tid & 7, on ? a.xd + (at >> 5) : nullptr);
+                if (on) *reinterpret_cast<uint32_t*>(a.xq + at) = q;
+            }
+        }
+        __syncthreads();
+    }
+}
+
+template <int D, int R>
+static int launch_join(lq_ctx* ctx, const PrefixAttnArgs& a, const PrefixPlan& p) {
+    constexpr int THREADS = D / 4 * R;
+    return launch_kernel(ctx, prefix_attn_q8_join_kernel<D, R>, dim3((unsigned)std::min(p.notes, 1024 / THREADS * ctx->sm_count)), dim3(THREADS), 0,
+                         "prefix_attn_q8_join", a, p);
+}
+
+int launch_prefix_attn_q8_join(lq_ctx* ctx, const PrefixAttnArgs& a, const PrefixPlan& p, int D) {
+    if (D == 64) return p.pb == 8 ? launch_join<64, 8>(ctx, a, p) : launch_join<64, 16>(ctx, a, p);
+    return p.pb == 8 ? launch_join<128, 8>(ctx, a, p) : launch_join<128, 16>(ctx, a, p);
 }
 
 template <int D, int R>

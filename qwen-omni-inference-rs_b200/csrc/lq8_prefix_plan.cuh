@@ -43,7 +43,8 @@ struct PrefixAttnArgs {
 // an own item that is cut between workers
 struct SplitItem {
     int rows;      // rows of its block (0: none)
-    int row0, kh, item;
+    int row0, kh;
+    int item;      // (streaming kernel: the last range that has a piece of it)
 };
 
 struct PrefixPlan {
@@ -181,8 +182,8 @@ __host__ __device__ __forceinline__ void flow_range(const Line& l, bool paired, 
 }
 
 // The line of a streaming kernel, prefix items first, cut into ranges that its workers take in turn: with
-// n workers and 16 steps for each, n ranges with half of the line, n with a quarter, n with three twentieths
-// and 2 n with the rest, else n equal ones. A worker may begin late (an SM that still holds another kernel's shared
+// n workers and 20 steps for each, n ranges with half of the line, n with a quarter, n with three twentieths
+// and 2 n with the rest, else n equal ones, or one for each step; none is empty. A worker may begin late (an SM that still holds another kernel's shared
 // memory took its third CTA 80 us late, and a fixed share for each ended 25 us after all others), and
 // memory serves some SMs faster than others. Which worker takes a range changes no result.
 struct Shares {
@@ -191,7 +192,8 @@ struct Shares {
     uint64_t mul;  // ceil(2^40 / n)
     __host__ __device__ __forceinline__ Shares(const PrefixPlan& p, int own_steps)
         : n(p.workers), sp(p.sp), total(p.sp + own_steps), ranges(n), size{total, 0, 0, 0}, mul(p.workers_mul) {
-        if (p.chunks > 0 && total >= 16 * n) {
+        if (total < n) ranges = total;
+        if (p.chunks > 0 && total >= 20 * n) {
             size[3] = total / 10;
             size[2] = total / 20 * 3;
             size[1] = total / 4;
@@ -206,10 +208,21 @@ struct Shares {
     }
     // the first step of range c <= ranges
     __host__ __device__ __forceinline__ int start(int c) const {
+        if (total < n) return c;
         if (c <= n) return part(size[0], c);
         if (c <= 2 * n) return size[0] + part(size[1], c - n);
         if (c <= 3 * n) return size[0] + size[1] + part(size[2], c - 2 * n);
         return size[0] + size[1] + size[2] + (part(size[3], c - 3 * n) >> 1);
+    }
+    // the range that has step x
+    __host__ __device__ __forceinline__ int owner(int x) const {
+        int lo = 0, hi = ranges;  // start(lo) <= x < start(hi)
+        while (hi - lo > 1) {
+            const int mid = (lo + hi) >> 1;
+            if (start(mid) <= x) lo = mid;
+            else hi = mid;
+        }
+        return lo;
     }
     // its steps of the prefix or of the own items
     __host__ __device__ __forceinline__ void range(int c, bool own, int& lo, int& hi) const {
