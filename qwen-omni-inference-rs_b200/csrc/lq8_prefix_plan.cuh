@@ -254,7 +254,11 @@ __host__ __device__ __forceinline__ HandOut hand_out(int f, bool first, bool liv
 constexpr int64_t PREFIX_MAX_STEPS = 1ll << 26;
 constexpr int PREFIX_ATTN_F32_WARPS = 8;  // workers of a CTA of the f32 kernel
 constexpr int PREFIX_ATTN_Q8_CTAS = 2;    // CTAs of the streaming kernel for 8-bit caches on an SM
-constexpr int PREFIX_ATTN_Q8_ROWS = 16;   // stacked rows of an item that it takes
+// Up to so many stacked rows the streaming kernel takes a part of the line, in blocks of 8 or 16, else the one
+// for tiles of 128 rows. 16 sequences of up to 8000 positions, 64 / 8 heads: 24 rows 41 and 61 us, 32
+// rows 43 and 60, 48 rows 86 and 61; 32 rows in all behind 32768 positions 49 and 63, behind 4096 27 and 38, 64
+// rows behind 32768 119 and 68.
+constexpr int PREFIX_ATTN_Q8_ROWS = 32;
 inline int64_t plan_cut(const PrefixAttnArgs& a, const PagedSeqs& s, bool f32, int sm_count, PrefixPlan* p, int warp_rows = 8,
                         int warps = PREFIX_ATTN_F32_WARPS, int warp_tile = 32) {
     const int64_t R = (int64_t)s.rows * a.group, most_q = std::min<int64_t>((int64_t)a.max_q, s.rows) * a.group;
