@@ -40,6 +40,8 @@
 #include "lq8_tcgen05.cuh"
 #include "lq8_tma.cuh"
 
+#include <cuda_fp16.h>
+
 #include <algorithm>
 #include <type_traits>
 
@@ -86,6 +88,7 @@ struct PaCtl {
     uint64_t raw_full[pa_raw(64)], raw_empty[pa_raw(64)], sc_full[2][PA_SCALES], sc_empty[2][PA_SCALES];
     alignas(16) float sc[2][PA_SCALES][2][8];
     int raw_end;    // the tile after the last one
+    int raw_v[pa_raw(64)];  // 1: V
     uint32_t tmem;
     int abort;
     int issued;     // copies that the producer started
@@ -98,9 +101,9 @@ struct PaCtl {
     int scan[PA_SCAN + 1];  // own steps before each entry
 };
 
-// D f32, A and B bf16, M 128, N n; B MN-major or K-major
-__host__ __device__ constexpr uint32_t pa_idesc(int n, int b_mn) {
-    return (1u << 4) | (1u << 7) | (1u << 10) | ((uint32_t)b_mn << 16) | ((uint32_t)(n >> 3) << 17) | (8u << 24);
+// D f32, A and B bf16 or fp16, M 128, N n; B MN-major or K-major
+__host__ __device__ constexpr uint32_t pa_idesc(int n, int b_mn, bool bf16 = true) {
+    return (1u << 4) | (bf16 ? (1u << 7) | (1u << 10) : 0u) | ((uint32_t)b_mn << 16) | ((uint32_t)(n >> 3) << 17) | (8u << 24);
 }
 __device__ __forceinline__ void mma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t acc) {
     asm volatile(
@@ -190,6 +193,24 @@ __device__ __forceinline__ uint32_t codes_bf16(uint32_t w, uint32_t sel) {
     const uint32_t x = __byte_perm(w, 0x43434343u, sel), lo = x & 0xff7fff7fu, up = x & 0xff80ff80u;
     const __nv_bfloat162 d = __hsub2(*reinterpret_cast<const __nv_bfloat162*>(&lo), *reinterpret_cast<const __nv_bfloat162*>(&up));
     return *reinterpret_cast<const uint32_t*>(&d);
+}
+
+// two bytes of w, which are codes + 128, as a pair of fp16: 0x6400 + b has the value 1024 + b; less 1152 that is
+// the code, exactly
+__device__ __forceinline__ uint32_t codes_f16(uint32_t w, uint32_t sel) {
+    const uint32_t x = __byte_perm(w, 0x64646464u, sel), bias = 0x64806480u;
+    const __half2 d = __hsub2(*reinterpret_cast<const __half2*>(&x), *reinterpret_cast<const __half2*>(&bias));
+    return *reinterpret_cast<const uint32_t*>(&d);
+}
+// P: bf16, or fp16 next to V's codes
+template <bool F16>
+__device__ __forceinline__ uint32_t pa_pack(float a, float b) {
+    if constexpr (F16) {
+        const __half2 h = __floats2half2_rn(a, b);
+        return *reinterpret_cast<const uint32_t*>(&h);
+    } else {
+        return pack_bf16x2(a, b);
+    }
 }
 
 // PP, PO: blocks of the prefix / of a sequence's own rows are two halves of 128 rows that share
@@ -326,6 +347,9 @@ prefix_attn_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_co
         const uint32_t t_s = tmem + t_lane + f * 128, t_o = tmem + t_lane + 256 + f * 128;
         const float cs = g.a.scale * 1.44269504088896340736f;  // scores in units of log2
         unsigned s_ph = 0, o_ph = 0, turn = 0;
+        // 8-bit caches: m is the running maximum of scores + log2 V's scale, and P is 2^7 times as large as that
+        // says, between 2^7 and 2^15 where it counts: fp16 rounds it by 2^-12
+        constexpr float BIAS = Q8 ? 7.0f : 0.0f;
         [[maybe_unused]] int sc_slot = 0;  // 8-bit caches: the round's scales
         [[maybe_unused]] unsigned sc_ph = 0;
         int joint = 0;  // segments of few rows
@@ -424,7 +448,7 @@ prefix_attn_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_co
                                 tmem_st16(t_o + i, r);
                             }
                         }
-                        return m == -INFINITY ? 0.0f : -m;
+                        return m == -INFINITY ? 0.0f : BIAS - m;
                     };
                     if (few) {
                         // warp w takes columns 32 w .. 32 w + 31 of its own copy of the rows, with
@@ -446,7 +470,8 @@ prefix_attn_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_co
                                 float mh = max_nan(s[16 * h], s[16 * h + 1]);
 #pragma unroll
                                 for (int i = 2; i < 16; i += 2) mh = max3(mh, s[16 * h + i], s[16 * h + i + 1]);
-                                mt = h ? max_nan(mt, mh * kc[1]) : mh * kc[0];
+                                mh = fmaf(mh, kc[h], of(v_add, 2 * wq + h));
+                                mt = h ? max_nan(mt, mh) : mh;
                             }
                         } else {
                             float mx[4] = {s[0], s[1], s[2], s[3]};
@@ -465,7 +490,7 @@ prefix_attn_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_co
                             const float2 x = __ffma2_rn(make_float2(s[2 * i], s[2 * i + 1]), make_float2(kc[i / 8], kc[i / 8]), make_float2(add, add));
                             const float2 e = make_float2(ex2(x.x), ex2(x.y));
                             sum = __fadd2_rn(sum, e);
-                            pk[i] = pack_bf16x2(e.x, e.y);
+                            pk[i] = pa_pack<Q8>(e.x, e.y);
                             if (Q8 && i % 8 == 7) {
                                 l = fmaf(sum.x + sum.y, of(v_per, 2 * wq + i / 8), l);
                                 sum = make_float2(0.0f, 0.0f);
@@ -495,7 +520,7 @@ prefix_attn_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_co
                                 float mh = max_nan(s[16 * h], s[16 * h + 1]);
 #pragma unroll
                                 for (int i = 2; i < 16; i += 2) mh = max3(mh, s[16 * h + i], s[16 * h + i + 1]);
-                                mt = max_nan(mt, mh * of(k_mul, h));
+                                mt = max_nan(mt, fmaf(mh, of(k_mul, h), of(v_add, h)));
                             }
                         } else {
                             float mx[4] = {s[0], s[1], s[2], s[3]};
@@ -522,7 +547,7 @@ prefix_attn_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_co
                                 const float2 x = __ffma2_rn(make_float2(s[32 * j + 2 * i], s[32 * j + 2 * i + 1]), cs2, neg2);
                                 const float2 e = make_float2(ex2(x.x), ex2(x.y));
                                 sum[i & 1] = __fadd2_rn(sum[i & 1], e);
-                                pk[i] = pack_bf16x2(e.x, e.y);
+                                pk[i] = pa_pack<Q8>(e.x, e.y);
                                 if constexpr (Q8)
                                     if (i % 8 == 7) {
                                         l = fmaf((sum[0].x + sum[0].y) + (sum[1].x + sum[1].y), of(v_per, 2 * j + i / 8), l);
@@ -565,7 +590,7 @@ prefix_attn_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_co
                                             float mh = max_nan(s[16 * h], s[16 * h + 1]);
 #pragma unroll
                                             for (int i = 2; i < 16; i += 2) mh = max3(mh, s[16 * h + i], s[16 * h + i + 1]);
-                                            mt = max_nan(mt, mh * kc[h]);
+                                            mt = max_nan(mt, fmaf(mh, kc[h], of(v_add, j / 16 + h)));
                                         }
                                     } else {
 #pragma unroll
@@ -578,7 +603,7 @@ prefix_attn_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_co
                                         const float p0 = ex2(fmaf(s[2 * i], kc[i / 8], add[i / 8])), p1 = ex2(fmaf(s[2 * i + 1], kc[i / 8], add[i / 8]));
                                         if constexpr (Q8) sum = fmaf(p0 + p1, per[i / 8], sum);
                                         else sum += p0 + p1;
-                                        pk[i] = pack_bf16x2(p0, p1);
+                                        pk[i] = pa_pack<Q8>(p0, p1);
                                     }
                                     // P of columns j.. lands on S columns j/2.., which have been read
                                     tmem_st16(t_s + j / 2, pk);
@@ -637,7 +662,7 @@ prefix_attn_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_co
                     if (ml.x != -INFINITY) L += ml.y * ex2(ml.x - M);
                 }
                 const float k = m == -INFINITY ? 0.0f : ex2(m - M) * (whole ? (L > 0.0f ? 1.0f / L : L) : 1.0f);
-                if (mine && wq == 0 && !whole) g.p.ml[own][(int64_t)sg.slot * cap + half + lane] = make_float2(M, L);
+                if (mine && wq == 0 && !whole) g.p.ml[own][(int64_t)sg.slot * cap + half + lane] = make_float2(M - BIAS, L);
                 const int r = row >> 4, e = (row & 15) * 2;  // two dims of a row to write
                 const int st_r = sg.row0 + min(r, sg.n - 1), tok_r = g.a.group_div(st_r);
 #pragma unroll 1
@@ -676,7 +701,7 @@ prefix_attn_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_co
             }
             const float inv = l > 0.0f ? 1.0f / l : 0.0f;
             const int at_o = half + row;
-            if (mine && !whole) g.p.ml[own][(int64_t)sg.slot * cap + at_o] = make_float2(m, l);
+            if (mine && !whole) g.p.ml[own][(int64_t)sg.slot * cap + at_o] = make_float2(m - BIAS, l);
             // four dims of all rows lie together, so that a warp's stores are 512 bytes each
             float4* po = reinterpret_cast<float4*>(g.p.o[own]) + (int64_t)sg.slot * (D / 4) * cap + at_o;
 #pragma unroll 1
@@ -727,6 +752,8 @@ prefix_attn_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_co
                     uint64_t* const there = Q8 ? &c.raw_full[slot] : &c.full[slot];
                     ok = pa_wait_warp(c, Q8 ? &c.raw_empty[slot] : &c.empty[slot], ph ^ 1u);
                     if (!ok) break;
+                    if constexpr (Q8)
+                        if (lane == 0) c.raw_v[slot] = which == 0;
                     if (lane == 0) mbar_expect_tx(there, Q8 ? RAW_BYTES : KV_BYTES);
                     __syncwarp();
                     const CUtensorMap* const map = which ? &map_k : &map_v;
@@ -808,7 +835,7 @@ prefix_attn_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_co
     } else if (warp == 9) {
         // ------------------------------ MMA issuer ------------------------------
         asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(PA_REGS_LOW));
-        constexpr uint32_t id_qk = pa_idesc(PA_TILE, 0), id_pv = pa_idesc(D, 1);
+        constexpr uint32_t id_qk = pa_idesc(PA_TILE, 0), id_pv = pa_idesc(D, 1, !Q8);
         int slot = 0, k_slot = 0, v_slot = 0;
         unsigned ph = 0;
         bool ok = true, both = false;  // both: this round's K is for the second flow too
@@ -1101,27 +1128,37 @@ prefix_attn_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_co
                 const uint8_t* const src = codes + rs * RAW_BYTES;
                 uint8_t* const dst = ring + slot * KV_BYTES;
                 const int w = warp - 12, q = lane >> 3, l = lane & 7;
+                auto convert = [&](auto to_f16) {
 #pragma unroll
-                for (int i = 0; i < D / 16; i++) {
-                    // vector v (16 dims) of row r
-                    int r, v;
-                    if constexpr (D == 128) {
-                        const int k = 4 * i + q, pair = k & 3;   // 32 rows a warp: 8 groups of 4 positions' pairs ...
-                        r = 32 * w + 8 * (i >> 1) + (l < 4 ? pair : pair ^ 5);
-                        v = (l & 3) + 4 * (i & 1);
-                    } else {
-                        r = 32 * w + 8 * i + 2 * q + (l >> 2);
-                        v = l & 3;
+                    for (int i = 0; i < D / 16; i++) {
+                        // vector v (16 dims) of row r
+                        int r, v;
+                        if constexpr (D == 128) {
+                            const int k = 4 * i + q, pair = k & 3;   // 32 rows a warp: 8 groups of 4 positions' pairs ...
+                            r = 32 * w + 8 * (i >> 1) + (l < 4 ? pair : pair ^ 5);
+                            v = (l & 3) + 4 * (i & 1);
+                        } else {
+                            r = 32 * w + 8 * i + 2 * q + (l >> 2);
+                            v = l & 3;
+                        }
+                        const uint4 u = *reinterpret_cast<const uint4*>(src + (D == 128 ? r * 128 + ((v ^ (r & 7)) << 4) : r * 64 + v * 16));
+                        const uint32_t x[4] = {u.x, u.y, u.z, u.w};
+                        uint8_t* const to = dst + (v >> 2) * HALF + r * 128;
+#pragma unroll
+                        for (int j = 0; j < 2; j++) {
+                            uint4* const vec = reinterpret_cast<uint4*>(to + (((2 * (v & 3) + j) ^ (r & 7)) << 4));
+                            if constexpr (decltype(to_f16)::value) {  // V, next to P
+                                const uint32_t y0 = x[2 * j] ^ 0x80808080u, y1 = x[2 * j + 1] ^ 0x80808080u;
+                                *vec = make_uint4(codes_f16(y0, 0x4140), codes_f16(y0, 0x4342), codes_f16(y1, 0x4140), codes_f16(y1, 0x4342));
+                            } else {  // K, next to Q
+                                *vec = make_uint4(codes_bf16(x[2 * j], 0x4140), codes_bf16(x[2 * j], 0x4342),
+                                                  codes_bf16(x[2 * j + 1], 0x4140), codes_bf16(x[2 * j + 1], 0x4342));
+                            }
+                        }
                     }
-                    const uint4 u = *reinterpret_cast<const uint4*>(src + (D == 128 ? r * 128 + ((v ^ (r & 7)) << 4) : r * 64 + v * 16));
-                    const uint32_t x[4] = {u.x, u.y, u.z, u.w};
-                    uint8_t* const to = dst + (v >> 2) * HALF + r * 128;
-#pragma unroll
-                    for (int j = 0; j < 2; j++)
-                        *reinterpret_cast<uint4*>(to + (((2 * (v & 3) + j) ^ (r & 7)) << 4)) =
-                            make_uint4(codes_bf16(x[2 * j], 0x4140), codes_bf16(x[2 * j], 0x4342),
-                                       codes_bf16(x[2 * j + 1], 0x4140), codes_bf16(x[2 * j + 1], 0x4342));
-                }
+                };
+                if (c.raw_v[rs]) convert(std::true_type{});
+                else convert(std::false_type{});
                 proxy_fence();
                 __syncwarp();
                 if (lane == 0) {
