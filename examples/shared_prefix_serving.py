@@ -82,14 +82,19 @@ class Weights:
 
 class PagedDecoder:
     """A batch behind a shared prompt. cache_dtype float32 keeps the model runner's numerics
-    (norm_bf16: its rounding points); bfloat16 halves the cache."""
+    (norm_bf16: its rounding points); bfloat16 halves the cache, int8 (codes, a scale for each page and kv
+    head) halves it again."""
 
     def __init__(self, weights, rotary, n_pages, cache_dtype=torch.float32):
         self.w, self.rotary = weights, rotary
         c = weights.cfg
         # every layer's pages in one allocation, page by page: [2, pages, layers, kv heads, page, dim]
         buf = torch.zeros((2, n_pages, c.layers, c.n_kv_heads, PAGE, c.head_dim), dtype=cache_dtype, device="cuda")
-        self.caches = [lq8.PagedKvCache(weights.ctx, buf[0][:, i], buf[1][:, i]) for i in range(c.layers)]
+        if cache_dtype == torch.int8:
+            scales = torch.zeros((2, n_pages, c.layers, c.n_kv_heads, 1), device="cuda")
+            self.caches = [lq8.PagedKvCacheQ8(weights.ctx, *(t[j][:, i] for t in (buf, scales) for j in (0, 1))) for i in range(c.layers)]
+        else:
+            self.caches = [lq8.PagedKvCache(weights.ctx, buf[0][:, i], buf[1][:, i]) for i in range(c.layers)]
         self.free = list(range(n_pages))[::-1]
         self.prefix_table, self.prefix_len = None, 0
 
@@ -217,7 +222,7 @@ def serve(cache_dtype=torch.float32, image=True, steps=6, seed=7, ctx=None):
 
 
 def main():
-    for dtype in (torch.float32, torch.bfloat16):
+    for dtype in (torch.float32, torch.bfloat16, torch.int8):
         for image in (True, False):
             t0 = time.time()
             got, want, runner = serve(dtype, image)
