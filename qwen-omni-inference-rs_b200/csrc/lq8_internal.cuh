@@ -84,9 +84,6 @@ int consume_device_error(lq_ctx* ctx, const char* what);
 // cudaFuncSetAttribute(MaxDynamicSharedMemorySize) for `func` on ctx->device, once per
 // (function, device) and again only when a launch needs more than was set before
 int ensure_func_smem(lq_ctx* ctx, const void* func, size_t bytes);
-// cudaFuncAttributePreferredSharedMemoryCarveout = all of it, once per (function, device): an SM that
-// runs such a kernel need not go idle before one with large shared memory can follow
-int ensure_func_carveout(lq_ctx* ctx, const void* func);
 
 }  // namespace lq
 

@@ -302,9 +302,6 @@ static int launch_merge(lq_ctx* ctx, const PrefixAttnArgs& a, const PagedSeqs& s
     const int64_t R = (int64_t)s.rows * a.group;
     const dim3 grid((unsigned)(p.np > 0 ? a.n_kv * (R / p.ob + s.n_seqs) : p.notes),
                     (unsigned)ceil_div(p.cap[1], mr));
-    const void* const func = mr == 8 ? (const void*)prefix_attn_merge_kernel<T, D, 8> : (const void*)prefix_attn_merge_kernel<T, D, 32>;
-    const int rc = ensure_func_carveout(ctx, func);
-    if (rc) return rc;
     return mr == 8 ? launch_kernel(ctx, prefix_attn_merge_kernel<T, D, 8>, grid, dim3(256), 0, "prefix_attn_merge", a, s, p, pp)
                    : launch_kernel(ctx, prefix_attn_merge_kernel<T, D, 32>, grid, dim3(256), 0, "prefix_attn_merge", a, s, p, pp);
 }
@@ -352,7 +349,7 @@ static int attend_q8(lq_ctx* ctx, const PrefixAttnArgs& a, const PagedSeqs& s, c
     if (rc) return rc;
     if (pre == &tc && (rc = launch_prefix_attn_tc(ctx, a, s, tc, D, &c))) return rc;
     if (own == &st && (rc = launch_prefix_attn_q8_decode(ctx, a, s, c, st, D))) return rc;
-    return own->streams == 3 && own->np == 0 ? launch_prefix_attn_q8_join(ctx, a, *own, D)
+    return own->streams == 3 && own->np == 0 ? launch_prefix_attn_q8_join(ctx, a, s, *own, D)
                                              : launch_merge<__nv_bfloat16, D>(ctx, a, s, *own, *pre);
 }
 

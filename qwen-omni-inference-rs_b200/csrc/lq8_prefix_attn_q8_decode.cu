@@ -1,9 +1,9 @@
-// lq8_prefix_attn_q8_decode.cu -- the shared-prefix attention for 8-bit caches with up to 16 stacked rows
-// a kv head (a decode step): codes go from memory into int8 products on tcgen05 as they are, and no
-// thread ever touches one.
+// lq8_prefix_attn_q8_decode.cu -- the shared-prefix attention for 8-bit caches with few stacked rows a kv
+// head (PREFIX_ATTN_Q8_ROWS; decode steps): codes go from memory into int8 products on tcgen05 as they
+// are, and no thread ever touches one.
 //
-// A CTA walks its share of the line of steps (Shares in lq8_prefix_plan.cuh), 128 positions each; three
-// CTAs fit on an SM (two with 16 rows) and hide each other's latency. With R = 8 or 16 rows:
+// CTAs, two to an SM, which hide each other's latency, claim ranges of the line of steps (Shares in
+// lq8_prefix_plan.cuh), 128 positions a step. With blocks of R = 8 or 16 rows:
 //   S^T = K Q^T   kind::i8, M 128 positions, N 2 R, K 128 dims: a row of Q is rounded to 16 bits of its
 //                 largest value (within amax / 65024) and split into two bytes, which are two
 //                 columns; 256 high + low is exact in 32 bits. K's tile as TMA brings it.
@@ -22,6 +22,13 @@
 // and brings tiles page by page (128-byte swizzle; pages past the end come as zeros); warp 5: TMEM
 // allocator and MMA issuer. Every wait is bounded by a number of polls; when one runs out all warps of the CTA
 // leave, its copies and MMAs in flight are waited for, and the error flag is set.
+// Bound: HBM with long sequences, else the latency of a tile (0.75 to 1.2 us from its bytes' arrival to O) and
+// of a segment's start. 64 sequences of up to 8000 positions, 64 / 8 heads of 128 dims: 88 us of the 106 us
+// of a call (530 MB, 6.0 TB/s, 92 % of a plain copy), the rest joins cut items; 48 of up to 4000 with 8 heads
+// of 64 dims and no group: 26 us (the bytes: 7.5); 16 sequences of 4 rows with up to 8000 positions: 43 us,
+// where tiles of 128 rows take 61. A kernel of warps that multiplied with mma.sync took 113 us for the
+// first of these.
+//
 // TMA loads here read only this GPU's memory and use no multicast.
 #include "lq8_async.cuh"
 #include "lq8_fused.cuh"
@@ -397,7 +404,7 @@ prefix_attn_q8_decode_kernel(const __grid_constant__ CUtensorMap map_k, const __
             };
 #pragma unroll 1
             for (int t = sg.t0; t < sg.t1; t++, n_tile++) {
-                const float k1 = ks, v1 = vs > 0.0f || vs != vs ? vs : 8.6736e-19f;  // (codes of a scale of zero are zero)
+                const float k1 = ks, v1 = max_nan(vs, PREFIX_ATTN_Q8_LEAST);
                 const float lv = __log2f(v1), per = __frcp_rn(v1);
                 id_next = id_then;
                 id_then = page_at(sg, t + 2);
@@ -785,7 +792,7 @@ prefix_attn_q8_decode_kernel(const __grid_constant__ CUtensorMap map_k, const __
 constexpr int PD_PIECES = 64;  // pieces looked at together
 
 template <int D, int R>
-__global__ void __launch_bounds__(D / 4 * R, 1024 / (D / 4 * R)) prefix_attn_q8_join_kernel(const __grid_constant__ PrefixAttnArgs a, const __grid_constant__ PrefixPlan p) {
+__global__ void __launch_bounds__(D / 4 * R, 1024 / (D / 4 * R)) prefix_attn_q8_join_kernel(const __grid_constant__ PrefixAttnArgs a, const __grid_constant__ PrefixPlan p, int stacked) {
     constexpr int CH = D / 4, THREADS = CH * R, AHEAD = 8;
     __shared__ float2 ml[PD_PIECES][R];
     __shared__ __align__(16) float stage[R][D + 4];
@@ -799,7 +806,8 @@ __global__ void __launch_bounds__(D / 4 * R, 1024 / (D / 4 * R)) prefix_attn_q8_
     for (int note = blockIdx.x; note < p.notes; note += gridDim.x) {
         const SplitItem w = next;
         if (note + gridDim.x < p.notes) next = p.split[note + gridDim.x];
-        if (w.rows <= 0) continue;
+        // (a kernel that gave up, or lengths that changed under it, may have left notes unwritten)
+        if (w.rows <= 0 || w.rows > cap || w.row0 < 0 || w.row0 > stacked - w.rows || (unsigned)w.kh >= (unsigned)a.n_kv) continue;
         const int v1 = min(max(w.item, note), ranges - 1), n = v1 - note + 1;
         auto slot = [&](int i) { return (int64_t)p.own_slot(0, note + i, i == 0); };
         const float4* const po = reinterpret_cast<const float4*>(p.o[1]) + (int64_t)ch * cap + r;
@@ -870,15 +878,16 @@ __global__ void __launch_bounds__(D / 4 * R, 1024 / (D / 4 * R)) prefix_attn_q8_
 }
 
 template <int D, int R>
-static int launch_join(lq_ctx* ctx, const PrefixAttnArgs& a, const PrefixPlan& p) {
+static int launch_join(lq_ctx* ctx, const PrefixAttnArgs& a, const PrefixPlan& p, int stacked) {
     constexpr int THREADS = D / 4 * R;
     return launch_kernel(ctx, prefix_attn_q8_join_kernel<D, R>, dim3((unsigned)std::min(p.notes, 1024 / THREADS * ctx->sm_count)), dim3(THREADS), 0,
-                         "prefix_attn_q8_join", a, p);
+                         "prefix_attn_q8_join", a, p, stacked);
 }
 
-int launch_prefix_attn_q8_join(lq_ctx* ctx, const PrefixAttnArgs& a, const PrefixPlan& p, int D) {
-    if (D == 64) return p.pb == 8 ? launch_join<64, 8>(ctx, a, p) : launch_join<64, 16>(ctx, a, p);
-    return p.pb == 8 ? launch_join<128, 8>(ctx, a, p) : launch_join<128, 16>(ctx, a, p);
+int launch_prefix_attn_q8_join(lq_ctx* ctx, const PrefixAttnArgs& a, const PagedSeqs& s, const PrefixPlan& p, int D) {
+    const int stacked = s.rows * a.group;  // (below 2^28)
+    if (D == 64) return p.pb == 8 ? launch_join<64, 8>(ctx, a, p, stacked) : launch_join<64, 16>(ctx, a, p, stacked);
+    return p.pb == 8 ? launch_join<128, 8>(ctx, a, p, stacked) : launch_join<128, 16>(ctx, a, p, stacked);
 }
 
 template <int D, int R>

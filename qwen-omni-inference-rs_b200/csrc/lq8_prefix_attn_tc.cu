@@ -54,7 +54,7 @@ constexpr int pa_stages(int D, bool q8 = false) { return q8 ? D == 64 ? 7 : 3 : 
 // 8-bit caches: tiles of codes (16 and 8 KB) on their way into the ring
 constexpr int pa_raw(int D) { return D == 64 ? 5 : 2; }
 constexpr int PA_SCALES = 4;      // rounds of a flow whose scales are kept
-// warps 0-7 softmax, 8 TMA, 9 MMA, 10 scheduler, 11 empty rows, 12-15 (8-bit caches) codes to bf16
+// warps 0-7 softmax, 8 TMA, 9 MMA, 10 scheduler, 11 empty rows, 12-15 (8-bit caches) codes to 16 bits
 constexpr int pa_threads(bool q8) { return q8 ? 512 : 384; }
 // registers: 384 x 168 at launch = 256 x 216 for the softmax warps + 128 x 72 for the others;
 // 512 x 128 = 256 x 184 + 256 x 72
@@ -408,14 +408,13 @@ prefix_attn_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_co
 #pragma unroll 1
             for (; t < sg.t1; t++) {
                 // 8-bit caches, lane i: the scales of the i-th 16 positions. K's in units of log2 (never so small
-                // that a masked score loses its minus infinity); V's as what a score gets on top and what a
-                // weight then counts for in l (codes of a scale of zero are zero: any other does)
+                // that a masked score loses its minus infinity); V's, no smaller than PREFIX_ATTN_Q8_LEAST,
+                // as what a score gets on top and what a weight then counts for in l
                 [[maybe_unused]] float k_mul = 0.0f, v_add = 0.0f, v_per = 0.0f;
                 if constexpr (Q8) {
                     if (!pa_wait(c, &c.sc_full[f][sc_slot], sc_ph)) break;
                     k_mul = max_nan(c.sc[f][sc_slot][0][lane & 7] * cs, 1e-37f);
-                    float v = c.sc[f][sc_slot][1][lane & 7];
-                    v = v > 0.0f || v != v ? v : 8.6736e-19f;
+                    const float v = max_nan(c.sc[f][sc_slot][1][lane & 7], PREFIX_ATTN_Q8_LEAST);
                     v_add = __log2f(v);
                     v_per = __frcp_rn(v);
                     __syncwarp();
@@ -1112,7 +1111,7 @@ prefix_attn_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_co
             o.flags = SEG_END;
             if (ok) put(o, hl == 0);
         } else if (Q8 && warp >= 12) {
-            // ------------------------------ codes to bf16 ------------------------------
+            // ------------------------------ codes to 16 bits ------------------------------
             // A quarter warp reads 16 bytes a lane of two positions of opposite parity (r and r ^ 5, with
             // D = 64 r and r + 1) and writes their two vectors of 8 dims each: under the swizzle both
             // touch every bank once.
@@ -1134,8 +1133,7 @@ prefix_attn_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_co
                         // vector v (16 dims) of row r
                         int r, v;
                         if constexpr (D == 128) {
-                            const int k = 4 * i + q, pair = k & 3;   // 32 rows a warp: 8 groups of 4 positions' pairs ...
-                            r = 32 * w + 8 * (i >> 1) + (l < 4 ? pair : pair ^ 5);
+                            r = 32 * w + 8 * (i >> 1) + (l < 4 ? q : q ^ 5);
                             v = (l & 3) + 4 * (i & 1);
                         } else {
                             r = 32 * w + 8 * i + 2 * q + (l >> 2);

@@ -228,17 +228,6 @@ int ensure_func_smem(lq_ctx* ctx, const void* func, size_t bytes) {
     return LQ_OK;
 }
 
-int ensure_func_carveout(lq_ctx* ctx, const void* func) {
-    static std::mutex mu;
-    static std::map<std::pair<const void*, int>, bool> done;
-    std::lock_guard<std::mutex> lock(mu);
-    bool& have = done[std::make_pair(func, ctx->device)];
-    if (have) return LQ_OK;
-    LQ_CUDA(ctx, cudaFuncSetAttribute(func, cudaFuncAttributePreferredSharedMemoryCarveout, cudaSharedmemCarveoutMaxShared));
-    have = true;
-    return LQ_OK;
-}
-
 int consume_device_error(lq_ctx* ctx, const char* what) {
     int h[4];
     LQ_CUDA(ctx, cudaMemcpyAsync(h, ctx->err_flag, sizeof h, cudaMemcpyDeviceToHost, ctx->stream));
