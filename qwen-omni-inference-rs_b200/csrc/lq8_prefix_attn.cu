@@ -315,13 +315,13 @@ static int attend_q8(lq_ctx* ctx, const PrefixAttnArgs& a, const PagedSeqs& s, c
     const bool stream_prefix = a.prefix_len == 0 ? stream_own : all_rows <= PREFIX_ATTN_Q8_ROWS;
     PrefixPlan tc, st;
     int64_t steps_tc = 0, steps_st = 0;
+    const int st_rows = (int)std::min<int64_t>(stream_prefix && a.prefix_len > 0 ? all_rows : own_rows, 16);  // of a block
     if (!stream_own || !stream_prefix) {
         steps_tc = plan_cut(a, s, false, ctx->sm_count, &tc);
         set_polls(&tc, false);
     }
     if (stream_own) {
-        const int rows = (stream_prefix && a.prefix_len > 0 ? all_rows : own_rows) > 8 ? 16 : 8;
-        steps_st = plan_cut(a, s, true, ctx->sm_count, &st, rows, PREFIX_ATTN_Q8_CTAS, 128);
+        steps_st = plan_cut(a, s, true, ctx->sm_count, &st, st_rows > 8 ? 16 : 8, PREFIX_ATTN_Q8_CTAS, 128);
         set_polls(&st, true);
         st.streams = stream_prefix ? 3 : 2;
         st.chunks = 1;
@@ -348,7 +348,7 @@ static int attend_q8(lq_ctx* ctx, const PrefixAttnArgs& a, const PagedSeqs& s, c
     int rc = make_workspace(ctx, who, a, s, D, own, pre);
     if (rc) return rc;
     if (pre == &tc && (rc = launch_prefix_attn_tc(ctx, a, s, tc, D, &c))) return rc;
-    if (own == &st && (rc = launch_prefix_attn_q8_decode(ctx, a, s, c, st, D))) return rc;
+    if (own == &st && (rc = launch_prefix_attn_q8_decode(ctx, a, s, c, st, D, st_rows))) return rc;
     return own->streams == 3 && own->np == 0 ? launch_prefix_attn_q8_join(ctx, a, s, *own, D)
                                              : launch_merge<__nv_bfloat16, D>(ctx, a, s, *own, *pre);
 }

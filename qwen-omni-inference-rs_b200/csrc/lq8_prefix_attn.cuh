@@ -93,7 +93,7 @@ __device__ __forceinline__ void zero_rows(const PrefixAttnArgs& a, int tok0, int
 constexpr float PREFIX_ATTN_Q8_LEAST = 8.2718061e-25f;
 
 int launch_prefix_attn_f32(lq_ctx* ctx, const PrefixAttnArgs& a, const PagedSeqs& s, const PrefixPlan& p, int D);
-int launch_prefix_attn_q8_decode(lq_ctx* ctx, const PrefixAttnArgs& a, const PagedSeqs& s, const PagedQ8& c, const PrefixPlan& p, int D);
+int launch_prefix_attn_q8_decode(lq_ctx* ctx, const PrefixAttnArgs& a, const PagedSeqs& s, const PagedQ8& c, const PrefixPlan& p, int D, int rows);
 int launch_prefix_attn_q8_join(lq_ctx* ctx, const PrefixAttnArgs& a, const PagedSeqs& s, const PrefixPlan& p, int D);  // its merge without a prefix
 // q8: a cache in 8 bits (else bf16)
 int launch_prefix_attn_tc(lq_ctx* ctx, const PrefixAttnArgs& a, const PagedSeqs& s, const PrefixPlan& p, int D, const PagedQ8* q8 = nullptr);

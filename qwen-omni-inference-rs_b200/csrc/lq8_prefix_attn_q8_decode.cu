@@ -23,7 +23,7 @@
 // allocator and MMA issuer. Every wait is bounded by a number of polls; when one runs out all warps of the CTA
 // leave, its copies and MMAs in flight are waited for, and the error flag is set.
 // Bound: HBM with long sequences, else the latency of a tile (0.75 to 1.2 us from its bytes' arrival to O) and
-// of a segment's start. 64 sequences of up to 8000 positions, 64 / 8 heads of 128 dims: 88 us of the 106 us
+// of a segment's start. 64 sequences of up to 8000 positions, 64 / 8 heads of 128 dims: 88 us of the 105 us
 // of a call (530 MB, 6.0 TB/s, 92 % of a plain copy), the rest joins cut items; 48 of up to 4000 with 8 heads
 // of 64 dims and no group: 26 us (the bytes: 7.5); 16 sequences of 4 rows with up to 8000 positions: 43 us,
 // where tiles of 128 rows take 61. A kernel of warps that multiplied with mma.sync took 113 us for the
@@ -75,6 +75,7 @@ struct PdCtl {
     alignas(16) float red[2][4][R];  // a warp's maxima, and at a segment's end its sums
     alignas(16) float qf[R];         // what a whole number of S counts for, without K's scale
     int scan[PD_SCAN + 1];           // own steps before each entry
+    int seq[PD_SCAN][3];             // up to so many sequences: q0, q, kv
 };
 
 struct PdArgs {
@@ -152,7 +153,8 @@ __device__ __forceinline__ float pd_warp_sums(float* v, int lane) {
     return t;
 }
 
-template <int D, int R>
+// L: rows of a block that the softmax warps look at (operands hold R, whatever is in the others)
+template <int D, int R, int L>
 __global__ void __launch_bounds__(PD_THREADS, PD_CTAS)
 prefix_attn_q8_decode_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v,
                              const __grid_constant__ PdArgs g) {
@@ -205,6 +207,10 @@ prefix_attn_q8_decode_kernel(const __grid_constant__ CUtensorMap map_k, const __
     const int per_entry = (s.n_seqs + PD_SCAN - 1) / PD_SCAN;
     const int n_entries = (s.n_seqs + per_entry - 1) / per_entry;
     const OwnSteps os{a, p};
+    // (Up to PD_SCAN sequences' lengths are kept. Looked up again, and with the notes for the join worked out before
+    // a segment's first copy instead of behind it, 64 sequences of up to 8000 positions took 106.4 us
+    // instead of 105.5, 48 of 64 dims 26.3 instead of 25.7, 2 short ones 14.1 instead of 13.8.)
+    auto seq_of = [&](int b) { return per_entry == 1 ? SeqInfo{c.seq[b][0], c.seq[b][1], c.seq[b][2]} : seq_info(a, s, b, false); };
     bool fell = false;
 #pragma unroll 1
     for (int e = tid; e < n_entries; e += PD_THREADS) {
@@ -214,6 +220,7 @@ prefix_attn_q8_decode_kernel(const __grid_constant__ CUtensorMap map_k, const __
             const SeqInfo si = seq_info(a, s, b, blockIdx.x == 0);
             fell |= falls(s, b);
             n += os.per_head(si) * a.n_kv;
+            if (per_entry == 1) c.seq[e][0] = si.q0, c.seq[e][1] = si.q, c.seq[e][2] = si.kv;
         }
         c.scan[e + 1] = n;
     }
@@ -270,13 +277,13 @@ prefix_attn_q8_decode_kernel(const __grid_constant__ CUtensorMap map_k, const __
         };
         PdSeg sg;
         bool ok = true;
-        float m[R], l[R], o[R];
+        float m[L], l[L], o[L];
         // this thread's dim of O: TMEM lanes are dims, or, with 64 of them, lanes 0-15 of each warp are
         const int dim = D == 128 ? tid : 16 * warp + lane;
         const bool has = D == 128 || lane < 16;
         auto finish = [&]() {    // rows of sg
 #pragma unroll
-            for (int r = 0; r < R; r++)
+            for (int r = 0; r < L; r++)
                 if (r < sg.n) {
                     const float y = l[r] == 0.0f ? 0.0f : o[r] * (l[r] > 0.0f ? 1.0f / l[r] : l[r]);
                     const int st = sg.row0 + r, tok = a.group_div(st);
@@ -308,18 +315,19 @@ prefix_attn_q8_decode_kernel(const __grid_constant__ CUtensorMap map_k, const __
         int nx_id[2] = {-1, -1};
         uint2 nx_q[DIMS / 4];
         float ks = 0.0f, vs = 1.0f;
-        // pages two tiles ahead, scales one
+        // Pages two tiles ahead, scales one. (A page id is looked at when its scales are asked for: looked at
+        // where it is loaded, it held a tile up by a trip to memory.)
         auto page_at = [&](const PdSeg& o, int t) {
             const int32_t* const table = o.flags & PD_OWN ? s.table + (int64_t)o.b * s.table_ld : a.prefix_table;
             const int x = t * PD_TILE + tid;
             int id = -1;
             if (t < o.t1 && x < o.kv_end) id = table[x >> s.page_shift];
-            return (unsigned)id < (unsigned)s.n_pages ? id : -1;  // (reported by the producer)
+            return id;
         };
         auto scales_at = [&](const PdSeg& o, int t, int id) {  // of this position
             ks = 0.0f;
             vs = 1.0f;
-            if (id >= 0) {
+            if ((unsigned)id < (unsigned)s.n_pages) {  // (reported by the producer)
                 const int64_t at = id * g.c.scale_stride + ((int64_t)o.kh << (s.page_shift - g.c.block_shift)) +
                                    (((t * PD_TILE + tid) & mask) >> g.c.block_shift);
                 ks = g.c.k_scale[at];
@@ -344,7 +352,7 @@ prefix_attn_q8_decode_kernel(const __grid_constant__ CUtensorMap map_k, const __
             }
             have = false;
             sg = nx;
-            int id_next = nx_id[0], id_then = nx_id[1];
+            int id_next = nx_id[1];
             // ---- Q in two bytes ----
             {
                 const int r = q_row, part = q_part;
@@ -388,9 +396,9 @@ prefix_attn_q8_decode_kernel(const __grid_constant__ CUtensorMap map_k, const __
                 return sg.flags & PD_OWN ? min(sg.kv_end, max(0, a.group_div(sg.row0 + min(r, sg.n - 1)) + sg.voff)) : sg.kv_end;
             };
             const int all_see = seen_by(0);  // (the first row's token comes first)
-            float w[R];                      // what the last tile's O counts for
+            float w[L];                      // what the last tile's O counts for
 #pragma unroll
-            for (int r = 0; r < R; r++) m[r] = -INFINITY, l[r] = o[r] = w[r] = 0.0f;
+            for (int r = 0; r < L; r++) m[r] = -INFINITY, l[r] = o[r] = w[r] = 0.0f;
             // O of the tile before
             auto take_o = [&](int k) {
                 if (!pd_wait(&c.abort, &c.o_full[k & 1], (k >> 1) & 1u, p.polls)) return false;
@@ -398,7 +406,7 @@ prefix_attn_q8_decode_kernel(const __grid_constant__ CUtensorMap map_k, const __
                 uint32_t v[N];
                 pd_ld<R>(v, t_lane + 2 * N + (k & 1) * N);
 #pragma unroll
-                for (int r = 0; r < R; r++) o[r] = fmaf((float)((int)v[r] * 256 + (int)v[R + r]), w[r], o[r]);
+                for (int r = 0; r < L; r++) o[r] = fmaf((float)((int)v[r] * 256 + (int)v[R + r]), w[r], o[r]);
                 tc_before();
                 return true;
             };
@@ -406,10 +414,9 @@ prefix_attn_q8_decode_kernel(const __grid_constant__ CUtensorMap map_k, const __
             for (int t = sg.t0; t < sg.t1; t++, n_tile++) {
                 const float k1 = ks, v1 = max_nan(vs, PREFIX_ATTN_Q8_LEAST);
                 const float lv = __log2f(v1), per = __frcp_rn(v1);
-                id_next = id_then;
-                id_then = page_at(sg, t + 2);
                 if (t + 1 < sg.t1) {
                     scales_at(sg, t + 1, id_next);
+                    id_next = page_at(sg, t + 2);
                 } else if (__all_sync(0xffffffffu, mbar_test_wait(&c.seg_full[taken & 1], (taken >> 1) & 1u))) {
                     have = fetch(nx);
                     ended = !have;
@@ -418,42 +425,42 @@ prefix_attn_q8_decode_kernel(const __grid_constant__ CUtensorMap map_k, const __
                 ok = pd_wait(&c.abort, &c.s_full[n_tile & 1], (n_tile >> 1) & 1u, p.polls);
                 if (!ok) break;
                 tc_after();
-                float e[R];
+                float e[L];
                 {
                     uint32_t v[N];
                     pd_ld<R>(v, t_lane + (n_tile & 1) * N);
 #pragma unroll
-                    for (int r = 0; r < R; r++) e[r] = fmaf((float)((int)v[r] * 256 + (int)v[R + r]), c.qf[r] * k1, lv);
+                    for (int r = 0; r < L; r++) e[r] = fmaf((float)((int)v[r] * 256 + (int)v[R + r]), c.qf[r] * k1, lv);
                 }
                 if ((t + 1) * PD_TILE > all_see) {
 #pragma unroll
-                    for (int r = 0; r < R; r++)
+                    for (int r = 0; r < L; r++)
                         if (t * PD_TILE + tid >= seen_by(r)) e[r] = -INFINITY;
                 }
                 float* const mine = c.red[meetings & 1][warp];
                 {
-                    float top[R];
+                    float top[L];
 #pragma unroll
-                    for (int r = 0; r < R; r++) top[r] = pd_warp_max(e[r]);
+                    for (int r = 0; r < L; r++) top[r] = pd_warp_max(e[r]);
                     if (lane == 0) {
 #pragma unroll
-                        for (int r = 0; r < R; r += 4) *reinterpret_cast<float4*>(mine + r) = make_float4(top[r], top[r + 1], top[r + 2], top[r + 3]);
+                        for (int r = 0; r < L; r += 4) *reinterpret_cast<float4*>(mine + r) = make_float4(top[r], top[r + 1], top[r + 2], top[r + 3]);
                     }
                 }
                 const float(*const all)[R] = c.red[meetings & 1];
                 ok = meet();
                 if (!ok) break;
-                float u[R];
+                float u[L];
                 bool grows = false;
 #pragma unroll
-                for (int r = 0; r < R; r++) {
+                for (int r = 0; r < L; r++) {
                     u[r] = fmaxf(fmaxf(all[0][r], all[1][r]), fmaxf(all[2][r], all[3][r]));
                     grows |= u[r] > m[r] + 8.0f;
                 }
                 // ---- P^T: column r the high bytes, R + r the low ones ----
                 uint8_t* const pt = p_sm + (n_tile & 1) * OPERAND;
 #pragma unroll
-                for (int r = 0; r < R; r++) {
+                for (int r = 0; r < L; r++) {
                     e[r] = ex2(e[r] - (u[r] == -INFINITY ? 0.0f : u[r]));
                     const uint32_t v = __float_as_uint(fmaf(e[r], 32512.0f, 12582912.0f));  // (whole number in the low bits)
                     const uint32_t at = pd_at<128>(r, tid);  // (rows r and R + r swizzle alike)
@@ -471,7 +478,7 @@ prefix_attn_q8_decode_kernel(const __grid_constant__ CUtensorMap map_k, const __
                 }
                 if (grows) {  // (the same in all threads: u and m are)
 #pragma unroll
-                    for (int r = 0; r < R; r++) {
+                    for (int r = 0; r < L; r++) {
                         const float mn = fmaxf(m[r], u[r]), f = mn == -INFINITY ? 1.0f : ex2(m[r] - mn);
                         m[r] = mn;
                         o[r] *= f;
@@ -479,7 +486,7 @@ prefix_attn_q8_decode_kernel(const __grid_constant__ CUtensorMap map_k, const __
                     }
                 }
 #pragma unroll
-                for (int r = 0; r < R; r++) {
+                for (int r = 0; r < L; r++) {
                     const float f = m[r] == -INFINITY ? 0.0f : ex2(u[r] - m[r]);
                     l[r] = fmaf(e[r], per * f, l[r]);
                     w[r] = f * (1.0f / 32512.0f);
@@ -491,13 +498,13 @@ prefix_attn_q8_decode_kernel(const __grid_constant__ CUtensorMap map_k, const __
             if (!ok) break;
             // ---- the segment's result: one dim of each row ----
             {
-                const float sum = pd_warp_sums<R>(l, lane);
-                if (lane % (32 / R) == 0) c.red[meetings & 1][warp][lane / (32 / R)] = sum;
+                const float sum = pd_warp_sums<L>(l, lane);
+                if (lane % (32 / L) == 0) c.red[meetings & 1][warp][lane / (32 / L)] = sum;
                 const float(*const all)[R] = c.red[meetings & 1];
                 ok = meet();
                 if (!ok) break;
 #pragma unroll
-                for (int r = 0; r < R; r++) l[r] = (all[0][r] + all[1][r]) + (all[2][r] + all[3][r]);
+                for (int r = 0; r < L; r++) l[r] = (all[0][r] + all[1][r]) + (all[2][r] + all[3][r]);
             }
             const bool own = sg.flags & PD_OWN;
             const int cap = p.cap[own];
@@ -505,7 +512,7 @@ prefix_attn_q8_decode_kernel(const __grid_constant__ CUtensorMap map_k, const __
                 finish();
             } else {
 #pragma unroll
-                for (int r = 0; r < R; r++)
+                for (int r = 0; r < L; r++)
                     if (r < sg.n) {
                         if (tid == r) p.ml[own][(int64_t)sg.slot * cap + r] = make_float2(m[r], l[r]);
                         if (has) p.o[own][(((int64_t)sg.slot * (D / 4) + (dim >> 2)) * cap + r) * 4 + (dim & 3)] = o[r];
@@ -570,32 +577,38 @@ prefix_attn_q8_decode_kernel(const __grid_constant__ CUtensorMap map_k, const __
                         else e1 = mid;
                     }
                     int rest = step - c.scan[e0], per = 1;
-                    // a lane looks at a sequence of the entry
+                    if (per_entry == 1) {
+                        b = e0;
+                        si = seq_of(b);
+                        per = max(1, os.per_head(si));
+                    } else {
+                        // a lane looks at a sequence of the entry
 #pragma unroll 1
-                    for (b = e0 * per_entry; b < s.n_seqs; b += 32) {
-                        int n = 0;
-                        if (b + lane < s.n_seqs) {
-                            si = seq_info(a, s, b + lane, false);
-                            n = os.per_head(si);
-                        }
-                        int upto = n * a.n_kv;
+                        for (b = e0 * per_entry; b < s.n_seqs; b += 32) {
+                            int n = 0;
+                            if (b + lane < s.n_seqs) {
+                                si = seq_info(a, s, b + lane, false);
+                                n = os.per_head(si);
+                            }
+                            int upto = n * a.n_kv;
 #pragma unroll
-                        for (int d = 1; d < 32; d <<= 1) {
-                            const int u = __shfl_up_sync(0xffffffffu, upto, d);
-                            if (lane >= d) upto += u;
+                            for (int d = 1; d < 32; d <<= 1) {
+                                const int u = __shfl_up_sync(0xffffffffu, upto, d);
+                                if (lane >= d) upto += u;
+                            }
+                            const unsigned past = __ballot_sync(0xffffffffu, upto > rest);
+                            if (past) {
+                                const int at = __ffs(past) - 1;
+                                rest -= __shfl_sync(0xffffffffu, upto - n * a.n_kv, at);
+                                per = __shfl_sync(0xffffffffu, n, at);
+                                si.q0 = __shfl_sync(0xffffffffu, si.q0, at);
+                                si.q = __shfl_sync(0xffffffffu, si.q, at);
+                                si.kv = __shfl_sync(0xffffffffu, si.kv, at);
+                                b += at;
+                                break;
+                            }
+                            rest -= __shfl_sync(0xffffffffu, upto, 31);
                         }
-                        const unsigned past = __ballot_sync(0xffffffffu, upto > rest);
-                        if (past) {
-                            const int at = __ffs(past) - 1;
-                            rest -= __shfl_sync(0xffffffffu, upto - n * a.n_kv, at);
-                            per = __shfl_sync(0xffffffffu, n, at);
-                            si.q0 = __shfl_sync(0xffffffffu, si.q0, at);
-                            si.q = __shfl_sync(0xffffffffu, si.q, at);
-                            si.kv = __shfl_sync(0xffffffffu, si.kv, at);
-                            b += at;
-                            break;
-                        }
-                        rest -= __shfl_sync(0xffffffffu, upto, 31);
                     }
                     if (b >= s.n_seqs) break;  // lengths that changed under the kernel
                     kh = rest / per;
@@ -626,41 +639,51 @@ prefix_attn_q8_decode_kernel(const __grid_constant__ CUtensorMap map_k, const __
                         const int n = max(1, min(p.pb, (own ? si.q : live_rows(s)) * a.group - rb * p.pb));
                         const int item = (own ? a.n_kv * os.base(si, b) : 0) + kh * n_rb + rb;
                         const bool begins = tile == 0, whole = a.prefix_len == 0 && begins && end == nt;
-                        if (lane == 0) {
-                            if (tile == 0) p.first[part][item] = worker;
-                            if (end == nt) p.last[part][item] = worker;
-                            if (a.prefix_len == 0 && tile == 0 && end < nt)
-                                p.split[worker] = SplitItem{n, row0, kh, line.owner(line.sp + step + nt - 1)};
-                        }
                         PdSeg sg;
                         sg.t0 = tile, sg.t1 = end, sg.n = n, sg.flags = (own ? PD_OWN : 0) | (whole ? PD_WHOLE : 0);
                         sg.kh = kh, sg.b = b, sg.kv_end = kv_end, sg.row0 = row0, sg.voff = own ? si.kv - si.q + 1 - si.q0 : 0;
                         sg.slot = own ? p.own_slot(item, worker, begins) : item + worker;
                         sg.pad[0] = sg.pad[1] = 0;
                         const int32_t* const table = own ? s.table + (int64_t)b * s.table_ld : a.prefix_table;
-                        auto page_at = [&](int t) {  // this lane's page of tile t; none: zeros
+                        // Page ids of 32 / boxes tiles come with one load, while those before are in use, and are looked
+                        // at when their tile's turn comes.
+                        const int per = 32 / boxes;
+                        auto ids_from = [&](int t) {  // lane i: the i-th page from tile t on
                             const int x = t * PD_TILE + lane * box;
-                            int id = s.n_pages;
-                            if (lane < boxes && t < end && x < kv_end) {
-                                id = table[x >> s.page_shift];
-                                if ((unsigned)id >= (unsigned)s.n_pages) {
-                                    flag_error(a.err, ERR_PAGE_ID, id);
-                                    id = s.n_pages;
-                                }
+                            return x < min(kv_end, end * PD_TILE) ? table[x >> s.page_shift] : -1;
+                        };
+                        int ids = ids_from(tile), ahead = ids_from(tile + per), base = tile;
+                        auto page_of = [&](int t) {  // this lane's page of tile t, asked for in turn; none: zeros
+                            if (t == base + per) ids = ahead, base = t, ahead = ids_from(t + per);
+                            int id = __shfl_sync(0xffffffffu, ids, ((t - base) * boxes + lane) & 31);
+                            if (lane >= boxes || t * PD_TILE + lane * box >= kv_end) {
+                                id = s.n_pages;
+                            } else if ((unsigned)id >= (unsigned)s.n_pages) {
+                                flag_error(a.err, ERR_PAGE_ID, id);
+                                id = s.n_pages;
                             }
                             return id;
                         };
-                        int id = page_at(tile), id_next = page_at(tile + 1);
                         put(sg);
                         // K of the next tile before V of this one, as the MMA warp takes them
+                        int id = page_of(tile);
                         if (ok) load(&map_k, kh, tile * PD_TILE, id);
-    #pragma unroll 1
+                        if (lane == 0) {  // (after the copies are on their way)
+                            if (tile == 0) p.first[part][item] = worker;
+                            if (end == nt) p.last[part][item] = worker;
+                            if (a.prefix_len == 0 && tile == 0 && end < nt)
+                                p.split[worker] = SplitItem{n, row0, kh, line.owner(line.sp + step + nt - 1)};
+                        }
+                        __syncwarp();
+#pragma unroll 1
                         for (int t = tile; t < end && ok; t++) {
-                            const int id_then = page_at(t + 2);
-                            if (t + 1 < end) load(&map_k, kh, (t + 1) * PD_TILE, id_next);
+                            int id_next = id;
+                            if (t + 1 < end) {
+                                id_next = page_of(t + 1);
+                                load(&map_k, kh, (t + 1) * PD_TILE, id_next);
+                            }
                             if (ok) load(&map_v, kh, t * PD_TILE, id);
                             id = id_next;
-                            id_next = id_then;
                         }
                     }
                     // ---- the next item with a step ----
@@ -676,7 +699,7 @@ prefix_attn_q8_decode_kernel(const __grid_constant__ CUtensorMap map_k, const __
                                     hi = step;
                                     break;
                                 }
-                                si = seq_info(a, s, b, false);
+                                si = seq_of(b);
                                 n_rb = os.blocks(si);
                                 if (n_rb == 0 || si.kv == 0) {  // nothing of this sequence
                                     kh = a.n_kv - 1;
@@ -890,7 +913,7 @@ int launch_prefix_attn_q8_join(lq_ctx* ctx, const PrefixAttnArgs& a, const Paged
     return p.pb == 8 ? launch_join<128, 8>(ctx, a, p, stacked) : launch_join<128, 16>(ctx, a, p, stacked);
 }
 
-template <int D, int R>
+template <int D, int R, int L>
 static int launch_decode(lq_ctx* ctx, const PdArgs& g) {
     const int page = 1 << g.s.page_shift;
     const uint64_t dims[4] = {(uint64_t)D, (uint64_t)page, (uint64_t)g.c.n_kv, (uint64_t)g.s.n_pages};
@@ -903,16 +926,22 @@ static int launch_decode(lq_ctx* ctx, const PdArgs& g) {
     rc = make_tensor_map_4d(ctx, &mv, CU_TENSOR_MAP_DATA_TYPE_UINT8, g.c.v, dims, strides, box, swz);
     if (rc) return rc;
     const size_t smem = 1024 + pd_stages(D) * PD_TILE * D + 3 * 2 * R * 128 + sizeof(PdCtl<R>);
-    rc = ensure_func_smem(ctx, (const void*)prefix_attn_q8_decode_kernel<D, R>, smem);
+    rc = ensure_func_smem(ctx, (const void*)prefix_attn_q8_decode_kernel<D, R, L>, smem);
     if (rc) return rc;
-    return launch_kernel(ctx, prefix_attn_q8_decode_kernel<D, R>, dim3((unsigned)g.p.workers), dim3(PD_THREADS), smem,
+    return launch_kernel(ctx, prefix_attn_q8_decode_kernel<D, R, L>, dim3((unsigned)g.p.workers), dim3(PD_THREADS), smem,
                          "prefix_attn_q8_decode", mk, mv, g);
 }
 
-int launch_prefix_attn_q8_decode(lq_ctx* ctx, const PrefixAttnArgs& a, const PagedSeqs& s, const PagedQ8& c, const PrefixPlan& p, int D) {
+// rows: the most of a block. (2 sequences of one row, groups of 4: 14.4 us with L = 4, 15.0 with 8; L = 1 changed
+// nothing for blocks of one row.)
+template <int D>
+static int launch_decode_rows(lq_ctx* ctx, const PdArgs& g, int rows) {
+    return rows <= 4 ? launch_decode<D, 8, 4>(ctx, g) : rows <= 8 ? launch_decode<D, 8, 8>(ctx, g) : launch_decode<D, 16, 16>(ctx, g);
+}
+
+int launch_prefix_attn_q8_decode(lq_ctx* ctx, const PrefixAttnArgs& a, const PagedSeqs& s, const PagedQ8& c, const PrefixPlan& p, int D, int rows) {
     const PdArgs g{a, s, p, c};
-    if (D == 64) return p.pb == 8 ? launch_decode<64, 8>(ctx, g) : launch_decode<64, 16>(ctx, g);
-    return p.pb == 8 ? launch_decode<128, 8>(ctx, g) : launch_decode<128, 16>(ctx, g);
+    return D == 64 ? launch_decode_rows<64>(ctx, g, rows) : launch_decode_rows<128>(ctx, g, rows);
 }
 
 }  // namespace lq
