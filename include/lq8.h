@@ -322,7 +322,8 @@ int lq_paged_read_q8(lq_ctx* ctx, const int8_t* k_codes_dev, const int8_t* v_cod
  * smaller than another's may lose its weight. With up to 32 stacked rows (max_q, behind a prefix all of the
  * call's, times n_heads / n_kv_heads) a row of q is rounded to 1 / 32512 of its largest value and
  * weights times V's scale to 1 / 32512 of the largest of their 128 positions, sums are exact; with more,
- * products are of 16-bit floats, q and codes exact, weights in fp16, sums f32. */
+ * products are of 16-bit floats, q and codes exact, weights in fp16 (times V's scale, those below 2^-32 of
+ * a row's largest are lost), sums f32. */
 int lq_prefix_attention_q8(lq_ctx* ctx, const uint16_t* q_dev, int64_t q_stride, int64_t rows, int64_t n_heads,
                            int64_t n_kv_heads, int64_t head_dim, float scale, const int8_t* k_codes_dev,
                            const int8_t* v_codes_dev, const float* k_scale_dev, const float* v_scale_dev,

@@ -22,6 +22,10 @@ namespace lq {
 // becomes zero, with codes of zero.
 // Blocks are numbered without a scan over the sequences: those of sequence b from
 // q_start[b] / B + 2 b on, which leaves room for one cut at either end.
+// Bound: HBM for large prompts, the latency of dependent loads (row, sequence, page, older codes) for small ones.
+// 16 prompts of up to 2000 rows of 32 + 16 heads, f32: 91 us with cold caches, 433 MB through DRAM (4.8 TB/s, 73 % of
+// a plain copy); 12 prompt chunks, bf16, q/k norm: 25 us (instructions 2.1 a cycle, DRAM 16 %); 8 rows:
+// one launch.
 // =========================================================================================
 struct TeamInfo {
     int q0, p0;      // the sequence's first new row and its position

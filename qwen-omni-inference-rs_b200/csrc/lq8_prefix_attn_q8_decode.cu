@@ -22,11 +22,12 @@
 // and brings tiles page by page (128-byte swizzle; pages past the end come as zeros); warp 5: TMEM
 // allocator and MMA issuer. Every wait is bounded by a number of polls; when one runs out all warps of the CTA
 // leave, its copies and MMAs in flight are waited for, and the error flag is set.
-// Bound: HBM with long sequences, else the latency of a tile (0.75 to 1.2 us from its bytes' arrival to O) and
-// of a segment's start. 64 sequences of up to 8000 positions, 64 / 8 heads of 128 dims: 88 us of the 105 us
-// of a call (530 MB, 6.0 TB/s, 92 % of a plain copy), the rest joins cut items; 48 of up to 4000 with 8 heads
-// of 64 dims and no group: 26 us (the bytes: 7.5); 16 sequences of 4 rows with up to 8000 positions: 43 us,
-// where tiles of 128 rows take 61. A kernel of warps that multiplied with mma.sync took 113 us for the
+// Bound: HBM with long sequences, else the latency of a tile (1900 cycles of a softmax warp: 520 for scales and
+// the next tile's loads, 140 for S, 280 to read and mask it, 140 to meet, 420 for P, 200 for O, 220 for the
+// sums) and of a segment's start (2 us). 64 sequences of up to 8000 positions, 64 / 8 heads of 128 dims: 88
+// us of the 105 us of a call (530 MB, 6.0 TB/s, 92 % of a plain copy), the rest joins cut items; 48 of up to 4000,
+// 32 / 4 heads of 64 dims: 26 us (the bytes: 7.5); 16 sequences of 4 rows with up to 8000 positions: 43
+// us, where tiles of 128 rows take 61. A kernel of warps that multiplied with mma.sync took 113 us for the
 // first of these.
 //
 // TMA loads here read only this GPU's memory and use no multicast.
@@ -630,7 +631,7 @@ prefix_attn_q8_decode_kernel(const __grid_constant__ CUtensorMap map_k, const __
                         kv_end = os.visible(si, rb);
                         nt = (kv_end + PD_TILE - 1) / PD_TILE;
                     }
-                    // (an own item counts for a step more than its tiles: a segment's beginning and end)
+                    // (an own item counts for more steps than its tiles: a segment's beginning and end)
                     const int ns = nt + (own && nt > 0 ? p.extra : 0), upto = min(ns, tile + hi - step), end = min(nt, upto);
                     if (upto <= tile) break;  // lengths that changed under the kernel
                     if (end > tile) {
@@ -932,8 +933,7 @@ static int launch_decode(lq_ctx* ctx, const PdArgs& g) {
                          "prefix_attn_q8_decode", mk, mv, g);
 }
 
-// rows: the most of a block. (2 sequences of one row, groups of 4: 14.4 us with L = 4, 15.0 with 8; L = 1 changed
-// nothing for blocks of one row.)
+// rows: the most of a block. (2 short sequences, groups of 2: 14.4 us with L = 4, 15.0 with 8.)
 template <int D>
 static int launch_decode_rows(lq_ctx* ctx, const PdArgs& g, int rows) {
     return rows <= 4 ? launch_decode<D, 8, 4>(ctx, g) : rows <= 8 ? launch_decode<D, 8, 8>(ctx, g) : launch_decode<D, 16, 16>(ctx, g);

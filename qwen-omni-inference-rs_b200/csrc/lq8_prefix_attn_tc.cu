@@ -1,5 +1,5 @@
-// lq8_prefix_attn_tc.cu -- the shared-prefix attention for bf16 caches on the tcgen05 tensor
-// cores.
+// lq8_prefix_attn_tc.cu -- the shared-prefix attention for bf16 caches, and for 8-bit ones with many
+// rows, on the tcgen05 tensor cores.
 //
 // One CTA per SM walks its share of the line of steps (lq8_prefix_plan.cuh). It runs two flows of
 // up to 128 stacked query rows, each with its own Q tile in shared memory and its own S and O
@@ -31,6 +31,14 @@
 // P. 128 sequences of 64 heads behind 32768 positions: 164 us for the prefix (837 TFLOP/s), 200 us
 // with 1000 own positions; 64 sequences of 32 heads behind 8191: 51 us (3.3 TB/s); 4 chunks of 1000
 // tokens behind 8192: 474 us (1047 TFLOP/s), all from cold L2, the merge in the first and last.
+//
+// 8-bit caches (Q8): codes come into a small ring of their own, and warps 12-15 turn K's into bf16 (next to
+// Q) and V's into fp16: exact. A score is s = S k_scale c + log2 v_scale: V's scale is in the exponent, so that
+// P V needs no more than P. P is fp16 below a running maximum of s, l adds P / v_scale; the producer copies the
+// scales of 16 positions each ahead of a round. Bound: a round takes 4665 cycles, a chain of QK, softmax
+// (2495), PV for either flow: P lies over S, and TMEM has no room for another S; shared memory serves the
+// converters (1024 cycles) next to the products (1536). 10 prompt chunks behind 2049 positions: 158 us; 128
+// sequences behind 32768: 217 us with their own positions (which the streaming kernel takes).
 //
 // TMA loads here read only this GPU's memory and use no multicast.
 #include "lq8_async.cuh"

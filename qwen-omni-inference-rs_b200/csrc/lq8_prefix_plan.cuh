@@ -183,9 +183,11 @@ __host__ __device__ __forceinline__ void flow_range(const Line& l, bool paired, 
 
 // The line of a streaming kernel, prefix items first, cut into ranges that its workers take in turn: with
 // n workers and 20 steps for each, n ranges with half of the line, n with a quarter, n with three twentieths
-// and 2 n with the rest, else n equal ones, or one for each step; none is empty. A worker may begin late (an SM that still holds another kernel's shared
-// memory took its third CTA 80 us late, and a fixed share for each ended 25 us after all others), and
-// memory serves some SMs faster than others. Which worker takes a range changes no result.
+// and 2 n with the rest, else n equal ones, or one for each step; none is empty. A worker may begin late (an
+// SM that still holds another kernel's shared memory took a third CTA 80 us late, and a fixed share for each
+// ended 25 us after all others), and memory serves some SMs faster than others. Which worker takes a range
+// changes no result. (With 10 steps for each enough for five ranges, 48 sequences of 64 dims, 12 steps,
+// took 41 us instead of 26: a range's start counts for several steps.)
 struct Shares {
     int n, sp, total, ranges;
     int size[4];   // steps of the four parts

@@ -8,15 +8,15 @@ Tolerances, with u = 2^-8 the unit roundoff of a bf16 output (0 for f32):
   a code is within 0.5 + 0.001 (and 2^-10 for the f32 product by the scale's reciprocal) of the exact
   quotient, the scale within 2^-17 of its own size; given the f32 values, codes and scales are exact;
 - codes rounded again, and rows read back: exact, in f32;
-- attention with up to 16 stacked rows a kv head: q is rounded to amax / 65024 at most, which moves a
+- attention with up to 32 stacked rows a kv head: q is rounded to amax / 65024 at most, which moves a
   score by at most d = c amax / 65024 sum |k| and a weight by a factor within e^(+-2d); f32 sums and
   exponentials stay within 2e-5 sum p |v| (the framework's tolerance for its f32 attention), the result
   is rounded once, u |o|. Weights p, times V's scale s, are rounded
   to whole 1 / 32512 parts of the largest p s of their 128 positions (the tiles begin at the prefix's and
   at the own positions' first), half of that at most: codes are up to 127, so that a tile gives at most
   128 127 max(p s) / 65024; w is the sum of 128 127 max(p s) over the tiles;
-- attention with more: q is exact, a weight is rounded to bf16 once, u sum p |v|; the rest as
-  above;
+- attention with more: q is exact, a weight (times V's scale) is rounded to 16 bits once, at most u sum
+  p |v|; the rest as above;
 - both: a weight below 2^-126 of the largest is zero in f32 (and flushed). Over up to 2^13 positions of
   |v| < 2^3 that is up to 2^-110, where the 64-bit result may be the like of 1e-116."""
 import numpy as np
@@ -438,7 +438,7 @@ def attention_case(ctx, lq8_lib, kv, q, Hq, Hkv, D, page, block, prefix, seed=11
     ctx.device_status()
     assert (out[:, Hq:] == 7.0).all()
     want = attention64(s, x, D ** -0.5)
-    # (which kernel ran: more than 16 stacked rows of one kv head take the tensor cores, where it exists)
+    # (which kernel ran: more than 32 stacked rows of one kv head take the tensor cores, where it exists)
     within(got, want[0], tolerance(want, streaming=False) + tolerance(want))
     again = s.cache.attend(x, s.batch)
     assert torch.equal(again, got)  # the same bits every time
