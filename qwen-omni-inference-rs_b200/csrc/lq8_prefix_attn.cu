@@ -340,6 +340,12 @@ static int attend_q8(lq_ctx* ctx, const PrefixAttnArgs& a, const PagedSeqs& s, c
         // either takes, 128 sequences behind 32768 positions took 295 us instead of 216, 64 behind 8191 64
         // instead of 60: an SM with few neighbours at work reads no faster.)
         tc.workers = std::max(1, std::min(ctx->sm_count, tc.sp));
+        // Short prefixes: as many CTAs for each item, so that none has the end of one and the beginning of the next
+        // (two sets of partials, about two steps more): 64 sequences of 4 rows behind 8191 positions 62.5 -> 57.6
+        // us, 64 of 8 behind 9000 51.6 -> 48.5, 128 of 4 behind 8192 80.9 -> 77.6. Not so from about ten steps
+        // a CTA on: 100 sequences of 8 rows behind 14900 positions 70.8 -> 77.7, behind 30000 108 -> 130.
+        const int items = a.n_kv * tc.n_rb, per = std::min(ctx->sm_count / items, tc.np);
+        if (per >= 1 && ceil_div(tc.np, per) <= std::min(8, (int)ceil_div(tc.sp, ctx->sm_count) + 1)) tc.workers = per * items;
         tc.workers_mul = ((1ull << 40) + tc.workers - 1) / tc.workers;
         tc.apart = 1;
         st.sp = 0;
