@@ -131,6 +131,8 @@ prefix_attn_merge_kernel(const __grid_constant__ PrefixAttnArgs a, const __grid_
                     const int part = c0 + i >= cnt[0];
                     float2 ml = make_float2(-INFINITY, 0.0f);
                     if (mine && slot[i] >= 0) ml = p.ml[part][(int64_t)slot[i] * p.cap[part] + in[part] + r];
+                    // (a maximum skips NaN, so that a piece of nothing else has -inf here: its sum tells)
+                    if (ml.y != ml.y) ml.x = ml.y;
                     if (pass == 0) {
                         const float up = fmaxf(M, ml.x);
                         if (up != -INFINITY) L = L * exp2f(M - up) + ml.y * exp2f(ml.x - up);
