@@ -66,3 +66,40 @@ def test_rows_that_are_nan_in_wider_caches(ctx, lq8_lib, dtype, rows, prefix):
     bad[at[1], 1] = bad[at[2], 2] = True
     bad[at[5], :2] = True
     check(got, want, (wide.U[dtype] + 2e-5) * mass + wide.U[dtype] * want.abs(), bad)
+
+
+# ------------------------------------------------------------------------------------------
+# scales that are NaN, in blocks that only the later rows of a sequence see
+# ------------------------------------------------------------------------------------------
+
+def spoil(s, places, heads):
+    """Scales of (K or V, sequence, kv head, block of positions) become NaN; the rows (rows, heads) that see them."""
+    import torch
+    bad = torch.zeros(s.rows, heads, dtype=torch.bool, device="cuda")
+    G, per = heads // s.n_kv, s.page // s.block
+    for which, b, kh, blk in places:
+        (s.ks if which == "k" else s.vs)[int(s.table[b, blk // per]), kh, blk % per] = float("nan")
+        for j in range(int(s.q[b])):
+            if int(s.kv[b] - s.q[b]) + j >= blk * s.block:
+                bad[int(s.start[b]) + j, kh * G:(kh + 1) * G] = True
+    return bad
+
+
+def hidden_case(ctx, lq8_lib, kv, q, Hq, Hkv, D, page, block, prefix, places, streaming):
+    s = q8.Cache(lq8_lib, ctx, kv, q, Hkv, D, page, block, prefix=prefix, seed=35).fill()
+    x = randn(36, s.rows, Hq, D, dtype="bf16")
+    want = q8.attention64(s, x, D ** -0.5)
+    bad = spoil(s, places, Hq)
+    assert bool(bad.any()) and not bool(bad.all())
+    got = s.cache.attend(x, s.batch)
+    ctx.device_status()
+    check(got, want[0], q8.tolerance(want) if streaming else q8.tolerance(want, streaming=False) + q8.tolerance(want), bad)
+
+
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("prefix", [0, 100])
+def test_nan_scales_that_few_rows_see(ctx, lq8_lib, prefix, D):
+    """Up to 32 stacked rows: the last rows of a sequence begin a block (of 16, of 64) that the first ones do not see."""
+    hidden_case(ctx, lq8_lib, [34, 131, 257, 18], [4, 3, 2, 4], 4, 2, D, 16, 16, prefix,
+                [("v", 0, 0, 2), ("k", 0, 1, 2), ("k", 1, 0, 8), ("v", 1, 1, 8), ("v", 2, 0, 16), ("v", 3, 1, 1)], True)
+    hidden_case(ctx, lq8_lib, [66, 130], [4, 3], 4, 2, D, 64, 64, prefix, [("v", 0, 0, 1), ("k", 1, 1, 2), ("v", 1, 0, 2)], True)
