@@ -417,17 +417,21 @@ prefix_attn_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_co
             for (; t < sg.t1; t++) {
                 // 8-bit caches, lane i: the scales of the i-th 16 positions. K's in units of log2 (never so small
                 // that a masked score loses its minus infinity); V's, no smaller than PREFIX_ATTN_Q8_LEAST,
-                // as what a score gets on top and what a weight then counts for in l
-                [[maybe_unused]] float k_mul = 0.0f, v_add = 0.0f, v_per = 0.0f;
+                // as what a score gets on top and what a weight then counts for in l. One that is NaN counts
+                // as the least (fmaxf), and makes l NaN where the row sees its positions: in the products it
+                // would reach rows from which it is masked.
+                [[maybe_unused]] float k_mul = 0.0f, v_add = 0.0f, v_per = 0.0f, both = 0.0f;
                 if constexpr (Q8) {
                     if (!pa_wait(c, &c.sc_full[f][sc_slot], sc_ph)) break;
-                    k_mul = max_nan(c.sc[f][sc_slot][0][lane & 7] * cs, 1e-37f);
-                    const float v = max_nan(c.sc[f][sc_slot][1][lane & 7], PREFIX_ATTN_Q8_LEAST);
+                    const float ks = c.sc[f][sc_slot][0][lane & 7], vs = c.sc[f][sc_slot][1][lane & 7];
+                    k_mul = fmaxf(ks * cs, 1e-37f);
+                    const float v = fmaxf(vs, PREFIX_ATTN_Q8_LEAST);
                     v_add = __log2f(v);
                     v_per = __frcp_rn(v);
                     __syncwarp();
                     if (lane == 0) mbar_arrive(&c.sc_empty[f][sc_slot]);
                     if (++sc_slot == PA_SCALES) sc_slot = 0, sc_ph ^= 1;
+                    both = ks * vs;
                 }
                 auto of = [](float x, int i) { return __shfl_sync(0xffffffffu, x, i); };
                 if (!pa_wait(c, &c.s_full[f], s_ph)) break;
@@ -625,6 +629,10 @@ prefix_attn_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_co
                 tc_before();
                 __syncwarp();
                 if (lane == 0) mbar_arrive(&c.p_full[f]);
+                if constexpr (Q8) {  // (here, where no product waits for it)
+                    const unsigned lost = __ballot_sync(0xffffffffu, both != both) & 0xffu;
+                    if (lost && (t < chain ? g.a.prefix_len : vis) - t * PA_TILE > 16 * (__ffs(lost) - 1)) l = __uint_as_float(0x7fffffffu);
+                }
                 if (t == sg.t0) {
                     more = next(true);
                     early = more == NX_SEG && q_ahead(sg, nx);
@@ -706,7 +714,7 @@ prefix_attn_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_co
                 tc_before();
                 continue;
             }
-            const float inv = l > 0.0f ? 1.0f / l : 0.0f;
+            const float inv = l > 0.0f ? 1.0f / l : l;  // (zero or NaN stays)
             const int at_o = half + row;
             if (mine && !whole) g.p.ml[own][(int64_t)sg.slot * cap + at_o] = make_float2(m - BIAS, l);
             // four dims of all rows lie together, so that a warp's stores are 512 bytes each

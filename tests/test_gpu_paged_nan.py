@@ -103,3 +103,24 @@ def test_nan_scales_that_few_rows_see(ctx, lq8_lib, prefix, D):
     hidden_case(ctx, lq8_lib, [34, 131, 257, 18], [4, 3, 2, 4], 4, 2, D, 16, 16, prefix,
                 [("v", 0, 0, 2), ("k", 0, 1, 2), ("k", 1, 0, 8), ("v", 1, 1, 8), ("v", 2, 0, 16), ("v", 3, 1, 1)], True)
     hidden_case(ctx, lq8_lib, [66, 130], [4, 3], 4, 2, D, 64, 64, prefix, [("v", 0, 0, 1), ("k", 1, 1, 2), ("v", 1, 0, 2)], True)
+
+
+@pytest.mark.parametrize("D", [64, 128])
+@pytest.mark.parametrize("prefix", [0, 100, 3000])
+@pytest.mark.parametrize("q", [[150, 3, 20, 60], [300, 3, 20, 300], [20, 3, 17, 2]])
+def test_nan_scales_that_later_rows_of_a_chunk_see(ctx, lq8_lib, q, prefix, D):
+    """More rows: tiles of 128 of them, of up to 64 and of up to 8."""
+    import torch
+    kv = [q[0] + 7, 33 + 128, q[2] + 40, q[3] + 300]
+    places = [("v", 0, 0, (kv[0] - 1) // 16), ("k", 0, 1, (q[0] // 2 + 7) // 16), ("v", 1, 0, 10), ("k", 1, 1, 10),
+              ("k", 2, 0, (kv[2] - 1) // 16), ("v", 2, 1, (kv[2] - 9) // 16), ("v", 3, 0, (kv[3] - 1) // 16), ("k", 3, 1, 18)]
+    hidden_case(ctx, lq8_lib, kv, q, 6, 2, D, 32, 16, prefix, places, False)
+    if prefix:  # a block of the prefix: every row of its kv head, and of no other
+        s = q8.Cache(lq8_lib, ctx, kv, q, 2, D, 32, 16, prefix=prefix, seed=37).fill()
+        x = randn(38, s.rows, 6, D, dtype="bf16")
+        want = q8.attention64(s, x, D ** -0.5)
+        s.vs[int(s.ptable[1]), 1, 0] = float("nan")
+        bad = torch.zeros(s.rows, 6, dtype=torch.bool, device="cuda")
+        bad[:, 3:] = True
+        check(s.cache.attend(x, s.batch), want[0], q8.tolerance(want, streaming=False) + q8.tolerance(want), bad)
+        ctx.device_status()
