@@ -57,7 +57,12 @@ prefix_attn_merge_kernel(const __grid_constant__ PrefixAttnArgs a, const __grid_
         }
         const SeqInfo si = seq_info(a, s, lo, false);
         const int rb = x - os.base(si, lo), nb = os.blocks(si);
-        if (rb < 0 || rb >= nb) return;
+        if (rb < 0 || rb >= nb) {
+            // (one CTA at least waits, so that this kernel does not end, and the next one does not begin on the
+            // workspace, before the attention is through: with padding rows alone all of them leave here)
+            if (blockIdx.x == 0 && blockIdx.y == 0) pdl_wait();
+            return;
+        }
         st0 = si.q0 * a.group + rb * p.ob + own_in;
         todo = min(MR, min(p.ob, si.q * a.group - rb * p.ob) - own_in);
         own_item = a.n_kv * x + kh * nb + rb - a.n_kv * rb;  // n_kv base + kh nb + rb
