@@ -522,7 +522,7 @@ __global__ void __launch_bounds__(ME_THREADS, 2) moe_mma_kernel(const __grid_con
                 }
                 if (bad) continue;
                 const uint8_t* st = sm + (size_t)s * ME_STAGE;
-                // this warp's slice of the stage into registers, then release the stage
+                // this warp's slice of the stage into registers
                 uint2 wa[8], wb[8];
 #pragma unroll
                 for (int j = 0; j < 8; j++) {
@@ -532,14 +532,18 @@ __global__ void __launch_bounds__(ME_THREADS, 2) moe_mma_kernel(const __grid_con
                 }
                 const uint4 sa = *reinterpret_cast<const uint4*>(st + sc_off);
                 const uint4 sb = *reinterpret_cast<const uint4*>(st + sc_off + 8 * 16);
-                __syncwarp();
-                if (lane == 0) mbar_arrive(&empty[s]);
                 // straight-line code for the chunk's 8 blocks (the n8-tile count is decided
                 // once, outside), so loads and MMAs of different blocks can overlap
                 const int8_t* xb = xs + (size_t)g * XS + c * ME_KC + 8 * t;
                 const float* db = xdf + c * 8 * TOK + 2 * t;
                 if (TOK > 8 && two) me_blocks<2>(acc, wa, wb, sa, sb, xb, 8 * XS, db, TOK);
                 else me_blocks<1>(acc, wa, wb, sa, sb, xb, 8 * XS, db, TOK);
+                // The stage is released once the products have used it. Released as soon as its loads were issued,
+                // the next copy could land before they had read (behind another CTA's burst of token rows):
+                // 1 % of the calls with 64 rows and 32 experts and nearly all with 512 rows were wrong in
+                // some rows, and no faster (64 rows, 128 experts: 144.2 -> 142.8 us).
+                __syncwarp();
+                if (lane == 0) mbar_arrive(&empty[s]);
             }
             // epilogue: value v of n-tile n is (row ra + 8 (v >> 1), token 8n + 2t + (v & 1))
             if (GU) {
