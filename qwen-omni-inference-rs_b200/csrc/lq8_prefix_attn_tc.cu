@@ -428,9 +428,6 @@ prefix_attn_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_co
                     const float v = fmaxf(vs, PREFIX_ATTN_Q8_LEAST);
                     v_add = __log2f(v);
                     v_per = __frcp_rn(v);
-                    __syncwarp();
-                    if (lane == 0) mbar_arrive(&c.sc_empty[f][sc_slot]);
-                    if (++sc_slot == PA_SCALES) sc_slot = 0, sc_ph ^= 1;
                     both = ks * vs;
                 }
                 auto of = [](float x, int i) { return __shfl_sync(0xffffffffu, x, i); };
@@ -632,6 +629,10 @@ prefix_attn_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_co
                 if constexpr (Q8) {  // (here, where no product waits for it)
                     const unsigned lost = __ballot_sync(0xffffffffu, both != both) & 0xffu;
                     if (lost && (t < chain ? g.a.prefix_len : vis) - t * PA_TILE > 16 * (__ffs(lost) - 1)) l = __uint_as_float(0x7fffffffu);
+                    // (the scales are given back here, where the vote has used them: a copy may land as soon as that is done,
+                    // also before loads that were only issued)
+                    if (lane == 0) mbar_arrive(&c.sc_empty[f][sc_slot]);
+                    if (++sc_slot == PA_SCALES) sc_slot = 0, sc_ph ^= 1;
                 }
                 if (t == sg.t0) {
                     more = next(true);
