@@ -221,6 +221,9 @@ __global__ void __launch_bounds__(GV_THREADS) q8_gemv_stream_kernel(const GvPara
                         dw[j] = h2f(drow[b]);
                     }
                 }
+                // (the loads are waited for: only issued, they might read what the next copy brings. Releasing after the
+                // products instead: 4 rows, 25600 x 5120 41.0 us against 40.4, one row 22.7 against 22.6)
+                __threadfence_block();
                 __syncwarp();
                 if (lane == 0) mbar_arrive(&S.empty[s]);
 #pragma unroll

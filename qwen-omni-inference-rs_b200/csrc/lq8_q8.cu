@@ -724,9 +724,9 @@ __global__ void __launch_bounds__(GS_THREADS, 2) q8_gemm_stream_kernel(const __g
                 if (lane == 0) mbar_arrive(&empty[s]);
                 continue;
             }
-            // one n8 tile: the warp's whole slice of the stage into registers and the stage
-            // released at once; two tiles: the token fragments are read block by block and
-            // the stage released after the blocks (fewer live registers)
+            // one n8 tile: the warp's whole slice of the stage into registers; two tiles: the token
+            // fragments are read block by block (fewer live registers). The stage is released after the
+            // products, when every load has come back (16 rows, 25600 x 5120: 44.9 -> 41.9 us)
             constexpr bool EARLY = NTW == 1;
             uint2 wa[8], wb[8], xv[EARLY ? 8 : 1];
             uint4 ua[NTW], ub[NTW];
@@ -743,10 +743,6 @@ __global__ void __launch_bounds__(GS_THREADS, 2) q8_gemm_stream_kernel(const __g
             for (int i = 0; i < NTW; i++) {
                 ua[i] = *reinterpret_cast<const uint4*>(st + xd_off + i * 8 * 16);
                 ub[i] = *reinterpret_cast<const uint4*>(st + xd_off + i * 8 * 16 + 16);
-            }
-            if constexpr (EARLY) {
-                __syncwarp();
-                if (lane == 0) mbar_arrive(&empty[s]);
             }
 #pragma unroll
             for (int j = 0; j < 8; j++) {
@@ -780,10 +776,8 @@ __global__ void __launch_bounds__(GS_THREADS, 2) q8_gemm_stream_kernel(const __g
                     acc[i][3] = __fadd_rn(acc[i][3], __fmul_rn(f3, __fmul_rn(dwb, dx1)));
                 }
             }
-            if constexpr (!EARLY) {
-                __syncwarp();
-                if (lane == 0) mbar_arrive(&empty[s]);
-            }
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&empty[s]);
         }
         if (bad || nact == 0) continue;
         // epilogue: value v of tile i is (row ra + 8 (v >> 1) of group q, token 8 (n0 + i) + 2t + (v & 1))
@@ -1100,7 +1094,8 @@ __global__ void __launch_bounds__(SK_THREADS, MINB) q8_gemm_skinny_kernel(const 
                 continue;
             }
             const uint8_t* st = sm + (size_t)cs * SK_STAGE;
-            // the warp's whole slice of the stage into registers, then the stage is released
+            // the warp's whole slice of the stage into registers; the stage is released after the
+            // products, when every load has come back
             uint2 wa[8], wb[8], xv[8];
 #pragma unroll
             for (int j = 0; j < 8; j++) {
@@ -1113,8 +1108,6 @@ __global__ void __launch_bounds__(SK_THREADS, MINB) q8_gemm_skinny_kernel(const 
             const uint4 sb = *reinterpret_cast<const uint4*>(st + sc_off + 8 * 16);
             const uint4 ua = *reinterpret_cast<const uint4*>(st + xd_off);
             const uint4 ub = *reinterpret_cast<const uint4*>(st + xd_off + 16);
-            __syncwarp();
-            if (lane == 0) mbar_arrive(&empty[cs]);
 #pragma unroll
             for (int j = 0; j < 8; j++) {
                 const uint32_t a[4] = {wa[j].x, wb[j].x, wa[j].y, wb[j].y};
@@ -1138,6 +1131,8 @@ __global__ void __launch_bounds__(SK_THREADS, MINB) q8_gemm_skinny_kernel(const 
                 acc[2] = __fadd_rn(acc[2], __fmul_rn(f2, __fmul_rn(dwb, dx0)));
                 acc[3] = __fadd_rn(acc[3], __fmul_rn(f3, __fmul_rn(dwb, dx1)));
             }
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&empty[cs]);
         }
         // ---- segment end: a whole tile is written; a cut tile goes through the partial buffer ----
         float v[4] = {acc[0], acc[1], acc[2], acc[3]};
