@@ -227,7 +227,8 @@ __global__ void __launch_bounds__(256, P == 8 ? 3 : 2) paged_append_q8_kernel(Ap
             for (int e = 0; e < 8; e++) lo[i][e] = hi[i][e] = 0.0f;
         }
     }
-    const float old = t.ok ? scales[scale_at] : 0.0f;  // as the cache has it
+    float old = t.ok ? scales[scale_at] : 0.0f;
+    if (old < 1.17549435e-38f) old = 0.0f;  // (one that a caller put there may have no reciprocal)
     if (!is_v) {
 #pragma unroll
         for (int i = 0; i < IT; i++) {

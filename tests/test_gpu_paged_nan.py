@@ -1,4 +1,4 @@
-"""GPU tests of NaN and infinities in the attention over paged caches: they reach the rows that see them, whichever
+"""GPU tests of NaN, infinities and scales that are no normal numbers in paged caches. In the attention they reach the rows that see them, whichever
 kernel has a row and whether or not its parts go through the merge, and no others. Definitions and
 tolerances of the other rows are those of test_gpu_paged.py and test_gpu_paged_q8.py."""
 import pytest
@@ -124,3 +124,33 @@ def test_nan_scales_that_later_rows_of_a_chunk_see(ctx, lq8_lib, q, prefix, D):
         bad[:, 3:] = True
         check(s.cache.attend(x, s.batch), want[0], q8.tolerance(want, streaming=False) + q8.tolerance(want), bad)
         ctx.device_status()
+
+
+# ------------------------------------------------------------------------------------------
+# scales below the normal numbers
+# ------------------------------------------------------------------------------------------
+
+@pytest.mark.parametrize("tiny", [2.0 ** -130, 2.0 ** -149, 1.1e-38, 0.0])
+@pytest.mark.parametrize("block", [16, 128])
+def test_append_behind_a_scale_below_the_normal_numbers(ctx, lq8_lib, tiny, block):
+    """A cache that its owner filled: such a scale counts as zero, as one that an append works out does."""
+    import torch
+    from test_gpu_paged import i32
+    D = 64
+    c = lq8_lib.PagedKvCacheQ8.empty(ctx, 3, 128, 1, D, block)
+    for t in (c.k, c.v):
+        t.fill_(5)
+    for t in (c.k_scale, c.v_scale):
+        t.fill_(tiny)
+    rotary, table = lq8_lib.Rotary.build(0, 1, 1e4), i32([[0], [1], [2]])
+    x = randn(3, 3, 3 * D)
+    x[0, D:] = 0.0
+    x[1, D:] = 1e-40
+    c.append(x, 1, lq8_lib.PagedBatch(table, i32([2, 2, 2])), rotary)
+    ctx.device_status()
+    both = lq8_lib.PagedBatch(table, i32([2, 2, 2]), q_start=i32([0, 2, 4, 6]), max_q=2)
+    for w, (codes, scale, got) in enumerate(zip((c.k, c.v), (c.k_scale, c.v_scale), c.read(both, rows=6, dtype=torch.float32))):
+        assert not codes[:2, 0, 1].any() and not scale[:2, 0, 0].any() and not got[:4].any()
+        want = x[2, (w + 1) * D:(w + 2) * D]
+        assert not codes[2, 0, 0].any() and int(codes[2, 0, 1].abs().max()) == 127 and not got[4].any()
+        assert float((got[5, 0] - want).abs().max()) <= float(want.abs().max()) / 127 * 0.51
