@@ -295,9 +295,10 @@ int lq_prefix_attention(lq_ctx* ctx, const void* q_dev, lq_dtype dtype, int64_t 
 /* lq_paged_append into such a cache. q to q_out as bf16. For the call's rows of one block and kv head,
  * with a the largest |x|: the scale becomes a / 127 where they begin the block, and the larger of
  * a / 127 and the present scale where older positions do; if it grows, the older codes become
- * rint(code * old / new). New codes are rint(x / scale), computed in f32. An infinity or a NaN makes
- * the scale NaN, and the block reads as NaN until its first position is appended again; a scale
- * below 2^-126 becomes zero. */
+ * rint(code * (old / new)). New codes are rint(x * r) with r the f32 reciprocal of the scale, of the exact
+ * product: within 2^-17 of halfway between two codes of x / scale that may be either of them (with bf16
+ * rows that is where |x| is half of a). An infinity or a NaN makes the scale NaN, and the block reads as
+ * NaN until its first position is appended again; a scale below 2^-126 becomes zero. */
 int lq_paged_append_q8(lq_ctx* ctx, const void* qkv_dev, lq_dtype qkv_dtype, int64_t row_stride, int64_t rows,
                        int64_t n_heads, int64_t n_kv_heads, int64_t head_dim, const uint16_t* q_norm_dev,
                        const uint16_t* k_norm_dev, float eps, int norm_bf16, int64_t rot_dim, const float* cos_dev,

@@ -13,7 +13,9 @@ namespace lq {
 //   s' = a / 127             where the call's rows begin the block,
 //   s' = max(s, a / 127)     where older positions do; if that is larger than s, their codes
 //                            become rint(c s / s'),
-//   c  = rint(x / s').
+//   c  = rint(x r), r = 1 / s' in f32, the product exact: it is off by up to 127 2^-24 from x / s', which only
+//        matters that close to halfway between two codes. (A division takes several instructions for each
+//        value, in a kernel that prompt chunks bind by its instructions.)
 // A team of B / 16 warps owns a block of one sequence, one kv head, K or V: a warp holds 16
 // positions in registers (a lane 8 rotary pairs of a position, D / 16 lanes a position), so that
 // rows are read once and the largest value is known before the first code is written. It is found as
