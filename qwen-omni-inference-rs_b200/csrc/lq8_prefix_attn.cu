@@ -22,10 +22,15 @@ namespace lq {
 // =========================================================================================
 constexpr int MERGE_CHUNK = 32;   // partials looked at together
 
-template <typename T, int D, int MR>
+// whose partials: of kernels whose CTAs have flows, of the streaming kernel, or the prefix's of the former and the own
+// items' of the latter
+enum { MERGE_FLOWS, MERGE_STREAM, MERGE_APART };
+
+template <typename T, int D, int MR, int KIND>
 __global__ void __launch_bounds__(256, MR == 32 ? 5 : 4)
 prefix_attn_merge_kernel(const __grid_constant__ PrefixAttnArgs a, const __grid_constant__ PagedSeqs s,
-                         const __grid_constant__ PrefixPlan p, const __grid_constant__ PrefixPlan pp) {
+                         const __grid_constant__ PrefixPlan p, const __grid_constant__ PrefixPlan prefix_plan) {
+    const PrefixPlan& pp = KIND == MERGE_APART ? prefix_plan : p;
     constexpr int CH = D / 4, SUBS = 256 / MR;  // vectors of a row; threads that share a row
     constexpr int VEC = (CH + SUBS - 1) / SUBS, BATCH = VEC == 1 ? 8 : 1;  // partials whose loads go out together
     __shared__ int slot[MERGE_CHUNK];
@@ -71,14 +76,13 @@ prefix_attn_merge_kernel(const __grid_constant__ PrefixAttnArgs a, const __grid_
     pdl_wait();
     pdl_trigger();
     const int own_steps = *p.own_steps;
-    const Line line(pp, pp.streams == p.streams ? own_steps : 0, pp.pair_p, pp.pair_o);
-    const Shares shares(p, p.streams ? own_steps : 0);
     // whether a worker between an item's first and last one has a step of it
     auto works = [&](int part, int v) {
         int lo, hi;
-        if (part ? p.streams & 2 : pp.streams & 1) {
-            shares.range(v, part, lo, hi);
+        if (part ? KIND != MERGE_FLOWS : KIND == MERGE_STREAM) {
+            Shares(p, own_steps).range(v, part, lo, hi);
         } else {
+            const Line line(pp, KIND == MERGE_FLOWS ? own_steps : 0, pp.pair_p, pp.pair_o);
             const bool paired = part ? pp.pair_o : pp.pair_p;
             flow_range(line, paired, paired ? v : v >> 1, paired ? 0 : v & 1, part, lo, hi);
         }
@@ -302,15 +306,15 @@ static int make_plan(lq_ctx* ctx, const PrefixAttnArgs& a, const PagedSeqs& s, b
     return make_workspace(ctx, "lq_prefix_attention", a, s, D, p, p);
 }
 
-template <typename T, int D>
+template <typename T, int D, int KIND = MERGE_FLOWS>
 static int launch_merge(lq_ctx* ctx, const PrefixAttnArgs& a, const PagedSeqs& s, const PrefixPlan& p, const PrefixPlan& pp) {
     // a row of few heads leaves most of a 32-row CTA idle
     const int mr = p.cap[1] <= 8 ? 8 : 32;
     const int64_t R = (int64_t)s.rows * a.group;
     const dim3 grid((unsigned)(p.np > 0 ? a.n_kv * (R / p.ob + s.n_seqs) : p.notes),
                     (unsigned)ceil_div(p.cap[1], mr));
-    return mr == 8 ? launch_kernel(ctx, prefix_attn_merge_kernel<T, D, 8>, grid, dim3(256), 0, "prefix_attn_merge", a, s, p, pp)
-                   : launch_kernel(ctx, prefix_attn_merge_kernel<T, D, 32>, grid, dim3(256), 0, "prefix_attn_merge", a, s, p, pp);
+    return mr == 8 ? launch_kernel(ctx, prefix_attn_merge_kernel<T, D, 8, KIND>, grid, dim3(256), 0, "prefix_attn_merge", a, s, p, pp)
+                   : launch_kernel(ctx, prefix_attn_merge_kernel<T, D, 32, KIND>, grid, dim3(256), 0, "prefix_attn_merge", a, s, p, pp);
 }
 
 // An 8-bit cache: which kernel takes which items.
@@ -362,8 +366,9 @@ static int attend_q8(lq_ctx* ctx, const PrefixAttnArgs& a, const PagedSeqs& s, c
     if (rc) return rc;
     if (pre == &tc && (rc = launch_prefix_attn_tc(ctx, a, s, tc, D, &c))) return rc;
     if (own == &st && (rc = launch_prefix_attn_q8_decode(ctx, a, s, c, st, D, st_rows))) return rc;
-    return own->streams == 3 && own->np == 0 ? launch_prefix_attn_q8_join(ctx, a, s, *own, D)
-                                             : launch_merge<__nv_bfloat16, D>(ctx, a, s, *own, *pre);
+    if (own != pre) return launch_merge<__nv_bfloat16, D, MERGE_APART>(ctx, a, s, *own, *pre);
+    if (own == &tc) return launch_merge<__nv_bfloat16, D>(ctx, a, s, tc, tc);
+    return st.np > 0 ? launch_merge<__nv_bfloat16, D, MERGE_STREAM>(ctx, a, s, st, st) : launch_prefix_attn_q8_join(ctx, a, s, st, D);
 }
 
 // checks and arguments shared by the entry points; esize: bytes of an element of q and out. page_stride:

@@ -277,10 +277,11 @@ prefix_attn_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_co
     const int per_entry = (g.s.n_seqs + PA_SCAN - 1) / PA_SCAN;
     const int n_entries = per_entry == 1 ? g.s.n_seqs : (g.s.n_seqs + per_entry - 1) / per_entry;
     const OwnSteps os{g.a, g.p};
+    auto apart = [&]() { return Q8 && g.p.apart; };
     const bool by_warp = PO && per_entry == 1 && g.a.max_q * g.a.group > 4 * g.p.ob;
     bool fell = false;
 #pragma unroll 1
-    for (int e = by_warp ? warp : tid; e < n_entries && !g.p.apart; e += by_warp ? PA_THREADS / 32 : PA_THREADS) {
+    for (int e = by_warp ? warp : tid; e < n_entries && !apart(); e += by_warp ? PA_THREADS / 32 : PA_THREADS) {
         int n = 0;
 #pragma unroll 1
         for (int b = e * per_entry; b < min(g.s.n_seqs, (e + 1) * per_entry); b++) {
@@ -307,8 +308,8 @@ prefix_attn_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_co
     __syncthreads();
     tc_after();
     const uint32_t tmem = __shfl_sync(0xffffffffu, c.tmem, 0);
-    const int so = fell || g.p.apart ? 0 : c.scan[n_entries];
-    if (blockIdx.x == 0 && tid == 0 && !g.p.apart) *g.p.own_steps = so;  // for the merge
+    const int so = fell || apart() ? 0 : c.scan[n_entries];
+    if (blockIdx.x == 0 && tid == 0 && !apart()) *g.p.own_steps = so;  // for the merge
     const int me = blockIdx.x, polls = g.p.polls;
     // own items count positions from the first tile of the prefix they begin with, whose last tile
     // may be partly empty

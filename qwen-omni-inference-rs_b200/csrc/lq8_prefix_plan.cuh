@@ -60,19 +60,20 @@ struct PrefixPlan {
     uint64_t workers_mul;       // ceil(2^40 / workers)
     int polls;                  // polls of a wait (f32: for a copy; bf16: for segments) before it gives up
     int hold;                   // fault injection: every CTA stops handing out segments after a few batches
-    int streams;                // parts whose items the streaming kernel takes (1: prefix, 2: own; 8-bit caches)
-    int chunks;                 // 1: it may hand out the line in ranges of falling size
-    int apart;                  // own items are another launch's
-    int ranges;                 // workers, or ranges of the line, that may have a piece of an item
-    int notes;                  // entries of split
     int cap[2];                 // rows a partial slot holds (prefix, own)
     int32_t* own_steps;         // [1] own steps in all, written by the first CTA
-    unsigned* claimed;          // [2] ranges handed out, CTAs that are through (behind own_steps; zero between calls)
     int32_t* first[2];          // per item (prefix, own): the first worker of its steps,
     int32_t* last[2];           // and the last
     SplitItem* split;           // per worker, without a prefix: the cut item it begins
     float* o[2];                // partials, unnormalised: [slot][D/4][cap] of four dims
     float2* ml[2];              // [slot][cap]: running maximum (log2 units) and sum
+    // (behind the fields that every kernel asks for when it begins)
+    int ranges;                 // workers, or ranges of the line, that may have a piece of an item
+    int streams;                // parts whose items the streaming kernel takes (1: prefix, 2: own; 8-bit caches)
+    int chunks;                 // 1: it may hand out the line in ranges of falling size
+    int apart;                  // own items are another launch's
+    int notes;                  // entries of split
+    unsigned* claimed;          // [2] ranges handed out, CTAs that are through (behind own_steps; zero between calls)
     // Where a worker's piece of an own item goes. Without prefix items only cut items leave partials:
     // a worker has one piece at most of an item that it begins and one of an item begun before it.
     __device__ __forceinline__ int own_slot(int item, int worker, bool begins) const {
