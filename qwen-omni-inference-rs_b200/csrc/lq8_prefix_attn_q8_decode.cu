@@ -413,9 +413,9 @@ prefix_attn_q8_decode_kernel(const __grid_constant__ CUtensorMap map_k, const __
             };
 #pragma unroll 1
             for (int t = sg.t0; t < sg.t1; t++, n_tile++) {
-                const float k1 = ks, v1 = max_nan(vs, PREFIX_ATTN_Q8_LEAST);
-                // (a scale that is NaN comes by way of the score, to the rows that see its position)
-                const float lv = __log2f(v1), per = v1 == v1 ? __frcp_rn(v1) : 1.0f;
+                // (a scale that is NaN comes by way of the score, to the rows that see its position, and is no factor of
+                // what the others have there: fmaxf takes the least one instead)
+                const float k1 = ks, lv = __log2f(max_nan(vs, PREFIX_ATTN_Q8_LEAST)), per = __frcp_rn(fmaxf(vs, PREFIX_ATTN_Q8_LEAST));
                 if (t + 1 < sg.t1) {
                     scales_at(sg, t + 1, id_next);
                     id_next = page_at(sg, t + 2);

@@ -413,6 +413,11 @@ prefix_attn_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_co
             const bool mine = my_row < sg.n, busy = few || wq * 32 < sg.n;
             const int vis = sg.flags & SEG_OWN ? chain * PA_TILE + max(0, tok + sg.voff) : sg.kv_end;
             float m = -INFINITY, l = 0.0f;
+            // 8-bit caches: positions that every row of the warp sees; a NaN among the scales of tiles within them. (A vote
+            // in every tile instead: 128 sequences behind 32768 positions 215.4 us instead of 213.3. With paired own
+            // blocks the vote takes less: 10 prompt chunks 160.7 us, 163.0 without.)
+            [[maybe_unused]] const int all_see = Q8 && !PO ? __reduce_min_sync(0xffffffffu, vis) : 0;
+            [[maybe_unused]] bool lost = false;
             int t = sg.t0;
 #pragma unroll 1
             for (; t < sg.t1; t++) {
@@ -628,9 +633,15 @@ prefix_attn_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_co
                 __syncwarp();
                 if (lane == 0) mbar_arrive(&c.p_full[f]);
                 if constexpr (Q8) {  // (here, where no product waits for it)
-                    const unsigned lost = __ballot_sync(0xffffffffu, both != both) & 0xffu;
-                    if (lost && (t < chain ? g.a.prefix_len : vis) - t * PA_TILE > 16 * (__ffs(lost) - 1)) l = __uint_as_float(0x7fffffffu);
-                    // (the scales are given back here, where the vote has used them: a copy may land as soon as that is done,
+                    const bool nan = both != both;
+                    if (!PO && (t + 1) * PA_TILE <= all_see) {  // (by the whole warp)
+                        lost |= nan;
+                        __syncwarp();
+                    } else {
+                        const unsigned at = __ballot_sync(0xffffffffu, nan) & 0xffu;
+                        if (at && (t < chain ? g.a.prefix_len : vis) - t * PA_TILE > 16 * (__ffs(at) - 1)) l = __uint_as_float(0x7fffffffu);
+                    }
+                    // (the scales are given back here, where they have been used: a copy may land as soon as that is done,
                     // also before loads that were only issued)
                     if (lane == 0) mbar_arrive(&c.sc_empty[f][sc_slot]);
                     if (++sc_slot == PA_SCALES) sc_slot = 0, sc_ph ^= 1;
@@ -642,6 +653,8 @@ prefix_attn_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_co
                 }
             }
             if (t < sg.t1) break;  // a wait ran out
+            if constexpr (Q8 && !PO)
+                if (__any_sync(0xffffffffu, lost)) l = __uint_as_float(0x7fffffffu);
             if (more == NX_LATER) more = next(false);
             if (more == NX_SEG) {
                 if (!early) q_start();  // this segment's Q has been read: its last S was complete
