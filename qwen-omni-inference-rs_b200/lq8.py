@@ -481,7 +481,9 @@ class PagedBatch:
 
 
 class _PagedCache:
-    """What the paged caches of all types share. `type` is that of q and of the attention's rows."""
+    """What the paged caches of all types share. `type` is that of q and of the attention's rows. A cache gives its
+    entry points (_append, _attend), their arguments for its pages (_into, _from), and the type that the
+    attention's asks for (_q_type): put together once, a call of few rows takes as long as the binding does."""
 
     @staticmethod
     def _row_stride(t, shape, dtype, what: str) -> int:
@@ -516,10 +518,10 @@ class _PagedCache:
         if pos is None and rotary.n_axes != 1:
             raise ValueError("append: several axes need positions")
         p, ps = (None, 0) if pos is None else rotary._pos(pos, rows)
-        rc = self._append(qkv.data_ptr(), dt, st[0] if rows > 1 else 0, rows, n_heads, self.n_kv_heads, D,
+        rc = self._append(self.ctx.h, qkv.data_ptr(), dt, st[0] if rows > 1 else 0, rows, n_heads, self.n_kv_heads, D,
                           None if q_norm is None else q_norm.data_ptr(), None if k_norm is None else k_norm.data_ptr(), eps,
-                          1 if norm_bf16 else 0, *rotary._args, p, ps, batch.prefix_len, *batch._seqs, *self._pages,
-                          *self._layout, q_out.data_ptr(), q_stride)
+                          1 if norm_bf16 else 0, *rotary._args, p, ps, batch.prefix_len, *batch._seqs, *self._into,
+                          q_out.data_ptr(), q_stride)
         if rc:
             self.ctx.check(rc)
         return q_out
@@ -550,9 +552,10 @@ class _PagedCache:
                              f"{self.page_size}")
         if rows == 0:
             return out
-        rc = self._attend(q.data_ptr(), q_stride, rows, heads, self.n_kv_heads, D, D ** -0.5 if scale is None else scale,
-                          *self._pages, *self._layout, batch._prefix_ptr, batch.prefix_len, *batch._seqs, batch.max_q,
-                          batch.ld * self.page_size if batch.max_kv is None else batch.max_kv, out.data_ptr(), out_stride, xq, xd)
+        rc = self._attend(self.ctx.h, q.data_ptr(), *self._q_type, q_stride, rows, heads, self.n_kv_heads, D,
+                          D ** -0.5 if scale is None else scale, *self._from, batch._prefix_ptr, batch.prefix_len, *batch._seqs,
+                          batch.max_q, batch.ld * self.page_size if batch.max_kv is None else batch.max_kv, out.data_ptr(),
+                          out_stride, xq, xd)
         if rc:
             self.ctx.check(rc)
         return out
@@ -573,7 +576,9 @@ class PagedKvCache(_PagedCache):
               "PagedKvCache: pages are dense inside and apart, K and V pages equally far")
         self.ctx, self.k, self.v, self.type = ctx, k, v, k.dtype
         self._pages = (k.data_ptr(), v.data_ptr())
-        self._layout = (self.n_pages, self.page_size, k.stride(0) if self.n_pages > 1 else self.n_kv_heads * inner[0])
+        layout = (self.n_pages, self.page_size, k.stride(0) if self.n_pages > 1 else self.n_kv_heads * inner[0])
+        self._append, self._attend = ctx.lib.lq_paged_append, ctx.lib.lq_prefix_attention
+        self._into, self._from, self._q_type = (*self._pages, self.dtype, *layout), (*self._pages, *layout), (self.dtype,)
         import torch
         self._norm_types = (torch.bfloat16, torch.int16)
 
@@ -582,14 +587,6 @@ class PagedKvCache(_PagedCache):
         import torch
         shape = (n_pages, n_kv_heads, page_size, head_dim)
         return cls(ctx, torch.empty(shape, dtype=dtype, device="cuda"), torch.empty(shape, dtype=dtype, device="cuda"))
-
-    def _append(self, *args):
-        # the cache's type stands between its pages and their layout
-        at = len(args) - 2 - len(self._layout)
-        return self.ctx.lib.lq_paged_append(self.ctx.h, *args[:at], self.dtype, *args[at:])
-
-    def _attend(self, q, *args):
-        return self.ctx.lib.lq_prefix_attention(self.ctx.h, q, self.dtype, *args)
 
 
 class PagedKvCacheQ8(_PagedCache):
@@ -617,9 +614,11 @@ class PagedKvCacheQ8(_PagedCache):
               (self.n_pages <= 1 or k_scale.stride(0) >= self.n_kv_heads * blocks),
               "PagedKvCacheQ8: pages are dense inside and apart, K and V pages equally far")
         self.ctx, self.k, self.v, self.k_scale, self.v_scale, self.type = ctx, k, v, k_scale, v_scale, torch.bfloat16
-        self._pages = (k.data_ptr(), v.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr())
         apart = (k.stride(0), k_scale.stride(0)) if self.n_pages > 1 else (0, 0)
+        self._pages = (k.data_ptr(), v.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr())
         self._layout = (self.n_pages, self.page_size, apart[0], self.block, apart[1])
+        self._append, self._attend = ctx.lib.lq_paged_append_q8, ctx.lib.lq_prefix_attention_q8
+        self._into, self._from, self._q_type = (*self._pages, *self._layout), (*self._pages, *self._layout), ()
         self._norm_types = (torch.bfloat16, torch.int16)
 
     @classmethod
@@ -628,12 +627,6 @@ class PagedKvCacheQ8(_PagedCache):
         shape, scales = (n_pages, n_kv_heads, page_size, head_dim), (n_pages, n_kv_heads, page_size // block)
         return cls(ctx, *(torch.empty(shape, dtype=torch.int8, device="cuda") for _ in range(2)),
                    *(torch.empty(scales, dtype=torch.float32, device="cuda") for _ in range(2)))
-
-    def _append(self, *args):
-        return self.ctx.lib.lq_paged_append_q8(self.ctx.h, *args)
-
-    def _attend(self, *args):
-        return self.ctx.lib.lq_prefix_attention_q8(self.ctx.h, *args)
 
     def read(self, batch: PagedBatch, k_out=None, v_out=None, rows: int | None = None, dtype=None):
         """The batch's rows as the cache holds them, code * scale: (k, v), [rows, n_kv_heads, head_dim] in f32
