@@ -226,9 +226,9 @@ int lq_fill_bf16(lq_ctx* ctx, uint64_t seed, uint64_t tensor_id, int64_t offset,
  * one), and kv_len_dev[b] is its number of own positions, those rows included, which come last.
  * Rows past the last sequence's are padding: what they hold has no effect, and nothing is written
  * for them. Positions outside the tables, lengths outside the page table and page ids outside the
- * cache skip the access and are reported by lq_device_status; so are row starts that fall, with which
- * the attention computes nothing. Pointers are aligned to their
- * elements.
+ * cache skip the access and are reported by lq_device_status. Row starts that fall are reported by the
+ * attention, which computes nothing with them; the operators that append and read may not meet them, and
+ * leave anything in the batch's own rows and pages then. Pointers are aligned to their elements.
  * ------------------------------------------------------------------------------------- */
 /* Waits for the context's stream; LQ_ERR_INVALID_ARG with the first code and value that a
  * kernel flagged since the last check (90 rotary position, 91 length, 92 page id, 93 row
