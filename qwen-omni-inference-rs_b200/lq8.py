@@ -597,6 +597,8 @@ class PagedKvCacheQ8(_PagedCache):
     their block's codes (and the block's older ones again, where its largest value grows), attend takes q
     and gives rows in bf16, read gives rows of the cache back."""
 
+    BLOCKS = (16, 32, 64, 128)
+
     def __init__(self, ctx: Context, k, v, k_scale, v_scale):
         import torch
         _need(k.dim() == 4 and k.shape == v.shape and k.dtype == v.dtype == torch.int8 and k.is_cuda and v.device == k.device,
@@ -607,6 +609,7 @@ class PagedKvCacheQ8(_PagedCache):
               self.page_size % k_scale.shape[2] == 0,
               "PagedKvCacheQ8: k_scale and v_scale are f32 CUDA tensors [n_pages, n_kv_heads, page_size / block]")
         self.block = self.page_size // k_scale.shape[2]
+        _need(self.block in self.BLOCKS, f"PagedKvCacheQ8: a scale for {self.block} positions, must be for 16, 32, 64 or 128")
         inner, blocks = (self.page_size * self.head_dim, self.head_dim, 1), k_scale.shape[2]
         _need(k.stride()[1:] == inner and v.stride()[1:] == inner and k.stride(0) == v.stride(0) and
               (self.n_pages <= 1 or k.stride(0) >= self.n_kv_heads * inner[0]) and
@@ -624,6 +627,8 @@ class PagedKvCacheQ8(_PagedCache):
     @classmethod
     def empty(cls, ctx: Context, n_pages: int, page_size: int, n_kv_heads: int, head_dim: int, block: int = 16):
         import torch
+        _need(block in cls.BLOCKS and page_size % block == 0,
+              f"PagedKvCacheQ8: block {block} must be 16, 32, 64 or 128 positions and divide a page of {page_size}")
         shape, scales = (n_pages, n_kv_heads, page_size, head_dim), (n_pages, n_kv_heads, page_size // block)
         return cls(ctx, *(torch.empty(shape, dtype=torch.int8, device="cuda") for _ in range(2)),
                    *(torch.empty(scales, dtype=torch.float32, device="cuda") for _ in range(2)))
