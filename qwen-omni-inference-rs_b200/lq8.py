@@ -380,9 +380,9 @@ class Rotary:
     def __init__(self, cos, sin, axis=None):
         import torch
         _need(cos.dtype == sin.dtype == torch.float32 and cos.dim() == 2 and cos.shape == sin.shape and
-              cos.is_cuda and sin.is_cuda and cos.is_contiguous() and sin.is_contiguous(),
-              "Rotary: cos and sin are contiguous f32 CUDA tables of one shape")
-        self.cos, self.sin = cos, sin
+              cos.is_cuda and sin.device == cos.device and cos.is_contiguous() and sin.is_contiguous(),
+              "Rotary: cos and sin are contiguous f32 CUDA tables of one shape on one device")
+        self.cos, self.sin, self.device = cos, sin, cos.get_device()
         self.table_len, self.pairs = cos.shape
         self.axis = None if axis is None else np.ascontiguousarray(axis, dtype=np.uint8)
         _need(self.axis is None or self.axis.shape == (self.pairs,), "Rotary: one axis a pair")
@@ -424,9 +424,10 @@ class Rotary:
     def _pos(self, pos, rows: int):
         """Checked (pointer, stride) of positions [n_axes, rows] (or [rows] for one axis)."""
         shape, stride = pos.shape, pos.stride()
-        if (pos.dtype != self._int32 or not pos.is_cuda or len(shape) not in (1, 2) or shape[-1] != rows or
+        if (pos.dtype != self._int32 or pos.get_device() != self.device or len(shape) not in (1, 2) or shape[-1] != rows or
                 (rows > 1 and stride[-1] != 1) or (shape[0] if len(shape) == 2 else 1) < self.n_axes):
-            raise ValueError(f"pos: int32 CUDA tensor [{self.n_axes}, {rows}] expected, got {pos.dtype} {list(shape)}")
+            raise ValueError(f"pos: int32 CUDA tensor [{self.n_axes}, {rows}] next to the tables expected, got {pos.dtype} "
+                             f"{list(shape)} on {pos.device}")
         return pos.data_ptr(), stride[0] if len(shape) == 2 and shape[0] > 1 else rows
 
 
@@ -438,10 +439,11 @@ def mrope(ctx: Context, x, rotary: Rotary, pos, out=None, inverse: bool = False)
         import torch
         out = torch.empty(x.shape, dtype=x.dtype, device=x.device)
     shape, xs, ys = x.shape, x.stride(), out.stride()
-    if len(shape) != 3 or not x.is_cuda or (shape[2] > 1 and xs[2] != 1):
-        raise ValueError("mrope: x is a CUDA tensor [rows, heads, head_dim] with contiguous dims")
-    if out.shape != shape or out.dtype != x.dtype or not out.is_cuda or (shape[2] > 1 and ys[2] != 1):
-        raise ValueError("mrope: out has x's shape and type")
+    device = ctx.device
+    if len(shape) != 3 or x.get_device() != device or rotary.device != device or (shape[2] > 1 and xs[2] != 1):
+        raise ValueError("mrope: x is a CUDA tensor [rows, heads, head_dim] with contiguous dims, on the context's device as the tables")
+    if out.shape != shape or out.dtype != x.dtype or out.get_device() != device or (shape[2] > 1 and ys[2] != 1):
+        raise ValueError("mrope: out has x's shape and type, on the context's device")
     rows, heads, D = shape
     if rows == 0:
         return out
@@ -463,7 +465,8 @@ class PagedBatch:
                  prefix_len: int = 0):
         _need_i32(page_table, "page_table", 2)
         _need_i32(kv_len, "kv_len", 1)
-        self.n_seqs = kv_len.shape[0]
+        self.n_seqs, self.device = kv_len.shape[0], kv_len.get_device()
+        _need(all(t is None or t.device == kv_len.device for t in (page_table, q_start, prefix_table)), "PagedBatch: tensors on one device")
         _need(page_table.shape[0] == self.n_seqs and page_table.is_contiguous(),
               "page_table: one row a sequence, contiguous")
         if q_start is not None:
@@ -485,16 +488,15 @@ class _PagedCache:
     entry points (_append, _attend), their arguments for its pages (_into, _from), and the type that the
     attention's asks for (_q_type): put together once, a call of few rows takes as long as the binding does."""
 
-    @staticmethod
-    def _row_stride(t, shape, dtype, what: str) -> int:
-        """Row stride of a CUDA tensor of `shape` [rows, heads, dim] whose rows are dense inside and
-        do not overlap (0: one row)."""
+    def _row_stride(self, t, shape, dtype, what: str) -> int:
+        """Row stride of a tensor of `shape` [rows, heads, dim] on the cache's device whose rows are dense inside
+        and do not overlap (0: one row)."""
         st = t.stride()
         rows, heads, dim = shape
-        if (tuple(t.shape) != shape or t.dtype != dtype or not t.is_cuda or st[2] != 1 or (heads > 1 and st[1] != dim) or
+        if (tuple(t.shape) != shape or t.dtype != dtype or t.get_device() != self.device or st[2] != 1 or (heads > 1 and st[1] != dim) or
                 (rows > 1 and st[0] < heads * dim)):
-            raise ValueError(f"{what}: CUDA tensor {list(shape)} in the cache's type, rows dense inside, expected; "
-                             f"got {t.dtype} {list(t.shape)} with strides {list(st)}")
+            raise ValueError(f"{what}: tensor {list(shape)} in the cache's type and on its device, rows dense inside, expected; "
+                             f"got {t.dtype} {list(t.shape)} with strides {list(st)} on {t.device}")
         return st[0] if rows > 1 else 0
 
     def append(self, qkv, n_heads: int, batch: PagedBatch, rotary: Rotary, pos=None, q_norm=None, k_norm=None,
@@ -505,11 +507,14 @@ class _PagedCache:
         dt = _paged_dtype(qkv, "append")
         D, st = self.head_dim, qkv.stride()
         rows, width = qkv.shape[0], (n_heads + 2 * self.n_kv_heads) * D
-        if len(st) != 2 or qkv.shape[1] != width or not qkv.is_cuda or st[1] != 1 or (rows > 1 and st[0] < width):
-            raise ValueError(f"append: rows of {width} contiguous values expected")
+        device = self.device
+        if len(st) != 2 or qkv.shape[1] != width or qkv.get_device() != device or st[1] != 1 or (rows > 1 and st[0] < width):
+            raise ValueError(f"append: rows of {width} contiguous values on the cache's device expected")
+        if batch.device != device or rotary.device != device:
+            raise ValueError("append: the batch and the rotary tables must be on the cache's device")
         for w in (q_norm, k_norm):
-            if w is not None and (w.dtype not in self._norm_types or w.shape != (D,) or not w.is_cuda or w.stride(0) != 1):
-                raise ValueError("append: norm weights are bf16 [head_dim]")
+            if w is not None and (w.dtype not in self._norm_types or w.shape != (D,) or w.get_device() != device or w.stride(0) != 1):
+                raise ValueError("append: norm weights are bf16 [head_dim] on the cache's device")
         if q_out is None:
             q_out = qkv.new_empty((rows, n_heads, D), dtype=self.type)
         q_stride = self._row_stride(q_out, (rows, n_heads, D), self.type, "append: q_out")
@@ -544,9 +549,11 @@ class _PagedCache:
             import torch
             xq, xd = quantized
             _need(xq.dtype == torch.int8 and xd.dtype == torch.int16 and xq.is_contiguous() and xd.is_contiguous() and
-                  xq.is_cuda and xd.is_cuda and xq.shape == (rows, heads * D) and xd.shape == (rows, heads * D // 32),
+                  xq.get_device() == xd.get_device() == self.device and xq.shape == (rows, heads * D) and xd.shape == (rows, heads * D // 32),
                   "attend: quantized is (int8 [rows, heads * dim], int16 [rows, heads * dim / 32]) on the GPU")
             xq, xd = xq.data_ptr(), xd.data_ptr()
+        if batch.device != self.device:
+            raise ValueError("attend: the batch must be on the cache's device")
         if batch.prefix_len > batch._prefix_pages * self.page_size:
             raise ValueError(f"attend: {batch.prefix_len} prefix positions, prefix_table has {batch._prefix_pages} pages of "
                              f"{self.page_size}")
@@ -567,14 +574,15 @@ class PagedKvCache(_PagedCache):
 
     def __init__(self, ctx: Context, k, v):
         self.dtype = _paged_dtype(k, "PagedKvCache")
-        _need(k.dim() == 4 and k.shape == v.shape and k.dtype == v.dtype and k.is_cuda and v.is_cuda,
+        _need(k.dim() == 4 and k.shape == v.shape and k.dtype == v.dtype and k.is_cuda and v.device == k.device,
               "PagedKvCache: k and v are CUDA tensors [n_pages, n_kv_heads, page_size, head_dim] of one type")
         self.n_pages, self.n_kv_heads, self.page_size, self.head_dim = k.shape
         inner = (self.page_size * self.head_dim, self.head_dim, 1)
         _need(k.stride()[1:] == inner and v.stride()[1:] == inner and k.stride(0) == v.stride(0) and
               (self.n_pages <= 1 or k.stride(0) >= self.n_kv_heads * inner[0]),
               "PagedKvCache: pages are dense inside and apart, K and V pages equally far")
-        self.ctx, self.k, self.v, self.type = ctx, k, v, k.dtype
+        _need(k.get_device() == ctx.device, f"PagedKvCache: k and v are on {k.device}, the context on device {ctx.device}")
+        self.ctx, self.k, self.v, self.type, self.device = ctx, k, v, k.dtype, ctx.device
         self._pages = (k.data_ptr(), v.data_ptr())
         layout = (self.n_pages, self.page_size, k.stride(0) if self.n_pages > 1 else self.n_kv_heads * inner[0])
         self._append, self._attend = ctx.lib.lq_paged_append, ctx.lib.lq_prefix_attention
@@ -586,7 +594,7 @@ class PagedKvCache(_PagedCache):
     def empty(cls, ctx: Context, n_pages: int, page_size: int, n_kv_heads: int, head_dim: int, dtype):
         import torch
         shape = (n_pages, n_kv_heads, page_size, head_dim)
-        return cls(ctx, torch.empty(shape, dtype=dtype, device="cuda"), torch.empty(shape, dtype=dtype, device="cuda"))
+        return cls(ctx, *(torch.empty(shape, dtype=dtype, device=f"cuda:{ctx.device}") for _ in range(2)))
 
 
 class PagedKvCacheQ8(_PagedCache):
@@ -616,7 +624,9 @@ class PagedKvCacheQ8(_PagedCache):
               k_scale.stride()[1:] == v_scale.stride()[1:] == (blocks, 1) and k_scale.stride(0) == v_scale.stride(0) and
               (self.n_pages <= 1 or k_scale.stride(0) >= self.n_kv_heads * blocks),
               "PagedKvCacheQ8: pages are dense inside and apart, K and V pages equally far")
+        _need(k.get_device() == ctx.device, f"PagedKvCacheQ8: the cache is on {k.device}, the context on device {ctx.device}")
         self.ctx, self.k, self.v, self.k_scale, self.v_scale, self.type = ctx, k, v, k_scale, v_scale, torch.bfloat16
+        self.device = ctx.device
         apart = (k.stride(0), k_scale.stride(0)) if self.n_pages > 1 else (0, 0)
         self._pages = (k.data_ptr(), v.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr())
         self._layout = (self.n_pages, self.page_size, apart[0], self.block, apart[1])
@@ -630,8 +640,8 @@ class PagedKvCacheQ8(_PagedCache):
         _need(block in cls.BLOCKS and page_size % block == 0,
               f"PagedKvCacheQ8: block {block} must be 16, 32, 64 or 128 positions and divide a page of {page_size}")
         shape, scales = (n_pages, n_kv_heads, page_size, head_dim), (n_pages, n_kv_heads, page_size // block)
-        return cls(ctx, *(torch.empty(shape, dtype=torch.int8, device="cuda") for _ in range(2)),
-                   *(torch.empty(scales, dtype=torch.float32, device="cuda") for _ in range(2)))
+        return cls(ctx, *(torch.empty(shape, dtype=torch.int8, device=f"cuda:{ctx.device}") for _ in range(2)),
+                   *(torch.empty(scales, dtype=torch.float32, device=f"cuda:{ctx.device}") for _ in range(2)))
 
     def read(self, batch: PagedBatch, k_out=None, v_out=None, rows: int | None = None, dtype=None):
         """The batch's rows as the cache holds them, code * scale: (k, v), [rows, n_kv_heads, head_dim] in f32
@@ -648,6 +658,8 @@ class PagedKvCacheQ8(_PagedCache):
             k_out, v_out = (torch.empty(shape, dtype=dtype or torch.bfloat16, device=self.k.device) for _ in range(2))
         else:
             _need(rows in (None, k_out.shape[0]) and dtype in (None, k_out.dtype), "read: rows and dtype are k_out's")
+        if batch.device != self.device:
+            raise ValueError("read: the batch must be on the cache's device")
         dt = _paged_dtype(k_out, "read")
         shape = (k_out.shape[0], self.n_kv_heads, self.head_dim)
         stride = self._row_stride(k_out, shape, k_out.dtype, "read: k_out")
