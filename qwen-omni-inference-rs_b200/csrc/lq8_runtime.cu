@@ -127,6 +127,11 @@ int ensure_split(lq_ctx* ctx, size_t bytes) {
 static int alloc_paged(lq_ctx* ctx, size_t bytes, PagedBuffer* b) {
     if (fault_injected("ensure_paged"))
         return set_error(ctx, LQ_ERR_INJECTED, "ensure_paged: injected fault (LQ_FAULT), %zu bytes", bytes);
+    // (another device's memory would be kept, although the launch on the context's stream fails then)
+    int device = -1;
+    LQ_CUDA(ctx, cudaGetDevice(&device));
+    LQ_REQUIRE(ctx, device == ctx->device, "paged attention workspace: device %d is current, the context is on device %d", device,
+               ctx->device);
     const size_t sz = (bytes + 0xFFFFF) & ~(size_t)0xFFFFF;
     // (an allocation is no stream work: it may be made while a graph is being captured)
     cudaStreamCaptureMode mode = cudaStreamCaptureModeRelaxed;
