@@ -276,7 +276,9 @@ prefix_attn_f32_kernel(const __grid_constant__ PrefixAttnArgs a, const __grid_co
                     mbar_wait_ns(&full[warp][after(slot, i)], slot + i < PF_SLOTS ? ph : ph ^ 1u, 2000000000ull);
             };
             auto done = [&]() {
-                __syncwarp();  // (read by every lane)
+                // (read by every lane: loads that were only issued might read what the next copy brings)
+                __threadfence_block();
+                __syncwarp();
                 if (++slot == PF_SLOTS) slot = 0, ph ^= 1;
             };
             // in flight: K and V of the first 16 positions, K of the next

@@ -75,3 +75,27 @@ def test_decode_steps_repeat(ctx, lq8_lib, B):
         assert all(np.array_equal(a, b) for a, b in zip(got, want))
     torch.cuda.synchronize()
     m.close()
+
+
+@pytest.mark.parametrize("kind", ["f32", "bf16", "q8"])
+@pytest.mark.parametrize("seqs,new,prefix", [(12, 1, 1000), (70, 1, 5000), (48, 1, 0), (6, 90, 700)])
+def test_paged_attention_repeats(ctx, lq8_lib, kind, seqs, new, prefix):
+    import torch
+    import test_gpu_paged as wide
+    import test_gpu_paged_q8 as q8
+    kv, q = [new + 37 * (b % 60) for b in range(seqs)], [new] * seqs
+    if kind == "q8":
+        s = q8.Cache(lq8_lib, ctx, kv, q, 4, 128, 16, 16, prefix=prefix, seed=61).fill()
+    else:
+        s = wide.Setup(lq8_lib, ctx, kind, kv, q, 4, 128, 16, prefix, seed=61).fill()
+    x = wide.randn(62, s.rows, 16, 128, dtype="f32" if kind == "f32" else "bf16")
+    want, busy = s.cache.attend(x, s.batch), Busy()
+    torch.cuda.synchronize()
+    wrong = torch.zeros((), dtype=torch.int64, device="cuda")
+    for i in range(100):
+        if i % 4 == 0:
+            busy.go()
+        wrong += (s.cache.attend(x, s.batch) != want).any()
+    torch.cuda.synchronize()
+    ctx.device_status()
+    assert int(wrong) == 0
