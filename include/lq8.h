@@ -319,9 +319,10 @@ int lq_paged_read_q8(lq_ctx* ctx, const int8_t* k_codes_dev, const int8_t* v_cod
                      int64_t table_ld, int64_t rows, void* k_out_dev, void* v_out_dev, lq_dtype out_dtype,
                      int64_t out_stride);
 /* lq_prefix_attention over such a cache, q and out bf16. Scales are zero, positive or NaN (which reaches the
- * rows that see its block); V's of less than 2^-80 count as 2^-80, and a block whose V scale is 2^100 times
+ * rows that see a position of its block, and no others); V's of less than 2^-80 count as 2^-80, and a block whose V scale is 2^100 times
  * smaller than another's may lose its weight. With up to 32 stacked rows (max_q, behind a prefix all of the
- * call's, times n_heads / n_kv_heads) a row of q is rounded to 1 / 32512 of its largest value and
+ * call's, times n_heads / n_kv_heads; what max_q says holds for every sequence, so that decode rows are
+ * faster in a call of their own than next to a chunk) a row of q is rounded to 1 / 32512 of its largest value and
  * weights times V's scale to 1 / 32512 of the largest of their 128 positions, sums are exact; with more,
  * products are of 16-bit floats, q and codes exact, weights in fp16 (times V's scale, those below 2^-32 of
  * a row's largest are lost), sums f32. */

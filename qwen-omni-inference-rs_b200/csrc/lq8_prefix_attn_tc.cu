@@ -37,8 +37,8 @@
 // P V needs no more than P. P is fp16 below a running maximum of s, l adds P / v_scale; the producer copies the
 // scales of 16 positions each ahead of a round. Bound: a round takes 4665 cycles, a chain of QK, softmax
 // (2495), PV for either flow: P lies over S, and TMEM has no room for another S; shared memory serves the
-// converters (1024 cycles) next to the products (1536). 10 prompt chunks behind 2049 positions: 158 us; 128
-// sequences behind 32768: 217 us with their own positions (which the streaming kernel takes).
+// converters (1024 cycles) next to the products (1536). 10 prompt chunks behind 2049 positions: 160 us; 128
+// sequences behind 32768: 214 us with their own positions (which the streaming kernel takes).
 //
 // TMA loads here read only this GPU's memory and use no multicast.
 #include "lq8_async.cuh"

@@ -603,7 +603,8 @@ class PagedKvCacheQ8(_PagedCache):
     n_kv_heads, page_size / block], one for each block of 16, 32, 64 or 128 positions of a kv head; a value is
     code * scale. Pages are dense inside and any distance apart. append rounds the rows' values to
     their block's codes (and the block's older ones again, where its largest value grows), attend takes q
-    and gives rows in bf16, read gives rows of the cache back."""
+    and gives rows in bf16, read gives rows of the cache back. A batch of decode rows is faster in a call of its own
+    than next to a prompt chunk: max_q decides how all of a call's sequences are computed."""
 
     BLOCKS = (16, 32, 64, 128)
 
